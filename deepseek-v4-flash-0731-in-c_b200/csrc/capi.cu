@@ -23,6 +23,9 @@
 #include "attn.cuh"
 #include "sample.cuh"
 #include "snapshot.cuh"
+#include "paged.cuh"
+#include "paged_attn.cuh"
+#include "logprob.cuh"
 #include "ep.cuh"
 #include "../../include/dsv4_cuda.h"
 
@@ -430,7 +433,10 @@ dsv4::MoeConfig to_cfg(const dsv4cuda_moe_config* c) {
 
 // ================================================================ exports ==
 
+namespace { void free_stream_scratch(); }
+
 DSV4_API void dsv4cuda_shutdown(void) {
+  free_stream_scratch();
   if (t_state.dbuf) cudaFree(t_state.dbuf);
   if (t_state.counter) cudaFree(t_state.counter);
   if (t_state.stream) cudaStreamDestroy(t_state.stream);
@@ -1544,6 +1550,268 @@ DSV4_API int dsv4cuda_accept_device(const int* proposal, int proposed, const flo
   cudaError_t e = dsv4::accept_device(proposal, proposed, logits, vocab, temperature, uniforms,
                                       eos_id, result, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) { record_error("accept_device: %s", cudaGetErrorString(e)); return -1; }
+  return 0;
+}
+
+// =============================================== paged cache, attention ==
+
+namespace {
+
+// Buffers for attention calls that bring no workspace: one per stream, so
+// that calls on several streams of a thread do not share one.
+struct StreamScratch {
+  int device;
+  cudaStream_t stream;
+  char* buf;
+  size_t cap;
+};
+thread_local std::vector<StreamScratch> t_scratch;
+
+// nullptr with the error recorded when there is none to be had.
+char* stream_scratch(const char* who, size_t bytes, cudaStream_t st) {
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  int dev = 0;
+  cudaError_t e = cudaStreamIsCapturing(st, &cap);
+  if (e == cudaSuccess) e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) { record_error("%s: %s", who, cudaGetErrorString(e)); return nullptr; }
+  if (cap != cudaStreamCaptureStatusNone) {
+    record_error("%s: give a workspace of %zu bytes while capturing", who, bytes);
+    return nullptr;
+  }
+  StreamScratch* s = nullptr;
+  for (auto& x : t_scratch)
+    if (x.device == dev && x.stream == st) s = &x;
+  if (!s) {
+    t_scratch.push_back({dev, st, nullptr, 0});
+    s = &t_scratch.back();
+  }
+  if (bytes > s->cap) {
+    if (s->buf) cudaFree(s->buf);
+    s->buf = nullptr;
+    s->cap = 0;
+    const size_t cap_bytes = bytes + bytes / 4;
+    if (cudaMalloc(&s->buf, cap_bytes) != cudaSuccess) {
+      (void)cudaGetLastError();
+      s->buf = nullptr;
+      record_error("%s: cannot allocate %zu bytes of workspace", who, cap_bytes);
+      return nullptr;
+    }
+    s->cap = cap_bytes;
+  }
+  return s->buf;
+}
+
+void free_stream_scratch() {
+  for (auto& x : t_scratch)
+    if (x.buf) cudaFree(x.buf);
+  t_scratch.clear();
+}
+
+// Checks the description and fills the kernels' form; false with the error
+// recorded.
+bool paged_state(const char* who, const dsv4cuda_paged* p, dsv4::PagedState* s) {
+  static_assert(DSV4CUDA_PAGED_MAX_LAYERS == dsv4::kPagedMaxLayers, "layer limit");
+  static_assert(DSV4CUDA_PAGED_MAX_SEQS == dsv4::kPagedMaxSeqs, "slot limit");
+  if (!p || !p->caches || !p->table || !p->length || !p->refs || !p->workspace ||
+      p->n_caches < 1 || p->n_caches > dsv4::kPagedMaxLayers || p->page_size < 1 ||
+      p->n_pages < 1 || p->n_seqs < 1 || p->n_seqs > dsv4::kPagedMaxSeqs || p->max_pages < 1 ||
+      static_cast<long long>(p->max_pages) * p->page_size > 0x7FFFFFFFll ||
+      static_cast<long long>(p->max_pages) * p->n_seqs > 0x7FFFFFFFll) {
+    record_error("%s: bad arguments (1..%d caches, 1..%d slots, positions and table entries below "
+                 "2^31)", who, dsv4::kPagedMaxLayers, dsv4::kPagedMaxSeqs);
+    return false;
+  }
+  const size_t need = dsv4::paged_workspace_bytes(p->n_pages, p->n_seqs);
+  if (p->workspace_bytes < need || reinterpret_cast<uintptr_t>(p->workspace) % 16) {
+    record_error("%s: workspace of %zu bytes, need %zu (16-byte aligned)", who, p->workspace_bytes,
+                 need);
+    return false;
+  }
+  s->layers = p->n_caches;
+  s->nope = p->caches[0].nope;
+  s->rope_dim = p->caches[0].rope_dim;
+  const long long rows = static_cast<long long>(p->n_pages) * p->page_size;
+  for (int l = 0; l < p->n_caches; ++l) {
+    const dsv4cuda_kv_cache* c = &p->caches[l];
+    if (!cache_ok(c) || c->nope != s->nope || c->rope_dim != s->rope_dim || c->rows < rows ||
+        reinterpret_cast<uintptr_t>(c->codes) % 16 || reinterpret_cast<uintptr_t>(c->rope) % 16 ||
+        reinterpret_cast<uintptr_t>(c->scales) % 8) {
+      record_error("%s: cache %d has other row sizes, fewer than %lld rows, or is not aligned "
+                   "(codes/rope 16 bytes, scales 8)", who, l, rows);
+      return false;
+    }
+    s->codes[l] = c->codes;
+    s->scales[l] = c->scales;
+    s->rope[l] = c->rope;
+  }
+  s->page = p->page_size;
+  s->n_pages = p->n_pages;
+  s->n_seqs = p->n_seqs;
+  s->max_pages = p->max_pages;
+  s->table = p->table;
+  s->length = p->length;
+  s->refs = p->refs;
+  s->status = p->status;
+  s->ws = p->workspace;
+  return true;
+}
+
+bool attn_problem(const char* who, const dsv4cuda_paged* p, const dsv4cuda_paged_attn_shape* s,
+                  dsv4::PagedAttnProblem* a) {
+  if (!s || !paged_state(who, p, &a->pages)) {
+    if (!s) record_error("%s: bad arguments", who);
+    return false;
+  }
+  const int d = a->pages.nope + a->pages.rope_dim;
+  const long long width = static_cast<long long>(s->heads) * s->head_dim;
+  const long long qs = s->q_stride ? s->q_stride : width;
+  const long long os = s->out_stride ? s->out_stride : width;
+  if (s->n_rows < 0 || s->heads < 1 || s->heads > 65535 || s->max_new < 0 || s->max_len < 0 ||
+      s->window < 0 || s->max_keys < 0 || s->rope_dim < 0 || s->rope_dim > s->head_dim ||
+      s->rope_dim % 2 || qs < width || os < width) {
+    record_error("%s: bad shape (rope_dim even, strides at least heads * head_dim)", who);
+    return false;
+  }
+  if (s->head_dim != d || d > 1024) {
+    record_error("%s: head_dim %d, the cache's rows have nope + rope_dim = %d (at most 1024)", who,
+                 s->head_dim, d);
+    return false;
+  }
+  a->bf16 = s->bf16 != 0;
+  a->q_stride = qs;
+  a->out_stride = os;
+  a->rope_out = s->rope_dim;
+  a->total = s->n_rows;
+  a->H = s->heads;
+  a->max_new = s->max_new < s->n_rows ? s->max_new : s->n_rows;
+  a->max_len = s->max_len;
+  a->window = s->window;
+  a->max_keys = s->max_keys;
+  a->scale = s->scale;
+  a->err = dsv4::device_error_word();
+  return true;
+}
+
+}  // namespace
+
+DSV4_API size_t dsv4cuda_paged_workspace_bytes(int n_pages, int n_seqs) {
+  return n_pages < 1 || n_seqs < 1 ? 0 : dsv4::paged_workspace_bytes(n_pages, n_seqs);
+}
+
+DSV4_API int dsv4cuda_paged_fork(const dsv4cuda_paged* p, const int* dst, const int* src, int n,
+                                 void* stream) {
+  dsv4::PagedState s;
+  if (!paged_state("dsv4cuda_paged_fork", p, &s)) return -1;
+  if (n < 0 || n > p->n_seqs || (n > 0 && (!dst || !src))) {
+    record_error("dsv4cuda_paged_fork: bad arguments (at most one op per slot)");
+    return -1;
+  }
+  cudaError_t e = dsv4::paged_fork(s, dst, src, n, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) { record_error("dsv4cuda_paged_fork: %s", cudaGetErrorString(e)); return -1; }
+  return 0;
+}
+
+DSV4_API int dsv4cuda_paged_append(const dsv4cuda_paged* p, const int* slots, const int* counts,
+                                   int n, long long* rows, long long n_rows, void* stream) {
+  dsv4::PagedState s;
+  if (!paged_state("dsv4cuda_paged_append", p, &s)) return -1;
+  if (n < 0 || n > p->n_seqs || (n > 0 && (!slots || !counts)) || n_rows < 0) {
+    record_error("dsv4cuda_paged_append: bad arguments (at most one op per slot)");
+    return -1;
+  }
+  cudaError_t e =
+      dsv4::paged_append(s, slots, counts, n, rows, n_rows, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) { record_error("dsv4cuda_paged_append: %s", cudaGetErrorString(e)); return -1; }
+  return 0;
+}
+
+DSV4_API int dsv4cuda_paged_compact(const dsv4cuda_paged* p, int* table_out, int* refs_out,
+                                    void* stream) {
+  dsv4::PagedState s;
+  if (!paged_state("dsv4cuda_paged_compact", p, &s)) return -1;
+  cudaError_t e = dsv4::paged_compact(s, table_out ? table_out : s.table,
+                                      refs_out ? refs_out : s.refs,
+                                      static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) { record_error("dsv4cuda_paged_compact: %s", cudaGetErrorString(e)); return -1; }
+  return 0;
+}
+
+DSV4_API size_t dsv4cuda_paged_attn_workspace_bytes(const dsv4cuda_paged* p,
+                                                    const dsv4cuda_paged_attn_shape* shape) {
+  dsv4::PagedAttnProblem a;
+  if (!attn_problem("dsv4cuda_paged_attn_workspace_bytes", p, shape, &a)) return 0;
+  return dsv4::paged_attn_workspace_bytes(a);
+}
+
+DSV4_API int dsv4cuda_paged_attn(void* out, const void* q, const dsv4cuda_paged* p, int layer,
+                                 const int* q_start, const float* sink, const float* rope_cos,
+                                 const float* rope_sin, float* lse,
+                                 const dsv4cuda_paged_attn_shape* shape, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  dsv4::PagedAttnProblem a;
+  if (!attn_problem("dsv4cuda_paged_attn", p, shape, &a)) return -1;
+  if (layer < 0 || layer >= p->n_caches || (rope_cos == nullptr) != (rope_sin == nullptr) ||
+      (shape->n_rows > 0 && (!out || !q || !q_start))) {
+    record_error("dsv4cuda_paged_attn: bad arguments");
+    return -1;
+  }
+  if (reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(out) % 16 ||
+      reinterpret_cast<uintptr_t>(workspace) % 256) {
+    record_error("dsv4cuda_paged_attn: q and out must be 16-byte aligned, workspace 256");
+    return -1;
+  }
+  if (shape->n_rows == 0) return 0;
+  a.layer = layer;
+  a.q = q;
+  a.out = out;
+  a.q_start = q_start;
+  a.sink = sink;
+  a.rope_cos = rope_cos;
+  a.rope_sin = rope_sin;
+  a.lse = lse;
+  const size_t need = dsv4::paged_attn_workspace_bytes(a);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  void* ws = workspace;
+  if (!ws && need > 0) {
+    ws = stream_scratch("dsv4cuda_paged_attn", need, st);
+    if (!ws) return -1;
+  } else if (ws && workspace_bytes < need) {
+    record_error("dsv4cuda_paged_attn: workspace of %zu bytes, need %zu", workspace_bytes, need);
+    return -1;
+  }
+  cudaError_t e = dsv4::paged_attn_forward(a, ws, st);
+  if (e != cudaSuccess) { record_error("dsv4cuda_paged_attn: %s", cudaGetErrorString(e)); return -1; }
+  return 0;
+}
+
+DSV4_API int dsv4cuda_token_logprobs(const void* logits, int bf16, int rows, int vocab,
+                                     long long stride, const int* tokens, float* logprob,
+                                     float* entropy, int* rank, int n_top, int* top_id,
+                                     float* top_logprob, void* stream) {
+  static_assert(DSV4CUDA_MAX_TOP_ALTERNATIVES == dsv4::kMaxTopAlternatives, "limit");
+  if (rows < 0 || vocab <= 0 || stride < vocab || n_top < 0 || n_top > vocab ||
+      n_top > dsv4::kMaxTopAlternatives ||
+      (rows > 0 && (!logits || !tokens || !logprob || (n_top > 0 && (!top_id || !top_logprob)))) ||
+      reinterpret_cast<uintptr_t>(logits) % (bf16 ? 2 : 4)) {
+    record_error("dsv4cuda_token_logprobs: bad arguments (0 <= n_top <= %d and vocab, stride >= "
+                 "vocab)", dsv4::kMaxTopAlternatives);
+    return -1;
+  }
+  dsv4::LogprobProblem p;
+  p.logits = logits;
+  p.bf16 = bf16 != 0;
+  p.rows = rows;
+  p.vocab = vocab;
+  p.stride = stride;
+  p.tokens = tokens;
+  p.logprob = logprob;
+  p.entropy = entropy;
+  p.rank = rank;
+  p.top = n_top;
+  p.top_id = top_id;
+  p.top_logprob = top_logprob;
+  cudaError_t e = dsv4::token_logprobs(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) { record_error("dsv4cuda_token_logprobs: %s", cudaGetErrorString(e)); return -1; }
   return 0;
 }
 

@@ -528,6 +528,24 @@ class LatentCache:
         self.struct = KvCache(self.codes.data_ptr(), self.scales.data_ptr(),
                               self.rope.data_ptr(), nope, rope_dim, rows)
 
+    @classmethod
+    def from_tensors(cls, codes, scales, rope):
+        """A cache over tensors that are there already: uint8 codes [rows][nope]
+        and scales [rows][8], int16 rope [rows][rope_dim], contiguous."""
+        c = cls.__new__(cls)
+        for t, name, width, size in ((codes, "codes", codes.shape[1], 1), (scales, "scales", 8, 1),
+                                     (rope, "rope", rope.shape[1], 2)):
+            if (not t.is_cuda or t.element_size() != size or not t.is_contiguous()
+                    or tuple(t.shape) != (codes.shape[0], width)):
+                raise ValueError(f"{name}: a contiguous CUDA tensor [rows][..] of {size}-byte "
+                                 "elements is wanted")
+        c.codes, c.scales, c.rope = codes, scales, rope
+        c.rows, c.nope = codes.shape
+        c.rope_dim = rope.shape[1]
+        c.struct = KvCache(codes.data_ptr(), scales.data_ptr(), rope.data_ptr(), c.nope,
+                           c.rope_dim, c.rows)
+        return c
+
     @property
     def bytes_per_row(self) -> int:
         return self.nope + 8 + 2 * self.rope_dim
@@ -587,6 +605,194 @@ def attn_timing_end():
     ms = C.c_float(0)
     _check(lib.dsv4cuda_attn_timing_end(C.byref(n), C.byref(ms)))
     return n.value, ms.value
+
+
+# ------------------------------------------------------ paged latent cache --
+class Paged(C.Structure):
+    _fields_ = [("caches", vp), ("n_caches", C.c_int), ("page_size", C.c_int),
+                ("n_pages", C.c_int), ("n_seqs", C.c_int), ("max_pages", C.c_int),
+                ("table", vp), ("length", vp), ("refs", vp), ("status", vp), ("workspace", vp),
+                ("workspace_bytes", C.c_size_t)]
+
+
+class PagedAttnShape(C.Structure):
+    _fields_ = [("n_rows", C.c_int), ("heads", C.c_int), ("head_dim", C.c_int), ("bf16", C.c_int),
+                ("q_stride", C.c_longlong), ("out_stride", C.c_longlong), ("max_new", C.c_int),
+                ("max_len", C.c_int), ("window", C.c_int), ("max_keys", C.c_longlong),
+                ("rope_dim", C.c_int), ("scale", C.c_float)]
+
+
+lib.dsv4cuda_paged_workspace_bytes.restype = C.c_size_t
+lib.dsv4cuda_paged_workspace_bytes.argtypes = [C.c_int, C.c_int]
+lib.dsv4cuda_paged_fork.restype = C.c_int
+lib.dsv4cuda_paged_fork.argtypes = [vp, vp, vp, C.c_int, vp]
+lib.dsv4cuda_paged_append.restype = C.c_int
+lib.dsv4cuda_paged_append.argtypes = [vp, vp, vp, C.c_int, vp, C.c_longlong, vp]
+lib.dsv4cuda_paged_compact.restype = C.c_int
+lib.dsv4cuda_paged_compact.argtypes = [vp, vp, vp, vp]
+lib.dsv4cuda_paged_attn_workspace_bytes.restype = C.c_size_t
+lib.dsv4cuda_paged_attn_workspace_bytes.argtypes = [vp, vp]
+lib.dsv4cuda_paged_attn.restype = C.c_int
+lib.dsv4cuda_paged_attn.argtypes = [vp, vp, vp, C.c_int, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]
+lib.dsv4cuda_token_logprobs.restype = C.c_int
+lib.dsv4cuda_token_logprobs.argtypes = [vp, C.c_int, C.c_int, C.c_int, C.c_longlong, vp, vp, vp, vp,
+                                        C.c_int, vp, vp, vp]
+
+
+def _dev(t, name, dtype, numel=None):
+    """The address of a contiguous CUDA tensor of `dtype` (None passes as NULL)."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous CUDA tensor of {dtype} is wanted, got {t.dtype} "
+                         f"on {t.device}")
+    if numel is not None and t.numel() < numel:
+        raise ValueError(f"{name}: {numel} elements are wanted, got {t.numel()}")
+    return t.data_ptr()
+
+
+class PagedCache:
+    """Latents of many sequences in pages of `page_size` rows of one LatentCache
+    per layer (dsv4cuda_paged): slot s holds length[s] positions in the pages
+    table[s]; refs counts the table entries that name a page. Tables may be
+    given (int32 CUDA tensors: table [n_seqs][max_pages], length [n_seqs],
+    refs [n_pages]); see PagedCache.empty for a pool with nothing in it. All
+    calls are asynchronous on the current stream (or `stream`) and share one
+    workspace, so calls on several streams have to be ordered."""
+
+    EXHAUSTED, BAD_OP, BOUNDS = 1, 2, 4
+
+    def __init__(self, caches, page_size, table, length, refs):
+        import torch
+        self._i32, self._i64 = torch.int32, torch.int64
+        self.caches, self.page_size = list(caches), page_size
+        self.table, self.length, self.refs = table, length, refs
+        if table.dim() != 2 or length.dim() != 1 or refs.dim() != 1:
+            raise ValueError("table [n_seqs][max_pages], length [n_seqs] and refs [n_pages] are "
+                             "wanted")
+        self.n_seqs, self.max_pages = table.shape
+        self.n_pages = refs.shape[0]
+        self.status_word = torch.zeros(1, dtype=torch.int32, device=table.device)
+        need = lib.dsv4cuda_paged_workspace_bytes(self.n_pages, self.n_seqs)
+        self.workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=table.device)
+        self._arr = (KvCache * max(len(self.caches), 1))(*[c.struct for c in self.caches])
+        self.struct = Paged(C.cast(self._arr, vp), len(self.caches), page_size, self.n_pages,
+                            self.n_seqs, self.max_pages,
+                            _dev(table, "table", torch.int32),
+                            _dev(length, "length", torch.int32, self.n_seqs),
+                            _dev(refs, "refs", torch.int32), self.status_word.data_ptr(),
+                            self.workspace.data_ptr(), need)
+        self._ref = C.byref(self.struct)
+
+    @classmethod
+    def empty(cls, caches, page_size, n_seqs, max_pages):
+        """A pool of all whole pages of the caches, every slot empty."""
+        import torch
+        dev = caches[0].codes.device
+        pages = min(c.rows for c in caches) // page_size
+        i32 = dict(dtype=torch.int32, device=dev)
+        return cls(caches, page_size, torch.full((n_seqs, max_pages), -1, **i32),
+                   torch.zeros(n_seqs, **i32), torch.zeros(pages, **i32))
+
+    def append(self, slots, counts, rows=None, stream=None):
+        """Slots grow by counts tokens (int32 CUDA tensors); rows (int64) receives
+        the new tokens' cache rows, as LatentCache.write takes them."""
+        n = slots.shape[0]
+        _check(lib.dsv4cuda_paged_append(
+            self._ref, _dev(slots, "slots", self._i32), _dev(counts, "counts", self._i32, n), n,
+            _dev(rows, "rows", self._i64), 0 if rows is None else rows.numel(), _stream(stream)))
+
+    def fork(self, dst, src, stream=None):
+        """Slots dst become copies of slots src (-1: emptied); int32 CUDA tensors."""
+        n = dst.shape[0]
+        _check(lib.dsv4cuda_paged_fork(self._ref, _dev(dst, "dst", self._i32),
+                                       _dev(src, "src", self._i32, n), n, _stream(stream)))
+
+    def free(self, slots, stream=None):
+        """Gives back the pages of `slots`."""
+        import torch
+        self.fork(slots, torch.full_like(slots, -1), stream)
+
+    def compact(self, table_out=None, refs_out=None, stream=None):
+        """Moves the pages in use to the lowest page numbers; the new tables go to
+        table_out / refs_out, or in place."""
+        _check(lib.dsv4cuda_paged_compact(
+            self._ref, _dev(table_out, "table_out", self._i32, self.n_seqs * self.max_pages),
+            _dev(refs_out, "refs_out", self._i32, self.n_pages), _stream(stream)))
+
+    def status(self, clear=True):
+        """The status bits since the last clear (synchronises)."""
+        v = int(self.status_word.item())
+        if clear and v:
+            self.status_word.zero_()
+        return v
+
+
+def _paged_attn_shape(q, out, paged, max_new, max_len, scale, window, rope_cos, max_keys):
+    import torch
+    if (q.dtype not in (torch.bfloat16, torch.float32) or out.dtype is not q.dtype or q.dim() != 3
+            or out.shape != q.shape or not q.is_cuda or not out.is_cuda):
+        raise ValueError("q and out: CUDA tensors [rows][heads][head_dim] of one type, bfloat16 or "
+                         "float32")
+    n, heads, d = q.shape
+    for t, name in ((q, "q"), (out, "out")):
+        if t.stride(2) != 1 or t.stride(1) != d:
+            raise ValueError(f"{name}: the heads of a row must lie one behind the other")
+    # the stride of a single row has no meaning to torch, nor here
+    return PagedAttnShape(n, heads, d, 1 if q.dtype is torch.bfloat16 else 0,
+                          q.stride(0) if n > 1 else 0, out.stride(0) if n > 1 else 0, max_new,
+                          max_len, window, max_keys,
+                          0 if rope_cos is None else 2 * rope_cos.shape[-1], scale)
+
+
+def paged_attn_workspace_bytes(q, paged, max_new, max_len, window=0, max_keys=0) -> int:
+    """Workspace of a paged_attn call of these sizes (q as there)."""
+    shape = _paged_attn_shape(q, q, paged, max_new, max_len, 1.0, window, None, max_keys)
+    return lib.dsv4cuda_paged_attn_workspace_bytes(paged._ref, C.byref(shape))
+
+
+def paged_attn(out, q, paged: PagedCache, layer, q_start, max_new, max_len, scale, sink=None,
+               window=0, rope_cos=None, rope_sin=None, lse=None, max_keys=0, workspace=None,
+               stream=None):
+    """dsv4cuda_paged_attn: slot s's new tokens are rows q_start[s] .. q_start[s + 1] - 1
+    of q [rows][heads][head_dim] (BF16 or fp32) and the last positions of its
+    length. max_new, max_len, max_keys: the caller's bounds of a slot's new
+    tokens, its length, and the positions seen in all. workspace: a CUDA uint8
+    tensor (needed while capturing)."""
+    import torch
+    f32 = torch.float32
+    shape = _paged_attn_shape(q, out, paged, max_new, max_len, scale, window, rope_cos, max_keys)
+    n, heads, _ = q.shape
+    half = n * (shape.rope_dim // 2)
+    _check(lib.dsv4cuda_paged_attn(
+        out.data_ptr(), q.data_ptr(), paged._ref, layer,
+        _dev(q_start, "q_start", torch.int32, paged.n_seqs + 1), _dev(sink, "sink", f32, heads),
+        _dev(rope_cos, "rope_cos", f32, half), _dev(rope_sin, "rope_sin", f32, half),
+        _dev(lse, "lse", f32, n * heads), C.byref(shape),
+        None if workspace is None else workspace.data_ptr(),
+        0 if workspace is None else workspace.numel() * workspace.element_size(),
+        _stream(stream)))
+
+
+def token_logprobs(logits, tokens, logprob, entropy=None, rank=None, top_id=None, top_logprob=None,
+                   stream=None):
+    """dsv4cuda_token_logprobs: logits [rows][vocab] (fp32 or BF16, rows may lie
+    apart), tokens int32 [rows]; logprob, entropy fp32 [rows], rank int32
+    [rows], top_id int32 and top_logprob fp32 [rows][n_top]."""
+    import torch
+    f32, i32 = torch.float32, torch.int32
+    if (logits.dtype not in (f32, torch.bfloat16) or logits.dim() != 2 or not logits.is_cuda
+            or logits.stride(1) != 1):
+        raise ValueError("logits: a CUDA tensor [rows][vocab] of float32 or bfloat16, the values of "
+                         "a row one behind the other")
+    n, vocab = logits.shape
+    top = 0 if top_id is None else top_id.shape[-1]
+    _check(lib.dsv4cuda_token_logprobs(
+        logits.data_ptr(), 1 if logits.dtype is torch.bfloat16 else 0, n, vocab,
+        logits.stride(0) if n > 1 else vocab, _dev(tokens, "tokens", i32, n),
+        _dev(logprob, "logprob", f32, n), _dev(entropy, "entropy", f32, n),
+        _dev(rank, "rank", i32, n), top, _dev(top_id, "top_id", i32, n * top),
+        _dev(top_logprob, "top_logprob", f32, n * top), _stream(stream)))
 
 
 # ------------------------------------------------- speculative acceptance --

@@ -495,6 +495,128 @@ int dsv4cuda_kv_copy_rows(const dsv4cuda_kv_cache *cache, const long long *src_r
                           const long long *dst_rows, int n, void *stream);
 
 /* ---------------------------------------------------------------------
+ * The latent cache in pages (no counterpart in the reference, which holds
+ * one sequence per context). Sequences sit in slots; a slot's latents live
+ * in pages of page_size cache rows that several slots may share, and one set
+ * of tables serves the caches of all layers:
+ *   cache row of position p of slot s =
+ *     table[s][p / page_size] * page_size + p % page_size
+ * Tables, lengths and reference counts are DEVICE memory of the caller, and
+ * every call below is a function of them alone (free pages are taken in
+ * ascending order, op after op), asynchronous on stream and capturable: a
+ * captured step can admit, fork and release sequences without the host.
+ * A slot's last page, where it is not full, belongs to that slot alone;
+ * full pages may be shared. */
+#define DSV4CUDA_PAGED_MAX_LAYERS 64
+#define DSV4CUDA_PAGED_MAX_SEQS 4096
+typedef struct {
+    const dsv4cuda_kv_cache *caches; /* host array [n_caches], one per layer, of
+                                        the same row sizes, each of at least
+                                        n_pages * page_size rows */
+    int n_caches;
+    int page_size;         /* rows per page, >= 1 */
+    int n_pages;
+    int n_seqs;            /* slots */
+    int max_pages;         /* entries per slot in table */
+    int *table;            /* [n_seqs][max_pages], -1 = no page */
+    int *length;           /* [n_seqs] positions held */
+    int *refs;             /* [n_pages] table entries that name the page; 0 = free */
+    unsigned int *status;  /* bits, ORed by the calls; may be NULL:
+                              1 an op did not find the free pages it needs,
+                              2 an op that cannot be done (a slot out of range
+                                or named twice, a source that another op
+                                replaces, more tokens than table or rows hold,
+                                tokens behind a shared partial page),
+                              4 a slot beyond the bounds of an attention call */
+    void *workspace;       /* dsv4cuda_paged_workspace_bytes(), 16-byte aligned;
+                              calls that share it must not overlap */
+    size_t workspace_bytes;
+} dsv4cuda_paged;
+
+size_t dsv4cuda_paged_workspace_bytes(int n_pages, int n_seqs);
+/* Fork and free: for i < n, slot dst[i] gives back its pages and takes the
+ * place of a copy of slot src[i] (-1: it is emptied; dst[i] itself: it stays):
+ * full pages are shared, the used rows of a partial last page are copied, in
+ * every layer, into the lowest free pages (an op is counted before a later
+ * one). All sources are read as they were before the call. An op that finds
+ * no page leaves dst[i] empty (status 1); a bad op does nothing (status 2).
+ * DEVICE arrays, n <= n_seqs. */
+int dsv4cuda_paged_fork(const dsv4cuda_paged *p, const int *dst, const int *src, int n,
+                        void *stream);
+/* Append: slot slots[i] grows by counts[i] tokens, taking the lowest free
+ * pages. rows [n_rows] (may be NULL) receives the cache rows of the new
+ * tokens, op after op, as dsv4cuda_kv_write takes them. An op that does not
+ * find its pages changes nothing (status 1), nor does a bad op (status 2);
+ * the rows of their tokens are -1, which dsv4cuda_kv_write skips. */
+int dsv4cuda_paged_append(const dsv4cuda_paged *p, const int *slots, const int *counts, int n,
+                          long long *rows, long long n_rows, void *stream);
+/* Compact: the pages in use move to page numbers 0 .. (pages in use) - 1 with
+ * the fewest copies: the i-th page in use beyond that range moves into the
+ * i-th hole in it, in every layer. table_out [n_seqs][max_pages] and refs_out
+ * [n_pages] receive the new tables (NULL: in place). With tables of their own
+ * the old ones stay valid until a page is taken again: the rows that moved
+ * are still where they were. */
+int dsv4cuda_paged_compact(const dsv4cuda_paged *p, int *table_out, int *refs_out, void *stream);
+
+typedef struct {
+    int n_rows;            /* rows of q: the new tokens of all slots */
+    int heads, head_dim;   /* head_dim = nope + rope_dim of the cache */
+    int bf16;              /* q and out: 1 BF16, 0 fp32 holding BF16 values */
+    long long q_stride;    /* elements between rows of q */
+    long long out_stride;  /* and of out (0: heads * head_dim) */
+    int max_new, max_len;  /* bounds of one slot's new tokens and length */
+    int window;            /* positions a token sees, itself included; 0 all */
+    long long max_keys;    /* bound of the positions seen, summed over the slots
+                              with new tokens (0: n_seqs times what one slot of
+                              max_len and max_new sees) */
+    int rope_dim;          /* inverse RoPE on the last rope_dim dims of out */
+    float scale;
+} dsv4cuda_paged_attn_shape;
+
+size_t dsv4cuda_paged_attn_workspace_bytes(const dsv4cuda_paged *p,
+                                           const dsv4cuda_paged_attn_shape *shape);
+/* Attention of new tokens over layer `layer` of the paged cache: a prompt's
+ * chunk, verify rows, or one decode token per slot. q_start [n_seqs + 1]:
+ * slot s brings rows q_start[s] .. q_start[s + 1] - 1 of q [n_rows][heads]
+ * [head_dim], the last positions of its length[s] (their latents are already
+ * in the cache). Each sees the earlier positions and itself (the last
+ * `window` of them), as far as the table names their pages: pages behind the
+ * window may have been given back. out as q; sink [heads] (may be NULL)
+ * joins the softmax's denominator; rope_cos / rope_sin [n_rows][rope_dim / 2]
+ * (NULL: no inverse RoPE); lse [n_rows][heads] (may be NULL) receives the log
+ * of the denominator, sink included. A token that sees nothing gets 0 (lse:
+ * its sink, or -inf); one that sees a latent with a NaN or infinity gets NaN,
+ * and latents that it does not see do nothing. DEVICE pointers, q and out
+ * 16-byte aligned. workspace may be NULL (a buffer per thread and stream that
+ * grows; give one, 256-byte aligned, while capturing). head_dim = 448 + 64
+ * with at most 128 heads and strides that are multiples of 8 runs the
+ * tensor-core kernel, other shapes (head_dim <= 1024) a general one. A slot beyond max_new, max_len or max_keys sets status 4 and
+ * gets NaN. */
+int dsv4cuda_paged_attn(void *out, const void *q, const dsv4cuda_paged *p, int layer,
+                        const int *q_start, const float *sink, const float *rope_cos,
+                        const float *rope_sin, float *lse, const dsv4cuda_paged_attn_shape *shape,
+                        void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------
+ * Log probabilities of given tokens (no counterpart in the reference, whose
+ * sampler keeps no probabilities): for each of `rows` rows of vocab logits
+ * (fp32, or BF16 when bf16 != 0; `stride` elements apart)
+ *   logprob[r]  log softmax of tokens[r] (outside [0, vocab): 0)
+ *   entropy[r]  of the row's distribution; may be NULL
+ *   rank[r]     values above the token's, equal ones at a lower index
+ *               included (0 = the greedy token; outside: -1); may be NULL
+ *   top_id, top_logprob [rows][n_top]  the n_top largest, the lower index
+ *               first among equals; n_top <= 32, <= vocab; NULL when 0
+ * -inf logits are tokens that a constraint has masked; a row of nothing else
+ * has log probabilities -inf and entropy 0. A NaN or +inf makes the row's log
+ * probabilities and entropy NaN; NaN is never among the top (id -1 where
+ * fewer are left). DEVICE pointers, async on stream, capturable. */
+#define DSV4CUDA_MAX_TOP_ALTERNATIVES 32
+int dsv4cuda_token_logprobs(const void *logits, int bf16, int rows, int vocab, long long stride,
+                            const int *tokens, float *logprob, float *entropy, int *rank,
+                            int n_top, int *top_id, float *top_logprob, void *stream);
+
+/* ---------------------------------------------------------------------
  * Whole-model decode on the device: dsv4_forward_token
  * (src/dsv4/dsv4_model.c:8388, public API include/dsv4/dsv4.h:161) with
  * every weight resident in HBM. Layers of compress ratio 0 attend to the
