@@ -103,6 +103,16 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
+// The same for a box of a 3-D map.
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+      : "memory");
+}
+
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
@@ -115,5 +125,11 @@ __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
 bool make_tma_map_u8(CUtensorMap* out, const void* base, uint64_t row_bytes, uint64_t rows,
                      uint32_t box_bytes, uint32_t box_rows, bool swizzle128,
                      bool use_cache = true);
+
+// Host: the same over `planes` planes of `rows` rows, plane_pitch bytes
+// apart, with the 128-byte swizzle; not cached.
+bool make_tma_map_u8_3d(CUtensorMap* out, const void* base, uint64_t row_bytes, uint64_t rows,
+                        uint64_t planes, uint64_t plane_pitch, uint32_t box_bytes,
+                        uint32_t box_rows, uint32_t box_planes);
 
 }  // namespace dsv4

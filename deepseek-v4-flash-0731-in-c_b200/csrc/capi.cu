@@ -1677,6 +1677,10 @@ bool attn_problem(const char* who, const dsv4cuda_paged* p, const dsv4cuda_paged
                  s->head_dim, d);
     return false;
   }
+  if (!(s->scale > 0.f) || s->scale > 3e38f) {
+    record_error("%s: scale must be positive and finite", who);
+    return false;
+  }
   a->bf16 = s->bf16 != 0;
   a->q_stride = qs;
   a->out_stride = os;

@@ -16,7 +16,10 @@
 #include <cuda_bf16.h>
 
 #include "attn.cuh"
+#include "bulk.cuh"
 #include "dsv4_common.cuh"
+#include "launch.cuh"
+#include "umma.cuh"
 
 namespace dsv4 {
 namespace {
@@ -67,7 +70,12 @@ __global__ void __launch_bounds__(32 * kSimtWarps) paged_attn_simt_kernel(
   __shared__ float sm_o[kMaxDim];
   __shared__ int sm_bad;
   const int s = slot_of(p.q_start, c.n_seqs, row);
-  if (threadIdx.x == 0) sm_bad = 0;
+  if (s < 0) return;
+  const bool beyond = p.q_start[s + 1] - p.q_start[s] > p.max_new || c.length[s] > p.max_len;
+  if (threadIdx.x == 0) {
+    sm_bad = beyond;
+    if (beyond && c.status) atomicOr(c.status, kPagedBounds);
+  }
   for (int i = threadIdx.x; i < d; i += blockDim.x) sm_o[i] = 0.f;
   __syncthreads();
   float m = -INFINITY, den = 0.f;
@@ -78,7 +86,7 @@ __global__ void __launch_bounds__(32 * kSimtWarps) paged_attn_simt_kernel(
     q[u] = i < d ? load_q(p, row * p.q_stride + static_cast<long long>(h) * d + i) : 0.f;
     o[u] = 0.f;
   }
-  if (s >= 0) {
+  {
     const int last = c.length[s] - p.q_start[s + 1] + row;
     const int first = p.window > 0 ? max(0, last - p.window + 1) : 0;
     const int* table = c.table + static_cast<size_t>(s) * c.max_pages;
@@ -150,12 +158,1188 @@ __global__ void __launch_bounds__(32 * kSimtWarps) paged_attn_simt_kernel(
     p.lse[static_cast<size_t>(row) * p.H + h] = bad ? NAN : (total == 0.f ? -INFINITY : M + logf(total));
 }
 
+// ===================================================== tensor-core path ==
+//
+// Three launches. (1) The latents that any new token sees are decoded once
+// into BF16 rows, sequence after sequence, each padded to whole blocks of 64
+// keys (a prompt's chunk reads them hundreds of times; pages, freed pages
+// and broken rows are dealt with here alone), and one block lists the tiles:
+// 128 (token, head) rows of one sequence, with the key blocks they see.
+// (2) The (tile, key block) pairs, laid end to end, are cut into equal
+// shares, one per pair of CTAs, whatever the lengths of the sequences; the
+// two CTAs of a pair accumulate 256 output dims each, because 128 rows of 512
+// fp32 sums fill all of TMEM. A tile inside one share is finished there.
+// (3) Tiles cut by a share's end are merged from their fp32 parts.
+
+constexpr int kD = 512, kNope = 448, kRope = 64;
+constexpr int kRows = 128;        // (token, head) rows of a tile: M of both products
+constexpr int kKeys = 64;         // keys of a block: N of Q K^T, K of P V
+constexpr int kHalf = 256;        // output dims of a CTA: N of P V
+constexpr int kMinShare = 2;      // blocks: a smaller share costs more to merge than it saves
+// A tile of at most this many blocks carries its weights in two BF16 terms:
+// where a row sees few keys, the rounding of one weight does not average out
+// (with one term a two-key row is off by up to 2^-8 of its value sum).
+constexpr int kTwoTermBlocks = 4;
+constexpr float kLazyMargin = 8.0f;  // log2 units: the running max moves only past this
+
+struct Tile {
+  long long start;  // blocks of the tiles before
+  int blocks;       // blocks that its tokens see
+  int block0;       // first of them among the decoded blocks
+  int key0;         // position of that block's first key
+  int row0;         // first row of q
+  int tokens;       // <= 128 / H
+  int pos0;         // position of its first token
+  int bad;          // beyond the caller's bounds: NaN
+  int pad[3];
+};
+static_assert(sizeof(Tile) == 48, "one warp reads a tile's description in one go");
+
+struct PlanHead {
+  long long total;  // blocks of all tiles
+  long long share;  // blocks per pair of CTAs
+  int tiles;
+};
+
+struct TcWs {
+  PlanHead* head;
+  Tile* tiles;
+  int* pair_tile;         // [pairs] tile that a share starts in
+  uint16_t* valid;        // [blocks][4] a bit per key
+  uint16_t* broken;       // [blocks][4] keys with a NaN or infinity (decoded as zeros)
+  float* part_m;          // [pairs][2][2 halves][128] log2 units
+  float* part_den;
+  float* part_o;          // [pairs][2][128][512]
+  __nv_bfloat16* stage;   // [blocks * 64][512]
+};
+
+struct TcShape {
+  int tile_cap, tokens_per_tile, pairs;
+  long long block_cap;
+};
+
+struct TcCall {
+  PagedAttnProblem p;
+  TcShape s;
+  TcWs w;
+};
+
+__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// One slot's new tokens and the positions they see.
+struct Slot {
+  int row0, tokens, len, first, klo, blocks, tiles;
+  bool bad;
+};
+
+__device__ __forceinline__ Slot slot_geometry(const PagedAttnProblem& p, int tokens_per_tile,
+                                              int s) {
+  Slot g;
+  g.row0 = p.q_start[s];
+  const int end = p.q_start[s + 1];
+  g.len = p.pages.length[s];
+  const bool rows_ok = g.row0 >= 0 && end >= g.row0 && end <= p.total;
+  g.tokens = rows_ok ? end - g.row0 : 0;
+  g.bad = g.tokens > 0 && (g.tokens > p.max_new || g.len > p.max_len);
+  if (!rows_ok || g.bad) {
+    if (p.pages.status) atomicOr(p.pages.status, kPagedBounds);
+  }
+  g.first = g.len - g.tokens;
+  g.klo = p.window > 0 ? max(0, g.first - p.window + 1) : 0;
+  g.tiles = ceil_div(g.tokens, tokens_per_tile);
+  g.blocks = g.tokens == 0 ? 0 : g.bad ? 1 : max(1, ceil_div(max(0, g.len - g.klo), kKeys));
+  return g;
+}
+
+constexpr int kStageThreads = 288;  // 36 pieces of a row, 8 rows at a time
+constexpr int kUnit = 16;           // rows decoded together
+
+// Exclusive prefix sum over the block; *total = the sum.
+__device__ int stage_scan(int v, int* total) {
+  __shared__ int part[kStageThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += u;
+  }
+  __syncthreads();
+  if (lane == 31) part[warp] = incl;
+  __syncthreads();
+  int before = 0, sum = 0;
+#pragma unroll
+  for (int w = 0; w < kStageThreads / 32; ++w) {
+    if (w < warp) before += part[w];
+    sum += part[w];
+  }
+  *total = sum;
+  return before + incl - v;
+}
+
+// Whole block: the tiles of all slots.
+__device__ void list_tiles(const TcCall& c, const int* block_start, const int* tile_start) {
+  const PagedAttnProblem& p = c.p;
+  const int n_seqs = p.pages.n_seqs, per = c.s.tokens_per_tile;
+  const int tiles = min(tile_start[n_seqs], c.s.tile_cap);
+  if (tile_start[n_seqs] > c.s.tile_cap && threadIdx.x == 0 && p.pages.status)
+    atomicOr(p.pages.status, kPagedBounds);
+  long long done = 0;
+  for (int base = 0; base < tiles; base += kStageThreads) {
+    const int t = base + threadIdx.x;
+    Tile tile = {};
+    if (t < tiles) {
+      int lo = 0, hi = n_seqs;  // the last slot with tile_start <= t
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (tile_start[mid] <= t) lo = mid;
+        else hi = mid;
+      }
+      // slots without tokens share their start with the next one
+      const Slot g = slot_geometry(p, per, lo);
+      const int i0 = (t - tile_start[lo]) * per;
+      tile.tokens = min(per, g.tokens - i0);
+      tile.row0 = g.row0 + i0;
+      tile.pos0 = g.first + i0;
+      tile.bad = g.bad || block_start[lo] + g.blocks > c.s.block_cap;
+      if (tile.bad) {
+        tile.blocks = 1;
+        if (p.pages.status) atomicOr(p.pages.status, kPagedBounds);
+      } else {
+        const int seen_from = p.window > 0 ? max(0, tile.pos0 - p.window + 1) : 0;
+        const int b0 = min(max(0, seen_from - g.klo) / kKeys, g.blocks - 1);
+        const int b1 = min(max(ceil_div(max(0, tile.pos0 + tile.tokens - g.klo), kKeys), b0 + 1),
+                           g.blocks);
+        tile.blocks = b1 - b0;
+        tile.block0 = block_start[lo] + b0;
+        tile.key0 = g.klo + b0 * kKeys;
+      }
+    }
+    int total;
+    tile.start = done + stage_scan(tile.blocks, &total);
+    if (t < tiles) c.w.tiles[t] = tile;
+    done += total;
+  }
+  if (threadIdx.x == 0) {
+    const long long pairs = c.s.pairs;
+    long long share = (done + pairs - 1) / pairs;
+    if (share < kMinShare) share = kMinShare;
+    *c.w.head = {done, share, tiles};
+  }
+}
+
+// Latents to BF16 rows. One row is 28 pieces of 16 codes and 8 of 8 RoPE
+// values, a thread per piece, two rows in flight.
+__global__ void __launch_bounds__(kStageThreads) stage_kernel(const __grid_constant__ TcCall c) {
+  extern __shared__ int sm[];
+  __shared__ int row_broken[kUnit], row_there[kUnit];
+  const PagedAttnProblem& p = c.p;
+  const PagedState& g = p.pages;
+  int* block_start = sm;                  // [n_seqs + 1]
+  int* tile_start = sm + g.n_seqs + 1;
+  const int tid = threadIdx.x;
+  pdl_wait();
+  pdl_trigger();
+  int blocks = 0, tiles = 0;
+  for (int base = 0; base < g.n_seqs; base += kStageThreads) {
+    const int s = base + tid;
+    int nb = 0, nt = 0;
+    if (s < g.n_seqs) {
+      const Slot slot = slot_geometry(p, c.s.tokens_per_tile, s);
+      nb = slot.blocks;
+      nt = slot.tiles;
+    }
+    int tb, tt;
+    const int b = blocks + stage_scan(nb, &tb), t = tiles + stage_scan(nt, &tt);
+    if (s < g.n_seqs) {
+      block_start[s] = b;
+      tile_start[s] = t;
+    }
+    blocks += tb;
+    tiles += tt;
+  }
+  if (tid == 0) {
+    block_start[g.n_seqs] = blocks;
+    tile_start[g.n_seqs] = tiles;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    list_tiles(c, block_start, tile_start);
+    return;
+  }
+  const long long units = min(static_cast<long long>(blocks), c.s.block_cap) * (kKeys / kUnit);
+  const int piece = tid % 36, r0 = tid / 36;
+  const uint8_t* codes = g.codes[p.layer];
+  const uint8_t* scales = g.scales[p.layer];
+  const uint16_t* rope = g.rope[p.layer];
+  for (long long u = blockIdx.x - 1; u < units; u += gridDim.x - 1) {
+    const int block = static_cast<int>(u / (kKeys / kUnit));
+    int lo = 0, hi = g.n_seqs;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (block_start[mid] <= block) lo = mid;
+      else hi = mid;
+    }
+    const int len = g.length[lo], first = len - (p.q_start[lo + 1] - p.q_start[lo]);
+    const int klo = p.window > 0 ? max(0, first - p.window + 1) : 0;
+    const int t0 = klo + (block - block_start[lo]) * kKeys +
+                   static_cast<int>(u % (kKeys / kUnit)) * kUnit;
+    if (tid < kUnit) row_broken[tid] = 0;
+    __syncthreads();
+    uint4 raw[2];
+    uint32_t sc[2] = {127u, 127u};
+    bool there[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int t = t0 + r0 + 8 * k;
+      raw[k] = make_uint4(0, 0, 0, 0);
+      there[k] = false;
+      if (t < len && t / g.page < g.max_pages) {
+        const int page = g.table[static_cast<size_t>(lo) * g.max_pages + t / g.page];
+        if (page >= 0 && page < g.n_pages) {
+          const long long r = static_cast<long long>(page) * g.page + t % g.page;
+          there[k] = true;
+          if (piece < 28) {
+            raw[k] = __ldg(reinterpret_cast<const uint4*>(codes + r * kNope) + piece);
+            sc[k] = __ldg(scales + r * kKvScaleSlots + piece / 4);
+          } else {
+            raw[k] = __ldg(reinterpret_cast<const uint4*>(rope + r * kRope) + (piece - 28));
+          }
+        }
+      }
+    }
+    uint4 lo16[2], hi16[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      bool broken = false;
+      if (piece < 28) {
+        const uint32_t nan = e4m3_nan_bytes(raw[k].x) | e4m3_nan_bytes(raw[k].y) |
+                             e4m3_nan_bytes(raw[k].z) | e4m3_nan_bytes(raw[k].w);
+        uint2 a, b, d, e;
+        if (sc[k] >= 10 && sc[k] <= 134) {
+          const uint32_t k2 = (sc[k] + 120) * 0x00800080u;
+          a = e4m3x4_to_bf16_mul(raw[k].x, k2);
+          b = e4m3x4_to_bf16_mul(raw[k].y, k2);
+          d = e4m3x4_to_bf16_mul(raw[k].z, k2);
+          e = e4m3x4_to_bf16_mul(raw[k].w, k2);
+          broken = nan != 0;
+        } else {
+          const float f = e8m0_decode(sc[k]);
+          a = e4m3x4_to_bf16(raw[k].x, f);
+          b = e4m3x4_to_bf16(raw[k].y, f);
+          d = e4m3x4_to_bf16(raw[k].z, f);
+          e = e4m3x4_to_bf16(raw[k].w, f);
+          const uint32_t v[8] = {a.x, a.y, b.x, b.y, d.x, d.y, e.x, e.y};
+          broken = nan != 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            broken = broken || (v[i] & 0x7F80u) == 0x7F80u || (v[i] & 0x7F800000u) == 0x7F800000u;
+        }
+        lo16[k] = make_uint4(a.x, a.y, b.x, b.y);
+        hi16[k] = make_uint4(d.x, d.y, e.x, e.y);
+      } else {
+        const uint32_t v[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          broken = broken || (v[i] & 0x7F80u) == 0x7F80u || (v[i] & 0x7F800000u) == 0x7F800000u;
+        lo16[k] = raw[k];
+        hi16[k] = make_uint4(0, 0, 0, 0);
+      }
+      if (broken) row_broken[r0 + 8 * k] = 1;
+      if (piece == 0) row_there[r0 + 8 * k] = there[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int r = r0 + 8 * k;
+      // a broken row takes part in no sum: zero times it would not be zero
+      if (row_broken[r]) lo16[k] = hi16[k] = make_uint4(0, 0, 0, 0);
+      uint4* dst = reinterpret_cast<uint4*>(c.w.stage + (u * kUnit + r) * kD);
+      if (piece < 28) {
+        dst[2 * piece] = lo16[k];
+        dst[2 * piece + 1] = hi16[k];
+      } else {
+        dst[56 + piece - 28] = lo16[k];
+      }
+    }
+    if (tid < 32) {
+      const bool in = tid < kUnit;
+      const unsigned v = __ballot_sync(0xffffffffu, in && row_there[tid & (kUnit - 1)]);
+      const unsigned b = __ballot_sync(
+          0xffffffffu, in && row_there[tid & (kUnit - 1)] && row_broken[tid & (kUnit - 1)]);
+      if (tid == 0) {
+        c.w.valid[u] = static_cast<uint16_t>(v);
+        c.w.broken[u] = static_cast<uint16_t>(b);
+      }
+    }
+    __syncthreads();  // row_broken is cleared for the next unit
+  }
+  // the attention kernel reads the rows through the async proxy
+  asm volatile("fence.proxy.async.global;" ::: "memory");
+}
+
+constexpr int kOwnStages = 3;    // 32 KB: a block's dims of this CTA's half, also the V of P V
+constexpr int kOtherStages = 2;  // 16 KB: half of its other dims
+constexpr uint32_t kBlk = kKeys * 128;       // 64 keys x 64 dims, one swizzled box (8 KB)
+constexpr uint32_t kQBlk = kRows * 128;      // 128 rows x 64 dims (16 KB)
+constexpr uint32_t kSmQ = 0;                 // Q dims 256-511 (64 KB)
+constexpr uint32_t kSmOwn = 4 * kQBlk;
+constexpr uint32_t kSmOther = kSmOwn + kOwnStages * 4 * kBlk;
+constexpr uint32_t kSmP = kSmOther + kOtherStages * 2 * kBlk;
+constexpr uint32_t kPBytes = kRows * kKeys * 2;            // P, and what its rounding left
+constexpr uint32_t kSmBar = kSmP + 2 * kPBytes;
+constexpr uint32_t kSmMax = kSmBar + 256;    // [2 blocks][2 key halves][128] row maxima
+constexpr uint32_t kTcBytes = kSmMax + 2 * 2 * kRows * 4;
+static_assert(kTcBytes <= 232448, "beyond the shared memory of a CTA");
+constexpr uint32_t kColS = 256, kColQ = 384, kCols = 512;  // O: 0-255, S: two of 64, Q dims 0-255
+
+constexpr int kSoftmaxWarps = 8, kLoadWarps = 4;
+constexpr int kWarpTma = kSoftmaxWarps + kLoadWarps, kWarpMma = kWarpTma + 1;
+constexpr int kTcThreads = 32 * (kWarpMma + 1);
+
+struct Bars {
+  uint64_t full_own[kOwnStages], empty_own[kOwnStages];
+  uint64_t full_other[kOtherStages], empty_other[kOtherStages];
+  uint64_t s_full[2], p_full, pv_done, q_full, q_free, fin, pair[4];
+  uint32_t tmem;
+  int abort_flag;
+};
+static_assert(sizeof(Bars) <= 256, "barriers exceed their room");
+
+// The tile that holds block F (whole warp; F < total): 32 probes a step.
+__device__ __forceinline__ int find_tile(const Tile* tiles, int n, long long F) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = n;  // tiles[lo].start <= F
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32;
+    const int at = lo + lane * step;
+    const bool ok = at < hi && tiles[at].start <= F;
+    const int k = __popc(__ballot_sync(0xffffffffu, ok)) - 1;
+    lo += k * step;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
+
+// A piece of a tile that one share holds.
+struct Segment {
+  Tile t;
+  int j0, j1;     // its blocks
+};
+
+// Walks a share's segments: every role runs the same walk.
+struct Walk {
+  const Tile* tiles;
+  long long F, end;
+  int t;
+  __device__ bool next(Segment& s) {
+    if (F >= end) return false;
+    s.t = tiles[t++];
+    s.j0 = static_cast<int>(F - s.t.start);
+    const long long left = end - F;
+    s.j1 = s.t.blocks - s.j0 > left ? s.j0 + static_cast<int>(left) : s.t.blocks;
+    F += s.j1 - s.j0;
+    return true;
+  }
+};
+
+__device__ __forceinline__ uint4 load_q8(const PagedAttnProblem& p, long long at) {
+  if (p.bf16)
+    return __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q) + at));
+  const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at);
+  const float4 a = __ldg(s), b = __ldg(s + 1);
+  return make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y),
+                    pack_bf16x2(b.z, b.w));
+}
+
+// 8 output dims of a row.
+__device__ __forceinline__ void store_o8(const PagedAttnProblem& p, long long at, const float* v) {
+  const uint4 w = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                             pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  if (p.bf16) {
+    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + at) = w;
+  } else {
+    float4* d = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      d[i] = make_float4(__uint_as_float(u[2 * i] << 16), __uint_as_float(u[2 * i] & 0xFFFF0000u),
+                         __uint_as_float(u[2 * i + 1] << 16),
+                         __uint_as_float(u[2 * i + 1] & 0xFFFF0000u));
+  }
+}
+
+// Inverse RoPE of 32 dims from d0 on, the pairs from r0 on; the row's factors
+// are loaded together.
+__device__ __forceinline__ void rope_dims(const PagedAttnProblem& p, long long row, int d0, int r0,
+                                          float (&v)[32]) {
+  const long long ra = row * (p.rope_out / 2);
+  float cs[16], sn[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const bool in = d0 + 2 * i >= r0;
+    const long long at = ra + (in ? (d0 + 2 * i - r0) / 2 : 0);
+    cs[i] = __ldg(p.rope_cos + at);
+    sn[i] = __ldg(p.rope_sin + at);
+    if (!in) {
+      cs[i] = 1.f;
+      sn[i] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float x0 = v[2 * i], x1 = v[2 * i + 1];
+    v[2 * i] = x0 * cs[i] + x1 * sn[i];
+    v[2 * i + 1] = x1 * cs[i] - x0 * sn[i];
+  }
+}
+
+// Denominator with the sink and what the sums are divided by, from the
+// running max m and sum den of the scores in log2 units.
+struct Norm {
+  float scale;  // of the value sums
+  float lse;
+};
+__device__ __forceinline__ Norm finish(float m, float den, const float* sink, int h) {
+  const float s2 = sink ? sink[h] * kLog2e : -INFINITY;
+  const float mx = fmaxf(m, s2);
+  if (den != den) return {NAN, NAN};
+  if (mx == -INFINITY) return {0.f, -INFINITY};  // nothing seen, no sink
+  const float f = m == -INFINITY ? 0.f : exp2f(m - mx);
+  const float total = den * f + exp2f(s2 - mx);
+  return {f / total, (mx + log2f(total)) * 0.69314718055994531f};
+}
+
+// Waits suspended in hardware rather than spinning: the softmax warps need
+// the issue slots.
+__device__ __forceinline__ bool long_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                          unsigned* err) {
+  auto wait = [&] {
+    uint32_t ok;
+    asm volatile(
+        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;"
+        " selp.u32 %0, 1, 0, p; }"
+        : "=r"(ok)
+        : "r"(smem_addr(bar)), "r"(parity), "r"(20000u)  // at most 20 us at a time
+        : "memory");
+    return ok != 0;
+  };
+  if (wait()) return true;
+  const unsigned long long t0 = global_timer_ns();
+  while (!wait()) {
+    if (*abort_flag) return false;
+    if (global_timer_ns() - t0 > kWaitLimitNs) {
+      if (err) atomicOr(err, kErrWait);
+      *abort_flag = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
+// The two warps of 32 rows meet (a barrier in shared memory, because a named
+// one could not give up).
+struct PairSync {
+  uint64_t* bar;
+  unsigned done;
+  volatile int* abort_flag;
+  unsigned* err;
+  __device__ __forceinline__ bool operator()() {
+    mbar_arrive(bar);
+    const bool ok = long_wait(bar, done & 1, abort_flag, err);
+    ++done;
+    return __all_sync(0xffffffffu, ok);
+  }
+};
+
+// 32 scores of a row (this thread's half of the block's keys) to weights.
+// kPlain: every key is visible and one BF16 term is enough.
+struct RowState {
+  float m, den;
+};
+template <bool kPlain>
+__device__ __forceinline__ bool softmax_block(uint32_t s_col, uint32_t mask, bool two_terms,
+                                              float sc2, float* max_mine, const float* max_other,
+                                              PairSync& meet, bool& ok, RowState& st, float& alpha,
+                                              uint32_t (&hi)[16], uint32_t (&lo)[16]) {
+  uint32_t r[32];
+  tmem_ld32(s_col, r);
+  float tm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    if (!kPlain && !((mask >> i) & 1u)) r[i] = 0xFF800000u;
+    tm[i & 3] = fmaxf(tm[i & 3], __uint_as_float(r[i]));
+  }
+  const float mine = fmaxf(fmaxf(tm[0], tm[1]), fmaxf(tm[2], tm[3]));
+  *max_mine = mine;
+  ok = meet();
+  const float tmax = fmaxf(mine, *max_other) * sc2;  // scale > 0
+  // the running max moves only when a score exceeds it by the margin:
+  // weights stay <= 2^8 and O is rarely rescaled
+  bool rescale = false;
+  alpha = 1.f;
+  if (tmax != -INFINITY) {
+    if (st.m == -INFINITY) {
+      st.m = tmax;
+    } else if (tmax > st.m + kLazyMargin) {
+      alpha = ex2_approx(st.m - tmax);
+      st.m = tmax;
+      rescale = true;
+    }
+  }
+  const float neg = st.m == -INFINITY ? 0.f : -st.m;
+  float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) {
+    const float e0 = ex2_approx(fmaf(__uint_as_float(r[i]), sc2, neg));
+    const float e1 = ex2_approx(fmaf(__uint_as_float(r[i + 1]), sc2, neg));
+    part[(i >> 1) & 3] += e0 + e1;
+    hi[i / 2] = pack_bf16x2(e0, e1);
+    if (!kPlain && two_terms)
+      lo[i / 2] = pack_bf16x2(e0 - __uint_as_float(hi[i / 2] << 16),
+                              e1 - __uint_as_float(hi[i / 2] & 0xFFFF0000u));
+  }
+  st.den = st.den * alpha + ((part[0] + part[1]) + (part[2] + part[3]));
+  return rescale;
+}
+
+// One share of (tile, block) pairs and one half of the output dims. Roles:
+//   warps 0-7  softmax and epilogue: row = TMEM lane, two threads a row, one
+//              for each half of a block's keys (and of the CTA's output dims)
+//   warps 8-11 Q of the next segment, once this one's last Q K^T is done: dims
+//              0-255 to TMEM (the first half of them waits in registers)
+//   warp 12    key blocks and Q's dims 256-511 by TMA (one lane)
+//   warp 13    TMEM allocation and MMA issue
+// Per block: S = Q K^T (32 MMAs of 128 x 64 x 16, the other half's dims first
+// so that their slots are free early), P = 2^(S - m) in BF16 to shared
+// memory, O += P V (4 MMAs of 128 x 256 x 16, the own half read MN-major).
+// P V of a block is issued after Q K^T of the next, so the tensor pipe works
+// while the softmax does.
+__global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
+    const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap qmap,
+    const __grid_constant__ TcCall c) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = smem_addr(smem);
+  Bars* bars = reinterpret_cast<Bars*>(smem + kSmBar);
+  volatile int* abort_flag = &bars->abort_flag;
+  const PagedAttnProblem& p = c.p;
+  unsigned* err = p.err;
+  const int half = blockIdx.x & 1, pair = blockIdx.x >> 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kOwnStages; ++i) {
+      mbar_init(&bars->full_own[i], 1);
+      mbar_init(&bars->empty_own[i], 1);
+    }
+    for (int i = 0; i < kOtherStages; ++i) {
+      mbar_init(&bars->full_other[i], 1);
+      mbar_init(&bars->empty_other[i], 1);
+    }
+    mbar_init(&bars->s_full[0], 1);
+    mbar_init(&bars->s_full[1], 1);
+    mbar_init(&bars->p_full, 32 * kSoftmaxWarps);
+    mbar_init(&bars->pv_done, 1);
+    mbar_init(&bars->q_full, 32 * kLoadWarps + 1);  // and the TMA warp's
+    mbar_init(&bars->q_free, 1);
+    mbar_init(&bars->fin, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(&bars->pair[i], 64);
+    bars->abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == kWarpTma && lane == 0) {
+    tma_prefetch_desc(&map);
+    tma_prefetch_desc(&qmap);
+  }
+  pdl_wait();  // the plan and the decoded rows
+  pdl_trigger();
+  if (warp == kWarpMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_addr(&bars->tmem)),
+                 "r"(kCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem;
+
+  const PlanHead head = *c.w.head;
+  Walk walk;
+  walk.tiles = c.w.tiles;
+  walk.F = static_cast<long long>(pair) * head.share;
+  walk.end = min(head.total, walk.F + head.share);
+  walk.t = walk.F < walk.end ? find_tile(c.w.tiles, head.tiles, walk.F) : 0;
+  Segment seg;
+
+  if (warp < kSoftmaxWarps) {
+    // ----------------------------------------------------- softmax, epilogue
+    if (half == 0 && threadIdx.x == 0 && walk.F < walk.end) c.w.pair_tile[pair] = walk.t;
+    const int side = warp >> 2, w4 = warp & 3;
+    const int row = w4 * 32 + lane;
+    const int tok = row / p.H, h = row - tok * p.H;
+    const uint32_t lanes = static_cast<uint32_t>(w4 * 32) << 16;
+    const uint32_t o_cols = tmem + lanes + side * (kHalf / 2);
+    const uint32_t prow = base + kSmP + (row >> 3) * 1024 + (row & 7) * 128;
+    float* maxima = reinterpret_cast<float*>(smem + kSmMax);
+    float* max_mine = maxima + side * kRows + row;
+    const float* max_other = maxima + (1 - side) * kRows + row;
+    const float sc2 = p.scale * kLog2e;
+    const long long share0 = walk.F;
+    PairSync meet = {&bars->pair[w4], 0, abort_flag, err};
+    unsigned n = 0;  // blocks done by this CTA
+    bool ok = true;
+    while (ok && walk.next(seg)) {
+      const Tile& t = seg.t;
+      const bool mine = tok < t.tokens;
+      const int last = mine ? t.pos0 + tok : -1;  // the position of this row's token
+      const int from = p.window > 0 ? max(0, last - p.window + 1) : 0;
+      const bool two_terms = t.blocks <= kTwoTermBlocks;
+      RowState st = {-INFINITY, 0.f};
+      bool bad = t.bad != 0;
+      const unsigned long long* valid =
+          reinterpret_cast<const unsigned long long*>(c.w.valid) + t.block0;
+      const unsigned long long* brk =
+          reinterpret_cast<const unsigned long long*>(c.w.broken) + t.block0;
+      unsigned long long mask_next = valid[seg.j0], broken_next = brk[seg.j0];
+      for (int j = seg.j0; j < seg.j1; ++j, ++n) {
+        const int key0 = t.key0 + j * kKeys;
+        unsigned long long mask = mask_next;
+        const unsigned long long broken = broken_next;
+        if (j + 1 < seg.j1) {
+          mask_next = valid[j + 1];
+          broken_next = brk[j + 1];
+        }
+        // bits 0 .. last - key0, and from there on the window's first
+        const int hi_key = last - key0, lo_key = from - key0;
+        mask &= hi_key < 0 ? 0ull : hi_key >= 63 ? ~0ull : (2ull << hi_key) - 1;
+        if (lo_key > 0) mask &= lo_key > 63 ? 0ull : ~0ull << lo_key;
+        if (broken & mask) bad = true;
+        mask &= ~broken;
+        const bool plain = __all_sync(0xffffffffu, mask == ~0ull) && !two_terms;
+        const uint32_t mask32 = static_cast<uint32_t>(mask >> (32 * side));
+        const int sb = n & 1;
+        if (!__all_sync(0xffffffffu, long_wait(&bars->s_full[sb], (n >> 1) & 1, abort_flag, err))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t s_col = tmem + lanes + kColS + sb * kKeys + side * 32;
+        const int buf = sb * 2 * kRows;
+        uint32_t hi[16], lo[16];
+        float alpha;
+        const bool rescale =
+            plain ? softmax_block<true>(s_col, mask32, false, sc2, max_mine + buf, max_other + buf,
+                                        meet, ok, st, alpha, hi, lo)
+                  : softmax_block<false>(s_col, mask32, two_terms, sc2, max_mine + buf,
+                                         max_other + buf, meet, ok, st, alpha, hi, lo);
+        if (!ok) break;
+        // P V of the block before has read P, and O holds all blocks before
+        if (n > 0 &&
+            !__all_sync(0xffffffffu, long_wait(&bars->pv_done, (n - 1) & 1, abort_flag, err))) {
+          ok = false;
+          break;
+        }
+        if (__any_sync(0xffffffffu, rescale)) {
+          tc_fence_after();
+#pragma unroll 1
+          for (int cb = 0; cb < kHalf / 2; cb += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_cols + cb, o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st32(o_cols + cb, o);
+          }
+          tmem_st_wait();
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          st_shared_v4(prow + (((4 * side + k) ^ (row & 7)) << 4),
+                       make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]));
+        if (two_terms) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            st_shared_v4(prow + kPBytes + (((4 * side + k) ^ (row & 7)) << 4),
+                         make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]));
+        }
+        fence_async_smem();
+        tc_fence_before();
+        mbar_arrive(&bars->p_full);
+      }
+      if (!ok) break;
+      // the row's denominator: both threads' sums (the buffer of the block
+      // before the last one is free)
+      const int buf = (n & 1) * 2 * kRows;
+      max_mine[buf] = st.den;
+      if (!(ok = meet())) break;
+      float den = st.den + max_other[buf];
+      if (!(ok = meet())) break;  // read before the next segment writes it
+      if (!__all_sync(0xffffffffu, long_wait(&bars->pv_done, (n - 1) & 1, abort_flag, err))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      if (bad) den = NAN;
+      const bool done = seg.j0 == 0 && seg.j1 == t.blocks;
+      if (done) {
+        const Norm norm = finish(st.m, den, p.sink, h < p.H && mine ? h : 0);
+        const long long at = static_cast<long long>(t.row0 + tok);
+        if (mine && half == 0 && side == 0 && p.lse) p.lse[at * p.H + h] = norm.lse;
+        const int r0 = kD - p.rope_out;
+#pragma unroll 1
+        for (int cb = 0; cb < kHalf / 2; cb += 32) {
+          uint32_t o[32];
+          tmem_ld32(o_cols + cb, o);
+          if (mine) {
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]) * norm.scale;
+            const int d0 = half * kHalf + side * (kHalf / 2) + cb;
+            if (p.rope_cos && d0 + 32 > r0) rope_dims(p, at, d0, r0, v);
+            const long long to = at * p.out_stride + static_cast<long long>(h) * kD + d0;
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) store_o8(p, to + i, v + i);
+          }
+        }
+      } else {
+        // a part: slot 0 where the tile began in an earlier share, else 1
+        const int slot = t.start < share0 ? 0 : 1;
+        const long long at = pair * 2 + slot;
+#pragma unroll 1
+        for (int cb = 0; cb < kHalf / 2; cb += 32) {
+          uint32_t o[32];
+          tmem_ld32(o_cols + cb, o);
+          if (mine) {
+            float4* dst = reinterpret_cast<float4*>(c.w.part_o + (at * kRows + row) * kD +
+                                                    half * kHalf + side * (kHalf / 2) + cb);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              dst[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                   __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+          }
+        }
+        if (mine && side == 0) {
+          c.w.part_m[(at * 2 + half) * kRows + row] = st.m;
+          c.w.part_den[(at * 2 + half) * kRows + row] = den;
+        }
+      }
+      tc_fence_before();  // O may be overwritten once the next block's P is there
+    }
+  } else if (warp < kWarpTma) {
+    // ------------------------------------------------------------- Q loaders
+    const int w4 = warp & 3, row = w4 * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(w4 * 32) << 16;
+    const int tok = row / p.H, h = row - tok * p.H;
+    const int size = p.bf16 ? 2 : 4;
+    unsigned it = 0;
+    while (walk.next(seg)) {
+      const Tile& t = seg.t;
+      const long long at = tok < t.tokens ? static_cast<long long>(t.row0 + tok) * p.q_stride +
+                                                static_cast<long long>(h) * kD
+                                          : -1ll;
+      uint4 a[16] = {};
+      if (at >= 0) {
+        bulk_prefetch_l2(static_cast<const uint8_t*>(p.q) + (at + kHalf / 2) * size,
+                         (kHalf / 2 + kHalf) * size);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) a[i] = load_q8(p, at + 8 * i);
+      }
+      if (it > 0 &&
+          !__all_sync(0xffffffffu, long_wait(&bars->q_free, (it - 1) & 1, abort_flag, err)))
+        break;
+      tc_fence_after();
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t r[32];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            r[4 * i] = a[8 * q + i].x;
+            r[4 * i + 1] = a[8 * q + i].y;
+            r[4 * i + 2] = a[8 * q + i].z;
+            r[4 * i + 3] = a[8 * q + i].w;
+          }
+          tmem_st32(tmem + lanes + kColQ + 64 * k + 32 * q, r);
+        }
+        if (k == 0 && at >= 0) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) a[i] = load_q8(p, at + 128 + 8 * i);
+        }
+      }
+      if (!p.bf16) {  // fp32 rows: converted on their way to shared memory
+        for (int i0 = 0; i0 < 32; i0 += 16) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const long long b = __shfl_sync(0xffffffffu, at, i0 + i);
+            if (b >= 0) a[i] = load_q8(p, b + kHalf + 8 * lane);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            st_shared_v4(base + kSmQ + sw128_off(w4 * 32 + i0 + i, lane, kRows), a[i]);
+        }
+        fence_async_smem();
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&bars->q_full);
+      ++it;
+    }
+  } else if (warp == kWarpTma) {
+    // ------------------------------------------------------------ key blocks
+    if (lane == 0) {
+      asm volatile("fence.proxy.async.global;" ::: "memory");
+      unsigned no = 0, nw = 0, it = 0;  // other / own slots and Q tiles filled so far
+      bool ok = true;
+      const uint32_t q_rows = (kRows / p.H) * p.H;
+      auto load_q = [&](const Tile& t) {  // dims 256-511
+        if (it > 0 && !long_wait(&bars->q_free, (it - 1) & 1, abort_flag, err)) return false;
+        ++it;
+        if (!p.bf16) {
+          mbar_arrive(&bars->q_full);
+          return true;
+        }
+        mbar_arrive_expect_tx(&bars->q_full, 4 * 128 * q_rows);
+        for (int b = 0; b < 4; ++b)
+          tma_load_3d(smem + kSmQ + b * kQBlk, &qmap, 512 + b * 128, 0, t.row0, &bars->q_full);
+        return true;
+      };
+      while (ok && walk.next(seg)) {
+        // the first key blocks are on their way before Q's room is free
+        bool q_due = true;
+        for (int j = seg.j0; j < seg.j1 && ok; ++j) {
+          const int y = (seg.t.block0 + j) * kKeys;
+          for (int q = 0; q < 2; ++q, ++no) {
+            const unsigned s = no % kOtherStages;
+            if (!long_wait(&bars->empty_other[s], ((no / kOtherStages) & 1) ^ 1, abort_flag, err)) {
+              ok = false;
+              break;
+            }
+            mbar_arrive_expect_tx(&bars->full_other[s], 2 * kBlk);
+            for (int b = 0; b < 2; ++b)
+              tma_load_2d(smem + kSmOther + (s * 2 + b) * kBlk, &map,
+                          (1 - half) * 512 + q * 256 + b * 128, y, &bars->full_other[s]);
+          }
+          if (!ok) break;
+          if (q_due) {
+            q_due = false;
+            if (!load_q(seg.t)) { ok = false; break; }
+          }
+          const unsigned s = nw % kOwnStages;
+          if (!long_wait(&bars->empty_own[s], ((nw / kOwnStages) & 1) ^ 1, abort_flag, err)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&bars->full_own[s], 4 * kBlk);
+          for (int b = 0; b < 4; ++b)
+            tma_load_2d(smem + kSmOwn + (s * 4 + b) * kBlk, &map, half * 512 + b * 128, y,
+                        &bars->full_own[s]);
+          ++nw;
+        }
+      }
+      // no copy may be in flight when the CTA ends: the last one of each slot
+      for (unsigned i = no > kOtherStages ? no - kOtherStages : 0; i < no; ++i)
+        mbar_wait(&bars->full_other[i % kOtherStages], (i / kOtherStages) & 1, err);
+      for (unsigned i = nw > kOwnStages ? nw - kOwnStages : 0; i < nw; ++i)
+        mbar_wait(&bars->full_own[i % kOwnStages], (i / kOwnStages) & 1, err);
+      if (it > 0) mbar_wait(&bars->q_full, (it - 1) & 1, err);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------- MMA issue
+    constexpr uint32_t idesc_qk = umma_idesc_bf16(kRows, kKeys, false);
+    constexpr uint32_t idesc_pv = umma_idesc_bf16(kRows, kHalf, true);
+    const uint64_t q_desc = umma_desc(base + kSmQ, 16, 1024);
+    const uint64_t p_desc = umma_desc(base + kSmP, 16, 1024);
+    auto waits = [&](uint64_t* bar, unsigned parity) {
+      const bool w = __all_sync(0xffffffffu, long_wait(bar, parity & 1, abort_flag, err));
+      tc_fence_after();
+      return w;
+    };
+    // Q K^T over 128 dims at column blocks cb, cb + 1 of a 256-dim half
+    auto qk = [&](uint32_t s_col, uint64_t k_desc, int q_half, int cb, bool first) {
+      if (q_half == 0) {
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          umma_bf16_ts_e(s_col, tmem + kColQ + cb * 32 + kk * 8,
+                         k_desc + ((kk >> 2) * kBlk + (kk & 3) * 32) / 16, idesc_qk,
+                         (first && kk == 0) ? 0u : 1u);
+      } else {
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          umma_bf16_e(s_col, q_desc + ((cb + (kk >> 2)) * kQBlk + (kk & 3) * 32) / 16,
+                      k_desc + ((kk >> 2) * kBlk + (kk & 3) * 32) / 16, idesc_qk,
+                      (first && kk == 0) ? 0u : 1u);
+      }
+    };
+    unsigned n = 0, no = 0, nw = 0, it = 0;
+    // O += P V of block number nb of this CTA
+    auto pv = [&](unsigned nb, bool first, bool two_terms) {
+      if (!waits(&bars->p_full, nb)) return false;
+      const unsigned s = nb % kOwnStages;
+      const uint64_t v = umma_desc(base + kSmOwn + s * 4 * kBlk, kBlk, 1024);
+#pragma unroll
+      for (int kk = 0; kk < kKeys / 16; ++kk)
+        umma_bf16_e(tmem, p_desc + kk * 2, v + kk * 128, idesc_pv, (first && kk == 0) ? 0u : 1u);
+      if (two_terms) {
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk)
+          umma_bf16_e(tmem, p_desc + kPBytes / 16 + kk * 2, v + kk * 128, idesc_pv, 1u);
+      }
+      umma_commit_e(&bars->pv_done);
+      umma_commit_e(&bars->empty_own[s]);
+      return true;
+    };
+    bool ok = true;
+    while (ok && walk.next(seg)) {
+      if (!waits(&bars->q_full, it)) break;
+      ++it;
+      const bool two_terms = seg.t.blocks <= kTwoTermBlocks;
+      for (int j = seg.j0; j < seg.j1 && ok; ++j) {
+        const uint32_t s_col = tmem + kColS + (n & 1) * kKeys;
+        for (int q = 0; q < 2; ++q, ++no) {
+          const unsigned s = no % kOtherStages;
+          if (!waits(&bars->full_other[s], no / kOtherStages)) { ok = false; break; }
+          qk(s_col, umma_desc(base + kSmOther + s * 2 * kBlk, 16, 1024), 1 - half, 2 * q, q == 0);
+          umma_commit_e(&bars->empty_other[s]);
+        }
+        if (!ok) break;
+        const unsigned s = nw % kOwnStages;
+        if (!waits(&bars->full_own[s], nw / kOwnStages)) { ok = false; break; }
+        const uint64_t k_desc = umma_desc(base + kSmOwn + s * 4 * kBlk, 16, 1024);
+        qk(s_col, k_desc, half, 0, false);
+        qk(s_col, k_desc + 2 * kBlk / 16, half, 2, false);
+        ++nw;
+        umma_commit_e(&bars->s_full[n & 1]);
+        if (j + 1 == seg.j1) umma_commit_e(&bars->q_free);
+        if (j > seg.j0 && !pv(n - 1, j - 1 == seg.j0, two_terms)) { ok = false; break; }
+        ++n;
+      }
+      if (ok && !pv(n - 1, seg.j1 - seg.j0 == 1, two_terms)) ok = false;
+    }
+    umma_commit_e(&bars->fin);
+    mbar_wait(&bars->fin, 0, err);
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kWarpMma)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols)
+                 : "memory");
+}
+
+// Tiles that a share's end cuts: a warp per (cut, row), 16 dims a lane.
+constexpr int kMergeWarps = 8;
+__global__ void __launch_bounds__(32 * kMergeWarps) paged_attn_merge_kernel(
+    const __grid_constant__ TcCall c) {
+  pdl_wait();
+  pdl_trigger();
+  const PagedAttnProblem& p = c.p;
+  const int cut = blockIdx.y + 1;
+  const int row = blockIdx.x * kMergeWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const PlanHead head = *c.w.head;
+  const long long F = cut * head.share;
+  if (F >= head.total) return;
+  const Tile t = c.w.tiles[c.w.pair_tile[cut]];
+  // the first cut inside a tile merges it
+  if (t.start >= F || t.start < F - head.share) return;
+  const int tok = row / p.H, h = row - tok * p.H;
+  if (tok >= t.tokens) return;
+  const int n = static_cast<int>((t.start + t.blocks - 1) / head.share) - (cut - 1) + 1;
+  auto part = [&](int i) { return static_cast<long long>(cut - 1 + i) * 2 + (i == 0 ? 1 : 0); };
+  // Each lane holds the weights of parts lane, lane + 32, ...; per half of the
+  // dims, whose maxima may differ in the last bit.
+  constexpr int kPer = 3;  // shares: at most 96 pairs
+  float wt[2][kPer], scale[2], lse = 0.f;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    float m[kPer], d[kPer], M = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int i = lane + 32 * k;
+      const long long at = (part(i) * 2 + half) * kRows + row;
+      m[k] = i < n ? c.w.part_m[at] : -INFINITY;
+      d[k] = i < n ? c.w.part_den[at] : 0.f;
+      M = fmaxf(M, m[k]);
+    }
+    M = warp_max(M);
+    float den = 0.f;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      wt[half][k] = m[k] == -INFINITY ? 0.f : exp2f(m[k] - M);
+      den += d[k] * wt[half][k];
+      // a part that saw a broken latent and nothing else has no maximum
+      if (d[k] != d[k]) den = NAN;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
+    const Norm norm = finish(M, den, p.sink, h);
+    scale[half] = norm.scale;
+    if (half == 0) lse = norm.lse;
+  }
+  // 16 bytes a lane, so that a warp's loads are whole lines: dims 4 lane +
+  // 128 q, q = 0 .. 3
+  float acc[4][4] = {};
+  constexpr int kBatch = 4;
+  for (int i0 = 0; i0 < n; i0 += kBatch) {
+    float4 v[kBatch][4];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+      if (i0 + k < n) {
+        const float* src = c.w.part_o + (part(i0 + k) * kRows + row) * kD + 4 * lane;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[k][q] = *reinterpret_cast<const float4*>(src + 128 * q);
+      }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int i = i0 + k, r = i >> 5;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const float mine = r == 0 ? wt[half][0] : r == 1 ? wt[half][1] : wt[half][2];
+        const float f = __shfl_sync(0xffffffffu, mine, i & 31);
+        if (i < n) {
+#pragma unroll
+          for (int q = 2 * half; q < 2 * half + 2; ++q) {
+            acc[q][0] = fmaf(v[k][q].x, f, acc[q][0]);
+            acc[q][1] = fmaf(v[k][q].y, f, acc[q][1]);
+            acc[q][2] = fmaf(v[k][q].z, f, acc[q][2]);
+            acc[q][3] = fmaf(v[k][q].w, f, acc[q][3]);
+          }
+        }
+      }
+    }
+  }
+  const long long at = static_cast<long long>(t.row0 + tok);
+  const int r0 = kD - p.rope_out;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int d0 = 128 * q + 4 * lane;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[q][i] *= scale[q >> 1];
+    if (p.rope_cos) {
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        if (d0 + i >= r0) {
+          const long long ra = at * (p.rope_out / 2) + (d0 + i - r0) / 2;
+          const float cs = p.rope_cos[ra], sn = p.rope_sin[ra];
+          const float y0 = acc[q][i] * cs + acc[q][i + 1] * sn;
+          const float y1 = acc[q][i + 1] * cs - acc[q][i] * sn;
+          acc[q][i] = y0;
+          acc[q][i + 1] = y1;
+        }
+      }
+    }
+    const long long to = at * p.out_stride + static_cast<long long>(h) * kD + d0;
+    const uint2 w = make_uint2(pack_bf16x2(acc[q][0], acc[q][1]), pack_bf16x2(acc[q][2], acc[q][3]));
+    if (p.bf16)
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + to) = w;
+    else
+      *reinterpret_cast<float4*>(static_cast<float*>(p.out) + to) =
+          make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u),
+                      __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u));
+  }
+  if (p.lse && lane == 0) p.lse[at * p.H + h] = lse;
+}
+
+// ------------------------------------------------------------------- host --
+
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 2)
+    return 148;
+  return n;
+}
+
+bool tc_shape_ok(const PagedAttnProblem& p) {
+  return p.pages.nope == kNope && p.pages.rope_dim == kRope && p.H <= kRows &&
+         p.q_stride % 8 == 0 && p.out_stride % 8 == 0 && p.rope_out % 2 == 0;
+}
+
+TcShape tc_shape(const PagedAttnProblem& p) {
+  TcShape s;
+  s.tokens_per_tile = kRows / p.H;
+  const long long active = p.pages.n_seqs < p.total ? p.pages.n_seqs : p.total;
+  const long long tiles = p.total / s.tokens_per_tile + active;
+  s.tile_cap = static_cast<int>(tiles < p.total ? tiles : p.total);
+  // positions that one slot's tokens see
+  long long one = p.max_len;
+  if (p.window > 0 && static_cast<long long>(p.max_new) + p.window - 1 < one)
+    one = static_cast<long long>(p.max_new) + p.window - 1;
+  long long keys = active * one;
+  if (p.max_keys > 0 && p.max_keys < keys) keys = p.max_keys;
+  s.block_cap = keys / kKeys + active;  // each slot rounds up to a whole block
+  const long long per_tile = one / kKeys + 2;
+  const long long most = (s.tile_cap * per_tile + kMinShare - 1) / kMinShare;
+  const int pairs = sm_count() / 2 < 96 ? sm_count() / 2 : 96;
+  s.pairs = static_cast<int>(most < pairs ? (most < 1 ? 1 : most) : pairs);
+  return s;
+}
+
+size_t up(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
+
+size_t tc_carve(const TcShape& s, char* base, TcWs* w) {
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    char* at = base + off;
+    off += up(bytes);
+    return at;
+  };
+  const size_t pairs = s.pairs, blocks = static_cast<size_t>(s.block_cap);
+  w->head = reinterpret_cast<PlanHead*>(take(sizeof(PlanHead)));
+  w->tiles = reinterpret_cast<Tile*>(take(sizeof(Tile) * s.tile_cap));
+  w->pair_tile = reinterpret_cast<int*>(take(sizeof(int) * pairs));
+  w->valid = reinterpret_cast<uint16_t*>(take(8 * blocks));
+  w->broken = reinterpret_cast<uint16_t*>(take(8 * blocks));
+  w->part_m = reinterpret_cast<float*>(take(sizeof(float) * pairs * 4 * kRows));
+  w->part_den = reinterpret_cast<float*>(take(sizeof(float) * pairs * 4 * kRows));
+  w->part_o = reinterpret_cast<float*>(take(sizeof(float) * pairs * 2 * kRows * kD));
+  w->stage = reinterpret_cast<__nv_bfloat16*>(take(2 * blocks * kKeys * kD));
+  return off;
+}
+
+cudaError_t tc_forward(const PagedAttnProblem& p, void* ws, cudaStream_t st) {
+  TcCall c;
+  c.p = p;
+  c.s = tc_shape(p);
+  tc_carve(c.s, static_cast<char*>(ws), &c.w);
+  if (c.s.block_cap * kKeys > 0x7FFFFFFFll) return cudaErrorInvalidValue;
+  CUtensorMap map;
+  if (!make_tma_map_u8(&map, c.w.stage, kD * 2, static_cast<uint64_t>(c.s.block_cap) * kKeys, 128,
+                       kKeys, true, false))
+    return cudaErrorInvalidValue;
+  CUtensorMap qmap = map;  // not read for fp32 rows
+  if (p.bf16 && !make_tma_map_u8_3d(&qmap, p.q, kD * 2, p.H, p.total, p.q_stride * 2, 128, p.H,
+                                    kRows / p.H))
+    return cudaErrorInvalidValue;
+  const size_t smem = sizeof(int) * 2 * (static_cast<size_t>(p.pages.n_seqs) + 1);
+  const long long units = c.s.block_cap * (kKeys / kUnit);
+  const int most = sm_count() * 6;
+  cudaError_t e = launch_pdl(stage_kernel, dim3(1 + static_cast<unsigned>(units < most ? units : most)),
+                             dim3(kStageThreads), smem, st, c);
+  if (e != cudaSuccess) return e;
+  e = set_max_dynamic_smem(reinterpret_cast<const void*>(paged_attn_tc_kernel), kTcBytes);
+  if (e != cudaSuccess) return e;
+  e = launch_pdl(paged_attn_tc_kernel, dim3(2 * c.s.pairs), dim3(kTcThreads), kTcBytes, st, map, qmap,
+                 c);
+  if (e != cudaSuccess || c.s.pairs == 1) return e;
+  return launch_pdl(paged_attn_merge_kernel, dim3(kRows / kMergeWarps, c.s.pairs - 1),
+                    dim3(32 * kMergeWarps), 0, st, c);
+}
+
 }  // namespace
 
-size_t paged_attn_workspace_bytes(const PagedAttnProblem&) { return 0; }
+size_t paged_attn_workspace_bytes(const PagedAttnProblem& p) {
+  if (!tc_shape_ok(p) || p.total <= 0) return 0;
+  TcWs w;
+  return tc_carve(tc_shape(p), nullptr, &w);
+}
 
-cudaError_t paged_attn_forward(const PagedAttnProblem& p, void*, cudaStream_t st) {
+cudaError_t paged_attn_forward(const PagedAttnProblem& p, void* ws, cudaStream_t st) {
   if (p.total <= 0) return cudaSuccess;
+  if (tc_shape_ok(p)) return tc_forward(p, ws, st);
   if (p.pages.nope + p.pages.rope_dim > kMaxDim) return cudaErrorInvalidValue;
   paged_attn_simt_kernel<<<dim3(p.total, p.H), 32 * kSimtWarps, 0, st>>>(p);
   return cudaGetLastError();
