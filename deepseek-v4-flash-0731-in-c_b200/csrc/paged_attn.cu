@@ -637,6 +637,37 @@ __device__ __forceinline__ bool long_wait(uint64_t* bar, uint32_t parity, volati
   return true;
 }
 
+// MMA issue by one thread of a role that only this thread runs: no election
+// per instruction, and no vote or fence at waits that order nothing but
+// copies, so that the issue stays ahead of the tensor pipe.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                       bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+          smem_addr(bar))
+      : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{ .reg .pred e; elect.sync _|e, 0xffffffff; selp.u32 %0, 1, 0, e; }" : "=r"(p));
+  return p != 0;
+}
+
 // The two warps of 32 rows meet (a barrier in shared memory, because a named
 // one could not give up).
 struct PairSync {
@@ -646,9 +677,7 @@ struct PairSync {
   unsigned* err;
   __device__ __forceinline__ bool operator()() {
     mbar_arrive(bar);
-    const bool ok = long_wait(bar, done & 1, abort_flag, err);
-    ++done;
-    return __all_sync(0xffffffffu, ok);
+    return long_wait(bar, done++ & 1, abort_flag, err);
   }
 };
 
@@ -672,7 +701,7 @@ __device__ __forceinline__ bool softmax_block(uint32_t s_col, uint32_t mask, boo
   }
   const float mine = fmaxf(fmaxf(tm[0], tm[1]), fmaxf(tm[2], tm[3]));
   *max_mine = mine;
-  ok = meet();
+  ok = meet() && ok;
   const float tmax = fmaxf(mine, *max_other) * sc2;  // scale > 0
   // the running max moves only when a score exceeds it by the margin:
   // weights stay <= 2^8 and O is rarely rescaled
@@ -811,19 +840,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
           mask_next = valid[j + 1];
           broken_next = brk[j + 1];
         }
-        // bits 0 .. last - key0, and from there on the window's first
+        // a block that every row sees whole needs no mask
         const int hi_key = last - key0, lo_key = from - key0;
-        mask &= hi_key < 0 ? 0ull : hi_key >= 63 ? ~0ull : (2ull << hi_key) - 1;
-        if (lo_key > 0) mask &= lo_key > 63 ? 0ull : ~0ull << lo_key;
-        if (broken & mask) bad = true;
-        mask &= ~broken;
-        const bool plain = __all_sync(0xffffffffu, mask == ~0ull) && !two_terms;
-        const uint32_t mask32 = static_cast<uint32_t>(mask >> (32 * side));
-        const int sb = n & 1;
-        if (!__all_sync(0xffffffffu, long_wait(&bars->s_full[sb], (n >> 1) & 1, abort_flag, err))) {
-          ok = false;
-          break;
+        const bool whole = hi_key >= kKeys - 1 && lo_key <= 0 && mask == ~0ull && broken == 0;
+        const bool plain = __all_sync(0xffffffffu, whole) && !two_terms;
+        uint32_t mask32 = ~0u;
+        if (!plain) {
+          // bits 0 .. last - key0, and from the window's first on
+          mask &= hi_key < 0 ? 0ull : hi_key >= 63 ? ~0ull : (2ull << hi_key) - 1;
+          if (lo_key > 0) mask &= lo_key > 63 ? 0ull : ~0ull << lo_key;
+          if (broken & mask) bad = true;
+          mask &= ~broken;
+          mask32 = static_cast<uint32_t>(mask >> (32 * side));
         }
+        // A wait that gives up ends the loop at the block's vote; what is
+        // computed until then is not used.
+        const int sb = n & 1;
+        bool good = long_wait(&bars->s_full[sb], (n >> 1) & 1, abort_flag, err);
+        __syncwarp();
         tc_fence_after();
         const uint32_t s_col = tmem + lanes + kColS + sb * kKeys + side * 32;
         const int buf = sb * 2 * kRows;
@@ -831,13 +865,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
         float alpha;
         const bool rescale =
             plain ? softmax_block<true>(s_col, mask32, false, sc2, max_mine + buf, max_other + buf,
-                                        meet, ok, st, alpha, hi, lo)
+                                        meet, good, st, alpha, hi, lo)
                   : softmax_block<false>(s_col, mask32, two_terms, sc2, max_mine + buf,
-                                         max_other + buf, meet, ok, st, alpha, hi, lo);
-        if (!ok) break;
+                                         max_other + buf, meet, good, st, alpha, hi, lo);
         // P V of the block before has read P, and O holds all blocks before
-        if (n > 0 &&
-            !__all_sync(0xffffffffu, long_wait(&bars->pv_done, (n - 1) & 1, abort_flag, err))) {
+        if (n > 0) good = long_wait(&bars->pv_done, (n - 1) & 1, abort_flag, err) && good;
+        if (!__all_sync(0xffffffffu, good)) {
           ok = false;
           break;
         }
@@ -872,10 +905,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
       // before the last one is free)
       const int buf = (n & 1) * 2 * kRows;
       max_mine[buf] = st.den;
-      if (!(ok = meet())) break;
+      bool good = meet();
       float den = st.den + max_other[buf];
-      if (!(ok = meet())) break;  // read before the next segment writes it
-      if (!__all_sync(0xffffffffu, long_wait(&bars->pv_done, (n - 1) & 1, abort_flag, err))) {
+      good = meet() && good;  // read before the next segment writes it
+      good = long_wait(&bars->pv_done, (n - 1) & 1, abort_flag, err) && good;
+      if (!__all_sync(0xffffffffu, good)) {
         ok = false;
         break;
       }
@@ -1048,78 +1082,83 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
     __syncwarp();
   } else {
     // ------------------------------------------------------------- MMA issue
-    constexpr uint32_t idesc_qk = umma_idesc_bf16(kRows, kKeys, false);
-    constexpr uint32_t idesc_pv = umma_idesc_bf16(kRows, kHalf, true);
-    const uint64_t q_desc = umma_desc(base + kSmQ, 16, 1024);
-    const uint64_t p_desc = umma_desc(base + kSmP, 16, 1024);
-    auto waits = [&](uint64_t* bar, unsigned parity) {
-      const bool w = __all_sync(0xffffffffu, long_wait(bar, parity & 1, abort_flag, err));
-      tc_fence_after();
-      return w;
-    };
-    // Q K^T over 128 dims at column blocks cb, cb + 1 of a 256-dim half
-    auto qk = [&](uint32_t s_col, uint64_t k_desc, int q_half, int cb, bool first) {
-      if (q_half == 0) {
+    if (elect_one()) {
+      constexpr uint32_t idesc_qk = umma_idesc_bf16(kRows, kKeys, false);
+      constexpr uint32_t idesc_pv = umma_idesc_bf16(kRows, kHalf, true);
+      const uint64_t q_desc = umma_desc(base + kSmQ, 16, 1024);
+      const uint64_t p_desc = umma_desc(base + kSmP, 16, 1024);
+      const uint64_t own_desc = umma_desc(base + kSmOwn, 16, 1024);
+      const uint64_t other_desc = umma_desc(base + kSmOther, 16, 1024);
+      const uint64_t v_desc = umma_desc(base + kSmOwn, kBlk, 1024);
+      auto waits = [&](uint64_t* bar, unsigned parity) {
+        return long_wait(bar, parity & 1, abort_flag, err);
+      };
+      // Q K^T over 128 dims at column blocks cb, cb + 1 of a 256-dim half
+      auto qk = [&](uint32_t s_col, uint64_t k_desc, int q_half, int cb, bool first) {
+        if (q_half == 0) {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          umma_bf16_ts_e(s_col, tmem + kColQ + cb * 32 + kk * 8,
-                         k_desc + ((kk >> 2) * kBlk + (kk & 3) * 32) / 16, idesc_qk,
-                         (first && kk == 0) ? 0u : 1u);
-      } else {
+          for (int kk = 0; kk < 8; ++kk)
+            mma_ts(s_col, tmem + kColQ + cb * 32 + kk * 8,
+                   k_desc + ((kk >> 2) * kBlk + (kk & 3) * 32) / 16, idesc_qk,
+                   !(first && kk == 0));
+        } else {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          umma_bf16_e(s_col, q_desc + ((cb + (kk >> 2)) * kQBlk + (kk & 3) * 32) / 16,
-                      k_desc + ((kk >> 2) * kBlk + (kk & 3) * 32) / 16, idesc_qk,
-                      (first && kk == 0) ? 0u : 1u);
-      }
-    };
-    unsigned n = 0, no = 0, nw = 0, it = 0;
-    // O += P V of block number nb of this CTA
-    auto pv = [&](unsigned nb, bool first, bool two_terms) {
-      if (!waits(&bars->p_full, nb)) return false;
-      const unsigned s = nb % kOwnStages;
-      const uint64_t v = umma_desc(base + kSmOwn + s * 4 * kBlk, kBlk, 1024);
-#pragma unroll
-      for (int kk = 0; kk < kKeys / 16; ++kk)
-        umma_bf16_e(tmem, p_desc + kk * 2, v + kk * 128, idesc_pv, (first && kk == 0) ? 0u : 1u);
-      if (two_terms) {
+          for (int kk = 0; kk < 8; ++kk)
+            mma_ss(s_col, q_desc + ((cb + (kk >> 2)) * kQBlk + (kk & 3) * 32) / 16,
+                   k_desc + ((kk >> 2) * kBlk + (kk & 3) * 32) / 16, idesc_qk,
+                   !(first && kk == 0));
+        }
+      };
+      unsigned n = 0, it = 0;
+      unsigned so = 0, po = 0, sw = 0, pw = 0;  // slot and phase of the other / own ring
+      unsigned sv = 0;                          // the own slot that P V reads next
+      // O += P V of block number nb of this CTA
+      auto pv = [&](unsigned nb, bool first, bool two_terms) {
+        if (!waits(&bars->p_full, nb)) return false;
+        tc_fence_after();  // the softmax's reads of S and writes of O
+        const uint64_t v = v_desc + sv * (4 * kBlk / 16);
 #pragma unroll
         for (int kk = 0; kk < kKeys / 16; ++kk)
-          umma_bf16_e(tmem, p_desc + kPBytes / 16 + kk * 2, v + kk * 128, idesc_pv, 1u);
-      }
-      umma_commit_e(&bars->pv_done);
-      umma_commit_e(&bars->empty_own[s]);
-      return true;
-    };
-    bool ok = true;
-    while (ok && walk.next(seg)) {
-      if (!waits(&bars->q_full, it)) break;
-      ++it;
-      const bool two_terms = seg.t.blocks <= kTwoTermBlocks;
-      for (int j = seg.j0; j < seg.j1 && ok; ++j) {
-        const uint32_t s_col = tmem + kColS + (n & 1) * kKeys;
-        for (int q = 0; q < 2; ++q, ++no) {
-          const unsigned s = no % kOtherStages;
-          if (!waits(&bars->full_other[s], no / kOtherStages)) { ok = false; break; }
-          qk(s_col, umma_desc(base + kSmOther + s * 2 * kBlk, 16, 1024), 1 - half, 2 * q, q == 0);
-          umma_commit_e(&bars->empty_other[s]);
+          mma_ss(tmem, p_desc + kk * 2, v + kk * 128, idesc_pv, !(first && kk == 0));
+        if (two_terms) {
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+            mma_ss(tmem, p_desc + kPBytes / 16 + kk * 2, v + kk * 128, idesc_pv, true);
         }
-        if (!ok) break;
-        const unsigned s = nw % kOwnStages;
-        if (!waits(&bars->full_own[s], nw / kOwnStages)) { ok = false; break; }
-        const uint64_t k_desc = umma_desc(base + kSmOwn + s * 4 * kBlk, 16, 1024);
-        qk(s_col, k_desc, half, 0, false);
-        qk(s_col, k_desc + 2 * kBlk / 16, half, 2, false);
-        ++nw;
-        umma_commit_e(&bars->s_full[n & 1]);
-        if (j + 1 == seg.j1) umma_commit_e(&bars->q_free);
-        if (j > seg.j0 && !pv(n - 1, j - 1 == seg.j0, two_terms)) { ok = false; break; }
-        ++n;
+        mma_commit(&bars->pv_done);
+        mma_commit(&bars->empty_own[sv]);
+        if (++sv == kOwnStages) sv = 0;
+        return true;
+      };
+      bool ok = true;
+      while (ok && walk.next(seg)) {
+        if (!waits(&bars->q_full, it)) break;
+        tc_fence_after();  // the loaders' writes of Q
+        ++it;
+        const bool two_terms = seg.t.blocks <= kTwoTermBlocks;
+        for (int j = seg.j0; j < seg.j1; ++j, ++n) {
+          const uint32_t s_col = tmem + kColS + (n & 1) * kKeys;
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            if (!(ok = waits(&bars->full_other[so], po))) break;
+            qk(s_col, other_desc + so * (2 * kBlk / 16), 1 - half, 2 * q, q == 0);
+            mma_commit(&bars->empty_other[so]);
+            if (++so == kOtherStages) { so = 0; po ^= 1; }
+          }
+          if (!ok || !(ok = waits(&bars->full_own[sw], pw))) break;
+          const uint64_t k_desc = own_desc + sw * (4 * kBlk / 16);
+          qk(s_col, k_desc, half, 0, false);
+          qk(s_col, k_desc + 2 * kBlk / 16, half, 2, false);
+          if (++sw == kOwnStages) { sw = 0; pw ^= 1; }
+          mma_commit(&bars->s_full[n & 1]);
+          if (j + 1 == seg.j1) mma_commit(&bars->q_free);
+          if (j > seg.j0 && !(ok = pv(n - 1, j - 1 == seg.j0, two_terms))) break;
+        }
+        ok = ok && pv(n - 1, seg.j1 - seg.j0 == 1, two_terms);
       }
-      if (ok && !pv(n - 1, seg.j1 - seg.j0 == 1, two_terms)) ok = false;
+      mma_commit(&bars->fin);
+      mbar_wait(&bars->fin, 0, err);
     }
-    umma_commit_e(&bars->fin);
-    mbar_wait(&bars->fin, 0, err);
     __syncwarp();
   }
   tc_fence_before();
