@@ -668,6 +668,15 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
 // The two warps of 32 rows meet (a barrier in shared memory, because a named
 // one could not give up).
 struct PairSync {
@@ -735,9 +744,9 @@ __device__ __forceinline__ bool softmax_block(uint32_t s_col, uint32_t mask, boo
 // One share of (tile, block) pairs and one half of the output dims. Roles:
 //   warps 0-7  softmax and epilogue: row = TMEM lane, two threads a row, one
 //              for each half of a block's keys (and of the CTA's output dims)
-//   warps 8-11 Q of the next segment, once this one's last Q K^T is done: dims
-//              0-255 to TMEM (the first half of them waits in registers)
-//   warp 12    key blocks and Q's dims 256-511 by TMA (one lane)
+//   warps 8-11 dims 0-255 of the next segment's Q to TMEM, once this one's last
+//              Q K^T is done
+//   warp 12    key blocks and Q by TMA (one lane)
 //   warp 13    TMEM allocation and MMA issue
 // Per block: S = Q K^T (32 MMAs of 128 x 64 x 16, the other half's dims first
 // so that their slots are free early), P = 2^(S - m) in BF16 to shared
@@ -811,6 +820,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
     const uint32_t lanes = static_cast<uint32_t>(w4 * 32) << 16;
     const uint32_t o_cols = tmem + lanes + side * (kHalf / 2);
     const uint32_t prow = base + kSmP + (row >> 3) * 1024 + (row & 7) * 128;
+    const uint32_t room = base + kSmP + warp * 4096;  // free once P V is done
     float* maxima = reinterpret_cast<float*>(smem + kSmMax);
     float* max_mine = maxima + side * kRows + row;
     const float* max_other = maxima + (1 - side) * kRows + row;
@@ -919,39 +929,70 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
       if (done) {
         const Norm norm = finish(st.m, den, p.sink, h < p.H && mine ? h : 0);
         const long long at = static_cast<long long>(t.row0 + tok);
+        const long long o_at = mine ? at * p.out_stride + static_cast<long long>(h) * kD : -1ll;
         if (mine && half == 0 && side == 0 && p.lse) p.lse[at * p.H + h] = norm.lse;
         const int r0 = kD - p.rope_out;
+        const int d_side = half * kHalf + side * (kHalf / 2);
+        const bool rope = p.rope_cos && d_side + kHalf / 2 > r0;
 #pragma unroll 1
         for (int cb = 0; cb < kHalf / 2; cb += 32) {
           uint32_t o[32];
           tmem_ld32(o_cols + cb, o);
-          if (mine) {
-            float v[32];
+          float v[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]) * norm.scale;
-            const int d0 = half * kHalf + side * (kHalf / 2) + cb;
-            if (p.rope_cos && d0 + 32 > r0) rope_dims(p, at, d0, r0, v);
-            const long long to = at * p.out_stride + static_cast<long long>(h) * kD + d0;
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]) * norm.scale;
+          const int d0 = d_side + cb;
+          if (rope && mine && d0 + 32 > r0) rope_dims(p, at, d0, r0, v);
+          if (p.bf16) {
+            // rows of 64 dims in this warp's room, then whole lines to memory
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) store_o8(p, to + i, v + i);
+            for (int k = 0; k < 4; ++k)
+              st_shared_v4(room + lane * 128 + ((((cb & 32) / 8 + k) ^ (lane & 7)) << 4),
+                           make_uint4(pack_bf16x2(v[8 * k], v[8 * k + 1]),
+                                      pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
+                                      pack_bf16x2(v[8 * k + 4], v[8 * k + 5]),
+                                      pack_bf16x2(v[8 * k + 6], v[8 * k + 7])));
+            if (cb & 32) {
+              __syncwarp();
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + (lane >> 3), ch = lane & 7;
+                const long long to = __shfl_sync(0xffffffffu, o_at, r);
+                const uint4 w = ld_shared_v4(room + r * 128 + ((ch ^ (r & 7)) << 4));
+                if (to >= 0)
+                  *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + to + d_side +
+                                            (cb & 64) + 8 * ch) = w;
+              }
+              __syncwarp();
+            }
+          } else if (mine) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) store_o8(p, o_at + d0 + i, v + i);
           }
         }
       } else {
         // a part: slot 0 where the tile began in an earlier share, else 1
         const int slot = t.start < share0 ? 0 : 1;
         const long long at = pair * 2 + slot;
+        float* part = c.w.part_o + (at * kRows + w4 * 32) * kD + half * kHalf + side * (kHalf / 2);
+        const unsigned rows = __ballot_sync(0xffffffffu, mine);
 #pragma unroll 1
         for (int cb = 0; cb < kHalf / 2; cb += 32) {
           uint32_t o[32];
           tmem_ld32(o_cols + cb, o);
-          if (mine) {
-            float4* dst = reinterpret_cast<float4*>(c.w.part_o + (at * kRows + row) * kD +
-                                                    half * kHalf + side * (kHalf / 2) + cb);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              dst[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                   __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+          for (int k = 0; k < 8; ++k)
+            st_shared_v4(room + lane * 128 + ((k ^ (lane & 7)) << 4),
+                         make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]));
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3), ch = lane & 7;
+            const uint4 w = ld_shared_v4(room + r * 128 + ((ch ^ (r & 7)) << 4));
+            if ((rows >> r) & 1u)
+              *reinterpret_cast<uint4*>(part + r * kD + cb + 4 * ch) = w;
           }
+          __syncwarp();
         }
         if (mine && side == 0) {
           c.w.part_m[(at * 2 + half) * kRows + row] = st.m;
@@ -964,50 +1005,66 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
     // ------------------------------------------------------------- Q loaders
     const int w4 = warp & 3, row = w4 * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(w4 * 32) << 16;
-    const int tok = row / p.H, h = row - tok * p.H;
-    const int size = p.bf16 ? 2 : 4;
-    unsigned it = 0;
+    unsigned it = 0, slot = 0, phase = 0;  // of the own ring
+    auto to_tmem = [&](const uint4 (&a)[16], int k) {  // dims 128 k ..
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t r[32];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          r[4 * i] = a[8 * q + i].x;
+          r[4 * i + 1] = a[8 * q + i].y;
+          r[4 * i + 2] = a[8 * q + i].z;
+          r[4 * i + 3] = a[8 * q + i].w;
+        }
+        tmem_st32(tmem + lanes + kColQ + 64 * k + 32 * q, r);
+      }
+    };
     while (walk.next(seg)) {
       const Tile& t = seg.t;
-      const long long at = tok < t.tokens ? static_cast<long long>(t.row0 + tok) * p.q_stride +
-                                                static_cast<long long>(h) * kD
-                                          : -1ll;
-      uint4 a[16] = {};
-      if (at >= 0) {
-        bulk_prefetch_l2(static_cast<const uint8_t*>(p.q) + (at + kHalf / 2) * size,
-                         (kHalf / 2 + kHalf) * size);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) a[i] = load_q8(p, at + 8 * i);
-      }
-      if (it > 0 &&
-          !__all_sync(0xffffffffu, long_wait(&bars->q_free, (it - 1) & 1, abort_flag, err)))
-        break;
+      bool good = true;
+      uint4 a[16];
+      // (also before the own ring is looked at: only now is the slot's phase
+      // the one before Q's)
+      if (it > 0) good = long_wait(&bars->q_free, (it - 1) & 1, abort_flag, err);
+      __syncwarp();
       tc_fence_after();
+      if (p.bf16) {
+        // dims 0-255 come through two slots of the own ring, ahead of the
+        // segment's first block
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < 2; ++k) {
+          good = long_wait(&bars->full_own[slot], phase, abort_flag, err) && good;
+          const uint8_t* src = smem + kSmOwn + slot * 4 * kBlk + row * 128;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          uint32_t r[32];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            r[4 * i] = a[8 * q + i].x;
-            r[4 * i + 1] = a[8 * q + i].y;
-            r[4 * i + 2] = a[8 * q + i].z;
-            r[4 * i + 3] = a[8 * q + i].w;
-          }
-          tmem_st32(tmem + lanes + kColQ + 64 * k + 32 * q, r);
+          for (int i = 0; i < 16; ++i)
+            a[i] = *reinterpret_cast<const uint4*>(src + (i >> 3) * kQBlk +
+                                                   (((i & 7) ^ (row & 7)) << 4));
+          to_tmem(a, k);
+          if (++slot == kOwnStages) { slot = 0; phase ^= 1; }
         }
-        if (k == 0 && at >= 0) {
+        slot += static_cast<unsigned>(seg.j1 - seg.j0);
+        phase ^= (slot / kOwnStages) & 1;
+        slot %= kOwnStages;
+      } else {
+        // fp32 rows are converted on their way
+        const int tok = row / p.H, h = row - tok * p.H;
+        const long long at = tok < t.tokens ? static_cast<long long>(t.row0 + tok) * p.q_stride +
+                                                  static_cast<long long>(h) * kD
+                                            : -1ll;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) a[i] = load_q8(p, at + 128 + 8 * i);
+        for (int k = 0; k < 2; ++k) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            a[i] = at >= 0 ? load_q8(p, at + 128 * k + 8 * i) : make_uint4(0, 0, 0, 0);
+          to_tmem(a, k);
         }
-      }
-      if (!p.bf16) {  // fp32 rows: converted on their way to shared memory
+#pragma unroll 1
         for (int i0 = 0; i0 < 32; i0 += 16) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const long long b = __shfl_sync(0xffffffffu, at, i0 + i);
-            if (b >= 0) a[i] = load_q8(p, b + kHalf + 8 * lane);
+            a[i] = b >= 0 ? load_q8(p, b + kHalf + 8 * lane) : make_uint4(0, 0, 0, 0);
           }
 #pragma unroll
           for (int i = 0; i < 16; ++i)
@@ -1019,6 +1076,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
       tc_fence_before();
       mbar_arrive(&bars->q_full);
       ++it;
+      if (!__all_sync(0xffffffffu, good)) break;
     }
   } else if (warp == kWarpTma) {
     // ------------------------------------------------------------ key blocks
@@ -1039,8 +1097,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
           tma_load_3d(smem + kSmQ + b * kQBlk, &qmap, 512 + b * 128, 0, t.row0, &bars->q_full);
         return true;
       };
+      auto load_own = [&](const CUtensorMap* m, int x, int y, bool q) {
+        const unsigned s = nw % kOwnStages;
+        if (!long_wait(&bars->empty_own[s], ((nw / kOwnStages) & 1) ^ 1, abort_flag, err))
+          return false;
+        mbar_arrive_expect_tx(&bars->full_own[s], q ? 2 * 128 * q_rows : 4 * kBlk);
+        if (q) {
+          for (int b = 0; b < 2; ++b)
+            tma_load_3d(smem + kSmOwn + s * 4 * kBlk + b * kQBlk, m, x + b * 128, 0, y,
+                        &bars->full_own[s]);
+        } else {
+          for (int b = 0; b < 4; ++b)
+            tma_load_2d(smem + kSmOwn + (s * 4 + b) * kBlk, m, x + b * 128, y, &bars->full_own[s]);
+        }
+        ++nw;
+        return true;
+      };
       while (ok && walk.next(seg)) {
-        // the first key blocks are on their way before Q's room is free
+        // Q and the first key blocks are on their way before Q's room is free
+        if (p.bf16) {
+          for (int k = 0; k < 2 && ok; ++k) ok = load_own(&qmap, 256 * k, seg.t.row0, true);
+        }
         bool q_due = true;
         for (int j = seg.j0; j < seg.j1 && ok; ++j) {
           const int y = (seg.t.block0 + j) * kKeys;
@@ -1060,16 +1137,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
             q_due = false;
             if (!load_q(seg.t)) { ok = false; break; }
           }
-          const unsigned s = nw % kOwnStages;
-          if (!long_wait(&bars->empty_own[s], ((nw / kOwnStages) & 1) ^ 1, abort_flag, err)) {
-            ok = false;
-            break;
-          }
-          mbar_arrive_expect_tx(&bars->full_own[s], 4 * kBlk);
-          for (int b = 0; b < 4; ++b)
-            tma_load_2d(smem + kSmOwn + (s * 4 + b) * kBlk, &map, half * 512 + b * 128, y,
-                        &bars->full_own[s]);
-          ++nw;
+          ok = load_own(&map, half * 512, y, false);
         }
       }
       // no copy may be in flight when the CTA ends: the last one of each slot
@@ -1135,6 +1203,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
         if (!waits(&bars->q_full, it)) break;
         tc_fence_after();  // the loaders' writes of Q
         ++it;
+        if (p.bf16) {  // its two slots of the own ring have been read
+          for (int k = 0; k < 2; ++k) {
+            mbar_arrive(&bars->empty_own[sw]);
+            if (++sw == kOwnStages) { sw = 0; pw ^= 1; }
+            if (++sv == kOwnStages) sv = 0;
+          }
+        }
         const bool two_terms = seg.t.blocks <= kTwoTermBlocks;
         for (int j = seg.j0; j < seg.j1; ++j, ++n) {
           const uint32_t s_col = tmem + kColS + (n & 1) * kKeys;
