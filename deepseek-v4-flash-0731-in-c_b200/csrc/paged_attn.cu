@@ -1114,6 +1114,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
         return true;
       };
       while (ok && walk.next(seg)) {
+        // the next segment's Q to L2, so that it is near when its room is free
+        if (p.bf16 && walk.F < walk.end) {
+          const int row0 = walk.tiles[walk.t].row0;
+          for (int b = 0; b < 8; ++b) tma_prefetch_3d(&qmap, b * 128, 0, row0);
+        }
         // Q and the first key blocks are on their way before Q's room is free
         if (p.bf16) {
           for (int k = 0; k < 2 && ok; ++k) ok = load_own(&qmap, 256 * k, seg.t.row0, true);
@@ -1158,8 +1163,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
       const uint64_t own_desc = umma_desc(base + kSmOwn, 16, 1024);
       const uint64_t other_desc = umma_desc(base + kSmOther, 16, 1024);
       const uint64_t v_desc = umma_desc(base + kSmOwn, kBlk, 1024);
-      auto waits = [&](uint64_t* bar, unsigned parity) {
-        return long_wait(bar, parity & 1, abort_flag, err);
+      // A barrier is looked at before the MMAs that come first are issued, so
+      // that its answer is there when they are.
+      auto peek = [&](uint64_t* bar, unsigned parity) { return mbar_try_wait(bar, parity & 1); };
+      auto waits = [&](bool ready, uint64_t* bar, unsigned parity) {
+        return ready || long_wait(bar, parity & 1, abort_flag, err);
       };
       // Q K^T over 128 dims at column blocks cb, cb + 1 of a 256-dim half
       auto qk = [&](uint32_t s_col, uint64_t k_desc, int q_half, int cb, bool first) {
@@ -1181,8 +1189,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
       unsigned so = 0, po = 0, sw = 0, pw = 0;  // slot and phase of the other / own ring
       unsigned sv = 0;                          // the own slot that P V reads next
       // O += P V of block number nb of this CTA
-      auto pv = [&](unsigned nb, bool first, bool two_terms) {
-        if (!waits(&bars->p_full, nb)) return false;
+      auto pv = [&](bool ready, unsigned nb, bool first, bool two_terms) {
+        if (!waits(ready, &bars->p_full, nb)) return false;
         tc_fence_after();  // the softmax's reads of S and writes of O
         const uint64_t v = v_desc + sv * (4 * kBlk / 16);
 #pragma unroll
@@ -1200,7 +1208,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
       };
       bool ok = true;
       while (ok && walk.next(seg)) {
-        if (!waits(&bars->q_full, it)) break;
+        if (!waits(false, &bars->q_full, it)) break;
         tc_fence_after();  // the loaders' writes of Q
         ++it;
         if (p.bf16) {  // its two slots of the own ring have been read
@@ -1211,25 +1219,32 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
           }
         }
         const bool two_terms = seg.t.blocks <= kTwoTermBlocks;
+        bool ready = false;
         for (int j = seg.j0; j < seg.j1; ++j, ++n) {
           const uint32_t s_col = tmem + kColS + (n & 1) * kKeys;
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            if (!(ok = waits(&bars->full_other[so], po))) break;
-            qk(s_col, other_desc + so * (2 * kBlk / 16), 1 - half, 2 * q, q == 0);
-            mma_commit(&bars->empty_other[so]);
+            if (!(ok = waits(ready, &bars->full_other[so], po))) break;
+            const unsigned s = so;
             if (++so == kOtherStages) { so = 0; po ^= 1; }
+            ready = q == 0 ? peek(&bars->full_other[so], po) : peek(&bars->full_own[sw], pw);
+            qk(s_col, other_desc + s * (2 * kBlk / 16), 1 - half, 2 * q, q == 0);
+            mma_commit(&bars->empty_other[s]);
           }
-          if (!ok || !(ok = waits(&bars->full_own[sw], pw))) break;
+          if (!ok || !(ok = waits(ready, &bars->full_own[sw], pw))) break;
           const uint64_t k_desc = own_desc + sw * (4 * kBlk / 16);
+          const bool pv_due = j > seg.j0;
+          ready = pv_due && peek(&bars->p_full, n - 1);
           qk(s_col, k_desc, half, 0, false);
           qk(s_col, k_desc + 2 * kBlk / 16, half, 2, false);
           if (++sw == kOwnStages) { sw = 0; pw ^= 1; }
           mma_commit(&bars->s_full[n & 1]);
           if (j + 1 == seg.j1) mma_commit(&bars->q_free);
-          if (j > seg.j0 && !(ok = pv(n - 1, j - 1 == seg.j0, two_terms))) break;
+          const bool p_ready = ready;
+          ready = peek(&bars->full_other[so], po);
+          if (pv_due && !(ok = pv(p_ready, n - 1, j - 1 == seg.j0, two_terms))) break;
         }
-        ok = ok && pv(n - 1, seg.j1 - seg.j0 == 1, two_terms);
+        ok = ok && pv(false, n - 1, seg.j1 - seg.j0 == 1, two_terms);
       }
       mma_commit(&bars->fin);
       mbar_wait(&bars->fin, 0, err);
