@@ -8,91 +8,439 @@
 // A row that is all -inf gives -inf log probabilities and entropy 0; a NaN
 // or +inf in a row makes its log probabilities and entropy NaN. NaN never
 // competes for the top alternatives: a place left over holds id -1 and NaN.
+//
+// One pass over the row: every thread keeps a running maximum and the two
+// sums relative to it. A candidate for the top is one 64-bit key, the value
+// in an order-preserving form above the inverted index, so that the larger
+// key is the better one, ties included. The block keeps the k best so far;
+// what comes later has a higher index and therefore has to exceed the k-th
+// strictly, which after the first step few values do (ties of any number
+// never do). Rows are cut over a cluster where there are too few of them to
+// fill the GPU; the parts meet in the first CTA's shared memory.
 #include "logprob.cuh"
 
 #include <climits>
 #include <cmath>
 #include <cuda_bf16.h>
 
+#include "launch.cuh"
+#include "umma.cuh"
+
 namespace dsv4 {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kStep = 16;            // values a thread reads per step
+constexpr int kRound = 4 * kThreads; // candidates that can join between two looks at their number
+constexpr int kCap = 2 * kRound;     // candidates held
+constexpr int kThin = 512;           // more than this many are thinned out to the best 32
+constexpr int kTop = kMaxTopAlternatives;
+constexpr int kMaxCluster = 8;
+constexpr float kLn2 = 0.69314718055994531f;
+using Key = unsigned long long;      // 0: nothing
 
-__device__ __forceinline__ float load(const LogprobProblem& p, int row, int i) {
-  const long long at = row * p.stride + i;
-  return p.bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.logits)[at])
-                : static_cast<const float*>(p.logits)[at];
+__device__ __forceinline__ Key make_key(float x, int i) {
+  uint32_t u = __float_as_uint(x + 0.0f);  // -0 -> +0
+  u = (u & 0x80000000u) ? ~u : u | 0x80000000u;
+  return (static_cast<Key>(u) << 32) | (0xFFFFFFFFu - static_cast<uint32_t>(i));
+}
+__device__ __forceinline__ float key_value(Key k) {
+  const uint32_t u = static_cast<uint32_t>(k >> 32);
+  return __uint_as_float((u & 0x80000000u) ? u & 0x7FFFFFFFu : ~u);
+}
+__device__ __forceinline__ int key_index(Key k) {
+  return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(k));
 }
 
-template <class T, class F>
-__device__ T block_fold(T v, F f) {
-  __shared__ T part[kThreads / 32];
+// One key per lane, descending over the lanes.
+__device__ __forceinline__ Key swap_step(Key k, int j, bool keep_max) {
+  const Key o = __shfl_xor_sync(0xffffffffu, k, j);
+  return keep_max ? (o > k ? o : k) : (o < k ? o : k);
+}
+__device__ __forceinline__ Key merge_sorted(Key k) {  // a bitonic sequence to descending
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+  for (int j = 16; j > 0; j >>= 1) k = swap_step(k, j, (lane & j) == 0);
+  return k;
+}
+__device__ __forceinline__ Key sort_lanes(Key k) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int n = 2; n <= 32; n <<= 1)
+#pragma unroll
+    for (int j = n >> 1; j > 0; j >>= 1) k = swap_step(k, j, ((lane & j) == 0) == ((lane & n) == 0));
+  return k;
+}
+// The 32 best of two descending sequences.
+__device__ __forceinline__ Key best_of(Key a, Key b) {
+  const Key r = __shfl_xor_sync(0xffffffffu, b, 31);  // reversed
+  return merge_sorted(a > r ? a : r);
+}
+
+struct Shared {
+  Key cand[kCap];
+  Key list[kWarps][kTop];
+  Key part[kTop];              // this CTA's best, for the cluster
+  float m[kWarps], z[kWarps], s[kWarps];
+  int above[kWarps];
+  float cta_m, cta_z, cta_s;   // this CTA's sums, for the cluster
+  int cta_above;
+  int n;                       // candidates held
+  Key limit;                   // the k-th best so far, 0: fewer than k
+};
+
+// The best 32 of the n candidates, descending, to cand[0 .. 31]; the k-th is
+// the new limit. Whole block.
+__device__ void compact(Shared& sh, int k) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  const int n = sh.n;
+  Key best = 0;
+  for (int base = warp * 32; base < n; base += kThreads) {
+    const int i = base + lane;
+    best = best_of(best, sort_lanes(i < n ? sh.cand[i] : 0));
+  }
+  // pairs of warps, then pairs of pairs
+  const int used = min(kWarps, (n + 31) / 32);
+  for (int s = 1; s < used; s <<= 1) {
+    if (warp & s) sh.list[warp][lane] = best;
+    __syncthreads();
+    if ((warp & (2 * s - 1)) == 0 && warp + s < used) best = best_of(best, sh.list[warp + s][lane]);
+  }
+  if (warp == 0) {
+    sh.cand[lane] = best;
+    const Key kth = __shfl_sync(0xffffffffu, best, k - 1);
+    if (lane == 0) {
+      sh.limit = kth;
+      sh.n = min(n, kTop);
+    }
+  }
   __syncthreads();
-  v = part[0];
-  for (int w = 1; w < kThreads / 32; ++w) v = f(v, part[w]);
+}
+
+// Running sums of a thread, in natural units relative to m.
+struct Sums {
+  float m, z, s;  // max, sum e^(x - m), sum e^(x - m) log2 e (x - m)
+  int above;
+};
+
+__device__ __forceinline__ void raise_max(Sums& t, float bm) {
+  if (bm > t.m) {  // m = -inf: nothing but zeros so far
+    const float d = fmaxf((t.m - bm) * kLog2e, -1e4f);  // (finite: it meets a zero)
+    const float f = t.m == -INFINITY ? 0.f : ex2_approx(d);
+    t.s = t.m == -INFINITY ? t.s : f * fmaf(d, t.z, t.s);
+    t.z = t.m == -INFINITY ? t.z : t.z * f;
+    t.m = bm;
+  }
+}
+
+__device__ __forceinline__ void add_value(Sums& t, float ref, float x) {
+  // x - ref first: exact where it matters, whatever the size of the logits
+  const float d = (x - ref) * kLog2e, e = ex2_approx(d);
+  t.z += e;
+  t.s = fmaf(e, fmaxf(d, -256.f), t.s);  // e = 0 below 2^-126: a masked value adds 0
+}
+
+// 16 bytes that are read once.
+__device__ __forceinline__ uint4 ldg_stream(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
   return v;
 }
 
-__global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobProblem p) {
-  const int row = blockIdx.x;
+template <bool kBf16>
+struct Vec {
+  static constexpr int kN = kBf16 ? 8 : 4;  // values of 16 bytes
+  static __device__ __forceinline__ float get(const uint4& v, int i) {
+    const uint32_t w = kBf16 ? (i < 2 ? v.x : i < 4 ? v.y : i < 6 ? v.z : v.w)
+                             : (i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w);
+    if (!kBf16) return __uint_as_float(w);
+    return __uint_as_float((i & 1) ? w & 0xFFFF0000u : w << 16);
+  }
+  // 16 bytes that hold -inf everywhere
+  static __device__ __forceinline__ uint4 none() {
+    const uint32_t w = kBf16 ? 0xFF80FF80u : 0xFF800000u;
+    return make_uint4(w, w, w, w);
+  }
+};
+
+template <bool kBf16>
+__global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProblem p, int parts) {
+  using V = Vec<kBf16>;
+  constexpr int kN = V::kN, kVecs = kStep / kN;
+  extern __shared__ __align__(16) uint8_t smem[];
+  Shared& sh = *reinterpret_cast<Shared*>(smem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int row = blockIdx.x / parts, part = blockIdx.x % parts;
+  constexpr int kSize = kBf16 ? 2 : 4;
+  const uint8_t* x_row = static_cast<const uint8_t*>(p.logits) + row * p.stride * kSize;
+  auto value_at = [&](int i) {
+    return kBf16 ? bf16_widen(reinterpret_cast<const uint16_t*>(x_row)[i])
+                 : reinterpret_cast<const float*>(x_row)[i];
+  };
   const int t = p.tokens[row];
   const bool asked = t >= 0 && t < p.vocab;
-  const float xt = asked ? load(p, row, t) : 0.f;
-  float m = -INFINITY;
-  int above = 0, nan = 0;
-  for (int i = threadIdx.x; i < p.vocab; i += kThreads) {
-    const float x = load(p, row, i);
-    m = fmaxf(m, x);
-    above += x > xt || (x == xt && i < t);
-    nan |= x != x;
+  const float xt = asked ? value_at(t) : NAN;  // NaN: nothing is above it
+  // values before the first 16-byte boundary, whole vectors, values behind the last
+  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(x_row) & 15);
+  const int head = min(p.vocab, off ? (16 - off) / kSize : 0);
+  const int vecs = (p.vocab - head) / kN;
+  const int tail0 = head + vecs * kN;
+  const int v0 = static_cast<int>(static_cast<long long>(vecs) * part / parts);
+  const int v1 = static_cast<int>(static_cast<long long>(vecs) * (part + 1) / parts);
+  const uint4* src = reinterpret_cast<const uint4*>(x_row + head * kSize);
+
+  if (tid == 0) {
+    sh.n = 0;
+    sh.limit = 0;
   }
-  m = block_fold(m, [](float a, float b) { return fmaxf(a, b); });
-  above = block_fold(above, [](int a, int b) { return a + b; });
-  nan = block_fold(nan, [](int a, int b) { return a | b; });
-  const float ref = m == -INFINITY ? 0.f : m;
-  float z = 0.f, xz = 0.f;
-  for (int i = threadIdx.x; i < p.vocab; i += kThreads) {
-    const float d = load(p, row, i) - ref, e = expf(d);
-    z += e;
-    if (e > 0.f) xz = fmaf(e, d, xz);
+  Sums sum = {-INFINITY, 0.f, 0.f, 0};
+  uint4 buf[kVecs];
+  auto load = [&](int base) {
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      const int v = base + u * kThreads + tid;
+      buf[u] = v < v1 ? ldg_stream(src + v) : V::none();
+    }
+  };
+  load(v0);
+  __syncthreads();
+  bool first = true;
+  for (int base = v0; base < v1; base += kVecs * kThreads) {
+    uint4 cur[kVecs];
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) cur[u] = buf[u];
+    if (base + kVecs * kThreads < v1) load(base + kVecs * kThreads);
+    float bm4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u)
+#pragma unroll
+      for (int i = 0; i < kN; ++i) bm4[i & 3] = fmaxf(bm4[i & 3], V::get(cur[u], i));
+    const float bm = fmaxf(fmaxf(bm4[0], bm4[1]), fmaxf(bm4[2], bm4[3]));
+    raise_max(sum, bm);
+    const float ref = sum.m == -INFINITY ? 0.f : sum.m;
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      const int v = base + u * kThreads + tid;
+      const int i0 = head + v * kN;
+#pragma unroll
+      for (int i = 0; i < kN; ++i) add_value(sum, ref, V::get(cur[u], i));
+      // equal values count where they come before the token
+      if (v < v1 && i0 + kN <= t) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) sum.above += V::get(cur[u], i) >= xt;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) sum.above += V::get(cur[u], i) > xt;
+        if (i0 < t && v < v1) {
+#pragma unroll
+          for (int i = 0; i < kN; ++i) sum.above += V::get(cur[u], i) == xt && i0 + i < t;
+        }
+      }
+    }
+    if (p.top > 0) {
+      if (first) {
+        // Every warp has kEach threads whose best value reaches its kEach-th
+        // best one, so kWarps * kEach >= k values reach the smallest of these.
+        constexpr int kEach = kTop / kWarps;
+        Key best = 0;
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u) {
+          const int v = base + u * kThreads + tid;
+#pragma unroll
+          for (int i = 0; i < kN; ++i) {
+            const float x = V::get(cur[u], i);
+            if (v < v1 && x == bm) {  // the first of them
+              const Key k = make_key(x, head + v * kN + i);
+              best = k > best ? k : best;
+            }
+          }
+        }
+        Key kth = best;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+          Key top = kth;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            const Key other = __shfl_xor_sync(0xffffffffu, top, o);
+            top = other > top ? other : top;
+          }
+          if (e + 1 < kEach) {
+            if (kth == top) kth = 0;
+          } else {
+            kth = top;
+          }
+        }
+        if (lane == 0) sh.list[warp][0] = kth;
+        __syncthreads();
+        kth = sh.list[lane % kWarps][0];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          const Key other = __shfl_xor_sync(0xffffffffu, kth, o);
+          kth = other < kth ? other : kth;
+        }
+        if (tid == 0 && kth) sh.limit = kth - 1;  // the one at the limit comes in
+        __syncthreads();
+      }
+      const Key limit = sh.limit;
+      const float lv = key_value(limit);
+      const bool look = limit == 0 || (first ? bm >= lv : bm > lv);
+      auto join = [&](int u, int i, Key above, float above_value) {
+        const float x = V::get(cur[u], i);
+        // (a key below the limit's with an equal value, or no limit yet)
+        if (!(x > above_value) && !(first && x == above_value) && above != 0) return;
+        const int v = base + u * kThreads + tid;
+        const Key k = make_key(x, head + v * kN + i);
+        if (v < v1 && x == x && k > above) sh.cand[atomicAdd(&sh.n, 1)] = k;
+      };
+      const int held = sh.n;  // (changes only behind the next barrier)
+      const int looking = __syncthreads_count(look);
+      if (looking > 0 && held + looking * kStep <= kCap - 64) {
+        if (look) {
+#pragma unroll
+          for (int u = 0; u < kVecs; ++u)
+#pragma unroll
+            for (int i = 0; i < kN; ++i) join(u, i, limit, lv);
+        }
+        __syncthreads();
+        const int n = sh.n;
+        if (n > (first ? 2 * kTop : kThin)) compact(sh, p.top);
+      } else if (looking > 0) {
+        // more than fit (values in ascending order, say): four a thread at a
+        // time, thinned out in between
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u)
+#pragma unroll
+          for (int i = 0; i < kN; ++i) {
+            if (look) join(u, i, sh.limit, key_value(sh.limit));
+            if (i % 4 == 3) {
+              __syncthreads();
+              const int n = sh.n;
+              __syncthreads();
+              if (n > kCap - 64 - kRound) compact(sh, p.top);
+            }
+          }
+        compact(sh, p.top);
+      }
+      first = false;
+    }
   }
-  auto add = [](float a, float b) { return a + b; };
-  z = block_fold(z, add);
-  xz = block_fold(xz, add);
-  const bool undefined = nan || m == INFINITY;
-  const float lz = m == -INFINITY ? 0.f : logf(z);
-  if (threadIdx.x == 0) {
+  // the values outside whole vectors: at most one a thread
+  {
+    const int n_head = part == 0 ? head : 0, n_tail = part == parts - 1 ? p.vocab - tail0 : 0;
+    const int i = tid < n_head ? tid : tid - n_head < n_tail ? tail0 + tid - n_head : -1;
+    if (n_head + n_tail > 0) {
+      const float x = i >= 0 ? value_at(i) : -INFINITY;
+      if (i >= 0) {
+        raise_max(sum, x);
+        add_value(sum, sum.m == -INFINITY ? 0.f : sum.m, x);
+        sum.above += x > xt || (x == xt && i < t);
+        if (p.top > 0 && x == x) sh.cand[atomicAdd(&sh.n, 1)] = make_key(x, i);
+      }
+    }
+  }
+  if (p.top > 0) compact(sh, p.top);  // sorted, whatever their number
+
+  // the CTA's sums
+  auto add_sums = [](Sums& a, float m, float z, float s) {  // b's sums to a's
+    const float mx = fmaxf(a.m, m);
+    if (mx == -INFINITY) {  // only zeros, or NaN on either side
+      a.z += z;
+      a.s += s;
+      return;
+    }
+    Sums b = {m, z, s, 0};
+    raise_max(a, mx);
+    raise_max(b, mx);
+    a.z += b.z;
+    a.s += b.s;
+  };
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m = __shfl_xor_sync(0xffffffffu, sum.m, o);
+    const float z = __shfl_xor_sync(0xffffffffu, sum.z, o);
+    const float s = __shfl_xor_sync(0xffffffffu, sum.s, o);
+    add_sums(sum, m, z, s);
+    sum.above += __shfl_xor_sync(0xffffffffu, sum.above, o);
+  }
+  if (lane == 0) {
+    sh.m[warp] = sum.m;
+    sh.z[warp] = sum.z;
+    sh.s[warp] = sum.s;
+    sh.above[warp] = sum.above;
+  }
+  __syncthreads();
+  Key best = 0;
+  if (warp == 0) {
+    sum = {sh.m[lane % kWarps], lane < kWarps ? sh.z[lane] : 0.f, lane < kWarps ? sh.s[lane] : 0.f,
+           lane < kWarps ? sh.above[lane] : 0};
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float m = __shfl_xor_sync(0xffffffffu, sum.m, o);
+      const float z = __shfl_xor_sync(0xffffffffu, sum.z, o);
+      const float s = __shfl_xor_sync(0xffffffffu, sum.s, o);
+      add_sums(sum, m, z, s);
+      sum.above += __shfl_xor_sync(0xffffffffu, sum.above, o);
+    }
+    if (p.top > 0) best = lane < sh.n ? sh.cand[lane] : 0;
+    sh.part[lane] = best;
+    if (lane == 0) {
+      sh.cta_m = sum.m;
+      sh.cta_z = sum.z;
+      sh.cta_s = sum.s;
+      sh.cta_above = sum.above;
+    }
+  }
+  if (parts > 1) {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::
+                     : "memory");
+    if (part == 0 && warp == 0) {
+      for (int c = 1; c < parts; ++c) {
+        auto remote = [&](const void* q) {
+          uint32_t a;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(q)), "r"(c));
+          return a;
+        };
+        auto remote_f = [&](const void* q) {
+          float f;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(remote(q)) : "memory");
+          return f;
+        };
+        const float m = remote_f(&sh.cta_m), z = remote_f(&sh.cta_z), s = remote_f(&sh.cta_s);
+        add_sums(sum, m, z, s);
+        sum.above += __float_as_int(remote_f(&sh.cta_above));
+        if (p.top > 0) {
+          Key k;
+          asm volatile("ld.shared::cluster.u64 %0, [%1];"
+                       : "=l"(k)
+                       : "r"(remote(&sh.part[lane]))
+                       : "memory");
+          best = best_of(best, k);
+        }
+      }
+    }
+    // the others' shared memory stays until it has been read
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::
+                     : "memory");
+  }
+  if (part != 0 || warp != 0) return;
+  const bool undefined = sum.z != sum.z || sum.m == INFINITY;
+  const float ref = sum.m == -INFINITY ? 0.f : sum.m;
+  const float lz = sum.m == -INFINITY ? 0.f : logf(sum.z);
+  if (lane == 0) {
     p.logprob[row] = !asked ? 0.f : undefined ? NAN : xt - ref - lz;
-    if (p.entropy) p.entropy[row] = undefined ? NAN : m == -INFINITY ? 0.f : lz - xz / z;
-    if (p.rank) p.rank[row] = asked ? above : -1;
+    if (p.entropy)
+      p.entropy[row] =
+          undefined ? NAN : sum.m == -INFINITY ? 0.f : fmaxf(lz - kLn2 * (sum.s / sum.z), 0.f);
+    if (p.rank) p.rank[row] = asked ? sum.above : -1;
   }
-  // k rounds, each the largest behind the last one taken
-  float lx = INFINITY;
-  int li = -1;
-  for (int k = 0; k < p.top; ++k) {
-    float bx = -INFINITY;
-    int bi = INT_MAX;
-    for (int i = threadIdx.x; i < p.vocab; i += kThreads) {
-      const float x = load(p, row, i);
-      const bool left = x < lx || (x == lx && i > li);
-      if (left && (x > bx || bi == INT_MAX)) { bx = x; bi = i; }
-    }
-    const float best = block_fold(bi == INT_MAX ? -INFINITY : bx,
-                                  [](float a, float b) { return fmaxf(a, b); });
-    const int at = block_fold(bi != INT_MAX && bx == best ? bi : INT_MAX,
-                              [](int a, int b) { return min(a, b); });
-    if (threadIdx.x == 0) {
-      p.top_id[static_cast<long long>(row) * p.top + k] = at == INT_MAX ? -1 : at;
-      p.top_logprob[static_cast<long long>(row) * p.top + k] =
-          at == INT_MAX || undefined ? NAN : best - ref - lz;
-    }
-    lx = best;
-    li = at == INT_MAX ? INT_MAX : at;
+  if (lane < p.top) {
+    const long long at = static_cast<long long>(row) * p.top + lane;
+    p.top_id[at] = best ? key_index(best) : -1;
+    p.top_logprob[at] = !best || undefined ? NAN : key_value(best) - ref - lz;
   }
 }
 
@@ -100,8 +448,32 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobProblem 
 
 cudaError_t token_logprobs(const LogprobProblem& p, cudaStream_t st) {
   if (p.rows <= 0) return cudaSuccess;
-  logprob_kernel<<<p.rows, kThreads, 0, st>>>(p);
-  return cudaGetLastError();
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return e;
+  // A row is cut over a cluster while the rows alone leave SMs idle (two CTAs
+  // fit one) and a part is still a step of the loop.
+  int parts = 1;
+  constexpr int step = kThreads * kStep;
+  while (parts < kMaxCluster && static_cast<long long>(p.rows) * parts * 2 <= 2 * sms &&
+         p.vocab / (parts * 2) >= step / 2)
+    parts *= 2;
+  if (static_cast<long long>(p.rows) * parts > 0x7FFFFFFFll) return cudaErrorInvalidValue;
+  auto kernel = p.bf16 ? logprob_kernel<true> : logprob_kernel<false>;
+  e = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), static_cast<int>(sizeof(Shared)));
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.rows * parts);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = sizeof(Shared);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {static_cast<unsigned>(parts), 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = parts > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, p, parts);
 }
 
 }  // namespace dsv4
