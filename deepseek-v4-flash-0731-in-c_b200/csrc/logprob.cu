@@ -32,9 +32,10 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kStep = 16;            // values a thread reads per step
-constexpr int kRound = 4 * kThreads; // candidates that can join between two looks at their number
+constexpr int kRound = 4 * kThreads; // candidates of four values a thread
 constexpr int kCap = 2 * kRound;     // candidates held
 constexpr int kThin = 512;           // more than this many are thinned out to the best 32
+constexpr int kWindow = 8;           // steps between two looks at their number
 constexpr int kTop = kMaxTopAlternatives;
 constexpr int kMaxCluster = 8;
 constexpr float kLn2 = 0.69314718055994531f;
@@ -119,27 +120,56 @@ __device__ void compact(Shared& sh, int k) {
   __syncthreads();
 }
 
-// Running sums of a thread, in natural units relative to m.
+// Two fp32 values in one register pair (the packed arithmetic rounds each as
+// the scalar one does).
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pack2(float a, float b) {
+  return (static_cast<F2>(__float_as_uint(b)) << 32) | __float_as_uint(a);
+}
+__device__ __forceinline__ float lo2(F2 v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float hi2(F2 v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// Running sums in natural units relative to m: sum e^(x - m) and
+// sum e^(x - m) log2 e (x - m), each in two parts while a thread adds up.
 struct Sums {
-  float m, z, s;  // max, sum e^(x - m), sum e^(x - m) log2 e (x - m)
-  int above;
+  float m;
+  F2 z, s;
 };
 
 __device__ __forceinline__ void raise_max(Sums& t, float bm) {
-  if (bm > t.m) {  // m = -inf: nothing but zeros so far
-    const float d = fmaxf((t.m - bm) * kLog2e, -1e4f);  // (finite: it meets a zero)
-    const float f = t.m == -INFINITY ? 0.f : ex2_approx(d);
-    t.s = t.m == -INFINITY ? t.s : f * fmaf(d, t.z, t.s);
-    t.z = t.m == -INFINITY ? t.z : t.z * f;
+  if (bm > t.m) {
+    if (t.m != -INFINITY) {  // (nothing but zeros, or NaN, so far)
+      const float d = fmaxf((t.m - bm) * kLog2e, -1e4f);  // finite: it meets a zero
+      const float f = ex2_approx(d);
+      t.s = mul2(pack2(f, f), fma2(pack2(d, d), t.z, t.s));
+      t.z = mul2(pack2(f, f), t.z);
+    }
     t.m = bm;
   }
 }
 
-__device__ __forceinline__ void add_value(Sums& t, float ref, float x) {
+__device__ __forceinline__ void add_pair(Sums& t, F2 minus_ref, F2 x) {
   // x - ref first: exact where it matters, whatever the size of the logits
-  const float d = (x - ref) * kLog2e, e = ex2_approx(d);
-  t.z += e;
-  t.s = fmaf(e, fmaxf(d, -256.f), t.s);  // e = 0 below 2^-126: a masked value adds 0
+  const F2 d = mul2(add2(x, minus_ref), pack2(kLog2e, kLog2e));
+  const F2 e = pack2(ex2_approx(lo2(d)), ex2_approx(hi2(d)));
+  t.z = add2(t.z, e);
+  // e = 0 below 2^-126: a masked value adds 0
+  t.s = fma2(e, pack2(fmaxf(lo2(d), -256.f), fmaxf(hi2(d), -256.f)), t.s);
 }
 
 // 16 bytes that are read once.
@@ -197,8 +227,9 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProbl
     sh.n = 0;
     sh.limit = 0;
   }
-  Sums sum = {-INFINITY, 0.f, 0.f, 0};
-  uint4 buf[kVecs];
+  Sums sum = {-INFINITY, 0, 0};
+  int above = 0;
+  uint4 cur[kVecs], buf[kVecs];
   auto load = [&](int base) {
 #pragma unroll
     for (int u = 0; u < kVecs; ++u) {
@@ -206,126 +237,162 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProbl
       buf[u] = v < v1 ? ldg_stream(src + v) : V::none();
     }
   };
+  constexpr int kStride = kVecs * kThreads;  // vectors of a step
+  // The values of this thread's step at `base` that exceed the limit join the
+  // candidates; `first`: those that equal its value may, too. Past the
+  // capacity they are only counted.
+  auto join = [&](int base, int u, int i, bool first, Key limit, float lv) {
+    const float x = V::get(cur[u], i);
+    if (!(x > lv) && !(first && x == lv) && limit != 0) return;
+    const int v = base + u * kThreads + tid;
+    const Key k = make_key(x, head + v * kN + i);
+    if (v < v1 && x == x && k > limit) {
+      const int at = atomicAdd(&sh.n, 1);
+      if (at < kCap) sh.cand[at] = k;
+    }
+  };
+  auto join_step = [&](int base, float bm, bool first) {
+    const Key limit = *static_cast<volatile Key*>(&sh.limit);  // an old one only lets more in
+    const float lv = key_value(limit);
+    if (limit == 0 || bm > lv || (first && bm == lv)) {
+#pragma unroll
+      for (int u = 0; u < kVecs; ++u)
+#pragma unroll
+        for (int i = 0; i < kN; ++i) join(base, u, i, first, limit, lv);
+    }
+  };
   load(v0);
   __syncthreads();
   bool first = true;
-  for (int base = v0; base < v1; base += kVecs * kThreads) {
-    uint4 cur[kVecs];
+  int held = 0;  // candidates from before the window
+  for (int w0 = v0; w0 < v1; w0 += kWindow * kStride) {
+    const int w1 = min(v1, w0 + kWindow * kStride);
+    const int before = held;
+    for (int base = w0; base < w1; base += kStride) {
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u) cur[u] = buf[u];
-    if (base + kVecs * kThreads < v1) load(base + kVecs * kThreads);
-    float bm4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      for (int u = 0; u < kVecs; ++u) cur[u] = buf[u];
+      if (base + kStride < v1) load(base + kStride);
+      float bm4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u)
+      for (int u = 0; u < kVecs; ++u)
 #pragma unroll
-      for (int i = 0; i < kN; ++i) bm4[i & 3] = fmaxf(bm4[i & 3], V::get(cur[u], i));
-    const float bm = fmaxf(fmaxf(bm4[0], bm4[1]), fmaxf(bm4[2], bm4[3]));
-    raise_max(sum, bm);
-    const float ref = sum.m == -INFINITY ? 0.f : sum.m;
+        for (int i = 0; i < kN; ++i) bm4[i & 3] = fmaxf(bm4[i & 3], V::get(cur[u], i));
+      const float bm = fmaxf(fmaxf(bm4[0], bm4[1]), fmaxf(bm4[2], bm4[3]));
+      raise_max(sum, bm);
+      const float ref = sum.m == -INFINITY ? 0.f : sum.m;
+      const F2 minus_ref = pack2(-ref, -ref);
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-      const int v = base + u * kThreads + tid;
-      const int i0 = head + v * kN;
+      for (int u = 0; u < kVecs; ++u) {
+        const int v = base + u * kThreads + tid;
+        const int i0 = head + v * kN;
 #pragma unroll
-      for (int i = 0; i < kN; ++i) add_value(sum, ref, V::get(cur[u], i));
-      // equal values count where they come before the token
-      if (v < v1 && i0 + kN <= t) {
+        for (int i = 0; i < kN; i += 2)
+          add_pair(sum, minus_ref, pack2(V::get(cur[u], i), V::get(cur[u], i + 1)));
+        // equal values count where they come before the token
+        if (v < v1 && i0 + kN <= t) {
 #pragma unroll
-        for (int i = 0; i < kN; ++i) sum.above += V::get(cur[u], i) >= xt;
-      } else {
+          for (int i = 0; i < kN; ++i) above += V::get(cur[u], i) >= xt;
+        } else {
 #pragma unroll
-        for (int i = 0; i < kN; ++i) sum.above += V::get(cur[u], i) > xt;
-        if (i0 < t && v < v1) {
+          for (int i = 0; i < kN; ++i) above += V::get(cur[u], i) > xt;
+          if (i0 < t && v < v1) {
 #pragma unroll
-          for (int i = 0; i < kN; ++i) sum.above += V::get(cur[u], i) == xt && i0 + i < t;
+            for (int i = 0; i < kN; ++i) above += V::get(cur[u], i) == xt && i0 + i < t;
+          }
+        }
+      }
+      if (p.top > 0) {
+        if (first) {
+          // Every warp has kEach threads whose best value reaches its kEach-th
+          // best one, so kWarps * kEach >= k values reach the smallest of these.
+          constexpr int kEach = kTop / kWarps;
+          Key best = 0;
+#pragma unroll
+          for (int u = 0; u < kVecs; ++u) {
+            const int v = base + u * kThreads + tid;
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+              const float x = V::get(cur[u], i);
+              if (v < v1 && x == bm) {  // the first of them
+                const Key k = make_key(x, head + v * kN + i);
+                best = k > best ? k : best;
+              }
+            }
+          }
+          Key kth = best;
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) {
+            Key top = kth;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+              const Key other = __shfl_xor_sync(0xffffffffu, top, o);
+              top = other > top ? other : top;
+            }
+            if (e + 1 < kEach) {
+              if (kth == top) kth = 0;
+            } else {
+              kth = top;
+            }
+          }
+          if (lane == 0) sh.list[warp][0] = kth;
+          __syncthreads();
+          kth = sh.list[lane % kWarps][0];
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            const Key other = __shfl_xor_sync(0xffffffffu, kth, o);
+            kth = other < kth ? other : kth;
+          }
+          if (tid == 0 && kth) sh.limit = kth - 1;  // the one at the limit comes in
+          __syncthreads();
+        }
+        join_step(base, bm, first);
+        if (first) {
+          __syncthreads();
+          const int n = sh.n;
+          __syncthreads();  // nobody adds to it before all have read it
+          if (n > 2 * kTop && n <= kCap) compact(sh, p.top);
+          first = false;
         }
       }
     }
     if (p.top > 0) {
-      if (first) {
-        // Every warp has kEach threads whose best value reaches its kEach-th
-        // best one, so kWarps * kEach >= k values reach the smallest of these.
-        constexpr int kEach = kTop / kWarps;
-        Key best = 0;
-#pragma unroll
-        for (int u = 0; u < kVecs; ++u) {
-          const int v = base + u * kThreads + tid;
-#pragma unroll
-          for (int i = 0; i < kN; ++i) {
-            const float x = V::get(cur[u], i);
-            if (v < v1 && x == bm) {  // the first of them
-              const Key k = make_key(x, head + v * kN + i);
-              best = k > best ? k : best;
-            }
-          }
+      __syncthreads();
+      const int n = sh.n;
+      __syncthreads();
+      held = n;
+      if (n > kThin) held = kTop;
+      if (n > kCap) {
+        // more than fit (values in ascending order, say): the window again,
+        // four values a thread at a time, thinned out in between (the limit
+        // may be a value of this window, which has to come in again)
+        if (tid == 0) {
+          sh.n = before;
+          if (sh.limit) sh.limit -= 1;
         }
-        Key kth = best;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-          Key top = kth;
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) {
-            const Key other = __shfl_xor_sync(0xffffffffu, top, o);
-            top = other > top ? other : top;
-          }
-          if (e + 1 < kEach) {
-            if (kth == top) kth = 0;
-          } else {
-            kth = top;
-          }
-        }
-        if (lane == 0) sh.list[warp][0] = kth;
         __syncthreads();
-        kth = sh.list[lane % kWarps][0];
+        for (int base = w0; base < w1; base += kStride) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          const Key other = __shfl_xor_sync(0xffffffffu, kth, o);
-          kth = other < kth ? other : kth;
-        }
-        if (tid == 0 && kth) sh.limit = kth - 1;  // the one at the limit comes in
-        __syncthreads();
-      }
-      const Key limit = sh.limit;
-      const float lv = key_value(limit);
-      const bool look = limit == 0 || (first ? bm >= lv : bm > lv);
-      auto join = [&](int u, int i, Key above, float above_value) {
-        const float x = V::get(cur[u], i);
-        // (a key below the limit's with an equal value, or no limit yet)
-        if (!(x > above_value) && !(first && x == above_value) && above != 0) return;
-        const int v = base + u * kThreads + tid;
-        const Key k = make_key(x, head + v * kN + i);
-        if (v < v1 && x == x && k > above) sh.cand[atomicAdd(&sh.n, 1)] = k;
-      };
-      const int held = sh.n;  // (changes only behind the next barrier)
-      const int looking = __syncthreads_count(look);
-      if (looking > 0 && held + looking * kStep <= kCap - 64) {
-        if (look) {
+          for (int u = 0; u < kVecs; ++u) {
+            const int v = base + u * kThreads + tid;
+            cur[u] = v < v1 ? ldg_stream(src + v) : V::none();
+          }
 #pragma unroll
           for (int u = 0; u < kVecs; ++u)
 #pragma unroll
-            for (int i = 0; i < kN; ++i) join(u, i, limit, lv);
-        }
-        __syncthreads();
-        const int n = sh.n;
-        if (n > (first ? 2 * kTop : kThin)) compact(sh, p.top);
-      } else if (looking > 0) {
-        // more than fit (values in ascending order, say): four a thread at a
-        // time, thinned out in between
-#pragma unroll
-        for (int u = 0; u < kVecs; ++u)
-#pragma unroll
-          for (int i = 0; i < kN; ++i) {
-            if (look) join(u, i, sh.limit, key_value(sh.limit));
-            if (i % 4 == 3) {
-              __syncthreads();
-              const int n = sh.n;
-              __syncthreads();
-              if (n > kCap - 64 - kRound) compact(sh, p.top);
+            for (int i = 0; i < kN; ++i) {
+              join(base, u, i, true, sh.limit, key_value(sh.limit));
+              if (i % 4 == 3) {
+                __syncthreads();
+                const int m = sh.n;
+                __syncthreads();
+                if (m > kCap - kRound) compact(sh, p.top);
+              }
             }
-          }
+        }
+        compact(sh, p.top);
+      } else if (n > kThin) {
         compact(sh, p.top);
       }
-      first = false;
     }
   }
   // the values outside whole vectors: at most one a thread
@@ -336,62 +403,60 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProbl
       const float x = i >= 0 ? value_at(i) : -INFINITY;
       if (i >= 0) {
         raise_max(sum, x);
-        add_value(sum, sum.m == -INFINITY ? 0.f : sum.m, x);
-        sum.above += x > xt || (x == xt && i < t);
+        const float ref = sum.m == -INFINITY ? 0.f : sum.m;
+        add_pair(sum, pack2(-ref, -ref), pack2(x, -INFINITY));
+        above += x > xt || (x == xt && i < t);
         if (p.top > 0 && x == x) sh.cand[atomicAdd(&sh.n, 1)] = make_key(x, i);
       }
     }
   }
   if (p.top > 0) compact(sh, p.top);  // sorted, whatever their number
 
-  // the CTA's sums
-  auto add_sums = [](Sums& a, float m, float z, float s) {  // b's sums to a's
+  // the CTA's sums: from here on one value each, in the lower halves
+  sum.z = pack2(lo2(sum.z) + hi2(sum.z), 0.f);
+  sum.s = pack2(lo2(sum.s) + hi2(sum.s), 0.f);
+  auto add_sums = [](Sums& a, float m, float z, float s) {
     const float mx = fmaxf(a.m, m);
-    if (mx == -INFINITY) {  // only zeros, or NaN on either side
-      a.z += z;
-      a.s += s;
-      return;
+    Sums b = {m, pack2(z, 0.f), pack2(s, 0.f)};
+    if (mx != -INFINITY) {  // else only zeros, or NaN, on either side
+      raise_max(a, mx);
+      raise_max(b, mx);
     }
-    Sums b = {m, z, s, 0};
-    raise_max(a, mx);
-    raise_max(b, mx);
-    a.z += b.z;
-    a.s += b.s;
+    a.z = add2(a.z, b.z);
+    a.s = add2(a.s, b.s);
   };
+  auto warp_sums = [&] {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m = __shfl_xor_sync(0xffffffffu, sum.m, o);
-    const float z = __shfl_xor_sync(0xffffffffu, sum.z, o);
-    const float s = __shfl_xor_sync(0xffffffffu, sum.s, o);
-    add_sums(sum, m, z, s);
-    sum.above += __shfl_xor_sync(0xffffffffu, sum.above, o);
-  }
+    for (int o = 16; o > 0; o >>= 1) {
+      const float m = __shfl_xor_sync(0xffffffffu, sum.m, o);
+      const float z = __shfl_xor_sync(0xffffffffu, lo2(sum.z), o);
+      const float s = __shfl_xor_sync(0xffffffffu, lo2(sum.s), o);
+      add_sums(sum, m, z, s);
+      above += __shfl_xor_sync(0xffffffffu, above, o);
+    }
+  };
+  warp_sums();
   if (lane == 0) {
     sh.m[warp] = sum.m;
-    sh.z[warp] = sum.z;
-    sh.s[warp] = sum.s;
-    sh.above[warp] = sum.above;
+    sh.z[warp] = lo2(sum.z);
+    sh.s[warp] = lo2(sum.s);
+    sh.above[warp] = above;
   }
   __syncthreads();
   Key best = 0;
   if (warp == 0) {
-    sum = {sh.m[lane % kWarps], lane < kWarps ? sh.z[lane] : 0.f, lane < kWarps ? sh.s[lane] : 0.f,
-           lane < kWarps ? sh.above[lane] : 0};
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float m = __shfl_xor_sync(0xffffffffu, sum.m, o);
-      const float z = __shfl_xor_sync(0xffffffffu, sum.z, o);
-      const float s = __shfl_xor_sync(0xffffffffu, sum.s, o);
-      add_sums(sum, m, z, s);
-      sum.above += __shfl_xor_sync(0xffffffffu, sum.above, o);
-    }
+    const bool in = lane < kWarps;
+    sum = {in ? sh.m[lane] : -INFINITY, pack2(in ? sh.z[lane] : 0.f, 0.f),
+           pack2(in ? sh.s[lane] : 0.f, 0.f)};
+    above = in ? sh.above[lane] : 0;
+    warp_sums();
     if (p.top > 0) best = lane < sh.n ? sh.cand[lane] : 0;
     sh.part[lane] = best;
     if (lane == 0) {
       sh.cta_m = sum.m;
-      sh.cta_z = sum.z;
-      sh.cta_s = sum.s;
-      sh.cta_above = sum.above;
+      sh.cta_z = lo2(sum.z);
+      sh.cta_s = lo2(sum.s);
+      sh.cta_above = above;
     }
   }
   if (parts > 1) {
@@ -411,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProbl
         };
         const float m = remote_f(&sh.cta_m), z = remote_f(&sh.cta_z), s = remote_f(&sh.cta_s);
         add_sums(sum, m, z, s);
-        sum.above += __float_as_int(remote_f(&sh.cta_above));
+        above += __float_as_int(remote_f(&sh.cta_above));
         if (p.top > 0) {
           Key k;
           asm volatile("ld.shared::cluster.u64 %0, [%1];"
@@ -427,15 +492,15 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProbl
                      : "memory");
   }
   if (part != 0 || warp != 0) return;
-  const bool undefined = sum.z != sum.z || sum.m == INFINITY;
-  const float ref = sum.m == -INFINITY ? 0.f : sum.m;
-  const float lz = sum.m == -INFINITY ? 0.f : logf(sum.z);
+  const float z = lo2(sum.z), ref = sum.m == -INFINITY ? 0.f : sum.m;
+  const bool undefined = z != z || sum.m == INFINITY;
+  const float lz = sum.m == -INFINITY ? 0.f : logf(z);
   if (lane == 0) {
     p.logprob[row] = !asked ? 0.f : undefined ? NAN : xt - ref - lz;
     if (p.entropy)
       p.entropy[row] =
-          undefined ? NAN : sum.m == -INFINITY ? 0.f : fmaxf(lz - kLn2 * (sum.s / sum.z), 0.f);
-    if (p.rank) p.rank[row] = asked ? sum.above : -1;
+          undefined ? NAN : sum.m == -INFINITY ? 0.f : fmaxf(lz - kLn2 * (lo2(sum.s) / z), 0.f);
+    if (p.rank) p.rank[row] = asked ? above : -1;
   }
   if (lane < p.top) {
     const long long at = static_cast<long long>(row) * p.top + lane;
