@@ -124,10 +124,20 @@ __device__ void compact(Shared& sh, int k) {
 // the scalar one does).
 using F2 = unsigned long long;
 __device__ __forceinline__ F2 pack2(float a, float b) {
-  return (static_cast<F2>(__float_as_uint(b)) << 32) | __float_as_uint(a);
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
 }
-__device__ __forceinline__ float lo2(F2 v) { return __uint_as_float(static_cast<uint32_t>(v)); }
-__device__ __forceinline__ float hi2(F2 v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ float lo2(F2 v) {
+  float a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+  return a;
+}
+__device__ __forceinline__ float hi2(F2 v) {
+  float a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+  return b;
+}
 __device__ __forceinline__ F2 add2(F2 a, F2 b) {
   F2 r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -136,6 +146,17 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
 __device__ __forceinline__ F2 mul2(F2 a, F2 b) {
   F2 r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 1 where a > b (a >= b), else 0: counts of up to 2^24 in a register
+__device__ __forceinline__ float gt1(float a, float b) {
+  float r;
+  asm("set.gt.f32.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float ge1(float a, float b) {
+  float r;
+  asm("set.ge.f32.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
@@ -228,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProbl
     sh.limit = 0;
   }
   Sums sum = {-INFINITY, 0, 0};
-  int above = 0;
+  F2 above = 0;  // 1.0 for each
   uint4 cur[kVecs], buf[kVecs];
   auto load = [&](int base) {
 #pragma unroll
@@ -238,27 +259,17 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProbl
     }
   };
   constexpr int kStride = kVecs * kThreads;  // vectors of a step
-  // The values of this thread's step at `base` that exceed the limit join the
-  // candidates; `first`: those that equal its value may, too. Past the
-  // capacity they are only counted.
-  auto join = [&](int base, int u, int i, bool first, Key limit, float lv) {
+  // A value of this thread's step at `base` joins the candidates if its key
+  // exceeds the limit. Past the capacity they are only counted.
+  auto join = [&](int base, int u, int i, Key limit, float lv) {
     const float x = V::get(cur[u], i);
-    if (!(x > lv) && !(first && x == lv) && limit != 0) return;
-    const int v = base + u * kThreads + tid;
-    const Key k = make_key(x, head + v * kN + i);
-    if (v < v1 && x == x && k > limit) {
-      const int at = atomicAdd(&sh.n, 1);
-      if (at < kCap) sh.cand[at] = k;
-    }
-  };
-  auto join_step = [&](int base, float bm, bool first) {
-    const Key limit = *static_cast<volatile Key*>(&sh.limit);  // an old one only lets more in
-    const float lv = key_value(limit);
-    if (limit == 0 || bm > lv || (first && bm == lv)) {
-#pragma unroll
-      for (int u = 0; u < kVecs; ++u)
-#pragma unroll
-        for (int i = 0; i < kN; ++i) join(base, u, i, first, limit, lv);
+    if (x >= lv || limit == 0) {
+      const int v = base + u * kThreads + tid;
+      const Key k = make_key(x, head + v * kN + i);
+      if (v < v1 && x == x && k > limit) {
+        const int at = atomicAdd(&sh.n, 1);
+        if (at < kCap) sh.cand[at] = k;
+      }
     }
   };
   load(v0);
@@ -272,12 +283,14 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProbl
 #pragma unroll
       for (int u = 0; u < kVecs; ++u) cur[u] = buf[u];
       if (base + kStride < v1) load(base + kStride);
-      float bm4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      float vm[kVecs], bm = -INFINITY;  // the best of each vector
 #pragma unroll
-      for (int u = 0; u < kVecs; ++u)
+      for (int u = 0; u < kVecs; ++u) {
+        vm[u] = fmaxf(V::get(cur[u], 0), V::get(cur[u], 1));
 #pragma unroll
-        for (int i = 0; i < kN; ++i) bm4[i & 3] = fmaxf(bm4[i & 3], V::get(cur[u], i));
-      const float bm = fmaxf(fmaxf(bm4[0], bm4[1]), fmaxf(bm4[2], bm4[3]));
+        for (int i = 2; i < kN; ++i) vm[u] = fmaxf(vm[u], V::get(cur[u], i));
+        bm = fmaxf(bm, vm[u]);
+      }
       raise_max(sum, bm);
       const float ref = sum.m == -INFINITY ? 0.f : sum.m;
       const F2 minus_ref = pack2(-ref, -ref);
@@ -291,61 +304,49 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProbl
         // equal values count where they come before the token
         if (v < v1 && i0 + kN <= t) {
 #pragma unroll
-          for (int i = 0; i < kN; ++i) above += V::get(cur[u], i) >= xt;
+          for (int i = 0; i < kN; i += 2)
+            above = add2(above, pack2(ge1(V::get(cur[u], i), xt), ge1(V::get(cur[u], i + 1), xt)));
         } else {
 #pragma unroll
-          for (int i = 0; i < kN; ++i) above += V::get(cur[u], i) > xt;
+          for (int i = 0; i < kN; i += 2)
+            above = add2(above, pack2(gt1(V::get(cur[u], i), xt), gt1(V::get(cur[u], i + 1), xt)));
           if (i0 < t && v < v1) {
 #pragma unroll
-            for (int i = 0; i < kN; ++i) above += V::get(cur[u], i) == xt && i0 + i < t;
+            for (int i = 0; i < kN; ++i)
+              if (i0 + i < t && V::get(cur[u], i) == xt) above = add2(above, pack2(1.f, 0.f));
           }
         }
       }
       if (p.top > 0) {
         if (first) {
-          // Every warp has kEach threads whose best value reaches its kEach-th
-          // best one, so kWarps * kEach >= k values reach the smallest of these.
-          constexpr int kEach = kTop / kWarps;
-          Key best = 0;
-#pragma unroll
-          for (int u = 0; u < kVecs; ++u) {
-            const int v = base + u * kThreads + tid;
-#pragma unroll
-            for (int i = 0; i < kN; ++i) {
-              const float x = V::get(cur[u], i);
-              if (v < v1 && x == bm) {  // the first of them
-                const Key k = make_key(x, head + v * kN + i);
-                best = k > best ? k : best;
-              }
-            }
-          }
-          Key kth = best;
-#pragma unroll
-          for (int e = 0; e < kEach; ++e) {
-            Key top = kth;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-              const Key other = __shfl_xor_sync(0xffffffffu, top, o);
-              top = other > top ? other : top;
-            }
-            if (e + 1 < kEach) {
-              if (kth == top) kth = 0;
-            } else {
-              kth = top;
-            }
-          }
-          if (lane == 0) sh.list[warp][0] = kth;
+          // Every warp has two threads whose best value reaches the second
+          // best of them, so 2 kWarps >= k values reach the smallest of these.
+          static_assert(2 * kWarps >= kTop, "values that reach the first limit");
+          float kth = warp_max(bm);
+          const unsigned at_top = __ballot_sync(0xffffffffu, bm == kth);
+          if (__popc(at_top) == 1) kth = warp_max((at_top >> lane) & 1u ? -INFINITY : bm);
+          if (lane == 0) sh.m[warp] = kth;
           __syncthreads();
-          kth = sh.list[lane % kWarps][0];
+          kth = sh.m[lane % kWarps];
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) {
-            const Key other = __shfl_xor_sync(0xffffffffu, kth, o);
-            kth = other < kth ? other : kth;
-          }
-          if (tid == 0 && kth) sh.limit = kth - 1;  // the one at the limit comes in
+          for (int o = 16; o > 0; o >>= 1)
+            kth = fminf(kth, __shfl_xor_sync(0xffffffffu, kth, o));
+          // just below every key of that value (-inf may stand for no value at
+          // all: then there is no limit)
+          if (tid == 0 && kth > -INFINITY) sh.limit = make_key(kth, -1);
           __syncthreads();
         }
-        join_step(base, bm, first);
+        const Key limit = *static_cast<volatile Key*>(&sh.limit);  // an old one only lets more in
+        const float lv = limit ? key_value(limit) : -INFINITY;
+        // equal values count in the first step alone: later ones come behind
+        if (limit == 0 || (first ? bm >= lv : bm > lv)) {
+#pragma unroll
+          for (int u = 0; u < kVecs; ++u)
+            if (vm[u] >= lv) {
+#pragma unroll
+              for (int i = 0; i < kN; ++i) join(base, u, i, limit, lv);
+            }
+        }
         if (first) {
           __syncthreads();
           const int n = sh.n;
@@ -380,7 +381,8 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProbl
           for (int u = 0; u < kVecs; ++u)
 #pragma unroll
             for (int i = 0; i < kN; ++i) {
-              join(base, u, i, true, sh.limit, key_value(sh.limit));
+              const Key limit = sh.limit;
+              join(base, u, i, limit, limit ? key_value(limit) : -INFINITY);
               if (i % 4 == 3) {
                 __syncthreads();
                 const int m = sh.n;
@@ -405,13 +407,14 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProbl
         raise_max(sum, x);
         const float ref = sum.m == -INFINITY ? 0.f : sum.m;
         add_pair(sum, pack2(-ref, -ref), pack2(x, -INFINITY));
-        above += x > xt || (x == xt && i < t);
+        if (x > xt || (x == xt && i < t)) above = add2(above, pack2(1.f, 0.f));
         if (p.top > 0 && x == x) sh.cand[atomicAdd(&sh.n, 1)] = make_key(x, i);
       }
     }
   }
   if (p.top > 0) compact(sh, p.top);  // sorted, whatever their number
 
+  int n_above = static_cast<int>(lo2(above)) + static_cast<int>(hi2(above));
   // the CTA's sums: from here on one value each, in the lower halves
   sum.z = pack2(lo2(sum.z) + hi2(sum.z), 0.f);
   sum.s = pack2(lo2(sum.s) + hi2(sum.s), 0.f);
@@ -432,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProbl
       const float z = __shfl_xor_sync(0xffffffffu, lo2(sum.z), o);
       const float s = __shfl_xor_sync(0xffffffffu, lo2(sum.s), o);
       add_sums(sum, m, z, s);
-      above += __shfl_xor_sync(0xffffffffu, above, o);
+      n_above += __shfl_xor_sync(0xffffffffu, n_above, o);
     }
   };
   warp_sums();
@@ -440,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProbl
     sh.m[warp] = sum.m;
     sh.z[warp] = lo2(sum.z);
     sh.s[warp] = lo2(sum.s);
-    sh.above[warp] = above;
+    sh.above[warp] = n_above;
   }
   __syncthreads();
   Key best = 0;
@@ -448,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProbl
     const bool in = lane < kWarps;
     sum = {in ? sh.m[lane] : -INFINITY, pack2(in ? sh.z[lane] : 0.f, 0.f),
            pack2(in ? sh.s[lane] : 0.f, 0.f)};
-    above = in ? sh.above[lane] : 0;
+    n_above = in ? sh.above[lane] : 0;
     warp_sums();
     if (p.top > 0) best = lane < sh.n ? sh.cand[lane] : 0;
     sh.part[lane] = best;
@@ -456,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProbl
       sh.cta_m = sum.m;
       sh.cta_z = lo2(sum.z);
       sh.cta_s = lo2(sum.s);
-      sh.cta_above = above;
+      sh.cta_above = n_above;
     }
   }
   if (parts > 1) {
@@ -476,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProbl
         };
         const float m = remote_f(&sh.cta_m), z = remote_f(&sh.cta_z), s = remote_f(&sh.cta_s);
         add_sums(sum, m, z, s);
-        above += __float_as_int(remote_f(&sh.cta_above));
+        n_above += __float_as_int(remote_f(&sh.cta_above));
         if (p.top > 0) {
           Key k;
           asm volatile("ld.shared::cluster.u64 %0, [%1];"
@@ -500,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProbl
     if (p.entropy)
       p.entropy[row] =
           undefined ? NAN : sum.m == -INFINITY ? 0.f : fmaxf(lz - kLn2 * (lo2(sum.s) / z), 0.f);
-    if (p.rank) p.rank[row] = asked ? above : -1;
+    if (p.rank) p.rank[row] = asked ? n_above : -1;
   }
   if (lane < p.top) {
     const long long at = static_cast<long long>(row) * p.top + lane;
