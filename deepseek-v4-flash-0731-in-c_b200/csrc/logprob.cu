@@ -29,12 +29,12 @@
 namespace dsv4 {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kStep = 16;            // values a thread reads per step
 constexpr int kRound = 4 * kThreads; // candidates of four values a thread
 constexpr int kCap = 2 * kRound;     // candidates held
-constexpr int kThin = 512;           // more than this many are thinned out to the best 32
+constexpr int kThin = 256;           // more than this many are thinned out to the best 32
 constexpr int kWindow = 8;           // steps between two looks at their number
 constexpr int kTop = kMaxTopAlternatives;
 constexpr int kMaxCluster = 8;
@@ -219,7 +219,7 @@ struct Vec {
 };
 
 template <bool kBf16>
-__global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProblem p, int parts) {
+__global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobProblem p, int parts) {
   using V = Vec<kBf16>;
   constexpr int kN = V::kN, kVecs = kStep / kN;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -232,9 +232,6 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProbl
     return kBf16 ? bf16_widen(reinterpret_cast<const uint16_t*>(x_row)[i])
                  : reinterpret_cast<const float*>(x_row)[i];
   };
-  const int t = p.tokens[row];
-  const bool asked = t >= 0 && t < p.vocab;
-  const float xt = asked ? value_at(t) : NAN;  // NaN: nothing is above it
   // values before the first 16-byte boundary, whole vectors, values behind the last
   const int off = static_cast<int>(reinterpret_cast<uintptr_t>(x_row) & 15);
   const int head = min(p.vocab, off ? (16 - off) / kSize : 0);
@@ -273,6 +270,9 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProbl
     }
   };
   load(v0);
+  const int t = p.tokens[row];
+  const bool asked = t >= 0 && t < p.vocab;
+  const float xt = asked ? value_at(t) : NAN;  // NaN: nothing is above it
   __syncthreads();
   bool first = true;
   int held = 0;  // candidates from before the window
@@ -319,12 +319,15 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobProbl
       }
       if (p.top > 0) {
         if (first) {
-          // Every warp has two threads whose best value reaches the second
-          // best of them, so 2 kWarps >= k values reach the smallest of these.
-          static_assert(2 * kWarps >= kTop, "values that reach the first limit");
-          float kth = warp_max(bm);
-          const unsigned at_top = __ballot_sync(0xffffffffu, bm == kth);
-          if (__popc(at_top) == 1) kth = warp_max((at_top >> lane) & 1u ? -INFINITY : bm);
+          // Every warp has `each` threads whose best value reaches the each-th
+          // best of them, so each * kWarps >= k values reach the smallest of
+          // these.
+          float mine = bm, kth = warp_max(mine);
+          for (int each = kWarps; each < p.top; each += kWarps) {
+            const unsigned at_top = __ballot_sync(0xffffffffu, mine == kth);
+            if (lane == __ffs(at_top) - 1) mine = -INFINITY;
+            kth = warp_max(mine);
+          }
           if (lane == 0) sh.m[warp] = kth;
           __syncthreads();
           kth = sh.m[lane % kWarps];
@@ -520,11 +523,11 @@ cudaError_t token_logprobs(const LogprobProblem& p, cudaStream_t st) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return e;
-  // A row is cut over a cluster while the rows alone leave SMs idle (two CTAs
+  // A row is cut over a cluster while the rows alone leave SMs idle (four CTAs
   // fit one) and a part is still a step of the loop.
   int parts = 1;
   constexpr int step = kThreads * kStep;
-  while (parts < kMaxCluster && static_cast<long long>(p.rows) * parts * 2 <= 2 * sms &&
+  while (parts < kMaxCluster && static_cast<long long>(p.rows) * parts * 2 <= 4 * sms &&
          p.vocab / (parts * 2) >= step / 2)
     parts *= 2;
   if (static_cast<long long>(p.rows) * parts > 0x7FFFFFFFll) return cudaErrorInvalidValue;
