@@ -31,13 +31,12 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kStep = 16;            // values a thread reads per step
 constexpr int kRound = 4 * kThreads; // candidates of four values a thread
 constexpr int kCap = 2 * kRound;     // candidates held
 constexpr int kThin = 256;           // more than this many are thinned out to the best 32
 constexpr int kWindow = 8;           // steps between two looks at their number
 constexpr int kTop = kMaxTopAlternatives;
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 16;
 constexpr float kLn2 = 0.69314718055994531f;
 using Key = unsigned long long;      // 0: nothing
 
@@ -79,42 +78,63 @@ __device__ __forceinline__ Key best_of(Key a, Key b) {
   return merge_sorted(a > r ? a : r);
 }
 
-struct Shared {
+struct alignas(16) Shared {
   Key cand[kCap];
   Key list[kWarps][kTop];
-  Key part[kTop];              // this CTA's best, for the cluster
+  float4 part_sums[kMaxCluster];  // the parts of a cluster, in its first CTA
+  Key part[kMaxCluster][kTop];
   float m[kWarps], z[kWarps], s[kWarps];
   int above[kWarps];
-  float cta_m, cta_z, cta_s;   // this CTA's sums, for the cluster
-  int cta_above;
   int n;                       // candidates held
   Key limit;                   // the k-th best so far, 0: fewer than k
 };
 
-// The best 32 of the n candidates, descending, to cand[0 .. 31]; the k-th is
-// the new limit. Whole block.
-__device__ void compact(Shared& sh, int k) {
+// Warp 0: the best of the first `used` warps' sequences, by pairs, then pairs
+// of pairs. Whole block.
+__device__ Key best_of_warps(Shared& sh, Key best, int used) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  __syncthreads();
-  const int n = sh.n;
-  Key best = 0;
-  for (int base = warp * 32; base < n; base += kThreads) {
-    const int i = base + lane;
-    best = best_of(best, sort_lanes(i < n ? sh.cand[i] : 0));
-  }
-  // pairs of warps, then pairs of pairs
-  const int used = min(kWarps, (n + 31) / 32);
   for (int s = 1; s < used; s <<= 1) {
     if (warp & s) sh.list[warp][lane] = best;
     __syncthreads();
     if ((warp & (2 * s - 1)) == 0 && warp + s < used) best = best_of(best, sh.list[warp + s][lane]);
   }
+  return best;
+}
+
+// The best 32 of the n candidates, descending, to cand[0 .. 31]; the k-th is
+// the new limit. Whole block.
+__device__ void compact(Shared& sh, int k) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  __syncthreads();
+  const int n = sh.n;
+  if (n <= kThreads) {
+    // a thread a key: its place is the number of larger ones (keys differ)
+    const Key mine = tid < n ? sh.cand[tid] : 0;
+    int rank = 0;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) rank += sh.cand[i] > mine;
+    __syncthreads();
+    if (tid < n && rank < kTop) {
+      sh.cand[rank] = mine;
+      if (rank == k - 1) sh.limit = mine;
+    }
+    if (tid == 0) sh.n = min(n, kTop);
+    __syncthreads();
+    return;
+  }
+  Key best = 0;
+  for (int base = warp * 32; base < n; base += kThreads) {
+    const int i = base + lane;
+    const Key next = sort_lanes(i < n ? sh.cand[i] : 0);
+    best = base == warp * 32 ? next : best_of(best, next);
+  }
+  best = best_of_warps(sh, best, kWarps);
   if (warp == 0) {
     sh.cand[lane] = best;
     const Key kth = __shfl_sync(0xffffffffu, best, k - 1);
     if (lane == 0) {
       sh.limit = kth;
-      sh.n = min(n, kTop);
+      sh.n = kTop;
     }
   }
   __syncthreads();
@@ -202,6 +222,13 @@ __device__ __forceinline__ uint4 ldg_stream(const uint4* p) {
   return v;
 }
 
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 template <bool kBf16>
 struct Vec {
   static constexpr int kN = kBf16 ? 8 : 4;  // values of 16 bytes
@@ -218,13 +245,15 @@ struct Vec {
   }
 };
 
-template <bool kBf16>
-__global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobProblem p, int parts) {
+// kStep: values a thread reads per step; kBlocks: blocks of an SM.
+template <bool kBf16, int kStep, int kBlocks>
+__global__ void __launch_bounds__(kThreads, kBlocks) logprob_kernel(const LogprobProblem p, int parts) {
   using V = Vec<kBf16>;
   constexpr int kN = V::kN, kVecs = kStep / kN;
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& sh = *reinterpret_cast<Shared*>(smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (parts > 1) cluster_arrive();
   const int row = blockIdx.x / parts, part = blockIdx.x % parts;
   constexpr int kSize = kBf16 ? 2 : 4;
   const uint8_t* x_row = static_cast<const uint8_t*>(p.logits) + row * p.stride * kSize;
@@ -283,14 +312,17 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobProbl
 #pragma unroll
       for (int u = 0; u < kVecs; ++u) cur[u] = buf[u];
       if (base + kStride < v1) load(base + kStride);
-      float vm[kVecs], bm = -INFINITY;  // the best of each vector
+      float vm[kVecs];
 #pragma unroll
       for (int u = 0; u < kVecs; ++u) {
         vm[u] = fmaxf(V::get(cur[u], 0), V::get(cur[u], 1));
 #pragma unroll
         for (int i = 2; i < kN; ++i) vm[u] = fmaxf(vm[u], V::get(cur[u], i));
-        bm = fmaxf(bm, vm[u]);
       }
+      float bm = vm[0];
+#pragma unroll
+      for (int u = 1; u < kVecs; ++u) bm = fmaxf(bm, vm[u]);
+      bm = fmaxf(bm, -INFINITY);  // NaN where every value is one
       raise_max(sum, bm);
       const float ref = sum.m == -INFINITY ? 0.f : sum.m;
       const F2 minus_ref = pack2(-ref, -ref);
@@ -341,11 +373,12 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobProbl
         }
         const Key limit = *static_cast<volatile Key*>(&sh.limit);  // an old one only lets more in
         const float lv = limit ? key_value(limit) : -INFINITY;
-        // equal values count in the first step alone: later ones come behind
+        // (equal values can count in the first step alone: later ones come
+        // behind)
         if (limit == 0 || (first ? bm >= lv : bm > lv)) {
 #pragma unroll
           for (int u = 0; u < kVecs; ++u)
-            if (vm[u] >= lv) {
+            if (limit == 0 || vm[u] >= lv) {
 #pragma unroll
               for (int i = 0; i < kN; ++i) join(base, u, i, limit, lv);
             }
@@ -354,7 +387,8 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobProbl
           __syncthreads();
           const int n = sh.n;
           __syncthreads();  // nobody adds to it before all have read it
-          if (n > 2 * kTop && n <= kCap) compact(sh, p.top);
+          // (worth it where enough is still to come)
+          if (n > kTop && n <= kCap && v1 - v0 > 2 * kStride) compact(sh, p.top);
           first = false;
         }
       }
@@ -421,25 +455,17 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobProbl
   // the CTA's sums: from here on one value each, in the lower halves
   sum.z = pack2(lo2(sum.z) + hi2(sum.z), 0.f);
   sum.s = pack2(lo2(sum.s) + hi2(sum.s), 0.f);
-  auto add_sums = [](Sums& a, float m, float z, float s) {
-    const float mx = fmaxf(a.m, m);
-    Sums b = {m, pack2(z, 0.f), pack2(s, 0.f)};
-    if (mx != -INFINITY) {  // else only zeros, or NaN, on either side
-      raise_max(a, mx);
-      raise_max(b, mx);
-    }
-    a.z = add2(a.z, b.z);
-    a.s = add2(a.s, b.s);
-  };
   auto warp_sums = [&] {
+    raise_max(sum, warp_max(sum.m));
+    float z = lo2(sum.z), w = lo2(sum.s);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      const float m = __shfl_xor_sync(0xffffffffu, sum.m, o);
-      const float z = __shfl_xor_sync(0xffffffffu, lo2(sum.z), o);
-      const float s = __shfl_xor_sync(0xffffffffu, lo2(sum.s), o);
-      add_sums(sum, m, z, s);
-      n_above += __shfl_xor_sync(0xffffffffu, n_above, o);
+      z += __shfl_xor_sync(0xffffffffu, z, o);
+      w += __shfl_xor_sync(0xffffffffu, w, o);
     }
+    sum.z = pack2(z, 0.f);
+    sum.s = pack2(w, 0.f);
+    n_above = __reduce_add_sync(0xffffffffu, n_above);
   };
   warp_sums();
   if (lane == 0) {
@@ -457,45 +483,41 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobProbl
     n_above = in ? sh.above[lane] : 0;
     warp_sums();
     if (p.top > 0) best = lane < sh.n ? sh.cand[lane] : 0;
-    sh.part[lane] = best;
-    if (lane == 0) {
-      sh.cta_m = sum.m;
-      sh.cta_z = lo2(sum.z);
-      sh.cta_s = lo2(sum.s);
-      sh.cta_above = n_above;
-    }
   }
   if (parts > 1) {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::
+    static_assert(kMaxCluster <= 2 * kWarps && kMaxCluster <= 32, "two parts a warp");
+    // every part writes into the first CTA's shared memory, which is there
+    // since all have arrived at the barrier of the start
+    cluster_wait();
+    if (warp == 0) {
+      auto remote = [&](const void* q) {
+        uint32_t a;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_addr(q)));
+        return a;
+      };
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote(&sh.part[part][lane])), "l"(best)
+                   : "memory");
+      if (lane == 0)
+        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(
+                         remote(&sh.part_sums[part])),
+                     "f"(sum.m), "f"(lo2(sum.z)), "f"(lo2(sum.s)), "f"(__int_as_float(n_above))
                      : "memory");
-    if (part == 0 && warp == 0) {
-      for (int c = 1; c < parts; ++c) {
-        auto remote = [&](const void* q) {
-          uint32_t a;
-          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(q)), "r"(c));
-          return a;
-        };
-        auto remote_f = [&](const void* q) {
-          float f;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(remote(q)) : "memory");
-          return f;
-        };
-        const float m = remote_f(&sh.cta_m), z = remote_f(&sh.cta_z), s = remote_f(&sh.cta_s);
-        add_sums(sum, m, z, s);
-        n_above += __float_as_int(remote_f(&sh.cta_above));
-        if (p.top > 0) {
-          Key k;
-          asm volatile("ld.shared::cluster.u64 %0, [%1];"
-                       : "=l"(k)
-                       : "r"(remote(&sh.part[lane]))
-                       : "memory");
-          best = best_of(best, k);
-        }
-      }
     }
-    // the others' shared memory stays until it has been read
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::
-                     : "memory");
+    cluster_arrive();
+    if (part != 0) return;
+    cluster_wait();
+    if (p.top > 0) {
+      best = warp < parts ? sh.part[warp][lane] : 0;
+      if (warp + kWarps < parts) best = best_of(best, sh.part[warp + kWarps][lane]);
+      best = best_of_warps(sh, best, min(parts, kWarps));
+    }
+    if (warp == 0) {
+      const float4 q = sh.part_sums[lane % parts];
+      const bool in = lane < parts;
+      sum = {in ? q.x : -INFINITY, pack2(in ? q.y : 0.f, 0.f), pack2(in ? q.z : 0.f, 0.f)};
+      n_above = in ? __float_as_int(q.w) : 0;
+      warp_sums();
+    }
   }
   if (part != 0 || warp != 0) return;
   const float z = lo2(sum.z), ref = sum.m == -INFINITY ? 0.f : sum.m;
@@ -523,16 +545,26 @@ cudaError_t token_logprobs(const LogprobProblem& p, cudaStream_t st) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return e;
-  // A row is cut over a cluster while the rows alone leave SMs idle (four CTAs
-  // fit one) and a part is still a step of the loop.
+  // Few rows: each is cut over a cluster so that a thread's 32 values are all
+  // it reads, and the k best are picked once. More rows than that leave room
+  // for: steps of 16 values, four blocks to an SM, rows cut while SMs idle.
+  constexpr int kShort = 32, kLong = 16;
   int parts = 1;
-  constexpr int step = kThreads * kStep;
-  while (parts < kMaxCluster && static_cast<long long>(p.rows) * parts * 2 <= 4 * sms &&
-         p.vocab / (parts * 2) >= step / 2)
-    parts *= 2;
+  while (parts < kMaxCluster && p.vocab > parts * kThreads * kShort) parts *= 2;
+  const bool few = static_cast<long long>(p.rows) * parts <= 2 * sms;
+  if (!few) {
+    parts = 1;
+    while (parts < 8 && static_cast<long long>(p.rows) * parts * 2 <= 4 * sms &&
+           p.vocab / (parts * 2) >= kThreads * kLong / 2)
+      parts *= 2;
+  }
   if (static_cast<long long>(p.rows) * parts > 0x7FFFFFFFll) return cudaErrorInvalidValue;
-  auto kernel = p.bf16 ? logprob_kernel<true> : logprob_kernel<false>;
-  e = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), static_cast<int>(sizeof(Shared)));
+  auto kernel = few ? (p.bf16 ? logprob_kernel<true, kShort, 2> : logprob_kernel<false, kShort, 2>)
+                    : (p.bf16 ? logprob_kernel<true, kLong, 4> : logprob_kernel<false, kLong, 4>);
+  const void* fn = reinterpret_cast<const void*>(kernel);
+  e = set_max_dynamic_smem(fn, static_cast<int>(sizeof(Shared)));
+  if (e == cudaSuccess && parts > 8)  // more than every device has to take
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.rows * parts);
