@@ -1656,12 +1656,19 @@ bool paged_state(const char* who, const dsv4cuda_paged* p, dsv4::PagedState* s) 
   return true;
 }
 
-bool attn_problem(const char* who, const dsv4cuda_paged* p, const dsv4cuda_paged_attn_shape* s,
-                  dsv4::PagedAttnProblem* a) {
-  if (!s || !paged_state(who, p, &a->pages)) {
+bool attn_problem(const char* who, const dsv4cuda_paged* p, int layer,
+                  const dsv4cuda_paged_attn_shape* s, dsv4::PagedAttnProblem* a) {
+  dsv4::PagedState g;
+  if (!s || !paged_state(who, p, &g)) {
     if (!s) record_error("%s: bad arguments", who);
     return false;
   }
+  if (layer < 0 || layer >= g.layers) {
+    record_error("%s: layer %d of %d", who, layer, g.layers);
+    return false;
+  }
+  a->pages = {g.codes[layer], g.scales[layer], g.rope[layer], g.nope,  g.rope_dim, g.page,
+              g.n_pages,      g.n_seqs,        g.max_pages,   g.table, g.length,   g.status};
   const int d = a->pages.nope + a->pages.rope_dim;
   const long long width = static_cast<long long>(s->heads) * s->head_dim;
   const long long qs = s->q_stride ? s->q_stride : width;
@@ -1743,7 +1750,7 @@ DSV4_API int dsv4cuda_paged_compact(const dsv4cuda_paged* p, int* table_out, int
 DSV4_API size_t dsv4cuda_paged_attn_workspace_bytes(const dsv4cuda_paged* p,
                                                     const dsv4cuda_paged_attn_shape* shape) {
   dsv4::PagedAttnProblem a;
-  if (!attn_problem("dsv4cuda_paged_attn_workspace_bytes", p, shape, &a)) return 0;
+  if (!attn_problem("dsv4cuda_paged_attn_workspace_bytes", p, 0, shape, &a)) return 0;
   return dsv4::paged_attn_workspace_bytes(a);
 }
 
@@ -1753,8 +1760,8 @@ DSV4_API int dsv4cuda_paged_attn(void* out, const void* q, const dsv4cuda_paged*
                                  const dsv4cuda_paged_attn_shape* shape, void* workspace,
                                  size_t workspace_bytes, void* stream) {
   dsv4::PagedAttnProblem a;
-  if (!attn_problem("dsv4cuda_paged_attn", p, shape, &a)) return -1;
-  if (layer < 0 || layer >= p->n_caches || (rope_cos == nullptr) != (rope_sin == nullptr) ||
+  if (!attn_problem("dsv4cuda_paged_attn", p, layer, shape, &a)) return -1;
+  if ((rope_cos == nullptr) != (rope_sin == nullptr) ||
       (shape->n_rows > 0 && (!out || !q || !q_start))) {
     record_error("dsv4cuda_paged_attn: bad arguments");
     return -1;
@@ -1765,7 +1772,6 @@ DSV4_API int dsv4cuda_paged_attn(void* out, const void* q, const dsv4cuda_paged*
     return -1;
   }
   if (shape->n_rows == 0) return 0;
-  a.layer = layer;
   a.q = q;
   a.out = out;
   a.q_start = q_start;

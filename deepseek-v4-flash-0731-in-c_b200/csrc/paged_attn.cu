@@ -28,13 +28,13 @@ constexpr int kMaxDim = 1024;              // of the general kernel
 constexpr int kLaneDims = kMaxDim / 32;
 constexpr int kSimtWarps = 8;
 
-__device__ __forceinline__ float latent_value(const PagedState& c, int layer, long long r, int i) {
+__device__ __forceinline__ float latent_value(const PagedLayer& c, long long r, int i) {
   if (i < c.nope) {
-    const float v = e4m3_decode(c.codes[layer][r * c.nope + i]) *
-                    e8m0_decode(c.scales[layer][r * kKvScaleSlots + i / 64]);
+    const float v = e4m3_decode(c.codes[r * c.nope + i]) *
+                    e8m0_decode(c.scales[r * kKvScaleSlots + i / 64]);
     return isfinite(v) ? bf16_round(v) : v;  // the rounding's carry would turn a NaN into a zero
   }
-  return bf16_widen(c.rope[layer][r * c.rope_dim + (i - c.nope)]);
+  return bf16_widen(c.rope[r * c.rope_dim + (i - c.nope)]);
 }
 
 // The slot whose rows hold row `row`: the last s with q_start[s] <= row that
@@ -62,7 +62,7 @@ __device__ __forceinline__ void store_out(const PagedAttnProblem& p, long long a
 // maximum and sum of a softmax per warp, merged at the end.
 __global__ void __launch_bounds__(32 * kSimtWarps) paged_attn_simt_kernel(
     const __grid_constant__ PagedAttnProblem p) {
-  const PagedState& c = p.pages;
+  const PagedLayer& c = p.pages;
   const int row = blockIdx.x, h = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int d = c.nope + c.rope_dim;
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(32 * kSimtWarps) paged_attn_simt_kernel(
 #pragma unroll
       for (int u = 0; u < kLaneDims; ++u) {
         const int i = u * 32 + lane;
-        k[u] = i < d ? latent_value(c, p.layer, r, i) : 0.f;
+        k[u] = i < d ? latent_value(c, r, i) : 0.f;
         fine = fine && isfinite(k[u]);
         dot = fmaf(q[u], k[u], dot);
       }
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(kStageThreads) stage_kernel(const __grid_const
   extern __shared__ int sm[];
   __shared__ int row_broken[kUnit], row_there[kUnit];
   const PagedAttnProblem& p = c.p;
-  const PagedState& g = p.pages;
+  const PagedLayer& g = p.pages;
   int* block_start = sm;                  // [n_seqs + 1]
   int* tile_start = sm + g.n_seqs + 1;
   const int tid = threadIdx.x;
@@ -369,9 +369,9 @@ __global__ void __launch_bounds__(kStageThreads) stage_kernel(const __grid_const
   }
   const long long units = min(static_cast<long long>(blocks), c.s.block_cap) * (kKeys / kUnit);
   const int piece = tid % 36, r0 = tid / 36;
-  const uint8_t* codes = g.codes[p.layer];
-  const uint8_t* scales = g.scales[p.layer];
-  const uint16_t* rope = g.rope[p.layer];
+  const uint8_t* codes = g.codes;
+  const uint8_t* scales = g.scales;
+  const uint16_t* rope = g.rope;
   for (long long u = blockIdx.x - 1; u < units; u += gridDim.x - 1) {
     const int block = static_cast<int>(u / (kKeys / kUnit));
     int lo = 0, hi = g.n_seqs;

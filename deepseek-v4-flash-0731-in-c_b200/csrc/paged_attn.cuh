@@ -8,9 +8,20 @@
 
 namespace dsv4 {
 
+// One layer's cache and the tables, as the attention kernels take them.
+struct PagedLayer {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  const uint16_t* rope;
+  int nope, rope_dim;
+  int page, n_pages, n_seqs, max_pages;
+  const int* table;
+  const int* length;
+  unsigned* status;
+};
+
 struct PagedAttnProblem {
-  PagedState pages;
-  int layer = 0;
+  PagedLayer pages;
   const void* q = nullptr;          // [total][H][d] BF16 or fp32 (BF16-valued)
   void* out = nullptr;              // as q
   bool bf16 = true;

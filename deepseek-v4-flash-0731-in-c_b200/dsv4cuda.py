@@ -123,7 +123,8 @@ def _f32(a):
 def _stream(stream):
     if stream is None:
         import torch
-        return torch.cuda.current_stream().cuda_stream
+        # the current stream's handle without a Stream object around it (3 us a call)
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
     return stream
 
 
@@ -728,26 +729,27 @@ class PagedCache:
         return v
 
 
-def _paged_attn_shape(q, out, paged, max_new, max_len, scale, window, rope_cos, max_keys):
+def _paged_attn_shape(q, out, max_new, max_len, scale, window, rope_cos, max_keys):
     import torch
-    if (q.dtype not in (torch.bfloat16, torch.float32) or out.dtype is not q.dtype or q.dim() != 3
-            or out.shape != q.shape or not q.is_cuda or not out.is_cuda):
+    dtype, shape = q.dtype, q.shape
+    bf16 = dtype is torch.bfloat16
+    if (not (bf16 or dtype is torch.float32) or out.dtype is not dtype or len(shape) != 3
+            or out.shape != shape or not q.is_cuda or not out.is_cuda):
         raise ValueError("q and out: CUDA tensors [rows][heads][head_dim] of one type, bfloat16 or "
                          "float32")
-    n, heads, d = q.shape
-    for t, name in ((q, "q"), (out, "out")):
-        if t.stride(2) != 1 or t.stride(1) != d:
-            raise ValueError(f"{name}: the heads of a row must lie one behind the other")
+    n, heads, d = shape
+    qs, os_ = q.stride(), out.stride()
+    if qs[2] != 1 or os_[2] != 1 or (heads > 1 and (qs[1] != d or os_[1] != d)):
+        raise ValueError("q and out: the heads of a row must lie one behind the other")
     # the stride of a single row has no meaning to torch, nor here
-    return PagedAttnShape(n, heads, d, 1 if q.dtype is torch.bfloat16 else 0,
-                          q.stride(0) if n > 1 else 0, out.stride(0) if n > 1 else 0, max_new,
-                          max_len, window, max_keys,
+    return PagedAttnShape(n, heads, d, 1 if bf16 else 0, qs[0] if n > 1 else 0,
+                          os_[0] if n > 1 else 0, max_new, max_len, window, max_keys,
                           0 if rope_cos is None else 2 * rope_cos.shape[-1], scale)
 
 
 def paged_attn_workspace_bytes(q, paged, max_new, max_len, window=0, max_keys=0) -> int:
     """Workspace of a paged_attn call of these sizes (q as there)."""
-    shape = _paged_attn_shape(q, q, paged, max_new, max_len, 1.0, window, None, max_keys)
+    shape = _paged_attn_shape(q, q, max_new, max_len, 1.0, window, None, max_keys)
     return lib.dsv4cuda_paged_attn_workspace_bytes(paged._ref, C.byref(shape))
 
 
@@ -761,8 +763,8 @@ def paged_attn(out, q, paged: PagedCache, layer, q_start, max_new, max_len, scal
     tensor (needed while capturing)."""
     import torch
     f32 = torch.float32
-    shape = _paged_attn_shape(q, out, paged, max_new, max_len, scale, window, rope_cos, max_keys)
-    n, heads, _ = q.shape
+    shape = _paged_attn_shape(q, out, max_new, max_len, scale, window, rope_cos, max_keys)
+    n, heads = shape.n_rows, shape.heads
     half = n * (shape.rope_dim // 2)
     _check(lib.dsv4cuda_paged_attn(
         out.data_ptr(), q.data_ptr(), paged._ref, layer,
