@@ -11,6 +11,8 @@
 
 #include <climits>
 
+#include "launch.cuh"
+
 namespace dsv4 {
 namespace {
 
@@ -24,7 +26,8 @@ struct PageJob {
 struct Ws {
   int* head;      // [0] jobs, [1] pages in use
   PageJob* jobs;  // [max(n_seqs, n_pages)]
-  int* map;       // [n_pages]
+  long long* first;  // [n_seqs + 1] first token of each op
+  int* map;          // [n_pages]
 };
 
 __host__ __device__ inline int max_jobs(int n_pages, int n_seqs) {
@@ -35,30 +38,34 @@ __host__ __device__ inline Ws carve(void* ws, int n_pages, int n_seqs) {
   Ws w;
   w.head = static_cast<int*>(ws);
   w.jobs = reinterpret_cast<PageJob*>(w.head + 64);
-  w.map = reinterpret_cast<int*>(w.jobs + max_jobs(n_pages, n_seqs));
+  // (12-byte jobs: rounded up to whole 16 bytes)
+  w.first = reinterpret_cast<long long*>(reinterpret_cast<char*>(w.jobs) +
+                                         ((sizeof(PageJob) * max_jobs(n_pages, n_seqs) + 15) & ~15ull));
+  w.map = reinterpret_cast<int*>(w.first + n_seqs + 1);
   return w;
 }
 
 // Exclusive prefix sum over the block's threads; *total = the block's sum.
-__device__ int block_scan(int v, int* total) {
-  __shared__ int part[32];
-  __shared__ int sum;
+template <class T>
+__device__ T block_scan(T v, T* total) {
+  __shared__ T part[32];
+  __shared__ T sum;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  int incl = v;
+  T incl = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, incl, o);
+    const T u = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += u;
   }
   __syncthreads();  // the previous call's reads of part and sum
   if (lane == 31) part[warp] = incl;
   __syncthreads();
   if (warp == 0) {
-    const int w = lane < nw ? part[lane] : 0;
-    int wi = w;
+    const T w = lane < nw ? part[lane] : 0;
+    T wi = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, wi, o);
+      const T u = __shfl_up_sync(0xffffffffu, wi, o);
       if (lane >= o) wi += u;
     }
     part[lane] = wi - w;
@@ -75,16 +82,33 @@ __device__ void raise(const PagedState& p, unsigned bits) {
   if (p.status) atomicOr(p.status, bits);
 }
 
+// Four counts of pages from q on; pages that there are not are in use.
+__device__ __forceinline__ int4 refs4(const PagedState& p, int q) {
+  if (q + 3 < p.n_pages && (reinterpret_cast<uintptr_t>(p.refs) & 15) == 0)
+    return *reinterpret_cast<const int4*>(p.refs + q);
+  return make_int4(q < p.n_pages ? p.refs[q] : 1, q + 1 < p.n_pages ? p.refs[q + 1] : 1,
+                   q + 2 < p.n_pages ? p.refs[q + 2] : 1, q + 3 < p.n_pages ? p.refs[q + 3] : 1);
+}
+
 // The lowest `want` free pages, ascending, into page[]; returns how many
-// there are. Whole block.
+// there are. Whole block: four pages a thread, the next four on their way.
 __device__ int take_free(const PagedState& p, int want, int* page) {
   int have = 0;
-  for (int base = 0; base < p.n_pages && have < want; base += blockDim.x) {
-    const int q = base + threadIdx.x;
-    const int is_free = q < p.n_pages && p.refs[q] == 0;
+  const int q0 = 4 * threadIdx.x;
+  int4 next = want > 0 ? refs4(p, q0) : make_int4(1, 1, 1, 1);
+  for (int base = 0; base < p.n_pages && have < want; base += 4 * blockDim.x) {
+    const int q = base + q0;
+    const int4 r = next;
+    if (base + 4 * static_cast<int>(blockDim.x) < p.n_pages) next = refs4(p, q + 4 * blockDim.x);
+    const int f[4] = {r.x == 0, r.y == 0, r.z == 0, r.w == 0};
     int total;
-    const int r = have + block_scan(is_free, &total);
-    if (is_free && r < want) page[r] = q;
+    int at = have + block_scan(f[0] + f[1] + f[2] + f[3], &total);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (f[i]) {
+        if (at < want) page[at] = q + i;
+        ++at;
+      }
     have += total;
   }
   __syncthreads();
@@ -107,6 +131,7 @@ __global__ void __launch_bounds__(kMetaThreads) fork_kernel(const __grid_constan
   int* owner = sm;                 // [n_seqs]
   int* rank = owner + p.n_seqs;    // [n] place among the ops that need a page; -1 none, -2 no op
   int* page = rank + n;            // [n] the pages taken
+  pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
   claim(p, dst, n, owner);
   // Which ops are done, and which of them need a page of their own: the
@@ -196,6 +221,7 @@ __global__ void __launch_bounds__(kMetaThreads) append_kernel(const __grid_const
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
   const Ws w = carve(p.ws, p.n_pages, p.n_seqs);
   int* page = w.map;
+  pdl_trigger();
   claim(p, slots, n, owner);
   int needs = 0;
   for (int base = 0; base < n; base += blockDim.x) {
@@ -223,25 +249,15 @@ __global__ void __launch_bounds__(kMetaThreads) append_kernel(const __grid_const
     needs += total;
   }
   const int got = take_free(p, min(needs, p.n_pages), page);
-  long long out = 0;  // tokens of the ops before
-  for (int base = 0; base < n; base += nw) {
-    // this round's ops: where their tokens' rows go
-    long long mine = out;
-    for (int k = 0; k < nw && base + k < n; ++k) {
-      const int c = max(counts[base + k], 0);
-      if (k < warp) mine += c;
-      out += c;
-    }
-    const int i = base + warp;
-    if (i >= n) continue;
-    const int s = slots[i], c = max(counts[i], 0), r = start[i];
-    bool done = r >= 0;
-    int len = 0;
-    if (done) {
+  for (int i = warp; i < n; i += nw) {
+    const int r = start[i];
+    int len = -1;  // not done
+    if (r >= 0) {
+      const int s = slots[i], c = counts[i];
       len = p.length[s];
       const int have = (len + p.page - 1) / p.page, want = (len + c + p.page - 1) / p.page;
       if (want > have && r + want - have > got) {
-        done = false;
+        len = -1;
         if (lane == 0) raise(p, kPagedExhausted);
       } else {
         int* row = p.table + static_cast<size_t>(s) * p.max_pages;
@@ -250,19 +266,49 @@ __global__ void __launch_bounds__(kMetaThreads) append_kernel(const __grid_const
           p.refs[page[r + j]] = 1;
         }
         __syncwarp();
+        if (lane == 0) p.length[s] = len + c;
       }
     }
-    if (rows) {
-      const int* row = done ? p.table + static_cast<size_t>(s) * p.max_pages : nullptr;
-      for (int t = lane; t < c && mine + t < n_rows; t += 32) {
-        const int pos = len + t;
-        rows[mine + t] =
-            done ? static_cast<long long>(row[pos / p.page]) * p.page + pos % p.page : -1;
-      }
-      if (mine + c > n_rows && lane == 0) raise(p, kPagedBadOp);
+    if (lane == 0) w.jobs[i].src = len;
+  }
+  // tokens of the ops before each: where their rows go
+  long long out = 0;
+  for (int base = 0; base < n; base += blockDim.x) {
+    const int i = base + threadIdx.x;
+    long long total;
+    const long long r = block_scan(i < n ? max(counts[i], 0) + 0ll : 0ll, &total);
+    if (i < n) w.first[i] = out + r;
+    out += total;
+  }
+  if (threadIdx.x == 0) {
+    w.first[n] = out;
+    if (rows && out > n_rows) raise(p, kPagedBadOp);
+  }
+}
+
+// The cache row of each new token.
+__global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ PagedState p,
+                                                   const int* __restrict__ slots, int n,
+                                                   long long* __restrict__ rows, long long n_rows) {
+  pdl_wait();
+  const Ws w = carve(p.ws, p.n_pages, p.n_seqs);
+  const long long total = min(w.first[n], n_rows);
+  for (long long t = blockIdx.x * 256ll + threadIdx.x; t < total; t += gridDim.x * 256ll) {
+    int lo = 0, hi = n;  // the last op with first <= t
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (w.first[mid] <= t) lo = mid;
+      else hi = mid;
     }
-    __syncwarp();
-    if (done && lane == 0) p.length[s] = len + c;
+    const int len = w.jobs[lo].src;
+    long long row = -1;
+    if (len >= 0) {
+      const int pos = len + static_cast<int>(t - w.first[lo]);
+      row = static_cast<long long>(
+                p.table[static_cast<size_t>(slots[lo]) * p.max_pages + pos / p.page]) * p.page +
+            pos % p.page;
+    }
+    rows[t] = row;
   }
 }
 
@@ -270,95 +316,182 @@ __global__ void __launch_bounds__(kMetaThreads) append_kernel(const __grid_const
 // it: no page is both, so all moves can run at once, and their number is
 // the smallest that makes the pool dense.
 __global__ void __launch_bounds__(kMetaThreads) compact_kernel(
-    const __grid_constant__ PagedState p, int* __restrict__ refs_out) {
+    const __grid_constant__ PagedState p, int* refs_out) {
+  pdl_trigger();
   const Ws w = carve(p.ws, p.n_pages, p.n_seqs);
   int live = 0;
-  for (int base = 0; base < p.n_pages; base += blockDim.x) {
-    const int q = base + threadIdx.x;
-    int total;
-    block_scan(q < p.n_pages && p.refs[q] > 0, &total);
-    live += total;
+  for (int q = 4 * threadIdx.x; q < p.n_pages; q += 4 * blockDim.x) {
+    const int4 r = refs4(p, q);
+    live += (r.x > 0) + (r.y > 0) + (r.z > 0) + (r.w > 0);
+    if (q + 3 >= p.n_pages)  // (the ones that there are not)
+      live -= min(3, q + 4 - p.n_pages);
   }
+  block_scan(live, &live);
   int holes = 0, moves = 0;
-  for (int base = 0; base < p.n_pages; base += blockDim.x) {
-    const int q = base + threadIdx.x;
-    const bool used = q < p.n_pages && p.refs[q] > 0;
-    const bool hole = q < live && !used, move = q >= live && used;
-    int th, tm;
-    const int h = holes + block_scan(hole, &th);
-    const int m = moves + block_scan(move, &tm);
-    if (hole) w.jobs[h].dst = q;
-    if (move) {
-      w.jobs[m].src = q;
-      w.jobs[m].rows = p.page;
-      w.map[q] = m;
+  for (int base = 0; base < p.n_pages; base += 4 * blockDim.x) {
+    const int q = base + 4 * threadIdx.x;
+    const int4 r4 = refs4(p, q);
+    const int r[4] = {r4.x, r4.y, r4.z, r4.w};
+    int h = 0, m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool in = q + i < p.n_pages;
+      h += in && q + i < live && r[i] == 0;
+      m += in && q + i >= live && r[i] > 0;
     }
-    holes += th;
-    moves += tm;
+    // both counts in one scan: below 2^16 a block's step
+    int total;
+    const int before = block_scan(h | (m << 16), &total);
+    int ha = holes + (before & 0xFFFF), ma = moves + (before >> 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (q + i >= p.n_pages) continue;
+      if (q + i < live) {
+        if (r[i] == 0) w.jobs[ha++].dst = q + i;
+      } else if (r[i] > 0) {
+        w.jobs[ma].src = q + i;
+        w.jobs[ma].rows = p.page;
+        w.map[q + i] = ma++;
+      } else {
+        w.map[q + i] = -1;  // free: no table names it
+      }
+    }
+    holes += total & 0xFFFF;
+    moves += total >> 16;
   }
   __syncthreads();
-  // refs_out may be refs: a move's two pages are read and written by one thread
-  for (int q = threadIdx.x; q < p.n_pages; q += blockDim.x) {
-    if (q >= live && p.refs[q] > 0) {
-      const int to = w.jobs[w.map[q]].dst, r = p.refs[q];
-      refs_out[to] = r;
-      refs_out[q] = 0;
-      w.map[q] = to;
-    } else if (q >= live) {
-      refs_out[q] = p.refs[q];
-      w.map[q] = -1;  // free: no table names it
-    } else if (p.refs[q] > 0) {
-      refs_out[q] = p.refs[q];
-    }
+  // (refs_out may be refs: a move's two pages are one thread's)
+  for (int i = threadIdx.x; i < moves; i += blockDim.x) {
+    const PageJob j = w.jobs[i];
+    const int r = p.refs[j.src];
+    w.map[j.src] = j.dst;
+    refs_out[j.dst] = r;
+    refs_out[j.src] = 0;
   }
+  __syncthreads();
+  if (refs_out != p.refs)
+    for (int q = threadIdx.x; q < p.n_pages; q += blockDim.x) {
+      const int r = p.refs[q];
+      if (q < live ? r > 0 : r <= 0) refs_out[q] = r;
+    }
   if (threadIdx.x == 0) {
     w.head[0] = moves;
     w.head[1] = live;
   }
 }
 
-__global__ void remap_kernel(const __grid_constant__ PagedState p, int* __restrict__ table_out) {
+constexpr int kCopyThreads = 256;
+constexpr int kCopyVecs = 10;  // 16-byte vectors in flight per thread: a page of 64 rows at once
+
+// `bytes` from src to dst in pieces of T, whose size divides all three.
+template <class T>
+__device__ __forceinline__ void copy_pieces(uint8_t* dst, const uint8_t* src, size_t bytes) {
+  const size_t n = bytes / sizeof(T);
+  for (size_t i = threadIdx.x; i < n; i += kCopyThreads)
+    reinterpret_cast<T*>(dst)[i] = reinterpret_cast<const T*>(src)[i];
+}
+
+__device__ void copy_any(uint8_t* dst, const uint8_t* src, size_t bytes) {
+  const uintptr_t a =
+      reinterpret_cast<uintptr_t>(dst) | reinterpret_cast<uintptr_t>(src) | bytes;
+  if (a % 16 == 0) copy_pieces<uint4>(dst, src, bytes);
+  else if (a % 8 == 0) copy_pieces<uint2>(dst, src, bytes);
+  else if (a % 4 == 0) copy_pieces<uint32_t>(dst, src, bytes);
+  else copy_pieces<uint16_t>(dst, src, bytes);  // rows of BF16 values
+}
+
+// The rows of one (job, layer) per block and round. A move is read and
+// written once, so the memory bounds it: all of a page's vectors are loaded
+// before the first is stored.
+__device__ void copy_jobs(const PagedState& p, long long block, long long blocks) {
+  const Ws w = carve(p.ws, p.n_pages, p.n_seqs);
+  const long long n = static_cast<long long>(w.head[0]) * p.layers;
+  for (long long b = block; b < n; b += blocks) {
+    const PageJob j = w.jobs[b / p.layers];
+    const int l = static_cast<int>(b % p.layers);
+    const size_t from = static_cast<size_t>(j.src) * p.page, to = static_cast<size_t>(j.dst) * p.page;
+    const size_t rows = j.rows;
+    const uint8_t* codes = p.codes[l] + from * p.nope;
+    uint8_t* codes_to = p.codes[l] + to * p.nope;
+    const uint8_t* rope = reinterpret_cast<const uint8_t*>(p.rope[l] + from * p.rope_dim);
+    uint8_t* rope_to = reinterpret_cast<uint8_t*>(p.rope[l] + to * p.rope_dim);
+    const uint2* scales = reinterpret_cast<const uint2*>(p.scales[l] + from * 8);
+    uint2* scales_to = reinterpret_cast<uint2*>(p.scales[l] + to * 8);
+    const size_t rope_bytes = rows * p.rope_dim * 2;
+    const bool wide =
+        ((reinterpret_cast<uintptr_t>(rope) | reinterpret_cast<uintptr_t>(rope_to) | rope_bytes) &
+         15) == 0;
+    // codes (64 a group: always whole vectors), then RoPE values
+    const int nc = static_cast<int>(rows * p.nope / 16);
+    const int nv = nc + (wide ? static_cast<int>(rope_bytes / 16) : 0);
+    uint2 sc = make_uint2(0, 0);
+    const bool one_scale = rows <= kCopyThreads;
+    if (one_scale && threadIdx.x < rows) sc = __ldg(scales + threadIdx.x);
+    for (int v0 = threadIdx.x; v0 < nv; v0 += kCopyVecs * kCopyThreads) {
+      uint4 x[kCopyVecs];
+#pragma unroll
+      for (int u = 0; u < kCopyVecs; ++u) {
+        const int v = v0 + u * kCopyThreads;
+        if (v < nv)
+          x[u] = v < nc ? __ldg(reinterpret_cast<const uint4*>(codes) + v)
+                        : __ldg(reinterpret_cast<const uint4*>(rope) + (v - nc));
+      }
+#pragma unroll
+      for (int u = 0; u < kCopyVecs; ++u) {
+        const int v = v0 + u * kCopyThreads;
+        if (v < nv) {
+          if (v < nc) reinterpret_cast<uint4*>(codes_to)[v] = x[u];
+          else reinterpret_cast<uint4*>(rope_to)[v - nc] = x[u];
+        }
+      }
+    }
+    if (one_scale) {
+      if (threadIdx.x < rows) scales_to[threadIdx.x] = sc;
+    } else {
+      for (size_t i = threadIdx.x; i < rows; i += kCopyThreads) scales_to[i] = __ldg(scales + i);
+    }
+    if (!wide) copy_any(rope_to, rope, rope_bytes);
+  }
+}
+
+__global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constant__ PagedState p) {
+  pdl_wait();
+  copy_jobs(p, blockIdx.x, gridDim.x);
+}
+
+// After compact_kernel: the tables in the first blocks, the rows in the others.
+__global__ void __launch_bounds__(kCopyThreads) move_kernel(const __grid_constant__ PagedState p,
+                                                            int* __restrict__ table_out,
+                                                            int table_blocks) {
+  pdl_wait();
+  if (static_cast<int>(blockIdx.x) >= table_blocks) {
+    copy_jobs(p, blockIdx.x - table_blocks, gridDim.x - table_blocks);
+    return;
+  }
   const Ws w = carve(p.ws, p.n_pages, p.n_seqs);
   const int live = w.head[1];
-  const size_t n = static_cast<size_t>(p.n_seqs) * p.max_pages;
-  for (size_t i = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; i < n;
-       i += static_cast<size_t>(gridDim.x) * blockDim.x) {
+  const int n = p.n_seqs * p.max_pages;
+  for (long long i = blockIdx.x * static_cast<long long>(kCopyThreads) + threadIdx.x; i < n;
+       i += static_cast<long long>(table_blocks) * kCopyThreads) {
     const int q = p.table[i];
     table_out[i] = q >= live && q < p.n_pages ? w.map[q] : q;
   }
 }
 
-__device__ void copy_bytes(uint8_t* dst, const uint8_t* src, size_t bytes) {
-  for (size_t i = threadIdx.x; i < bytes; i += blockDim.x) dst[i] = src[i];
-}
-
-// One block per (job, layer), jobs striding over the grid.
-__global__ void __launch_bounds__(256) copy_kernel(const __grid_constant__ PagedState p) {
-  const Ws w = carve(p.ws, p.n_pages, p.n_seqs);
-  const long long n = static_cast<long long>(w.head[0]) * p.layers;
-  for (long long b = blockIdx.x; b < n; b += gridDim.x) {
-    const PageJob j = w.jobs[b / p.layers];
-    const int l = static_cast<int>(b % p.layers);
-    const size_t from = static_cast<size_t>(j.src) * p.page, to = static_cast<size_t>(j.dst) * p.page;
-    copy_bytes(p.codes[l] + to * p.nope, p.codes[l] + from * p.nope,
-               static_cast<size_t>(j.rows) * p.nope);
-    copy_bytes(p.scales[l] + to * 8, p.scales[l] + from * 8, static_cast<size_t>(j.rows) * 8);
-    copy_bytes(reinterpret_cast<uint8_t*>(p.rope[l] + to * p.rope_dim),
-               reinterpret_cast<const uint8_t*>(p.rope[l] + from * p.rope_dim),
-               static_cast<size_t>(j.rows) * p.rope_dim * 2);
-  }
-}
-
-cudaError_t smem_limit(const void* fn, size_t bytes) {
-  return bytes <= 48 * 1024 ? cudaSuccess
-                            : cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   static_cast<int>(bytes));
+// Blocks that keep the memory busy: eight an SM hold what one of them waits for.
+int copy_blocks(long long most) {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess)
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const long long all = 8ll * sms;
+  return static_cast<int>(most < 1 ? 1 : most < all ? most : all);
 }
 
 }  // namespace
 
 size_t paged_workspace_bytes(int n_pages, int n_seqs) {
-  return 256 + sizeof(PageJob) * static_cast<size_t>(max_jobs(n_pages, n_seqs)) +
+  return 256 + sizeof(PageJob) * static_cast<size_t>(max_jobs(n_pages, n_seqs)) + 16 +
+         sizeof(long long) * (static_cast<size_t>(n_seqs) + 1) +
          sizeof(int) * static_cast<size_t>(n_pages);
 }
 
@@ -366,28 +499,39 @@ cudaError_t paged_fork(const PagedState& p, const int* dst, const int* src, int 
                        cudaStream_t st) {
   if (n <= 0) return cudaSuccess;
   const size_t smem = sizeof(int) * (static_cast<size_t>(p.n_seqs) + 2 * static_cast<size_t>(n));
-  cudaError_t e = smem_limit(reinterpret_cast<const void*>(fork_kernel), smem);
+  cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(fork_kernel),
+                                       sizeof(int) * 3 * kPagedMaxSeqs);
   if (e != cudaSuccess) return e;
   fork_kernel<<<1, kMetaThreads, smem, st>>>(p, dst, src, n);
-  copy_kernel<<<148 * 8, 256, 0, st>>>(p);
-  return cudaGetLastError();
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  return launch_pdl(copy_kernel, dim3(copy_blocks(static_cast<long long>(n) * p.layers)),
+                    dim3(kCopyThreads), 0, st, p);
 }
 
 cudaError_t paged_append(const PagedState& p, const int* slots, const int* counts, int n,
                          long long* rows, long long n_rows, cudaStream_t st) {
   if (n <= 0) return cudaSuccess;
   const size_t smem = sizeof(int) * (static_cast<size_t>(p.n_seqs) + static_cast<size_t>(n));
-  cudaError_t e = smem_limit(reinterpret_cast<const void*>(append_kernel), smem);
+  cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(append_kernel),
+                                       sizeof(int) * 2 * kPagedMaxSeqs);
   if (e != cudaSuccess) return e;
   append_kernel<<<1, kMetaThreads, smem, st>>>(p, slots, counts, n, rows, n_rows);
-  return cudaGetLastError();
+  e = cudaGetLastError();
+  if (e != cudaSuccess || !rows || n_rows <= 0) return e;
+  return launch_pdl(rows_kernel, dim3(copy_blocks((n_rows + 255) / 256)), dim3(256), 0, st, p,
+                    slots, n, rows, n_rows);
 }
 
 cudaError_t paged_compact(const PagedState& p, int* table_out, int* refs_out, cudaStream_t st) {
   compact_kernel<<<1, kMetaThreads, 0, st>>>(p, refs_out);
-  remap_kernel<<<148, 256, 0, st>>>(p, table_out);
-  copy_kernel<<<148 * 8, 256, 0, st>>>(p);
-  return cudaGetLastError();
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  const int table_blocks =
+      copy_blocks((static_cast<long long>(p.n_seqs) * p.max_pages + 1023) / 1024);
+  return launch_pdl(move_kernel,
+                    dim3(table_blocks + copy_blocks(static_cast<long long>(p.n_pages / 2) * p.layers)),
+                    dim3(kCopyThreads), 0, st, p, table_out, table_blocks);
 }
 
 }  // namespace dsv4
