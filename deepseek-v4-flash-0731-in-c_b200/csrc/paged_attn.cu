@@ -204,9 +204,9 @@ struct PlanHead {
 struct TcWs {
   PlanHead* head;
   Tile* tiles;
-  int* pair_tile;         // [pairs] tile that a share starts in
-  uint16_t* valid;        // [blocks][4] a bit per key
-  uint16_t* broken;       // [blocks][4] keys with a NaN or infinity (decoded as zeros)
+  Tile* first_tile;       // [pairs] the tile that a share starts in
+  uint8_t* valid;         // [blocks][8] a bit per key
+  uint8_t* broken;        // [blocks][8] keys with a NaN or infinity (decoded as zeros)
   float* part_m;          // [pairs][2][2 halves][128] log2 units
   float* part_den;
   float* part_o;          // [pairs][2][128][512]
@@ -251,8 +251,8 @@ __device__ __forceinline__ Slot slot_geometry(const PagedAttnProblem& p, int tok
   return g;
 }
 
-constexpr int kStageThreads = 288;  // 36 pieces of a row, 8 rows at a time
-constexpr int kUnit = 16;           // rows decoded together
+constexpr int kStageThreads = 256;
+constexpr int kUnit = 8;            // rows that a warp decodes together
 
 // Exclusive prefix sum over the block; *total = the sum.
 __device__ int stage_scan(int v, int* total) {
@@ -328,11 +328,19 @@ __device__ void list_tiles(const TcCall& c, const int* block_start, const int* t
   }
 }
 
-// Latents to BF16 rows. One row is 28 pieces of 16 codes and 8 of 8 RoPE
-// values, a thread per piece, two rows in flight.
+__device__ __forceinline__ void st_global_32(void* p, uint4 a, uint4 b) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x),
+               "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
+
+// Latents to BF16 rows: a warp per 8 rows, no barriers. Lane l has the dims
+// 16 l .. 16 l + 15 of each: 16 codes, or (lanes 28-31) the first 8 of 16 RoPE
+// values, whose other 8 are lane 4 r + (l - 28)'s for row r. All loads of the
+// 8 rows are on their way before the first is used; a row's codes leave as
+// whole sectors.
 __global__ void __launch_bounds__(kStageThreads) stage_kernel(const __grid_constant__ TcCall c) {
   extern __shared__ int sm[];
-  __shared__ int row_broken[kUnit], row_there[kUnit];
   const PagedAttnProblem& p = c.p;
   const PagedLayer& g = p.pages;
   int* block_start = sm;                  // [n_seqs + 1]
@@ -368,11 +376,25 @@ __global__ void __launch_bounds__(kStageThreads) stage_kernel(const __grid_const
     return;
   }
   const long long units = min(static_cast<long long>(blocks), c.s.block_cap) * (kKeys / kUnit);
-  const int piece = tid % 36, r0 = tid / 36;
-  const uint8_t* codes = g.codes;
-  const uint8_t* scales = g.scales;
-  const uint16_t* rope = g.rope;
-  for (long long u = blockIdx.x - 1; u < units; u += gridDim.x - 1) {
+  const int lane = tid & 31, warps = kStageThreads / 32;
+  const bool is_code = lane < 28;
+  const uint8_t* lane_src = is_code ? g.codes + 16 * lane
+                                    : reinterpret_cast<const uint8_t*>(g.rope) + 32 * (lane - 28);
+  const size_t pitch = is_code ? kNope : 2 * kRope;
+  // Non-zero where one of this lane's values is not finite: the E4M3 NaN has
+  // all magnitude bits set, a BF16 NaN or infinity all exponent bits, and
+  // adding one to the field carries into the bit above it.
+  const uint32_t field = is_code ? 0x7F7F7F7Fu : 0x7F807F80u;
+  const uint32_t one = is_code ? 0x01010101u : 0x00800080u;
+  const uint32_t above = is_code ? 0x80808080u : 0x80008000u;
+  auto special4 = [](const uint4& v, uint32_t f, uint32_t o, uint32_t a) {
+    return (((v.x & f) + o) | ((v.y & f) + o) | ((v.z & f) + o) | ((v.w & f) + o)) & a;
+  };
+  auto special_bf16 = [&](const uint4& v) {
+    return special4(v, 0x7F807F80u, 0x00800080u, 0x80008000u);
+  };
+  for (long long u = (blockIdx.x - 1ll) * warps + (tid >> 5); u < units;
+       u += (gridDim.x - 1ll) * warps) {
     const int block = static_cast<int>(u / (kKeys / kUnit));
     int lo = 0, hi = g.n_seqs;
     while (hi - lo > 1) {
@@ -382,97 +404,82 @@ __global__ void __launch_bounds__(kStageThreads) stage_kernel(const __grid_const
     }
     const int len = g.length[lo], first = len - (p.q_start[lo + 1] - p.q_start[lo]);
     const int klo = p.window > 0 ? max(0, first - p.window + 1) : 0;
-    const int t0 = klo + (block - block_start[lo]) * kKeys +
-                   static_cast<int>(u % (kKeys / kUnit)) * kUnit;
-    if (tid < kUnit) row_broken[tid] = 0;
-    __syncthreads();
-    uint4 raw[2];
-    uint32_t sc[2] = {127u, 127u};
-    bool there[2];
+    // lanes 0-7: the cache row of their key, -1: none
+    const int t = klo + (block - block_start[lo]) * kKeys +
+                  static_cast<int>(u % (kKeys / kUnit)) * kUnit + (lane & 7);
+    int row = -1;
+    if (lane < kUnit && t < len && t / g.page < g.max_pages) {
+      const int page = g.table[static_cast<size_t>(lo) * g.max_pages + t / g.page];
+      if (page >= 0 && page < g.n_pages) row = page * g.page + t % g.page;
+    }
+    const unsigned there = __ballot_sync(0xffffffffu, row >= 0);
+    const int rc = max(row, 0);  // (an absent key's lanes load row 0 and do not use it)
+    uint4 raw[kUnit];
+    // 4 scale codes: of key lane & 7, groups 0-3 or (lanes 16-31) 4-7
+    const uint32_t sc = __ldg(reinterpret_cast<const uint32_t*>(
+        g.scales + static_cast<size_t>(__shfl_sync(0xffffffffu, rc, lane & 7)) * kKvScaleSlots +
+        4 * (lane >> 4)));
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int t = t0 + r0 + 8 * k;
-      raw[k] = make_uint4(0, 0, 0, 0);
-      there[k] = false;
-      if (t < len && t / g.page < g.max_pages) {
-        const int page = g.table[static_cast<size_t>(lo) * g.max_pages + t / g.page];
-        if (page >= 0 && page < g.n_pages) {
-          const long long r = static_cast<long long>(page) * g.page + t % g.page;
-          there[k] = true;
-          if (piece < 28) {
-            raw[k] = __ldg(reinterpret_cast<const uint4*>(codes + r * kNope) + piece);
-            sc[k] = __ldg(scales + r * kKvScaleSlots + piece / 4);
-          } else {
-            raw[k] = __ldg(reinterpret_cast<const uint4*>(rope + r * kRope) + (piece - 28));
-          }
-        }
+    for (int r = 0; r < kUnit; ++r)
+      raw[r] = __ldg(reinterpret_cast<const uint4*>(
+          lane_src + static_cast<size_t>(__shfl_sync(0xffffffffu, rc, r)) * pitch));
+    const uint4 more = __ldg(reinterpret_cast<const uint4*>(
+        reinterpret_cast<const uint8_t*>(g.rope) +
+        static_cast<size_t>(__shfl_sync(0xffffffffu, rc, lane >> 2)) * (2 * kRope) +
+        32 * (lane & 3) + 16));
+    uint32_t code[kUnit];  // the scale code of this lane's dims
+    bool in_range = true;
+    unsigned bad = special_bf16(more) ? 1u << (lane >> 2) : 0u;
+#pragma unroll
+    for (int r = 0; r < kUnit; ++r) {
+      code[r] = (__shfl_sync(0xffffffffu, sc, r + (lane & 16)) >> (8 * ((lane >> 2) & 3))) & 0xFFu;
+      in_range = in_range && code[r] - 10u <= 124u;
+      bad |= (special4(raw[r], field, one, above) ? 1u : 0u) << r;
+    }
+    const bool fast = __all_sync(0xffffffffu, in_range || !is_code);
+    if (!fast && is_code) {  // a large scale may take a finite code beyond BF16's range
+#pragma unroll
+      for (int r = 0; r < kUnit; ++r) {
+        const float f = e8m0_decode(code[r]);
+        const uint2 a = e4m3x4_to_bf16(raw[r].x, f), b = e4m3x4_to_bf16(raw[r].y, f);
+        const uint2 d = e4m3x4_to_bf16(raw[r].z, f), e = e4m3x4_to_bf16(raw[r].w, f);
+        if (special_bf16(make_uint4(a.x, a.y, b.x, b.y)) | special_bf16(make_uint4(d.x, d.y, e.x, e.y)))
+          bad |= 1u << r;
       }
     }
-    uint4 lo16[2], hi16[2];
+    bad = __reduce_or_sync(0xffffffffu, bad) & there;
+    const unsigned keep = there & ~bad;  // the others are zeros: they take part in no sum
+    uint8_t* dst = reinterpret_cast<uint8_t*>(c.w.stage + u * kUnit * kD) + 32 * lane;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      bool broken = false;
-      if (piece < 28) {
-        const uint32_t nan = e4m3_nan_bytes(raw[k].x) | e4m3_nan_bytes(raw[k].y) |
-                             e4m3_nan_bytes(raw[k].z) | e4m3_nan_bytes(raw[k].w);
-        uint2 a, b, d, e;
-        if (sc[k] >= 10 && sc[k] <= 134) {
-          const uint32_t k2 = (sc[k] + 120) * 0x00800080u;
-          a = e4m3x4_to_bf16_mul(raw[k].x, k2);
-          b = e4m3x4_to_bf16_mul(raw[k].y, k2);
-          d = e4m3x4_to_bf16_mul(raw[k].z, k2);
-          e = e4m3x4_to_bf16_mul(raw[k].w, k2);
-          broken = nan != 0;
+    for (int r = 0; r < kUnit; ++r) {
+      uint4 x = make_uint4(0, 0, 0, 0), y = x;
+      if ((keep >> r) & 1u) {
+        if (fast) {
+          const uint32_t k2 = (code[r] + 120) * 0x00800080u;
+          const uint2 a = e4m3x4_to_bf16_mul(raw[r].x, k2), b = e4m3x4_to_bf16_mul(raw[r].y, k2);
+          const uint2 d = e4m3x4_to_bf16_mul(raw[r].z, k2), e = e4m3x4_to_bf16_mul(raw[r].w, k2);
+          x = make_uint4(a.x, a.y, b.x, b.y);
+          y = make_uint4(d.x, d.y, e.x, e.y);
         } else {
-          const float f = e8m0_decode(sc[k]);
-          a = e4m3x4_to_bf16(raw[k].x, f);
-          b = e4m3x4_to_bf16(raw[k].y, f);
-          d = e4m3x4_to_bf16(raw[k].z, f);
-          e = e4m3x4_to_bf16(raw[k].w, f);
-          const uint32_t v[8] = {a.x, a.y, b.x, b.y, d.x, d.y, e.x, e.y};
-          broken = nan != 0;
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            broken = broken || (v[i] & 0x7F80u) == 0x7F80u || (v[i] & 0x7F800000u) == 0x7F800000u;
+          const float f = e8m0_decode(code[r]);
+          const uint2 a = e4m3x4_to_bf16(raw[r].x, f), b = e4m3x4_to_bf16(raw[r].y, f);
+          const uint2 d = e4m3x4_to_bf16(raw[r].z, f), e = e4m3x4_to_bf16(raw[r].w, f);
+          x = make_uint4(a.x, a.y, b.x, b.y);
+          y = make_uint4(d.x, d.y, e.x, e.y);
         }
-        lo16[k] = make_uint4(a.x, a.y, b.x, b.y);
-        hi16[k] = make_uint4(d.x, d.y, e.x, e.y);
-      } else {
-        const uint32_t v[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          broken = broken || (v[i] & 0x7F80u) == 0x7F80u || (v[i] & 0x7F800000u) == 0x7F800000u;
-        lo16[k] = raw[k];
-        hi16[k] = make_uint4(0, 0, 0, 0);
+        if (!is_code) x = raw[r];
       }
-      if (broken) row_broken[r0 + 8 * k] = 1;
-      if (piece == 0) row_there[r0 + 8 * k] = there[k];
+      if (is_code) st_global_32(dst + r * (2 * kD), x, y);
+      else *reinterpret_cast<uint4*>(dst + r * (2 * kD)) = x;
     }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int r = r0 + 8 * k;
-      // a broken row takes part in no sum: zero times it would not be zero
-      if (row_broken[r]) lo16[k] = hi16[k] = make_uint4(0, 0, 0, 0);
-      uint4* dst = reinterpret_cast<uint4*>(c.w.stage + (u * kUnit + r) * kD);
-      if (piece < 28) {
-        dst[2 * piece] = lo16[k];
-        dst[2 * piece + 1] = hi16[k];
-      } else {
-        dst[56 + piece - 28] = lo16[k];
-      }
+    // row lane / 4, second halves of its RoPE quarters
+    *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(c.w.stage + (u * kUnit + (lane >> 2)) * kD) +
+                              2 * kNope + 32 * (lane & 3) + 16) =
+        (keep >> (lane >> 2)) & 1u ? more : make_uint4(0, 0, 0, 0);
+    if (lane == 0) {
+      c.w.valid[u] = static_cast<uint8_t>(there);
+      c.w.broken[u] = static_cast<uint8_t>(bad);
     }
-    if (tid < 32) {
-      const bool in = tid < kUnit;
-      const unsigned v = __ballot_sync(0xffffffffu, in && row_there[tid & (kUnit - 1)]);
-      const unsigned b = __ballot_sync(
-          0xffffffffu, in && row_there[tid & (kUnit - 1)] && row_broken[tid & (kUnit - 1)]);
-      if (tid == 0) {
-        c.w.valid[u] = static_cast<uint16_t>(v);
-        c.w.broken[u] = static_cast<uint16_t>(b);
-      }
-    }
-    __syncthreads();  // row_broken is cleared for the next unit
   }
   // the attention kernel reads the rows through the async proxy
   asm volatile("fence.proxy.async.global;" ::: "memory");
@@ -813,7 +820,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
 
   if (warp < kSoftmaxWarps) {
     // ----------------------------------------------------- softmax, epilogue
-    if (half == 0 && threadIdx.x == 0 && walk.F < walk.end) c.w.pair_tile[pair] = walk.t;
+    if (half == 0 && threadIdx.x == 0 && walk.F < walk.end) c.w.first_tile[pair] = c.w.tiles[walk.t];
     const int side = warp >> 2, w4 = warp & 3;
     const int row = w4 * 32 + lane;
     const int tok = row / p.H, h = row - tok * p.H;
@@ -1259,83 +1266,77 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
                  : "memory");
 }
 
-// Tiles that a share's end cuts: a warp per (cut, row), 16 dims a lane.
+// Tiles that a share's end cuts: a warp per (cut, row, half of the dims), 8
+// dims a lane. Everything it reads is asked for as early as its address is
+// known: the plan and the cut's tile, then maxima, sums and the first parts.
 constexpr int kMergeWarps = 8;
 __global__ void __launch_bounds__(32 * kMergeWarps) paged_attn_merge_kernel(
     const __grid_constant__ TcCall c) {
   pdl_wait();
   pdl_trigger();
   const PagedAttnProblem& p = c.p;
-  const int cut = blockIdx.y + 1;
-  const int row = blockIdx.x * kMergeWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int cut = blockIdx.y + 1, lane = threadIdx.x & 31;
+  const int wid = blockIdx.x * kMergeWarps + (threadIdx.x >> 5), row = wid >> 1, half = wid & 1;
   const PlanHead head = *c.w.head;
+  const Tile t = c.w.first_tile[cut];  // (holds anything where the share is empty)
   const long long F = cut * head.share;
   if (F >= head.total) return;
-  const Tile t = c.w.tiles[c.w.pair_tile[cut]];
   // the first cut inside a tile merges it
   if (t.start >= F || t.start < F - head.share) return;
   const int tok = row / p.H, h = row - tok * p.H;
   if (tok >= t.tokens) return;
   const int n = static_cast<int>((t.start + t.blocks - 1) / head.share) - (cut - 1) + 1;
   auto part = [&](int i) { return static_cast<long long>(cut - 1 + i) * 2 + (i == 0 ? 1 : 0); };
-  // Each lane holds the weights of parts lane, lane + 32, ...; per half of the
-  // dims, whose maxima may differ in the last bit.
-  constexpr int kPer = 3;  // shares: at most 96 pairs
-  float wt[2][kPer], scale[2], lse = 0.f;
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    float m[kPer], d[kPer], M = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int i = lane + 32 * k;
-      const long long at = (part(i) * 2 + half) * kRows + row;
-      m[k] = i < n ? c.w.part_m[at] : -INFINITY;
-      d[k] = i < n ? c.w.part_den[at] : 0.f;
-      M = fmaxf(M, m[k]);
-    }
-    M = warp_max(M);
-    float den = 0.f;
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      wt[half][k] = m[k] == -INFINITY ? 0.f : exp2f(m[k] - M);
-      den += d[k] * wt[half][k];
-      // a part that saw a broken latent and nothing else has no maximum
-      if (d[k] != d[k]) den = NAN;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
-    const Norm norm = finish(M, den, p.sink, h);
-    scale[half] = norm.scale;
-    if (half == 0) lse = norm.lse;
-  }
-  // 16 bytes a lane, so that a warp's loads are whole lines: dims 4 lane +
-  // 128 q, q = 0 .. 3
-  float acc[4][4] = {};
-  constexpr int kBatch = 4;
-  for (int i0 = 0; i0 < n; i0 += kBatch) {
-    float4 v[kBatch][4];
+  // dims 4 lane + 128 q of the half: a warp's loads are whole lines
+  const float* src = c.w.part_o + half * kHalf + 4 * lane;
+  constexpr int kBatch = 8;
+  float4 v[kBatch][2];
+  auto load = [&](int i0) {
 #pragma unroll
     for (int k = 0; k < kBatch; ++k)
       if (i0 + k < n) {
-        const float* src = c.w.part_o + (part(i0 + k) * kRows + row) * kD + 4 * lane;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[k][q] = *reinterpret_cast<const float4*>(src + 128 * q);
+        const float* at = src + (part(i0 + k) * kRows + row) * kD;
+        v[k][0] = __ldcg(reinterpret_cast<const float4*>(at));
+        v[k][1] = __ldcg(reinterpret_cast<const float4*>(at + 128));
       }
+  };
+  load(0);
+  constexpr int kPer = 3;  // a lane's parts: lane, lane + 32, lane + 64 of at most 96
+  float wt[kPer], m[kPer], d[kPer], M = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int i = lane + 32 * k;
+    const long long at = (part(i) * 2 + half) * kRows + row;
+    m[k] = i < n ? __ldcg(c.w.part_m + at) : -INFINITY;
+    d[k] = i < n ? __ldcg(c.w.part_den + at) : 0.f;
+    M = fmaxf(M, m[k]);
+  }
+  M = warp_max(M);
+  float den = 0.f;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    wt[k] = m[k] == -INFINITY ? 0.f : exp2f(m[k] - M);
+    den += d[k] * wt[k];
+    // a part that saw a broken latent and nothing else has no maximum
+    if (d[k] != d[k]) den = NAN;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
+  const Norm norm = finish(M, den, p.sink, h);
+  float acc[2][4] = {};
+  for (int i0 = 0; i0 < n; i0 += kBatch) {
+    if (i0 > 0) load(i0);
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
       const int i = i0 + k, r = i >> 5;
+      const float f = __shfl_sync(0xffffffffu, r == 0 ? wt[0] : r == 1 ? wt[1] : wt[2], i & 31);
+      if (i < n) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const float mine = r == 0 ? wt[half][0] : r == 1 ? wt[half][1] : wt[half][2];
-        const float f = __shfl_sync(0xffffffffu, mine, i & 31);
-        if (i < n) {
-#pragma unroll
-          for (int q = 2 * half; q < 2 * half + 2; ++q) {
-            acc[q][0] = fmaf(v[k][q].x, f, acc[q][0]);
-            acc[q][1] = fmaf(v[k][q].y, f, acc[q][1]);
-            acc[q][2] = fmaf(v[k][q].z, f, acc[q][2]);
-            acc[q][3] = fmaf(v[k][q].w, f, acc[q][3]);
-          }
+        for (int q = 0; q < 2; ++q) {
+          acc[q][0] = fmaf(v[k][q].x, f, acc[q][0]);
+          acc[q][1] = fmaf(v[k][q].y, f, acc[q][1]);
+          acc[q][2] = fmaf(v[k][q].z, f, acc[q][2]);
+          acc[q][3] = fmaf(v[k][q].w, f, acc[q][3]);
         }
       }
     }
@@ -1343,10 +1344,10 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_attn_merge_kernel(
   const long long at = static_cast<long long>(t.row0 + tok);
   const int r0 = kD - p.rope_out;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int d0 = 128 * q + 4 * lane;
+  for (int q = 0; q < 2; ++q) {
+    const int d0 = half * kHalf + 128 * q + 4 * lane;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[q][i] *= scale[q >> 1];
+    for (int i = 0; i < 4; ++i) acc[q][i] *= norm.scale;
     if (p.rope_cos) {
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
@@ -1369,7 +1370,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_attn_merge_kernel(
           make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u),
                       __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u));
   }
-  if (p.lse && lane == 0) p.lse[at * p.H + h] = lse;
+  if (p.lse && half == 0 && lane == 0) p.lse[at * p.H + h] = norm.lse;
 }
 
 // ------------------------------------------------------------------- host --
@@ -1419,9 +1420,9 @@ size_t tc_carve(const TcShape& s, char* base, TcWs* w) {
   const size_t pairs = s.pairs, blocks = static_cast<size_t>(s.block_cap);
   w->head = reinterpret_cast<PlanHead*>(take(sizeof(PlanHead)));
   w->tiles = reinterpret_cast<Tile*>(take(sizeof(Tile) * s.tile_cap));
-  w->pair_tile = reinterpret_cast<int*>(take(sizeof(int) * pairs));
-  w->valid = reinterpret_cast<uint16_t*>(take(8 * blocks));
-  w->broken = reinterpret_cast<uint16_t*>(take(8 * blocks));
+  w->first_tile = reinterpret_cast<Tile*>(take(sizeof(Tile) * pairs));
+  w->valid = reinterpret_cast<uint8_t*>(take(8 * blocks));
+  w->broken = reinterpret_cast<uint8_t*>(take(8 * blocks));
   w->part_m = reinterpret_cast<float*>(take(sizeof(float) * pairs * 4 * kRows));
   w->part_den = reinterpret_cast<float*>(take(sizeof(float) * pairs * 4 * kRows));
   w->part_o = reinterpret_cast<float*>(take(sizeof(float) * pairs * 2 * kRows * kD));
@@ -1444,8 +1445,9 @@ cudaError_t tc_forward(const PagedAttnProblem& p, void* ws, cudaStream_t st) {
                                     kRows / p.H))
     return cudaErrorInvalidValue;
   const size_t smem = sizeof(int) * 2 * (static_cast<size_t>(p.pages.n_seqs) + 1);
-  const long long units = c.s.block_cap * (kKeys / kUnit);
-  const int most = sm_count() * 6;
+  const long long units =
+      (c.s.block_cap * (kKeys / kUnit) + kStageThreads / 32 - 1) / (kStageThreads / 32);
+  const int most = sm_count() * 4;
   cudaError_t e = launch_pdl(stage_kernel, dim3(1 + static_cast<unsigned>(units < most ? units : most)),
                              dim3(kStageThreads), smem, st, c);
   if (e != cudaSuccess) return e;
@@ -1454,7 +1456,7 @@ cudaError_t tc_forward(const PagedAttnProblem& p, void* ws, cudaStream_t st) {
   e = launch_pdl(paged_attn_tc_kernel, dim3(2 * c.s.pairs), dim3(kTcThreads), kTcBytes, st, map, qmap,
                  c);
   if (e != cudaSuccess || c.s.pairs == 1) return e;
-  return launch_pdl(paged_attn_merge_kernel, dim3(kRows / kMergeWarps, c.s.pairs - 1),
+  return launch_pdl(paged_attn_merge_kernel, dim3(2 * kRows / kMergeWarps, c.s.pairs - 1),
                     dim3(32 * kMergeWarps), 0, st, c);
 }
 
