@@ -175,7 +175,10 @@ constexpr int kD = 512, kNope = 448, kRope = 64;
 constexpr int kRows = 128;        // (token, head) rows of a tile: M of both products
 constexpr int kKeys = 64;         // keys of a block: N of Q K^T, K of P V
 constexpr int kHalf = 256;        // output dims of a CTA: N of P V
-constexpr int kMinShare = 2;      // blocks: a smaller share costs more to merge than it saves
+// What a tile costs besides its blocks (Q in, O out), in blocks: shares are
+// cut by the sum, so that many short tiles weigh as much as a long one.
+constexpr int kTileCost = 3;
+constexpr int kMinShare = 2 + kTileCost;  // a smaller share costs more to merge than it saves
 // A tile of at most this many blocks carries its weights in two BF16 terms:
 // where a row sees few keys, the rounding of one weight does not average out
 // (with one term a two-key row is off by up to 2^-8 of its value sum).
@@ -183,7 +186,7 @@ constexpr int kTwoTermBlocks = 4;
 constexpr float kLazyMargin = 8.0f;  // log2 units: the running max moves only past this
 
 struct Tile {
-  long long start;  // blocks of the tiles before
+  long long start;  // units of the tiles before: kTileCost and the blocks of each
   int blocks;       // blocks that its tokens see
   int block0;       // first of them among the decoded blocks
   int key0;         // position of that block's first key
@@ -196,8 +199,8 @@ struct Tile {
 static_assert(sizeof(Tile) == 48, "one warp reads a tile's description in one go");
 
 struct PlanHead {
-  long long total;  // blocks of all tiles
-  long long share;  // blocks per pair of CTAs
+  long long total;  // units of all tiles
+  long long share;  // units per pair of CTAs
   int tiles;
 };
 
@@ -316,7 +319,7 @@ __device__ void list_tiles(const TcCall& c, const int* block_start, const int* t
       }
     }
     int total;
-    tile.start = done + stage_scan(tile.blocks, &total);
+    tile.start = done + stage_scan(t < tiles ? tile.blocks + kTileCost : 0, &total);
     if (t < tiles) c.w.tiles[t] = tile;
     done += total;
   }
@@ -513,7 +516,7 @@ struct Bars {
 };
 static_assert(sizeof(Bars) <= 256, "barriers exceed their room");
 
-// The tile that holds block F (whole warp; F < total): 32 probes a step.
+// The tile that holds unit F (whole warp; F < total): 32 probes a step.
 __device__ __forceinline__ int find_tile(const Tile* tiles, int n, long long F) {
   const int lane = threadIdx.x & 31;
   int lo = 0, hi = n;  // tiles[lo].start <= F
@@ -534,7 +537,8 @@ struct Segment {
   int j0, j1;     // its blocks
 };
 
-// Walks a share's segments: every role runs the same walk.
+// Walks a share's segments: every role runs the same walk. Block j of a tile
+// is its unit kTileCost + j and belongs to the share that has it.
 struct Walk {
   const Tile* tiles;
   long long F, end;
@@ -542,10 +546,15 @@ struct Walk {
   __device__ bool next(Segment& s) {
     if (F >= end) return false;
     s.t = tiles[t++];
-    s.j0 = static_cast<int>(F - s.t.start);
-    const long long left = end - F;
-    s.j1 = s.t.blocks - s.j0 > left ? s.j0 + static_cast<int>(left) : s.t.blocks;
-    F += s.j1 - s.j0;
+    const long long first = s.t.start + kTileCost;
+    s.j0 = F > first ? static_cast<int>(F - first) : 0;
+    const long long to = end - first;
+    if (to <= 0) {  // the share ends before the tile's first block
+      F = end;
+      return false;
+    }
+    s.j1 = to < s.t.blocks ? static_cast<int>(to) : s.t.blocks;
+    F = first + s.j1;
     return true;
   }
 };
@@ -697,16 +706,20 @@ struct PairSync {
   }
 };
 
-// 32 scores of a row (this thread's half of the block's keys) to weights.
-// kPlain: every key is visible and one BF16 term is enough.
+// 32 scores of a row (this thread's half of the block's keys) to weights in
+// shared memory. kPlain: every key is visible and one BF16 term is enough;
+// then P V of the block before is waited for as late as possible, when the
+// weights are there. `rescale`: O (and what was summed before) is to be
+// multiplied by alpha.
 struct RowState {
   float m, den;
 };
-template <bool kPlain>
+template <bool kPlain, class WaitPv>
 __device__ __forceinline__ bool softmax_block(uint32_t s_col, uint32_t mask, bool two_terms,
                                               float sc2, float* max_mine, const float* max_other,
-                                              PairSync& meet, bool& ok, RowState& st, float& alpha,
-                                              uint32_t (&hi)[16], uint32_t (&lo)[16]) {
+                                              PairSync& meet, bool& good, RowState& st,
+                                              float& alpha, uint32_t prow, int chunk0, int row,
+                                              WaitPv wait_pv) {
   uint32_t r[32];
   tmem_ld32(s_col, r);
   float tm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -717,7 +730,7 @@ __device__ __forceinline__ bool softmax_block(uint32_t s_col, uint32_t mask, boo
   }
   const float mine = fmaxf(fmaxf(tm[0], tm[1]), fmaxf(tm[2], tm[3]));
   *max_mine = mine;
-  ok = meet() && ok;
+  good = meet() && good;
   const float tmax = fmaxf(mine, *max_other) * sc2;  // scale > 0
   // the running max moves only when a score exceeds it by the margin:
   // weights stay <= 2^8 and O is rarely rescaled
@@ -734,15 +747,42 @@ __device__ __forceinline__ bool softmax_block(uint32_t s_col, uint32_t mask, boo
   }
   const float neg = st.m == -INFINITY ? 0.f : -st.m;
   float part[4] = {0.f, 0.f, 0.f, 0.f};
+  if (kPlain) {
 #pragma unroll
-  for (int i = 0; i < 32; i += 2) {
-    const float e0 = ex2_approx(fmaf(__uint_as_float(r[i]), sc2, neg));
-    const float e1 = ex2_approx(fmaf(__uint_as_float(r[i + 1]), sc2, neg));
-    part[(i >> 1) & 3] += e0 + e1;
-    hi[i / 2] = pack_bf16x2(e0, e1);
-    if (!kPlain && two_terms)
-      lo[i / 2] = pack_bf16x2(e0 - __uint_as_float(hi[i / 2] << 16),
-                              e1 - __uint_as_float(hi[i / 2] & 0xFFFF0000u));
+    for (int i = 0; i < 32; i += 2) {
+      const float e0 = ex2_approx(fmaf(__uint_as_float(r[i]), sc2, neg));
+      const float e1 = ex2_approx(fmaf(__uint_as_float(r[i + 1]), sc2, neg));
+      part[(i >> 1) & 3] += e0 + e1;
+      r[i / 2] = pack_bf16x2(e0, e1);
+    }
+    good = wait_pv() && good;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      st_shared_v4(prow + (((chunk0 + k) ^ (row & 7)) << 4),
+                   make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]));
+  } else {
+    good = wait_pv() && good;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float e[8];
+      uint32_t h[4];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = ex2_approx(fmaf(__uint_as_float(r[8 * k + i]), sc2, neg));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        part[i] += e[2 * i] + e[2 * i + 1];
+        h[i] = pack_bf16x2(e[2 * i], e[2 * i + 1]);
+      }
+      const uint32_t at = prow + (((chunk0 + k) ^ (row & 7)) << 4);
+      st_shared_v4(at, make_uint4(h[0], h[1], h[2], h[3]));
+      if (two_terms) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          h[i] = pack_bf16x2(e[2 * i] - __uint_as_float(h[i] << 16),
+                             e[2 * i + 1] - __uint_as_float(h[i] & 0xFFFF0000u));
+        st_shared_v4(at + kPBytes, make_uint4(h[0], h[1], h[2], h[3]));
+      }
+    }
   }
   st.den = st.den * alpha + ((part[0] + part[1]) + (part[2] + part[3]));
   return rescale;
@@ -878,15 +918,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
         tc_fence_after();
         const uint32_t s_col = tmem + lanes + kColS + sb * kKeys + side * 32;
         const int buf = sb * 2 * kRows;
-        uint32_t hi[16], lo[16];
         float alpha;
+        // P V of the block before has read P, and O holds all blocks before
+        auto wait_pv = [&] {
+          return n == 0 || long_wait(&bars->pv_done, (n - 1) & 1, abort_flag, err);
+        };
         const bool rescale =
             plain ? softmax_block<true>(s_col, mask32, false, sc2, max_mine + buf, max_other + buf,
-                                        meet, good, st, alpha, hi, lo)
+                                        meet, good, st, alpha, prow, 4 * side, row, wait_pv)
                   : softmax_block<false>(s_col, mask32, two_terms, sc2, max_mine + buf,
-                                         max_other + buf, meet, good, st, alpha, hi, lo);
-        // P V of the block before has read P, and O holds all blocks before
-        if (n > 0) good = long_wait(&bars->pv_done, (n - 1) & 1, abort_flag, err) && good;
+                                         max_other + buf, meet, good, st, alpha, prow, 4 * side,
+                                         row, wait_pv);
         if (!__all_sync(0xffffffffu, good)) {
           ok = false;
           break;
@@ -902,16 +944,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
             tmem_st32(o_cols + cb, o);
           }
           tmem_st_wait();
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          st_shared_v4(prow + (((4 * side + k) ^ (row & 7)) << 4),
-                       make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]));
-        if (two_terms) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            st_shared_v4(prow + kPBytes + (((4 * side + k) ^ (row & 7)) << 4),
-                         make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]));
         }
         fence_async_smem();
         tc_fence_before();
@@ -941,45 +973,53 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
         const int r0 = kD - p.rope_out;
         const int d_side = half * kHalf + side * (kHalf / 2);
         const bool rope = p.rope_cos && d_side + kHalf / 2 > r0;
+        // rows of 64 dims to this warp's room, then whole lines to memory
+        long long to[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          to[i] = __shfl_sync(0xffffffffu, o_at, i * 4 + (lane >> 3));
 #pragma unroll 1
-        for (int cb = 0; cb < kHalf / 2; cb += 32) {
-          uint32_t o[32];
-          tmem_ld32(o_cols + cb, o);
-          float v[32];
+        for (int cb = 0; cb < kHalf / 2; cb += 64) {
+          uint32_t o[2][32];
+          tmem_ld32(o_cols + cb, o[0]);
+          tmem_ld32(o_cols + cb + 32, o[1]);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]) * norm.scale;
-          const int d0 = d_side + cb;
-          if (rope && mine && d0 + 32 > r0) rope_dims(p, at, d0, r0, v);
-          if (p.bf16) {
-            // rows of 64 dims in this warp's room, then whole lines to memory
+          for (int q = 0; q < 2; ++q) {
+            const int d0 = d_side + cb + 32 * q;
+            float v[32];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              st_shared_v4(room + lane * 128 + ((((cb & 32) / 8 + k) ^ (lane & 7)) << 4),
-                           make_uint4(pack_bf16x2(v[8 * k], v[8 * k + 1]),
-                                      pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
-                                      pack_bf16x2(v[8 * k + 4], v[8 * k + 5]),
-                                      pack_bf16x2(v[8 * k + 6], v[8 * k + 7])));
-            if (cb & 32) {
-              __syncwarp();
+            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[q][i]) * norm.scale;
+            if (rope && mine && d0 + 32 > r0) rope_dims(p, at, d0, r0, v);
+            if (p.bf16) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int r = i * 4 + (lane >> 3), ch = lane & 7;
-                const long long to = __shfl_sync(0xffffffffu, o_at, r);
-                const uint4 w = ld_shared_v4(room + r * 128 + ((ch ^ (r & 7)) << 4));
-                if (to >= 0)
-                  *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + to + d_side +
-                                            (cb & 64) + 8 * ch) = w;
-              }
-              __syncwarp();
+              for (int k = 0; k < 4; ++k)
+                st_shared_v4(room + lane * 128 + (((4 * q + k) ^ (lane & 7)) << 4),
+                             make_uint4(pack_bf16x2(v[8 * k], v[8 * k + 1]),
+                                        pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
+                                        pack_bf16x2(v[8 * k + 4], v[8 * k + 5]),
+                                        pack_bf16x2(v[8 * k + 6], v[8 * k + 7])));
+            } else if (mine) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 8) store_o8(p, o_at + d0 + i, v + i);
             }
-          } else if (mine) {
+          }
+          if (p.bf16) {
+            __syncwarp();
+            const int ch = lane & 7;
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) store_o8(p, o_at + d0 + i, v + i);
+            for (int i = 0; i < 8; ++i) {
+              const int r = i * 4 + (lane >> 3);
+              const uint4 w = ld_shared_v4(room + r * 128 + ((ch ^ (r & 7)) << 4));
+              if (to[i] >= 0)
+                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + to[i] + d_side + cb +
+                                          8 * ch) = w;
+            }
+            __syncwarp();
           }
         }
       } else {
         // a part: slot 0 where the tile began in an earlier share, else 1
-        const int slot = t.start < share0 ? 0 : 1;
+        const int slot = t.start + kTileCost < share0 ? 0 : 1;
         const long long at = pair * 2 + slot;
         float* part = c.w.part_o + (at * kRows + w4 * 32) * kD + half * kHalf + side * (kHalf / 2);
         const unsigned rows = __ballot_sync(0xffffffffu, mine);
@@ -1282,10 +1322,11 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_attn_merge_kernel(
   const long long F = cut * head.share;
   if (F >= head.total) return;
   // the first cut inside a tile merges it
-  if (t.start >= F || t.start < F - head.share) return;
+  const long long first = t.start + kTileCost;  // its first block's unit
+  if (first >= F || first < F - head.share) return;
   const int tok = row / p.H, h = row - tok * p.H;
   if (tok >= t.tokens) return;
-  const int n = static_cast<int>((t.start + t.blocks - 1) / head.share) - (cut - 1) + 1;
+  const int n = static_cast<int>((first + t.blocks - 1) / head.share) - (cut - 1) + 1;
   auto part = [&](int i) { return static_cast<long long>(cut - 1 + i) * 2 + (i == 0 ? 1 : 0); };
   // dims 4 lane + 128 q of the half: a warp's loads are whole lines
   const float* src = c.w.part_o + half * kHalf + 4 * lane;
@@ -1401,7 +1442,7 @@ TcShape tc_shape(const PagedAttnProblem& p) {
   long long keys = active * one;
   if (p.max_keys > 0 && p.max_keys < keys) keys = p.max_keys;
   s.block_cap = keys / kKeys + active;  // each slot rounds up to a whole block
-  const long long per_tile = one / kKeys + 2;
+  const long long per_tile = one / kKeys + 2 + kTileCost;
   const long long most = (s.tile_cap * per_tile + kMinShare - 1) / kMinShare;
   const int pairs = sm_count() / 2 < 96 ? sm_count() / 2 : 96;
   s.pairs = static_cast<int>(most < pairs ? (most < 1 ? 1 : most) : pairs);
