@@ -177,8 +177,8 @@ constexpr int kKeys = 64;         // keys of a block: N of Q K^T, K of P V
 constexpr int kHalf = 256;        // output dims of a CTA: N of P V
 // What a tile costs besides its blocks (Q in, O out), in blocks: shares are
 // cut by the sum, so that many short tiles weigh as much as a long one.
-constexpr int kTileCost = 3;
-constexpr int kMinShare = 2 + kTileCost;  // a smaller share costs more to merge than it saves
+constexpr int kTileCost = 4;
+constexpr int kMinShare = 2;  // a smaller share costs more to merge than it saves
 // A tile of at most this many blocks carries its weights in two BF16 terms:
 // where a row sees few keys, the rounding of one weight does not average out
 // (with one term a two-key row is off by up to 2^-8 of its value sum).
@@ -499,7 +499,8 @@ constexpr uint32_t kSmP = kSmOther + kOtherStages * 2 * kBlk;
 constexpr uint32_t kPBytes = kRows * kKeys * 2;            // P, and what its rounding left
 constexpr uint32_t kSmBar = kSmP + 2 * kPBytes;
 constexpr uint32_t kSmMax = kSmBar + 256;    // [2 blocks][2 key halves][128] row maxima
-constexpr uint32_t kTcBytes = kSmMax + 2 * 2 * kRows * 4;
+constexpr uint32_t kSmScale = kSmMax + 2 * 2 * kRows * 4;  // [128] what O is multiplied by
+constexpr uint32_t kTcBytes = kSmScale + kRows * 4;
 static_assert(kTcBytes <= 232448, "beyond the shared memory of a CTA");
 constexpr uint32_t kColS = 256, kColQ = 384, kCols = 512;  // O: 0-255, S: two of 64, Q dims 0-255
 
@@ -510,7 +511,7 @@ constexpr int kTcThreads = 32 * (kWarpMma + 1);
 struct Bars {
   uint64_t full_own[kOwnStages], empty_own[kOwnStages];
   uint64_t full_other[kOtherStages], empty_other[kOtherStages];
-  uint64_t s_full[2], p_full, pv_done, q_full, q_free, fin, pair[4];
+  uint64_t s_full[2], p_full, pv_done, q_full, q_free, o_ready, o_free, fin, pair[4];
   uint32_t tmem;
   int abort_flag;
 };
@@ -568,38 +569,60 @@ __device__ __forceinline__ uint4 load_q8(const PagedAttnProblem& p, long long at
                     pack_bf16x2(b.z, b.w));
 }
 
-// 8 output dims of a row.
-__device__ __forceinline__ void store_o8(const PagedAttnProblem& p, long long at, const float* v) {
-  const uint4 w = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
-                             pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+__device__ __forceinline__ int part_slot(const Tile& t, long long share0) {
+  return t.start + kTileCost < share0 ? 0 : 1;  // 0: the tile began in an earlier share
+}
+
+// 16 output dims of a row (16-byte aligned; whole sectors where 32 fit).
+__device__ __forceinline__ void store_o16(const PagedAttnProblem& p, long long at, const float* v) {
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
   if (p.bf16) {
-    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + at) = w;
+    __nv_bfloat16* d = static_cast<__nv_bfloat16*>(p.out) + at;
+    const uint4 a = make_uint4(w[0], w[1], w[2], w[3]), b = make_uint4(w[4], w[5], w[6], w[7]);
+    if (p.out_32) {
+      st_global_32(d, a, b);
+    } else {
+      reinterpret_cast<uint4*>(d)[0] = a;
+      reinterpret_cast<uint4*>(d)[1] = b;
+    }
   } else {
     float4* d = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      d[i] = make_float4(__uint_as_float(u[2 * i] << 16), __uint_as_float(u[2 * i] & 0xFFFF0000u),
-                         __uint_as_float(u[2 * i + 1] << 16),
-                         __uint_as_float(u[2 * i + 1] & 0xFFFF0000u));
+    for (int i = 0; i < 4; ++i)
+      d[i] = make_float4(__uint_as_float(w[2 * i] << 16), __uint_as_float(w[2 * i] & 0xFFFF0000u),
+                         __uint_as_float(w[2 * i + 1] << 16),
+                         __uint_as_float(w[2 * i + 1] & 0xFFFF0000u));
   }
 }
 
 // Inverse RoPE of 32 dims from d0 on, the pairs from r0 on; the row's factors
-// are loaded together.
+// are loaded together, in whole vectors where they are whole.
 __device__ __forceinline__ void rope_dims(const PagedAttnProblem& p, long long row, int d0, int r0,
                                           float (&v)[32]) {
   const long long ra = row * (p.rope_out / 2);
   float cs[16], sn[16];
+  if (p.rope_vec) {  // all 32 dims, 16-byte aligned
+    const float4* c4 = reinterpret_cast<const float4*>(p.rope_cos + ra + (d0 - r0) / 2);
+    const float4* s4 = reinterpret_cast<const float4*>(p.rope_sin + ra + (d0 - r0) / 2);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const bool in = d0 + 2 * i >= r0;
-    const long long at = ra + (in ? (d0 + 2 * i - r0) / 2 : 0);
-    cs[i] = __ldg(p.rope_cos + at);
-    sn[i] = __ldg(p.rope_sin + at);
-    if (!in) {
-      cs[i] = 1.f;
-      sn[i] = 0.f;
+    for (int i = 0; i < 4; ++i) {
+      const float4 a = __ldg(c4 + i), b = __ldg(s4 + i);
+      cs[4 * i] = a.x, cs[4 * i + 1] = a.y, cs[4 * i + 2] = a.z, cs[4 * i + 3] = a.w;
+      sn[4 * i] = b.x, sn[4 * i + 1] = b.y, sn[4 * i + 2] = b.z, sn[4 * i + 3] = b.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const bool in = d0 + 2 * i >= r0;
+      const long long at = ra + (in ? (d0 + 2 * i - r0) / 2 : 0);
+      cs[i] = __ldg(p.rope_cos + at);
+      sn[i] = __ldg(p.rope_sin + at);
+      if (!in) {
+        cs[i] = 1.f;
+        sn[i] = 0.f;
+      }
     }
   }
 #pragma unroll
@@ -611,13 +634,12 @@ __device__ __forceinline__ void rope_dims(const PagedAttnProblem& p, long long r
 }
 
 // Denominator with the sink and what the sums are divided by, from the
-// running max m and sum den of the scores in log2 units.
+// running max m, the sum den of the scores and the sink s2, in log2 units.
 struct Norm {
   float scale;  // of the value sums
   float lse;
 };
-__device__ __forceinline__ Norm finish(float m, float den, const float* sink, int h) {
-  const float s2 = sink ? sink[h] * kLog2e : -INFINITY;
+__device__ __forceinline__ Norm finish(float m, float den, float s2) {
   const float mx = fmaxf(m, s2);
   if (den != den) return {NAN, NAN};
   if (mx == -INFINITY) return {0.f, -INFINITY};  // nothing seen, no sink
@@ -789,10 +811,10 @@ __device__ __forceinline__ bool softmax_block(uint32_t s_col, uint32_t mask, boo
 }
 
 // One share of (tile, block) pairs and one half of the output dims. Roles:
-//   warps 0-7  softmax and epilogue: row = TMEM lane, two threads a row, one
-//              for each half of a block's keys (and of the CTA's output dims)
+//   warps 0-7  softmax: row = TMEM lane, two threads a row, one for each half of
+//              a block's keys
 //   warps 8-11 dims 0-255 of the next segment's Q to TMEM, once this one's last
-//              Q K^T is done
+//              Q K^T is done, then this one's O out, while the others go on
 //   warp 12    key blocks and Q by TMA (one lane)
 //   warp 13    TMEM allocation and MMA issue
 // Per block: S = Q K^T (32 MMAs of 128 x 64 x 16, the other half's dims first
@@ -827,6 +849,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
     mbar_init(&bars->pv_done, 1);
     mbar_init(&bars->q_full, 32 * kLoadWarps + 1);  // and the TMA warp's
     mbar_init(&bars->q_free, 1);
+    mbar_init(&bars->o_ready, 32 * kSoftmaxWarps);
+    mbar_init(&bars->o_free, 32 * kLoadWarps);
     mbar_init(&bars->fin, 1);
     for (int i = 0; i < 4; ++i) mbar_init(&bars->pair[i], 64);
     bars->abort_flag = 0;
@@ -867,14 +891,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
     const uint32_t lanes = static_cast<uint32_t>(w4 * 32) << 16;
     const uint32_t o_cols = tmem + lanes + side * (kHalf / 2);
     const uint32_t prow = base + kSmP + (row >> 3) * 1024 + (row & 7) * 128;
-    const uint32_t room = base + kSmP + warp * 4096;  // free once P V is done
     float* maxima = reinterpret_cast<float*>(smem + kSmMax);
     float* max_mine = maxima + side * kRows + row;
     const float* max_other = maxima + (1 - side) * kRows + row;
     const float sc2 = p.scale * kLog2e;
+    const float sink2 = p.sink && h < p.H && tok < kRows / p.H ? p.sink[h] * kLog2e : -INFINITY;
     const long long share0 = walk.F;
     PairSync meet = {&bars->pair[w4], 0, abort_flag, err};
-    unsigned n = 0;  // blocks done by this CTA
+    unsigned n = 0, segs = 0;  // blocks and segments done by this CTA
     bool ok = true;
     while (ok && walk.next(seg)) {
       const Tile& t = seg.t;
@@ -957,102 +981,36 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
       bool good = meet();
       float den = st.den + max_other[buf];
       good = meet() && good;  // read before the next segment writes it
-      good = long_wait(&bars->pv_done, (n - 1) & 1, abort_flag, err) && good;
+      // the segment before is out, so its factors may be overwritten
+      if (segs > 0) good = long_wait(&bars->o_free, (segs - 1) & 1, abort_flag, err) && good;
+      ++segs;
       if (!__all_sync(0xffffffffu, good)) {
         ok = false;
         break;
       }
-      tc_fence_after();
       if (bad) den = NAN;
-      const bool done = seg.j0 == 0 && seg.j1 == t.blocks;
-      if (done) {
-        const Norm norm = finish(st.m, den, p.sink, h < p.H && mine ? h : 0);
-        const long long at = static_cast<long long>(t.row0 + tok);
-        const long long o_at = mine ? at * p.out_stride + static_cast<long long>(h) * kD : -1ll;
-        if (mine && half == 0 && side == 0 && p.lse) p.lse[at * p.H + h] = norm.lse;
-        const int r0 = kD - p.rope_out;
-        const int d_side = half * kHalf + side * (kHalf / 2);
-        const bool rope = p.rope_cos && d_side + kHalf / 2 > r0;
-        // rows of 64 dims to this warp's room, then whole lines to memory
-        long long to[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          to[i] = __shfl_sync(0xffffffffu, o_at, i * 4 + (lane >> 3));
-#pragma unroll 1
-        for (int cb = 0; cb < kHalf / 2; cb += 64) {
-          uint32_t o[2][32];
-          tmem_ld32(o_cols + cb, o[0]);
-          tmem_ld32(o_cols + cb + 32, o[1]);
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const int d0 = d_side + cb + 32 * q;
-            float v[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[q][i]) * norm.scale;
-            if (rope && mine && d0 + 32 > r0) rope_dims(p, at, d0, r0, v);
-            if (p.bf16) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                st_shared_v4(room + lane * 128 + (((4 * q + k) ^ (lane & 7)) << 4),
-                             make_uint4(pack_bf16x2(v[8 * k], v[8 * k + 1]),
-                                        pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
-                                        pack_bf16x2(v[8 * k + 4], v[8 * k + 5]),
-                                        pack_bf16x2(v[8 * k + 6], v[8 * k + 7])));
-            } else if (mine) {
-#pragma unroll
-              for (int i = 0; i < 32; i += 8) store_o8(p, o_at + d0 + i, v + i);
-            }
-          }
-          if (p.bf16) {
-            __syncwarp();
-            const int ch = lane & 7;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = i * 4 + (lane >> 3);
-              const uint4 w = ld_shared_v4(room + r * 128 + ((ch ^ (r & 7)) << 4));
-              if (to[i] >= 0)
-                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + to[i] + d_side + cb +
-                                          8 * ch) = w;
-            }
-            __syncwarp();
-          }
+      if (seg.j0 == 0 && seg.j1 == t.blocks) {
+        const Norm norm = finish(st.m, den, sink2);
+        if (side == 0) {
+          reinterpret_cast<float*>(smem + kSmScale)[row] = norm.scale;
+          if (mine && half == 0 && p.lse)
+            p.lse[static_cast<long long>(t.row0 + tok) * p.H + h] = norm.lse;
         }
-      } else {
-        // a part: slot 0 where the tile began in an earlier share, else 1
-        const int slot = t.start + kTileCost < share0 ? 0 : 1;
-        const long long at = pair * 2 + slot;
-        float* part = c.w.part_o + (at * kRows + w4 * 32) * kD + half * kHalf + side * (kHalf / 2);
-        const unsigned rows = __ballot_sync(0xffffffffu, mine);
-#pragma unroll 1
-        for (int cb = 0; cb < kHalf / 2; cb += 32) {
-          uint32_t o[32];
-          tmem_ld32(o_cols + cb, o);
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            st_shared_v4(room + lane * 128 + ((k ^ (lane & 7)) << 4),
-                         make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]));
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = i * 4 + (lane >> 3), ch = lane & 7;
-            const uint4 w = ld_shared_v4(room + r * 128 + ((ch ^ (r & 7)) << 4));
-            if ((rows >> r) & 1u)
-              *reinterpret_cast<uint4*>(part + r * kD + cb + 4 * ch) = w;
-          }
-          __syncwarp();
-        }
-        if (mine && side == 0) {
-          c.w.part_m[(at * 2 + half) * kRows + row] = st.m;
-          c.w.part_den[(at * 2 + half) * kRows + row] = den;
-        }
+      } else if (mine && side == 0) {
+        const long long at = pair * 2 + part_slot(t, share0);
+        c.w.part_m[(at * 2 + half) * kRows + row] = st.m;
+        c.w.part_den[(at * 2 + half) * kRows + row] = den;
       }
-      tc_fence_before();  // O may be overwritten once the next block's P is there
+      mbar_arrive(&bars->o_ready);
     }
   } else if (warp < kWarpTma) {
-    // ------------------------------------------------------------- Q loaders
+    // ------------------------------------------------------- Q in, O out
     const int w4 = warp & 3, row = w4 * 32 + lane;
+    const int tok = row / p.H, h = row - tok * p.H;
     const uint32_t lanes = static_cast<uint32_t>(w4 * 32) << 16;
-    unsigned it = 0, slot = 0, phase = 0;  // of the own ring
+    const long long share0 = walk.F;
+    unsigned it = 0, slot = 0, phase = 0;  // slot and phase of the own ring
+    unsigned n = 0;                        // blocks of the segments before
     auto to_tmem = [&](const uint4 (&a)[16], int k) {  // dims 128 k ..
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
@@ -1067,8 +1025,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
         tmem_st32(tmem + lanes + kColQ + 64 * k + 32 * q, r);
       }
     };
-    while (walk.next(seg)) {
-      const Tile& t = seg.t;
+    auto load_q = [&](const Segment& sg) {
+      const Tile& t = sg.t;
       bool good = true;
       uint4 a[16];
       // (also before the own ring is looked at: only now is the slot's phase
@@ -1090,12 +1048,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
           to_tmem(a, k);
           if (++slot == kOwnStages) { slot = 0; phase ^= 1; }
         }
-        slot += static_cast<unsigned>(seg.j1 - seg.j0);
+        slot += static_cast<unsigned>(sg.j1 - sg.j0);
         phase ^= (slot / kOwnStages) & 1;
         slot %= kOwnStages;
       } else {
         // fp32 rows are converted on their way
-        const int tok = row / p.H, h = row - tok * p.H;
         const long long at = tok < t.tokens ? static_cast<long long>(t.row0 + tok) * p.q_stride +
                                                   static_cast<long long>(h) * kD
                                             : -1ll;
@@ -1122,9 +1079,69 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&bars->q_full);
+      return __all_sync(0xffffffffu, good);
+    };
+    // O of segment number i, whose last block is block number nb
+    auto store_o = [&](const Segment& sg, unsigned i, unsigned nb) {
+      const Tile& t = sg.t;
+      const bool mine = tok < t.tokens;
+      bool good = long_wait(&bars->o_ready, i & 1, abort_flag, err);
+      good = long_wait(&bars->pv_done, nb & 1, abort_flag, err) && good;
+      if (!__all_sync(0xffffffffu, good)) return false;
+      tc_fence_after();
+      if (sg.j0 == 0 && sg.j1 == t.blocks) {
+        const float scale = reinterpret_cast<const volatile float*>(smem + kSmScale)[row];
+        const long long at = static_cast<long long>(t.row0 + tok);
+        const long long o_at = at * p.out_stride + static_cast<long long>(h) * kD + half * kHalf;
+        const int r0 = kD - p.rope_out;
+#pragma unroll 1
+        for (int cb = 0; cb < kHalf; cb += 32) {
+          uint32_t o[32];
+          tmem_ld32(tmem + lanes + cb, o);
+          float v[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(o[k]) * scale;
+          const int d0 = half * kHalf + cb;
+          if (mine) {
+            if (p.rope_cos && d0 + 32 > r0) rope_dims(p, at, d0, r0, v);
+#pragma unroll
+            for (int k = 0; k < 32; k += 16) store_o16(p, o_at + cb + k, v + k);
+          }
+        }
+      } else {
+        float* part = c.w.part_o +
+                      ((pair * 2 + part_slot(t, share0)) * static_cast<long long>(kRows) + row) * kD +
+                      half * kHalf;
+#pragma unroll 1
+        for (int cb = 0; cb < kHalf; cb += 32) {
+          uint32_t o[32];
+          tmem_ld32(tmem + lanes + cb, o);
+          if (mine) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 8)
+              st_global_32(part + cb + k, make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]),
+                           make_uint4(o[k + 4], o[k + 5], o[k + 6], o[k + 7]));
+          }
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(&bars->o_free);  // the next segment's P V may overwrite it
+      return true;
+    };
+    // The next segment's Q goes in as soon as this one's last Q K^T is done,
+    // before this one's O comes out.
+    Segment before;
+    bool ok = true;
+    while (ok && walk.next(seg)) {
+      ok = load_q(seg);
+      if (ok && it > 0) {
+        n += before.j1 - before.j0;
+        ok = store_o(before, it - 1, n - 1);
+      }
+      before = seg;
       ++it;
-      if (!__all_sync(0xffffffffu, good)) break;
     }
+    if (ok && it > 0) store_o(before, it - 1, n + (before.j1 - before.j0) - 1);
   } else if (warp == kWarpTma) {
     // ------------------------------------------------------------ key blocks
     if (lane == 0) {
@@ -1238,7 +1255,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
       // O += P V of block number nb of this CTA
       auto pv = [&](bool ready, unsigned nb, bool first, bool two_terms) {
         if (!waits(ready, &bars->p_full, nb)) return false;
-        tc_fence_after();  // the softmax's reads of S and writes of O
+        if (first && it > 1 && !waits(false, &bars->o_free, it - 2)) return false;
+        tc_fence_after();  // the softmax's reads of S and writes of O, the reads of O
         const uint64_t v = v_desc + sv * (4 * kBlk / 16);
 #pragma unroll
         for (int kk = 0; kk < kKeys / 16; ++kk)
@@ -1363,7 +1381,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_attn_merge_kernel(
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
-  const Norm norm = finish(M, den, p.sink, h);
+  const Norm norm = finish(M, den, p.sink ? p.sink[h] * kLog2e : -INFINITY);
   float acc[2][4] = {};
   for (int i0 = 0; i0 < n; i0 += kBatch) {
     if (i0 > 0) load(i0);
@@ -1474,6 +1492,10 @@ size_t tc_carve(const TcShape& s, char* base, TcWs* w) {
 cudaError_t tc_forward(const PagedAttnProblem& p, void* ws, cudaStream_t st) {
   TcCall c;
   c.p = p;
+  auto aligned = [](const void* q, uintptr_t n) { return reinterpret_cast<uintptr_t>(q) % n == 0; };
+  c.p.out_32 = aligned(p.out, 32) && p.out_stride % 16 == 0;
+  c.p.rope_vec = p.rope_cos && p.rope_out % 32 == 0 && aligned(p.rope_cos, 16) &&
+                 aligned(p.rope_sin, 16);
   c.s = tc_shape(p);
   tc_carve(c.s, static_cast<char*>(ws), &c.w);
   if (c.s.block_cap * kKeys > 0x7FFFFFFFll) return cudaErrorInvalidValue;

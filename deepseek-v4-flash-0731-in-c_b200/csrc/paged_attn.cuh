@@ -39,6 +39,8 @@ struct PagedAttnProblem {
   long long max_keys = 0;           // bound of the positions seen, all slots together
   float scale = 0.f;
   unsigned* err = nullptr;          // device error word
+  bool out_32 = false;              // rows of out (BF16) are 32-byte aligned
+  bool rope_vec = false;            // RoPE factors of 32 dims are whole, aligned vectors
 };
 
 size_t paged_attn_workspace_bytes(const PagedAttnProblem& p);
