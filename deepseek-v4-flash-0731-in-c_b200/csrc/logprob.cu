@@ -140,34 +140,6 @@ __device__ void compact(Shared& sh, int k) {
   __syncthreads();
 }
 
-// Two fp32 values in one register pair (the packed arithmetic rounds each as
-// the scalar one does).
-using F2 = unsigned long long;
-__device__ __forceinline__ F2 pack2(float a, float b) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float lo2(F2 v) {
-  float a, b;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-  return a;
-}
-__device__ __forceinline__ float hi2(F2 v) {
-  float a, b;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-  return b;
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 // 1 where a > b (a >= b), else 0: counts of up to 2^24 in a register
 __device__ __forceinline__ float gt1(float a, float b) {
   float r;
@@ -179,17 +151,17 @@ __device__ __forceinline__ float ge1(float a, float b) {
   asm("set.ge.f32.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
 // Running sums in natural units relative to m: sum e^(x - m) and
-// sum e^(x - m) log2 e (x - m), each in two parts while a thread adds up.
+// sum e^(x - m) log2 e (x - m). (Plain fp32 arithmetic: with the packed kind
+// more instructions went into pairing registers than it saved.)
 struct Sums {
-  float m;
-  F2 z, s;
+  float m, z, s;
 };
 
 __device__ __forceinline__ void raise_max(Sums& t, float bm) {
@@ -197,20 +169,18 @@ __device__ __forceinline__ void raise_max(Sums& t, float bm) {
     if (t.m != -INFINITY) {  // (nothing but zeros, or NaN, so far)
       const float d = fmaxf((t.m - bm) * kLog2e, -1e4f);  // finite: it meets a zero
       const float f = ex2_approx(d);
-      t.s = mul2(pack2(f, f), fma2(pack2(d, d), t.z, t.s));
-      t.z = mul2(pack2(f, f), t.z);
+      t.s = f * fmaf(d, t.z, t.s);
+      t.z = f * t.z;
     }
     t.m = bm;
   }
 }
 
-__device__ __forceinline__ void add_pair(Sums& t, F2 minus_ref, F2 x) {
+__device__ __forceinline__ void add_value(Sums& t, float ref, float x) {
   // x - ref first: exact where it matters, whatever the size of the logits
-  const F2 d = mul2(add2(x, minus_ref), pack2(kLog2e, kLog2e));
-  const F2 e = pack2(ex2_approx(lo2(d)), ex2_approx(hi2(d)));
-  t.z = add2(t.z, e);
-  // e = 0 below 2^-126: a masked value adds 0
-  t.s = fma2(e, pack2(fmaxf(lo2(d), -256.f), fmaxf(hi2(d), -256.f)), t.s);
+  const float d = (x - ref) * kLog2e, e = ex2_approx(d);
+  t.z += e;
+  t.s = fmaf(e, fmaxf(d, -256.f), t.s);  // e = 0 below 2^-126: a masked value adds 0
 }
 
 // 16 bytes that are read once.
@@ -274,8 +244,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks) logprob_kernel(const Logpro
     sh.n = 0;
     sh.limit = 0;
   }
-  Sums sum = {-INFINITY, 0, 0};
-  F2 above = 0;  // 1.0 for each
+  Sums sum = {-INFINITY, 0.f, 0.f}, odd = sum;
+  float above = 0.f;
   uint4 cur[kVecs], buf[kVecs];
   auto load = [&](int base) {
 #pragma unroll
@@ -312,40 +282,49 @@ __global__ void __launch_bounds__(kThreads, kBlocks) logprob_kernel(const Logpro
 #pragma unroll
       for (int u = 0; u < kVecs; ++u) cur[u] = buf[u];
       if (base + kStride < v1) load(base + kStride);
-      float vm[kVecs];
+      float vm[kVecs];  // the best of each vector
 #pragma unroll
       for (int u = 0; u < kVecs; ++u) {
         vm[u] = fmaxf(V::get(cur[u], 0), V::get(cur[u], 1));
 #pragma unroll
-        for (int i = 2; i < kN; ++i) vm[u] = fmaxf(vm[u], V::get(cur[u], i));
+        for (int i = 2; i < kN; i += 2) vm[u] = max3(vm[u], V::get(cur[u], i), V::get(cur[u], i + 1));
       }
       float bm = vm[0];
 #pragma unroll
       for (int u = 1; u < kVecs; ++u) bm = fmaxf(bm, vm[u]);
       bm = fmaxf(bm, -INFINITY);  // NaN where every value is one
+      raise_max(odd, bm);  // (the two chains of sums have one maximum)
       raise_max(sum, bm);
       const float ref = sum.m == -INFINITY ? 0.f : sum.m;
-      const F2 minus_ref = pack2(-ref, -ref);
 #pragma unroll
-      for (int u = 0; u < kVecs; ++u) {
-        const int v = base + u * kThreads + tid;
-        const int i0 = head + v * kN;
+      for (int u = 0; u < kVecs; ++u)
 #pragma unroll
-        for (int i = 0; i < kN; i += 2)
-          add_pair(sum, minus_ref, pack2(V::get(cur[u], i), V::get(cur[u], i + 1)));
-        // equal values count where they come before the token
-        if (v < v1 && i0 + kN <= t) {
+        for (int i = 0; i < kN; ++i) {
+          Sums& q = (i & 1) ? odd : sum;
+          add_value(q, ref, V::get(cur[u], i));
+        }
+      // Values above the token's; equal ones count where they come before it.
+      // Most steps lie on one side of it.
+      const int i_lo = head + base * kN, i_hi = i_lo + kStride * kN;
+      if (base + kStride <= v1 && i_hi <= t) {
 #pragma unroll
-          for (int i = 0; i < kN; i += 2)
-            above = add2(above, pack2(ge1(V::get(cur[u], i), xt), ge1(V::get(cur[u], i + 1), xt)));
-        } else {
+        for (int u = 0; u < kVecs; ++u)
 #pragma unroll
-          for (int i = 0; i < kN; i += 2)
-            above = add2(above, pack2(gt1(V::get(cur[u], i), xt), gt1(V::get(cur[u], i + 1), xt)));
-          if (i0 < t && v < v1) {
+          for (int i = 0; i < kN; ++i) above += ge1(V::get(cur[u], i), xt);
+      } else {
 #pragma unroll
-            for (int i = 0; i < kN; ++i)
-              if (i0 + i < t && V::get(cur[u], i) == xt) above = add2(above, pack2(1.f, 0.f));
+        for (int u = 0; u < kVecs; ++u)
+#pragma unroll
+          for (int i = 0; i < kN; ++i) above += gt1(V::get(cur[u], i), xt);
+        if (i_lo < t) {
+#pragma unroll
+          for (int u = 0; u < kVecs; ++u) {
+            const int v = base + u * kThreads + tid, i0 = head + v * kN;
+            if (v < v1 && i0 < t) {
+#pragma unroll
+              for (int i = 0; i < kN; ++i)
+                if (i0 + i < t && V::get(cur[u], i) == xt) above += 1.f;
+            }
           }
         }
       }
@@ -441,45 +420,40 @@ __global__ void __launch_bounds__(kThreads, kBlocks) logprob_kernel(const Logpro
     if (n_head + n_tail > 0) {
       const float x = i >= 0 ? value_at(i) : -INFINITY;
       if (i >= 0) {
+        raise_max(odd, x);
         raise_max(sum, x);
-        const float ref = sum.m == -INFINITY ? 0.f : sum.m;
-        add_pair(sum, pack2(-ref, -ref), pack2(x, -INFINITY));
-        if (x > xt || (x == xt && i < t)) above = add2(above, pack2(1.f, 0.f));
+        add_value(sum, sum.m == -INFINITY ? 0.f : sum.m, x);
+        if (x > xt || (x == xt && i < t)) above += 1.f;
         if (p.top > 0 && x == x) sh.cand[atomicAdd(&sh.n, 1)] = make_key(x, i);
       }
     }
   }
   if (p.top > 0) compact(sh, p.top);  // sorted, whatever their number
 
-  int n_above = static_cast<int>(lo2(above)) + static_cast<int>(hi2(above));
-  // the CTA's sums: from here on one value each, in the lower halves
-  sum.z = pack2(lo2(sum.z) + hi2(sum.z), 0.f);
-  sum.s = pack2(lo2(sum.s) + hi2(sum.s), 0.f);
+  int n_above = static_cast<int>(above);
+  sum.z += odd.z;
+  sum.s += odd.s;
   auto warp_sums = [&] {
     raise_max(sum, warp_max(sum.m));
-    float z = lo2(sum.z), w = lo2(sum.s);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      z += __shfl_xor_sync(0xffffffffu, z, o);
-      w += __shfl_xor_sync(0xffffffffu, w, o);
+      sum.z += __shfl_xor_sync(0xffffffffu, sum.z, o);
+      sum.s += __shfl_xor_sync(0xffffffffu, sum.s, o);
     }
-    sum.z = pack2(z, 0.f);
-    sum.s = pack2(w, 0.f);
     n_above = __reduce_add_sync(0xffffffffu, n_above);
   };
   warp_sums();
   if (lane == 0) {
     sh.m[warp] = sum.m;
-    sh.z[warp] = lo2(sum.z);
-    sh.s[warp] = lo2(sum.s);
+    sh.z[warp] = sum.z;
+    sh.s[warp] = sum.s;
     sh.above[warp] = n_above;
   }
   __syncthreads();
   Key best = 0;
   if (warp == 0) {
     const bool in = lane < kWarps;
-    sum = {in ? sh.m[lane] : -INFINITY, pack2(in ? sh.z[lane] : 0.f, 0.f),
-           pack2(in ? sh.s[lane] : 0.f, 0.f)};
+    sum = {in ? sh.m[lane] : -INFINITY, in ? sh.z[lane] : 0.f, in ? sh.s[lane] : 0.f};
     n_above = in ? sh.above[lane] : 0;
     warp_sums();
     if (p.top > 0) best = lane < sh.n ? sh.cand[lane] : 0;
@@ -500,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) logprob_kernel(const Logpro
       if (lane == 0)
         asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(
                          remote(&sh.part_sums[part])),
-                     "f"(sum.m), "f"(lo2(sum.z)), "f"(lo2(sum.s)), "f"(__int_as_float(n_above))
+                     "f"(sum.m), "f"(sum.z), "f"(sum.s), "f"(__int_as_float(n_above))
                      : "memory");
     }
     cluster_arrive();
@@ -514,20 +488,20 @@ __global__ void __launch_bounds__(kThreads, kBlocks) logprob_kernel(const Logpro
     if (warp == 0) {
       const float4 q = sh.part_sums[lane % parts];
       const bool in = lane < parts;
-      sum = {in ? q.x : -INFINITY, pack2(in ? q.y : 0.f, 0.f), pack2(in ? q.z : 0.f, 0.f)};
+      sum = {in ? q.x : -INFINITY, in ? q.y : 0.f, in ? q.z : 0.f};
       n_above = in ? __float_as_int(q.w) : 0;
       warp_sums();
     }
   }
   if (part != 0 || warp != 0) return;
-  const float z = lo2(sum.z), ref = sum.m == -INFINITY ? 0.f : sum.m;
+  const float z = sum.z, ref = sum.m == -INFINITY ? 0.f : sum.m;
   const bool undefined = z != z || sum.m == INFINITY;
   const float lz = sum.m == -INFINITY ? 0.f : logf(z);
   if (lane == 0) {
     p.logprob[row] = !asked ? 0.f : undefined ? NAN : xt - ref - lz;
     if (p.entropy)
       p.entropy[row] =
-          undefined ? NAN : sum.m == -INFINITY ? 0.f : fmaxf(lz - kLn2 * (lo2(sum.s) / z), 0.f);
+          undefined ? NAN : sum.m == -INFINITY ? 0.f : fmaxf(lz - kLn2 * (sum.s / z), 0.f);
     if (p.rank) p.rank[row] = asked ? n_above : -1;
   }
   if (lane < p.top) {
