@@ -255,6 +255,7 @@ __device__ __forceinline__ Slot slot_geometry(const PagedAttnProblem& p, int tok
 }
 
 constexpr int kStageThreads = 256;
+constexpr int kStageBlocks = 3;     // of an SM: their loads are what keeps the memory busy
 constexpr int kUnit = 8;            // rows that a warp decodes together
 
 // Exclusive prefix sum over the block; *total = the sum.
@@ -342,7 +343,7 @@ __device__ __forceinline__ void st_global_32(void* p, uint4 a, uint4 b) {
 // values, whose other 8 are lane 4 r + (l - 28)'s for row r. All loads of the
 // 8 rows are on their way before the first is used; a row's codes leave as
 // whole sectors.
-__global__ void __launch_bounds__(kStageThreads) stage_kernel(const __grid_constant__ TcCall c) {
+__global__ void __launch_bounds__(kStageThreads, kStageBlocks) stage_kernel(const __grid_constant__ TcCall c) {
   extern __shared__ int sm[];
   const PagedAttnProblem& p = c.p;
   const PagedLayer& g = p.pages;
@@ -396,8 +397,9 @@ __global__ void __launch_bounds__(kStageThreads) stage_kernel(const __grid_const
   auto special_bf16 = [&](const uint4& v) {
     return special4(v, 0x7F807F80u, 0x00800080u, 0x80008000u);
   };
-  for (long long u = (blockIdx.x - 1ll) * warps + (tid >> 5); u < units;
-       u += (gridDim.x - 1ll) * warps) {
+  // The cache row of key lane & 7 of unit u, -1: none. Found while the unit
+  // before is decoded, so that a unit waits for its rows alone.
+  auto find_row = [&](long long u) {
     const int block = static_cast<int>(u / (kKeys / kUnit));
     int lo = 0, hi = g.n_seqs;
     while (hi - lo > 1) {
@@ -407,15 +409,21 @@ __global__ void __launch_bounds__(kStageThreads) stage_kernel(const __grid_const
     }
     const int len = g.length[lo], first = len - (p.q_start[lo + 1] - p.q_start[lo]);
     const int klo = p.window > 0 ? max(0, first - p.window + 1) : 0;
-    // lanes 0-7: the cache row of their key, -1: none
     const int t = klo + (block - block_start[lo]) * kKeys +
                   static_cast<int>(u % (kKeys / kUnit)) * kUnit + (lane & 7);
     int row = -1;
-    if (lane < kUnit && t < len && t / g.page < g.max_pages) {
+    if (t < len && t / g.page < g.max_pages) {
       const int page = g.table[static_cast<size_t>(lo) * g.max_pages + t / g.page];
       if (page >= 0 && page < g.n_pages) row = page * g.page + t % g.page;
     }
-    const unsigned there = __ballot_sync(0xffffffffu, row >= 0);
+    return row;
+  };
+  const long long step = (gridDim.x - 1ll) * warps;
+  long long u = (blockIdx.x - 1ll) * warps + (tid >> 5);
+  int next_row = u < units ? find_row(u) : -1;
+  for (; u < units; u += step) {
+    const int row = next_row;
+    const unsigned there = __ballot_sync(0xffffffffu, row >= 0) & 0xFFu;
     const int rc = max(row, 0);  // (an absent key's lanes load row 0 and do not use it)
     uint4 raw[kUnit];
     // 4 scale codes: of key lane & 7, groups 0-3 or (lanes 16-31) 4-7
@@ -430,6 +438,7 @@ __global__ void __launch_bounds__(kStageThreads) stage_kernel(const __grid_const
         reinterpret_cast<const uint8_t*>(g.rope) +
         static_cast<size_t>(__shfl_sync(0xffffffffu, rc, lane >> 2)) * (2 * kRope) +
         32 * (lane & 3) + 16));
+    if (u + step < units) next_row = find_row(u + step);
     uint32_t code[kUnit];  // the scale code of this lane's dims
     bool in_range = true;
     unsigned bad = special_bf16(more) ? 1u << (lane >> 2) : 0u;
@@ -489,20 +498,19 @@ __global__ void __launch_bounds__(kStageThreads) stage_kernel(const __grid_const
 }
 
 constexpr int kOwnStages = 3;    // 32 KB: a block's dims of this CTA's half, also the V of P V
-constexpr int kOtherStages = 2;  // 16 KB: half of its other dims
+constexpr int kOtherStages = 4;  // 16 KB: half of its other dims
 constexpr uint32_t kBlk = kKeys * 128;       // 64 keys x 64 dims, one swizzled box (8 KB)
 constexpr uint32_t kQBlk = kRows * 128;      // 128 rows x 64 dims (16 KB)
 constexpr uint32_t kSmQ = 0;                 // Q dims 256-511 (64 KB)
 constexpr uint32_t kSmOwn = 4 * kQBlk;
 constexpr uint32_t kSmOther = kSmOwn + kOwnStages * 4 * kBlk;
-constexpr uint32_t kSmP = kSmOther + kOtherStages * 2 * kBlk;
-constexpr uint32_t kPBytes = kRows * kKeys * 2;            // P, and what its rounding left
-constexpr uint32_t kSmBar = kSmP + 2 * kPBytes;
+constexpr uint32_t kSmBar = kSmOther + kOtherStages * 2 * kBlk;
 constexpr uint32_t kSmMax = kSmBar + 256;    // [2 blocks][2 key halves][128] row maxima
 constexpr uint32_t kSmScale = kSmMax + 2 * 2 * kRows * 4;  // [128] what O is multiplied by
 constexpr uint32_t kTcBytes = kSmScale + kRows * 4;
 static_assert(kTcBytes <= 232448, "beyond the shared memory of a CTA");
-constexpr uint32_t kColS = 256, kColQ = 384, kCols = 512;  // O: 0-255, S: two of 64, Q dims 0-255
+// TMEM: O 0-255, S, P and what its rounding left (two values a column), Q dims 0-255
+constexpr uint32_t kColS = 256, kColP = 320, kColQ = 384, kCols = 512;
 
 constexpr int kSoftmaxWarps = 8, kLoadWarps = 4;
 constexpr int kWarpTma = kSoftmaxWarps + kLoadWarps, kWarpMma = kWarpTma + 1;
@@ -511,7 +519,7 @@ constexpr int kTcThreads = 32 * (kWarpMma + 1);
 struct Bars {
   uint64_t full_own[kOwnStages], empty_own[kOwnStages];
   uint64_t full_other[kOtherStages], empty_other[kOtherStages];
-  uint64_t s_full[2], p_full, pv_done, q_full, q_free, o_ready, o_free, fin, pair[4];
+  uint64_t s_full, s_free, p_full, pv_done, q_full, q_free, o_ready, o_free, fin, pair[4];
   uint32_t tmem;
   int abort_flag;
 };
@@ -706,15 +714,6 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
-}
-
 // The two warps of 32 rows meet (a barrier in shared memory, because a named
 // one could not give up).
 struct PairSync {
@@ -729,9 +728,9 @@ struct PairSync {
 };
 
 // 32 scores of a row (this thread's half of the block's keys) to weights in
-// shared memory. kPlain: every key is visible and one BF16 term is enough;
-// then P V of the block before is waited for as late as possible, when the
-// weights are there. `rescale`: O (and what was summed before) is to be
+// TMEM. kPlain: every key is visible and one BF16 term is enough. P V of the
+// block before, which reads them there, is waited for when the new ones are
+// ready. `rescale`: O (and what was summed before) is to be
 // multiplied by alpha.
 struct RowState {
   float m, den;
@@ -740,10 +739,12 @@ template <bool kPlain, class WaitPv>
 __device__ __forceinline__ bool softmax_block(uint32_t s_col, uint32_t mask, bool two_terms,
                                               float sc2, float* max_mine, const float* max_other,
                                               PairSync& meet, bool& good, RowState& st,
-                                              float& alpha, uint32_t prow, int chunk0, int row,
+                                              float& alpha, uint32_t p_col, uint64_t* s_free,
                                               WaitPv wait_pv) {
   uint32_t r[32];
   tmem_ld32(s_col, r);
+  tc_fence_before();
+  mbar_arrive(s_free);  // the next block's scores may come
   float tm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
@@ -778,34 +779,28 @@ __device__ __forceinline__ bool softmax_block(uint32_t s_col, uint32_t mask, boo
       r[i / 2] = pack_bf16x2(e0, e1);
     }
     good = wait_pv() && good;
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      st_shared_v4(prow + (((chunk0 + k) ^ (row & 7)) << 4),
-                   make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]));
+    __syncwarp();
+    tc_fence_after();
+    tmem_st16(p_col, r);
   } else {
-    good = wait_pv() && good;
+    uint32_t less[16];  // what the rounding left
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float e[8];
-      uint32_t h[4];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = ex2_approx(fmaf(__uint_as_float(r[8 * k + i]), sc2, neg));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        part[i] += e[2 * i] + e[2 * i + 1];
-        h[i] = pack_bf16x2(e[2 * i], e[2 * i + 1]);
-      }
-      const uint32_t at = prow + (((chunk0 + k) ^ (row & 7)) << 4);
-      st_shared_v4(at, make_uint4(h[0], h[1], h[2], h[3]));
-      if (two_terms) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          h[i] = pack_bf16x2(e[2 * i] - __uint_as_float(h[i] << 16),
-                             e[2 * i + 1] - __uint_as_float(h[i] & 0xFFFF0000u));
-        st_shared_v4(at + kPBytes, make_uint4(h[0], h[1], h[2], h[3]));
-      }
+    for (int i = 0; i < 32; i += 2) {
+      const float e0 = ex2_approx(fmaf(__uint_as_float(r[i]), sc2, neg));
+      const float e1 = ex2_approx(fmaf(__uint_as_float(r[i + 1]), sc2, neg));
+      part[(i >> 1) & 3] += e0 + e1;
+      const uint32_t h = pack_bf16x2(e0, e1);
+      less[i / 2] =
+          pack_bf16x2(e0 - __uint_as_float(h << 16), e1 - __uint_as_float(h & 0xFFFF0000u));
+      r[i / 2] = h;
     }
+    good = wait_pv() && good;
+    __syncwarp();
+    tc_fence_after();
+    tmem_st16(p_col, r);
+    if (two_terms) tmem_st16(p_col + kKeys / 2, less);
   }
+  tmem_st_wait();
   st.den = st.den * alpha + ((part[0] + part[1]) + (part[2] + part[3]));
   return rescale;
 }
@@ -818,10 +813,14 @@ __device__ __forceinline__ bool softmax_block(uint32_t s_col, uint32_t mask, boo
 //   warp 12    key blocks and Q by TMA (one lane)
 //   warp 13    TMEM allocation and MMA issue
 // Per block: S = Q K^T (32 MMAs of 128 x 64 x 16, the other half's dims first
-// so that their slots are free early), P = 2^(S - m) in BF16 to shared
-// memory, O += P V (4 MMAs of 128 x 256 x 16, the own half read MN-major).
-// P V of a block is issued after Q K^T of the next, so the tensor pipe works
-// while the softmax does.
+// so that their slots are free early), P = 2^(S - m) in BF16 back to TMEM,
+// O += P V (4 MMAs of 128 x 256 x 16, P the A operand in TMEM, the own half
+// read MN-major). Q K^T of a block is issued once the scores of the one before
+// are in registers, P V of that one after it, so the tensor pipe works while
+// the softmax does. P in TMEM leaves 32 KB to the ring of the other dims, two
+// blocks ahead instead of one: where the rows come from DRAM that is what
+// counts (32 sequences of 4.6k keys: 55 us of 64; keys that L2 holds: 2% more
+// than with P in shared memory and two buffers of S).
 __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
     const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap qmap,
     const __grid_constant__ TcCall c) {
@@ -843,8 +842,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
       mbar_init(&bars->full_other[i], 1);
       mbar_init(&bars->empty_other[i], 1);
     }
-    mbar_init(&bars->s_full[0], 1);
-    mbar_init(&bars->s_full[1], 1);
+    mbar_init(&bars->s_full, 1);
+    mbar_init(&bars->s_free, 32 * kSoftmaxWarps);
     mbar_init(&bars->p_full, 32 * kSoftmaxWarps);
     mbar_init(&bars->pv_done, 1);
     mbar_init(&bars->q_full, 32 * kLoadWarps + 1);  // and the TMA warp's
@@ -890,7 +889,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
     const int tok = row / p.H, h = row - tok * p.H;
     const uint32_t lanes = static_cast<uint32_t>(w4 * 32) << 16;
     const uint32_t o_cols = tmem + lanes + side * (kHalf / 2);
-    const uint32_t prow = base + kSmP + (row >> 3) * 1024 + (row & 7) * 128;
+    const uint32_t s_col = tmem + lanes + kColS + side * 32, p_col = tmem + lanes + kColP + side * 16;
     float* maxima = reinterpret_cast<float*>(smem + kSmMax);
     float* max_mine = maxima + side * kRows + row;
     const float* max_other = maxima + (1 - side) * kRows + row;
@@ -936,12 +935,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
         }
         // A wait that gives up ends the loop at the block's vote; what is
         // computed until then is not used.
-        const int sb = n & 1;
-        bool good = long_wait(&bars->s_full[sb], (n >> 1) & 1, abort_flag, err);
+        bool good = long_wait(&bars->s_full, n & 1, abort_flag, err);
         __syncwarp();
         tc_fence_after();
-        const uint32_t s_col = tmem + lanes + kColS + sb * kKeys + side * 32;
-        const int buf = sb * 2 * kRows;
+        const int buf = static_cast<int>(n & 1) * 2 * kRows;
         float alpha;
         // P V of the block before has read P, and O holds all blocks before
         auto wait_pv = [&] {
@@ -949,10 +946,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
         };
         const bool rescale =
             plain ? softmax_block<true>(s_col, mask32, false, sc2, max_mine + buf, max_other + buf,
-                                        meet, good, st, alpha, prow, 4 * side, row, wait_pv)
+                                        meet, good, st, alpha, p_col, &bars->s_free, wait_pv)
                   : softmax_block<false>(s_col, mask32, two_terms, sc2, max_mine + buf,
-                                         max_other + buf, meet, good, st, alpha, prow, 4 * side,
-                                         row, wait_pv);
+                                         max_other + buf, meet, good, st, alpha, p_col,
+                                         &bars->s_free, wait_pv);
         if (!__all_sync(0xffffffffu, good)) {
           ok = false;
           break;
@@ -969,7 +966,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
           }
           tmem_st_wait();
         }
-        fence_async_smem();
         tc_fence_before();
         mbar_arrive(&bars->p_full);
       }
@@ -1223,7 +1219,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
       constexpr uint32_t idesc_qk = umma_idesc_bf16(kRows, kKeys, false);
       constexpr uint32_t idesc_pv = umma_idesc_bf16(kRows, kHalf, true);
       const uint64_t q_desc = umma_desc(base + kSmQ, 16, 1024);
-      const uint64_t p_desc = umma_desc(base + kSmP, 16, 1024);
       const uint64_t own_desc = umma_desc(base + kSmOwn, 16, 1024);
       const uint64_t other_desc = umma_desc(base + kSmOther, 16, 1024);
       const uint64_t v_desc = umma_desc(base + kSmOwn, kBlk, 1024);
@@ -1260,11 +1255,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
         const uint64_t v = v_desc + sv * (4 * kBlk / 16);
 #pragma unroll
         for (int kk = 0; kk < kKeys / 16; ++kk)
-          mma_ss(tmem, p_desc + kk * 2, v + kk * 128, idesc_pv, !(first && kk == 0));
+          mma_ts(tmem, tmem + kColP + kk * 8, v + kk * 128, idesc_pv, !(first && kk == 0));
         if (two_terms) {
 #pragma unroll
           for (int kk = 0; kk < kKeys / 16; ++kk)
-            mma_ss(tmem, p_desc + kPBytes / 16 + kk * 2, v + kk * 128, idesc_pv, true);
+            mma_ts(tmem, tmem + kColP + kKeys / 2 + kk * 8, v + kk * 128, idesc_pv, true);
         }
         mma_commit(&bars->pv_done);
         mma_commit(&bars->empty_own[sv]);
@@ -1286,7 +1281,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
         const bool two_terms = seg.t.blocks <= kTwoTermBlocks;
         bool ready = false;
         for (int j = seg.j0; j < seg.j1; ++j, ++n) {
-          const uint32_t s_col = tmem + kColS + (n & 1) * kKeys;
+          // the softmax has read the scores of the block before
+          if (n > 0) {
+            if (!(ok = waits(false, &bars->s_free, n - 1))) break;
+            tc_fence_after();
+          }
+          const uint32_t s_col = tmem + kColS;
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             if (!(ok = waits(ready, &bars->full_other[so], po))) break;
@@ -1303,7 +1303,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
           qk(s_col, k_desc, half, 0, false);
           qk(s_col, k_desc + 2 * kBlk / 16, half, 2, false);
           if (++sw == kOwnStages) { sw = 0; pw ^= 1; }
-          mma_commit(&bars->s_full[n & 1]);
+          mma_commit(&bars->s_full);
           if (j + 1 == seg.j1) mma_commit(&bars->q_free);
           const bool p_ready = ready;
           ready = peek(&bars->full_other[so], po);
@@ -1510,7 +1510,7 @@ cudaError_t tc_forward(const PagedAttnProblem& p, void* ws, cudaStream_t st) {
   const size_t smem = sizeof(int) * 2 * (static_cast<size_t>(p.pages.n_seqs) + 1);
   const long long units =
       (c.s.block_cap * (kKeys / kUnit) + kStageThreads / 32 - 1) / (kStageThreads / 32);
-  const int most = sm_count() * 4;
+  const int most = sm_count() * kStageBlocks - 1;
   cudaError_t e = launch_pdl(stage_kernel, dim3(1 + static_cast<unsigned>(units < most ? units : most)),
                              dim3(kStageThreads), smem, st, c);
   if (e != cudaSuccess) return e;
