@@ -115,6 +115,14 @@ __device__ int take_free(const PagedState& p, int want, int* page) {
   return have < want ? have : want;
 }
 
+// This lane's next entries of a table row, all on their way at once; -1
+// behind its end.
+constexpr int kAhead = 4;
+__device__ __forceinline__ void load_pages(const int* row, int j0, int n, int (&q)[kAhead]) {
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) q[k] = j0 + 32 * k < n ? row[j0 + 32 * k] : -1;
+}
+
 // ops' first claims on a slot: owner[s] = the lowest op that names it.
 __device__ void claim(const PagedState& p, const int* slots, int n, int* owner) {
   for (int s = threadIdx.x; s < p.n_seqs; s += blockDim.x) owner[s] = INT_MAX;
@@ -167,10 +175,14 @@ __global__ void __launch_bounds__(kMetaThreads) fork_kernel(const __grid_constan
   for (int i = warp; i < n; i += nw) {
     if (rank[i] == -2) continue;
     int* row = p.table + static_cast<size_t>(dst[i]) * p.max_pages;
-    for (int j = lane; j < p.max_pages; j += 32) {
-      const int q = row[j];
-      if (in_range(q, p.n_pages)) atomicSub(&p.refs[q], 1);
-      row[j] = -1;
+    for (int j0 = lane; j0 < p.max_pages; j0 += 32 * kAhead) {
+      int q[kAhead];
+      load_pages(row, j0, p.max_pages, q);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        if (in_range(q[k], p.n_pages)) atomicSub(&p.refs[q[k]], 1);
+        if (j0 + 32 * k < p.max_pages) row[j0 + 32 * k] = -1;
+      }
     }
   }
   __syncthreads();
@@ -192,12 +204,15 @@ __global__ void __launch_bounds__(kMetaThreads) fork_kernel(const __grid_constan
     const int f = len / p.page;
     const int* from = p.table + static_cast<size_t>(s) * p.max_pages;
     int* row = p.table + static_cast<size_t>(d) * p.max_pages;
-    for (int j = lane; j < f; j += 32) {
-      const int q = from[j];
-      if (in_range(q, p.n_pages)) {
-        atomicAdd(&p.refs[q], 1);
-        row[j] = q;
-      }
+    for (int j0 = lane; j0 < f; j0 += 32 * kAhead) {
+      int q[kAhead];
+      load_pages(from, j0, f, q);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (in_range(q[k], p.n_pages)) {
+          atomicAdd(&p.refs[q[k]], 1);
+          row[j0 + 32 * k] = q[k];
+        }
     }
     if (lane == 0) {
       p.length[d] = len;
@@ -290,20 +305,23 @@ __global__ void __launch_bounds__(kMetaThreads) append_kernel(const __grid_const
 __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ PagedState p,
                                                    const int* __restrict__ slots, int n,
                                                    long long* __restrict__ rows, long long n_rows) {
+  extern __shared__ long long first[];  // [n + 1]
   pdl_wait();
   const Ws w = carve(p.ws, p.n_pages, p.n_seqs);
-  const long long total = min(w.first[n], n_rows);
+  for (int i = threadIdx.x; i <= n; i += 256) first[i] = w.first[i];
+  __syncthreads();
+  const long long total = min(first[n], n_rows);
   for (long long t = blockIdx.x * 256ll + threadIdx.x; t < total; t += gridDim.x * 256ll) {
     int lo = 0, hi = n;  // the last op with first <= t
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (w.first[mid] <= t) lo = mid;
+      if (first[mid] <= t) lo = mid;
       else hi = mid;
     }
     const int len = w.jobs[lo].src;
     long long row = -1;
     if (len >= 0) {
-      const int pos = len + static_cast<int>(t - w.first[lo]);
+      const int pos = len + static_cast<int>(t - first[lo]);
       row = static_cast<long long>(
                 p.table[static_cast<size_t>(slots[lo]) * p.max_pages + pos / p.page]) * p.page +
             pos % p.page;
@@ -519,8 +537,8 @@ cudaError_t paged_append(const PagedState& p, const int* slots, const int* count
   append_kernel<<<1, kMetaThreads, smem, st>>>(p, slots, counts, n, rows, n_rows);
   e = cudaGetLastError();
   if (e != cudaSuccess || !rows || n_rows <= 0) return e;
-  return launch_pdl(rows_kernel, dim3(copy_blocks((n_rows + 255) / 256)), dim3(256), 0, st, p,
-                    slots, n, rows, n_rows);
+  return launch_pdl(rows_kernel, dim3(copy_blocks((n_rows + 255) / 256)), dim3(256),
+                    sizeof(long long) * (static_cast<size_t>(n) + 1), st, p, slots, n, rows, n_rows);
 }
 
 cudaError_t paged_compact(const PagedState& p, int* table_out, int* refs_out, cudaStream_t st) {
