@@ -399,3 +399,60 @@ def test_refusals(cuda):
         cuda.paged_attn(odd, c.q, c.pool, 0, c.q_start, 2, 30, 1.0)
     c.run()                                       # still usable
     c.check()
+
+
+@pytest.mark.parametrize("nope,rope", [(448, 64), (64, 16)])
+@pytest.mark.parametrize("max_new,max_len", [(4, 400), (5, 199), (5, 399), (4, 199)])
+def test_slots_beyond_the_bounds(cuda, nope, rope, max_new, max_len):
+    """A slot with more tokens, or a longer one, than was said: NaN and a
+    status bit; the others are not touched by it."""
+    c = Case(cuda, [(3, 100), (5, 200), (1, 400), (2, 64)], 16, page=16, nope=nope, rope=rope,
+             seed=41)
+    cuda.paged_attn(c.out, c.q, c.pool, 0, c.q_start, max_new, max_len, c.scale, sink=c.sink,
+                    rope_cos=c.cos, rope_sin=c.sin, lse=c.lse)
+    assert c.pool.status() == 4
+    c.pool.status_word.zero_()
+    bad = [r for s, (n, length) in enumerate(c.seqs) if n > max_new or length > max_len
+           for r in range(c.starts[s], c.starts[s + 1])]
+    assert torch.isnan(c.out[bad]).all() and torch.isnan(c.lse[bad]).all()
+    c.check(rows=set(range(11)) - set(bad))
+
+
+def test_more_keys_than_the_workspace_was_made_for(cuda):
+    c = Case(cuda, [(2, 100), (1, 3000), (0, 0)], 64, seed=43)
+    for last, fits in ((3000, False), (1500, True)):
+        c.pool.length[1] = last
+        c.seqs[1] = (1, last)
+        c.out.fill_(77.0)
+        cuda.paged_attn(c.out, c.q, c.pool, 0, c.q_start, 2, 3000, c.scale, sink=c.sink,
+                        rope_cos=c.cos, rope_sin=c.sin, lse=c.lse, max_keys=1600)
+        assert c.pool.status() == (0 if fits else 4)
+        c.pool.status_word.zero_()
+        if not fits:
+            assert torch.isnan(c.out[2]).all() and torch.isnan(c.lse[2]).all()
+        c.check(rows=None if fits else {0, 1})
+
+
+@pytest.mark.parametrize("nope,rope", [(448, 64), (64, 16)])
+def test_rows_of_no_slot_are_left_out(cuda, nope, rope):
+    c = Case(cuda, [(4, 90), (3, 40), (6, 200)], 32, page=16, nope=nope, rope=rope, seed=47)
+    c.q_start.copy_(torch.tensor([2, 4, 7, 11]))       # rows 0, 1, 11 and 12 belong to nobody
+    c.starts = np.array([2, 4, 7, 11])
+    c.seqs = [(2, 90), (3, 40), (4, 200)]
+    c.run()
+    c.check()
+    for r in (0, 1, 11, 12):
+        assert (c.out[r] == 77).all() and (c.lse[r] == 77).all()
+
+
+@pytest.mark.parametrize("nope,rope", [(448, 64), (64, 16)])
+def test_tokens_before_the_first_position(cuda, nope, rope):
+    """More new tokens than positions: the first of them see nothing."""
+    c = Case(cuda, [(5, 90), (1, 30)], 16, page=16, nope=nope, rope=rope, seed=53)
+    c.use_sink = False
+    c.pool.length[0] = 3                               # tokens at -2 .. 2
+    c.run()
+    torch.cuda.synchronize()
+    assert (c.out[:2] == 0).all() and torch.isneginf(c.lse[:2]).all()
+    c.seqs[0] = (5, 3)
+    c.check(rows={2, 3, 4, 5})
