@@ -59,7 +59,9 @@ __device__ __forceinline__ void store_out(const PagedAttnProblem& p, long long a
 }
 
 // General form: one block per (head, token), a warp per key, the running
-// maximum and sum of a softmax per warp, merged at the end.
+// maximum and sum of a softmax per warp, merged at the end. For shapes that the
+// tensor-core kernel does not take; the arithmetic is plain fp32, and every
+// head decodes its keys again, which bounds it (GENERAL).
 __global__ void __launch_bounds__(32 * kSimtWarps) paged_attn_simt_kernel(
     const __grid_constant__ PagedAttnProblem p) {
   const PagedLayer& c = p.pages;
@@ -176,12 +178,18 @@ constexpr int kRows = 128;        // (token, head) rows of a tile: M of both pro
 constexpr int kKeys = 64;         // keys of a block: N of Q K^T, K of P V
 constexpr int kHalf = 256;        // output dims of a CTA: N of P V
 // What a tile costs besides its blocks (Q in, O out), in blocks: shares are
-// cut by the sum, so that many short tiles weigh as much as a long one.
+// cut by the sum, so that many short tiles weigh as much as a long one (2000
+// tiles of three blocks: 208 us, 273 where a tile costs nothing, 207 at 8; 8
+// sequences of 3 tiles of 32 to 63 blocks: 51.9, 55.7 and 53.2).
 constexpr int kTileCost = 4;
-constexpr int kMinShare = 2;  // a smaller share costs more to merge than it saves
+// A smaller share costs more to merge than it saves (one tile of 32 blocks:
+// 21.7 us, 23.7 with shares from one unit on, 21.8 from four).
+constexpr int kMinShare = 2;
 // A tile of at most this many blocks carries its weights in two BF16 terms:
 // where a row sees few keys, the rounding of one weight does not average out
-// (with one term a two-key row is off by up to 2^-8 of its value sum).
+// (with one term a two-key row is off by up to 2^-8 of its value sum). Twice
+// the MMAs of P V there: 208 us for 2000 tiles of three blocks, 205 with one
+// term. In longer tiles the sum of many roundings is far below that of one.
 constexpr int kTwoTermBlocks = 4;
 constexpr float kLazyMargin = 8.0f;  // log2 units: the running max moves only past this
 
@@ -343,6 +351,12 @@ __device__ __forceinline__ void st_global_32(void* p, uint4 a, uint4 b) {
 // values, whose other 8 are lane 4 r + (l - 28)'s for row r. All loads of the
 // 8 rows are on their way before the first is used; a row's codes leave as
 // whole sectors.
+// What bounds it is the latency of its loads at the 24 warps an SM that the
+// registers allow: 147k rows (86 MB read, 151 MB written) in 45 us, 5.3 TB/s;
+// 53 us with blocks in two waves and a unit's rows looked up when it is due.
+// Rows decoded inside the attention kernel would spare the 151 MB, but the
+// conversions then share the issue slots with the softmax: 153 to 202 us for
+// that call, where decoding ahead took 150 at the time.
 __global__ void __launch_bounds__(kStageThreads, kStageBlocks) stage_kernel(const __grid_constant__ TcCall c) {
   extern __shared__ int sm[];
   const PagedAttnProblem& p = c.p;
@@ -1326,7 +1340,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
 
 // Tiles that a share's end cuts: a warp per (cut, row, half of the dims), 8
 // dims a lane. Everything it reads is asked for as early as its address is
-// known: the plan and the cut's tile, then maxima, sums and the first parts.
+// known: the plan and the cut's tile, then maxima, sums and the first parts;
+// that chain bounds it (7 us for one tile in 19 parts, 12 for 32 tiles of 64
+// rows in 74 shares, 14 MB of parts).
 constexpr int kMergeWarps = 8;
 __global__ void __launch_bounds__(32 * kMergeWarps) paged_attn_merge_kernel(
     const __grid_constant__ TcCall c) {
