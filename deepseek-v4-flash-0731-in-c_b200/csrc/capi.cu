@@ -1632,7 +1632,10 @@ bool paged_state(const char* who, const dsv4cuda_paged* p, dsv4::PagedState* s) 
   s->rope_dim = p->caches[0].rope_dim;
   const long long rows = static_cast<long long>(p->n_pages) * p->page_size;
   for (int l = 0; l < p->n_caches; ++l) {
-    const dsv4cuda_kv_cache* c = &p->caches[l];
+    dsv4cuda_kv_cache cache = p->caches[l];
+    if (cache.rope_dim == 0 && !cache.rope)  // nothing is read there
+      cache.rope = reinterpret_cast<uint16_t*>(cache.codes);
+    const dsv4cuda_kv_cache* c = &cache;
     if (!cache_ok(c) || c->nope != s->nope || c->rope_dim != s->rope_dim || c->rows < rows ||
         reinterpret_cast<uintptr_t>(c->codes) % 16 || reinterpret_cast<uintptr_t>(c->rope) % 16 ||
         reinterpret_cast<uintptr_t>(c->scales) % 8) {
@@ -1677,6 +1680,10 @@ bool attn_problem(const char* who, const dsv4cuda_paged* p, int layer,
       s->window < 0 || s->max_keys < 0 || s->rope_dim < 0 || s->rope_dim > s->head_dim ||
       s->rope_dim % 2 || qs < width || os < width) {
     record_error("%s: bad shape (rope_dim even, strides at least heads * head_dim)", who);
+    return false;
+  }
+  if (a->pages.rope_dim % 2) {
+    record_error("%s: rows of an odd rope_dim (%d)", who, a->pages.rope_dim);
     return false;
   }
   if (s->head_dim != d || d > 1024) {

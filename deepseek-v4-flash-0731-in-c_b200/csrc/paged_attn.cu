@@ -24,19 +24,6 @@
 namespace dsv4 {
 namespace {
 
-constexpr int kMaxDim = 1024;              // of the general kernel
-constexpr int kLaneDims = kMaxDim / 32;
-constexpr int kSimtWarps = 8;
-
-__device__ __forceinline__ float latent_value(const PagedLayer& c, long long r, int i) {
-  if (i < c.nope) {
-    const float v = e4m3_decode(c.codes[r * c.nope + i]) *
-                    e8m0_decode(c.scales[r * kKvScaleSlots + i / 64]);
-    return isfinite(v) ? bf16_round(v) : v;  // the rounding's carry would turn a NaN into a zero
-  }
-  return bf16_widen(c.rope[r * c.rope_dim + (i - c.nope)]);
-}
-
 // The slot whose rows hold row `row`: the last s with q_start[s] <= row that
 // is not empty. -1: none.
 __device__ __forceinline__ int slot_of(const int* q_start, int n_seqs, int row) {
@@ -58,106 +45,290 @@ __device__ __forceinline__ void store_out(const PagedAttnProblem& p, long long a
   else static_cast<float*>(p.out)[at] = __bfloat162float(__float2bfloat16_rn(v));
 }
 
-// General form: one block per (head, token), a warp per key, the running
-// maximum and sum of a softmax per warp, merged at the end. For shapes that the
-// tensor-core kernel does not take; the arithmetic is plain fp32, and every
-// head decodes its keys again, which bounds it (GENERAL).
-__global__ void __launch_bounds__(32 * kSimtWarps) paged_attn_simt_kernel(
-    const __grid_constant__ PagedAttnProblem p) {
+// ========================================================== general path ==
+//
+// For shapes that the tensor-core kernel does not take: a block per token, 8
+// or 16 heads and a piece of the keys, in fp32. 32 keys at a time are decoded
+// to BF16 (what the cache's values round to) in shared memory, once for all
+// heads of the block; then a lane has a key for the scores and two neighbouring
+// dims of each 64 for the sums, a warp one head or two. The pieces are a
+// cluster's blocks, which merge through one another's shared memory, each
+// some of the heads. Shared-memory reads and FMAs of few warps bound it: 64
+// heads of 576 dims on 2048 keys take 100 us for one token (1.7 ms with a
+// block per head that decodes its own keys), 1.29 ms for 64 (21.7 ms).
+constexpr int kMaxDim = 1024;
+constexpr int kGenWarps = 8;
+constexpr int kGenThreads = 32 * kGenWarps;
+constexpr int kGenKeys = 32;       // of a step
+constexpr int kGenParts = 8;       // at most, of a token's keys
+
+// Words of a decoded key: odd, so that lanes on 32 keys meet 32 banks.
+__host__ __device__ inline int gen_pitch(int d) { return (d / 2) | 1; }
+
+__device__ __forceinline__ uint32_t in_part(const void* p, int rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float ld_part(uint32_t a) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_part2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void all_parts() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" :::
+                   "memory");
+}
+
+// One of two BF16 values is a NaN or an infinity.
+__device__ __forceinline__ bool special2(uint32_t w) {
+  return (((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u) != 0;
+}
+
+// kHeads: of a warp; kWords: pairs of dims of a lane, dim <= 64 kWords.
+template <int kHeads, int kWords>
+__global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(
+    const __grid_constant__ PagedAttnProblem p, int parts) {
+  constexpr int kBlockHeads = kGenWarps * kHeads;
+  extern __shared__ __align__(16) float sm_q[];  // [kBlockHeads][d]: q, at the end the sums
+  __shared__ float sm_m[kBlockHeads], sm_den[kBlockHeads];
+  __shared__ int sm_row[kGenKeys];
+  __shared__ unsigned sm_there, sm_broken;
+  __shared__ float sm_bad;
   const PagedLayer& c = p.pages;
-  const int row = blockIdx.x, h = blockIdx.y;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int d = c.nope + c.rope_dim;
-  __shared__ float sm_m[kSimtWarps], sm_den[kSimtWarps];
-  __shared__ float sm_o[kMaxDim];
-  __shared__ int sm_bad;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int row = blockIdx.x / parts, part = blockIdx.x % parts, head0 = blockIdx.y * kBlockHeads;
+  const int d = c.nope + c.rope_dim, words = d / 2, pitch = gen_pitch(d);
+  uint32_t* sm_k = reinterpret_cast<uint32_t*>(sm_q + kBlockHeads * d);
   const int s = slot_of(p.q_start, c.n_seqs, row);
-  if (s < 0) return;
-  const bool beyond = p.q_start[s + 1] - p.q_start[s] > p.max_new || c.length[s] > p.max_len;
-  if (threadIdx.x == 0) {
-    sm_bad = beyond;
-    if (beyond && c.status) atomicOr(c.status, kPagedBounds);
+  if (s < 0) return;  // (the whole cluster)
+  const int len = c.length[s], end = p.q_start[s + 1];
+  const bool beyond = end - p.q_start[s] > p.max_new || len > p.max_len;
+  if (beyond && tid == 0 && c.status) atomicOr(c.status, kPagedBounds);
+  const int self = len - end + row;  // the token's position
+  const int first = p.window > 0 ? max(0, self - p.window + 1) : 0;
+  const int last = min(self, c.max_pages * c.page - 1);
+  const int steps = beyond || last < first ? 0 : (last - first) / kGenKeys + 1;
+  const int step0 = static_cast<int>(static_cast<long long>(steps) * part / parts);
+  const int step1 = static_cast<int>(static_cast<long long>(steps) * (part + 1) / parts);
+  for (int hl = warp * kHeads; hl < (warp + 1) * kHeads; ++hl)  // read by this warp alone
+    for (int i = lane; i < d; i += 32)
+      sm_q[hl * d + i] = head0 + hl < p.H
+                             ? load_q(p, row * p.q_stride + static_cast<long long>(head0 + hl) * d + i)
+                             : 0.f;
+  const int* table = c.table + static_cast<size_t>(s) * c.max_pages;
+  const int units = c.nope / 16, pairs = c.rope_dim / 2;  // of a key
+  const bool idle = head0 + warp * kHeads >= p.H;
+  bool bad = beyond;
+  float m[kHeads], den[kHeads], o[kHeads][2 * kWords];  // den: this lane's keys
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    m[i] = -INFINITY;
+    den[i] = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2 * kWords; ++u) o[i][u] = 0.f;
   }
-  for (int i = threadIdx.x; i < d; i += blockDim.x) sm_o[i] = 0.f;
-  __syncthreads();
-  float m = -INFINITY, den = 0.f;
-  float q[kLaneDims], o[kLaneDims];
-#pragma unroll
-  for (int u = 0; u < kLaneDims; ++u) {
-    const int i = u * 32 + lane;
-    q[u] = i < d ? load_q(p, row * p.q_stride + static_cast<long long>(h) * d + i) : 0.f;
-    o[u] = 0.f;
-  }
-  {
-    const int last = c.length[s] - p.q_start[s + 1] + row;
-    const int first = p.window > 0 ? max(0, last - p.window + 1) : 0;
-    const int* table = c.table + static_cast<size_t>(s) * c.max_pages;
-    for (int t = first + warp; t <= last && t / c.page < c.max_pages; t += kSimtWarps) {
-      const int page = table[t / c.page];
-      if (page < 0 || page >= c.n_pages) continue;
-      const long long r = static_cast<long long>(page) * c.page + t % c.page;
-      float k[kLaneDims], dot = 0.f;
-      bool fine = true;
-#pragma unroll
-      for (int u = 0; u < kLaneDims; ++u) {
-        const int i = u * 32 + lane;
-        k[u] = i < d ? latent_value(c, r, i) : 0.f;
-        fine = fine && isfinite(k[u]);
-        dot = fmaf(q[u], k[u], dot);
-      }
-      if (!__all_sync(0xffffffffu, fine)) {
-        if (lane == 0) sm_bad = 1;
-        continue;
-      }
-#pragma unroll
-      for (int u = 16; u > 0; u >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, u);
-      const float x = dot * p.scale;
-      const float mx = fmaxf(m, x);
-      const float a = m == -INFINITY ? 0.f : expf(m - mx), w = expf(x - mx);
-      den = den * a + w;
-#pragma unroll
-      for (int u = 0; u < kLaneDims; ++u) o[u] = o[u] * a + w * k[u];
-      m = mx;
-    }
-  }
-  if (lane == 0) sm_m[warp] = m;
-  __syncthreads();
-  float M = p.sink ? p.sink[h] : -INFINITY;
-  for (int w = 0; w < kSimtWarps; ++w) M = fmaxf(M, sm_m[w]);
-  const float f = m == -INFINITY ? 0.f : expf(m - M);
-  if (lane == 0) sm_den[warp] = den * f;
-#pragma unroll
-  for (int u = 0; u < kLaneDims; ++u) o[u] *= f;
-  for (int w = 0; w < kSimtWarps; ++w) {  // in warp order: the sum does not depend on timing
-    if (warp == w) {
-#pragma unroll
-      for (int u = 0; u < kLaneDims; ++u) {
-        const int i = u * 32 + lane;
-        if (i < d) sm_o[i] += o[u];
+  // the cache row of this lane's key of a step, -1: none
+  auto find_row = [&](int step) {
+    const int t = first + step * kGenKeys + lane;
+    if (step >= step1 || t > last) return -1;
+    const int page = table[t / c.page];
+    return page >= 0 && page < c.n_pages ? page * c.page + t % c.page : -1;
+  };
+  int next_row = warp == 0 ? find_row(step0) : -1;
+  constexpr int kAhead = 4;  // loads of a thread on their way together
+  for (int step = step0; step < step1; ++step) {
+    __syncthreads();  // the keys before have been used
+    if (warp == 0) {
+      sm_row[lane] = next_row;
+      const unsigned there = __ballot_sync(0xffffffffu, next_row >= 0);
+      if (lane == 0) {
+        sm_there = there;
+        sm_broken = 0;
       }
     }
     __syncthreads();
-  }
-  float total = p.sink && M != -INFINITY ? expf(p.sink[h] - M) : 0.f;
-  for (int w = 0; w < kSimtWarps; ++w) total += sm_den[w];
-  const bool bad = sm_bad != 0;
-  const float inv = bad ? NAN : (total == 0.f ? 0.f : 1.f / total);
-  const int r0 = d - p.rope_out;
-  for (int i = 2 * threadIdx.x; i < d; i += 2 * blockDim.x) {
-    float x0 = sm_o[i] * inv, x1 = i + 1 < d ? sm_o[i + 1] * inv : 0.f;
-    if (p.rope_cos && i >= r0) {
-      const long long at = static_cast<long long>(row) * (p.rope_out / 2) + (i - r0) / 2;
-      const float cs = p.rope_cos[at], sn = p.rope_sin[at];
-      const float y0 = x0 * cs + x1 * sn, y1 = x1 * cs - x0 * sn;
-      x0 = y0;
-      x1 = y1;
+    if (warp == 0) next_row = find_row(step + 1);
+    // 16 codes at a time
+    for (int i0 = tid; i0 < kGenKeys * units; i0 += kAhead * kGenThreads) {
+      uint4 v[kAhead];
+      uint32_t scale[kAhead];
+      int at[kAhead];
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        const int i = i0 + x * kGenThreads, k = i / units, u = i - k * units;
+        const int r = i < kGenKeys * units ? sm_row[k] : -1;
+        at[x] = i < kGenKeys * units ? (k << 16) | u : -1;
+        v[x] = make_uint4(0, 0, 0, 0);
+        scale[x] = 127;
+        if (r >= 0) {
+          v[x] = __ldg(reinterpret_cast<const uint4*>(c.codes + static_cast<size_t>(r) * c.nope) + u);
+          scale[x] = __ldg(c.scales + static_cast<size_t>(r) * kKvScaleSlots + u / 4);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        if (at[x] < 0) continue;
+        const int k = at[x] >> 16, u = at[x] & 0xFFFF;
+        const float f = e8m0_decode(scale[x]);
+        const uint2 w[4] = {e4m3x4_to_bf16(v[x].x, f), e4m3x4_to_bf16(v[x].y, f),
+                            e4m3x4_to_bf16(v[x].z, f), e4m3x4_to_bf16(v[x].w, f)};
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          odd = odd || special2(w[j].x) || special2(w[j].y);
+          sm_k[k * pitch + 8 * u + 2 * j] = w[j].x;
+          sm_k[k * pitch + 8 * u + 2 * j + 1] = w[j].y;
+        }
+        if (odd) atomicOr(&sm_broken, 1u << k);
+      }
     }
-    const long long at = row * p.out_stride + static_cast<long long>(h) * d + i;
-    store_out(p, at, x0);
-    if (i + 1 < d) store_out(p, at + 1, x1);
+    for (int i0 = tid; i0 < kGenKeys * pairs; i0 += kAhead * kGenThreads) {
+      uint32_t v[kAhead];
+      int at[kAhead];
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        const int i = i0 + x * kGenThreads, k = i / pairs, j = i - k * pairs;
+        const int r = i < kGenKeys * pairs ? sm_row[k] : -1;
+        at[x] = i < kGenKeys * pairs ? (k << 16) | j : -1;
+        v[x] = r < 0 ? 0u
+                     : __ldg(reinterpret_cast<const uint32_t*>(
+                                 c.rope + static_cast<size_t>(r) * c.rope_dim) + j);
+      }
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        if (at[x] < 0) continue;
+        const int k = at[x] >> 16;
+        sm_k[k * pitch + c.nope / 2 + (at[x] & 0xFFFF)] = v[x];
+        if (special2(v[x])) atomicOr(&sm_broken, 1u << k);
+      }
+    }
+    __syncthreads();
+    if (sm_broken) bad = true;  // every key of these is visible
+    const unsigned use = sm_there & ~sm_broken;
+    if (use == 0 || idle) continue;
+    float w[kHeads];
+    {
+      float acc[kHeads][2] = {};
+      const uint32_t* kr = sm_k + lane * pitch;
+      const float2* q = reinterpret_cast<const float2*>(sm_q + warp * kHeads * d);
+#pragma unroll 8
+      for (int j = 0; j < words; ++j) {
+        const uint32_t kw = kr[j];
+        const float x = __uint_as_float(kw << 16), y = __uint_as_float(kw & 0xFFFF0000u);
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+          const float2 qv = q[i * words + j];
+          acc[i][0] = fmaf(qv.x, x, acc[i][0]);
+          acc[i][1] = fmaf(qv.y, y, acc[i][1]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i) {
+        const float x = (use >> lane) & 1u ? (acc[i][0] + acc[i][1]) * p.scale : -INFINITY;
+        const float mx = fmaxf(m[i], warp_max(x));
+        const float a = m[i] == -INFINITY ? 0.f : expf(m[i] - mx);
+        w[i] = x == -INFINITY ? 0.f : expf(x - mx);
+        den[i] = den[i] * a + w[i];
+        if (a != 1.f) {
+#pragma unroll
+          for (int u = 0; u < 2 * kWords; ++u) o[i][u] *= a;
+        }
+        m[i] = mx;
+      }
+    }
+#pragma unroll 2
+    for (int k = 0; k < kGenKeys; ++k) {
+      float wk[kHeads];
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i) wk[i] = __shfl_sync(0xffffffffu, w[i], k);
+      if (!((use >> k) & 1u)) continue;  // (may hold a NaN)
+      const uint32_t* kr = sm_k + k * pitch;
+#pragma unroll
+      for (int u = 0; u < kWords; ++u) {
+        const int j = lane + 32 * u;
+        const uint32_t kw = j < words ? kr[j] : 0u;
+        const float x = __uint_as_float(kw << 16), y = __uint_as_float(kw & 0xFFFF0000u);
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+          o[i][2 * u] = fmaf(wk[i], x, o[i][2 * u]);
+          o[i][2 * u + 1] = fmaf(wk[i], y, o[i][2 * u + 1]);
+        }
+      }
+    }
   }
-  if (p.lse && threadIdx.x == 0)
-    p.lse[static_cast<size_t>(row) * p.H + h] = bad ? NAN : (total == 0.f ? -INFINITY : M + logf(total));
+  // each part's sums where its q was
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    const int hl = warp * kHeads + i;
+    float sum = den[i];
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    if (lane == 0) {
+      sm_m[hl] = m[i];
+      sm_den[hl] = sum;
+    }
+#pragma unroll
+    for (int u = 0; u < kWords; ++u) {
+      const int j = lane + 32 * u;
+      if (j < words)
+        reinterpret_cast<float2*>(sm_q + hl * d)[j] = make_float2(o[i][2 * u], o[i][2 * u + 1]);
+    }
+  }
+  if (tid == 0) sm_bad = bad ? 1.f : 0.f;
+  all_parts();
+  const int r0 = d - p.rope_out;
+  for (int hl = part + parts * warp; hl < kBlockHeads; hl += parts * kGenWarps) {
+    const int h = head0 + hl;
+    if (h >= p.H) break;
+    float pm = -INFINITY, pden = 0.f, pbad = 0.f;  // lane: part
+    if (lane < parts) {
+      pm = ld_part(in_part(&sm_m[hl], lane));
+      pden = ld_part(in_part(&sm_den[hl], lane));
+      pbad = ld_part(in_part(&sm_bad, lane));
+    }
+    const float sink = p.sink ? p.sink[h] : -INFINITY;
+    const float M = fmaxf(warp_max(pm), sink);
+    const float f = pm == -INFINITY ? 0.f : expf(pm - M);
+    float total = pden * f;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
+    if (sink != -INFINITY) total += expf(sink - M);
+    const bool nan = __any_sync(0xffffffffu, pbad != 0.f);
+    const float inv = nan ? NAN : total == 0.f ? 0.f : 1.f / total;
+    for (int j = lane; j < ((words + 31) & ~31); j += 32) {
+      float x0 = 0.f, x1 = 0.f;
+      for (int q = 0; q < parts; ++q) {
+        const float fq = __shfl_sync(0xffffffffu, f, q);
+        if (j < words) {
+          const float2 v = ld_part2(in_part(sm_q + hl * d + 2 * j, q));
+          x0 = fmaf(v.x, fq, x0);
+          x1 = fmaf(v.y, fq, x1);
+        }
+      }
+      if (j >= words) continue;
+      x0 *= inv;
+      x1 *= inv;
+      if (p.rope_cos && 2 * j >= r0) {
+        const long long at = static_cast<long long>(row) * (p.rope_out / 2) + (2 * j - r0) / 2;
+        const float cs = p.rope_cos[at], sn = p.rope_sin[at];
+        const float y0 = x0 * cs + x1 * sn, y1 = x1 * cs - x0 * sn;
+        x0 = y0;
+        x1 = y1;
+      }
+      const long long at = row * p.out_stride + static_cast<long long>(h) * d + 2 * j;
+      store_out(p, at, x0);
+      store_out(p, at + 1, x1);
+    }
+    if (p.lse && lane == 0)
+      p.lse[static_cast<size_t>(row) * p.H + h] = nan ? NAN : total == 0.f ? -INFINITY : M + logf(total);
+  }
+  all_parts();  // nobody leaves while its sums are read
 }
 
 // ===================================================== tensor-core path ==
@@ -1539,6 +1710,53 @@ cudaError_t tc_forward(const PagedAttnProblem& p, void* ws, cudaStream_t st) {
                     dim3(32 * kMergeWarps), 0, st, c);
 }
 
+// Two heads a warp share a key's reads (8 tokens of 64 heads on 2048 keys: 184
+// us, 268 with one head); one where there are no more heads than warps, or so
+// few tokens that more blocks are worth more (1 token: 100 us, 182 with two
+// before the loads were put ahead). The keys are cut until every SM has a
+// block, not below 64 a piece (1 token: 8 pieces, 666 us uncut; cut on to two
+// blocks an SM, 16 tokens take 363 us instead of 341).
+template <int kWords>
+cudaError_t general_launch(const PagedAttnProblem& p, cudaStream_t st) {
+  const int d = p.pages.nope + p.pages.rope_dim, sms = sm_count();
+  const bool one = p.H <= kGenWarps ||
+                   static_cast<long long>(p.total) * ((p.H + 15) / 16) * kGenParts <= sms;
+  auto kernel = one ? paged_attn_general_kernel<1, kWords> : paged_attn_general_kernel<2, kWords>;
+  const int heads = kGenWarps * (one ? 1 : 2), groups = (p.H + heads - 1) / heads;
+  const int keys = p.window > 0 && p.window < p.max_len ? p.window : p.max_len;
+  int parts = 1;
+  while (parts < kGenParts && static_cast<long long>(p.total) * groups * parts < sms &&
+         keys > 2 * kGenKeys * parts)
+    parts *= 2;
+  if (static_cast<long long>(p.total) * parts > 0x7FFFFFFFll) return cudaErrorInvalidValue;
+  auto bytes = [&](int dim) {
+    return sizeof(float) * static_cast<size_t>(heads) * dim + 4 * static_cast<size_t>(kGenKeys) * gen_pitch(dim);
+  };
+  const void* fn = reinterpret_cast<const void*>(kernel);
+  cudaError_t e = set_max_dynamic_smem(fn, static_cast<int>(bytes(64 * kWords)));
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.total * parts, groups);
+  cfg.blockDim = dim3(kGenThreads);
+  cfg.dynamicSmemBytes = bytes(d);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {static_cast<unsigned>(parts), 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p, parts);
+}
+
+// The sums of a lane stay in registers: as many as the dims need, so that small
+// rows do not pay for large ones.
+cudaError_t general_forward(const PagedAttnProblem& p, cudaStream_t st) {
+  const int d = p.pages.nope + p.pages.rope_dim;
+  if (d <= 256) return general_launch<4>(p, st);
+  if (d <= 640) return general_launch<10>(p, st);
+  return d <= kMaxDim ? general_launch<kMaxDim / 64>(p, st) : cudaErrorInvalidValue;
+}
+
 }  // namespace
 
 size_t paged_attn_workspace_bytes(const PagedAttnProblem& p) {
@@ -1550,9 +1768,7 @@ size_t paged_attn_workspace_bytes(const PagedAttnProblem& p) {
 cudaError_t paged_attn_forward(const PagedAttnProblem& p, void* ws, cudaStream_t st) {
   if (p.total <= 0) return cudaSuccess;
   if (tc_shape_ok(p)) return tc_forward(p, ws, st);
-  if (p.pages.nope + p.pages.rope_dim > kMaxDim) return cudaErrorInvalidValue;
-  paged_attn_simt_kernel<<<dim3(p.total, p.H), 32 * kSimtWarps, 0, st>>>(p);
-  return cudaGetLastError();
+  return general_forward(p, st);
 }
 
 }  // namespace dsv4

@@ -590,7 +590,8 @@ size_t dsv4cuda_paged_attn_workspace_bytes(const dsv4cuda_paged *p,
  * 16-byte aligned. workspace may be NULL (a buffer per thread and stream that
  * grows; give one, 256-byte aligned, while capturing). head_dim = 448 + 64
  * with at most 128 heads and strides that are multiples of 8 runs the
- * tensor-core kernel, other shapes (head_dim <= 1024) a general one. A slot
+ * tensor-core kernel, other shapes (head_dim <= 1024, an even rope_dim of the
+ * cache) a general one. A slot
  * beyond max_new or max_len (in the tensor-core kernel also one for which
  * max_keys leaves no room) sets status 4 and gets NaN; rows of q that belong
  * to no slot are left out. */

@@ -456,3 +456,40 @@ def test_tokens_before_the_first_position(cuda, nope, rope):
     assert (c.out[:2] == 0).all() and torch.isneginf(c.lse[:2]).all()
     c.seqs[0] = (5, 3)
     c.check(rows={2, 3, 4, 5})
+
+
+@pytest.mark.parametrize("nope,rope,heads", [(64, 16, 1), (448, 64, 130), (512, 128, 5),
+                                             (512, 512, 17), (64, 2, 40), (64, 0, 9)])
+@pytest.mark.parametrize("seqs", [((1, 1),), ((1, 31), (1, 33)), ((1, 1500),),
+                                  ((40, 100), (0, 5), (3, 300))])
+def test_general_shapes_and_lengths(cuda, nope, rope, heads, seqs):
+    """One token to many, keys in one piece and in several, heads that do not
+    fill their blocks, rows without RoPE values."""
+    c = Case(cuda, list(seqs), heads, page=48, nope=nope, rope=rope, seed=nope + heads)
+    c.use_rope = rope > 0
+    c.run()
+    c.check()
+    a, b = c.out.clone(), c.lse.clone()
+    c.run()
+    assert torch.equal(a, c.out) and torch.equal(b, c.lse)
+
+
+def test_general_shapes_with_windows_and_holes(cuda):
+    c = Case(cuda, [(30, 300), (1, 700), (2, 2)], 20, page=16, window=130, nope=128, rope=32,
+             freed=True, seed=59)
+    c.table[1, 38:41] = -1
+    c.pool.table.copy_(torch.from_numpy(c.table).int())
+    c.run()
+    c.check()
+
+
+def test_odd_rows_are_refused(cuda):
+    cache = cuda.LatentCache.from_tensors(
+        torch.zeros(64, 64, dtype=torch.uint8, device="cuda"),
+        torch.zeros(64, 8, dtype=torch.uint8, device="cuda"),
+        torch.zeros(64, 3, dtype=torch.int16, device="cuda"))
+    pool = cuda.PagedCache.empty([cache], 16, 2, 4)
+    q = torch.zeros(1, 4, 67, device="cuda")
+    with pytest.raises(cuda.Dsv4CudaError, match="odd"):
+        cuda.paged_attn(torch.empty_like(q), q, pool, 0,
+                        torch.zeros(3, dtype=torch.int32, device="cuda"), 1, 16, 1.0)
