@@ -522,9 +522,9 @@ __device__ __forceinline__ void st_global_32(void* p, uint4 a, uint4 b) {
 // values, whose other 8 are lane 4 r + (l - 28)'s for row r. All loads of the
 // 8 rows are on their way before the first is used; a row's codes leave as
 // whole sectors.
-// What bounds it is the latency of its loads at the 24 warps an SM that the
-// registers allow: 147k rows (86 MB read, 151 MB written) in 45 us, 5.3 TB/s;
-// 53 us with blocks in two waves and a unit's rows looked up when it is due.
+// Memory bounds it: 147k rows (86 MB read, 151 MB written) in 42 us, 5.6 TB/s
+// where a copy reaches 6.5; 53 us with blocks in two waves and a unit's rows
+// looked up when it is due, 45 without the prefetch of the next unit's.
 // Rows decoded inside the attention kernel would spare the 151 MB, but the
 // conversions then share the issue slots with the softmax: 153 to 202 us for
 // that call, where decoding ahead took 150 at the time.
@@ -646,6 +646,12 @@ __global__ void __launch_bounds__(kStageThreads, kStageBlocks) stage_kernel(cons
     }
     bad = __reduce_or_sync(0xffffffffu, bad) & there;
     const unsigned keep = there & ~bad;  // the others are zeros: they take part in no sum
+    if (next_row >= 0) {  // the next unit's rows to L2: lane's key, a line of its codes each
+      const uint8_t* at = g.codes + static_cast<size_t>(next_row) * kNope + 128 * (lane >> 3);
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+      if (lane < kUnit)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(g.rope + static_cast<size_t>(next_row) * kRope));
+    }
     uint8_t* dst = reinterpret_cast<uint8_t*>(c.w.stage + u * kUnit * kD) + 32 * lane;
 #pragma unroll
     for (int r = 0; r < kUnit; ++r) {
@@ -1512,10 +1518,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
 // Tiles that a share's end cuts: a warp per (cut, row, half of the dims), 8
 // dims a lane. Everything it reads is asked for as early as its address is
 // known: the plan and the cut's tile, then maxima, sums and the first parts;
-// that chain bounds it (7 us for one tile in 19 parts, 12 for 32 tiles of 64
-// rows in 74 shares, 14 MB of parts).
-constexpr int kMergeWarps = 8;
-__global__ void __launch_bounds__(32 * kMergeWarps) paged_attn_merge_kernel(
+// that chain bounds it, and how many of the blocks, most of which have nothing
+// to merge, run at once (73 cuts, 32 tiles of 64 rows: 7.4 us with four blocks
+// an SM and four parts asked for together, 9.6 with two and eight; one tile in
+// 19 parts: 5.7 and 5.5).
+constexpr int kMergeWarps = 8, kMergeBlocks = 4;  // blocks of an SM
+__global__ void __launch_bounds__(32 * kMergeWarps, kMergeBlocks) paged_attn_merge_kernel(
     const __grid_constant__ TcCall c) {
   pdl_wait();
   pdl_trigger();
@@ -1535,7 +1543,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_attn_merge_kernel(
   auto part = [&](int i) { return static_cast<long long>(cut - 1 + i) * 2 + (i == 0 ? 1 : 0); };
   // dims 4 lane + 128 q of the half: a warp's loads are whole lines
   const float* src = c.w.part_o + half * kHalf + 4 * lane;
-  constexpr int kBatch = 8;
+  constexpr int kBatch = 4;
   float4 v[kBatch][2];
   auto load = [&](int i0) {
 #pragma unroll
@@ -1705,8 +1713,10 @@ cudaError_t tc_forward(const PagedAttnProblem& p, void* ws, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   e = launch_pdl(paged_attn_tc_kernel, dim3(2 * c.s.pairs), dim3(kTcThreads), kTcBytes, st, map, qmap,
                  c);
-  if (e != cudaSuccess || c.s.pairs == 1) return e;
-  return launch_pdl(paged_attn_merge_kernel, dim3(2 * kRows / kMergeWarps, c.s.pairs - 1),
+  const int rows = p.H * (c.s.tokens_per_tile < p.max_new ? c.s.tokens_per_tile : p.max_new);
+  if (e != cudaSuccess || c.s.pairs == 1 || rows <= 0) return e;
+  return launch_pdl(paged_attn_merge_kernel,
+                    dim3((2 * rows + kMergeWarps - 1) / kMergeWarps, c.s.pairs - 1),
                     dim3(32 * kMergeWarps), 0, st, c);
 }
 

@@ -493,3 +493,11 @@ def test_odd_rows_are_refused(cuda):
     with pytest.raises(cuda.Dsv4CudaError, match="odd"):
         cuda.paged_attn(torch.empty_like(q), q, pool, 0,
                         torch.zeros(3, dtype=torch.int32, device="cuda"), 1, 16, 1.0)
+
+
+@pytest.mark.parametrize("nope,rope", [(448, 64), (64, 16)])
+def test_every_slot_beyond(cuda, nope, rope):
+    c = Case(cuda, [(3, 100), (1, 700)], 16, page=16, nope=nope, rope=rope, seed=61)
+    cuda.paged_attn(c.out, c.q, c.pool, 0, c.q_start, 0, 700, c.scale, lse=c.lse)
+    assert c.pool.status() == 4
+    assert torch.isnan(c.out).all() and torch.isnan(c.lse).all()
