@@ -196,3 +196,24 @@ def test_refusals(cuda):
     with pytest.raises(ValueError):
         cuda.token_logprobs(x, t, lp, None, None, top(3)[0], torch.zeros(2, 2, device="cuda"))
     cuda.token_logprobs(x[:0], t[:0], lp[:0])                      # no rows: nothing to do
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,vocab,pad", [(1, V, 0), (48, V, 37), (700, 20011, 0), (9, 1260, 3),
+                                         (1500, 1260, 0), (5, 300, 1)])
+@pytest.mark.parametrize("top", [1, 5, 32])
+def test_few_values_left(cuda, dtype, n, vocab, pad, top):
+    """Masks that leave less than the alternatives asked for: what is masked fills
+    up by its index, NaN among the first values does not."""
+    rng = np.random.default_rng(vocab + top)
+    x = rows(rng, n, vocab, dtype, pad)
+    for r in range(n):
+        left = [0, 1, top - 1, top, top + 1, 40][r % 6]
+        keep = torch.from_numpy(rng.choice(vocab, left, replace=False)).cuda()
+        values = x[r, keep].clone()
+        x[r] = -math.inf
+        if r % 5 == 3:
+            x[r, :250] = math.nan
+        x[r, keep] = values
+    t = torch.from_numpy(rng.integers(0, vocab, n).astype(np.int32)).cuda()
+    check(cuda, x, t, top)
