@@ -113,14 +113,6 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
-// A box of a 3-D map into L2.
-__device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* map, int x, int y, int z) {
-  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(
-                   reinterpret_cast<uint64_t>(map)),
-               "r"(x), "r"(y), "r"(z)
-               : "memory");
-}
-
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
@@ -134,10 +126,10 @@ bool make_tma_map_u8(CUtensorMap* out, const void* base, uint64_t row_bytes, uin
                      uint32_t box_bytes, uint32_t box_rows, bool swizzle128,
                      bool use_cache = true);
 
-// Host: the same over `planes` planes of `rows` rows, plane_pitch bytes
-// apart, with the 128-byte swizzle; not cached.
+// Host: the same over `planes` planes, plane_pitch bytes apart, of `rows` rows,
+// row_pitch bytes apart, with the 128-byte swizzle; not cached.
 bool make_tma_map_u8_3d(CUtensorMap* out, const void* base, uint64_t row_bytes, uint64_t rows,
-                        uint64_t planes, uint64_t plane_pitch, uint32_t box_bytes,
-                        uint32_t box_rows, uint32_t box_planes);
+                        uint64_t row_pitch, uint64_t planes, uint64_t plane_pitch,
+                        uint32_t box_bytes, uint32_t box_rows, uint32_t box_planes);
 
 }  // namespace dsv4

@@ -93,14 +93,14 @@ bool make_tma_map_u8(CUtensorMap* out, const void* base, uint64_t row_bytes, uin
 }
 
 bool make_tma_map_u8_3d(CUtensorMap* out, const void* base, uint64_t row_bytes, uint64_t rows,
-                        uint64_t planes, uint64_t plane_pitch, uint32_t box_bytes,
-                        uint32_t box_rows, uint32_t box_planes) {
+                        uint64_t row_pitch, uint64_t planes, uint64_t plane_pitch,
+                        uint32_t box_bytes, uint32_t box_rows, uint32_t box_planes) {
   auto fn = encode_fn();
   if (!fn || reinterpret_cast<uintptr_t>(base) % 16 != 0 || row_bytes % 16 != 0 ||
-      plane_pitch % 16 != 0 || box_bytes % 16 != 0 || rows == 0 || planes == 0)
+      row_pitch % 16 != 0 || plane_pitch % 16 != 0 || box_bytes % 16 != 0 || rows == 0 || planes == 0)
     return false;
   const cuuint64_t dims[3] = {row_bytes, rows, planes};
-  const cuuint64_t strides[2] = {row_bytes, plane_pitch};
+  const cuuint64_t strides[2] = {row_pitch, plane_pitch};
   const cuuint32_t box[3] = {box_bytes, box_rows, box_planes};
   const cuuint32_t estr[3] = {1, 1, 1};
   return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box,

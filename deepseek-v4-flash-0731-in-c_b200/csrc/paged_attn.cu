@@ -1358,19 +1358,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
             tma_load_3d(smem + kSmOwn + s * 4 * kBlk + b * kQBlk, m, x + b * 128, 0, y,
                         &bars->full_own[s]);
         } else {
-          for (int b = 0; b < 4; ++b)
-            tma_load_2d(smem + kSmOwn + (s * 4 + b) * kBlk, m, x + b * 128, y, &bars->full_own[s]);
+          for (int b = 0; b < 4; b += 2)
+            tma_load_3d(smem + kSmOwn + (s * 4 + b) * kBlk, m, 0, y, x + b, &bars->full_own[s]);
         }
         ++nw;
         return true;
       };
       while (ok && walk.next(seg)) {
-        // the next segment's Q to L2, so that it is near when its room is free
-        if (p.bf16 && walk.F < walk.end) {
-          const int row0 = walk.tiles[walk.t].row0;
-          for (int b = 0; b < 8; ++b) tma_prefetch_3d(&qmap, b * 128, 0, row0);
-        }
-        // Q and the first key blocks are on their way before Q's room is free
+        // Q and the first key blocks are on their way before Q's room is free (2000
+        // tiles: 191 us, 198 with Q's second part behind them)
         if (p.bf16) {
           for (int k = 0; k < 2 && ok; ++k) ok = load_own(&qmap, 256 * k, seg.t.row0, true);
         }
@@ -1384,16 +1380,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
               break;
             }
             mbar_arrive_expect_tx(&bars->full_other[s], 2 * kBlk);
-            for (int b = 0; b < 2; ++b)
-              tma_load_2d(smem + kSmOther + (s * 2 + b) * kBlk, &map,
-                          (1 - half) * 512 + q * 256 + b * 128, y, &bars->full_other[s]);
+            tma_load_3d(smem + kSmOther + s * 2 * kBlk, &map, 0, y, (1 - half) * 4 + q * 2,
+                        &bars->full_other[s]);
           }
           if (!ok) break;
           if (q_due) {
             q_due = false;
             if (!load_q(seg.t)) { ok = false; break; }
           }
-          ok = load_own(&map, half * 512, y, false);
+          ok = load_own(&map, half * 4, y, false);
         }
       }
       // no copy may be in flight when the CTA ends: the last one of each slot
@@ -1695,11 +1690,14 @@ cudaError_t tc_forward(const PagedAttnProblem& p, void* ws, cudaStream_t st) {
   tc_carve(c.s, static_cast<char*>(ws), &c.w);
   if (c.s.block_cap * kKeys > 0x7FFFFFFFll) return cudaErrorInvalidValue;
   CUtensorMap map;
-  if (!make_tma_map_u8(&map, c.w.stage, kD * 2, static_cast<uint64_t>(c.s.block_cap) * kKeys, 128,
-                       kKeys, true, false))
+  // 64 keys x 128 dims a copy: two column blocks of 128 bytes as planes (2000
+  // tiles of three blocks: 203 us, 207 with a copy a column block, and 193
+  // since the next tile's Q is not prefetched to L2 as well)
+  if (!make_tma_map_u8_3d(&map, c.w.stage, 128, static_cast<uint64_t>(c.s.block_cap) * kKeys, kD * 2,
+                          kD / 64, 128, 128, kKeys, 2))
     return cudaErrorInvalidValue;
   CUtensorMap qmap = map;  // not read for fp32 rows
-  if (p.bf16 && !make_tma_map_u8_3d(&qmap, p.q, kD * 2, p.H, p.total, p.q_stride * 2, 128, p.H,
+  if (p.bf16 && !make_tma_map_u8_3d(&qmap, p.q, kD * 2, p.H, kD * 2, p.total, p.q_stride * 2, 128, p.H,
                                     kRows / p.H))
     return cudaErrorInvalidValue;
   const size_t smem = sizeof(int) * 2 * (static_cast<size_t>(p.pages.n_seqs) + 1);
