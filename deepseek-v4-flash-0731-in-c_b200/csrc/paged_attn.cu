@@ -13,6 +13,7 @@
 #include "paged_attn.cuh"
 
 #include <cmath>
+#include <type_traits>
 #include <cuda_bf16.h>
 
 #include "attn.cuh"
@@ -356,11 +357,16 @@ constexpr int kTileCost = 4;
 // A smaller share costs more to merge than it saves (one tile of 32 blocks:
 // 21.7 us, 23.7 with shares from one unit on, 21.8 from four).
 constexpr int kMinShare = 2;
-// A tile of at most this many blocks carries its weights in two BF16 terms:
-// where a row sees few keys, the rounding of one weight does not average out
-// (with one term a two-key row is off by up to 2^-8 of its value sum). Twice
-// the MMAs of P V there: 208 us for 2000 tiles of three blocks, 205 with one
-// term. In longer tiles the sum of many roundings is far below that of one.
+// The weights of P V are BF16, each off by up to 2^-8 of itself. Their sum as
+// P V takes them is kept next to the exact one, and O is multiplied by the
+// ratio: then what is left of the roundings is sum p_t d_t (v_t - o), |d_t| <=
+// 2^-8, which is nothing where one key has the row, whatever its weight (up
+// to 2^8: the running maximum lags), and averages out where many keys share
+// it. lse takes the exact sum. (A sum more in the softmax: 2048 tokens on 11987
+// keys 3684 us, 3640 with the weights off by their rounding.) Where a row sees
+// few keys that is not enough: a tile of at most this many blocks carries its
+// weights in two BF16 terms, at twice the MMAs of P V (2000 tiles of three
+// blocks: 208 us, 205 with one term, in one build).
 constexpr int kTwoTermBlocks = 4;
 constexpr float kLazyMargin = 8.0f;  // log2 units: the running max moves only past this
 
@@ -391,6 +397,7 @@ struct TcWs {
   uint8_t* broken;        // [blocks][8] keys with a NaN or infinity (decoded as zeros)
   float* part_m;          // [pairs][2][2 halves][128] log2 units
   float* part_den;
+  float* part_back;       // what the part's O is multiplied by
   float* part_o;          // [pairs][2][128][512]
   __nv_bfloat16* stage;   // [blocks * 64][512]
 };
@@ -919,16 +926,16 @@ struct PairSync {
 };
 
 // 32 scores of a row (this thread's half of the block's keys) to weights in
-// TMEM. kPlain: every key is visible and one BF16 term is enough. P V of the
-// block before, which reads them there, is waited for when the new ones are
+// TMEM, in one BF16 term or two. P V of the block before, which reads them there, is waited for when the new ones are
 // ready. `rescale`: O (and what was summed before) is to be
 // multiplied by alpha.
 struct RowState {
   float m, den;
+  float held;  // the sum of the weights as P V takes them
 };
-template <bool kPlain, class WaitPv>
-__device__ __forceinline__ bool softmax_block(uint32_t s_col, uint32_t mask, bool two_terms,
-                                              float sc2, float* max_mine, const float* max_other,
+template <bool kMasked, bool kTwoTerms, class WaitPv>
+__device__ __forceinline__ bool softmax_block(uint32_t s_col, uint32_t mask, float sc2,
+                                              float* max_mine, const float* max_other,
                                               PairSync& meet, bool& good, RowState& st,
                                               float& alpha, uint32_t p_col, uint64_t* s_free,
                                               WaitPv wait_pv) {
@@ -939,7 +946,7 @@ __device__ __forceinline__ bool softmax_block(uint32_t s_col, uint32_t mask, boo
   float tm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
-    if (!kPlain && !((mask >> i) & 1u)) r[i] = 0xFF800000u;
+    if (kMasked && !((mask >> i) & 1u)) r[i] = 0xFF800000u;
     tm[i & 3] = fmaxf(tm[i & 3], __uint_as_float(r[i]));
   }
   const float mine = fmaxf(fmaxf(tm[0], tm[1]), fmaxf(tm[2], tm[3]));
@@ -960,39 +967,28 @@ __device__ __forceinline__ bool softmax_block(uint32_t s_col, uint32_t mask, boo
     }
   }
   const float neg = st.m == -INFINITY ? 0.f : -st.m;
-  float part[4] = {0.f, 0.f, 0.f, 0.f};
-  if (kPlain) {
+  float part[4] = {0.f, 0.f, 0.f, 0.f}, held[2] = {0.f, 0.f};
+  uint32_t less[16];  // what the rounding left
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      const float e0 = ex2_approx(fmaf(__uint_as_float(r[i]), sc2, neg));
-      const float e1 = ex2_approx(fmaf(__uint_as_float(r[i + 1]), sc2, neg));
-      part[(i >> 1) & 3] += e0 + e1;
-      r[i / 2] = pack_bf16x2(e0, e1);
-    }
-    good = wait_pv() && good;
-    __syncwarp();
-    tc_fence_after();
-    tmem_st16(p_col, r);
-  } else {
-    uint32_t less[16];  // what the rounding left
-#pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      const float e0 = ex2_approx(fmaf(__uint_as_float(r[i]), sc2, neg));
-      const float e1 = ex2_approx(fmaf(__uint_as_float(r[i + 1]), sc2, neg));
-      part[(i >> 1) & 3] += e0 + e1;
-      const uint32_t h = pack_bf16x2(e0, e1);
-      less[i / 2] =
-          pack_bf16x2(e0 - __uint_as_float(h << 16), e1 - __uint_as_float(h & 0xFFFF0000u));
-      r[i / 2] = h;
-    }
-    good = wait_pv() && good;
-    __syncwarp();
-    tc_fence_after();
-    tmem_st16(p_col, r);
-    if (two_terms) tmem_st16(p_col + kKeys / 2, less);
+  for (int i = 0; i < 32; i += 2) {
+    const float e0 = ex2_approx(fmaf(__uint_as_float(r[i]), sc2, neg));
+    const float e1 = ex2_approx(fmaf(__uint_as_float(r[i + 1]), sc2, neg));
+    part[(i >> 1) & 3] += e0 + e1;
+    const uint32_t h = pack_bf16x2(e0, e1);
+    const float h0 = __uint_as_float(h << 16), h1 = __uint_as_float(h & 0xFFFF0000u);
+    if (kTwoTerms) less[i / 2] = pack_bf16x2(e0 - h0, e1 - h1);
+    else held[(i >> 1) & 1] += h0 + h1;
+    r[i / 2] = h;
   }
+  good = wait_pv() && good;
+  __syncwarp();
+  tc_fence_after();
+  tmem_st16(p_col, r);
+  if (kTwoTerms) tmem_st16(p_col + kKeys / 2, less);
   tmem_st_wait();
-  st.den = st.den * alpha + ((part[0] + part[1]) + (part[2] + part[3]));
+  const float sum = (part[0] + part[1]) + (part[2] + part[3]);
+  st.den = st.den * alpha + sum;
+  if (!kTwoTerms) st.held = st.held * alpha + (held[0] + held[1]);
   return rescale;
 }
 
@@ -1012,6 +1008,8 @@ __device__ __forceinline__ bool softmax_block(uint32_t s_col, uint32_t mask, boo
 // blocks ahead instead of one: where the rows come from DRAM that is what
 // counts (32 sequences of 4.6k keys: 55 us of 64; keys that L2 holds: 2% more
 // than with P in shared memory and two buffers of S).
+// kShort: no tile has more than kTwoTermBlocks blocks.
+template <bool kShort>
 __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
     const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap qmap,
     const __grid_constant__ TcCall c) {
@@ -1095,8 +1093,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
       const bool mine = tok < t.tokens;
       const int last = mine ? t.pos0 + tok : -1;  // the position of this row's token
       const int from = p.window > 0 ? max(0, last - p.window + 1) : 0;
-      const bool two_terms = t.blocks <= kTwoTermBlocks;
-      RowState st = {-INFINITY, 0.f};
+      const bool two_terms = kShort || t.blocks <= kTwoTermBlocks;
+      RowState st = {-INFINITY, 0.f, 0.f};
       bool bad = t.bad != 0;
       const unsigned long long* valid =
           reinterpret_cast<const unsigned long long*>(c.w.valid) + t.block0;
@@ -1114,9 +1112,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
         // a block that every row sees whole needs no mask
         const int hi_key = last - key0, lo_key = from - key0;
         const bool whole = hi_key >= kKeys - 1 && lo_key <= 0 && mask == ~0ull && broken == 0;
-        const bool plain = __all_sync(0xffffffffu, whole) && !two_terms;
+        const bool masked = two_terms || !__all_sync(0xffffffffu, whole);
         uint32_t mask32 = ~0u;
-        if (!plain) {
+        if (masked) {
           // bits 0 .. last - key0, and from the window's first on
           mask &= hi_key < 0 ? 0ull : hi_key >= 63 ? ~0ull : (2ull << hi_key) - 1;
           if (lo_key > 0) mask &= lo_key > 63 ? 0ull : ~0ull << lo_key;
@@ -1135,12 +1133,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
         auto wait_pv = [&] {
           return n == 0 || long_wait(&bars->pv_done, (n - 1) & 1, abort_flag, err);
         };
-        const bool rescale =
-            plain ? softmax_block<true>(s_col, mask32, false, sc2, max_mine + buf, max_other + buf,
-                                        meet, good, st, alpha, p_col, &bars->s_free, wait_pv)
-                  : softmax_block<false>(s_col, mask32, two_terms, sc2, max_mine + buf,
-                                         max_other + buf, meet, good, st, alpha, p_col,
-                                         &bars->s_free, wait_pv);
+        auto softmax = [&](auto m, auto two) {
+          return softmax_block<m.value, two.value>(s_col, mask32, sc2, max_mine + buf,
+                                                   max_other + buf, meet, good, st, alpha, p_col,
+                                                   &bars->s_free, wait_pv);
+        };
+        bool rescale;
+        if constexpr (kShort)
+          rescale = softmax(std::true_type(), std::true_type());
+        else
+          rescale = !masked     ? softmax(std::false_type(), std::false_type())
+                    : two_terms ? softmax(std::true_type(), std::true_type())
+                                : softmax(std::true_type(), std::false_type());
         if (!__all_sync(0xffffffffu, good)) {
           ok = false;
           break;
@@ -1161,13 +1165,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
         mbar_arrive(&bars->p_full);
       }
       if (!ok) break;
-      // the row's denominator: both threads' sums (the buffer of the block
-      // before the last one is free)
-      const int buf = (n & 1) * 2 * kRows;
+      // the row's denominators: both threads' sums (the buffer of the block
+      // before the last one is free, the last one's once both have been here)
+      const int buf = (n & 1) * 2 * kRows, buf_held = 2 * kRows - buf;
       max_mine[buf] = st.den;
       bool good = meet();
       float den = st.den + max_other[buf];
+      if (!two_terms) max_mine[buf_held] = st.held;
       good = meet() && good;  // read before the next segment writes it
+      // O has the weights as P V took them: times this, they sum to den
+      float back = 1.f;
+      if (!two_terms) {
+        const float held = st.held + max_other[buf_held];
+        if (held > 0.f) back = den / held;
+      }
       // the segment before is out, so its factors may be overwritten
       if (segs > 0) good = long_wait(&bars->o_free, (segs - 1) & 1, abort_flag, err) && good;
       ++segs;
@@ -1179,7 +1190,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
       if (seg.j0 == 0 && seg.j1 == t.blocks) {
         const Norm norm = finish(st.m, den, sink2);
         if (side == 0) {
-          reinterpret_cast<float*>(smem + kSmScale)[row] = norm.scale;
+          reinterpret_cast<float*>(smem + kSmScale)[row] = norm.scale * back;
           if (mine && half == 0 && p.lse)
             p.lse[static_cast<long long>(t.row0 + tok) * p.H + h] = norm.lse;
         }
@@ -1187,6 +1198,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
         const long long at = pair * 2 + part_slot(t, share0);
         c.w.part_m[(at * 2 + half) * kRows + row] = st.m;
         c.w.part_den[(at * 2 + half) * kRows + row] = den;
+        c.w.part_back[(at * 2 + half) * kRows + row] = back;
       }
       mbar_arrive(&bars->o_ready);
     }
@@ -1464,7 +1476,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
             if (++sv == kOwnStages) sv = 0;
           }
         }
-        const bool two_terms = seg.t.blocks <= kTwoTermBlocks;
+        const bool two_terms = kShort || seg.t.blocks <= kTwoTermBlocks;
         bool ready = false;
         for (int j = seg.j0; j < seg.j1; ++j, ++n) {
           // the softmax has read the scores of the block before
@@ -1551,13 +1563,14 @@ __global__ void __launch_bounds__(32 * kMergeWarps, kMergeBlocks) paged_attn_mer
   };
   load(0);
   constexpr int kPer = 3;  // a lane's parts: lane, lane + 32, lane + 64 of at most 96
-  float wt[kPer], m[kPer], d[kPer], M = -INFINITY;
+  float wt[kPer], m[kPer], d[kPer], back[kPer], M = -INFINITY;
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
     const int i = lane + 32 * k;
     const long long at = (part(i) * 2 + half) * kRows + row;
     m[k] = i < n ? __ldcg(c.w.part_m + at) : -INFINITY;
     d[k] = i < n ? __ldcg(c.w.part_den + at) : 0.f;
+    back[k] = i < n ? __ldcg(c.w.part_back + at) : 0.f;
     M = fmaxf(M, m[k]);
   }
   M = warp_max(M);
@@ -1568,6 +1581,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps, kMergeBlocks) paged_attn_mer
     den += d[k] * wt[k];
     // a part that saw a broken latent and nothing else has no maximum
     if (d[k] != d[k]) den = NAN;
+    wt[k] *= back[k];
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
@@ -1657,6 +1671,20 @@ TcShape tc_shape(const PagedAttnProblem& p) {
   return s;
 }
 
+// No tile sees more than kTwoTermBlocks blocks: n positions from any on touch
+// at most (n + 62) / 64 + 1. They take a kernel of their own, without the code
+// of one-term weights: 2000 tiles of three blocks 187 us, 200 in the kernel that
+// has both.
+bool short_tiles(const PagedAttnProblem& p, const TcShape& s) {
+  long long n = p.max_len;
+  if (p.window > 0) {
+    const long long most =
+        p.window - 1ll + (s.tokens_per_tile < p.max_new ? s.tokens_per_tile : p.max_new);
+    if (most < n) n = most;
+  }
+  return (n + kKeys - 2) / kKeys + 1 <= kTwoTermBlocks;
+}
+
 size_t up(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
 
 size_t tc_carve(const TcShape& s, char* base, TcWs* w) {
@@ -1674,6 +1702,7 @@ size_t tc_carve(const TcShape& s, char* base, TcWs* w) {
   w->broken = reinterpret_cast<uint8_t*>(take(8 * blocks));
   w->part_m = reinterpret_cast<float*>(take(sizeof(float) * pairs * 4 * kRows));
   w->part_den = reinterpret_cast<float*>(take(sizeof(float) * pairs * 4 * kRows));
+  w->part_back = reinterpret_cast<float*>(take(sizeof(float) * pairs * 4 * kRows));
   w->part_o = reinterpret_cast<float*>(take(sizeof(float) * pairs * 2 * kRows * kD));
   w->stage = reinterpret_cast<__nv_bfloat16*>(take(2 * blocks * kKeys * kD));
   return off;
@@ -1707,9 +1736,10 @@ cudaError_t tc_forward(const PagedAttnProblem& p, void* ws, cudaStream_t st) {
   cudaError_t e = launch_pdl(stage_kernel, dim3(1 + static_cast<unsigned>(units < most ? units : most)),
                              dim3(kStageThreads), smem, st, c);
   if (e != cudaSuccess) return e;
-  e = set_max_dynamic_smem(reinterpret_cast<const void*>(paged_attn_tc_kernel), kTcBytes);
+  auto attn = short_tiles(p, c.s) ? paged_attn_tc_kernel<true> : paged_attn_tc_kernel<false>;
+  e = set_max_dynamic_smem(reinterpret_cast<const void*>(attn), kTcBytes);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(paged_attn_tc_kernel, dim3(2 * c.s.pairs), dim3(kTcThreads), kTcBytes, st, map, qmap,
+  e = launch_pdl(attn, dim3(2 * c.s.pairs), dim3(kTcThreads), kTcBytes, st, map, qmap,
                  c);
   const int rows = p.H * (c.s.tokens_per_tile < p.max_new ? c.s.tokens_per_tile : p.max_new);
   if (e != cudaSuccess || c.s.pairs == 1 || rows <= 0) return e;
