@@ -1720,7 +1720,7 @@ DSV4_API int dsv4cuda_paged_fork(const dsv4cuda_paged* p, const int* dst, const 
                                  void* stream) {
   dsv4::PagedState s;
   if (!paged_state("dsv4cuda_paged_fork", p, &s)) return -1;
-  if (n < 0 || n > p->n_seqs || (n > 0 && (!dst || !src))) {
+  if (n < 0 || n > p->n_seqs || (n > 0 && !dst)) {
     record_error("dsv4cuda_paged_fork: bad arguments (at most one op per slot)");
     return -1;
   }

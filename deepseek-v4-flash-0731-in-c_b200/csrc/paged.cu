@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(kMetaThreads) fork_kernel(const __grid_constan
     const int i = base + threadIdx.x;
     int need = 0, state = -2;
     if (i < n) {
-      const int d = dst[i], s = src[i];
+      const int d = dst[i], s = src ? src[i] : -1;
       bool ok = in_range(d, p.n_seqs) && s >= -1 && s < p.n_seqs && owner[d] == i;
       // a source that another op replaces is no longer what was asked for
       if (ok && s >= 0 && s != d && owner[s] != INT_MAX && src[owner[s]] != s) ok = false;
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(kMetaThreads) fork_kernel(const __grid_constan
   for (int i = warp; i < n; i += nw) {
     const int r = rank[i];
     if (r == -2) continue;
-    const int d = dst[i], s = src[i];
+    const int d = dst[i], s = src ? src[i] : -1;
     if (s < 0 || r >= got) {  // emptied, or no page left for it
       if (lane == 0) {
         p.length[d] = 0;

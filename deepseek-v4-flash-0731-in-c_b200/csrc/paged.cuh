@@ -31,7 +31,8 @@ struct PagedState {
 
 size_t paged_workspace_bytes(int n_pages, int n_seqs);
 
-// Slot dst[i] takes the place of a copy of slot src[i] (-1: emptied).
+// Slot dst[i] takes the place of a copy of slot src[i] (-1, or src null:
+// emptied).
 cudaError_t paged_fork(const PagedState& p, const int* dst, const int* src, int n,
                        cudaStream_t st);
 // Slot slots[i] grows by counts[i] tokens; rows (may be null) receives the

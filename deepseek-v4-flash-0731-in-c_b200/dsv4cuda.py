@@ -711,8 +711,8 @@ class PagedCache:
 
     def free(self, slots, stream=None):
         """Gives back the pages of `slots`."""
-        import torch
-        self.fork(slots, torch.full_like(slots, -1), stream)
+        _check(lib.dsv4cuda_paged_fork(self._ref, _dev(slots, "slots", self._i32), None,
+                                       slots.shape[0], _stream(stream)))
 
     def compact(self, table_out=None, refs_out=None, stream=None):
         """Moves the pages in use to the lowest page numbers; the new tables go to

@@ -535,7 +535,7 @@ typedef struct {
 
 size_t dsv4cuda_paged_workspace_bytes(int n_pages, int n_seqs);
 /* Fork and free: for i < n, slot dst[i] gives back its pages and takes the
- * place of a copy of slot src[i] (-1: it is emptied; dst[i] itself: it stays):
+ * place of a copy of slot src[i] (-1, or src NULL: it is emptied; dst[i] itself: it stays):
  * full pages are shared, the used rows of a partial last page are copied, in
  * every layer, into the lowest free pages (an op is counted before a later
  * one). All sources are read as they were before the call. An op that finds
