@@ -741,6 +741,9 @@ def _paged_attn_shape(q, out, max_new, max_len, scale, window, rope_cos, max_key
     qs, os_ = q.stride(), out.stride()
     if qs[2] != 1 or os_[2] != 1 or (heads > 1 and (qs[1] != d or os_[1] != d)):
         raise ValueError("q and out: the heads of a row must lie one behind the other")
+    # (0, an expanded row, would be the call's word for heads * head_dim)
+    if n > 1 and min(qs[0], os_[0]) < heads * d:
+        raise ValueError("q and out: the rows must not overlap")
     # the stride of a single row has no meaning to torch, nor here
     return PagedAttnShape(n, heads, d, 1 if bf16 else 0, qs[0] if n > 1 else 0,
                           os_[0] if n > 1 else 0, max_new, max_len, window, max_keys,

@@ -71,3 +71,30 @@ def test_free_reads_nothing_that_another_stream_writes(calls, pool):
     slots = Fake([3], torch.int32)
     pool.free(slots, stream=77)
     assert calls == [("dsv4cuda_paged_fork", (pool._ref, slots.address, None, 3, 77))]
+
+
+def attn(pool, q, out, **kw):
+    dsv4cuda.paged_attn(out, q, pool, 0, Fake([pool.n_seqs + 1], torch.int32), 4, 64, 1.0,
+                        stream=77, **kw)
+
+
+@pytest.mark.parametrize("stride", [0, 4 * 512 - 8])
+@pytest.mark.parametrize("which", ["q", "out"])
+def test_rows_that_overlap_are_refused(calls, pool, which, stride):
+    """One row expanded to several, or rows that begin inside the one before."""
+    whole, over = Fake([3, 4, 512], torch.bfloat16), \
+        Fake([3, 4, 512], torch.bfloat16, (stride, 512, 1))
+    with pytest.raises(ValueError, match="overlap"):
+        attn(pool, *((over, whole) if which == "q" else (whole, over)))
+    if which == "q":
+        with pytest.raises(ValueError, match="overlap"):
+            dsv4cuda.paged_attn_workspace_bytes(over, pool, 4, 64)
+    assert not calls
+
+
+def test_the_stride_of_a_single_row_does_not_matter(calls, pool):
+    one = Fake([1, 4, 512], torch.bfloat16, (0, 512, 1))
+    attn(pool, one, Fake([1, 4, 512], torch.bfloat16))
+    apart = Fake([3, 4, 512], torch.bfloat16, (4 * 512 + 8, 512, 1))
+    attn(pool, apart, Fake([3, 4, 512], torch.bfloat16))
+    assert len(calls) == 2
