@@ -774,8 +774,7 @@ def paged_attn(out, q, paged: PagedCache, layer, q_start, max_new, max_len, scal
         _dev(q_start, "q_start", torch.int32, paged.n_seqs + 1), _dev(sink, "sink", f32, heads),
         _dev(rope_cos, "rope_cos", f32, half), _dev(rope_sin, "rope_sin", f32, half),
         _dev(lse, "lse", f32, n * heads), C.byref(shape),
-        None if workspace is None else workspace.data_ptr(),
-        0 if workspace is None else workspace.numel() * workspace.element_size(),
+        _dev(workspace, "workspace", torch.uint8), 0 if workspace is None else workspace.numel(),
         _stream(stream)))
 
 

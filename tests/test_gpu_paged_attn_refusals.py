@@ -32,3 +32,12 @@ def test_expanded_rows(call):
             call(**kw)
     assert (one == 1).all()
     assert (call() == 0).all()                  # still usable
+
+
+def test_a_workspace_that_is_none(call):
+    for ws in (torch.empty(1 << 24, dtype=torch.uint8),
+               torch.empty(1 << 22, dtype=torch.float32, device="cuda"),
+               torch.empty(1 << 25, dtype=torch.uint8, device="cuda")[::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            call(workspace=ws)
+    assert (call(workspace=torch.empty(1 << 24, dtype=torch.uint8, device="cuda")) == 0).all()

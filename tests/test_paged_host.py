@@ -98,3 +98,17 @@ def test_the_stride_of_a_single_row_does_not_matter(calls, pool):
     apart = Fake([3, 4, 512], torch.bfloat16, (4 * 512 + 8, 512, 1))
     attn(pool, apart, Fake([3, 4, 512], torch.bfloat16))
     assert len(calls) == 2
+
+
+@pytest.mark.parametrize("workspace", [
+    torch.empty(1 << 20, dtype=torch.uint8),                        # not on the GPU
+    Fake([1 << 20], torch.float32), Fake([1 << 20], torch.int8),
+    Fake([1 << 20], torch.uint8, (2,))], ids=["host", "fp32", "int8", "every other byte"])
+def test_a_workspace_that_is_none(calls, pool, workspace):
+    q = Fake([3, 4, 512], torch.bfloat16)
+    with pytest.raises(ValueError, match="workspace"):
+        attn(pool, q, q, workspace=workspace)
+    assert not calls
+    good = Fake([1 << 20], torch.uint8, address=1 << 30)
+    attn(pool, q, q, workspace=good)
+    assert calls[0][1][-3:] == (1 << 30, 1 << 20, 77)
