@@ -311,8 +311,10 @@ __global__ void __launch_bounds__(kMetaThreads) append_kernel(const __grid_const
   }
 }
 
-// The cache row of each new token: a thread per token finds its op by a
-// search in shared memory (the ops' starts are loaded once a block; in global
+// The cache row of each new token, -1 behind the last one (a captured step has
+// rows for the most tokens that it may bring, and what it does not bring must
+// not be written where the step before had its own): a thread per token finds
+// its op by a search in shared memory (the ops' starts are loaded once a block; in global
 // memory every probe costs an L2 access), 54,000 tokens of 48 ops in 3.4 us.
 __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ PagedState p,
                                                    const int* __restrict__ slots, int n,
@@ -322,15 +324,15 @@ __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ Paged
   const Ws w = carve(p.ws, p.n_pages, p.n_seqs);
   for (int i = threadIdx.x; i <= n; i += 256) first[i] = w.first[i];
   __syncthreads();
-  const long long total = min(first[n], n_rows);
-  for (long long t = blockIdx.x * 256ll + threadIdx.x; t < total; t += gridDim.x * 256ll) {
+  const long long total = first[n];
+  for (long long t = blockIdx.x * 256ll + threadIdx.x; t < n_rows; t += gridDim.x * 256ll) {
     int lo = 0, hi = n;  // the last op with first <= t
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (first[mid] <= t) lo = mid;
       else hi = mid;
     }
-    const int len = w.jobs[lo].src;
+    const int len = t < total ? w.jobs[lo].src : -1;
     long long row = -1;
     if (len >= 0) {
       const int pos = len + static_cast<int>(t - first[lo]);
@@ -548,7 +550,9 @@ cudaError_t paged_fork(const PagedState& p, const int* dst, const int* src, int 
 
 cudaError_t paged_append(const PagedState& p, const int* slots, const int* counts, int n,
                          long long* rows, long long n_rows, cudaStream_t st) {
-  if (n <= 0) return cudaSuccess;
+  if (n <= 0)
+    return rows && n_rows > 0 ? cudaMemsetAsync(rows, 0xFF, sizeof(long long) * n_rows, st)
+                              : cudaSuccess;
   const size_t smem = sizeof(int) * (static_cast<size_t>(p.n_seqs) + static_cast<size_t>(n));
   cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(append_kernel),
                                        sizeof(int) * 2 * kPagedMaxSeqs);

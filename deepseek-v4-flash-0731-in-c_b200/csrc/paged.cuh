@@ -36,7 +36,7 @@ size_t paged_workspace_bytes(int n_pages, int n_seqs);
 cudaError_t paged_fork(const PagedState& p, const int* dst, const int* src, int n,
                        cudaStream_t st);
 // Slot slots[i] grows by counts[i] tokens; rows (may be null) receives the
-// cache rows of the new tokens, op after op.
+// cache rows of the new tokens, op after op, and -1 behind them.
 cudaError_t paged_append(const PagedState& p, const int* slots, const int* counts, int n,
                          long long* rows, long long n_rows, cudaStream_t st);
 // Pages in use move to the lowest page numbers; table_out / refs_out may be

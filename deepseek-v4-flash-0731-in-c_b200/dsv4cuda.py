@@ -697,7 +697,7 @@ class PagedCache:
 
     def append(self, slots, counts, rows=None, stream=None):
         """Slots grow by counts tokens (int32 CUDA tensors); rows (int64) receives
-        the new tokens' cache rows, as LatentCache.write takes them."""
+        the new tokens' cache rows, as LatentCache.write takes them, and -1 behind them."""
         n = slots.shape[0]
         _check(lib.dsv4cuda_paged_append(
             self._ref, _dev(slots, "slots", self._i32), _dev(counts, "counts", self._i32, n), n,
