@@ -249,13 +249,18 @@ __global__ void __launch_bounds__(kMetaThreads) append_kernel(const __grid_const
   pdl_trigger();
   claim(p, slots, n, owner);
   int needs = 0;
+  long long out = 0;  // tokens of the ops before: where an op's rows begin
   for (int base = 0; base < n; base += blockDim.x) {
     const int i = base + threadIdx.x;
     int need = 0;
     bool ok = false;
+    long long tokens;
+    const long long begin = out + block_scan(i < n ? max(counts[i], 0) + 0ll : 0ll, &tokens);
+    out += tokens;
     if (i < n) {
       const int s = slots[i], c = counts[i];
-      ok = in_range(s, p.n_seqs) && c >= 0 && owner[s] == i;
+      w.first[i] = begin;
+      ok = in_range(s, p.n_seqs) && c >= 0 && owner[s] == i && (!rows || begin + c <= n_rows);
       if (ok) {
         const int len = p.length[s], cap = p.max_pages * p.page;
         ok = len >= 0 && len <= cap && c <= cap - len;
@@ -296,19 +301,7 @@ __global__ void __launch_bounds__(kMetaThreads) append_kernel(const __grid_const
     }
     if (lane == 0) w.jobs[i].src = len;
   }
-  // tokens of the ops before each: where their rows go
-  long long out = 0;
-  for (int base = 0; base < n; base += blockDim.x) {
-    const int i = base + threadIdx.x;
-    long long total;
-    const long long r = block_scan(i < n ? max(counts[i], 0) + 0ll : 0ll, &total);
-    if (i < n) w.first[i] = out + r;
-    out += total;
-  }
-  if (threadIdx.x == 0) {
-    w.first[n] = out;
-    if (rows && out > n_rows) raise(p, kPagedBadOp);
-  }
+  if (threadIdx.x == 0) w.first[n] = out;
 }
 
 // The cache row of each new token, -1 behind the last one (a captured step has

@@ -698,10 +698,13 @@ class PagedCache:
     def append(self, slots, counts, rows=None, stream=None):
         """Slots grow by counts tokens (int32 CUDA tensors); rows (int64) receives
         the new tokens' cache rows, as LatentCache.write takes them, and -1 behind them."""
-        n = slots.shape[0]
+        n, at, n_rows = slots.shape[0], _dev(rows, "rows", self._i64), 0
+        if rows is not None:
+            n_rows = rows.numel()
+            at = at or self.workspace.data_ptr()  # no rows: a place that is not NULL
         _check(lib.dsv4cuda_paged_append(
             self._ref, _dev(slots, "slots", self._i32), _dev(counts, "counts", self._i32, n), n,
-            _dev(rows, "rows", self._i64), 0 if rows is None else rows.numel(), _stream(stream)))
+            at, n_rows, _stream(stream)))
 
     def fork(self, dst, src, stream=None):
         """Slots dst become copies of slots src (-1: emptied); int32 CUDA tensors."""

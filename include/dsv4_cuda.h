@@ -546,9 +546,10 @@ int dsv4cuda_paged_fork(const dsv4cuda_paged *p, const int *dst, const int *src,
 /* Append: slot slots[i] grows by counts[i] tokens, taking the lowest free
  * pages. rows [n_rows] (may be NULL) receives the cache rows of the new
  * tokens, op after op, as dsv4cuda_kv_write takes them. An op that does not
- * find its pages changes nothing (status 1), nor does a bad op (status 2);
- * the rows of their tokens are -1, which dsv4cuda_kv_write skips, and so are
- * those behind the last token. */
+ * find its pages changes nothing (status 1), nor does a bad op, one whose
+ * tokens do not all have a row among them (status 2); the rows of their tokens
+ * are -1, which dsv4cuda_kv_write skips, and so are those behind the last
+ * token. */
 int dsv4cuda_paged_append(const dsv4cuda_paged *p, const int *slots, const int *counts, int n,
                           long long *rows, long long n_rows, void *stream);
 /* Compact: the pages in use move to page numbers 0 .. (pages in use) - 1 with

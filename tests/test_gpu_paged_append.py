@@ -49,3 +49,25 @@ def test_a_captured_step_brings_fewer_tokens_than_before(cuda):
         g.replay()
         assert rows.tolist() == want
     assert pool.status() == 0
+
+
+def test_tokens_beyond_the_rows_are_refused(cuda):
+    """An op whose tokens have no room in rows changes nothing."""
+    pool = pool_of(cuda)
+    pool.append(dev([0]), dev([6]))
+    rows = rows_of(8)
+    pool.append(dev([0, 1, 2, 3]), dev([3, 4, 2, 0]), rows)     # 9 tokens, the last 2 too many
+    assert rows.tolist() == [6, 7, 8, 12, 13, 14, 15, -1]
+    assert pool.length.tolist() == [9, 4, 0, 0]
+    assert pool.table.tolist() == [[0, 1, 2, -1], [3, -1, -1, -1], [-1] * 4, [-1] * 4]
+    assert pool.refs.tolist() == [1] * 4 + [0] * 12
+    assert pool.status() == pool.BAD_OP
+    # an op that is left out for another reason has its place in rows all the same
+    rows = rows_of(4)
+    pool.append(dev([2, 9, 3]), dev([1, 2, 2]), rows)
+    assert rows.tolist() == [16, -1, -1, -1]
+    assert pool.length.tolist() == [9, 4, 1, 0] and pool.status() == pool.BAD_OP
+    pool.append(dev([3]), dev([1]), torch.empty(0, dtype=torch.int64, device="cuda"))
+    assert pool.length.tolist() == [9, 4, 1, 0] and pool.status() == pool.BAD_OP
+    pool.append(dev([3]), dev([1]))                             # no rows wanted: no limit
+    assert pool.length.tolist() == [9, 4, 1, 1] and pool.status() == 0
