@@ -9,6 +9,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <new>
 #include <string>
 #include <vector>
 #include <atomic>
@@ -1558,14 +1559,34 @@ DSV4_API int dsv4cuda_accept_device(const int* proposal, int proposed, const flo
 namespace {
 
 // Buffers for attention calls that bring no workspace: one per stream, so
-// that calls on several streams of a thread do not share one.
+// that calls on several streams of a thread do not share one. They go with
+// their thread, whose end must not disturb a capture that another thread has
+// under way.
 struct StreamScratch {
   int device;
   cudaStream_t stream;
   char* buf;
   size_t cap;
+  StreamScratch* next;
 };
-thread_local std::vector<StreamScratch> t_scratch;
+struct StreamScratchList {
+  StreamScratch* first = nullptr;
+  void release() {
+    while (first) {
+      StreamScratch* s = first;
+      first = s->next;
+      if (s->buf) cudaFree(s->buf);
+      delete s;
+    }
+  }
+  ~StreamScratchList() {
+    if (!first) return;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    release();
+  }
+};
+thread_local StreamScratchList t_scratch;
 
 // nullptr with the error recorded when there is none to be had.
 char* stream_scratch(const char* who, size_t bytes, cudaStream_t st) {
@@ -1579,11 +1600,12 @@ char* stream_scratch(const char* who, size_t bytes, cudaStream_t st) {
     return nullptr;
   }
   StreamScratch* s = nullptr;
-  for (auto& x : t_scratch)
-    if (x.device == dev && x.stream == st) s = &x;
+  for (StreamScratch* x = t_scratch.first; x; x = x->next)
+    if (x->device == dev && x->stream == st) s = x;
   if (!s) {
-    t_scratch.push_back({dev, st, nullptr, 0});
-    s = &t_scratch.back();
+    s = new (std::nothrow) StreamScratch{dev, st, nullptr, 0, t_scratch.first};
+    if (!s) { record_error("%s: out of host memory", who); return nullptr; }
+    t_scratch.first = s;
   }
   if (bytes > s->cap) {
     if (s->buf) cudaFree(s->buf);
@@ -1601,11 +1623,7 @@ char* stream_scratch(const char* who, size_t bytes, cudaStream_t st) {
   return s->buf;
 }
 
-void free_stream_scratch() {
-  for (auto& x : t_scratch)
-    if (x.buf) cudaFree(x.buf);
-  t_scratch.clear();
-}
+void free_stream_scratch() { t_scratch.release(); }
 
 // Checks the description and fills the kernels' form; false with the error
 // recorded.

@@ -590,7 +590,9 @@ size_t dsv4cuda_paged_attn_workspace_bytes(const dsv4cuda_paged *p,
  * its sink, or -inf); one that sees a latent with a NaN or infinity gets NaN,
  * and latents that it does not see do nothing. DEVICE pointers, q and out
  * 16-byte aligned. workspace may be NULL (a buffer per thread and stream that
- * grows; give one, 256-byte aligned, while capturing). head_dim = 448 + 64
+ * grows, released when the thread ends or calls dsv4cuda_shutdown: 1 KB for
+ * each position that max_keys, or n_seqs and max_len, allow; give one,
+ * 256-byte aligned, while capturing). head_dim = 448 + 64
  * with at most 128 heads and strides that are multiples of 8 runs the
  * tensor-core kernel, other shapes (head_dim <= 1024, an even rope_dim of the
  * cache) a general one. A slot
