@@ -90,7 +90,7 @@ __device__ __forceinline__ int4 refs4(const PagedState& p, int q) {
                    q + 2 < p.n_pages ? p.refs[q + 2] : 1, q + 3 < p.n_pages ? p.refs[q + 3] : 1);
 }
 
-// The lowest `want` free pages, ascending, into page[]; returns how many
+// The lowest `want` free pages (a count below 0 is no use either), ascending, into page[]; returns how many
 // there are. Whole block: four pages a thread, the next four on their way.
 __device__ int take_free(const PagedState& p, int want, int* page) {
   int have = 0;
@@ -100,7 +100,7 @@ __device__ int take_free(const PagedState& p, int want, int* page) {
     const int q = base + q0;
     const int4 r = next;
     if (base + 4 * static_cast<int>(blockDim.x) < p.n_pages) next = refs4(p, q + 4 * blockDim.x);
-    const int f[4] = {r.x == 0, r.y == 0, r.z == 0, r.w == 0};
+    const int f[4] = {r.x <= 0, r.y <= 0, r.z <= 0, r.w <= 0};
     int total;
     int at = have + block_scan(f[0] + f[1] + f[2] + f[3], &total);
 #pragma unroll
@@ -339,7 +339,8 @@ __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ Paged
 
 // The i-th page in use beyond the live count moves to the i-th hole below
 // it: no page is both, so all moves can run at once, and their number is
-// the smallest that makes the pool dense.
+// the smallest that makes the pool dense. (A page is in use or a hole whatever
+// its count, one below 0 too: there are as many holes as moves in any state.)
 __global__ void __launch_bounds__(kMetaThreads) compact_kernel(
     const __grid_constant__ PagedState p, int* refs_out) {
   pdl_trigger();
@@ -361,7 +362,7 @@ __global__ void __launch_bounds__(kMetaThreads) compact_kernel(
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const bool in = q + i < p.n_pages;
-      h += in && q + i < live && r[i] == 0;
+      h += in && q + i < live && r[i] <= 0;
       m += in && q + i >= live && r[i] > 0;
     }
     // both counts in one scan: below 2^16 a block's step
@@ -372,7 +373,7 @@ __global__ void __launch_bounds__(kMetaThreads) compact_kernel(
     for (int i = 0; i < 4; ++i) {
       if (q + i >= p.n_pages) continue;
       if (q + i < live) {
-        if (r[i] == 0) w.jobs[ha++].dst = q + i;
+        if (r[i] <= 0) w.jobs[ha++].dst = q + i;
       } else if (r[i] > 0) {
         w.jobs[ma].src = q + i;
         w.jobs[ma].rows = p.page;

@@ -24,7 +24,7 @@ struct PagedState {
   int page, n_pages, n_seqs, max_pages;
   int* table;        // [n_seqs][max_pages], -1 = no page
   int* length;       // [n_seqs]
-  int* refs;         // [n_pages] table entries that name the page, 0 = free
+  int* refs;         // [n_pages] table entries that name the page, 0 (or less) = free
   unsigned* status;  // may be null
   void* ws;          // paged_workspace_bytes()
 };

@@ -520,7 +520,9 @@ typedef struct {
     int max_pages;         /* entries per slot in table */
     int *table;            /* [n_seqs][max_pages], -1 = no page */
     int *length;           /* [n_seqs] positions held */
-    int *refs;             /* [n_pages] table entries that name the page; 0 = free */
+    int *refs;             /* [n_pages] table entries that name the page; 0 = free
+                              (so is less, which a table that names pages
+                              without a count leaves when it is given back) */
     unsigned int *status;  /* bits, ORed by the calls; may be NULL:
                               1 an op did not find the free pages it needs,
                               2 an op that cannot be done (a slot out of range
