@@ -37,6 +37,15 @@ __device__ __forceinline__ int slot_of(const int* q_start, int n_seqs, int row) 
   return lo < n_seqs && q_start[lo] <= row ? lo : -1;
 }
 
+// The first position that a token at `pos` sees. (No difference is formed that
+// could leave the range of an int, whatever the window.)
+__device__ __forceinline__ int seen_from(int window, int pos) {
+  return window > 0 && pos >= window ? pos - window + 1 : 0;
+}
+
+// Positions of a slot; what is not a length counts as none.
+__device__ __forceinline__ int slot_length(const PagedLayer& c, int s) { return max(c.length[s], 0); }
+
 __device__ __forceinline__ float load_q(const PagedAttnProblem& p, long long at) {
   return p.bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.q)[at])
                 : bf16_round(static_cast<const float*>(p.q)[at]);
@@ -108,11 +117,11 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(
   uint32_t* sm_k = reinterpret_cast<uint32_t*>(sm_q + kBlockHeads * d);
   const int s = slot_of(p.q_start, c.n_seqs, row);
   if (s < 0) return;  // (the whole cluster)
-  const int len = c.length[s], end = p.q_start[s + 1];
+  const int len = slot_length(c, s), end = p.q_start[s + 1];
   const bool beyond = end - p.q_start[s] > p.max_new || len > p.max_len;
   if (beyond && tid == 0 && c.status) atomicOr(c.status, kPagedBounds);
   const int self = len - end + row;  // the token's position
-  const int first = p.window > 0 ? max(0, self - p.window + 1) : 0;
+  const int first = seen_from(p.window, self);
   const int last = min(self, c.max_pages * c.page - 1);
   const int steps = beyond || last < first ? 0 : (last - first) / kGenKeys + 1;
   const int step0 = static_cast<int>(static_cast<long long>(steps) * part / parts);
@@ -136,10 +145,10 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(
   }
   // the cache row of this lane's key of a step, -1: none
   auto find_row = [&](int step) {
-    const int t = first + step * kGenKeys + lane;
-    if (step >= step1 || t > last) return -1;
-    const int page = table[t / c.page];
-    return page >= 0 && page < c.n_pages ? page * c.page + t % c.page : -1;
+    const unsigned t = static_cast<unsigned>(first) + step * kGenKeys + lane;
+    if (step >= step1 || t > static_cast<unsigned>(last)) return -1;
+    const int page = table[static_cast<int>(t) / c.page];
+    return page >= 0 && page < c.n_pages ? page * c.page + static_cast<int>(t) % c.page : -1;
   };
   int next_row = warp == 0 ? find_row(step0) : -1;
   constexpr int kAhead = 4;  // loads of a thread on their way together
@@ -413,7 +422,7 @@ struct TcCall {
   TcWs w;
 };
 
-__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+__device__ __forceinline__ int ceil_div(int a, int b) { return a / b + (a % b > 0); }
 
 // One slot's new tokens and the positions they see.
 struct Slot {
@@ -426,7 +435,7 @@ __device__ __forceinline__ Slot slot_geometry(const PagedAttnProblem& p, int tok
   Slot g;
   g.row0 = p.q_start[s];
   const int end = p.q_start[s + 1];
-  g.len = p.pages.length[s];
+  g.len = slot_length(p.pages, s);
   const bool rows_ok = g.row0 >= 0 && end >= g.row0 && end <= p.total;
   g.tokens = rows_ok ? end - g.row0 : 0;
   g.bad = g.tokens > 0 && (g.tokens > p.max_new || g.len > p.max_len);
@@ -434,7 +443,7 @@ __device__ __forceinline__ Slot slot_geometry(const PagedAttnProblem& p, int tok
     if (p.pages.status) atomicOr(p.pages.status, kPagedBounds);
   }
   g.first = g.len - g.tokens;
-  g.klo = p.window > 0 ? max(0, g.first - p.window + 1) : 0;
+  g.klo = seen_from(p.window, g.first);
   g.tiles = ceil_div(g.tokens, tokens_per_tile);
   g.blocks = g.tokens == 0 ? 0 : g.bad ? 1 : max(1, ceil_div(max(0, g.len - g.klo), kKeys));
   return g;
@@ -496,8 +505,8 @@ __device__ void list_tiles(const TcCall& c, const int* block_start, const int* t
         tile.blocks = 1;
         if (p.pages.status) atomicOr(p.pages.status, kPagedBounds);
       } else {
-        const int seen_from = p.window > 0 ? max(0, tile.pos0 - p.window + 1) : 0;
-        const int b0 = min(max(0, seen_from - g.klo) / kKeys, g.blocks - 1);
+        const int from = seen_from(p.window, tile.pos0);
+        const int b0 = min(max(0, from - g.klo) / kKeys, g.blocks - 1);
         const int b1 = min(max(ceil_div(max(0, tile.pos0 + tile.tokens - g.klo), kKeys), b0 + 1),
                            g.blocks);
         tile.blocks = b1 - b0;
@@ -599,12 +608,13 @@ __global__ void __launch_bounds__(kStageThreads, kStageBlocks) stage_kernel(cons
       if (block_start[mid] <= block) lo = mid;
       else hi = mid;
     }
-    const int len = g.length[lo], first = len - (p.q_start[lo + 1] - p.q_start[lo]);
-    const int klo = p.window > 0 ? max(0, first - p.window + 1) : 0;
-    const int t = klo + (block - block_start[lo]) * kKeys +
-                  static_cast<int>(u % (kKeys / kUnit)) * kUnit + (lane & 7);
+    const int len = slot_length(g, lo), first = len - (p.q_start[lo + 1] - p.q_start[lo]);
+    const unsigned at = static_cast<unsigned>(seen_from(p.window, first)) +
+                        (block - block_start[lo]) * kKeys +
+                        static_cast<int>(u % (kKeys / kUnit)) * kUnit + (lane & 7);
+    const int t = static_cast<int>(at);
     int row = -1;
-    if (t < len && t / g.page < g.max_pages) {
+    if (at < static_cast<unsigned>(len) && t / g.page < g.max_pages) {
       const int page = g.table[static_cast<size_t>(lo) * g.max_pages + t / g.page];
       if (page >= 0 && page < g.n_pages) row = page * g.page + t % g.page;
     }
@@ -1092,7 +1102,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
       const Tile& t = seg.t;
       const bool mine = tok < t.tokens;
       const int last = mine ? t.pos0 + tok : -1;  // the position of this row's token
-      const int from = p.window > 0 ? max(0, last - p.window + 1) : 0;
+      const int from = seen_from(p.window, last);
       const bool two_terms = kShort || t.blocks <= kTwoTermBlocks;
       RowState st = {-INFINITY, 0.f, 0.f};
       bool bad = t.bad != 0;
