@@ -232,7 +232,8 @@ __global__ void __launch_bounds__(kMetaThreads) fork_kernel(const __grid_constan
 }
 
 // One block, as the fork: the ops' needs, prefix sums of them (so the pages of
-// an op do not depend on timing), the lowest free pages in one scan of the
+// an op do not depend on timing; an op that finds none keeps its place, so that
+// no later one overtakes it), the lowest free pages in one scan of the
 // counts, four a thread, the next four on their way (48 ops that take 3,400
 // of 16,384 pages: 9 us).
 __global__ void __launch_bounds__(kMetaThreads) append_kernel(const __grid_constant__ PagedState p,

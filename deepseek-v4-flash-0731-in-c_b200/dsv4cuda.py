@@ -697,7 +697,8 @@ class PagedCache:
 
     def append(self, slots, counts, rows=None, stream=None):
         """Slots grow by counts tokens (int32 CUDA tensors); rows (int64) receives
-        the new tokens' cache rows, as LatentCache.write takes them, and -1 behind them."""
+        the new tokens' cache rows, as LatentCache.write takes them, and -1 behind them.
+        Behind a slot that does not find its pages no later one takes a page."""
         n, at, n_rows = slots.shape[0], _dev(rows, "rows", self._i64), 0
         if rows is not None:
             n_rows = rows.numel()

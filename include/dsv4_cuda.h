@@ -546,7 +546,10 @@ size_t dsv4cuda_paged_workspace_bytes(int n_pages, int n_seqs);
 int dsv4cuda_paged_fork(const dsv4cuda_paged *p, const int *dst, const int *src, int n,
                         void *stream);
 /* Append: slot slots[i] grows by counts[i] tokens, taking the lowest free
- * pages. rows [n_rows] (may be NULL) receives the cache rows of the new
+ * pages, op after op: behind an op that does not find its pages no later one
+ * takes a page (status 1 for it too, however few it needs: a long prompt is not
+ * overtaken by short ones), while ops that need none are done. Put first what
+ * has to go on, a running slot's token before a new prompt. rows [n_rows] (may be NULL) receives the cache rows of the new
  * tokens, op after op, as dsv4cuda_kv_write takes them. An op that does not
  * find its pages changes nothing (status 1), nor does a bad op, one whose
  * tokens do not all have a row among them (status 2); the rows of their tokens

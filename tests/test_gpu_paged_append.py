@@ -71,3 +71,15 @@ def test_tokens_beyond_the_rows_are_refused(cuda):
     assert pool.length.tolist() == [9, 4, 1, 0] and pool.status() == pool.BAD_OP
     pool.append(dev([3]), dev([1]))                             # no rows wanted: no limit
     assert pool.length.tolist() == [9, 4, 1, 1] and pool.status() == 0
+
+
+def test_nobody_overtakes_an_op_without_pages(cuda):
+    """4 pages, 1 of them taken: the second op needs 4, the third one that there is, the
+    last none."""
+    pool = pool_of(cuda, pages=4)
+    pool.append(dev([3]), dev([2]))
+    rows = rows_of(25)
+    pool.append(dev([0, 1, 2, 3]), dev([4, 16, 3, 2]), rows)
+    assert rows.tolist() == [4, 5, 6, 7] + [-1] * 19 + [2, 3]
+    assert pool.length.tolist() == [4, 0, 0, 4]
+    assert pool.refs.tolist() == [1, 1, 0, 0] and pool.status() == pool.EXHAUSTED
