@@ -35,8 +35,8 @@ constexpr int kRound = 4 * kThreads; // candidates of four values a thread
 constexpr int kCap = 2 * kRound;     // candidates held
 // More candidates than kThin are thinned out to the best 32, looked at every
 // kWindow steps: a tighter limit keeps later values out, a look costs two
-// barriers. (2048 rows of 129280 fp32 values, top 8: 212 us; 229 with 256,
-// 215 with windows of 2, 4, 8, 8 .. steps, 214 with windows of 4.)
+// barriers. (2048 rows of 129280 fp32 values, top 8: 211 us; 226 with 256, 213
+// with windows of 4.)
 constexpr int kThin = 64;
 constexpr int kWindow = 8;
 constexpr int kTop = kMaxTopAlternatives;
@@ -114,7 +114,7 @@ __device__ void compact(Shared& sh, int k) {
   if (n <= kThreads) {
     // a thread a key: its place is the number of larger ones (keys differ).
     // Shorter than the sort below where there are no more keys than threads (1
-    // row: 10.2 us, 11.4 to 12.3 with the sort alone).
+    // row: 10.3 us, 11.6 to 12.0 with the sort alone).
     const Key mine = tid < n ? sh.cand[tid] : 0;
     int rank = 0;
 #pragma unroll 4
@@ -223,13 +223,13 @@ struct Vec {
 
 // kStep: values a thread reads per step; kBlocks: blocks of an SM.
 //
-// 2048 rows of 129280 fp32 values, top 8: 212 us, 5.0 TB/s of the 6.5 that a
-// copy reaches. Instructions bound it: an exponential, two FMAs, a compare,
-// a share of a maximum and of the bookkeeping a value; BF16 rows, whose bytes
-// are half, take 209. 256 threads, four blocks an SM: 229 us against 252 with
-// two of 512 (before the candidates were thinned out earlier). 1 row: 9.6 us,
-// a chain of one read, the choice among 32 values a thread, the cluster's
-// meeting and the final merge.
+// 2048 rows of 129280 fp32 values, top 8: 211 us, 5.0 TB/s of the 6.5 that a
+// copy reaches. Instructions bound it: an exponential, two FMAs, compares, a
+// share of a maximum and of the bookkeeping are 20 a value, and 77% of the
+// issue slots are taken (600 rows, start and end included; memory 46%, in BF16
+// rows, whose bytes are half, 25% at 95% of the time). 256 threads, four blocks
+// an SM: 9% less than with two of 512. 1 row: 10.3 us, a chain of one read, the
+// choice among 32 values a thread, the cluster's meeting and the final merge.
 template <bool kBf16, int kStep, int kBlocks>
 __global__ void __launch_bounds__(kThreads, kBlocks) logprob_kernel(const LogprobProblem p, int parts) {
   using V = Vec<kBf16>;
@@ -557,8 +557,8 @@ cudaError_t token_logprobs(const LogprobProblem& p, cudaStream_t st) {
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return e;
   // Few rows: each is cut over a cluster so that a thread's 32 values are all
-  // it reads, and the k best are picked once (1 row of 129280: 11.5 us where
-  // steps of 16 values took 17.1). More rows than that leave room for: steps of
+  // it reads, and the k best are picked once (1 row of 129280: 10.3 us where
+  // the kernel of many rows takes 14.3). More rows than that leave room for: steps of
   // 16 values, four blocks to an SM, rows cut while SMs idle (48 rows: 16.4 us,
   // 32 uncut).
   constexpr int kShort = 32, kLong = 16;

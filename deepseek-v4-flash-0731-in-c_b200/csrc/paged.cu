@@ -90,8 +90,9 @@ __device__ __forceinline__ int4 refs4(const PagedState& p, int q) {
                    q + 2 < p.n_pages ? p.refs[q + 2] : 1, q + 3 < p.n_pages ? p.refs[q + 3] : 1);
 }
 
-// The lowest `want` free pages (a count below 0 is no use either), ascending, into page[]; returns how many
-// there are. Whole block: four pages a thread, the next four on their way.
+// The lowest `want` free pages (a count below 0 is no use either), ascending,
+// into page[]; returns how many there are. Whole block: four pages a thread, the
+// next four on their way.
 __device__ int take_free(const PagedState& p, int want, int* page) {
   int have = 0;
   const int q0 = 4 * threadIdx.x;

@@ -360,11 +360,11 @@ constexpr int kKeys = 64;         // keys of a block: N of Q K^T, K of P V
 constexpr int kHalf = 256;        // output dims of a CTA: N of P V
 // What a tile costs besides its blocks (Q in, O out), in blocks: shares are
 // cut by the sum, so that many short tiles weigh as much as a long one (2000
-// tiles of three blocks: 208 us, 273 where a tile costs nothing, 207 at 8; 8
-// sequences of 3 tiles of 32 to 63 blocks: 51.9, 55.7 and 53.2).
+// tiles of three blocks: 189 us, 251 where a tile costs nothing, 186 at 8; 8
+// sequences of 3 tiles of 32 to 63 blocks: 47.7, 50.1 and 49.4).
 constexpr int kTileCost = 4;
 // A smaller share costs more to merge than it saves (one tile of 32 blocks:
-// 21.7 us, 23.7 with shares from one unit on, 21.8 from four).
+// 20.7 us, 22.8 with shares from one unit on, 22.0 from four).
 constexpr int kMinShare = 2;
 // The weights of P V are BF16, each off by up to 2^-8 of itself. Their sum as
 // P V takes them is kept next to the exact one, and O is multiplied by the
@@ -374,8 +374,8 @@ constexpr int kMinShare = 2;
 // it. lse takes the exact sum. (A sum more in the softmax: 2048 tokens on 11987
 // keys 3684 us, 3640 with the weights off by their rounding.) Where a row sees
 // few keys that is not enough: a tile of at most this many blocks carries its
-// weights in two BF16 terms, at twice the MMAs of P V (2000 tiles of three
-// blocks: 208 us, 205 with one term, in one build).
+// weights in two BF16 terms. Twice the MMAs of P V there do not show (2000 tiles
+// of three blocks in the kernel that has both: 199 us with one term or two).
 constexpr int kTwoTermBlocks = 4;
 constexpr float kLazyMargin = 8.0f;  // log2 units: the running max moves only past this
 
@@ -1388,7 +1388,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(
       };
       while (ok && walk.next(seg)) {
         // Q and the first key blocks are on their way before Q's room is free (2000
-        // tiles: 191 us, 198 with Q's second part behind them)
+        // tiles take 4% longer with Q's second part behind them)
         if (p.bf16) {
           for (int k = 0; k < 2 && ok; ++k) ok = load_own(&qmap, 256 * k, seg.t.row0, true);
         }
@@ -1683,7 +1683,7 @@ TcShape tc_shape(const PagedAttnProblem& p) {
 
 // No tile sees more than kTwoTermBlocks blocks: n positions from any on touch
 // at most (n + 62) / 64 + 1. They take a kernel of their own, without the code
-// of one-term weights: 2000 tiles of three blocks 187 us, 200 in the kernel that
+// of one-term weights: 2000 tiles of three blocks 189 us, 199 in the kernel that
 // has both.
 bool short_tiles(const PagedAttnProblem& p, const TcShape& s) {
   long long n = p.max_len;
@@ -1730,8 +1730,7 @@ cudaError_t tc_forward(const PagedAttnProblem& p, void* ws, cudaStream_t st) {
   if (c.s.block_cap * kKeys > 0x7FFFFFFFll) return cudaErrorInvalidValue;
   CUtensorMap map;
   // 64 keys x 128 dims a copy: two column blocks of 128 bytes as planes (2000
-  // tiles of three blocks: 203 us, 207 with a copy a column block, and 193
-  // since the next tile's Q is not prefetched to L2 as well)
+  // tiles of three blocks take 2% longer with a copy a column block)
   if (!make_tma_map_u8_3d(&map, c.w.stage, 128, static_cast<uint64_t>(c.s.block_cap) * kKeys, kD * 2,
                           kD / 64, 128, 128, kKeys, 2))
     return cudaErrorInvalidValue;
