@@ -214,7 +214,7 @@ def prepare(case, seed):
             weights = dict(hidden=h, moe_inter=i, n_experts=e, topk=k, swiglu_limit=c["limit"],
                            route_scale=1.5, gate_w=torch.zeros(e, h, dtype=torch.int16, device="cuda"),
                            **{m: s[m] for m in ("w1", "s1", "w3", "s3", "w2", "s2")})
-            s["layer"] = _binding().MoeLayer(weights, max_tokens=1)
+            s["layer"] = _binding().MoeLayer(weights, max_tokens=1, device=True)
         return s
     if c["op"] == "grouped":
         e, m, k, rows = c["experts"], c["outs"], c["width"], c["rows"]
