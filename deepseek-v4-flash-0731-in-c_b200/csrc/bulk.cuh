@@ -132,4 +132,13 @@ bool make_tma_map_u8_3d(CUtensorMap* out, const void* base, uint64_t row_bytes, 
                         uint64_t row_pitch, uint64_t planes, uint64_t plane_pitch,
                         uint32_t box_bytes, uint32_t box_rows, uint32_t box_planes);
 
+// Host: a 3-D map over `planes` planes of `rows` rows of `cols` packed 4-bit
+// elements (cols a multiple of 128, base 32-byte aligned) with boxes of 128
+// elements by box_rows, 128-byte swizzle; not cached. A box lands in shared
+// memory with 16 elements in the first half of every 16 bytes, as the mixed
+// 8-, 6- and 4-bit MMAs take them; on the mbarrier it counts with the bytes
+// that are read. The inner coordinate is in elements.
+bool make_tma_map_u4_3d(CUtensorMap* out, const void* base, uint64_t cols, uint64_t rows,
+                        uint64_t planes, uint32_t box_rows);
+
 }  // namespace dsv4

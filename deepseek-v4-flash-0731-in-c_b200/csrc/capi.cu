@@ -26,6 +26,7 @@
 #include "snapshot.cuh"
 #include "paged.cuh"
 #include "paged_attn.cuh"
+#include "grouped.cuh"
 #include "logprob.cuh"
 #include "ep.cuh"
 #include "../../include/dsv4_cuda.h"
@@ -1847,6 +1848,144 @@ DSV4_API int dsv4cuda_token_logprobs(const void* logits, int bf16, int rows, int
   p.top_logprob = top_logprob;
   cudaError_t e = dsv4::token_logprobs(p, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) { record_error("dsv4cuda_token_logprobs: %s", cudaGetErrorString(e)); return -1; }
+  return 0;
+}
+
+// =================================================== grouped products ==
+
+namespace {
+
+bool experts_problem(const char* who, const dsv4cuda_moe_layer* L, int n, dsv4::ExpertsProblem* p) {
+  static_assert(dsv4::kGroupedMaxExperts == 1024, "limit named below");
+  if (!L || n < 0) {
+    record_error("%s: bad arguments", who);
+    return false;
+  }
+  const dsv4::MoeConfig& c = L->cfg;
+  const int experts = dsv4::moe_local_hi(c) - c.expert_lo;
+  if (c.hidden % 128 || c.moe_inter % 128 || experts < 1 || experts > dsv4::kGroupedMaxExperts ||
+      static_cast<long long>(n) * c.topk > 0x3FFFFFFFll ||
+      static_cast<long long>(n) * (c.hidden / 8) > 0x7FFFFFFF00ll) {
+    record_error("%s: hidden %d and moe_inter %d must be multiples of 128, experts 1..1024, routes "
+                 "below 2^30", who, c.hidden, c.moe_inter);
+    return false;
+  }
+  p->n = n;
+  p->topk = c.topk;
+  p->hidden = c.hidden;
+  p->inter = c.moe_inter;
+  p->lo = c.expert_lo;
+  p->experts = experts;
+  p->w1 = L->w.w1; p->s1 = L->w.s1;
+  p->w3 = L->w.w3; p->s3 = L->w.s3;
+  p->w2 = L->w.w2; p->s2 = L->w.s2;
+  p->limit = static_cast<float>(c.swiglu_limit);
+  return true;
+}
+
+bool grouped_problem(const char* who, const dsv4cuda_grouped_shape* s, dsv4::GroupedProblem* p) {
+  if (!s || s->n_groups < 1 || s->n_groups > dsv4::kGroupedMaxExperts || s->n_rows < 0 ||
+      s->n_rows > 0x3FFFFFFF || s->x_rows < 0 || s->out_rows < 0 || s->outs < 1 || s->width < 128 ||
+      s->width % 128 || s->outs > 0x3FFFFFFF || (s->out_stride && s->out_stride < s->outs)) {
+    record_error("%s: bad shape (1..1024 groups, width a multiple of 128, out_stride at least outs)",
+                 who);
+    return false;
+  }
+  p->experts = s->n_groups;
+  p->rows = s->n_rows;
+  p->x_rows = s->x_rows;
+  p->out_rows = s->out_rows;
+  p->outs = s->outs;
+  p->width = s->width;
+  p->fp8 = s->fp8 != 0;
+  p->bf16 = s->bf16 != 0;
+  p->out_stride = s->out_stride ? s->out_stride : s->outs;
+  return true;
+}
+
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// The caller's workspace, or this thread's for the stream; nullptr with the
+// error recorded.
+void* pick_workspace(const char* who, void* ws, size_t bytes, size_t need, cudaStream_t st) {
+  if (!ws) return stream_scratch(who, need, st);
+  if (bytes < need || !aligned(ws, 256)) {
+    record_error("%s: workspace of %zu bytes, need %zu (256-byte aligned)", who, bytes, need);
+    return nullptr;
+  }
+  return ws;
+}
+
+}  // namespace
+
+DSV4_API size_t dsv4cuda_moe_experts_workspace_bytes(const dsv4cuda_moe_layer* L, int n_tokens) {
+  dsv4::ExpertsProblem p;
+  if (!experts_problem("dsv4cuda_moe_experts_workspace_bytes", L, n_tokens, &p)) return 0;
+  return dsv4::experts_workspace_bytes(p);
+}
+
+DSV4_API int dsv4cuda_moe_experts(dsv4cuda_moe_layer* L, const uint8_t* xq, const uint8_t* xs,
+                                  const int* idx, const float* wt, int n_tokens, uint16_t* out,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "dsv4cuda_moe_experts";
+  dsv4::ExpertsProblem p;
+  if (!experts_problem(who, L, n_tokens, &p)) return -1;
+  if (n_tokens == 0) return 0;
+  if (!xq || !xs || !idx || !wt || !out || !aligned(xq, 32) || !aligned(out, 32) ||
+      !aligned(p.w1, 32) || !aligned(p.w3, 32) || !aligned(p.w2, 32) || !aligned(p.s1, 4) ||
+      !aligned(p.s3, 4) || !aligned(p.s2, 4)) {
+    record_error("%s: bad arguments (xq, out and the layer's w1, w3, w2 32-byte aligned, its scales 4)",
+                 who);
+    return -1;
+  }
+  p.xq = xq;
+  p.xs = xs;
+  p.idx = idx;
+  p.wt = wt;
+  p.out = out;
+  p.err = dsv4::device_error_word();
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  void* ws = pick_workspace(who, workspace, workspace_bytes, dsv4::experts_workspace_bytes(p), st);
+  if (!ws) return -1;
+  cudaError_t e = dsv4::experts_forward(p, ws, st);
+  if (e != cudaSuccess) { record_error("%s: %s", who, cudaGetErrorString(e)); return -1; }
+  return 0;
+}
+
+DSV4_API size_t dsv4cuda_grouped_workspace_bytes(const dsv4cuda_grouped_shape* shape) {
+  dsv4::GroupedProblem p;
+  if (!grouped_problem("dsv4cuda_grouped_workspace_bytes", shape, &p)) return 0;
+  return dsv4::grouped_workspace_bytes(p);
+}
+
+DSV4_API int dsv4cuda_grouped_gemm(void* out, const uint8_t* xq, const uint8_t* xs, const uint8_t* w,
+                                   const uint8_t* ws, const int* offsets, const int* src,
+                                   const int* dst, const dsv4cuda_grouped_shape* shape,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "dsv4cuda_grouped_gemm";
+  dsv4::GroupedProblem p;
+  if (!grouped_problem(who, shape, &p)) return -1;
+  if (p.rows == 0 || p.out_rows == 0) return 0;
+  if (!out || !xq || !xs || !w || !ws || !offsets || p.x_rows < 1 || !aligned(xq, 16) ||
+      !aligned(w, 32) || (!p.fp8 && !aligned(ws, 4)) || !aligned(out, p.bf16 ? 2 : 4)) {
+    record_error("%s: bad arguments (xq 16-byte aligned, w 32, ws 4 with E2M1 weights)", who);
+    return -1;
+  }
+  p.xq = xq;
+  p.xs = xs;
+  p.w[0] = w;
+  p.ws[0] = ws;
+  p.offsets = offsets;
+  p.src = src;
+  p.dst = dst;
+  p.out = out;
+  p.err = dsv4::device_error_word();
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  void* work = pick_workspace(who, workspace, workspace_bytes, dsv4::grouped_workspace_bytes(p), st);
+  if (!work) return -1;
+  cudaError_t e = dsv4::grouped_reset(work, st);
+  if (e == cudaSuccess) e = dsv4::grouped_forward(p, work, st);
+  if (e != cudaSuccess) { record_error("%s: %s", who, cudaGetErrorString(e)); return -1; }
   return 0;
 }
 

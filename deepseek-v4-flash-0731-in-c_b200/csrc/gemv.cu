@@ -108,6 +108,21 @@ bool make_tma_map_u8_3d(CUtensorMap* out, const void* base, uint64_t row_bytes, 
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool make_tma_map_u4_3d(CUtensorMap* out, const void* base, uint64_t cols, uint64_t rows,
+                        uint64_t planes, uint32_t box_rows) {
+  auto fn = encode_fn();
+  if (!fn || reinterpret_cast<uintptr_t>(base) % 32 != 0 || cols % 128 != 0 || cols == 0 ||
+      rows == 0 || planes == 0)
+    return false;
+  const cuuint64_t dims[3] = {cols, rows, planes};
+  const cuuint64_t strides[2] = {cols / 2, cols / 2 * rows};
+  const cuuint32_t box[3] = {128, box_rows, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return fn(out, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 3, const_cast<void*>(base), dims, strides,
+            box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 unsigned int* device_error_word() {
   static unsigned int* words[64] = {};
   int dev = 0;

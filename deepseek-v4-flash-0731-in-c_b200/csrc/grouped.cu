@@ -1,0 +1,1070 @@
+// grouped.cu - products of many rows grouped by expert, on the block-scaled
+// tensor cores, and the routed experts of a MoE layer built from them.
+//
+//   out[r, i] = sum_k x[r, k] W_e[i, k]          for the rows r of group e
+//
+// x is E4M3 with a power of two per 128 columns, W E2M1 with one per 32 (or
+// E4M3 with one per 128 x 128): exactly what tcgen05.mma's mxf8f6f4 kind
+// multiplies, scales included, into fp32 sums. The weights are the A operand
+// (128 outputs are the M of an instruction) and a group's rows its N, so that
+// a group of a few rows wastes columns of a small N instead of rows of a
+// large M: a decode step's experts are read at the same cost as a GEMV's.
+//
+// One block per SM takes an equal share of all (tile, 128-column chunk) units
+// laid end to end; a tile is 256 outputs (or 128 gate and 128 up outputs) of
+// up to 192 rows. A tile that a share's end cuts is written as fp32 parts,
+// and whoever brings its last part adds them in the order of the columns, so
+// that results do not depend on timing.
+//
+// Roles: warps 0-7 epilogue, 8-11 scales (registers to TMEM, the copies of
+// all four lane quarters at once), 12 copies, 13 MMAs.
+#include "grouped.cuh"
+
+#include <cuda_bf16.h>
+
+#include "launch.cuh"
+#include "umma.cuh"
+
+namespace dsv4 {
+namespace {
+
+constexpr int kChunk = 128;              // columns of a stage: one row of swizzled shared memory
+constexpr int kTileRows = 128;           // M of an instruction
+constexpr int kATile = kTileRows * kChunk;
+constexpr int kEpiWarps = 8, kScaleWarps = 4;
+constexpr int kWarpCopy = kEpiWarps + kScaleWarps, kWarpMma = kWarpCopy + 1;
+constexpr int kThreads = 32 * (kWarpMma + 1);
+constexpr int kBlockCols = 16;           // rows of a group that an epilogue step takes
+constexpr int kMaxN = 192, kHalfN = 96;  // rows of a tile; up to kHalfN two tiles' sums fit in TMEM
+constexpr int kMaxStages = 5;
+// TMEM columns: two buffers of scales (four chunks: 2 x 4 columns of weights'
+// and 8 of rows' scales each), then the sums.
+constexpr int kScaleCols = 64, kSumCol = 2 * kScaleCols, kTmemCols = 512;
+constexpr int kMaxShares = 256;          // blocks
+
+struct Args {
+  GroupedProblem p;
+  int shares;         // blocks
+  int n_max, stages;  // rows of a tile; stages of the ring
+  int* counters;      // [kMaxShares] chunks whose parts are there
+  float* parts;       // [shares][2][2][n_max][128]
+};
+
+struct alignas(16) Control {
+  uint64_t full[kMaxStages], empty[kMaxStages];
+  uint64_t scale_full[2], scale_empty[2];
+  uint64_t sum_full[2], sum_empty[2];
+  uint64_t fin;
+  uint32_t tmem;
+  int abort_flag;
+  int last;      // the block brought a tile's last part
+  alignas(16) uint32_t top[2][2][4][kBlockCols];  // largest |h| of a warp's 32 outputs
+  alignas(16) uint8_t codes[2][2][kBlockCols][kTileRows];
+};
+
+__host__ __device__ constexpr int stage_bytes(int n_max) { return 2 * kATile + n_max * kChunk; }
+__host__ __device__ inline size_t smem_bytes(int n_max, int stages, int experts) {
+  return static_cast<size_t>(stages) * stage_bytes(n_max) + sizeof(Control) +
+         (experts + 1) * (sizeof(long long) + sizeof(int));
+}
+
+// Suspended waits: the epilogue needs the issue slots.
+__device__ __forceinline__ bool try_wait_long(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;"
+      " selp.u32 %0, 1, 0, p; }"
+      : "=r"(ok)
+      : "r"(smem_addr(bar)), "r"(parity), "r"(20000u)  // at most 20 us at a time
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                         unsigned* err) {
+  if (try_wait_long(bar, parity)) return true;
+  const unsigned long long t0 = global_timer_ns();
+  while (!try_wait_long(bar, parity)) {
+    if (*abort_flag) return false;
+    if (global_timer_ns() - t0 > kWaitLimitNs) {
+      if (err) atomicOr(err, kErrWait);
+      *abort_flag = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
+// D (+)= A B with block scales: A and B types in idesc, one E8M0 per 32
+// columns, byte `k` of each scale column.
+__device__ __forceinline__ void mma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                           uint32_t scale_a, uint32_t scale_b, bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X"
+      " [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+          smem_addr(bar))
+      : "memory");
+}
+// Four rows of a tensor map with one-row boxes, one behind the other; a row
+// outside the map is zeros.
+__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, int x, const int (&y)[4],
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]),
+      "r"(smem_addr(bar))
+      : "memory");
+}
+
+// 16 consecutive TMEM columns of this thread's lane.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+// The wait names the registers so that no use is scheduled before it.
+__device__ __forceinline__ void tmem_ld_wait16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                 "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
+                 "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+}
+
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// ------------------------------------------------------------------ plan --
+
+// How a group of n rows is cut: tiles of the same number of rows, a multiple
+// of 16, and what a chunk of one costs. Up to some 90 rows a chunk costs what
+// its weights take to come from memory, beyond that what the MMAs take.
+struct Cut {
+  int tiles, rows, cost;
+};
+constexpr int kMemoryCost = 90;
+__device__ __forceinline__ Cut cut_group(int n, int n_max) {
+  Cut c;
+  c.tiles = (n + n_max - 1) / n_max;
+  c.rows = c.tiles ? ((n + c.tiles - 1) / c.tiles + 15) & ~15 : 16;
+  c.tiles = c.tiles ? (n + c.rows - 1) / c.rows : 0;
+  c.cost = c.rows > kMemoryCost ? c.rows : kMemoryCost;
+  return c;
+}
+
+// A share's part of one tile.
+struct Piece {
+  int e, row_tile;     // matrix, 256 (gated: 128) outputs
+  int row0, rows, n;   // first row of the tile, rows there are, columns of the MMAs
+  int lo, hi;          // chunks
+  long long start;     // of the tile, in cost
+  int cost;            // of a chunk
+};
+
+struct Walk {
+  const long long* prefix;  // [experts + 1] cost before each group
+  const int* offsets;       // [experts + 1]
+  int experts, row_tiles, chunks, n_max;
+  long long b0, b1;         // this share
+  int e, item;
+  bool done;
+
+  __device__ void begin() {
+    done = b0 >= b1;
+    if (done) return;
+    int lo = 0, hi = experts;  // the last group whose start is not behind b0
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (prefix[mid] <= b0) lo = mid; else hi = mid;
+    }
+    e = lo;
+    const Cut c = cut_group(offsets[e + 1] - offsets[e], n_max);
+    item = static_cast<int>((b0 - prefix[e]) / (static_cast<long long>(chunks) * c.cost));
+  }
+  // The chunk of the tile that starts at `start` in which position b lies.
+  __device__ int chunk_at(long long b, long long start, int cost) const {
+    const long long d = b - start;
+    return d <= 0 ? 0
+                  : d >= static_cast<long long>(chunks) * cost
+                        ? chunks
+                        : static_cast<int>(static_cast<unsigned>(d) / static_cast<unsigned>(cost));
+  }
+  __device__ bool next(Piece* p) {
+    if (done) return false;
+    Cut c;
+    while (true) {
+      if (e >= experts) {
+        done = true;
+        return false;
+      }
+      c = cut_group(offsets[e + 1] - offsets[e], n_max);
+      if (item < c.tiles * row_tiles) break;
+      ++e;
+      item = 0;
+    }
+    p->start = prefix[e] + static_cast<long long>(item) * chunks * c.cost;
+    p->cost = c.cost;
+    p->lo = chunk_at(b0, p->start, c.cost);
+    p->hi = chunk_at(b1, p->start, c.cost);
+    if (p->lo >= p->hi) {
+      done = true;
+      return false;
+    }
+    // the tiles of the same weights follow one another: the second reads them
+    // from L2
+    const int t = item % c.tiles;
+    p->e = e;
+    p->row_tile = item / c.tiles;
+    p->row0 = offsets[e] + t * c.rows;
+    const int left = offsets[e + 1] - p->row0;
+    p->rows = left < c.rows ? left : c.rows;
+    p->n = c.rows;
+    if (p->hi < chunks) done = true;
+    ++item;
+    return true;
+  }
+};
+
+// -------------------------------------------------------------- products --
+
+template <bool kFp8, bool kGated>
+__global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
+    const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUtensorMap map1,
+    const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Args a) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const GroupedProblem& p = a.p;
+  Control* ctl = reinterpret_cast<Control*>(smem + static_cast<size_t>(a.stages) * stage_bytes(a.n_max));
+  long long* prefix = reinterpret_cast<long long*>(ctl + 1);
+  int* offsets = reinterpret_cast<int*>(prefix + p.experts + 1);
+  volatile int* abort_flag = &ctl->abort_flag;
+  unsigned* err = p.err;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int chunks = p.width / kChunk;
+  constexpr int kOuts = kGated ? kTileRows : 2 * kTileRows;  // of a tile
+  const int row_tiles = (p.outs + kOuts - 1) / kOuts;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < a.stages; ++i) {
+      mbar_init(&ctl->full[i], 1);
+      mbar_init(&ctl->empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&ctl->scale_full[i], 32 * kScaleWarps);
+      mbar_init(&ctl->scale_empty[i], 1);
+      mbar_init(&ctl->sum_full[i], 1);
+      mbar_init(&ctl->sum_empty[i], 32 * kEpiWarps);
+    }
+    mbar_init(&ctl->fin, 1);
+    ctl->abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == kWarpCopy && lane == 0) {
+    tma_prefetch_desc(&map0);
+    if (kGated) tma_prefetch_desc(&map1);
+    tma_prefetch_desc(&xmap);
+  }
+  if (warp == kWarpMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_addr(&ctl->tmem)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait();  // offsets, rows and counters of the kernels before
+  pdl_trigger();
+  // offsets that are out of order or beyond `rows` leave groups empty
+  for (int e = threadIdx.x; e <= p.experts; e += kThreads)
+    offsets[e] = min(max(p.offsets[e], 0), p.rows);
+  __syncthreads();
+  if (warp == 0) {
+    long long run = 0;
+    int at = 0;  // offsets in ascending order
+    for (int e0 = 0; e0 <= p.experts; e0 += 32) {
+      const int e = e0 + lane;
+      int o = e <= p.experts ? offsets[e] : p.rows;
+      o = max(o, at);
+#pragma unroll
+      for (int s = 1; s < 32; s <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, o, s);
+        if (lane >= s) o = max(o, u);
+      }
+      if (e <= p.experts) offsets[e] = o;
+      at = __shfl_sync(0xffffffffu, o, 31);
+    }
+    __syncwarp();
+    for (int e0 = 0; e0 <= p.experts; e0 += 32) {
+      const int e = e0 + lane;
+      const Cut c = cut_group(e < p.experts ? offsets[e + 1] - offsets[e] : 0, a.n_max);
+      const long long mine = static_cast<long long>(c.tiles) * row_tiles * chunks * c.cost;
+      long long incl = mine;
+#pragma unroll
+      for (int s = 1; s < 32; s <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, incl, s);
+        if (lane >= s) incl += u;
+      }
+      if (e <= p.experts) prefix[e] = run + incl - mine;
+      run += __shfl_sync(0xffffffffu, incl, 31);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl->tmem;
+  const long long total = prefix[p.experts];
+  // Shares of a few chunks at least: a cut costs two fp32 parts.
+  constexpr int kMinChunks = 4;
+  const long long most = total / (kMinChunks * kMemoryCost);
+  const int shares = most < 1 ? 1 : most < a.shares ? static_cast<int>(most) : a.shares;
+  auto bound = [&](int c) { return c >= shares ? total : total * c / shares; };
+  const int me = blockIdx.x;
+  Walk walk;
+  walk.prefix = prefix;
+  walk.offsets = offsets;
+  walk.experts = p.experts;
+  walk.row_tiles = row_tiles;
+  walk.chunks = chunks;
+  walk.n_max = a.n_max;
+  walk.b0 = bound(me);
+  walk.b1 = bound(me + 1);
+  walk.begin();
+  Piece piece;
+  auto two_tiles = [&](const Piece& q) {
+    return kGated || q.row_tile * kOuts + kTileRows < p.outs;
+  };
+
+  if (warp < kEpiWarps) {
+    // ------------------------------------------------------------ epilogue
+    const int side = warp >> 2, quarter = warp & 3;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const int at = quarter * 32 + lane;  // output of a tile
+    unsigned uses[2] = {0, 0};           // of each half of the sums' columns
+    int half = 0, flip = 0;
+    while (walk.next(&piece)) {
+      const bool big = piece.n > kHalfN;
+      const int blocks = piece.n / kBlockCols;
+      // this lane's column of each block: its weight or its row of out
+      float weight[kMaxN / kBlockCols / 2];
+      int row_out[kMaxN / kBlockCols / 2];
+#pragma unroll
+      for (int i = 0; i < kMaxN / kBlockCols / 2; ++i) {
+        const int r = (2 * i + side) * kBlockCols + (lane & 15);
+        const bool in = r < piece.rows;
+        if (kGated) {
+          weight[i] = in && p.weight ? p.weight[piece.row0 + r] : 1.f;
+        } else {
+          const int d = !in ? -1 : p.dst ? p.dst[piece.row0 + r] : piece.row0 + r;
+          row_out[i] = d < p.out_rows ? d : -1;
+        }
+      }
+      const int h = big ? 0 : half;
+      const uint32_t sums = tmem + lanes + kSumCol + (big ? 0 : h * (kMaxN));
+      const uint32_t sums1 = sums + (big ? kMaxN : kHalfN);
+      if (big) {
+        wait_bar(&ctl->sum_full[0], uses[0]++ & 1, abort_flag, err);
+        wait_bar(&ctl->sum_full[1], uses[1]++ & 1, abort_flag, err);
+      } else {
+        wait_bar(&ctl->sum_full[h], uses[h]++ & 1, abort_flag, err);
+        half ^= 1;
+      }
+      tc_fence_after();
+      auto release = [&] {
+        tc_fence_before();
+        if (big) {
+          mbar_arrive(&ctl->sum_empty[0]);
+          mbar_arrive(&ctl->sum_empty[1]);
+        } else {
+          mbar_arrive(&ctl->sum_empty[h]);
+        }
+      };
+      const bool cut = piece.lo > 0 || piece.hi < chunks;
+      const bool second = two_tiles(piece);
+      const size_t tile_floats = static_cast<size_t>(a.n_max) * kTileRows;
+      auto part_of = [&](int c) {  // share c's part of this tile
+        const int slot = bound(c) >= piece.start ? 0 : 1;
+        return a.parts + (static_cast<size_t>(c) * 2 + slot) * 2 * tile_floats + at;
+      };
+      int c0 = me, c1 = me;
+      if (cut) {
+        float* mine = part_of(me);
+        for (int b = side; b < blocks; b += 2) {
+          uint32_t r0[16], r1[16];
+          tmem_ld16(sums + b * kBlockCols, r0);
+          if (second) tmem_ld16(sums1 + b * kBlockCols, r1);
+          tmem_ld_wait16(r0);
+          if (second) tmem_ld_wait16(r1);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float* q = mine + static_cast<size_t>(b * kBlockCols + i) * kTileRows;
+            __stcg(q, __uint_as_float(r0[i]));
+            if (second) __stcg(q + tile_floats, __uint_as_float(r1[i]));
+          }
+        }
+        release();
+        while (walk.chunk_at(bound(c0), piece.start, piece.cost) > 0) --c0;
+        while (walk.chunk_at(bound(c1 + 1), piece.start, piece.cost) < chunks) ++c1;
+        __threadfence();
+        bar_sync(1, 32 * kEpiWarps);
+        if (threadIdx.x == 0) {
+          const int n = piece.hi - piece.lo;
+          ctl->last = atomicAdd(a.counters + c0, n) + n == chunks;
+          __threadfence();
+        }
+        bar_sync(1, 32 * kEpiWarps);
+        const bool last = *static_cast<volatile int*>(&ctl->last) != 0;
+        bar_sync(1, 32 * kEpiWarps);  // read by all before it is written again
+        if (!last) continue;
+        __threadfence();
+      }
+      // the sums of 16 rows of the group, this lane's output(s)
+      auto take = [&](int b, float (&v0)[16], float (&v1)[16]) {
+        if (!cut) {
+          uint32_t r0[16], r1[16];
+          tmem_ld16(sums + b * kBlockCols, r0);
+          if (second) tmem_ld16(sums1 + b * kBlockCols, r1);
+          tmem_ld_wait16(r0);
+          if (second) tmem_ld_wait16(r1);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            v0[i] = __uint_as_float(r0[i]);
+            v1[i] = second ? __uint_as_float(r1[i]) : 0.f;
+          }
+          return;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v0[i] = v1[i] = 0.f;
+        for (int c = c0; c <= c1; ++c) {
+          if (walk.chunk_at(bound(c), piece.start, piece.cost) >=
+              walk.chunk_at(bound(c + 1), piece.start, piece.cost))
+            continue;
+          const float* q = part_of(c) + static_cast<size_t>(b) * kBlockCols * kTileRows;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            v0[i] += __ldcg(q + i * kTileRows);
+            if (second) v1[i] += __ldcg(q + tile_floats + i * kTileRows);
+          }
+        }
+      };
+#pragma unroll
+      for (int i = 0; i < kMaxN / kBlockCols / 2; ++i) {
+        const int b = 2 * i + side;
+        if (b >= blocks) break;
+        float v0[16], v1[16];
+        take(b, v0, v1);
+        const int n = min(kBlockCols, piece.rows - b * kBlockCols);
+        if (kGated) {
+          uint32_t top[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float g = fminf(v0[j], p.limit), u = fminf(fmaxf(v1[j], -p.limit), p.limit);
+            // (a NaN would be lost in the limits)
+            const float y = g / (1.f + ex2_approx(-g * kLog2e)) * u *
+                            __shfl_sync(0xffffffffu, weight[i], j);
+            v0[j] = v0[j] != v0[j] || v1[j] != v1[j] ? NAN : y;
+            top[j] = __reduce_max_sync(0xffffffffu, __float_as_uint(v0[j]) & 0x7FFFFFFFu);
+          }
+          if (lane == 0) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 4)
+              *reinterpret_cast<uint4*>(&ctl->top[side][flip][quarter][j]) =
+                  make_uint4(top[j], top[j + 1], top[j + 2], top[j + 3]);
+          }
+          bar_sync(2 + side, 128);
+          uint8_t scale_code = 0;  // of column `lane`
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const uint32_t m = max(max(ctl->top[side][flip][0][j], ctl->top[side][flip][1][j]),
+                                   max(ctl->top[side][flip][2][j], ctl->top[side][flip][3][j]));
+            uint8_t code = 0x7F, e8 = 255;  // an infinity or NaN makes the block NaN
+            if (m < 0x7F800000u) {
+              const uint32_t s = __float_as_uint(pow2_scale_448(__uint_as_float(m))) >> 23;
+              const float q = v0[j] * __uint_as_float((254u - s) << 23);
+              unsigned short t;
+              asm("{ .reg .b16 h; cvt.rn.satfinite.e4m3x2.f32 h, %1, %1; mov.b16 %0, h; }"
+                  : "=h"(t) : "f"(q));
+              code = static_cast<uint8_t>(t & 0xFF);
+              e8 = static_cast<uint8_t>(s);
+            }
+            ctl->codes[side][flip][j][at] = code;
+            if (lane == j) scale_code = e8;
+          }
+          if (quarter == 0 && lane < n)
+            p.hs[static_cast<size_t>(piece.row0 + b * kBlockCols + lane) * (p.outs / kTileRows) +
+                 piece.row_tile] = scale_code;
+          bar_sync(2 + side, 128);
+          const int t = (threadIdx.x & 127) >> 3, v = threadIdx.x & 7;
+          if (t < n)
+            *reinterpret_cast<uint4*>(
+                p.hq + static_cast<size_t>(piece.row0 + b * kBlockCols + t) * p.outs +
+                piece.row_tile * kTileRows + v * 16) =
+                *reinterpret_cast<const uint4*>(&ctl->codes[side][flip][t][v * 16]);
+          flip ^= 1;
+        } else {
+          const int o0 = piece.row_tile * kOuts + at, o1 = o0 + kTileRows;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int d = __shfl_sync(0xffffffffu, row_out[i], j);
+            if (d < 0) continue;
+            const size_t base = static_cast<size_t>(d) * p.out_stride;
+            if (p.bf16) {
+              __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + base;
+              if (o0 < p.outs) o[o0] = __float2bfloat16_rn(v0[j]);
+              if (o1 < p.outs) o[o1] = __float2bfloat16_rn(v1[j]);
+            } else {
+              float* o = static_cast<float*>(p.out) + base;
+              if (o0 < p.outs) o[o0] = v0[j];
+              if (o1 < p.outs) o[o1] = v1[j];
+            }
+          }
+        }
+      }
+      if (!cut) release();
+    }
+  } else if (warp < kWarpCopy) {
+    // -------------------------------------------------------------- scales
+    // Lane l of each quarter holds outputs (rows) l, 32 + l, ... in
+    // consecutive columns; a column's four bytes are a chunk's four groups.
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const int pitch = p.width / 32;
+    const bool whole = chunks % 4 == 0;
+    const bool wide = whole && (reinterpret_cast<uintptr_t>(p.ws[0]) & 15) == 0 &&
+                      (!kGated || (reinterpret_cast<uintptr_t>(p.ws[1]) & 15) == 0);
+    const bool x_words = whole && (reinterpret_cast<uintptr_t>(p.xs) & 3) == 0;
+    unsigned n = 0;
+    bool good = true;
+    while (good && walk.next(&piece)) {
+      const uint8_t* wrow[2][4];
+      bool there[2][4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int row = piece.row_tile * kOuts + (kGated ? 0 : t * kTileRows) + j * 32 + lane;
+          there[t][j] = row < p.outs;
+          const uint8_t* base = p.ws[kGated ? t : 0];
+          if (kFp8)
+            wrow[t][j] = base + (static_cast<size_t>(piece.e) * ((p.outs + 127) / 128) +
+                                 min(row, p.outs - 1) / 128) * chunks;
+          else
+            wrow[t][j] = base + (static_cast<size_t>(piece.e) * p.outs + min(row, p.outs - 1)) * pitch;
+        }
+      const uint8_t* xrow[6];
+      bool x_there[6];
+#pragma unroll
+      for (int j = 0; j < 6; ++j) {
+        const int r = j * 32 + lane;
+        int s = -1;
+        if (r < piece.rows) s = p.src ? p.src[piece.row0 + r] : piece.row0 + r;
+        x_there[j] = s >= 0 && s < p.x_rows;
+        xrow[j] = p.xs + static_cast<size_t>(x_there[j] ? s : 0) * chunks;
+      }
+      for (int q = piece.lo / 4; good && q <= (piece.hi - 1) / 4; ++q) {
+        uint32_t wa[32], xb[32];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t v[4] = {0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu};
+            if (there[t][j]) {
+              if (kFp8) {
+                // (one block of 128 outputs: the same in every lane)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                  if (4 * q + c < chunks) v[c] = wrow[t][j][4 * q + c] * 0x01010101u;
+              } else if (wide) {
+                const uint4 u = __ldg(reinterpret_cast<const uint4*>(wrow[t][j] + 16 * q));
+                v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+              } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                  if (4 * q + c < chunks)
+                    v[c] = __ldg(reinterpret_cast<const uint32_t*>(wrow[t][j] + 16 * q) + c);
+              }
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) wa[c * 8 + t * 4 + j] = v[c];
+          }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint32_t w = 0x7F7F7F7Fu;
+          if (j < 6 && x_there[j < 6 ? j : 0]) {
+            const uint8_t* s = xrow[j < 6 ? j : 0] + 4 * q;
+            if (x_words) {
+              w = __ldg(reinterpret_cast<const uint32_t*>(s));
+            } else {
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                if (4 * q + c < chunks) w = (w & ~(0xFFu << (8 * c))) | (static_cast<uint32_t>(s[c]) << (8 * c));
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c) xb[c * 8 + j] = ((w >> (8 * c)) & 0xFFu) * 0x01010101u;
+        }
+        const int buf = n & 1;
+        good = wait_bar(&ctl->scale_empty[buf], ((n >> 1) & 1) ^ 1, abort_flag, err);
+        if (!good) break;
+        tc_fence_after();
+        tmem_st32(tmem + lanes + buf * kScaleCols, wa);
+        tmem_st32(tmem + lanes + buf * kScaleCols + 32, xb);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&ctl->scale_full[buf]);
+        ++n;
+      }
+    }
+  } else if (warp == kWarpCopy) {
+    // -------------------------------------------------------------- copies
+    unsigned n = 0;
+    bool good = true;
+    int s = 0;
+    uint32_t phase = 1;
+    while (good && walk.next(&piece)) {
+      int rows[2][4];
+      const int gathers = piece.n / 4;
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = (g * 32 + lane) * 4 + i;
+          rows[g][i] = -1;
+          if (r < piece.rows) rows[g][i] = p.src ? p.src[piece.row0 + r] : piece.row0 + r;
+        }
+      const bool second = two_tiles(piece);
+      // (a tile of E2M1 takes a byte an element in shared memory, but counts
+      // with what is read)
+      constexpr int kTileTx = kFp8 ? kATile : kATile / 2;
+      const uint32_t tx = (second ? 2 : 1) * kTileTx + piece.n * kChunk;
+      const int row = piece.row_tile * kOuts;
+      for (int c = piece.lo; c < piece.hi; ++c) {
+        good = wait_bar(&ctl->empty[s], phase, abort_flag, err);
+        good = __all_sync(0xffffffffu, good);
+        if (!good) break;
+        uint8_t* st = smem + static_cast<size_t>(s) * stage_bytes(a.n_max);
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&ctl->full[s], tx);
+          tma_load_3d(st, &map0, c * kChunk, row, piece.e, &ctl->full[s]);
+          if (second)
+            tma_load_3d(st + kATile, kGated ? &map1 : &map0, c * kChunk,
+                        kGated ? row : row + kTileRows, piece.e, &ctl->full[s]);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          if (g * 32 + lane < gathers)
+            tma_gather4(st + 2 * kATile + (g * 32 + lane) * 4 * kChunk, &xmap, c * kChunk, rows[g],
+                        &ctl->full[s]);
+        ++n;
+        if (++s == a.stages) {
+          s = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    // after an abort: no copy may be under way when the block ends
+    if (!good && lane == 0)
+      for (unsigned i = n < static_cast<unsigned>(a.stages) ? 0 : n - a.stages; i < n; ++i)
+        mbar_wait(&ctl->full[i % a.stages], (i / a.stages) & 1, err);
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- MMAs
+    if (lane == 0) {
+      const uint32_t idesc0 = ((kFp8 ? 0u : 5u) << 7) | (1u << 23) | (8u << 24);
+      unsigned uses[2] = {0, 0}, scales = 0;
+      int half = 0, s = 0;
+      uint32_t phase = 0;
+      bool good = true;
+      while (good && walk.next(&piece)) {
+        const bool big = piece.n > kHalfN, second = two_tiles(piece);
+        const int h = big ? 0 : half;
+        if (big) {
+          good = wait_bar(&ctl->sum_empty[0], (uses[0]++ & 1) ^ 1, abort_flag, err) &&
+                 wait_bar(&ctl->sum_empty[1], (uses[1]++ & 1) ^ 1, abort_flag, err);
+        } else {
+          good = wait_bar(&ctl->sum_empty[h], (uses[h]++ & 1) ^ 1, abort_flag, err);
+          half ^= 1;
+        }
+        const uint32_t d0 = tmem + kSumCol + (big ? 0 : h * kMaxN), d1 = d0 + (big ? kMaxN : kHalfN);
+        const uint32_t idesc = idesc0 | (static_cast<uint32_t>(piece.n >> 3) << 17);
+        for (int c = piece.lo; good && c < piece.hi; ++c) {
+          const int buf = scales & 1;
+          if (c == piece.lo || (c & 3) == 0)
+            good = wait_bar(&ctl->scale_full[buf], (scales >> 1) & 1, abort_flag, err);
+          good = good && wait_bar(&ctl->full[s], phase, abort_flag, err);
+          if (!good) break;
+          tc_fence_after();
+          const uint32_t base = smem_addr(smem + static_cast<size_t>(s) * stage_bytes(a.n_max));
+          const uint64_t a0 = umma_desc(base, 0, 1024), a1 = umma_desc(base + kATile, 0, 1024);
+          const uint64_t b0 = umma_desc(base + 2 * kATile, 0, 1024);
+          const uint32_t sa = tmem + buf * kScaleCols + (c & 3) * 8, sb = sa + 32;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t id = idesc | (static_cast<uint32_t>(k) << 4) | (static_cast<uint32_t>(k) << 29);
+            mma_scaled(d0, a0 + 2 * k, b0 + 2 * k, id, sa, sb, k > 0 || c > piece.lo);
+            if (second) mma_scaled(d1, a1 + 2 * k, b0 + 2 * k, id, sa + 4, sb, k > 0 || c > piece.lo);
+          }
+          mma_commit(&ctl->empty[s]);
+          if ((c & 3) == 3 || c + 1 == piece.hi) {
+            mma_commit(&ctl->scale_empty[buf]);
+            ++scales;
+          }
+          if (++s == a.stages) {
+            s = 0;
+            phase ^= 1;
+          }
+        }
+        if (!good) break;
+        mma_commit(&ctl->sum_full[h]);
+        if (big) mma_commit(&ctl->sum_full[1]);
+      }
+      mma_commit(&ctl->fin);
+      mbar_wait(&ctl->fin, 0, err);
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kWarpMma)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(kTmemCols)
+                 : "memory");
+}
+
+__global__ void grouped_reset_kernel(int* counters) {
+  pdl_wait();
+  pdl_trigger();
+  counters[threadIdx.x] = 0;
+}
+
+// --------------------------------------------------- routes, tokens' sums --
+
+constexpr int kGroupThreads = 1024, kGroupWarps = kGroupThreads / 32;
+constexpr int kGroupAhead = 8;
+
+struct GroupArgs {
+  const int* idx;    // [slots]
+  const float* wt;   // [slots]
+  int slots, topk, lo, experts;
+  int* offsets;      // [experts + 1]
+  int* slot;         // [slots] sorted by expert, in slot order within one
+  int* token;        // [slots] their tokens
+  float* weight;     // [slots] their weights
+  int* counters;     // two products' [kMaxShares]
+};
+
+// A stable counting sort by one block: each warp counts, then places, its own
+// stretch of the slots.
+__global__ void __launch_bounds__(kGroupThreads) group_kernel(const GroupArgs a) {
+  extern __shared__ int count[];  // [kGroupWarps][experts]
+  __shared__ int total[32], before;
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x < 2 * kMaxShares) a.counters[threadIdx.x] = 0;
+  for (int i = threadIdx.x; i < kGroupWarps * a.experts; i += kGroupThreads) count[i] = 0;
+  __syncthreads();
+  int* mine = count + warp * a.experts;
+  const int each = ((a.slots + kGroupThreads - 1) / kGroupThreads) * 32;  // slots of a warp
+  const int s0 = min(warp * each, a.slots), s1 = min(s0 + each, a.slots);
+  auto walk = [&](auto&& f) {
+    for (int base = s0; base < s1; base += 32 * kGroupAhead) {
+      int e[kGroupAhead];
+#pragma unroll
+      for (int i = 0; i < kGroupAhead; ++i) {
+        const int s = base + i * 32 + lane;
+        e[i] = s < s1 ? a.idx[s] - a.lo : -1;
+        if (e[i] >= a.experts || e[i] < 0) e[i] = -1;
+      }
+#pragma unroll
+      for (int i = 0; i < kGroupAhead; ++i) {
+        if (base + i * 32 >= s1) break;
+        const unsigned same = __match_any_sync(0xffffffffu, e[i]);
+        const int first = __ffs(same) - 1;
+        int at = 0;
+        if (lane == first && e[i] >= 0) {
+          at = mine[e[i]];
+          mine[e[i]] = at + __popc(same);
+        }
+        at = __shfl_sync(0xffffffffu, at, first) + __popc(same & ((1u << lane) - 1));
+        __syncwarp();
+        if (e[i] >= 0) f(base + i * 32 + lane, at);
+      }
+    }
+  };
+  walk([](int, int) {});
+  __syncthreads();
+  // counts to first places: over the experts, and the warps of one
+  if (threadIdx.x == 0) before = 0;
+  for (int e0 = 0; e0 < a.experts; e0 += kGroupThreads) {
+    const int e = e0 + threadIdx.x;
+    int sum = 0;
+    if (e < a.experts)
+      for (int w = 0; w < kGroupWarps; ++w) {
+        const int c = count[w * a.experts + e];
+        count[w * a.experts + e] = sum;
+        sum += c;
+      }
+    int incl = sum;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, incl, s);
+      if (lane >= s) incl += u;
+    }
+    if (lane == 31) total[warp] = incl;
+    __syncthreads();
+    if (warp == 0) {
+      const int t = total[lane];
+      int i = t;
+#pragma unroll
+      for (int s = 1; s < 32; s <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, i, s);
+        if (lane >= s) i += u;
+      }
+      total[lane] = i - t;
+    }
+    __syncthreads();
+    const int first = before + total[warp] + incl - sum;
+    __syncthreads();
+    if (e < a.experts) {
+      a.offsets[e] = first;
+      for (int w = 0; w < kGroupWarps; ++w) count[w * a.experts + e] += first;
+      if (e == a.experts - 1) a.offsets[a.experts] = first + sum;
+    }
+    if (threadIdx.x == kGroupThreads - 1) before = first + sum;
+    __syncthreads();
+  }
+  walk([&](int s, int at) {
+    a.slot[at] = s;
+    a.token[at] = s / a.topk;
+    a.weight[at] = a.wt[s];
+  });
+}
+
+// out[t] = the sum of the token's slots in route order; slots of experts that
+// are not here were not written. The slots are BF16, which is what a GEMV of
+// the layer hands on; their sum is fp32 and rounded once.
+__global__ void __launch_bounds__(256) experts_combine_kernel(const uint16_t* __restrict__ y,
+                                                              const int* __restrict__ idx, int n, int topk,
+                                                              int hidden, int lo, int experts,
+                                                              uint16_t* __restrict__ out) {
+  pdl_wait();
+  pdl_trigger();
+  const int vecs = hidden / 8;
+  const long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
+  if (i >= static_cast<long long>(n) * vecs) return;
+  const int t = static_cast<int>(i / vecs), v = static_cast<int>(i % vecs);
+  float sum[8] = {};
+  for (int k0 = 0; k0 < topk; k0 += 8) {
+    uint4 r[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      r[k] = make_uint4(0, 0, 0, 0);
+      if (k0 + k < topk) {
+        const int s = t * topk + k0 + k, e = idx[s] - lo;
+        if (e >= 0 && e < experts)
+          r[k] = __ldcs(reinterpret_cast<const uint4*>(y + static_cast<size_t>(s) * hidden) + v);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t w[4] = {r[k].x, r[k].y, r[k].z, r[k].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        sum[2 * j] += __uint_as_float(w[j] << 16);
+        sum[2 * j + 1] += __uint_as_float(w[j] & 0xFFFF0000u);
+      }
+    }
+  }
+  reinterpret_cast<uint4*>(out + static_cast<size_t>(t) * hidden)[v] =
+      make_uint4(pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3]),
+                 pack_bf16x2(sum[4], sum[5]), pack_bf16x2(sum[6], sum[7]));
+}
+
+// ------------------------------------------------------------------ host --
+
+int sm_count() {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 0;
+  return sms < kMaxShares ? sms : kMaxShares;
+}
+
+struct Shape {
+  int n_max, stages;
+};
+Shape tile_shape(const GroupedProblem& p) {
+  // rows of a group on average
+  if (p.rows <= 64ll * p.experts) return {64, 5};
+  return {kMaxN, 3};
+}
+
+size_t parts_bytes(const GroupedProblem& p) {
+  return static_cast<size_t>(sm_count()) * 4 * tile_shape(p).n_max * kTileRows * sizeof(float);
+}
+
+constexpr size_t kCounterBytes = kMaxShares * sizeof(int);
+
+bool weight_map(CUtensorMap* m, const GroupedProblem& p, const uint8_t* w) {
+  if (p.fp8)
+    return make_tma_map_u8_3d(m, w, p.width, p.outs, p.width, p.experts,
+                              static_cast<uint64_t>(p.outs) * p.width, kChunk, kTileRows, 1);
+  return make_tma_map_u4_3d(m, w, p.width, p.outs, p.experts, kTileRows);
+}
+
+cudaError_t launch(const GroupedProblem& p, int* counters, float* parts, cudaStream_t st) {
+  const bool gated = p.w[1] != nullptr;
+  CUtensorMap map0, map1, xmap;
+  if (!weight_map(&map0, p, p.w[0]) || !weight_map(&map1, p, gated ? p.w[1] : p.w[0]) ||
+      !make_tma_map_u8(&xmap, p.xq, p.width, p.x_rows, kChunk, 1, true, false))
+    return cudaErrorInvalidValue;
+  Args a;
+  a.p = p;
+  a.shares = sm_count();
+  const Shape s = tile_shape(p);
+  a.n_max = s.n_max;
+  a.stages = s.stages;
+  a.counters = counters;
+  a.parts = parts;
+  if (a.shares < 1) return cudaErrorInvalidDevice;
+  if (gated && p.fp8) return cudaErrorInvalidValue;
+  auto kernel = gated ? grouped_kernel<false, true>
+                      : p.fp8 ? grouped_kernel<true, false> : grouped_kernel<false, false>;
+  cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), 227 * 1024);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kernel, dim3(a.shares), dim3(kThreads),
+                    smem_bytes(s.n_max, s.stages, p.experts), st, map0, map1, xmap, a);
+}
+
+// Pieces of a buffer, 256-byte aligned.
+struct Carver {
+  char* at;
+  size_t used = 0;
+  template <class T>
+  T* take(size_t n) {
+    T* p = reinterpret_cast<T*>(at + used);
+    used += (n * sizeof(T) + 255) & ~static_cast<size_t>(255);
+    return p;
+  }
+};
+
+struct ExpertsWork {
+  int *counters, *offsets, *slot, *token;
+  float *weight, *parts;
+  uint8_t *hq, *hs;
+  uint16_t* y;
+  size_t bytes;
+};
+
+GroupedProblem gate_up(const ExpertsProblem& p, const ExpertsWork& w) {
+  GroupedProblem g;
+  g.experts = p.experts;
+  g.rows = p.n * p.topk;
+  g.outs = p.inter;
+  g.width = p.hidden;
+  g.w[0] = p.w1; g.ws[0] = p.s1;
+  g.w[1] = p.w3; g.ws[1] = p.s3;
+  g.xq = p.xq;
+  g.xs = p.xs;
+  g.x_rows = p.n;
+  g.offsets = w.offsets;
+  g.src = w.token;
+  g.limit = p.limit;
+  g.weight = w.weight;
+  g.hq = w.hq;
+  g.hs = w.hs;
+  g.err = p.err;
+  return g;
+}
+
+ExpertsWork experts_work(const ExpertsProblem& p, void* base) {
+  Carver c{static_cast<char*>(base)};
+  const size_t slots = static_cast<size_t>(p.n) * p.topk;
+  ExpertsWork w;
+  w.counters = c.take<int>(2 * kMaxShares);
+  w.offsets = c.take<int>(p.experts + 1);
+  w.slot = c.take<int>(slots);
+  w.token = c.take<int>(slots);
+  w.weight = c.take<float>(slots);
+  w.hq = c.take<uint8_t>(slots * p.inter);
+  w.hs = c.take<uint8_t>(slots * (p.inter / 128));
+  w.y = c.take<uint16_t>(slots * p.hidden);
+  w.parts = c.take<float>(parts_bytes(gate_up(p, w)) / sizeof(float));
+  w.bytes = c.used;
+  return w;
+}
+
+}  // namespace
+
+size_t grouped_workspace_bytes(const GroupedProblem& p) { return kCounterBytes + parts_bytes(p); }
+
+cudaError_t grouped_reset(void* ws, cudaStream_t st) {
+  return launch_pdl(grouped_reset_kernel, dim3(1), dim3(kMaxShares), 0, st, static_cast<int*>(ws));
+}
+
+cudaError_t grouped_forward(const GroupedProblem& p, void* ws, cudaStream_t st) {
+  if (p.rows <= 0) return cudaSuccess;
+  return launch(p, static_cast<int*>(ws),
+                reinterpret_cast<float*>(static_cast<char*>(ws) + kCounterBytes), st);
+}
+
+size_t experts_workspace_bytes(const ExpertsProblem& p) { return experts_work(p, nullptr).bytes; }
+
+cudaError_t experts_forward(const ExpertsProblem& p, void* ws, cudaStream_t st) {
+  if (p.n <= 0) return cudaSuccess;
+  const ExpertsWork w = experts_work(p, ws);
+  GroupArgs a;
+  a.idx = p.idx;
+  a.wt = p.wt;
+  a.slots = p.n * p.topk;
+  a.topk = p.topk;
+  a.lo = p.lo;
+  a.experts = p.experts;
+  a.offsets = w.offsets;
+  a.slot = w.slot;
+  a.token = w.token;
+  a.weight = w.weight;
+  a.counters = w.counters;
+  const size_t smem = sizeof(int) * kGroupWarps * p.experts;
+  cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(group_kernel),
+                                       static_cast<int>(sizeof(int)) * kGroupWarps * kGroupedMaxExperts);
+  if (e == cudaSuccess) e = launch_pdl(group_kernel, dim3(1), dim3(kGroupThreads), smem, st, a);
+  if (e != cudaSuccess) return e;
+  const GroupedProblem g = gate_up(p, w);
+  e = launch(g, w.counters, w.parts, st);
+  if (e != cudaSuccess) return e;
+  GroupedProblem d;
+  d.experts = p.experts;
+  d.rows = g.rows;
+  d.outs = p.hidden;
+  d.width = p.inter;
+  d.w[0] = p.w2;
+  d.ws[0] = p.s2;
+  d.xq = w.hq;
+  d.xs = w.hs;
+  d.x_rows = g.rows;
+  d.offsets = w.offsets;
+  d.dst = w.slot;
+  d.out_rows = g.rows;
+  d.out = w.y;
+  d.out_stride = p.hidden;
+  d.err = p.err;
+  e = launch(d, w.counters + kMaxShares, w.parts, st);
+  if (e != cudaSuccess) return e;
+  const long long vecs = static_cast<long long>(p.n) * (p.hidden / 8);
+  return launch_pdl(experts_combine_kernel, dim3(static_cast<unsigned>((vecs + 255) / 256)), dim3(256),
+                    0, st, static_cast<const uint16_t*>(w.y), p.idx, p.n, p.topk, p.hidden, p.lo,
+                    p.experts, p.out);
+}
+
+}  // namespace dsv4

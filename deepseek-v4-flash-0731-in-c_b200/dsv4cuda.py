@@ -88,6 +88,10 @@ lib.dsv4cuda_moe_ep_push.restype = C.c_int
 lib.dsv4cuda_moe_ep_push.argtypes = [vp, C.c_int, vp]
 lib.dsv4cuda_moe_ep_combine.restype = C.c_int
 lib.dsv4cuda_moe_ep_combine.argtypes = [vp, C.c_int, vp, vp]
+lib.dsv4cuda_moe_experts_workspace_bytes.restype = C.c_size_t
+lib.dsv4cuda_moe_experts_workspace_bytes.argtypes = [vp, C.c_int]
+lib.dsv4cuda_moe_experts.restype = C.c_int
+lib.dsv4cuda_moe_experts.argtypes = [vp, vp, vp, vp, vp, C.c_int, vp, vp, C.c_size_t, vp]
 lib.dsv4cuda_ipc_alloc.restype = C.c_int
 lib.dsv4cuda_ipc_alloc.argtypes = [C.c_size_t, C.POINTER(vp), C.c_char_p]
 lib.dsv4cuda_ipc_open.restype = C.c_int
@@ -381,6 +385,26 @@ class MoeLayer:
         _check(lib.dsv4cuda_moe_forward_local(self.handle, x.data_ptr(),
                                               None if token_ids is None else token_ids.data_ptr(),
                                               x.shape[0], _stream(stream)))
+
+    def experts_workspace_bytes(self, n_tokens) -> int:
+        """Workspace of an experts call of n_tokens."""
+        return lib.dsv4cuda_moe_experts_workspace_bytes(self.handle, n_tokens)
+
+    def experts(self, xq, xs, idx, wt, out, workspace=None, stream=None):
+        """The routed experts of any number of tokens (dsv4cuda_moe_experts): xq uint8
+        [n][hidden] E4M3 codes, xs uint8 [n][hidden / 128] E8M0 scales, idx int32 and
+        wt fp32 [n][topk], out BF16 [n][hidden]. workspace: a CUDA uint8 tensor (needed
+        while capturing)."""
+        import torch
+        n = xq.shape[0]
+        u8 = torch.uint8
+        if xq.dim() != 2 or xq.shape[1] != self.hidden:
+            raise ValueError(f"xq: [n][{self.hidden}] is wanted")
+        _check(lib.dsv4cuda_moe_experts(
+            self.handle, _dev(xq, "xq", u8), _dev(xs, "xs", u8, n * (self.hidden // 128)),
+            _dev(idx, "idx", torch.int32, n * self.topk), _dev(wt, "wt", torch.float32, n * self.topk),
+            n, _dev(out, "out", torch.bfloat16, n * self.hidden), _dev(workspace, "workspace", u8),
+            0 if workspace is None else workspace.numel(), _stream(stream)))
 
     def routed_slots(self, n_tokens):
         """torch CUDA float32 view [n][topk][H] of the layer's routed slots."""
@@ -779,6 +803,64 @@ def paged_attn(out, q, paged: PagedCache, layer, q_start, max_new, max_len, scal
         _dev(rope_cos, "rope_cos", f32, half), _dev(rope_sin, "rope_sin", f32, half),
         _dev(lse, "lse", f32, n * heads), C.byref(shape),
         _dev(workspace, "workspace", torch.uint8), 0 if workspace is None else workspace.numel(),
+        _stream(stream)))
+
+
+# ------------------------------------------------------- grouped products --
+class GroupedShape(C.Structure):
+    _fields_ = [("n_groups", C.c_int), ("n_rows", C.c_int), ("x_rows", C.c_int),
+                ("out_rows", C.c_int), ("outs", C.c_int), ("width", C.c_int), ("fp8", C.c_int),
+                ("bf16", C.c_int), ("out_stride", C.c_longlong)]
+
+
+lib.dsv4cuda_grouped_workspace_bytes.restype = C.c_size_t
+lib.dsv4cuda_grouped_workspace_bytes.argtypes = [vp]
+lib.dsv4cuda_grouped_gemm.restype = C.c_int
+lib.dsv4cuda_grouped_gemm.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]
+
+
+def _grouped_shape(out, xq, w, n_rows):
+    import torch
+    if w.dim() != 3 or xq.dim() != 2 or out.dim() != 2:
+        raise ValueError("out [rows][outs], xq [rows][width] and w [groups][outs][width or width / 2] "
+                         "are wanted")
+    groups, outs, held = w.shape
+    width = xq.shape[1]
+    if held not in (width, width // 2) or out.shape[1] != outs:
+        raise ValueError(f"w: rows of {width} E4M3 or {width // 2} packed E2M1 bytes and {out.shape[1]} "
+                         f"outputs are wanted, got {held} and {outs}")
+    if out.dtype not in (torch.bfloat16, torch.float32) or not out.is_cuda or out.stride(1) != 1:
+        raise ValueError("out: a CUDA tensor of bfloat16 or float32, the values of a row one behind "
+                         "the other")
+    if out.shape[0] > 1 and out.stride(0) < outs:
+        raise ValueError("out: the rows must not overlap")
+    return GroupedShape(groups, n_rows, xq.shape[0], out.shape[0], outs, width, int(held == width),
+                        int(out.dtype is torch.bfloat16), out.stride(0) if out.shape[0] > 1 else 0)
+
+
+def grouped_workspace_bytes(out, xq, w, n_rows) -> int:
+    """Workspace of a grouped_gemm call of these tensors (n_rows: of src, or of xq)."""
+    return lib.dsv4cuda_grouped_workspace_bytes(C.byref(_grouped_shape(out, xq, w, n_rows)))
+
+
+def grouped_gemm(out, xq, xs, w, ws, offsets, src=None, dst=None, workspace=None, stream=None):
+    """dsv4cuda_grouped_gemm: out (BF16 or fp32) rows dst[r] = row src[r] of x times
+    matrix g of w, for offsets[g] <= r < offsets[g + 1]. uint8 CUDA tensors: xq [x_rows][width]
+    E4M3 codes with xs [x_rows][width / 128] E8M0 scales, w [groups][outs][width / 2] packed
+    E2M1 with ws [groups][outs][width / 32], or w [groups][outs][width] E4M3 with ws
+    [groups][ceil(outs / 128)][width / 128]; int32: offsets [groups + 1], src and dst (both
+    optional: row r). workspace: a CUDA uint8 tensor (needed while capturing)."""
+    import torch
+    u8, i32 = torch.uint8, torch.int32
+    rows = src.numel() if src is not None else dst.numel() if dst is not None else xq.shape[0]
+    s = _grouped_shape(out, xq, w, rows)
+    scales = s.n_groups * (((s.outs + 127) // 128) * (s.width // 128) if s.fp8
+                           else s.outs * (s.width // 32))
+    _check(lib.dsv4cuda_grouped_gemm(
+        out.data_ptr(), _dev(xq, "xq", u8), _dev(xs, "xs", u8, s.x_rows * (s.width // 128)),
+        _dev(w, "w", u8), _dev(ws, "ws", u8, scales), _dev(offsets, "offsets", i32, s.n_groups + 1),
+        _dev(src, "src", i32, rows), _dev(dst, "dst", i32, rows), C.byref(s),
+        _dev(workspace, "workspace", u8), 0 if workspace is None else workspace.numel(),
         _stream(stream)))
 
 

@@ -256,6 +256,63 @@ int dsv4cuda_moe_forward_noalloc(const dsv4cuda_moe_config *cfg,
                                  const dsv4cuda_moe_weights *device_weights,
                                  const float *x, const int *token_ids, int n_tokens,
                                  float *out, void *stream);
+/* ---- The routed experts of many rows (moe_forward_batch's expert part,
+ * src/dsv4/dsv4_model.c:6812, for any number of tokens: a prompt's chunk, a
+ * batch of sequences, one token) on the block-scaled tensor cores. x comes
+ * as E4M3 codes xq [n][hidden] with one E8M0 scale per 128 columns xs
+ * [n][hidden / 128] (dsv4cuda_norm_quant's), the routes as idx [n][topk] with
+ * their weights wt [n][topk]:
+ *   h   = silu(min(x w1, L)) * clamp(x w3, -L, L) * wt, quantised like x
+ *         (L the layer's swiglu_limit)
+ *   out [n][hidden] BF16 = the sum of h w2 over the token's routes, in their
+ *         order; the slots that are summed are BF16, as the layer's GEMVs
+ *         leave them.
+ * Products are summed in fp32 in an order of their own: results agree with
+ * dsv4cuda_moe_forward's within the rounding of its BF16 boundaries, and are
+ * the same from call to call. Routes to experts that are not here (an
+ * expert-parallel layer's others, or any number outside) add nothing. A NaN
+ * code or scale (255) makes what it enters NaN (the GEMVs skip such scales),
+ * a value of h that is not finite its block of 128. The router and the shared
+ * expert are not part of it. hidden and moe_inter have to be multiples of 128,
+ * at most 1024 experts; idx, wt, out are DEVICE pointers, xq, w1, w3, w2 and
+ * out aligned to 32 bytes. workspace may be NULL (a buffer per thread and
+ * stream that grows); give one, 256-byte aligned, while capturing. Calls that
+ * share a workspace must not overlap. */
+size_t dsv4cuda_moe_experts_workspace_bytes(const dsv4cuda_moe_layer *L, int n_tokens);
+int dsv4cuda_moe_experts(dsv4cuda_moe_layer *L, const uint8_t *xq, const uint8_t *xs,
+                         const int *idx, const float *wt, int n_tokens, uint16_t *out,
+                         void *workspace, size_t workspace_bytes, void *stream);
+
+/* Products of rows grouped by matrix (batched forms of dsv4_gemv_fp4_batch_q
+ * and dsv4_gemv_fp8_batch_q, src/dsv4/dsv4_model.c:967-1220, :678, without
+ * their limit of rows): row r with offsets[g] <= r < offsets[g + 1] is
+ * multiplied with matrix g of w [n_groups][outs][width]:
+ *   out[dst[r]][i] = sum_k x[src[r]][k] w[g][i][k]
+ * offsets [n_groups + 1] are read on the device, ascending, at most n_rows;
+ * groups may be empty. One group is a dense product. src, dst [n_rows] may be
+ * NULL (row r); a src outside x_rows stands for zeros, a dst outside out_rows
+ * is not written, nor are the rows of out that no dst names. width is a
+ * multiple of 128. Weights: fp8 = 0 packed E2M1 (the low nibble first) with
+ * E8M0 ws [n_groups][outs][width / 32]; fp8 = 1 E4M3 with ws
+ * [n_groups][ceil(outs / 128)][width / 128]. x as above. out: BF16 or fp32, the
+ * fp32 sums rounded once. Results are the same from call to call. DEVICE
+ * pointers; xq 16-byte aligned, w 32, ws 4 (E2M1). workspace as above. */
+typedef struct {
+    int n_groups;         /* 1 .. 1024 */
+    int n_rows;           /* rows of src and dst; bound of offsets */
+    int x_rows, out_rows;
+    int outs, width;
+    int fp8;              /* type of w */
+    int bf16;             /* type of out: 1 BF16, 0 fp32 */
+    long long out_stride; /* elements between rows of out (0: outs) */
+} dsv4cuda_grouped_shape;
+
+size_t dsv4cuda_grouped_workspace_bytes(const dsv4cuda_grouped_shape *shape);
+int dsv4cuda_grouped_gemm(void *out, const uint8_t *xq, const uint8_t *xs, const uint8_t *w,
+                          const uint8_t *ws, const int *offsets, const int *src, const int *dst,
+                          const dsv4cuda_grouped_shape *shape, void *workspace,
+                          size_t workspace_bytes, void *stream);
+
 /* Device bytes the layer holds (weights it owns + workspace). */
 size_t dsv4cuda_moe_device_bytes(const dsv4cuda_moe_layer *L);
 
