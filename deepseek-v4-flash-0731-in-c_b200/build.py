@@ -17,7 +17,8 @@ CSRC = os.path.join(PKG, "csrc")
 LIBDIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIBDIR, "libdsv4_cuda.so")
 SOURCES = ["gemv.cu", "moe.cu", "attn.cu", "sample.cu", "snapshot.cu", "ep.cu", "decode.cu",
-           "paged.cu", "paged_attn.cu", "logprob.cu", "grouped.cu", "capi.cu"]
+           "paged.cu", "paged_attn.cu", "logprob.cu", "grouped.cu", "norm.cu",
+           "beam.cu", "capi.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",

@@ -26,8 +26,10 @@
 #include "snapshot.cuh"
 #include "paged.cuh"
 #include "paged_attn.cuh"
+#include "beam.cuh"
 #include "grouped.cuh"
 #include "logprob.cuh"
+#include "norm.cuh"
 #include "ep.cuh"
 #include "../../include/dsv4_cuda.h"
 
@@ -1985,6 +1987,145 @@ DSV4_API int dsv4cuda_grouped_gemm(void* out, const uint8_t* xq, const uint8_t* 
   if (!work) return -1;
   cudaError_t e = dsv4::grouped_reset(work, st);
   if (e == cudaSuccess) e = dsv4::grouped_forward(p, work, st);
+  if (e != cudaSuccess) { record_error("%s: %s", who, cudaGetErrorString(e)); return -1; }
+  return 0;
+}
+
+// ============================================ norm, latents' write, beams ==
+
+DSV4_API int dsv4cuda_norm_quant(const void* x, const void* residual, void* sum, void* out,
+                                 const uint16_t* gain, uint8_t* codes, uint8_t* scales,
+                                 const dsv4cuda_norm_shape* s, void* stream) {
+  const char* who = "dsv4cuda_norm_quant";
+  if (!s || s->n_rows < 0 || s->width < 1 || s->width > dsv4::kNormMaxWidth || !(s->eps > 0.f) ||
+      s->eps > 3e38f) {
+    record_error("%s: bad shape (width 1..%d, eps positive and finite)", who, dsv4::kNormMaxWidth);
+    return -1;
+  }
+  if (s->n_rows == 0) return 0;
+  dsv4::NormProblem p;
+  p.rows = s->n_rows;
+  p.width = s->width;
+  p.bf16 = s->bf16 != 0;
+  p.x_stride = s->x_stride ? s->x_stride : s->width;
+  p.residual_stride = s->residual_stride ? s->residual_stride : s->width;
+  p.sum_stride = s->sum_stride ? s->sum_stride : s->width;
+  p.out_stride = s->out_stride ? s->out_stride : s->width;
+  const size_t size = p.bf16 ? 2 : 4;
+  if (!x || !codes || !scales || !aligned(x, size) || !aligned(residual, size) ||
+      !aligned(sum, size) || !aligned(out, size) || !aligned(gain, 2) || p.x_stride < s->width ||
+      p.residual_stride < s->width || p.sum_stride < s->width || p.out_stride < s->width) {
+    record_error("%s: bad arguments (strides at least width)", who);
+    return -1;
+  }
+  p.x = x;
+  p.residual = residual;
+  p.sum = sum;
+  p.out = out;
+  p.gain = gain;
+  p.eps = s->eps;
+  p.codes = codes;
+  p.scales = scales;
+  cudaError_t e = dsv4::norm_quant(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) { record_error("%s: %s", who, cudaGetErrorString(e)); return -1; }
+  return 0;
+}
+
+DSV4_API int dsv4cuda_paged_write(const dsv4cuda_paged* p, int layer, const void* kv, int bf16,
+                                  long long stride, const long long* rows, int n,
+                                  const uint16_t* gain, float eps, const float* rope_cos,
+                                  const float* rope_sin, void* stream) {
+  const char* who = "dsv4cuda_paged_write";
+  dsv4::PagedState s;
+  if (!paged_state(who, p, &s)) return -1;
+  if (layer < 0 || layer >= s.layers || n < 0) {
+    record_error("%s: layer %d of %d, %d latents", who, layer, s.layers, n);
+    return -1;
+  }
+  if (n == 0) return 0;
+  const int d = s.nope + s.rope_dim;
+  dsv4::LatentWrite a;
+  a.stride = stride ? stride : d;
+  if (!kv || !rows || !aligned(kv, bf16 ? 2 : 4) || !aligned(gain, 2) || a.stride < d ||
+      s.rope_dim % 2 || (rope_cos == nullptr) != (rope_sin == nullptr) ||
+      (gain && !(eps > 0.f && eps < 3e38f))) {
+    record_error("%s: bad arguments (stride at least nope + rope_dim, an even rope_dim, cos and sin "
+                 "together, eps positive and finite)", who);
+    return -1;
+  }
+  a.cache.codes = s.codes[layer];
+  a.cache.scales = s.scales[layer];
+  a.cache.rope = s.rope[layer];
+  a.cache.nope = s.nope;
+  a.cache.rope_dim = s.rope_dim;
+  a.cache.rows = static_cast<long long>(s.n_pages) * s.page;
+  a.kv = kv;
+  a.bf16 = bf16 != 0;
+  a.rows = rows;
+  a.n = n;
+  a.gain = gain;
+  a.eps = eps;
+  a.rope_cos = rope_cos;
+  a.rope_sin = rope_sin;
+  cudaError_t e = dsv4::latent_write(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) { record_error("%s: %s", who, cudaGetErrorString(e)); return -1; }
+  return 0;
+}
+
+namespace {
+bool beam_problem(const char* who, const dsv4cuda_beam_shape* s, dsv4::BeamProblem* p) {
+  static_assert(DSV4CUDA_MAX_BEAMS == dsv4::kMaxBeams, "limit");
+  static_assert(DSV4CUDA_MAX_BEAM_CANDIDATES == dsv4::kMaxBeamCandidates, "limit");
+  if (!s || s->n_groups < 0 || s->beams < 1 || s->beams > dsv4::kMaxBeams || s->n_cands < 1 ||
+      s->n_cands > dsv4::kMaxBeamCandidates || s->vocab < 1 || (s->stride && s->stride < s->vocab) ||
+      static_cast<long long>(s->n_groups) * s->beams > 0x7FFFFFFFll) {
+    record_error("%s: bad shape (1..%d beams and candidates, stride at least vocab)", who,
+                 dsv4::kMaxBeams);
+    return false;
+  }
+  p->groups = s->n_groups;
+  p->beams = s->beams;
+  p->cands = s->n_cands;
+  p->vocab = s->vocab;
+  p->bf16 = s->bf16 != 0;
+  p->eos = s->eos < 0 ? -2 : s->eos;  // -1 is a candidate's token where there is none
+  p->stride = s->stride ? s->stride : s->vocab;
+  return true;
+}
+}  // namespace
+
+DSV4_API size_t dsv4cuda_beam_workspace_bytes(const dsv4cuda_beam_shape* shape) {
+  dsv4::BeamProblem p;
+  if (!beam_problem("dsv4cuda_beam_workspace_bytes", shape, &p)) return 0;
+  return dsv4::beam_workspace_bytes(p);
+}
+
+DSV4_API int dsv4cuda_beam_select(const void* logits, const float* score, int* parent, int* token,
+                                  float* total, int* next, const int* slot, int* dst, int* src,
+                                  const dsv4cuda_beam_shape* shape, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  const char* who = "dsv4cuda_beam_select";
+  dsv4::BeamProblem p;
+  if (!beam_problem(who, shape, &p)) return -1;
+  if (p.groups == 0) return 0;
+  if (!logits || !score || !parent || !token || !total || !next || !aligned(logits, p.bf16 ? 2 : 4) ||
+      (slot != nullptr) != (dst != nullptr) || (slot != nullptr) != (src != nullptr)) {
+    record_error("%s: bad arguments (slot, dst and src together)", who);
+    return -1;
+  }
+  p.logits = logits;
+  p.score = score;
+  p.parent = parent;
+  p.token = token;
+  p.total = total;
+  p.next = next;
+  p.slot = slot;
+  p.dst = dst;
+  p.src = src;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  void* ws = pick_workspace(who, workspace, workspace_bytes, dsv4::beam_workspace_bytes(p), st);
+  if (!ws) return -1;
+  cudaError_t e = dsv4::beam_select(p, ws, st);
   if (e != cudaSuccess) { record_error("%s: %s", who, cudaGetErrorString(e)); return -1; }
   return 0;
 }

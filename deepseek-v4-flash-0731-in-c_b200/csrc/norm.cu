@@ -1,0 +1,383 @@
+// norm.cu - RMS norm of rows with the residual's addition and an 8-bit
+// output, and the write of new latents into their pages.
+//
+//   v = x + residual,  y = v / sqrt(mean v^2 + eps) * gain
+//   per 128 columns: 2^e the smallest power of two with max |y| <= 448 2^e,
+//   codes = E4M3(y / 2^e)
+//
+// One read and one write: a row stays in the registers of its threads, eight
+// consecutive values a vector, so that 16 lanes hold a block of 128 and its
+// maximum is four shuffles. Sum and square are fp32 from the inputs' sum on;
+// each output is rounded once, from fp32.
+#include "norm.cuh"
+
+#include <cmath>
+#include <cuda_bf16.h>
+
+#include "launch.cuh"
+#include "umma.cuh"
+
+namespace dsv4 {
+namespace {
+
+constexpr int kVec = 8;  // values of a vector
+
+template <bool kBf16>
+__device__ __forceinline__ void load8(const void* row, int i, int n, bool wide, float (&v)[kVec]) {
+  if (kBf16) {
+    const uint16_t* p = static_cast<const uint16_t*>(row) + i;
+    if (wide) {
+      const uint4 u = *reinterpret_cast<const uint4*>(p);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[2 * k] = __uint_as_float(w[k] << 16);
+        v[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+      }
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) v[k] = k < n ? bf16_widen(p[k]) : 0.f;
+  } else {
+    const float* p = static_cast<const float*>(row) + i;
+    if (wide) {
+      const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) v[k] = k < n ? p[k] : 0.f;
+  }
+}
+
+template <bool kBf16>
+__device__ __forceinline__ void store8(void* row, int i, int n, bool wide, const float (&v)[kVec]) {
+  if (kBf16) {
+    __nv_bfloat16* p = static_cast<__nv_bfloat16*>(row) + i;
+    if (wide) {
+      *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                                pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < kVec; ++k)
+      if (k < n) p[k] = __float2bfloat16_rn(v[k]);
+  } else {
+    float* p = static_cast<float*>(row) + i;
+    if (wide) {
+      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < kVec; ++k)
+      if (k < n) p[k] = v[k];
+  }
+}
+
+// Eight E4M3 codes of v * inv, low byte first; an exact zero of either sign is +0,
+// as the cache's other writers have it.
+__device__ __forceinline__ uint2 codes8(const float (&v)[kVec], float inv) {
+  uint32_t h[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    unsigned short t;
+    asm("{ .reg .b16 h; cvt.rn.satfinite.e4m3x2.f32 h, %2, %1; mov.b16 %0, h; }"
+        : "=h"(t) : "f"(fmaf(v[2 * k], inv, 0.f)), "f"(fmaf(v[2 * k + 1], inv, 0.f)));
+    h[k] = t;
+  }
+  return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+}
+
+// The magnitude bits order like the magnitudes, infinities and NaN above all.
+__device__ __forceinline__ uint32_t top8(const float (&v)[kVec]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int k = 0; k < kVec; ++k) m = max(m, __float_as_uint(v[k]) & 0x7FFFFFFFu);
+  return m;
+}
+
+struct NormArgs {
+  NormProblem p;
+  int threads;                       // of a row
+  bool wide_x, wide_r, wide_s, wide_o, wide_g, wide_c;  // whole aligned vectors
+};
+
+// kVecs vectors a thread; blockDim.x / threads rows a block.
+template <bool kBf16, int kVecs>
+__global__ void __launch_bounds__(1024) norm_quant_kernel(const NormArgs a) {
+  __shared__ float part[32];
+  const NormProblem& p = a.p;
+  const int sub = threadIdx.x / a.threads, tid = threadIdx.x - sub * a.threads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x / a.threads) + sub;
+  const bool live = row < p.rows;
+  constexpr int kSize = kBf16 ? 2 : 4;
+  auto at = [&](const void* base, long long stride) {
+    return static_cast<const char*>(base) + row * stride * kSize;
+  };
+  pdl_wait();
+  pdl_trigger();
+  float v[kVecs][kVec];
+  float squares = 0.f;
+#pragma unroll
+  for (int j = 0; j < kVecs; ++j) {
+    const int i = (tid + j * a.threads) * kVec, n = min(kVec, p.width - i);
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) v[j][k] = 0.f;
+    if (live && n > 0) load8<kBf16>(at(p.x, p.x_stride), i, n, a.wide_x, v[j]);
+  }
+  if (p.residual) {
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) {
+      const int i = (tid + j * a.threads) * kVec, n = min(kVec, p.width - i);
+      float r[kVec];
+      if (live && n > 0) {
+        load8<kBf16>(at(p.residual, p.residual_stride), i, n, a.wide_r, r);
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) v[j][k] += r[k];
+      }
+    }
+  }
+  if (p.sum && live) {
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) {
+      const int i = (tid + j * a.threads) * kVec, n = min(kVec, p.width - i);
+      if (n > 0) store8<kBf16>(const_cast<char*>(at(p.sum, p.sum_stride)), i, n, a.wide_s, v[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kVecs; ++j)
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) squares = fmaf(v[j][k], v[j][k], squares);
+  // over the row's warps
+  const int warps = a.threads >> 5, first = warp - (tid >> 5);
+  auto row_sum = [&](float s) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (warps > 1) {
+      if (lane == 0) part[warp] = s;
+      __syncthreads();
+      s = lane < warps ? part[first + lane] : 0.f;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    }
+    return s;
+  };
+  float mean = row_sum(squares) / p.width, eps = p.eps;
+  // Squares beyond fp32 (values from 1.8e19 on): again, of values times
+  // 2^-76. All rows of a block take the step together.
+  const bool over = !(mean <= 3.0e38f);
+  if (__syncthreads_or(over)) {
+    constexpr float kDown = 1.3234889800848443e-23f;  // 2^-76
+    squares = 0.f;
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j)
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) {
+        const float d = v[j][k] * kDown;
+        squares = fmaf(d, d, squares);
+      }
+    const float m = row_sum(squares) / p.width;
+    if (over) {
+      mean = m;
+      eps = 0.f;  // eps 2^-152 is nothing beside it
+#pragma unroll
+      for (int j = 0; j < kVecs; ++j)
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) v[j][k] *= kDown;
+    }
+  }
+  const float rs = rsqrtf(mean + eps);
+  const int blocks = (p.width + 127) / 128;
+#pragma unroll
+  for (int j = 0; j < kVecs; ++j) {
+    const int i = (tid + j * a.threads) * kVec, n = min(kVec, p.width - i);
+    const bool in = live && n > 0;
+    float g[kVec];
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) g[k] = 1.f;
+    if (p.gain && n > 0) load8<true>(p.gain, i, n, a.wide_g, g);
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) v[j][k] = k < n ? v[j][k] * rs * g[k] : 0.f;
+    if (p.out && in) store8<kBf16>(const_cast<char*>(at(p.out, p.out_stride)), i, n, a.wide_o, v[j]);
+    uint32_t top = top8(v[j]);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    uint2 c = make_uint2(0x7F7F7F7Fu, 0x7F7F7F7Fu);  // an infinity or NaN makes the block NaN
+    uint32_t e8 = 255;
+    if (top < 0x7F800000u) {
+      e8 = __float_as_uint(pow2_scale_448(__uint_as_float(top))) >> 23;
+      c = codes8(v[j], __uint_as_float((254u - e8) << 23));
+    }
+    if (!in) continue;
+    uint8_t* to = p.codes + row * p.width + i;
+    if (a.wide_c) {
+      *reinterpret_cast<uint2*>(to) = c;
+    } else {
+#pragma unroll
+      for (int k = 0; k < kVec; ++k)
+        if (k < n) to[k] = static_cast<uint8_t>((k < 4 ? c.x : c.y) >> (8 * (k & 3)));
+    }
+    if ((tid & 15) == 0) p.scales[row * blocks + i / 128] = static_cast<uint8_t>(e8);
+  }
+}
+
+// A warp per latent: the non-RoPE dims eight a vector (a scale's 64 are eight
+// lanes), the RoPE dims a pair a lane.
+constexpr int kLatentWarps = 4;
+struct LatentArgs {
+  LatentWrite p;
+  bool wide, wide_g;
+};
+template <bool kBf16>
+__global__ void __launch_bounds__(32 * kLatentWarps) latent_write_kernel(const LatentArgs a) {
+  const LatentWrite& p = a.p;
+  const Fp8KvCache& c = p.cache;
+  const int lane = threadIdx.x & 31;
+  const long long i = static_cast<long long>(blockIdx.x) * kLatentWarps + (threadIdx.x >> 5);
+  pdl_wait();
+  pdl_trigger();
+  if (i >= p.n) return;
+  const long long r = p.rows[i];
+  if (r < 0 || r >= c.rows) return;
+  const void* x = static_cast<const char*>(p.kv) + i * p.stride * (kBf16 ? 2 : 4);
+  auto value = [&](int k) {
+    return kBf16 ? bf16_widen(static_cast<const uint16_t*>(x)[k]) : static_cast<const float*>(x)[k];
+  };
+  const int vecs = c.nope / kVec, pairs = c.rope_dim / 2;
+  constexpr int kVecs = 2;  // 512 dims
+  float v[kVecs][kVec];
+  float squares = 0.f;
+#pragma unroll
+  for (int j = 0; j < kVecs; ++j) {
+    const int at = lane + 32 * j;
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) v[j][k] = 0.f;
+    if (at < vecs) load8<kBf16>(x, at * kVec, kVec, a.wide, v[j]);
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) squares = fmaf(v[j][k], v[j][k], squares);
+  }
+  float p0 = 0.f, p1 = 0.f;  // the lane's first pair
+  for (int q = lane; q < pairs; q += 32) {
+    const float x0 = value(c.nope + 2 * q), x1 = value(c.nope + 2 * q + 1);
+    if (q == lane) { p0 = x0; p1 = x1; }
+    squares = fmaf(x0, x0, fmaf(x1, x1, squares));
+  }
+  float rs = 1.f, down = 1.f;
+  if (p.gain) {
+    const float d = static_cast<float>(c.nope + c.rope_dim);
+    auto warp_sum = [](float s) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      return s;
+    };
+    float mean = warp_sum(squares) / d, eps = p.eps;
+    if (!(mean <= 3.0e38f)) {  // squares beyond fp32: of values times 2^-76
+      down = 1.3234889800848443e-23f;
+      squares = 0.f;
+#pragma unroll
+      for (int j = 0; j < kVecs; ++j)
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) squares = fmaf(v[j][k] * down, v[j][k] * down, squares);
+      for (int q = lane; q < pairs; q += 32) {
+        const float x0 = value(c.nope + 2 * q) * down, x1 = value(c.nope + 2 * q + 1) * down;
+        squares = fmaf(x0, x0, fmaf(x1, x1, squares));
+      }
+      mean = warp_sum(squares) / d;
+      eps = 0.f;
+    }
+    rs = rsqrtf(mean + eps);
+  }
+  uint8_t* codes = c.codes + r * c.nope;
+#pragma unroll
+  for (int j = 0; j < kVecs; ++j) {
+    const int at = lane + 32 * j;
+    float g[kVec];
+    if (p.gain) {
+      if (at < vecs) load8<true>(p.gain, at * kVec, kVec, a.wide_g, g);
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) v[j][k] = at < vecs ? v[j][k] * down * rs * g[k] : 0.f;
+    }
+    uint32_t top = top8(v[j]);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    // (the attention tells a broken latent by its codes: NaN under a scale of 1)
+    uint2 q = make_uint2(0x7F7F7F7Fu, 0x7F7F7F7Fu);
+    uint32_t e8 = 127;
+    if (top < 0x7F800000u) {
+      e8 = __float_as_uint(pow2_scale_448(__uint_as_float(top))) >> 23;
+      q = codes8(v[j], __uint_as_float((254u - e8) << 23));
+    }
+    if (at >= vecs) continue;
+    *reinterpret_cast<uint2*>(codes + at * kVec) = q;
+    if ((lane & 7) == 0) c.scales[r * kKvScaleSlots + at / 8] = static_cast<uint8_t>(e8);
+  }
+  for (int q = lane; q < pairs; q += 32) {
+    float x0 = p0, x1 = p1;
+    if (q != lane) { x0 = value(c.nope + 2 * q); x1 = value(c.nope + 2 * q + 1); }
+    if (p.gain) {
+      x0 = x0 * down * rs * bf16_widen(p.gain[c.nope + 2 * q]);
+      x1 = x1 * down * rs * bf16_widen(p.gain[c.nope + 2 * q + 1]);
+    }
+    if (p.rope_cos) {
+      const float co = p.rope_cos[i * pairs + q], si = p.rope_sin[i * pairs + q];
+      const float y0 = x0 * co - x1 * si;
+      x1 = x0 * si + x1 * co;
+      x0 = y0;
+    }
+    uint16_t* to = c.rope + r * c.rope_dim + 2 * q;
+    *reinterpret_cast<uint32_t*>(to) = pack_bf16x2(x0, x1);  // rope_dim is even, rope aligned
+  }
+}
+
+// Rows of whole vectors that start on a 16-byte boundary.
+bool whole_vectors(const void* base, long long stride, int rows, int width, int size) {
+  return width % kVec == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0 &&
+         (rows <= 1 || stride * size % 16 == 0);
+}
+
+}  // namespace
+
+cudaError_t norm_quant(const NormProblem& p, cudaStream_t st) {
+  if (p.rows <= 0) return cudaSuccess;
+  NormArgs a;
+  a.p = p;
+  const int size = p.bf16 ? 2 : 4;
+  a.wide_x = whole_vectors(p.x, p.x_stride, p.rows, p.width, size);
+  a.wide_r = whole_vectors(p.residual, p.residual_stride, p.rows, p.width, size);
+  a.wide_s = whole_vectors(p.sum, p.sum_stride, p.rows, p.width, size);
+  a.wide_o = whole_vectors(p.out, p.out_stride, p.rows, p.width, size);
+  a.wide_g = p.width % kVec == 0 && reinterpret_cast<uintptr_t>(p.gain) % 16 == 0;
+  a.wide_c = p.width % kVec == 0 && reinterpret_cast<uintptr_t>(p.codes) % 8 == 0;
+  const int vecs = (p.width + kVec - 1) / kVec;
+  int per = 1;
+  while (per < 4 && vecs > 256 * per) per *= 2;
+  a.threads = ((vecs + per - 1) / per + 31) / 32 * 32;
+  if (a.threads > 1024) return cudaErrorInvalidValue;
+  const int rows = a.threads >= 128 ? 1 : 128 / a.threads;
+  const dim3 grid(static_cast<unsigned>((p.rows + rows - 1) / rows)), block(rows * a.threads);
+  if (p.bf16) {
+    auto kernel = per == 1 ? norm_quant_kernel<true, 1> : per == 2 ? norm_quant_kernel<true, 2>
+                                                                   : norm_quant_kernel<true, 4>;
+    return launch_pdl(kernel, grid, block, 0, st, a);
+  }
+  auto kernel = per == 1 ? norm_quant_kernel<false, 1> : per == 2 ? norm_quant_kernel<false, 2>
+                                                                  : norm_quant_kernel<false, 4>;
+  return launch_pdl(kernel, grid, block, 0, st, a);
+}
+
+cudaError_t latent_write(const LatentWrite& p, cudaStream_t st) {
+  if (p.n <= 0) return cudaSuccess;
+  LatentArgs a;
+  a.p = p;
+  const int size = p.bf16 ? 2 : 4;
+  a.wide = reinterpret_cast<uintptr_t>(p.kv) % 16 == 0 && (p.n <= 1 || p.stride * size % 16 == 0);
+  a.wide_g = reinterpret_cast<uintptr_t>(p.gain) % 16 == 0;
+  auto kernel = p.bf16 ? latent_write_kernel<true> : latent_write_kernel<false>;
+  return launch_pdl(kernel, dim3(static_cast<unsigned>((p.n + kLatentWarps - 1) / kLatentWarps)),
+                    dim3(32 * kLatentWarps), 0, st, a);
+}
+
+}  // namespace dsv4

@@ -676,6 +676,20 @@ def _dev(t, name, dtype, numel=None):
     return t.data_ptr()
 
 
+def _row_tensor(t, name, width, like=None):
+    """(1 for BF16 or 0 for fp32, elements between rows or 0) of CUDA rows [n][width]."""
+    import torch
+    if (t.dtype not in (torch.bfloat16, torch.float32) or t.dim() != 2 or t.shape[1] != width
+            or not t.is_cuda or (width > 1 and t.stride(1) != 1)):
+        raise ValueError(f"{name}: a CUDA tensor [rows][{width}] of bfloat16 or float32, the values of "
+                         f"a row one behind the other")
+    if like is not None and (t.dtype is not like.dtype or t.shape[0] != like.shape[0]):
+        raise ValueError(f"{name}: {like.shape[0]} rows of {like.dtype} are wanted")
+    if t.shape[0] > 1 and t.stride(0) < width:
+        raise ValueError(f"{name}: the rows must not overlap")
+    return int(t.dtype is torch.bfloat16), t.stride(0) if t.shape[0] > 1 else 0
+
+
 class PagedCache:
     """Latents of many sequences in pages of `page_size` rows of one LatentCache
     per layer (dsv4cuda_paged): slot s holds length[s] positions in the pages
@@ -730,6 +744,24 @@ class PagedCache:
         _check(lib.dsv4cuda_paged_append(
             self._ref, _dev(slots, "slots", self._i32), _dev(counts, "counts", self._i32, n), n,
             at, n_rows, _stream(stream)))
+
+    def write(self, layer, kv, rows, gain=None, eps=1e-6, rope_cos=None, rope_sin=None, stream=None):
+        """New tokens' latents into their pages (dsv4cuda_paged_write): kv [n][nope +
+        rope_dim] BF16 or fp32 (rows may lie apart) to cache rows rows (int64 [n], as append
+        gives them; -1 is left out) of `layer`, normed with gain (BF16, None: not normed) and
+        eps, the RoPE dims turned by rope_cos / rope_sin fp32 [n][rope_dim / 2]."""
+        import torch
+        if not 0 <= layer < len(self.caches):
+            raise ValueError(f"layer {layer} of {len(self.caches)}")
+        c = self.caches[layer].struct
+        d = c.nope + c.rope_dim
+        bf16, stride = _row_tensor(kv, "kv", d)
+        n = kv.shape[0]
+        half = n * (c.rope_dim // 2)
+        _check(lib.dsv4cuda_paged_write(
+            self._ref, layer, kv.data_ptr(), bf16, stride, _dev(rows, "rows", self._i64, n), n,
+            _dev(gain, "gain", torch.bfloat16, d), eps, _dev(rope_cos, "rope_cos", torch.float32, half),
+            _dev(rope_sin, "rope_sin", torch.float32, half), _stream(stream)))
 
     def fork(self, dst, src, stream=None):
         """Slots dst become copies of slots src (-1: emptied); int32 CUDA tensors."""
@@ -804,6 +836,87 @@ def paged_attn(out, q, paged: PagedCache, layer, q_start, max_new, max_len, scal
         _dev(lse, "lse", f32, n * heads), C.byref(shape),
         _dev(workspace, "workspace", torch.uint8), 0 if workspace is None else workspace.numel(),
         _stream(stream)))
+
+
+# ------------------------------------------------------------ norm, beams --
+class NormShape(C.Structure):
+    _fields_ = [("n_rows", C.c_int), ("width", C.c_int), ("bf16", C.c_int), ("eps", C.c_float),
+                ("x_stride", C.c_longlong), ("residual_stride", C.c_longlong),
+                ("sum_stride", C.c_longlong), ("out_stride", C.c_longlong)]
+
+
+class BeamShape(C.Structure):
+    _fields_ = [("n_groups", C.c_int), ("beams", C.c_int), ("n_cands", C.c_int), ("vocab", C.c_int),
+                ("bf16", C.c_int), ("eos", C.c_int), ("stride", C.c_longlong)]
+
+
+lib.dsv4cuda_norm_quant.restype = C.c_int
+lib.dsv4cuda_norm_quant.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp]
+lib.dsv4cuda_paged_write.restype = C.c_int
+lib.dsv4cuda_paged_write.argtypes = [vp, C.c_int, vp, C.c_int, C.c_longlong, vp, C.c_int, vp, C.c_float,
+                                     vp, vp, vp]
+lib.dsv4cuda_beam_workspace_bytes.restype = C.c_size_t
+lib.dsv4cuda_beam_workspace_bytes.argtypes = [vp]
+lib.dsv4cuda_beam_select.restype = C.c_int
+lib.dsv4cuda_beam_select.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]
+
+
+def norm_quant(x, gain, codes, scales, eps=1e-6, residual=None, sum_out=None, out=None, stream=None):
+    """dsv4cuda_norm_quant: RMS norm of x (+ residual) [rows][width] (BF16 or fp32, rows
+    may lie apart) with gain (BF16 [width] or None) to E4M3 codes uint8 [rows][width] and
+    E8M0 scales uint8 [rows][ceil(width / 128)], as MoeLayer.experts and grouped_gemm take
+    them. sum_out (may be x or residual) receives x + residual, out the normalised rows; both
+    of x's type."""
+    import torch
+    if x.dim() != 2:
+        raise ValueError("x: [rows][width] is wanted")
+    n, width = x.shape
+    bf16, xs = _row_tensor(x, "x", width)
+    strides = [xs]
+    for t, name in ((residual, "residual"), (sum_out, "sum_out"), (out, "out")):
+        strides.append(0 if t is None else _row_tensor(t, name, width, like=x)[1])
+    shape = NormShape(n, width, bf16, eps, *strides)
+    _check(lib.dsv4cuda_norm_quant(
+        x.data_ptr(), None if residual is None else residual.data_ptr(),
+        None if sum_out is None else sum_out.data_ptr(), None if out is None else out.data_ptr(),
+        _dev(gain, "gain", torch.bfloat16, width), _dev(codes, "codes", torch.uint8, n * width),
+        _dev(scales, "scales", torch.uint8, n * ((width + 127) // 128)), C.byref(shape),
+        _stream(stream)))
+
+
+def _beam_shape(logits, score, cands, eos):
+    import torch
+    if score.dim() != 2 or logits.dim() != 2 or logits.shape[0] != score.numel():
+        raise ValueError("score [groups][beams] and logits [groups * beams][vocab] are wanted")
+    bf16, stride = _row_tensor(logits, "logits", logits.shape[1])
+    return BeamShape(score.shape[0], score.shape[1], cands, logits.shape[1], bf16, eos, stride)
+
+
+def beam_workspace_bytes(logits, score, n_cands) -> int:
+    """Workspace of a beam_select call of these sizes."""
+    return lib.dsv4cuda_beam_workspace_bytes(C.byref(_beam_shape(logits, score, n_cands, -1)))
+
+
+def beam_select(logits, score, parent, token, total, next, slot=None, dst=None, src=None, eos=-1,
+                workspace=None, stream=None):
+    """dsv4cuda_beam_select: the best continuations of each group's beams by score [groups]
+    [beams] + log softmax of logits [groups * beams][vocab] (fp32 or BF16, rows may lie apart):
+    parent, token int32 and total fp32 [groups][candidates], next int32 [groups][beams] the
+    candidates that go on (their token is not eos), and, of the beams' slots slot int32 [groups]
+    [beams], the dst and src of PagedCache.fork. workspace: a CUDA uint8 tensor (needed while
+    capturing)."""
+    import torch
+    i32, f32 = torch.int32, torch.float32
+    if parent.dim() != 2:
+        raise ValueError("parent [groups][candidates] is wanted")
+    shape = _beam_shape(logits, score, parent.shape[1], eos)
+    all_c, all_b = shape.n_groups * shape.n_cands, shape.n_groups * shape.beams
+    _check(lib.dsv4cuda_beam_select(
+        logits.data_ptr(), _dev(score, "score", f32), _dev(parent, "parent", i32, all_c),
+        _dev(token, "token", i32, all_c), _dev(total, "total", f32, all_c),
+        _dev(next, "next", i32, all_b), _dev(slot, "slot", i32, all_b), _dev(dst, "dst", i32, all_b),
+        _dev(src, "src", i32, all_b), C.byref(shape), _dev(workspace, "workspace", torch.uint8),
+        0 if workspace is None else workspace.numel(), _stream(stream)))
 
 
 # ------------------------------------------------------- grouped products --

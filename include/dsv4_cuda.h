@@ -622,6 +622,24 @@ int dsv4cuda_paged_append(const dsv4cuda_paged *p, const int *slots, const int *
  * are still where they were. */
 int dsv4cuda_paged_compact(const dsv4cuda_paged *p, int *table_out, int *refs_out, void *stream);
 
+/* Write of new tokens' latents into their pages, with the norm and the rotation
+ * on the way (kv_norm, dsv4_rope_apply_buf and the cache's quantisation,
+ * src/dsv4/dsv4_model.c:5300-5304, :1555, in one pass): latent i of kv [n]
+ * [nope + rope_dim] (BF16, or fp32 when bf16 is 0; `stride` elements apart,
+ * 0: nope + rope_dim) goes to row rows[i] of layer `layer`'s cache, as
+ * dsv4cuda_paged_append gave them (rows outside the pages, -1 among them, are
+ * left out; a row named twice gets one of the two):
+ *   v = kv / sqrt(mean kv^2 + eps) * gain        (gain NULL: v = kv)
+ *   the first nope dims as E4M3 codes with one E8M0 scale per 64,
+ *   pair (2j, 2j + 1) of the others turned by rope_cos / rope_sin [n]
+ *   [rope_dim / 2] (NULL: not turned) and stored as BF16.
+ * fp32 from the inputs on, each value rounded once. A group of 64 with a NaN or
+ * infinity becomes NaN. gain [nope + rope_dim] BF16; DEVICE pointers, async on
+ * stream, capturable. The cos / sin rows are those of dsv4cuda_paged_attn. */
+int dsv4cuda_paged_write(const dsv4cuda_paged *p, int layer, const void *kv, int bf16,
+                         long long stride, const long long *rows, int n, const uint16_t *gain,
+                         float eps, const float *rope_cos, const float *rope_sin, void *stream);
+
 typedef struct {
     int n_rows;            /* rows of q: the new tokens of all slots */
     int heads, head_dim;   /* head_dim = nope + rope_dim of the cache */
@@ -684,6 +702,68 @@ int dsv4cuda_paged_attn(void *out, const void *q, const dsv4cuda_paged *p, int l
 int dsv4cuda_token_logprobs(const void *logits, int bf16, int rows, int vocab, long long stride,
                             const int *tokens, float *logprob, float *entropy, int *rank,
                             int n_top, int *top_id, float *top_logprob, void *stream);
+
+/* ---------------------------------------------------------------------
+ * Selection of beams (no counterpart in the reference): group g's beams are
+ * rows g * beams .. of logits (fp32, or BF16 when bf16 != 0; `stride` elements
+ * apart, 0: vocab) with the running scores score [n_groups][beams], -inf for a
+ * beam that is not there. The n_cands best continuations of a group by
+ *   total = score[b] + log softmax(row b)[t]
+ * come out in descending order, the lower (beam, token) first among equals
+ * (totals are compared in 64 bits): parent, token, total [n_groups][n_cands];
+ * -1, -1, -inf where fewer are left: a logit of -inf is masked, a row with a NaN
+ * or +inf has no continuations, nor has a beam whose score is not finite.
+ *   next [n_groups][beams]  the candidates that go on, in order: those whose
+ *       token is not eos (eos < 0: all); -1 where there are fewer
+ *   dst, src [n_groups][beams]  with slot [n_groups][beams] (all three may be
+ *       NULL), the slots that hold the beams' latents: new beam i lives in slot
+ *       dst[i] and comes from src[i] (-1: from none). A parent's first child
+ *       stays where it is (dst = src), the others take the slots of beams
+ *       without children, so dsv4cuda_paged_fork(dst, src) puts all in place.
+ * beams and n_cands 1 .. 32. DEVICE pointers, async on stream. workspace may be
+ * NULL (a buffer per thread and stream); give one, 256-byte aligned, while
+ * capturing. */
+#define DSV4CUDA_MAX_BEAMS 32
+#define DSV4CUDA_MAX_BEAM_CANDIDATES 32
+typedef struct {
+    int n_groups, beams, n_cands;
+    int vocab;
+    int bf16;
+    int eos;
+    long long stride;
+} dsv4cuda_beam_shape;
+
+size_t dsv4cuda_beam_workspace_bytes(const dsv4cuda_beam_shape *shape);
+int dsv4cuda_beam_select(const void *logits, const float *score, int *parent, int *token,
+                         float *total, int *next, const int *slot, int *dst, int *src,
+                         const dsv4cuda_beam_shape *shape, void *workspace,
+                         size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------
+ * RMS norm of rows with the residual's addition and an 8-bit output
+ * (rmsnorm_bf16 and the activation quantisation, src/dsv4/dsv4_model.c:4934,
+ * :5580, of many rows in one pass):
+ *   v = x + residual, stored to sum;  y = v / sqrt(mean v^2 + eps) * gain
+ *   codes [n_rows][width] E4M3 with scales [n_rows][ceil(width / 128)] E8M0: per
+ *   128 columns the smallest power of two that brings the largest |y| (1e-4 at
+ *   least) to 448 or below
+ *   out = y unquantised, e.g. for a router
+ * x, residual (may be NULL), sum (NULL; may be x or residual themselves, with
+ * their stride) and out (NULL) are BF16, or fp32 when bf16 is 0, their rows
+ * `*_stride` elements apart (0: width). fp32 from the inputs on (y is taken of
+ * the sum before it is rounded), each output rounded once. gain [width] BF16
+ * (NULL: 1). A block of 128 with a NaN or infinity gets scale 255. width 1 ..
+ * 32768, eps > 0. DEVICE pointers, async on stream, capturable. */
+typedef struct {
+    int n_rows, width;
+    int bf16;
+    float eps;
+    long long x_stride, residual_stride, sum_stride, out_stride;
+} dsv4cuda_norm_shape;
+
+int dsv4cuda_norm_quant(const void *x, const void *residual, void *sum, void *out,
+                        const uint16_t *gain, uint8_t *codes, uint8_t *scales,
+                        const dsv4cuda_norm_shape *shape, void *stream);
 
 /* ---------------------------------------------------------------------
  * Whole-model decode on the device: dsv4_forward_token
