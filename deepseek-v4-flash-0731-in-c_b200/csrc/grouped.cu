@@ -16,8 +16,8 @@
 // and whoever brings its last part adds them in the order of the columns, so
 // that results do not depend on timing.
 //
-// Roles: warps 0-7 epilogue, 8-11 scales (registers to TMEM, the copies of
-// all four lane quarters at once), 12 copies, 13 MMAs.
+// Roles: warps 0-7 epilogue, 8-11 scales (to TMEM, each warp the copy of its
+// lane quarter), 12-15 rows of x, 16 copies of weights, 17 MMAs.
 #include "grouped.cuh"
 
 #include <cuda_bf16.h>
@@ -31,8 +31,9 @@ namespace {
 constexpr int kChunk = 128;              // columns of a stage: one row of swizzled shared memory
 constexpr int kTileRows = 128;           // M of an instruction
 constexpr int kATile = kTileRows * kChunk;
-constexpr int kEpiWarps = 8, kScaleWarps = 4;
-constexpr int kWarpCopy = kEpiWarps + kScaleWarps, kWarpMma = kWarpCopy + 1;
+constexpr int kEpiWarps = 8, kScaleWarps = 4, kRowWarps = 4;
+constexpr int kWarpRows = kEpiWarps + kScaleWarps, kWarpCopy = kWarpRows + kRowWarps;
+constexpr int kWarpMma = kWarpCopy + 1;
 constexpr int kThreads = 32 * (kWarpMma + 1);
 constexpr int kBlockCols = 16;           // rows of a group that an epilogue step takes
 constexpr int kMaxN = 192, kHalfN = 96;  // rows of a tile; up to kHalfN two tiles' sums fit in TMEM
@@ -41,6 +42,7 @@ constexpr int kMaxStages = 5;
 // and 8 of rows' scales each), then the sums.
 constexpr int kScaleCols = 64, kSumCol = 2 * kScaleCols, kTmemCols = 512;
 constexpr int kMaxShares = 256;          // blocks
+constexpr size_t kMaxSmem = 227 * 1024;
 
 struct Args {
   GroupedProblem p;
@@ -59,13 +61,21 @@ struct alignas(16) Control {
   int abort_flag;
   int last;      // the block brought a tile's last part
   alignas(16) uint32_t top[2][2][4][kBlockCols];  // largest |h| of a warp's 32 outputs
-  alignas(16) uint8_t codes[2][2][kBlockCols][kTileRows];
+  alignas(16) uint8_t codes[2][kBlockCols][kTileRows];
 };
+
+// The ring of scales: an entry holds four chunks' of 256 outputs and n_max rows.
+constexpr int kScaleEntries = 4, kScaleBytes = 2 * kTileRows * 16;
+__host__ __device__ constexpr int scale_entry_bytes(int n_max) { return kScaleBytes + n_max * 4; }
+// Behind it the rows of x of two pieces.
+__host__ __device__ constexpr int scale_ring_bytes(int n_max) {
+  return kScaleEntries * scale_entry_bytes(n_max) + 2 * n_max * 4;
+}
 
 __host__ __device__ constexpr int stage_bytes(int n_max) { return 2 * kATile + n_max * kChunk; }
 __host__ __device__ inline size_t smem_bytes(int n_max, int stages, int experts) {
-  return static_cast<size_t>(stages) * stage_bytes(n_max) + sizeof(Control) +
-         (experts + 1) * (sizeof(long long) + sizeof(int));
+  return static_cast<size_t>(stages) * stage_bytes(n_max) + scale_ring_bytes(n_max) +
+         sizeof(Control) + (experts + 1) * (sizeof(long long) + sizeof(int));
 }
 
 // Suspended waits: the epilogue needs the issue slots.
@@ -105,24 +115,17 @@ __device__ __forceinline__ void mma_scaled(uint32_t d, uint64_t a, uint64_t b, u
       "l"(a), "l"(b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate ? 1u : 0u)
       : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{ .reg .pred e; elect.sync _|e, 0xffffffff; selp.u32 %0, 1, 0, e; }" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile(
       "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
           smem_addr(bar))
       : "memory");
 }
-// Four rows of a tensor map with one-row boxes, one behind the other; a row
-// outside the map is zeros.
-__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, int x, const int (&y)[4],
-                                            uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]),
-      "r"(smem_addr(bar))
-      : "memory");
-}
-
 // 16 consecutive TMEM columns of this thread's lane.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
@@ -139,6 +142,27 @@ __device__ __forceinline__ void tmem_ld_wait16(uint32_t (&r)[16]) {
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
                  "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
                  "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+// Zeros where there is nothing to be read.
+__device__ __forceinline__ void cp_async16_or_0(uint32_t to, const void* from, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0)
+               : "memory");
+}
+// This thread's arrival once all its copies so far are there.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ void bar_sync(int id, int threads) {
@@ -168,70 +192,72 @@ struct Piece {
   int e, row_tile;     // matrix, 256 (gated: 128) outputs
   int row0, rows, n;   // first row of the tile, rows there are, columns of the MMAs
   int lo, hi;          // chunks
-  long long start;     // of the tile, in cost
-  int cost;            // of a chunk
 };
 
+// The chunk of a tile of `cost` a chunk in which position d behind its start lies.
+__device__ __forceinline__ int chunk_at(long long d, int chunks, int cost) {
+  return d <= 0 ? 0
+                : d >= static_cast<long long>(chunks) * cost
+                      ? chunks
+                      : static_cast<int>(static_cast<unsigned>(d) / static_cast<unsigned>(cost));
+}
+
+// Each role walks its share's pieces by itself. All of it stays in registers:
+// there is no L1 to speak of beside 227 KB of shared memory, so a stack costs
+// an L2 access each time.
 struct Walk {
-  const long long* prefix;  // [experts + 1] cost before each group
   const int* offsets;       // [experts + 1]
   int experts, row_tiles, chunks, n_max;
-  long long b0, b1;         // this share
-  int e, item;
-  bool done;
+  Cut cut;                  // of group e
+  int e, row_tile, t, lo;   // the next piece
+  long long left;           // from its tile's start to the share's end, in cost
 
-  __device__ void begin() {
-    done = b0 >= b1;
-    if (done) return;
-    int lo = 0, hi = experts;  // the last group whose start is not behind b0
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (prefix[mid] <= b0) lo = mid; else hi = mid;
+  __device__ __forceinline__ void recut() { cut = cut_group(offsets[e + 1] - offsets[e], n_max); }
+  // prefix [experts + 1]: cost before each group; the share is b0 .. b1.
+  __device__ __forceinline__ void begin(const long long* prefix, long long b0, long long b1) {
+    left = 0;
+    if (b0 >= b1) return;
+    int low = 0, high = experts;  // the last group whose start is not behind b0
+    while (high - low > 1) {
+      const int mid = (low + high) >> 1;
+      if (prefix[mid] <= b0) low = mid; else high = mid;
     }
-    e = lo;
-    const Cut c = cut_group(offsets[e + 1] - offsets[e], n_max);
-    item = static_cast<int>((b0 - prefix[e]) / (static_cast<long long>(chunks) * c.cost));
+    e = low;
+    recut();
+    const long long tile = static_cast<long long>(chunks) * cut.cost, d = b0 - prefix[e];
+    const int item = static_cast<int>(d / tile);
+    row_tile = item / cut.tiles;
+    t = item - row_tile * cut.tiles;
+    const long long start = prefix[e] + item * tile;
+    lo = chunk_at(b0 - start, chunks, cut.cost);
+    left = b1 - start;
   }
-  // The chunk of the tile that starts at `start` in which position b lies.
-  __device__ int chunk_at(long long b, long long start, int cost) const {
-    const long long d = b - start;
-    return d <= 0 ? 0
-                  : d >= static_cast<long long>(chunks) * cost
-                        ? chunks
-                        : static_cast<int>(static_cast<unsigned>(d) / static_cast<unsigned>(cost));
-  }
-  __device__ bool next(Piece* p) {
-    if (done) return false;
-    Cut c;
-    while (true) {
-      if (e >= experts) {
-        done = true;
-        return false;
-      }
-      c = cut_group(offsets[e + 1] - offsets[e], n_max);
-      if (item < c.tiles * row_tiles) break;
-      ++e;
-      item = 0;
-    }
-    p->start = prefix[e] + static_cast<long long>(item) * chunks * c.cost;
-    p->cost = c.cost;
-    p->lo = chunk_at(b0, p->start, c.cost);
-    p->hi = chunk_at(b1, p->start, c.cost);
+  __device__ __forceinline__ bool next(Piece* p) {
+    if (left <= 0) return false;
+    p->lo = lo;
+    p->hi = chunk_at(left, chunks, cut.cost);
     if (p->lo >= p->hi) {
-      done = true;
+      left = 0;
       return false;
     }
+    p->e = e;
+    p->row_tile = row_tile;
+    p->row0 = offsets[e] + t * cut.rows;
+    p->rows = min(offsets[e + 1] - p->row0, cut.rows);
+    p->n = cut.rows;
+    lo = 0;
+    left -= static_cast<long long>(chunks) * cut.cost;
     // the tiles of the same weights follow one another: the second reads them
     // from L2
-    const int t = item % c.tiles;
-    p->e = e;
-    p->row_tile = item / c.tiles;
-    p->row0 = offsets[e] + t * c.rows;
-    const int left = offsets[e + 1] - p->row0;
-    p->rows = left < c.rows ? left : c.rows;
-    p->n = c.rows;
-    if (p->hi < chunks) done = true;
-    ++item;
+    if (++t == cut.tiles) {
+      t = 0;
+      if (++row_tile == row_tiles && left > 0) {
+        row_tile = 0;
+        do ++e; while (e + 1 < experts && offsets[e + 1] == offsets[e]);
+        recut();
+        if (cut.tiles == 0) left = 0;
+      }
+    }
     return true;
   }
 };
@@ -241,10 +267,12 @@ struct Walk {
 template <bool kFp8, bool kGated>
 __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUtensorMap map1,
-    const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Args a) {
+    const __grid_constant__ Args a) {
   extern __shared__ __align__(1024) uint8_t smem[];
   const GroupedProblem& p = a.p;
-  Control* ctl = reinterpret_cast<Control*>(smem + static_cast<size_t>(a.stages) * stage_bytes(a.n_max));
+  uint8_t* scale_ring = smem + static_cast<size_t>(a.stages) * stage_bytes(a.n_max);
+  int* row_table = reinterpret_cast<int*>(scale_ring + kScaleEntries * scale_entry_bytes(a.n_max));
+  Control* ctl = reinterpret_cast<Control*>(scale_ring + scale_ring_bytes(a.n_max));
   long long* prefix = reinterpret_cast<long long*>(ctl + 1);
   int* offsets = reinterpret_cast<int*>(prefix + p.experts + 1);
   volatile int* abort_flag = &ctl->abort_flag;
@@ -256,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.stages; ++i) {
-      mbar_init(&ctl->full[i], 1);
+      mbar_init(&ctl->full[i], 1 + 32 * kRowWarps);  // the weights' copy, the threads' parts of the rows
       mbar_init(&ctl->empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -272,7 +300,6 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
   if (warp == kWarpCopy && lane == 0) {
     tma_prefetch_desc(&map0);
     if (kGated) tma_prefetch_desc(&map1);
-    tma_prefetch_desc(&xmap);
   }
   if (warp == kWarpMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -329,15 +356,13 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
   auto bound = [&](int c) { return c >= shares ? total : total * c / shares; };
   const int me = blockIdx.x;
   Walk walk;
-  walk.prefix = prefix;
   walk.offsets = offsets;
   walk.experts = p.experts;
   walk.row_tiles = row_tiles;
   walk.chunks = chunks;
   walk.n_max = a.n_max;
-  walk.b0 = bound(me);
-  walk.b1 = bound(me + 1);
-  walk.begin();
+  const long long share_end = bound(me + 1);
+  walk.begin(prefix, bound(me), share_end);
   Piece piece;
   auto two_tiles = [&](const Piece& q) {
     return kGated || q.row_tile * kOuts + kTileRows < p.outs;
@@ -350,23 +375,22 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     const int at = quarter * 32 + lane;  // output of a tile
     unsigned uses[2] = {0, 0};           // of each half of the sums' columns
     int half = 0, flip = 0;
-    while (walk.next(&piece)) {
+    while (true) {
+      // where its tile starts and what a chunk of it costs
+      const long long start = share_end - walk.left;
+      const int cost = walk.cut.cost;
+      if (!walk.next(&piece)) break;
       const bool big = piece.n > kHalfN;
       const int blocks = piece.n / kBlockCols;
-      // this lane's column of each block: its weight or its row of out
-      float weight[kMaxN / kBlockCols / 2];
-      int row_out[kMaxN / kBlockCols / 2];
-#pragma unroll
-      for (int i = 0; i < kMaxN / kBlockCols / 2; ++i) {
-        const int r = (2 * i + side) * kBlockCols + (lane & 15);
-        const bool in = r < piece.rows;
-        if (kGated) {
-          weight[i] = in && p.weight ? p.weight[piece.row0 + r] : 1.f;
-        } else {
-          const int d = !in ? -1 : p.dst ? p.dst[piece.row0 + r] : piece.row0 + r;
-          row_out[i] = d < p.out_rows ? d : -1;
-        }
-      }
+      // this lane's row of a block: its weight, or its row of out
+      auto lane_row = [&](int b) {
+        const int r = b * kBlockCols + (lane & 15);
+        const bool in = b < blocks && r < piece.rows;
+        if (kGated) return in && p.weight ? __float_as_int(p.weight[piece.row0 + r]) : 0x3F800000;
+        const int d = !in ? -1 : p.dst ? p.dst[piece.row0 + r] : piece.row0 + r;
+        return d < p.out_rows ? d : -1;
+      };
+      int row_next = lane_row(side);
       const int h = big ? 0 : half;
       const uint32_t sums = tmem + lanes + kSumCol + (big ? 0 : h * (kMaxN));
       const uint32_t sums1 = sums + (big ? kMaxN : kHalfN);
@@ -391,12 +415,13 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
       const bool second = two_tiles(piece);
       const size_t tile_floats = static_cast<size_t>(a.n_max) * kTileRows;
       auto part_of = [&](int c) {  // share c's part of this tile
-        const int slot = bound(c) >= piece.start ? 0 : 1;
+        const int slot = bound(c) >= start ? 0 : 1;
         return a.parts + (static_cast<size_t>(c) * 2 + slot) * 2 * tile_floats + at;
       };
       int c0 = me, c1 = me;
       if (cut) {
         float* mine = part_of(me);
+#pragma unroll 1
         for (int b = side; b < blocks; b += 2) {
           uint32_t r0[16], r1[16];
           tmem_ld16(sums + b * kBlockCols, r0);
@@ -411,8 +436,8 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
           }
         }
         release();
-        while (walk.chunk_at(bound(c0), piece.start, piece.cost) > 0) --c0;
-        while (walk.chunk_at(bound(c1 + 1), piece.start, piece.cost) < chunks) ++c1;
+        while (chunk_at(bound(c0) - start, chunks, cost) > 0) --c0;
+        while (chunk_at(bound(c1 + 1) - start, chunks, cost) < chunks) ++c1;
         __threadfence();
         bar_sync(1, 32 * kEpiWarps);
         if (threadIdx.x == 0) {
@@ -443,9 +468,9 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) v0[i] = v1[i] = 0.f;
+#pragma unroll 1
         for (int c = c0; c <= c1; ++c) {
-          if (walk.chunk_at(bound(c), piece.start, piece.cost) >=
-              walk.chunk_at(bound(c + 1), piece.start, piece.cost))
+          if (chunk_at(bound(c) - start, chunks, cost) >= chunk_at(bound(c + 1) - start, chunks, cost))
             continue;
           const float* q = part_of(c) + static_cast<size_t>(b) * kBlockCols * kTileRows;
 #pragma unroll
@@ -455,229 +480,304 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
           }
         }
       };
-#pragma unroll
-      for (int i = 0; i < kMaxN / kBlockCols / 2; ++i) {
-        const int b = 2 * i + side;
-        if (b >= blocks) break;
+      // (not unrolled, nor in the parts above and below: what a piece runs once has
+      // to come from the instruction caches; six blocks' code in a row took 8,000
+      // clocks a block)
+#pragma unroll 1
+      for (int b = side; b < blocks; b += 2) {
+        const int row_data = row_next;
+        row_next = lane_row(b + 2);
         float v0[16], v1[16];
         take(b, v0, v1);
         const int n = min(kBlockCols, piece.rows - b * kBlockCols);
         if (kGated) {
-          uint32_t top[16];
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             const float g = fminf(v0[j], p.limit), u = fminf(fmaxf(v1[j], -p.limit), p.limit);
-            // (a NaN would be lost in the limits)
-            const float y = g / (1.f + ex2_approx(-g * kLog2e)) * u *
-                            __shfl_sync(0xffffffffu, weight[i], j);
-            v0[j] = v0[j] != v0[j] || v1[j] != v1[j] ? NAN : y;
-            top[j] = __reduce_max_sync(0xffffffffu, __float_as_uint(v0[j]) & 0x7FFFFFFFu);
-          }
-          if (lane == 0) {
-#pragma unroll
-            for (int j = 0; j < 16; j += 4)
-              *reinterpret_cast<uint4*>(&ctl->top[side][flip][quarter][j]) =
-                  make_uint4(top[j], top[j + 1], top[j + 2], top[j + 3]);
+            const float y = __fdividef(g, 1.f + ex2_approx(-g * kLog2e)) * u *
+                            __int_as_float(__shfl_sync(0xffffffffu, row_data, j));
+            v0[j] = v0[j] != v0[j] || v1[j] != v1[j] ? NAN : y;  // (lost in the limits)
+            const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(v0[j]) & 0x7FFFFFFFu);
+            if (lane == j) ctl->top[side][flip][quarter][j] = top;
           }
           bar_sync(2 + side, 128);
-          uint8_t scale_code = 0;  // of column `lane`
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const uint32_t m = max(max(ctl->top[side][flip][0][j], ctl->top[side][flip][1][j]),
-                                   max(ctl->top[side][flip][2][j], ctl->top[side][flip][3][j]));
-            uint8_t code = 0x7F, e8 = 255;  // an infinity or NaN makes the block NaN
-            if (m < 0x7F800000u) {
-              const uint32_t s = __float_as_uint(pow2_scale_448(__uint_as_float(m))) >> 23;
-              const float q = v0[j] * __uint_as_float((254u - s) << 23);
-              unsigned short t;
-              asm("{ .reg .b16 h; cvt.rn.satfinite.e4m3x2.f32 h, %1, %1; mov.b16 %0, h; }"
-                  : "=h"(t) : "f"(q));
-              code = static_cast<uint8_t>(t & 0xFF);
-              e8 = static_cast<uint8_t>(s);
-            }
-            ctl->codes[side][flip][j][at] = code;
-            if (lane == j) scale_code = e8;
+          // lane l of each warp: block's scale of row l
+          const uint32_t(*tops)[kBlockCols] = ctl->top[side][flip];
+          const int l = lane & 15;
+          const uint32_t m = max(max(tops[0][l], tops[1][l]), max(tops[2][l], tops[3][l]));
+          uint32_t e8 = 255;  // an infinity or NaN makes the block NaN
+          float inv = NAN;
+          if (m < 0x7F800000u) {
+            e8 = __float_as_uint(pow2_scale_448(__uint_as_float(m))) >> 23;
+            inv = __uint_as_float((254u - e8) << 23);
           }
           if (quarter == 0 && lane < n)
             p.hs[static_cast<size_t>(piece.row0 + b * kBlockCols + lane) * (p.outs / kTileRows) +
-                 piece.row_tile] = scale_code;
+                 piece.row_tile] = static_cast<uint8_t>(e8);
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            unsigned short t;
+            asm("{ .reg .b16 h; cvt.rn.satfinite.e4m3x2.f32 h, %2, %1; mov.b16 %0, h; }"
+                : "=h"(t)
+                : "f"(v0[j] * __shfl_sync(0xffffffffu, inv, j)),
+                  "f"(v0[j + 1] * __shfl_sync(0xffffffffu, inv, j + 1)));
+            ctl->codes[side][j][at] = static_cast<uint8_t>(t);
+            ctl->codes[side][j + 1][at] = static_cast<uint8_t>(t >> 8);
+          }
           bar_sync(2 + side, 128);
           const int t = (threadIdx.x & 127) >> 3, v = threadIdx.x & 7;
           if (t < n)
             *reinterpret_cast<uint4*>(
                 p.hq + static_cast<size_t>(piece.row0 + b * kBlockCols + t) * p.outs +
                 piece.row_tile * kTileRows + v * 16) =
-                *reinterpret_cast<const uint4*>(&ctl->codes[side][flip][t][v * 16]);
+                *reinterpret_cast<const uint4*>(&ctl->codes[side][t][v * 16]);
           flip ^= 1;
         } else {
           const int o0 = piece.row_tile * kOuts + at, o1 = o0 + kTileRows;
+          const bool in0 = o0 < p.outs, in1 = o1 < p.outs;
+          auto put = [&](auto* o, int d, auto x0, auto x1) {
+            o += d * p.out_stride;
+            if (in0 && d >= 0) o[o0] = x0;
+            if (in1 && d >= 0) o[o1] = x1;
+          };
+          if (p.bf16) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int d = __shfl_sync(0xffffffffu, row_out[i], j);
-            if (d < 0) continue;
-            const size_t base = static_cast<size_t>(d) * p.out_stride;
-            if (p.bf16) {
-              __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + base;
-              if (o0 < p.outs) o[o0] = __float2bfloat16_rn(v0[j]);
-              if (o1 < p.outs) o[o1] = __float2bfloat16_rn(v1[j]);
-            } else {
-              float* o = static_cast<float*>(p.out) + base;
-              if (o0 < p.outs) o[o0] = v0[j];
-              if (o1 < p.outs) o[o1] = v1[j];
-            }
+            for (int j = 0; j < 16; ++j)
+              put(static_cast<__nv_bfloat16*>(p.out), __shfl_sync(0xffffffffu, row_data, j),
+                  __float2bfloat16_rn(v0[j]), __float2bfloat16_rn(v1[j]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              put(static_cast<float*>(p.out), __shfl_sync(0xffffffffu, row_data, j), v0[j], v1[j]);
           }
         }
       }
       if (!cut) release();
     }
-  } else if (warp < kWarpCopy) {
+  } else if (warp < kWarpRows) {
     // -------------------------------------------------------------- scales
     // Lane l of each quarter holds outputs (rows) l, 32 + l, ... in
     // consecutive columns; a column's four bytes are a chunk's four groups.
+    // They come through a ring in shared memory, four chunks an entry, some
+    // ten chunks ahead of their use.
+    const int st = threadIdx.x - 32 * kEpiWarps;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const int pitch = p.width / 32;
     const bool whole = chunks % 4 == 0;
-    const bool wide = whole && (reinterpret_cast<uintptr_t>(p.ws[0]) & 15) == 0 &&
-                      (!kGated || (reinterpret_cast<uintptr_t>(p.ws[1]) & 15) == 0);
+    const uintptr_t off = reinterpret_cast<uintptr_t>(p.ws[0]) |
+                          (kGated ? reinterpret_cast<uintptr_t>(p.ws[1]) : 0);
+    const bool wide = whole && (off & (kFp8 ? 3 : 15)) == 0;
     const bool x_words = whole && (reinterpret_cast<uintptr_t>(p.xs) & 3) == 0;
-    unsigned n = 0;
-    bool good = true;
-    while (good && walk.next(&piece)) {
-      const uint8_t* wrow[2][4];
-      bool there[2][4];
+    const int entry_bytes = scale_entry_bytes(a.n_max);
+    // entries are filled piece after piece, its chunks by fours
+    bool more = walk.next(&piece);
+    int q = piece.lo / 4;
+    unsigned filled = 0;
+    int xrow[2];  // rows of x whose scales this thread fetches, -1: none
+    auto find_rows = [&] {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int row = piece.row_tile * kOuts + (kGated ? 0 : t * kTileRows) + j * 32 + lane;
-          there[t][j] = row < p.outs;
-          const uint8_t* base = p.ws[kGated ? t : 0];
-          if (kFp8)
-            wrow[t][j] = base + (static_cast<size_t>(piece.e) * ((p.outs + 127) / 128) +
-                                 min(row, p.outs - 1) / 128) * chunks;
-          else
-            wrow[t][j] = base + (static_cast<size_t>(piece.e) * p.outs + min(row, p.outs - 1)) * pitch;
-        }
-      const uint8_t* xrow[6];
-      bool x_there[6];
-#pragma unroll
-      for (int j = 0; j < 6; ++j) {
-        const int r = j * 32 + lane;
-        int s = -1;
-        if (r < piece.rows) s = p.src ? p.src[piece.row0 + r] : piece.row0 + r;
-        x_there[j] = s >= 0 && s < p.x_rows;
-        xrow[j] = p.xs + static_cast<size_t>(x_there[j] ? s : 0) * chunks;
+      for (int i = 0; i < 2; ++i) {
+        const int r = st + i * 32 * kScaleWarps;
+        int v = -1;
+        if (r < piece.rows) v = p.src ? p.src[piece.row0 + r] : piece.row0 + r;
+        xrow[i] = v >= 0 && v < p.x_rows ? v : -1;
       }
-      for (int q = piece.lo / 4; good && q <= (piece.hi - 1) / 4; ++q) {
-        uint32_t wa[32], xb[32];
+    };
+    const int blocks128 = (p.outs + kTileRows - 1) / kTileRows;
+    auto fetch = [&] {
+      if (more) {
+        uint8_t* entry = scale_ring + (filled % kScaleEntries) * entry_bytes;
+        const int left = min(chunks - 4 * q, 4);  // chunks there are
+        if (kFp8) {
+          // one block of 128 outputs: the same in every lane
+          if (st < 2) {
+            const int rb = min(piece.row_tile * 2 + st, blocks128 - 1);
+            const uint8_t* from =
+                p.ws[0] + (static_cast<size_t>(piece.e) * blocks128 + rb) * chunks + 4 * q;
+            if (wide) {
+              cp_async4(smem_addr(entry + 4 * st), from);
+            } else {
+#pragma unroll 1
+              for (int c = 0; c < left; ++c) entry[4 * st + c] = from[c];
+            }
+          }
+        } else {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+          for (int t = 0; t < 2; ++t) {
+            const int row = piece.row_tile * kOuts + (kGated ? 0 : t * kTileRows) + st;
+            const uint8_t* from =
+                p.ws[kGated ? t : 0] +
+                (static_cast<size_t>(piece.e) * p.outs + min(row, p.outs - 1)) * (p.width / 32) + 16 * q;
+            const uint32_t to = smem_addr(entry + (t * kTileRows + st) * 16);
+            if (wide) {
+              cp_async16(to, from);
+            } else {
+#pragma unroll 1
+              for (int c = 0; c < left; ++c) cp_async4(to + 4 * c, from + 4 * c);
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = st + i * 32 * kScaleWarps;
+          if (r >= piece.n) continue;
+          uint8_t* to = entry + kScaleBytes + r * 4;
+          const uint8_t* from = p.xs + static_cast<size_t>(max(xrow[i], 0)) * chunks + 4 * q;
+          if (xrow[i] < 0) {
+            *reinterpret_cast<uint32_t*>(to) = 0x7F7F7F7Fu;
+          } else if (x_words) {
+            cp_async4(smem_addr(to), from);
+          } else {
+#pragma unroll 1
+            for (int c = 0; c < left; ++c) to[c] = from[c];
+          }
+        }
+        ++filled;
+        if (++q > (piece.hi - 1) / 4) {
+          more = walk.next(&piece);
+          q = piece.lo / 4;
+          if (more) find_rows();
+        }
+      }
+      cp_async_commit();
+    };
+    if (more) find_rows();
+#pragma unroll 1
+    for (int i = 0; i < kScaleEntries - 1; ++i) fetch();
+    for (unsigned n = 0; n < filled; ++n) {
+      cp_async_wait<kScaleEntries - 2>();
+      bar_sync(4, 32 * kScaleWarps);  // all have this entry's copies, and have read the one before
+      const uint8_t* entry = scale_ring + (n % kScaleEntries) * entry_bytes;
+      fetch();
+      const int buf = n & 1;
+      // (no break after an abort: the others wait at the barrier above)
+      wait_bar(&ctl->scale_empty[buf], ((n >> 1) & 1) ^ 1, abort_flag, err);
+      tc_fence_after();
+      // (what lies behind a tile's rows or chunks is not used)
+      uint32_t v[32];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (kFp8) {
+          const uint32_t u = *reinterpret_cast<const uint32_t*>(entry + 4 * t);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[c * 8 + t * 4 + j] = ((u >> (8 * c)) & 0xFFu) * 0x01010101u;
+        } else {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            uint32_t v[4] = {0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu};
-            if (there[t][j]) {
-              if (kFp8) {
-                // (one block of 128 outputs: the same in every lane)
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                  if (4 * q + c < chunks) v[c] = wrow[t][j][4 * q + c] * 0x01010101u;
-              } else if (wide) {
-                const uint4 u = __ldg(reinterpret_cast<const uint4*>(wrow[t][j] + 16 * q));
-                v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
-              } else {
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                  if (4 * q + c < chunks)
-                    v[c] = __ldg(reinterpret_cast<const uint32_t*>(wrow[t][j] + 16 * q) + c);
-              }
-            }
-#pragma unroll
-            for (int c = 0; c < 4; ++c) wa[c * 8 + t * 4 + j] = v[c];
+            const uint4 u = *reinterpret_cast<const uint4*>(entry + (t * kTileRows + j * 32 + lane) * 16);
+            v[t * 4 + j] = u.x;
+            v[8 + t * 4 + j] = u.y;
+            v[16 + t * 4 + j] = u.z;
+            v[24 + t * 4 + j] = u.w;
           }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          uint32_t w = 0x7F7F7F7Fu;
-          if (j < 6 && x_there[j < 6 ? j : 0]) {
-            const uint8_t* s = xrow[j < 6 ? j : 0] + 4 * q;
-            if (x_words) {
-              w = __ldg(reinterpret_cast<const uint32_t*>(s));
-            } else {
-#pragma unroll
-              for (int c = 0; c < 4; ++c)
-                if (4 * q + c < chunks) w = (w & ~(0xFFu << (8 * c))) | (static_cast<uint32_t>(s[c]) << (8 * c));
-            }
-          }
-#pragma unroll
-          for (int c = 0; c < 4; ++c) xb[c * 8 + j] = ((w >> (8 * c)) & 0xFFu) * 0x01010101u;
         }
-        const int buf = n & 1;
-        good = wait_bar(&ctl->scale_empty[buf], ((n >> 1) & 1) ^ 1, abort_flag, err);
-        if (!good) break;
-        tc_fence_after();
-        tmem_st32(tmem + lanes + buf * kScaleCols, wa);
-        tmem_st32(tmem + lanes + buf * kScaleCols + 32, xb);
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(&ctl->scale_full[buf]);
-        ++n;
       }
+      tmem_st32(tmem + lanes + buf * kScaleCols, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint32_t w = 0;
+        if (j * 32 < a.n_max)
+          w = *reinterpret_cast<const uint32_t*>(entry + kScaleBytes + (j * 32 + lane) * 4);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c * 8 + j] = ((w >> (8 * c)) & 0xFFu) * 0x01010101u;
+      }
+      tmem_st32(tmem + lanes + buf * kScaleCols + 32, v);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&ctl->scale_full[buf]);
     }
-  } else if (warp == kWarpCopy) {
-    // -------------------------------------------------------------- copies
-    unsigned n = 0;
-    bool good = true;
-    int s = 0;
+    cp_async_wait<0>();
+  } else if (warp < kWarpCopy) {
+    // ---------------------------------------------------------------- rows
+    // 16 bytes a thread, eight threads a row, swizzled. (A gather by TMA took
+    // some 100 clocks for four rows: 8,192 tokens of 4096 x 2048 4.4 ms.)
+    const int st = threadIdx.x - 32 * kWarpRows;
+    const uint8_t* x_from = p.xq + (st & 7) * 16;
+    const uint32_t x_to = 2 * kATile + (st >> 3) * kChunk + (((st & 7) ^ ((st >> 3) & 7)) << 4);
+    Piece next;
+    int rows[2];  // of the next piece, asked for while this one's are copied; -1: zeros
+    auto find_rows = [&] {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = st + i * 32 * kRowWarps;
+        int v = -1;
+        if (r < next.rows) v = p.src ? p.src[next.row0 + r] : next.row0 + r;
+        rows[i] = v >= 0 && v < p.x_rows ? v : -1;
+      }
+    };
+    int s = 0, turn = 0;
     uint32_t phase = 1;
-    while (good && walk.next(&piece)) {
-      int rows[2][4];
-      const int gathers = piece.n / 4;
+    bool good = true, more = walk.next(&next);
+    if (more) find_rows();
+    while (more) {
+      int* table = row_table + turn * a.n_max;
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = (g * 32 + lane) * 4 + i;
-          rows[g][i] = -1;
-          if (r < piece.rows) rows[g][i] = p.src ? p.src[piece.row0 + r] : piece.row0 + r;
-        }
-      const bool second = two_tiles(piece);
-      // (a tile of E2M1 takes a byte an element in shared memory, but counts
-      // with what is read)
-      constexpr int kTileTx = kFp8 ? kATile : kATile / 2;
-      const uint32_t tx = (second ? 2 : 1) * kTileTx + piece.n * kChunk;
-      const int row = piece.row_tile * kOuts;
+      for (int i = 0; i < 2; ++i)
+        if (st + i * 32 * kRowWarps < a.n_max) table[st + i * 32 * kRowWarps] = rows[i];
+      bar_sync(5, 32 * kRowWarps);  // (two tables: nobody is two pieces behind)
+      piece = next;
+      more = walk.next(&next);
+      if (more) find_rows();
+      table += st >> 3;
       for (int c = piece.lo; c < piece.hi; ++c) {
-        good = wait_bar(&ctl->empty[s], phase, abort_flag, err);
-        good = __all_sync(0xffffffffu, good);
-        if (!good) break;
-        uint8_t* st = smem + static_cast<size_t>(s) * stage_bytes(a.n_max);
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&ctl->full[s], tx);
-          tma_load_3d(st, &map0, c * kChunk, row, piece.e, &ctl->full[s]);
-          if (second)
-            tma_load_3d(st + kATile, kGated ? &map1 : &map0, c * kChunk,
-                        kGated ? row : row + kTileRows, piece.e, &ctl->full[s]);
+        good = good && wait_bar(&ctl->empty[s], phase, abort_flag, err);
+        if (good) {
+          const uint32_t to = smem_addr(smem + static_cast<size_t>(s) * stage_bytes(a.n_max)) + x_to;
+          const uint8_t* from = x_from + c * kChunk;
+#pragma unroll 4
+          for (int r = 0; r < piece.n; r += 16) {
+            const int row = table[r];
+            cp_async16_or_0(to + r * kChunk, from + static_cast<size_t>(max(row, 0)) * p.width, row >= 0);
+          }
+          cp_async_arrive(&ctl->full[s]);
         }
-        __syncwarp();
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-          if (g * 32 + lane < gathers)
-            tma_gather4(st + 2 * kATile + (g * 32 + lane) * 4 * kChunk, &xmap, c * kChunk, rows[g],
-                        &ctl->full[s]);
-        ++n;
         if (++s == a.stages) {
           s = 0;
           phase ^= 1;
         }
       }
+      turn ^= 1;
     }
-    // after an abort: no copy may be under way when the block ends
-    if (!good && lane == 0)
-      for (unsigned i = n < static_cast<unsigned>(a.stages) ? 0 : n - a.stages; i < n; ++i)
-        mbar_wait(&ctl->full[i % a.stages], (i / a.stages) & 1, err);
+    cp_async_wait<0>();
+  } else if (warp == kWarpCopy) {
+    // -------------------------------------------------------------- copies
+    if (lane == 0) {
+      unsigned n = 0;
+      bool good = true;
+      int s = 0;
+      uint32_t phase = 1;
+      while (good && walk.next(&piece)) {
+        const bool second = two_tiles(piece);
+        // (a tile of E2M1 takes a byte an element in shared memory, but counts
+        // with what is read)
+        constexpr int kTileTx = kFp8 ? kATile : kATile / 2;
+        const int row = piece.row_tile * kOuts;
+        for (int c = piece.lo; c < piece.hi; ++c) {
+          good = wait_bar(&ctl->empty[s], phase, abort_flag, err);
+          if (!good) break;
+          uint8_t* st = smem + static_cast<size_t>(s) * stage_bytes(a.n_max);
+          mbar_arrive_expect_tx(&ctl->full[s], (second ? 2 : 1) * kTileTx);
+          tma_load_3d(st, &map0, c * kChunk, row, piece.e, &ctl->full[s]);
+          if (second)
+            tma_load_3d(st + kATile, kGated ? &map1 : &map0, c * kChunk,
+                        kGated ? row : row + kTileRows, piece.e, &ctl->full[s]);
+          ++n;
+          if (++s == a.stages) {
+            s = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      // after an abort: no copy may be under way when the block ends
+      if (!good)
+        for (unsigned i = n < static_cast<unsigned>(a.stages) ? 0 : n - a.stages; i < n; ++i)
+          mbar_wait(&ctl->full[i % a.stages], (i / a.stages) & 1, err);
+    }
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- MMAs
-    if (lane == 0) {
+    if (elect_one()) {
       const uint32_t idesc0 = ((kFp8 ? 0u : 5u) << 7) | (1u << 23) | (8u << 24);
       unsigned uses[2] = {0, 0}, scales = 0;
       int half = 0, s = 0;
@@ -702,6 +802,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
           good = good && wait_bar(&ctl->full[s], phase, abort_flag, err);
           if (!good) break;
           tc_fence_after();
+          fence_async_smem();  // the rows' copies are ordinary writes
           const uint32_t base = smem_addr(smem + static_cast<size_t>(s) * stage_bytes(a.n_max));
           const uint64_t a0 = umma_desc(base, 0, 1024), a1 = umma_desc(base + kATile, 0, 1024);
           const uint64_t b0 = umma_desc(base + 2 * kATile, 0, 1024);
@@ -905,8 +1006,10 @@ struct Shape {
 };
 Shape tile_shape(const GroupedProblem& p) {
   // rows of a group on average
-  if (p.rows <= 64ll * p.experts) return {64, 5};
-  return {kMaxN, 3};
+  const int n_max = p.rows <= 64ll * p.experts ? 64 : kMaxN;
+  int stages = kMaxStages;
+  while (smem_bytes(n_max, stages, p.experts) > kMaxSmem) --stages;
+  return {n_max, stages};
 }
 
 size_t parts_bytes(const GroupedProblem& p) {
@@ -924,9 +1027,8 @@ bool weight_map(CUtensorMap* m, const GroupedProblem& p, const uint8_t* w) {
 
 cudaError_t launch(const GroupedProblem& p, int* counters, float* parts, cudaStream_t st) {
   const bool gated = p.w[1] != nullptr;
-  CUtensorMap map0, map1, xmap;
-  if (!weight_map(&map0, p, p.w[0]) || !weight_map(&map1, p, gated ? p.w[1] : p.w[0]) ||
-      !make_tma_map_u8(&xmap, p.xq, p.width, p.x_rows, kChunk, 1, true, false))
+  CUtensorMap map0, map1;
+  if (!weight_map(&map0, p, p.w[0]) || !weight_map(&map1, p, gated ? p.w[1] : p.w[0]))
     return cudaErrorInvalidValue;
   Args a;
   a.p = p;
@@ -940,10 +1042,10 @@ cudaError_t launch(const GroupedProblem& p, int* counters, float* parts, cudaStr
   if (gated && p.fp8) return cudaErrorInvalidValue;
   auto kernel = gated ? grouped_kernel<false, true>
                       : p.fp8 ? grouped_kernel<true, false> : grouped_kernel<false, false>;
-  cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), 227 * 1024);
+  cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), static_cast<int>(kMaxSmem));
   if (e != cudaSuccess) return e;
   return launch_pdl(kernel, dim3(a.shares), dim3(kThreads),
-                    smem_bytes(s.n_max, s.stages, p.experts), st, map0, map1, xmap, a);
+                    smem_bytes(s.n_max, s.stages, p.experts), st, map0, map1, a);
 }
 
 // Pieces of a buffer, 256-byte aligned.
