@@ -17,7 +17,7 @@
 // that results do not depend on timing.
 //
 // Roles: warps 0-7 epilogue, 8-11 scales (to TMEM, each warp the copy of its
-// lane quarter), 12-15 rows of x, 16 copies of weights, 17 MMAs.
+// lane quarter), 12-13 copies of rows of x, 14 copies of weights, 15 MMAs.
 #include "grouped.cuh"
 
 #include <cuda_bf16.h>
@@ -31,7 +31,7 @@ namespace {
 constexpr int kChunk = 128;              // columns of a stage: one row of swizzled shared memory
 constexpr int kTileRows = 128;           // M of an instruction
 constexpr int kATile = kTileRows * kChunk;
-constexpr int kEpiWarps = 8, kScaleWarps = 4, kRowWarps = 4;
+constexpr int kEpiWarps = 8, kScaleWarps = 4, kRowWarps = 2;
 constexpr int kWarpRows = kEpiWarps + kScaleWarps, kWarpCopy = kWarpRows + kRowWarps;
 constexpr int kWarpMma = kWarpCopy + 1;
 constexpr int kThreads = 32 * (kWarpMma + 1);
@@ -48,6 +48,7 @@ struct Args {
   GroupedProblem p;
   int shares;         // blocks
   int n_max, stages;  // rows of a tile; stages of the ring
+  bool wide;          // out is BF16 and takes four outputs of a row at once
   int* counters;      // [kMaxShares] chunks whose parts are there
   float* parts;       // [shares][2][2][n_max][128]
 };
@@ -65,11 +66,11 @@ struct alignas(16) Control {
 };
 
 // The ring of scales: an entry holds four chunks' of 256 outputs and n_max rows.
+// Behind it each row warp's rows of x.
 constexpr int kScaleEntries = 4, kScaleBytes = 2 * kTileRows * 16;
 __host__ __device__ constexpr int scale_entry_bytes(int n_max) { return kScaleBytes + n_max * 4; }
-// Behind it the rows of x of two pieces.
 __host__ __device__ constexpr int scale_ring_bytes(int n_max) {
-  return kScaleEntries * scale_entry_bytes(n_max) + 2 * n_max * 4;
+  return kScaleEntries * scale_entry_bytes(n_max) + kRowWarps * n_max * 4;
 }
 
 __host__ __device__ constexpr int stage_bytes(int n_max) { return 2 * kATile + n_max * kChunk; }
@@ -126,35 +127,34 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
           smem_addr(bar))
       : "memory");
 }
-// 16 consecutive TMEM columns of this thread's lane.
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+// Four rows of a tensor map with one-row boxes, one behind the other; a row
+// outside the map is zeros.
+__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, int x, const int4& y,
+                                            uint64_t* bar) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
-      "%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w),
+      "r"(smem_addr(bar))
+      : "memory");
+}
+
+// 8 consecutive TMEM columns of this thread's lane.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+                 "=r"(r[7])
+               : "r"(taddr));
 }
 // The wait names the registers so that no use is scheduled before it.
-__device__ __forceinline__ void tmem_ld_wait16(uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_ld_wait8(uint32_t (&r)[8]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
-                 "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
-                 "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+                 "+r"(r[7])::"memory");
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-}
-// Zeros where there is nothing to be read.
-__device__ __forceinline__ void cp_async16_or_0(uint32_t to, const void* from, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0)
-               : "memory");
-}
-// This thread's arrival once all its copies so far are there.
-__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 __device__ __forceinline__ void cp_async4(uint32_t to, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
@@ -267,7 +267,7 @@ struct Walk {
 template <bool kFp8, bool kGated>
 __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUtensorMap map1,
-    const __grid_constant__ Args a) {
+    const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Args a) {
   extern __shared__ __align__(1024) uint8_t smem[];
   const GroupedProblem& p = a.p;
   uint8_t* scale_ring = smem + static_cast<size_t>(a.stages) * stage_bytes(a.n_max);
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.stages; ++i) {
-      mbar_init(&ctl->full[i], 1 + 32 * kRowWarps);  // the weights' copy, the threads' parts of the rows
+      mbar_init(&ctl->full[i], 1 + kRowWarps);
       mbar_init(&ctl->empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -300,6 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
   if (warp == kWarpCopy && lane == 0) {
     tma_prefetch_desc(&map0);
     if (kGated) tma_prefetch_desc(&map1);
+    tma_prefetch_desc(&xmap);
   }
   if (warp == kWarpMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -422,15 +423,15 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
       if (cut) {
         float* mine = part_of(me);
 #pragma unroll 1
-        for (int b = side; b < blocks; b += 2) {
-          uint32_t r0[16], r1[16];
-          tmem_ld16(sums + b * kBlockCols, r0);
-          if (second) tmem_ld16(sums1 + b * kBlockCols, r1);
-          tmem_ld_wait16(r0);
-          if (second) tmem_ld_wait16(r1);
+        for (int r = side * 8; r < piece.n; r += 16) {
+          uint32_t r0[8], r1[8];
+          tmem_ld8(sums + r, r0);
+          tmem_ld8(sums1 + r, r1);  // (not used where there is no second tile)
+          tmem_ld_wait8(r0);
+          tmem_ld_wait8(r1);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float* q = mine + static_cast<size_t>(b * kBlockCols + i) * kTileRows;
+          for (int i = 0; i < 8; ++i) {
+            float* q = mine + static_cast<size_t>(r + i) * kTileRows;
             __stcg(q, __uint_as_float(r0[i]));
             if (second) __stcg(q + tile_floats, __uint_as_float(r1[i]));
           }
@@ -451,30 +452,30 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
         if (!last) continue;
         __threadfence();
       }
-      // the sums of 16 rows of the group, this lane's output(s)
-      auto take = [&](int b, float (&v0)[16], float (&v1)[16]) {
+      // the sums of 8 rows of the group from r on, this lane's output(s)
+      auto take = [&](int r, float* v0, float* v1) {
         if (!cut) {
-          uint32_t r0[16], r1[16];
-          tmem_ld16(sums + b * kBlockCols, r0);
-          if (second) tmem_ld16(sums1 + b * kBlockCols, r1);
-          tmem_ld_wait16(r0);
-          if (second) tmem_ld_wait16(r1);
+          uint32_t r0[8], r1[8];
+          tmem_ld8(sums + r, r0);
+          tmem_ld8(sums1 + r, r1);
+          tmem_ld_wait8(r0);
+          tmem_ld_wait8(r1);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < 8; ++i) {
             v0[i] = __uint_as_float(r0[i]);
-            v1[i] = second ? __uint_as_float(r1[i]) : 0.f;
+            v1[i] = __uint_as_float(r1[i]);
           }
           return;
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v0[i] = v1[i] = 0.f;
+        for (int i = 0; i < 8; ++i) v0[i] = v1[i] = 0.f;
 #pragma unroll 1
         for (int c = c0; c <= c1; ++c) {
           if (chunk_at(bound(c) - start, chunks, cost) >= chunk_at(bound(c + 1) - start, chunks, cost))
             continue;
-          const float* q = part_of(c) + static_cast<size_t>(b) * kBlockCols * kTileRows;
+          const float* q = part_of(c) + static_cast<size_t>(r) * kTileRows;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < 8; ++i) {
             v0[i] += __ldcg(q + i * kTileRows);
             if (second) v1[i] += __ldcg(q + tile_floats + i * kTileRows);
           }
@@ -487,10 +488,11 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
       for (int b = side; b < blocks; b += 2) {
         const int row_data = row_next;
         row_next = lane_row(b + 2);
-        float v0[16], v1[16];
-        take(b, v0, v1);
-        const int n = min(kBlockCols, piece.rows - b * kBlockCols);
         if (kGated) {
+          const int n = min(kBlockCols, piece.rows - b * kBlockCols);
+          float v0[16], v1[16];
+          take(b * kBlockCols, v0, v1);
+          take(b * kBlockCols + 8, v0 + 8, v1 + 8);
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             const float g = fminf(v0[j], p.limit), u = fminf(fmaxf(v1[j], -p.limit), p.limit);
@@ -535,20 +537,53 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
         } else {
           const int o0 = piece.row_tile * kOuts + at, o1 = o0 + kTileRows;
           const bool in0 = o0 < p.outs, in1 = o1 < p.outs;
-          auto put = [&](auto* o, int d, auto x0, auto x1) {
-            o += d * p.out_stride;
-            if (in0 && d >= 0) o[o0] = x0;
-            if (in1 && d >= 0) o[o1] = x1;
-          };
-          if (p.bf16) {
+#pragma unroll 1
+          for (int r = 0; r < kBlockCols; r += 8) {
+            float v0[8], v1[8];
+            take(b * kBlockCols + r, v0, v1);
+            if (a.wide) {
+              // BF16, four outputs of a row a lane: pairs of rows as a word, and
+              // two exchanges turn rows into outputs (half the time of stores
+              // of two bytes a lane)
+              const int k = lane & 3;
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              put(static_cast<__nv_bfloat16*>(p.out), __shfl_sync(0xffffffffu, row_data, j),
-                  __float2bfloat16_rn(v0[j]), __float2bfloat16_rn(v1[j]));
-          } else {
+              for (int t = 0; t < 2; ++t) {
+                const float* v = t ? v1 : v0;
+                const int o = (t ? o1 : o0) - k;
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              put(static_cast<float*>(p.out), __shfl_sync(0xffffffffu, row_data, j), v0[j], v1[j]);
+                for (int j = 0; j < 8; j += 4) {
+                  uint32_t w0 = pack_bf16x2(v[j], v[j + 1]), w1 = pack_bf16x2(v[j + 2], v[j + 3]);
+                  // lane 2i: rows j and j + 2 of outputs 2i, 2i + 1; lane 2i + 1: the others
+                  const uint32_t x0 = __shfl_xor_sync(0xffffffffu, w0, 1);
+                  const uint32_t x1 = __shfl_xor_sync(0xffffffffu, w1, 1);
+                  const uint32_t pick = (k & 1) ? 0x3276u : 0x5410u;
+                  w0 = __byte_perm(w0, x0, pick);
+                  w1 = __byte_perm(w1, x1, pick);
+                  // lane 4i + k: row j + (k & 1) + (k & 2) of outputs 4i .. 4i + 3
+                  const uint32_t y = __shfl_xor_sync(0xffffffffu, (k & 2) ? w0 : w1, 2);
+                  const uint2 word = (k & 2) ? make_uint2(y, w1) : make_uint2(w0, y);
+                  const int d = __shfl_sync(0xffffffffu, row_data, r + j + k);
+                  if (d >= 0 && o < p.outs)
+                    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + d * p.out_stride + o) = word;
+                }
+              }
+            } else {
+              auto put = [&](auto* o, int d, auto x0, auto x1) {
+                o += d * p.out_stride;
+                if (in0 && d >= 0) o[o0] = x0;
+                if (in1 && d >= 0) o[o1] = x1;
+              };
+              if (p.bf16) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  put(static_cast<__nv_bfloat16*>(p.out), __shfl_sync(0xffffffffu, row_data, r + j),
+                      __float2bfloat16_rn(v0[j]), __float2bfloat16_rn(v1[j]));
+              } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  put(static_cast<float*>(p.out), __shfl_sync(0xffffffffu, row_data, r + j), v0[j], v1[j]);
+              }
+            }
           }
         }
       }
@@ -690,56 +725,66 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     cp_async_wait<0>();
   } else if (warp < kWarpCopy) {
     // ---------------------------------------------------------------- rows
-    // 16 bytes a thread, eight threads a row, swizzled. (A gather by TMA took
-    // some 100 clocks for four rows: 8,192 tokens of 4096 x 2048 4.4 ms.)
-    const int st = threadIdx.x - 32 * kWarpRows;
-    const uint8_t* x_from = p.xq + (st & 7) * 16;
-    const uint32_t x_to = 2 * kATile + (st >> 3) * kChunk + (((st & 7) ^ ((st >> 3) & 7)) << 4);
-    Piece next;
-    int rows[2];  // of the next piece, asked for while this one's are copied; -1: zeros
-    auto find_rows = [&] {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = st + i * 32 * kRowWarps;
-        int v = -1;
-        if (r < next.rows) v = p.src ? p.src[next.row0 + r] : next.row0 + r;
-        rows[i] = v >= 0 && v < p.x_rows ? v : -1;
-      }
-    };
-    int s = 0, turn = 0;
+    // Each warp's elected thread copies half of a tile's rows: rows in their
+    // order 16 at a time, others by gathers of four. (Copies of 16 bytes a
+    // thread moved 27 bytes a clock at most.)
+    const int part = warp - kWarpRows;
+    int* table = row_table + part * a.n_max;
+    int s = 0;
     uint32_t phase = 1;
-    bool good = true, more = walk.next(&next);
-    if (more) find_rows();
-    while (more) {
-      int* table = row_table + turn * a.n_max;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (st + i * 32 * kRowWarps < a.n_max) table[st + i * 32 * kRowWarps] = rows[i];
-      bar_sync(5, 32 * kRowWarps);  // (two tables: nobody is two pieces behind)
-      piece = next;
-      more = walk.next(&next);
-      if (more) find_rows();
-      table += st >> 3;
-      for (int c = piece.lo; c < piece.hi; ++c) {
-        good = good && wait_bar(&ctl->empty[s], phase, abort_flag, err);
-        if (good) {
-          const uint32_t to = smem_addr(smem + static_cast<size_t>(s) * stage_bytes(a.n_max)) + x_to;
-          const uint8_t* from = x_from + c * kChunk;
-#pragma unroll 4
-          for (int r = 0; r < piece.n; r += 16) {
-            const int row = table[r];
-            cp_async16_or_0(to + r * kChunk, from + static_cast<size_t>(max(row, 0)) * p.width, row >= 0);
-          }
-          cp_async_arrive(&ctl->full[s]);
+    unsigned n = 0;
+    bool good = true;
+    while (walk.next(&piece)) {
+      if (p.src) {
+        for (int r = lane; r < piece.n; r += 32) {
+          int v = -1;  // outside the map: zeros
+          if (r < piece.rows) v = p.src[piece.row0 + r];
+          table[r] = v;
         }
-        if (++s == a.stages) {
-          s = 0;
-          phase ^= 1;
-        }
+        __syncwarp();
       }
-      turn ^= 1;
+      if (elect_one()) {
+        const int step = p.src ? 4 : 16;
+        const int copies = (piece.n / step + kRowWarps - 1 - part) / kRowWarps;
+        const uint32_t bytes = copies * step * kChunk;
+        for (int c = piece.lo; c < piece.hi; ++c) {
+          good = good && wait_bar(&ctl->empty[s], phase, abort_flag, err);
+          if (!good) break;
+          uint8_t* to = smem + static_cast<size_t>(s) * stage_bytes(a.n_max) + 2 * kATile;
+          mbar_arrive_expect_tx(&ctl->full[s], bytes);
+          if (p.src) {
+            const int4* rows = reinterpret_cast<const int4*>(table) + part;
+            to += part * 4 * kChunk;
+            int4 next = rows[0];
+#pragma unroll 1
+            for (int i = 0; i < copies; ++i) {
+              const int4 r = next;
+              rows += kRowWarps;
+              if (i + 1 < copies) next = rows[0];
+              tma_gather4(to, &xmap, c * kChunk, r, &ctl->full[s]);
+              to += kRowWarps * 4 * kChunk;
+            }
+          } else {
+            to += part * 16 * kChunk;
+            int r = piece.row0 + part * 16;
+#pragma unroll 1
+            for (int i = 0; i < copies; ++i) {
+              tma_load_2d(to, &xmap, c * kChunk, r, &ctl->full[s]);
+              r += kRowWarps * 16;
+              to += kRowWarps * 16 * kChunk;
+            }
+          }
+          ++n;
+          if (++s == a.stages) {
+            s = 0;
+            phase ^= 1;
+          }
+        }
+        // after an abort: no copy may be under way when the block ends
+        if (!good && n > 0) mbar_wait(&ctl->full[(n - 1) % a.stages], ((n - 1) / a.stages) & 1, err);
+      }
+      __syncwarp();
     }
-    cp_async_wait<0>();
   } else if (warp == kWarpCopy) {
     // -------------------------------------------------------------- copies
     if (lane == 0) {
@@ -769,7 +814,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
           }
         }
       }
-      // after an abort: no copy may be under way when the block ends
+      // after an abort: as above
       if (!good)
         for (unsigned i = n < static_cast<unsigned>(a.stages) ? 0 : n - a.stages; i < n; ++i)
           mbar_wait(&ctl->full[i % a.stages], (i / a.stages) & 1, err);
@@ -802,7 +847,6 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
           good = good && wait_bar(&ctl->full[s], phase, abort_flag, err);
           if (!good) break;
           tc_fence_after();
-          fence_async_smem();  // the rows' copies are ordinary writes
           const uint32_t base = smem_addr(smem + static_cast<size_t>(s) * stage_bytes(a.n_max));
           const uint64_t a0 = umma_desc(base, 0, 1024), a1 = umma_desc(base + kATile, 0, 1024);
           const uint64_t b0 = umma_desc(base + 2 * kATile, 0, 1024);
@@ -839,6 +883,25 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                  "r"(kTmemCols)
                  : "memory");
+}
+
+// Rows src[r] of x and their scales one behind the other, zeros for rows that
+// are none. A block a row.
+__global__ void __launch_bounds__(128) gather_rows_kernel(const uint8_t* __restrict__ xq,
+                                                          const uint8_t* __restrict__ xs,
+                                                          const int* __restrict__ src, int x_rows,
+                                                          int width, uint8_t* __restrict__ yq,
+                                                          uint8_t* __restrict__ ys) {
+  pdl_wait();
+  pdl_trigger();
+  const size_t r = blockIdx.x;
+  const int v = src[r], groups = width / kChunk;
+  const bool there = v >= 0 && v < x_rows;
+  const size_t from = there ? v : 0;
+  const uint4* a = reinterpret_cast<const uint4*>(xq + from * width);
+  uint4* b = reinterpret_cast<uint4*>(yq + r * width);
+  for (int i = threadIdx.x; i < width / 16; i += 128) b[i] = there ? a[i] : make_uint4(0, 0, 0, 0);
+  for (int i = threadIdx.x; i < groups; i += 128) ys[r * groups + i] = there ? xs[from * groups + i] : 0x7F;
 }
 
 __global__ void grouped_reset_kernel(int* counters) {
@@ -883,22 +946,28 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(const GroupArgs a)
 #pragma unroll
       for (int i = 0; i < kGroupAhead; ++i) {
         const int s = base + i * 32 + lane;
-        e[i] = s < s1 ? a.idx[s] - a.lo : -1;
-        if (e[i] >= a.experts || e[i] < 0) e[i] = -1;
+        e[i] = s < s1 ? a.idx[s] - a.lo : a.experts;
+        if (e[i] >= a.experts || e[i] < 0) e[i] = a.experts;  // none of these
       }
 #pragma unroll
       for (int i = 0; i < kGroupAhead; ++i) {
         if (base + i * 32 >= s1) break;
-        const unsigned same = __match_any_sync(0xffffffffu, e[i]);
+        // the lanes with this lane's expert (a match instruction took 3,000
+        // clocks for 32 experts: 12,000 slots 41 us)
+        unsigned same = 0xffffffffu;
+        for (int b = 1; b <= a.experts; b <<= 1) {
+          const unsigned set = __ballot_sync(0xffffffffu, e[i] & b);
+          same &= (e[i] & b) ? set : ~set;
+        }
         const int first = __ffs(same) - 1;
         int at = 0;
-        if (lane == first && e[i] >= 0) {
+        if (lane == first && e[i] < a.experts) {
           at = mine[e[i]];
           mine[e[i]] = at + __popc(same);
         }
         at = __shfl_sync(0xffffffffu, at, first) + __popc(same & ((1u << lane) - 1));
         __syncwarp();
-        if (e[i] >= 0) f(base + i * 32 + lane, at);
+        if (e[i] < a.experts) f(base + i * 32 + lane, at);
       }
     }
   };
@@ -1005,8 +1074,8 @@ struct Shape {
   int n_max, stages;
 };
 Shape tile_shape(const GroupedProblem& p) {
-  // rows of a group on average
-  const int n_max = p.rows <= 64ll * p.experts ? 64 : kMaxN;
+  const long long rows = p.rows, each = p.experts;  // rows of a group on average
+  const int n_max = rows <= 8 * each ? 16 : rows <= 24 * each ? 32 : rows <= 96 * each ? 128 : kMaxN;
   int stages = kMaxStages;
   while (smem_bytes(n_max, stages, p.experts) > kMaxSmem) --stages;
   return {n_max, stages};
@@ -1018,6 +1087,21 @@ size_t parts_bytes(const GroupedProblem& p) {
 
 constexpr size_t kCounterBytes = kMaxShares * sizeof(int);
 
+size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+// Rows that are not in their order are brought into it beforehand where a
+// group has more than a few: their copy by TMA gathers takes 48 clocks for four
+// rows, which the weights' copy covers up to some 16 rows a tile (32 tokens of
+// 7168 x 2048: 646 us, 655 with the copy).
+bool gathers_first(const GroupedProblem& p, bool has_src) {
+  return has_src && p.rows > 16ll * p.experts;
+}
+size_t gather_bytes(const GroupedProblem& p, bool has_src) {
+  if (!gathers_first(p, has_src)) return 0;
+  return up256(static_cast<size_t>(p.rows) * p.width) +
+         up256(static_cast<size_t>(p.rows) * (p.width / kChunk));
+}
+
 bool weight_map(CUtensorMap* m, const GroupedProblem& p, const uint8_t* w) {
   if (p.fp8)
     return make_tma_map_u8_3d(m, w, p.width, p.outs, p.width, p.experts,
@@ -1025,10 +1109,23 @@ bool weight_map(CUtensorMap* m, const GroupedProblem& p, const uint8_t* w) {
   return make_tma_map_u4_3d(m, w, p.width, p.outs, p.experts, kTileRows);
 }
 
-cudaError_t launch(const GroupedProblem& p, int* counters, float* parts, cudaStream_t st) {
+// gathered: gather_bytes() where the rows are brought into their order first.
+cudaError_t launch(GroupedProblem p, int* counters, float* parts, void* gathered, cudaStream_t st) {
   const bool gated = p.w[1] != nullptr;
-  CUtensorMap map0, map1;
-  if (!weight_map(&map0, p, p.w[0]) || !weight_map(&map1, p, gated ? p.w[1] : p.w[0]))
+  if (gathers_first(p, p.src != nullptr)) {
+    uint8_t* yq = static_cast<uint8_t*>(gathered);
+    uint8_t* ys = yq + up256(static_cast<size_t>(p.rows) * p.width);
+    cudaError_t e = launch_pdl(gather_rows_kernel, dim3(p.rows), dim3(128), 0, st, p.xq, p.xs, p.src,
+                               p.x_rows, p.width, yq, ys);
+    if (e != cudaSuccess) return e;
+    p.xq = yq;
+    p.xs = ys;
+    p.src = nullptr;
+    p.x_rows = p.rows;
+  }
+  CUtensorMap map0, map1, xmap;
+  if (!weight_map(&map0, p, p.w[0]) || !weight_map(&map1, p, gated ? p.w[1] : p.w[0]) ||
+      !make_tma_map_u8(&xmap, p.xq, p.width, p.x_rows, kChunk, p.src ? 1 : 16, true, false))
     return cudaErrorInvalidValue;
   Args a;
   a.p = p;
@@ -1036,6 +1133,8 @@ cudaError_t launch(const GroupedProblem& p, int* counters, float* parts, cudaStr
   const Shape s = tile_shape(p);
   a.n_max = s.n_max;
   a.stages = s.stages;
+  a.wide = p.bf16 && p.outs % 4 == 0 && p.out_stride % 4 == 0 &&
+           reinterpret_cast<uintptr_t>(p.out) % 8 == 0;
   a.counters = counters;
   a.parts = parts;
   if (a.shares < 1) return cudaErrorInvalidDevice;
@@ -1045,7 +1144,7 @@ cudaError_t launch(const GroupedProblem& p, int* counters, float* parts, cudaStr
   cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), static_cast<int>(kMaxSmem));
   if (e != cudaSuccess) return e;
   return launch_pdl(kernel, dim3(a.shares), dim3(kThreads),
-                    smem_bytes(s.n_max, s.stages, p.experts), st, map0, map1, a);
+                    smem_bytes(s.n_max, s.stages, p.experts), st, map0, map1, xmap, a);
 }
 
 // Pieces of a buffer, 256-byte aligned.
@@ -1063,7 +1162,7 @@ struct Carver {
 struct ExpertsWork {
   int *counters, *offsets, *slot, *token;
   float *weight, *parts;
-  uint8_t *hq, *hs;
+  uint8_t *hq, *hs, *gathered;
   uint16_t* y;
   size_t bytes;
 };
@@ -1101,14 +1200,18 @@ ExpertsWork experts_work(const ExpertsProblem& p, void* base) {
   w.hq = c.take<uint8_t>(slots * p.inter);
   w.hs = c.take<uint8_t>(slots * (p.inter / 128));
   w.y = c.take<uint16_t>(slots * p.hidden);
-  w.parts = c.take<float>(parts_bytes(gate_up(p, w)) / sizeof(float));
+  const GroupedProblem g = gate_up(p, w);
+  w.parts = c.take<float>(parts_bytes(g) / sizeof(float));
+  w.gathered = c.take<uint8_t>(gather_bytes(g, true));
   w.bytes = c.used;
   return w;
 }
 
 }  // namespace
 
-size_t grouped_workspace_bytes(const GroupedProblem& p) { return kCounterBytes + parts_bytes(p); }
+size_t grouped_workspace_bytes(const GroupedProblem& p) {
+  return kCounterBytes + up256(parts_bytes(p)) + gather_bytes(p, true);  // should src be given
+}
 
 cudaError_t grouped_reset(void* ws, cudaStream_t st) {
   return launch_pdl(grouped_reset_kernel, dim3(1), dim3(kMaxShares), 0, st, static_cast<int*>(ws));
@@ -1116,8 +1219,8 @@ cudaError_t grouped_reset(void* ws, cudaStream_t st) {
 
 cudaError_t grouped_forward(const GroupedProblem& p, void* ws, cudaStream_t st) {
   if (p.rows <= 0) return cudaSuccess;
-  return launch(p, static_cast<int*>(ws),
-                reinterpret_cast<float*>(static_cast<char*>(ws) + kCounterBytes), st);
+  char* at = static_cast<char*>(ws) + kCounterBytes;
+  return launch(p, static_cast<int*>(ws), reinterpret_cast<float*>(at), at + up256(parts_bytes(p)), st);
 }
 
 size_t experts_workspace_bytes(const ExpertsProblem& p) { return experts_work(p, nullptr).bytes; }
@@ -1143,7 +1246,7 @@ cudaError_t experts_forward(const ExpertsProblem& p, void* ws, cudaStream_t st) 
   if (e == cudaSuccess) e = launch_pdl(group_kernel, dim3(1), dim3(kGroupThreads), smem, st, a);
   if (e != cudaSuccess) return e;
   const GroupedProblem g = gate_up(p, w);
-  e = launch(g, w.counters, w.parts, st);
+  e = launch(g, w.counters, w.parts, w.gathered, st);
   if (e != cudaSuccess) return e;
   GroupedProblem d;
   d.experts = p.experts;
@@ -1161,7 +1264,7 @@ cudaError_t experts_forward(const ExpertsProblem& p, void* ws, cudaStream_t st) 
   d.out = w.y;
   d.out_stride = p.hidden;
   d.err = p.err;
-  e = launch(d, w.counters + kMaxShares, w.parts, st);
+  e = launch(d, w.counters + kMaxShares, w.parts, nullptr, st);
   if (e != cudaSuccess) return e;
   const long long vecs = static_cast<long long>(p.n) * (p.hidden / 8);
   return launch_pdl(experts_combine_kernel, dim3(static_cast<unsigned>((vecs + 255) / 256)), dim3(256),
