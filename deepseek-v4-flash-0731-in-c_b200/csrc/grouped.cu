@@ -60,6 +60,7 @@ struct alignas(16) Control {
   uint64_t fin;
   uint32_t tmem;
   int abort_flag;
+  int shares, snap;
   int last;      // the block brought a tile's last part
   alignas(16) uint32_t top[2][2][4][kBlockCols];  // largest |h| of a warp's 32 outputs
   alignas(16) uint8_t codes[2][kBlockCols][kTileRows];
@@ -76,7 +77,8 @@ __host__ __device__ constexpr int scale_ring_bytes(int n_max) {
 __host__ __device__ constexpr int stage_bytes(int n_max) { return 2 * kATile + n_max * kChunk; }
 __host__ __device__ inline size_t smem_bytes(int n_max, int stages, int experts) {
   return static_cast<size_t>(stages) * stage_bytes(n_max) + scale_ring_bytes(n_max) +
-         sizeof(Control) + (experts + 1) * (sizeof(long long) + sizeof(int));
+         sizeof(Control) + (kMaxShares + 1) * sizeof(long long) +
+         (experts + 1) * (sizeof(long long) + sizeof(int));
 }
 
 // Suspended waits: the epilogue needs the issue slots.
@@ -153,6 +155,22 @@ __device__ __forceinline__ void tmem_ld_wait8(uint32_t (&r)[8]) {
                  "+r"(r[7])::"memory");
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_wait16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                 "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
+                 "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+}
+
 __device__ __forceinline__ void cp_async16(uint32_t to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
@@ -178,6 +196,7 @@ struct Cut {
   int tiles, rows, cost;
 };
 constexpr int kMemoryCost = 90;
+constexpr int kSnapTiles = 8;  // shares of so many tiles on average are not cut
 __device__ __forceinline__ Cut cut_group(int n, int n_max) {
   Cut c;
   c.tiles = (n + n_max - 1) / n_max;
@@ -202,6 +221,16 @@ __device__ __forceinline__ int chunk_at(long long d, int chunks, int cost) {
                       : static_cast<int>(static_cast<unsigned>(d) / static_cast<unsigned>(cost));
 }
 
+// The last group that does not start behind position b; prefix [experts + 1].
+__device__ __forceinline__ int group_at(const long long* prefix, int experts, long long b) {
+  int low = 0, high = experts;
+  while (high - low > 1) {
+    const int mid = (low + high) >> 1;
+    if (prefix[mid] <= b) low = mid; else high = mid;
+  }
+  return low;
+}
+
 // Each role walks its share's pieces by itself. All of it stays in registers:
 // there is no L1 to speak of beside 227 KB of shared memory, so a stack costs
 // an L2 access each time.
@@ -217,12 +246,7 @@ struct Walk {
   __device__ __forceinline__ void begin(const long long* prefix, long long b0, long long b1) {
     left = 0;
     if (b0 >= b1) return;
-    int low = 0, high = experts;  // the last group whose start is not behind b0
-    while (high - low > 1) {
-      const int mid = (low + high) >> 1;
-      if (prefix[mid] <= b0) low = mid; else high = mid;
-    }
-    e = low;
+    e = group_at(prefix, experts, b0);
     recut();
     const long long tile = static_cast<long long>(chunks) * cut.cost, d = b0 - prefix[e];
     const int item = static_cast<int>(d / tile);
@@ -273,7 +297,8 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
   uint8_t* scale_ring = smem + static_cast<size_t>(a.stages) * stage_bytes(a.n_max);
   int* row_table = reinterpret_cast<int*>(scale_ring + kScaleEntries * scale_entry_bytes(a.n_max));
   Control* ctl = reinterpret_cast<Control*>(scale_ring + scale_ring_bytes(a.n_max));
-  long long* prefix = reinterpret_cast<long long*>(ctl + 1);
+  long long* bounds = reinterpret_cast<long long*>(ctl + 1);  // [shares + 1] in cost
+  long long* prefix = bounds + kMaxShares + 1;                // [experts + 1] cost before each group
   int* offsets = reinterpret_cast<int*>(prefix + p.experts + 1);
   volatile int* abort_flag = &ctl->abort_flag;
   unsigned* err = p.err;
@@ -331,9 +356,11 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
       at = __shfl_sync(0xffffffffu, o, 31);
     }
     __syncwarp();
+    long long tiles = 0;
     for (int e0 = 0; e0 <= p.experts; e0 += 32) {
       const int e = e0 + lane;
       const Cut c = cut_group(e < p.experts ? offsets[e + 1] - offsets[e] : 0, a.n_max);
+      tiles += c.tiles;
       const long long mine = static_cast<long long>(c.tiles) * row_tiles * chunks * c.cost;
       long long incl = mine;
 #pragma unroll
@@ -344,17 +371,36 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
       if (e <= p.experts) prefix[e] = run + incl - mine;
       run += __shfl_sync(0xffffffffu, incl, 31);
     }
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, s);
+    if (lane == 0) {
+      // Shares of a few chunks at least: a cut costs two fp32 parts, their
+      // writing, meeting and reading.
+      constexpr int kMinChunks = 4;
+      const long long most = run / (kMinChunks * kMemoryCost);
+      ctl->shares = most < 1 ? 1 : most < a.shares ? static_cast<int>(most) : a.shares;
+      ctl->snap = tiles * row_tiles >= static_cast<long long>(kSnapTiles) * ctl->shares;
+    }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ctl->tmem;
-  const long long total = prefix[p.experts];
-  // Shares of a few chunks at least: a cut costs two fp32 parts.
-  constexpr int kMinChunks = 4;
-  const long long most = total / (kMinChunks * kMemoryCost);
-  const int shares = most < 1 ? 1 : most < a.shares ? static_cast<int>(most) : a.shares;
-  auto bound = [&](int c) { return c >= shares ? total : total * c / shares; };
+  const int shares = ctl->shares;
+  // Where each share begins. Shares of many tiles take whole ones.
+  for (int c = threadIdx.x; c <= shares; c += kThreads) {
+    const long long total = prefix[p.experts];
+    long long b = total * c / shares;
+    if (ctl->snap && c > 0 && c < shares) {
+      const int e = group_at(prefix, p.experts, b);
+      const Cut g = cut_group(offsets[e + 1] - offsets[e], a.n_max);
+      const unsigned tile = chunks * g.cost;
+      b = prefix[e] + static_cast<long long>((static_cast<unsigned long long>(b - prefix[e]) + tile / 2) / tile) * tile;
+    }
+    bounds[c] = b;
+  }
+  __syncthreads();
+  auto bound = [&](int c) { return bounds[c]; };  // c <= shares
   const int me = blockIdx.x;
   Walk walk;
   walk.offsets = offsets;
@@ -362,8 +408,8 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
   walk.row_tiles = row_tiles;
   walk.chunks = chunks;
   walk.n_max = a.n_max;
-  const long long share_end = bound(me + 1);
-  walk.begin(prefix, bound(me), share_end);
+  const long long share_end = me < shares ? bound(me + 1) : 0;
+  walk.begin(prefix, me < shares ? bound(me) : 0, share_end);
   Piece piece;
   auto two_tiles = [&](const Piece& q) {
     return kGated || q.row_tile * kOuts + kTileRows < p.outs;
@@ -452,32 +498,45 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
         if (!last) continue;
         __threadfence();
       }
-      // the sums of 8 rows of the group from r on, this lane's output(s)
-      auto take = [&](int r, float* v0, float* v1) {
+      // the sums of a block's 16 rows, this lane's output(s); from TMEM they are
+      // asked for a block ahead
+      uint32_t ahead0[16], ahead1[16];
+      if (!cut && side < blocks) {
+        tmem_ld16(sums + side * kBlockCols, ahead0);
+        tmem_ld16(sums1 + side * kBlockCols, ahead1);
+      }
+      auto take = [&](int b, float (&v0)[16], float (&v1)[16]) {
         if (!cut) {
-          uint32_t r0[8], r1[8];
-          tmem_ld8(sums + r, r0);
-          tmem_ld8(sums1 + r, r1);
-          tmem_ld_wait8(r0);
-          tmem_ld_wait8(r1);
+          tmem_ld_wait16(ahead0);
+          tmem_ld_wait16(ahead1);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            v0[i] = __uint_as_float(r0[i]);
-            v1[i] = __uint_as_float(r1[i]);
+          for (int i = 0; i < 16; ++i) {
+            v0[i] = __uint_as_float(ahead0[i]);
+            v1[i] = __uint_as_float(ahead1[i]);
+          }
+          if (b + 2 < blocks) {
+            tmem_ld16(sums + (b + 2) * kBlockCols, ahead0);
+            tmem_ld16(sums1 + (b + 2) * kBlockCols, ahead1);
           }
           return;
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v0[i] = v1[i] = 0.f;
+        for (int i = 0; i < 16; ++i) v0[i] = v1[i] = 0.f;
 #pragma unroll 1
         for (int c = c0; c <= c1; ++c) {
           if (chunk_at(bound(c) - start, chunks, cost) >= chunk_at(bound(c + 1) - start, chunks, cost))
             continue;
-          const float* q = part_of(c) + static_cast<size_t>(r) * kTileRows;
+          const float* q = part_of(c) + static_cast<size_t>(b) * kBlockCols * kTileRows;
+          float x0[16], x1[16];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            v0[i] += __ldcg(q + i * kTileRows);
-            if (second) v1[i] += __ldcg(q + tile_floats + i * kTileRows);
+          for (int i = 0; i < 16; ++i) {
+            x0[i] = __ldcg(q + i * kTileRows);
+            x1[i] = second ? __ldcg(q + tile_floats + i * kTileRows) : 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            v0[i] += x0[i];
+            v1[i] += x1[i];
           }
         }
       };
@@ -488,11 +547,10 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
       for (int b = side; b < blocks; b += 2) {
         const int row_data = row_next;
         row_next = lane_row(b + 2);
+        float v0[16], v1[16];
+        take(b, v0, v1);
         if (kGated) {
           const int n = min(kBlockCols, piece.rows - b * kBlockCols);
-          float v0[16], v1[16];
-          take(b * kBlockCols, v0, v1);
-          take(b * kBlockCols + 8, v0 + 8, v1 + 8);
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             const float g = fminf(v0[j], p.limit), u = fminf(fmaxf(v1[j], -p.limit), p.limit);
@@ -537,10 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
         } else {
           const int o0 = piece.row_tile * kOuts + at, o1 = o0 + kTileRows;
           const bool in0 = o0 < p.outs, in1 = o1 < p.outs;
-#pragma unroll 1
-          for (int r = 0; r < kBlockCols; r += 8) {
-            float v0[8], v1[8];
-            take(b * kBlockCols + r, v0, v1);
+          {
             if (a.wide) {
               // BF16, four outputs of a row a lane: pairs of rows as a word, and
               // two exchanges turn rows into outputs (half the time of stores
@@ -551,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
                 const float* v = t ? v1 : v0;
                 const int o = (t ? o1 : o0) - k;
 #pragma unroll
-                for (int j = 0; j < 8; j += 4) {
+                for (int j = 0; j < 16; j += 4) {
                   uint32_t w0 = pack_bf16x2(v[j], v[j + 1]), w1 = pack_bf16x2(v[j + 2], v[j + 3]);
                   // lane 2i: rows j and j + 2 of outputs 2i, 2i + 1; lane 2i + 1: the others
                   const uint32_t x0 = __shfl_xor_sync(0xffffffffu, w0, 1);
@@ -562,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
                   // lane 4i + k: row j + (k & 1) + (k & 2) of outputs 4i .. 4i + 3
                   const uint32_t y = __shfl_xor_sync(0xffffffffu, (k & 2) ? w0 : w1, 2);
                   const uint2 word = (k & 2) ? make_uint2(y, w1) : make_uint2(w0, y);
-                  const int d = __shfl_sync(0xffffffffu, row_data, r + j + k);
+                  const int d = __shfl_sync(0xffffffffu, row_data, j + k);
                   if (d >= 0 && o < p.outs)
                     *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + d * p.out_stride + o) = word;
                 }
@@ -575,13 +630,13 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
               };
               if (p.bf16) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  put(static_cast<__nv_bfloat16*>(p.out), __shfl_sync(0xffffffffu, row_data, r + j),
+                for (int j = 0; j < 16; ++j)
+                  put(static_cast<__nv_bfloat16*>(p.out), __shfl_sync(0xffffffffu, row_data, j),
                       __float2bfloat16_rn(v0[j]), __float2bfloat16_rn(v1[j]));
               } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  put(static_cast<float*>(p.out), __shfl_sync(0xffffffffu, row_data, r + j), v0[j], v1[j]);
+                for (int j = 0; j < 16; ++j)
+                  put(static_cast<float*>(p.out), __shfl_sync(0xffffffffu, row_data, j), v0[j], v1[j]);
               }
             }
           }
@@ -1075,7 +1130,7 @@ struct Shape {
 };
 Shape tile_shape(const GroupedProblem& p) {
   const long long rows = p.rows, each = p.experts;  // rows of a group on average
-  const int n_max = rows <= 8 * each ? 16 : rows <= 24 * each ? 32 : rows <= 96 * each ? 128 : kMaxN;
+  const int n_max = rows <= 8 * each ? 16 : rows <= 24 * each ? 32 : rows <= 64 * each ? kHalfN : kMaxN;
   int stages = kMaxStages;
   while (smem_bytes(n_max, stages, p.experts) > kMaxSmem) --stages;
   return {n_max, stages};
