@@ -5,11 +5,12 @@
 // that each takes.
 //
 // Only a beam's `cands` largest logits can be among the prompt's `cands` best,
-// so the first kernel keeps, of every part of a row, that many values and the
-// part's maximum and sum of exponentials: one read, the part in registers. The
-// second merges a prompt's parts. Within a beam the logits alone decide, so
-// nothing is rounded there; between beams the totals are compared in 64 bits
-// (the sums behind them are fp32 over 32 values and 64 bits beyond).
+// so a block keeps, of every part of a row, that many values and the part's
+// maximum and sum of exponentials, in one read. The parts of a prompt are dealt
+// out over a cluster of blocks, whose first one merges them out of the others'
+// shared memory. Within a beam the logits alone decide, so nothing is rounded
+// there; between beams the totals are compared in 64 bits (the sums behind them
+// are fp32 over a step's values of a thread and 64 bits beyond).
 // Which thread adds which value depends on the value's index alone, whatever
 // the row's alignment, so that beams with equal rows have equal totals and tie.
 #include "beam.cuh"
@@ -23,11 +24,45 @@
 namespace dsv4 {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kPer = 32;                  // values of a thread
-constexpr int kSpan = kThreads * kPer;    // of a part
-constexpr int kCap = 2048;                // candidates held
+// Many rows: 256 threads, four blocks an SM. Few prompts, whose clusters do not
+// fill the GPU: 512 threads, a block an SM, and more of a row on its way at once.
+template <bool kFew>
+constexpr int kThreads = kFew ? 512 : 256;
+template <bool kFew>
+constexpr int kBlocks = kFew ? 1 : 4;
+constexpr int kCap = 512;                 // candidates held
+// Candidates beyond the best are thinned out once there are this many more.
+constexpr int kThin = 48;
+constexpr int kMaxParts = 64;             // of a row
+constexpr int kJobs = 512;                // threads with candidates, between two looks
+constexpr int kMaxWarps = 16;
 using Key = unsigned long long;           // ordered value above inverted index; 0: nothing
+
+constexpr double kLn2 = 0.69314718055994530942;
+constexpr double kLog2eRest = 1.4426950408889634074 - static_cast<double>(kLog2e);
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+__constant__ double kReciprocal[12] = {0.0, 1.0, 1.0 / 2, 1.0 / 3, 1.0 / 4, 1.0 / 5,
+                                        1.0 / 6, 1.0 / 7, 1.0 / 8, 1.0 / 9, 1.0 / 10, 1.0 / 11};
+// 2^x for x <= 2 to 1e-13 of itself (0 below 2^-1000): Taylor's series around the
+// nearest whole number. One copy of it, since it is seldom run.
+__device__ __noinline__ double pow2(double x) {
+  if (!(x > -1000.0)) return x == x ? 0.0 : x;
+  const double n = rint(x), t = (x - n) * kLn2;
+  double r = 1.0;
+#pragma unroll
+  for (int k = 11; k > 0; --k) r = fma(r * t, kReciprocal[k], 1.0);
+  return r * __hiloint2double((1023 + static_cast<int>(n)) << 20, 0);
+}
+
+// Values of a thread in a step.
+template <bool kBf16, bool kFew>
+constexpr int kPer = kBf16 || kFew ? 32 : 16;
 
 __device__ __forceinline__ uint32_t ordered(float x) {
   const uint32_t u = __float_as_uint(x + 0.0f);  // -0 -> +0
@@ -44,153 +79,282 @@ __device__ __forceinline__ int key_index(Key k) {
   return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(k));
 }
 
-struct Part {
-  double z;  // sum of e^(x - m)
-  float m;   // maximum
-};
+// The next smaller value of a finite one (or of +inf).
+__device__ __forceinline__ float below(float x) {
+  const uint32_t u = ordered(x) - (x == 0.f ? 2 : 1);  // (-0 is not below 0)
+  return __uint_as_float((u & 0x80000000u) ? u & 0x7FFFFFFFu : ~u);
+}
 
-struct Work {
-  Part* part;  // [rows][parts]
-  Key* key;    // [rows][parts][cands], descending, 0 behind the last
+struct Part {
+  double z;  // sum of 2^(x log2 e - m)
+  float m;   // -inf: of nothing
 };
 
 struct BeamArgs {
   BeamProblem p;
-  int parts;
-  bool wide;  // 16-byte aligned rows
-  Work w;
+  int parts, steps;  // of a row; steps of a part
+  int blocks;        // of a prompt: part u of its beams * parts is block u % blocks's
+  bool wide;         // 16-byte aligned rows
 };
 
-template <bool kBf16>
-__global__ void __launch_bounds__(kThreads, 4) beam_parts_kernel(const BeamArgs a) {
-  __shared__ Key cand[kCap];
-  __shared__ float warp_m[kWarps], warp_t[kWarps];
-  __shared__ double warp_z[kWarps];
-  __shared__ Key best[kWarps];
-  __shared__ int held;
+template <bool kBf16, bool kFew>
+struct Values {
+  static constexpr int kN = kBf16 ? 8 : 4, kVecs = kPer<kBf16, kFew> / kN;  // values of 16 bytes
+  uint4 v[kVecs];
+  __device__ __forceinline__ float get(int k) const {
+    const uint4& r = v[k / kN];
+    const int i = k % kN, w = kBf16 ? i / 2 : i;
+    const uint32_t u = w == 0 ? r.x : w == 1 ? r.y : w == 2 ? r.z : r.w;
+    if (!kBf16) return __uint_as_float(u);
+    return __uint_as_float((i & 1) ? u & 0xFFFF0000u : u << 16);
+  }
+  // value k of the step at i0: index i0 + (k / kN * kThreads + tid) * kN + k % kN
+  static __device__ __forceinline__ int index(int i0, int k) {
+    return i0 + ((k / kN) * kThreads<kFew> + static_cast<int>(threadIdx.x)) * kN + k % kN;
+  }
+  __device__ __forceinline__ void load(const void* row, int i0, int vocab, bool wide) {
+    if (wide && i0 + kThreads<kFew> * kPer<kBf16, kFew> <= vocab) {
+      const char* q = static_cast<const char*>(row) + static_cast<size_t>(index(i0, 0)) * (kBf16 ? 2 : 4);
+#pragma unroll
+      for (int u = 0; u < kVecs; ++u)
+        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v[u].x), "=r"(v[u].y), "=r"(v[u].z), "=r"(v[u].w)
+                     : "l"(q + u * kThreads<kFew> * 16));
+      return;
+    }
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      const int i = index(i0, u * kN);
+      const uint32_t none = kBf16 ? 0xFF80FF80u : 0xFF800000u;  // -inf
+      v[u] = make_uint4(none, none, none, none);
+      if (wide && i + kN <= vocab) {
+        const void* q = static_cast<const char*>(row) + static_cast<size_t>(i) * (kBf16 ? 2 : 4);
+        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v[u].x), "=r"(v[u].y), "=r"(v[u].z), "=r"(v[u].w) : "l"(q));
+      } else if (i < vocab) {
+        uint32_t w[4] = {none, none, none, none};
+#pragma unroll
+        for (int k = 0; k < kN; ++k)
+          if (i + k < vocab) {
+            if (!kBf16) {
+              w[k & 3] = static_cast<const uint32_t*>(row)[i + k];
+            } else {
+              const uint32_t h = static_cast<const uint16_t*>(row)[i + k];
+              w[k / 2] = (k & 1) ? (w[k / 2] & 0xFFFFu) | (h << 16) : (w[k / 2] & 0xFFFF0000u) | h;
+            }
+          }
+        v[u] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+};
+
+struct Held {
+  Key cand[2][kCap];
+  Key best[kMaxWarps];
+  double z[kMaxWarps];
+  float m[kMaxWarps], t[kMaxWarps];
+  uint32_t job[kJobs];         // step and thread
+  int n, jobs;
+};
+
+// The best `keep` of cand[from][0 .. n), descending, to the other list; a key's
+// place is the number of larger ones (keys differ). Whole block; n is the same
+// for all.
+__device__ __forceinline__ void thin(Held& h, int from, int n, int keep) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const Key k = h.cand[from][i];
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) rank += h.cand[from][j] > k;
+    if (rank < keep) h.cand[from ^ 1][rank] = k;
+  }
+  if (threadIdx.x == 0) h.n = min(n, keep);
+  __syncthreads();
+}
+
+// Part `part` of row `row`: its best `cands` values, descending (0 behind the
+// last), its maximum and sum. Whole block.
+template <bool kBf16, bool kFew>
+__device__ __forceinline__ void take_part(Held& h, const BeamArgs& a, long long row, int part,
+                                          Part* out, Key* keys) {
+  constexpr int kEach = kPer<kBf16, kFew>, kTids = kThreads<kFew>, kSpan = kTids * kEach;
+  constexpr int kWarps = kTids / 32, kTidBits = kFew ? 9 : 8;
   const BeamProblem& p = a.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
-  constexpr int kN = kBf16 ? 8 : 4, kVecs = kPer / kN;  // values of 16 bytes
-  const long long at = row * p.stride;
-  const int i0 = part * kSpan;
-  pdl_wait();
-  pdl_trigger();
-  if (tid == 0) held = 0;
-  // value k of vector u: index i0 + (u * kThreads + tid) * kN + k
-  float v[kPer];
+  const void* x = static_cast<const char*>(p.logits) + row * p.stride * (kBf16 ? 2 : 4);
+  int i0 = part * a.steps * kSpan;
+  const int i1 = min(p.vocab, i0 + a.steps * kSpan);
+  Values<kBf16, kFew> next;
+  next.load(x, i0, i1, a.wide);
+  __syncthreads();  // the part before has been written down
+  if (tid == 0) h.n = h.jobs = 0;
+  // The sum is of 2^(v log2 e - c), c = ref log2 e: ref is a maximum of some
+  // values of this thread, moved when one exceeds it by more than 8 (some thread
+  // of a warp has a new maximum at every step).
+  float ref = -INFINITY, c = 0.f;
+  float above = -INFINITY;  // candidates exceed it; -inf never is one
+  double z = 0.0;
+  const int part_i0 = i0;
+  int list = 0, kept = 0, w0 = i0, step = 0;
+  for (; i0 < i1; i0 += kSpan, ++step) {
+    float v[kEach];
 #pragma unroll
-  for (int u = 0; u < kVecs; ++u) {
-    const int i = i0 + (u * kThreads + tid) * kN;
-    if (a.wide && i + kN <= p.vocab) {
-      uint4 r;
-      const void* q = kBf16 ? static_cast<const void*>(static_cast<const uint16_t*>(p.logits) + at + i)
-                            : static_cast<const void*>(static_cast<const float*>(p.logits) + at + i);
-      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(q));
-      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    for (int k = 0; k < kEach; ++k) v[k] = next.get(k);
+    if (i0 + kSpan < i1) next.load(x, i0 + kSpan, i1, a.wide);
+    float top = fmaxf(v[0], -INFINITY);  // (stays so where every value is NaN)
 #pragma unroll
-      for (int k = 0; k < kN; ++k)
-        v[u * kN + k] = !kBf16 ? __uint_as_float(w[k & 3])
-                               : __uint_as_float((k & 1) ? w[k >> 1] & 0xFFFF0000u : w[k >> 1] << 16);
-    } else {
-#pragma unroll
-      for (int k = 0; k < kN; ++k)
-        v[u * kN + k] = i + k >= p.vocab ? -INFINITY
-                        : kBf16 ? bf16_widen(static_cast<const uint16_t*>(p.logits)[at + i + k])
-                                : static_cast<const float*>(p.logits)[at + i + k];
+    for (int k = 1; k + 1 < kEach; k += 2) top = max3(top, v[k], v[k + 1]);
+    top = fmaxf(top, v[kEach - 1]);
+    if (top > ref + 8.f) {
+      const float to = top * kLog2e;
+      if (ref != -INFINITY) z *= pow2(static_cast<double>(c) - static_cast<double>(to));
+      ref = top;
+      c = to;
     }
-  }
-  float mine = v[0];
+    float z0 = 0.f, z1 = 0.f;
 #pragma unroll
-  for (int k = 1; k < kPer; ++k) mine = fmaxf(mine, v[k]);
-  mine = fmaxf(mine, -INFINITY);  // NaN where every value is one
-  // Every warp has `each` threads whose largest value reaches the each-th
-  // largest of them, so each * kWarps >= cands values reach the smallest of
-  // these.
-  float top = warp_max(mine), kth = top, left = mine;
-  for (int each = kWarps; each < p.cands; each += kWarps) {
-    const unsigned who = __ballot_sync(0xffffffffu, left == kth);
-    if (lane == __ffs(who) - 1) left = -INFINITY;
-    kth = warp_max(left);
-  }
-  if (lane == 0) {
-    warp_m[warp] = top;
-    warp_t[warp] = kth;
-  }
-  __syncthreads();
-  float m = warp_m[0], limit = warp_t[0];
+    for (int k = 0; k < kEach; k += 2) {
+      z0 += ex2_approx(fmaf(v[k], kLog2e, -c));
+      z1 += ex2_approx(fmaf(v[k + 1], kLog2e, -c));
+    }
+    z += z0 + z1;
+    if (step == 0) {
+      // Every warp has `each` threads whose largest value reaches the each-th
+      // largest of them, so each * kWarps >= cands values reach the smallest
+      // of these.
+      float kth = warp_max(top), left = top;
+      for (int each = kWarps; each < p.cands; each += kWarps) {
+        const unsigned who = __ballot_sync(0xffffffffu, left == kth);
+        if (lane == __ffs(who) - 1) left = -INFINITY;
+        kth = warp_max(left);
+      }
+      if (lane == 0) h.t[warp] = kth;
+      __syncthreads();
+      float limit = h.t[0];
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) {
-    m = fmaxf(m, warp_m[w]);
-    limit = fminf(limit, warp_t[w]);
-  }
-  const float ref = m == -INFINITY ? 0.f : m;
-  float each_z = 0.f;
+      for (int w = 1; w < kWarps; ++w) limit = fminf(limit, h.t[w]);
+      above = limit > -INFINITY ? below(limit) : limit;
+    }
+    // A thread with a candidate only says so: what runs seldom costs more in
+    // instruction fetches than it does (a loop over the values here took 1,000
+    // clocks each time that one was found).
+    if (top > above) {
+      const int at = atomicAdd(&h.jobs, 1);
+      if (at < kJobs) h.job[at] = static_cast<uint32_t>(step) << kTidBits | tid;
+    }
+    // looked at after one step, two, four, and every fourth from there (of two
+    // steps both at once)
+    if (i0 + kSpan < i1 && i0 + 2 * kSpan >= i1 && step == 0) continue;
+    if ((step & (step < 4 ? step + 1 : 3)) != (step < 4 ? 0 : 3) && i0 + kSpan < i1) continue;
+    __syncthreads();
+    const int jobs = h.jobs;
+    if (jobs <= kJobs) {
+      // a warp a thread's values of a step, read again, four threads' at a time
+      constexpr int kN = Values<kBf16, kFew>::kN, kAtOnce = 4;
+      const int in_step = (lane / kN) * kTids * kN + lane % kN;
+#pragma unroll 1
+      for (int j = warp; j < jobs; j += kAtOnce * kWarps) {
+        float y[kAtOnce];
+        int i[kAtOnce];
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) each_z += ex2_approx((v[k] - ref) * kLog2e);
-  double z = each_z;
+        for (int q = 0; q < kAtOnce; ++q) {
+          const uint32_t job = j + q * kWarps < jobs ? h.job[j + q * kWarps] : 0;
+          i[q] = part_i0 + static_cast<int>(job >> kTidBits) * kSpan + in_step +
+                 static_cast<int>(job & (kTids - 1)) * kN;
+          y[q] = -INFINITY;
+          if (j + q * kWarps < jobs && lane < kEach && i[q] < i1)
+            y[q] = kBf16 ? bf16_widen(static_cast<const uint16_t*>(x)[i[q]])
+                         : static_cast<const float*>(x)[i[q]];
+        }
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q)
+          if (y[q] > above) {
+            const int at = atomicAdd(&h.n, 1);
+            if (at < kCap) h.cand[list][at] = make_key(y[q], i[q]);
+          }
+      }
+    }
+    __syncthreads();
+    const int n = jobs <= kJobs ? h.n : kCap + 1;
+    __syncthreads();  // nobody adds to either before all have read them
+    if (tid == 0) h.jobs = 0;
+    if (n > kCap) {
+      // more values exceed the limit than fit (equal ones, or ascending): the
+      // block's best, one after the other, of the values since the last look,
+      // read again, and those kept
+      Key before = ~0ull;
+#pragma unroll 1
+      for (int r = 0; r < p.cands; ++r) {
+        Key k = tid < kept ? h.cand[list][tid] : 0;
+        if (k >= before) k = 0;
+#pragma unroll 1
+        for (int i = w0 + tid; i < min(i1, i0 + kSpan); i += kTids) {
+          const float y = kBf16 ? bf16_widen(static_cast<const uint16_t*>(x)[i])
+                                : static_cast<const float*>(x)[i];
+          const Key q = y > -INFINITY ? make_key(y, i) : 0;
+          if (q < before && q > k) k = q;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          const Key q = __shfl_xor_sync(0xffffffffu, k, o);
+          k = q > k ? q : k;
+        }
+        if (lane == 0) h.best[warp] = k;
+        __syncthreads();
+        k = h.best[0];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) k = h.best[w] > k ? h.best[w] : k;
+        if (tid == 0) h.cand[list ^ 1][r] = k;
+        before = k;
+        __syncthreads();
+      }
+      list ^= 1;
+      kept = p.cands;  // (at least so many: n > kCap)
+      if (tid == 0) h.n = kept;
+      above = key_value(h.cand[list][p.cands - 1]);
+      __syncthreads();
+    } else if (n > p.cands + (step == 0 ? 0 : kThin)) {  // (the first limit is loose)
+      thin(h, list, n, p.cands);
+      list ^= 1;
+      kept = p.cands;
+      above = key_value(h.cand[list][p.cands - 1]);
+    } else {
+      kept = n;
+      __syncthreads();  // jobs
+    }
+    w0 = i0 + kSpan;
+  }
+  thin(h, list, kept, p.cands);  // sorted
+  list ^= 1;
+  // the block's sum, relative to the largest c; a thread whose ref is not the
+  // row's maximum is corrected for log2 e's rounding by its own (the rest of it is
+  // below 2^-25 of the distance between them)
+  if (ref != -INFINITY) z *= pow2(static_cast<double>(ref) * kLog2eRest);  // (NaN stays)
+  const float mine = ref != -INFINITY ? c : -INFINITY, top = warp_max(mine);
+  if (mine != -INFINITY) z *= pow2(static_cast<double>(c) - static_cast<double>(top));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-  if (lane == 0) warp_z[warp] = z;
-  if (mine >= limit) {
-#pragma unroll
-    for (int k = 0; k < kPer; ++k)
-      if (v[k] >= limit && v[k] > -INFINITY) {
-        const int n = atomicAdd(&held, 1);
-        if (n < kCap)
-          cand[n] = make_key(v[k], i0 + ((k / kN) * kThreads + tid) * kN + k % kN);
-      }
+  if (lane == 0) {
+    h.m[warp] = top;
+    h.z[warp] = z;
   }
   __syncthreads();
-  const int n = held;
-  Key* out = a.w.key + static_cast<long long>(blockIdx.x) * p.cands;
-  if (tid == 0) {
-    double sum = 0.0;
+  if (warp == 0) {
+    const bool in = lane < kWarps;
+    const float one = in ? h.m[lane] : -INFINITY, all = warp_max(one);
+    z = in ? h.z[lane] : 0.0;
+    if (one != -INFINITY) z *= pow2(static_cast<double>(one) - static_cast<double>(all));
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) sum += warp_z[w];
-    a.w.part[blockIdx.x] = {sum, m};
-  }
-  if (n <= kCap) {
-    // a key's place is the number of larger ones (keys differ)
-    for (int i = tid; i < n; i += kThreads) {
-      const Key k = cand[i];
-      int rank = 0;
-      for (int j = 0; j < n && rank < p.cands; ++j) rank += cand[j] > k;
-      if (rank < p.cands) out[rank] = k;
-    }
-    for (int i = n + tid; i < p.cands; i += kThreads) out[i] = 0;
-    return;
-  }
-  // More values reach the limit than fit (a row of equal values): one of the
-  // block's best after the other.
-  Key before = ~0ull;
-  for (int r = 0; r < p.cands; ++r) {
-    Key k = 0;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const Key q = v[j] > -INFINITY
-                        ? make_key(v[j], i0 + ((j / kN) * kThreads + tid) * kN + j % kN) : 0;
-      if (q < before && q > k) k = q;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const Key q = __shfl_xor_sync(0xffffffffu, k, o);
-      k = q > k ? q : k;
-    }
-    if (lane == 0) best[warp] = k;
-    __syncthreads();
-    k = best[0];
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) k = best[w] > k ? best[w] : k;
-    if (tid == 0) out[r] = k;
-    before = k;
-    __syncthreads();
+    for (int o = kWarps / 2; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    if (lane == 0) *out = {z, all};
+    if (lane < p.cands) keys[lane] = lane < h.n ? h.cand[list][lane] : 0;
   }
 }
 
 // A candidate of the second kernel: what it is compared by, larger first, then
-// its place among the prompt's continuations, smaller first. place < 0: none.
+// its place (beam, then token), smaller first. place < 0: none.
 struct Cand {
   double total;
   long long place;
@@ -232,48 +396,110 @@ __device__ __forceinline__ int nth_bit(unsigned mask, int n) {
   return mask ? __ffs(mask) - 1 : 32;
 }
 
-__global__ void __launch_bounds__(kThreads) beam_group_kernel(const BeamArgs a) {
-  __shared__ Cand list[kWarps][32];
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// 8 bytes of block `rank`'s shared memory, at the place that q has here.
+__device__ __forceinline__ unsigned long long ld_block(const void* q, int rank) {
+  uint32_t at;
+  unsigned long long v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(q)), "r"(rank));
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
+  return v;
+}
+
+struct Merge {
+  Cand list[kMaxWarps][32];
+  double moved[kMaxBeams];
+};
+
+// One prompt's parts: the block that merges them.
+template <bool kFew>
+__device__ __forceinline__ void merge_group(Merge& sh, const BeamArgs& a, int g, const Part* part,
+                                            const Key* keys) {
+  constexpr int kWarps = kThreads<kFew> / 32;
   const BeamProblem& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = blockIdx.x;
-  pdl_wait();
-  pdl_trigger();
-  Cand mine = {0.0, -1};
+  auto key_of = [&](int u) { return ld_block(keys + (u / a.blocks) * p.cands + lane, u % a.blocks); };
+  auto part_of = [&](int u) {
+    const Part* q = part + u / a.blocks;
+    const int rank = u % a.blocks;
+    return Part{__longlong_as_double(ld_block(&q->z, rank)),
+                __uint_as_float(static_cast<uint32_t>(ld_block(&q->m, rank)))};
+  };
+  // Eight parts of a row at a time: their lists are asked for together and
+  // merged by pairs, the first ones while the rows' sums are on their way.
+  constexpr int kTake = 8;
+  const int takes = (a.parts + kTake - 1) / kTake, units = p.beams * takes;
+  Key k[kTake];
+  auto load_keys = [&](int u) {
+    const int b = u / takes, first = (u - b * takes) * kTake;
+#pragma unroll
+    for (int i = 0; i < kTake; ++i)
+      k[i] = first + i < a.parts && lane < p.cands ? key_of(b * a.parts + first + i) : 0;
+  };
+  auto best_key = [&](int u) {
+    const int first = (u % takes) * kTake;
+#pragma unroll
+    for (int w = 1; w < kTake; w *= 2)
+#pragma unroll
+      for (int i = 0; i < kTake; i += 2 * w)
+        if (first + i + w < a.parts) k[i] = best_of(k[i], k[i + w]);
+  };
+  if (warp < units) load_keys(warp);
+  // what a row's values are moved by: its score less its log sum
   for (int b = warp; b < p.beams; b += kWarps) {
     const long long row = static_cast<long long>(g) * p.beams + b;
-    const Part* part = a.w.part + row * a.parts;
-    const Key* key = a.w.key + row * a.parts * p.cands;
+    const double score = p.score[row];
+    Part q[kMaxParts / 32];
     float m = -INFINITY;
-    for (int i = lane; i < a.parts; i += 32) m = fmaxf(m, part[i].m);
+#pragma unroll
+    for (int i = 0; i < kMaxParts / 32; ++i) {
+      q[i] = i * 32 + lane < a.parts ? part_of(b * a.parts + i * 32 + lane) : Part{0.0, -INFINITY};
+      m = fmaxf(m, q[i].m);
+    }
     m = warp_max(m);
     double z = 0.0;
-    for (int i = lane; i < a.parts; i += 32) {
-      const Part q = part[i];
-      // (NaN stays; a part of nothing has z 0)
-      z += q.m == -INFINITY ? q.z : q.z * exp(static_cast<double>(q.m) - m);
-    }
+#pragma unroll
+    for (int i = 0; i < kMaxParts / 32; ++i)  // (NaN stays; a part of nothing has z 0)
+      if (i * 32 < a.parts) z += q[i].m == -INFINITY ? q[i].z : q[i].z * pow2(static_cast<double>(q[i].m) - m);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-    Key k = lane < p.cands ? key[lane] : 0;
-    for (int i = 1; i < a.parts; ++i)
-      k = best_of(k, lane < p.cands ? key[static_cast<long long>(i) * p.cands + lane] : 0);
-    const double off = static_cast<double>(p.score[row]) - (m + log(z));
-    Cand c = {0.0, -1};
-    if (k) {
-      c.total = key_value(k) + off;
-      // a dead beam, or a row with a NaN or +inf, has no candidates
-      if (fabs(c.total) <= 1.7e308) c.place = static_cast<long long>(b) * p.vocab + key_index(k);
-    }
-    mine = best_of(mine, c);
+    if (lane == 0) sh.moved[b] = score - (m + log2(z)) * kLn2;
   }
-  list[warp][lane] = mine;
+  if (warp < units) best_key(warp);
   __syncthreads();
+  Cand mine = {0.0, -1};
+  for (int u = warp; u < units; u += kWarps) {
+    if (u != warp) {
+      load_keys(u);
+      best_key(u);
+    }
+    const int b = u / takes;
+    Cand c = {0.0, -1};
+    if (k[0]) {
+      c.total = key_value(k[0]) + sh.moved[b];
+      // a dead beam, or a row with a NaN or +inf, has no candidates
+      if (fabs(c.total) <= 1.7e308) c.place = static_cast<long long>(b) << 32 | key_index(k[0]);
+    }
+    mine = u == warp ? c : best_of(mine, c);
+  }
+  sh.list[warp][lane] = mine;
+  const int used = min(kWarps, units);
+  for (int s = 1; s < used; s <<= 1) {
+    __syncthreads();
+    if ((warp & (2 * s - 1)) == 0 && warp + s < used) {
+      mine = best_of(mine, sh.list[warp + s][lane]);
+      sh.list[warp][lane] = mine;
+    }
+  }
   if (warp != 0) return;
-  for (int w = 1; w < min(kWarps, p.beams); ++w) mine = best_of(mine, list[w][lane]);
   const bool live = lane < p.cands && mine.place >= 0;
-  const int parent = live ? static_cast<int>(mine.place / p.vocab) : -1;
-  const int token = live ? static_cast<int>(mine.place - static_cast<long long>(parent) * p.vocab) : -1;
+  const int parent = live ? static_cast<int>(mine.place >> 32) : -1;
+  const int token = live ? static_cast<int>(mine.place) : -1;
   if (lane < p.cands) {
     const long long at = static_cast<long long>(g) * p.cands + lane;
     p.parent[at] = parent;
@@ -303,30 +529,104 @@ __global__ void __launch_bounds__(kThreads) beam_group_kernel(const BeamArgs a) 
   p.src[at] = mother >= 0 ? p.slot[row + mother] : -1;
 }
 
-int parts_of(const BeamProblem& p) { return (p.vocab + kSpan - 1) / kSpan; }
+constexpr int kMaxBlocks = 16;  // of a cluster
+
+__host__ __device__ inline int slots_of(int beams, int parts, int blocks) {
+  return (beams * parts + blocks - 1) / blocks;
+}
+
+template <bool kBf16, bool kFew>
+__global__ void __launch_bounds__(kThreads<kFew>, kBlocks<kFew>) beam_kernel(const BeamArgs a) {
+  extern __shared__ __align__(16) uint8_t smem[];  // this block's parts, then their keys
+  __shared__ union {
+    Held held;
+    Merge merge;
+  } sh;
+  const int slots = slots_of(a.p.beams, a.parts, a.blocks), units = a.p.beams * a.parts;
+  Part* part = reinterpret_cast<Part*>(smem);
+  Key* keys = reinterpret_cast<Key*>(part + slots);
+  const int g = blockIdx.x / a.blocks, rank = blockIdx.x - g * a.blocks;
+  pdl_wait();
+  pdl_trigger();
+  for (int u = rank, slot = 0; u < units; u += a.blocks, ++slot) {
+    const int b = u / a.parts;
+    take_part<kBf16, kFew>(sh.held, a, static_cast<long long>(g) * a.p.beams + b, u - b * a.parts, part + slot,
+                     keys + slot * a.p.cands);
+  }
+  cluster_arrive();
+  cluster_wait();
+  if (rank == 0) merge_group<kFew>(sh.merge, a, g, part, keys);
+  __syncwarp();
+  cluster_arrive();  // until then the others' shared memory is read
+  cluster_wait();
+}
+
+// How rows are cut and over how many blocks a prompt's parts are dealt out: what
+// the slowest place of the GPU takes in steps, a part's start, choice and end
+// counted as three, and the merge of eight parts as one.
+void deal(const BeamProblem& p, int span, int places, BeamArgs* a) {
+  const int steps = (p.vocab - 1) / span + 1;
+  const int most = steps < kMaxParts ? steps : kMaxParts;
+  double least = 0.0;
+  a->parts = 0;
+  for (int n = 1; n <= most; ++n) {
+    const int each = (steps + n - 1) / n;
+    if (n > 1 && (steps + n - 2) / (n - 1) == each) continue;  // no shorter
+    for (int blocks = 1; blocks <= kMaxBlocks && blocks < 2 * p.beams * n; blocks *= 2) {
+      const double waves = static_cast<double>((static_cast<long long>(p.groups) * blocks + places - 1) / places);
+      const double cost = waves * slots_of(p.beams, n, blocks) * (each + 3) + p.beams * n / 64 + n / 8;
+      if (a->parts == 0 || cost < least) {
+        least = cost;
+        a->parts = n;
+        a->steps = each;
+        a->blocks = blocks;
+      }
+    }
+  }
+}
 
 }  // namespace
 
-size_t beam_workspace_bytes(const BeamProblem& p) {
-  const size_t parts = static_cast<size_t>(p.groups) * p.beams * parts_of(p);
-  return parts * (sizeof(Part) + sizeof(Key) * p.cands);
-}
-
-cudaError_t beam_select(const BeamProblem& p, void* ws, cudaStream_t st) {
+cudaError_t beam_select(const BeamProblem& p, cudaStream_t st) {
   if (p.groups <= 0) return cudaSuccess;
   BeamArgs a;
   a.p = p;
-  a.parts = parts_of(p);
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return e;
+  const bool few = p.groups * static_cast<long long>(kMaxBlocks) <= sms;
+  if (few)
+    deal(p, kThreads<true> * (p.bf16 ? kPer<true, true> : kPer<false, true>), kBlocks<true> * sms, &a);
+  else
+    deal(p, kThreads<false> * (p.bf16 ? kPer<true, false> : kPer<false, false>), kBlocks<false> * sms, &a);
   const int size = p.bf16 ? 2 : 4;
   a.wide = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.stride * size % 16 == 0;
-  const long long blocks = static_cast<long long>(p.groups) * p.beams * a.parts;
-  if (blocks > 0x7FFFFFFFll) return cudaErrorInvalidValue;
-  a.w.key = static_cast<Key*>(ws);
-  a.w.part = reinterpret_cast<Part*>(a.w.key + blocks * p.cands);
-  cudaError_t e = launch_pdl(p.bf16 ? beam_parts_kernel<true> : beam_parts_kernel<false>,
-                             dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, a);
+  if (static_cast<long long>(p.groups) * a.blocks > 0x7FFFFFFFll) return cudaErrorInvalidValue;
+  auto kernel = few ? (p.bf16 ? beam_kernel<true, true> : beam_kernel<false, true>)
+                    : (p.bf16 ? beam_kernel<true, false> : beam_kernel<false, false>);
+  const void* fn = reinterpret_cast<const void*>(kernel);
+  const int bytes = slots_of(p.beams, a.parts, a.blocks) *
+                    static_cast<int>(sizeof(Part) + sizeof(Key) * p.cands);
+  prefer_max_shared(fn);
+  e = set_max_dynamic_smem(fn, 160 * 1024);
+  if (e == cudaSuccess && bytes > 160 * 1024) e = cudaErrorInvalidValue;
+  if (e == cudaSuccess && a.blocks > 8)  // more than every device has to take
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;
-  return launch_pdl(beam_group_kernel, dim3(p.groups), dim3(kThreads), 0, st, a);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.groups * a.blocks));
+  cfg.blockDim = dim3(few ? kThreads<true> : kThreads<false>);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {static_cast<unsigned>(a.blocks), 1, 1};
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
 }  // namespace dsv4

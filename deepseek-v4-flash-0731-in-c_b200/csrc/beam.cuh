@@ -1,7 +1,6 @@
 // beam.cuh - selection of beams over their continuations, and the slots that
 // the chosen ones take.
 #pragma once
-#include <cstddef>
 #include <cuda_runtime.h>
 
 namespace dsv4 {
@@ -26,7 +25,6 @@ struct BeamProblem {
   int* src = nullptr;
 };
 
-size_t beam_workspace_bytes(const BeamProblem& p);
-cudaError_t beam_select(const BeamProblem& p, void* ws, cudaStream_t st);
+cudaError_t beam_select(const BeamProblem& p, cudaStream_t st);
 
 }  // namespace dsv4

@@ -2077,7 +2077,7 @@ bool beam_problem(const char* who, const dsv4cuda_beam_shape* s, dsv4::BeamProbl
   static_assert(DSV4CUDA_MAX_BEAMS == dsv4::kMaxBeams, "limit");
   static_assert(DSV4CUDA_MAX_BEAM_CANDIDATES == dsv4::kMaxBeamCandidates, "limit");
   if (!s || s->n_groups < 0 || s->beams < 1 || s->beams > dsv4::kMaxBeams || s->n_cands < 1 ||
-      s->n_cands > dsv4::kMaxBeamCandidates || s->vocab < 1 || (s->stride && s->stride < s->vocab) ||
+      s->n_cands > dsv4::kMaxBeamCandidates || s->vocab < 1 || s->vocab > 0x3FFFFFFF || (s->stride && s->stride < s->vocab) ||
       static_cast<long long>(s->n_groups) * s->beams > 0x7FFFFFFFll) {
     record_error("%s: bad shape (1..%d beams and candidates, stride at least vocab)", who,
                  dsv4::kMaxBeams);
@@ -2094,16 +2094,9 @@ bool beam_problem(const char* who, const dsv4cuda_beam_shape* s, dsv4::BeamProbl
 }
 }  // namespace
 
-DSV4_API size_t dsv4cuda_beam_workspace_bytes(const dsv4cuda_beam_shape* shape) {
-  dsv4::BeamProblem p;
-  if (!beam_problem("dsv4cuda_beam_workspace_bytes", shape, &p)) return 0;
-  return dsv4::beam_workspace_bytes(p);
-}
-
 DSV4_API int dsv4cuda_beam_select(const void* logits, const float* score, int* parent, int* token,
                                   float* total, int* next, const int* slot, int* dst, int* src,
-                                  const dsv4cuda_beam_shape* shape, void* workspace,
-                                  size_t workspace_bytes, void* stream) {
+                                  const dsv4cuda_beam_shape* shape, void* stream) {
   const char* who = "dsv4cuda_beam_select";
   dsv4::BeamProblem p;
   if (!beam_problem(who, shape, &p)) return -1;
@@ -2122,10 +2115,7 @@ DSV4_API int dsv4cuda_beam_select(const void* logits, const float* score, int* p
   p.slot = slot;
   p.dst = dst;
   p.src = src;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  void* ws = pick_workspace(who, workspace, workspace_bytes, dsv4::beam_workspace_bytes(p), st);
-  if (!ws) return -1;
-  cudaError_t e = dsv4::beam_select(p, ws, st);
+  cudaError_t e = dsv4::beam_select(p, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) { record_error("%s: %s", who, cudaGetErrorString(e)); return -1; }
   return 0;
 }

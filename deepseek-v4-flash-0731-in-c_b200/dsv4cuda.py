@@ -12,6 +12,7 @@ raises.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 
 import numpy as np
@@ -668,7 +669,7 @@ def _dev(t, name, dtype, numel=None):
     """The address of a contiguous CUDA tensor of `dtype` (None passes as NULL)."""
     if t is None:
         return None
-    if t.dtype is not dtype or not t.is_cuda or not t.is_contiguous():
+    if not (t.dtype is dtype and t.is_cuda and t.is_contiguous()):
         raise ValueError(f"{name}: a contiguous CUDA tensor of {dtype} is wanted, got {t.dtype} "
                          f"on {t.device}")
     if numel is not None and t.numel() < numel:
@@ -676,18 +677,32 @@ def _dev(t, name, dtype, numel=None):
     return t.data_ptr()
 
 
-def _row_tensor(t, name, width, like=None):
-    """(1 for BF16 or 0 for fp32, elements between rows or 0) of CUDA rows [n][width]."""
-    import torch
-    if (t.dtype not in (torch.bfloat16, torch.float32) or t.dim() != 2 or t.shape[1] != width
-            or not t.is_cuda or (width > 1 and t.stride(1) != 1)):
-        raise ValueError(f"{name}: a CUDA tensor [rows][{width}] of bfloat16 or float32, the values of "
-                         f"a row one behind the other")
-    if like is not None and (t.dtype is not like.dtype or t.shape[0] != like.shape[0]):
-        raise ValueError(f"{name}: {like.shape[0]} rows of {like.dtype} are wanted")
-    if t.shape[0] > 1 and t.stride(0) < width:
+def _rows_of(t, name, shape, dtype):
+    """Elements between the rows (0: of one row, or of none between them) of a CUDA tensor
+    [rows][width] of `shape` and `dtype`."""
+    if t.dtype is not dtype or t.shape != shape or not t.is_cuda:
+        raise ValueError(f"{name}: a CUDA tensor {list(shape)} of {dtype} is wanted, got {t.dtype} "
+                         f"{list(t.shape)} on {t.device}")
+    n, width = shape
+    stride, inner = t.stride()
+    if width > 1 and inner != 1:
+        raise ValueError(f"{name}: the values of a row must lie one behind the other")
+    if n <= 1:
+        return 0
+    if stride < width:
         raise ValueError(f"{name}: the rows must not overlap")
-    return int(t.dtype is torch.bfloat16), t.stride(0) if t.shape[0] > 1 else 0
+    return stride
+
+
+def _float_rows(t, name, width=None):
+    """(dtype, 1 for BF16 or 0 for fp32, shape) of rows [n][width]."""
+    import torch
+    dtype, shape = t.dtype, t.shape
+    bf16 = dtype is torch.bfloat16
+    if not (bf16 or dtype is torch.float32) or len(shape) != 2 or width not in (None, shape[1]):
+        raise ValueError(f"{name}: a CUDA tensor [rows][{width or 'width'}] of bfloat16 or float32 is "
+                         f"wanted, got {dtype} {list(shape)}")
+    return dtype, 1 if bf16 else 0, shape
 
 
 class PagedCache:
@@ -755,8 +770,8 @@ class PagedCache:
             raise ValueError(f"layer {layer} of {len(self.caches)}")
         c = self.caches[layer].struct
         d = c.nope + c.rope_dim
-        bf16, stride = _row_tensor(kv, "kv", d)
-        n = kv.shape[0]
+        dtype, bf16, shape = _float_rows(kv, "kv", d)
+        stride, n = _rows_of(kv, "kv", shape, dtype), shape[0]
         half = n * (c.rope_dim // 2)
         _check(lib.dsv4cuda_paged_write(
             self._ref, layer, kv.data_ptr(), bf16, stride, _dev(rows, "rows", self._i64, n), n,
@@ -855,10 +870,13 @@ lib.dsv4cuda_norm_quant.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp]
 lib.dsv4cuda_paged_write.restype = C.c_int
 lib.dsv4cuda_paged_write.argtypes = [vp, C.c_int, vp, C.c_int, C.c_longlong, vp, C.c_int, vp, C.c_float,
                                      vp, vp, vp]
-lib.dsv4cuda_beam_workspace_bytes.restype = C.c_size_t
-lib.dsv4cuda_beam_workspace_bytes.argtypes = [vp]
 lib.dsv4cuda_beam_select.restype = C.c_int
-lib.dsv4cuda_beam_select.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]
+lib.dsv4cuda_beam_select.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_shape(*fields):
+    return C.byref(NormShape(*fields))  # (1 us a call)
 
 
 def norm_quant(x, gain, codes, scales, eps=1e-6, residual=None, sum_out=None, out=None, stream=None):
@@ -868,43 +886,39 @@ def norm_quant(x, gain, codes, scales, eps=1e-6, residual=None, sum_out=None, ou
     them. sum_out (may be x or residual) receives x + residual, out the normalised rows; both
     of x's type."""
     import torch
-    if x.dim() != 2:
-        raise ValueError("x: [rows][width] is wanted")
-    n, width = x.shape
-    bf16, xs = _row_tensor(x, "x", width)
-    strides = [xs]
-    for t, name in ((residual, "residual"), (sum_out, "sum_out"), (out, "out")):
-        strides.append(0 if t is None else _row_tensor(t, name, width, like=x)[1])
-    shape = NormShape(n, width, bf16, eps, *strides)
+    dtype, bf16, size = _float_rows(x, "x")
+    n, width = size
+    u8, q = torch.uint8, _rows_of(x, "x", size, dtype)
+    r = s = o = 0
+    at_r = at_s = at_o = None
+    if residual is not None:
+        r, at_r = _rows_of(residual, "residual", size, dtype), residual.data_ptr()
+    if sum_out is not None:
+        s, at_s = _rows_of(sum_out, "sum_out", size, dtype), sum_out.data_ptr()
+    if out is not None:
+        o, at_o = _rows_of(out, "out", size, dtype), out.data_ptr()
     _check(lib.dsv4cuda_norm_quant(
-        x.data_ptr(), None if residual is None else residual.data_ptr(),
-        None if sum_out is None else sum_out.data_ptr(), None if out is None else out.data_ptr(),
-        _dev(gain, "gain", torch.bfloat16, width), _dev(codes, "codes", torch.uint8, n * width),
-        _dev(scales, "scales", torch.uint8, n * ((width + 127) // 128)), C.byref(shape),
-        _stream(stream)))
+        x.data_ptr(), at_r, at_s, at_o, _dev(gain, "gain", torch.bfloat16, width),
+        _dev(codes, "codes", u8, n * width), _dev(scales, "scales", u8, n * ((width + 127) // 128)),
+        _norm_shape(n, width, bf16, eps, q, r, s, o), _stream(stream)))
 
 
 def _beam_shape(logits, score, cands, eos):
-    import torch
-    if score.dim() != 2 or logits.dim() != 2 or logits.shape[0] != score.numel():
+    dtype, bf16, (n, vocab) = _float_rows(logits, "logits")
+    if score.dim() != 2 or n != score.numel():
         raise ValueError("score [groups][beams] and logits [groups * beams][vocab] are wanted")
-    bf16, stride = _row_tensor(logits, "logits", logits.shape[1])
-    return BeamShape(score.shape[0], score.shape[1], cands, logits.shape[1], bf16, eos, stride)
-
-
-def beam_workspace_bytes(logits, score, n_cands) -> int:
-    """Workspace of a beam_select call of these sizes."""
-    return lib.dsv4cuda_beam_workspace_bytes(C.byref(_beam_shape(logits, score, n_cands, -1)))
+    groups, beams = score.shape
+    return BeamShape(groups, beams, cands, vocab, bf16, eos,
+                     _rows_of(logits, "logits", logits.shape, dtype))
 
 
 def beam_select(logits, score, parent, token, total, next, slot=None, dst=None, src=None, eos=-1,
-                workspace=None, stream=None):
+                stream=None):
     """dsv4cuda_beam_select: the best continuations of each group's beams by score [groups]
     [beams] + log softmax of logits [groups * beams][vocab] (fp32 or BF16, rows may lie apart):
     parent, token int32 and total fp32 [groups][candidates], next int32 [groups][beams] the
     candidates that go on (their token is not eos), and, of the beams' slots slot int32 [groups]
-    [beams], the dst and src of PagedCache.fork. workspace: a CUDA uint8 tensor (needed while
-    capturing)."""
+    [beams], the dst and src of PagedCache.fork."""
     import torch
     i32, f32 = torch.int32, torch.float32
     if parent.dim() != 2:
@@ -915,8 +929,7 @@ def beam_select(logits, score, parent, token, total, next, slot=None, dst=None, 
         logits.data_ptr(), _dev(score, "score", f32), _dev(parent, "parent", i32, all_c),
         _dev(token, "token", i32, all_c), _dev(total, "total", f32, all_c),
         _dev(next, "next", i32, all_b), _dev(slot, "slot", i32, all_b), _dev(dst, "dst", i32, all_b),
-        _dev(src, "src", i32, all_b), C.byref(shape), _dev(workspace, "workspace", torch.uint8),
-        0 if workspace is None else workspace.numel(), _stream(stream)))
+        _dev(src, "src", i32, all_b), C.byref(shape), _stream(stream)))
 
 
 # ------------------------------------------------------- grouped products --

@@ -720,9 +720,8 @@ int dsv4cuda_token_logprobs(const void *logits, int bf16, int rows, int vocab, l
  *       dst[i] and comes from src[i] (-1: from none). A parent's first child
  *       stays where it is (dst = src), the others take the slots of beams
  *       without children, so dsv4cuda_paged_fork(dst, src) puts all in place.
- * beams and n_cands 1 .. 32. DEVICE pointers, async on stream. workspace may be
- * NULL (a buffer per thread and stream); give one, 256-byte aligned, while
- * capturing. */
+ * beams and n_cands 1 .. 32, vocab below 2^30. DEVICE pointers, async on stream,
+ * capturable; no workspace. */
 #define DSV4CUDA_MAX_BEAMS 32
 #define DSV4CUDA_MAX_BEAM_CANDIDATES 32
 typedef struct {
@@ -733,11 +732,9 @@ typedef struct {
     long long stride;
 } dsv4cuda_beam_shape;
 
-size_t dsv4cuda_beam_workspace_bytes(const dsv4cuda_beam_shape *shape);
 int dsv4cuda_beam_select(const void *logits, const float *score, int *parent, int *token,
                          float *total, int *next, const int *slot, int *dst, int *src,
-                         const dsv4cuda_beam_shape *shape, void *workspace,
-                         size_t workspace_bytes, void *stream);
+                         const dsv4cuda_beam_shape *shape, void *stream);
 
 /* ---------------------------------------------------------------------
  * RMS norm of rows with the residual's addition and an 8-bit output

@@ -168,14 +168,13 @@ def test_slots_with_fork(cuda):
 
 def test_captured_and_on_streams(cuda):
     x, score, slot = rows(3, 5, 10000, torch.bfloat16)
-    work = torch.empty(cuda.beam_workspace_bytes(x, score, 10), dtype=torch.uint8, device="cuda")
-    select(cuda, x, score, 10, slot=slot, workspace=work)
+    select(cuda, x, score, 10, slot=slot)
     i32 = dict(dtype=torch.int32, device="cuda")
     parent, token, total = torch.empty(3, 10, **i32), torch.empty(3, 10, **i32), torch.empty(3, 10, device="cuda")
     nxt, dst, src = (torch.empty(3, 5, **i32) for _ in range(3))
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        cuda.beam_select(x, score, parent, token, total, nxt, slot=slot, dst=dst, src=src, workspace=work)
+        cuda.beam_select(x, score, parent, token, total, nxt, slot=slot, dst=dst, src=src)
     for seed in (7, 8):
         y, s, _ = rows(3, 5, 10000, torch.bfloat16, seed)
         x.copy_(y)
@@ -195,6 +194,3 @@ def test_captured_and_on_streams(cuda):
     for r in got:
         for a, w in zip(r, want):
             assert torch.equal(a.cpu(), w)
-    with torch.cuda.graph(torch.cuda.CUDAGraph()):
-        with pytest.raises(cuda.Dsv4CudaError, match="workspace"):
-            select(cuda, x, score, 10)
