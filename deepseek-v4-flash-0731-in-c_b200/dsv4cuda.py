@@ -737,6 +737,7 @@ class PagedCache:
                             _dev(refs, "refs", torch.int32), self.status_word.data_ptr(),
                             self.workspace.data_ptr(), need)
         self._ref = C.byref(self.struct)
+        self._dims = (self.caches[0].struct.nope, self.caches[0].struct.rope_dim) if self.caches else (0, 0)
 
     @classmethod
     def empty(cls, caches, page_size, n_seqs, max_pages):
@@ -768,11 +769,10 @@ class PagedCache:
         import torch
         if not 0 <= layer < len(self.caches):
             raise ValueError(f"layer {layer} of {len(self.caches)}")
-        c = self.caches[layer].struct
-        d = c.nope + c.rope_dim
+        d = self._dims[0] + self._dims[1]
         dtype, bf16, shape = _float_rows(kv, "kv", d)
         stride, n = _rows_of(kv, "kv", shape, dtype), shape[0]
-        half = n * (c.rope_dim // 2)
+        half = n * (self._dims[1] // 2)
         _check(lib.dsv4cuda_paged_write(
             self._ref, layer, kv.data_ptr(), bf16, stride, _dev(rows, "rows", self._i64, n), n,
             _dev(gain, "gain", torch.bfloat16, d), eps, _dev(rope_cos, "rope_cos", torch.float32, half),
