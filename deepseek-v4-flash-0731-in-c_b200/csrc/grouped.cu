@@ -11,13 +11,14 @@
 // large M: a decode step's experts are read at the same cost as a GEMV's.
 //
 // One block per SM takes an equal share of all (tile, 128-column chunk) units
-// laid end to end; a tile is 256 outputs (or 128 gate and 128 up outputs) of
-// up to 192 rows. A tile that a share's end cuts is written as fp32 parts,
+// laid end to end; a tile is 256 outputs (128 gate and 128 up outputs; 128
+// where groups are large) of up to 192 rows. A tile that a share's end cuts is written as fp32 parts,
 // and whoever brings its last part adds them in the order of the columns, so
 // that results do not depend on timing.
 //
 // Roles: warps 0-7 epilogue, 8-11 scales (to TMEM, each warp the copy of its
-// lane quarter), 12-13 copies of rows of x, 14 copies of weights, 15 MMAs.
+// lane quarter), 12 copies of rows of x, 13 copies of weights, 14-15 MMAs (a
+// tile of 128 outputs each).
 #include "grouped.cuh"
 
 #include <cuda_bf16.h>
@@ -31,10 +32,10 @@ namespace {
 constexpr int kChunk = 128;              // columns of a stage: one row of swizzled shared memory
 constexpr int kTileRows = 128;           // M of an instruction
 constexpr int kATile = kTileRows * kChunk;
-constexpr int kEpiWarps = 8, kScaleWarps = 4, kRowWarps = 2;
-constexpr int kWarpRows = kEpiWarps + kScaleWarps, kWarpCopy = kWarpRows + kRowWarps;
-constexpr int kWarpMma = kWarpCopy + 1;
-constexpr int kThreads = 32 * (kWarpMma + 1);
+constexpr int kEpiWarps = 8, kScaleWarps = 4;
+constexpr int kWarpRows = kEpiWarps + kScaleWarps, kWarpCopy = kWarpRows + 1;
+constexpr int kWarpMma = kWarpCopy + 1;  // and the next, for a second tile
+constexpr int kThreads = 32 * (kWarpMma + 2);
 constexpr int kBlockCols = 16;           // rows of a group that an epilogue step takes
 constexpr int kMaxN = 192, kHalfN = 96;  // rows of a tile; up to kHalfN two tiles' sums fit in TMEM
 constexpr int kMaxStages = 5;
@@ -67,16 +68,16 @@ struct alignas(16) Control {
 };
 
 // The ring of scales: an entry holds four chunks' of 256 outputs and n_max rows.
-// Behind it each row warp's rows of x.
+// Behind it a tile's rows of x.
 constexpr int kScaleEntries = 4, kScaleBytes = 2 * kTileRows * 16;
 __host__ __device__ constexpr int scale_entry_bytes(int n_max) { return kScaleBytes + n_max * 4; }
 __host__ __device__ constexpr int scale_ring_bytes(int n_max) {
-  return kScaleEntries * scale_entry_bytes(n_max) + kRowWarps * n_max * 4;
+  return kScaleEntries * scale_entry_bytes(n_max) + n_max * 4;
 }
 
-__host__ __device__ constexpr int stage_bytes(int n_max) { return 2 * kATile + n_max * kChunk; }
-__host__ __device__ inline size_t smem_bytes(int n_max, int stages, int experts) {
-  return static_cast<size_t>(stages) * stage_bytes(n_max) + scale_ring_bytes(n_max) +
+__host__ __device__ constexpr int stage_bytes(int tiles, int n_max) { return tiles * kATile + n_max * kChunk; }
+__host__ __device__ inline size_t smem_bytes(int tiles, int n_max, int stages, int experts) {
+  return static_cast<size_t>(stages) * stage_bytes(tiles, n_max) + scale_ring_bytes(n_max) +
          sizeof(Control) + (kMaxShares + 1) * sizeof(long long) +
          (experts + 1) * (sizeof(long long) + sizeof(int));
 }
@@ -108,14 +109,17 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
 }
 
 // D (+)= A B with block scales: A and B types in idesc, one E8M0 per 32
-// columns, byte `k` of each scale column.
-__device__ __forceinline__ void mma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+// columns. a and b: shared memory in 16 bytes, of tiles with the 128-byte
+// swizzle whose groups of eight rows lie one behind the other.
+__device__ __forceinline__ void mma_scaled(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
                                            uint32_t scale_a, uint32_t scale_b, bool accumulate) {
+  constexpr uint32_t kHigh = (1024 >> 4) | (1u << 14) | (2u << 29);  // as umma_desc has it
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+      "{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.b32 p, %6, 0;\n"
+      " mov.b64 x, {%1, %7};\n mov.b64 y, {%2, %7};\n"
       " tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X"
-      " [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate ? 1u : 0u)
+      " [%0], x, y, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate ? 1u : 0u), "r"(kHigh)
       : "memory");
 }
 __device__ __forceinline__ bool elect_one() {
@@ -288,13 +292,13 @@ struct Walk {
 
 // -------------------------------------------------------------- products --
 
-template <bool kFp8, bool kGated>
+template <bool kFp8, bool kGated, int kTiles>
 __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUtensorMap map1,
     const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Args a) {
   extern __shared__ __align__(1024) uint8_t smem[];
   const GroupedProblem& p = a.p;
-  uint8_t* scale_ring = smem + static_cast<size_t>(a.stages) * stage_bytes(a.n_max);
+  uint8_t* scale_ring = smem + static_cast<size_t>(a.stages) * stage_bytes(kTiles, a.n_max);
   int* row_table = reinterpret_cast<int*>(scale_ring + kScaleEntries * scale_entry_bytes(a.n_max));
   Control* ctl = reinterpret_cast<Control*>(scale_ring + scale_ring_bytes(a.n_max));
   long long* bounds = reinterpret_cast<long long*>(ctl + 1);  // [shares + 1] in cost
@@ -304,21 +308,22 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
   unsigned* err = p.err;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int chunks = p.width / kChunk;
-  constexpr int kOuts = kGated ? kTileRows : 2 * kTileRows;  // of a tile
+  constexpr int kOuts = kGated ? kTileRows : kTiles * kTileRows;  // of a tile
+  static_assert(!kGated || kTiles == 2, "gate and up");
   const int row_tiles = (p.outs + kOuts - 1) / kOuts;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.stages; ++i) {
-      mbar_init(&ctl->full[i], 1 + kRowWarps);
-      mbar_init(&ctl->empty[i], 1);
+      mbar_init(&ctl->full[i], 2);  // rows and weights
+      mbar_init(&ctl->empty[i], kTiles);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl->scale_full[i], 32 * kScaleWarps);
-      mbar_init(&ctl->scale_empty[i], 1);
-      mbar_init(&ctl->sum_full[i], 1);
+      mbar_init(&ctl->scale_empty[i], kTiles);
+      mbar_init(&ctl->sum_full[i], kTiles);
       mbar_init(&ctl->sum_empty[i], 32 * kEpiWarps);
     }
-    mbar_init(&ctl->fin, 1);
+    mbar_init(&ctl->fin, kTiles);
     ctl->abort_flag = 0;
     mbar_fence_init();
   }
@@ -412,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
   walk.begin(prefix, me < shares ? bound(me) : 0, share_end);
   Piece piece;
   auto two_tiles = [&](const Piece& q) {
-    return kGated || q.row_tile * kOuts + kTileRows < p.outs;
+    return kGated || (kTiles == 2 && q.row_tile * kOuts + kTileRows < p.outs);
   };
 
   if (warp < kEpiWarps) {
@@ -427,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
       const long long start = share_end - walk.left;
       const int cost = walk.cut.cost;
       if (!walk.next(&piece)) break;
-      const bool big = piece.n > kHalfN;
+      const bool big = kTiles == 2 && piece.n > kHalfN;
       const int blocks = piece.n / kBlockCols;
       // this lane's row of a block: its weight, or its row of out
       auto lane_row = [&](int b) {
@@ -472,9 +477,9 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
         for (int r = side * 8; r < piece.n; r += 16) {
           uint32_t r0[8], r1[8];
           tmem_ld8(sums + r, r0);
-          tmem_ld8(sums1 + r, r1);  // (not used where there is no second tile)
+          if (kTiles == 2) tmem_ld8(sums1 + r, r1);  // (not used where there is no second tile)
           tmem_ld_wait8(r0);
-          tmem_ld_wait8(r1);
+          if (kTiles == 2) tmem_ld_wait8(r1);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             float* q = mine + static_cast<size_t>(r + i) * kTileRows;
@@ -503,20 +508,20 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
       uint32_t ahead0[16], ahead1[16];
       if (!cut && side < blocks) {
         tmem_ld16(sums + side * kBlockCols, ahead0);
-        tmem_ld16(sums1 + side * kBlockCols, ahead1);
+        if (kTiles == 2) tmem_ld16(sums1 + side * kBlockCols, ahead1);
       }
       auto take = [&](int b, float (&v0)[16], float (&v1)[16]) {
         if (!cut) {
           tmem_ld_wait16(ahead0);
-          tmem_ld_wait16(ahead1);
+          if (kTiles == 2) tmem_ld_wait16(ahead1);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             v0[i] = __uint_as_float(ahead0[i]);
-            v1[i] = __uint_as_float(ahead1[i]);
+            v1[i] = kTiles == 2 ? __uint_as_float(ahead1[i]) : 0.f;
           }
           if (b + 2 < blocks) {
             tmem_ld16(sums + (b + 2) * kBlockCols, ahead0);
-            tmem_ld16(sums1 + (b + 2) * kBlockCols, ahead1);
+            if (kTiles == 2) tmem_ld16(sums1 + (b + 2) * kBlockCols, ahead1);
           }
           return;
         }
@@ -594,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
           flip ^= 1;
         } else {
           const int o0 = piece.row_tile * kOuts + at, o1 = o0 + kTileRows;
-          const bool in0 = o0 < p.outs, in1 = o1 < p.outs;
+          const bool in0 = o0 < p.outs, in1 = kTiles == 2 && o1 < p.outs;
           {
             if (a.wide) {
               // BF16, four outputs of a row a lane: pairs of rows as a word, and
@@ -602,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
               // of two bytes a lane)
               const int k = lane & 3;
 #pragma unroll
-              for (int t = 0; t < 2; ++t) {
+              for (int t = 0; t < kTiles; ++t) {
                 const float* v = t ? v1 : v0;
                 const int o = (t ? o1 : o0) - k;
 #pragma unroll
@@ -679,8 +684,8 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
         const int left = min(chunks - 4 * q, 4);  // chunks there are
         if (kFp8) {
           // one block of 128 outputs: the same in every lane
-          if (st < 2) {
-            const int rb = min(piece.row_tile * 2 + st, blocks128 - 1);
+          if (st < kTiles) {
+            const int rb = min(piece.row_tile * kTiles + st, blocks128 - 1);
             const uint8_t* from =
                 p.ws[0] + (static_cast<size_t>(piece.e) * blocks128 + rb) * chunks + 4 * q;
             if (wide) {
@@ -692,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
           }
         } else {
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
+          for (int t = 0; t < kTiles; ++t) {
             const int row = piece.row_tile * kOuts + (kGated ? 0 : t * kTileRows) + st;
             const uint8_t* from =
                 p.ws[kGated ? t : 0] +
@@ -743,9 +748,9 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
       wait_bar(&ctl->scale_empty[buf], ((n >> 1) & 1) ^ 1, abort_flag, err);
       tc_fence_after();
       // (what lies behind a tile's rows or chunks is not used)
-      uint32_t v[32];
+      uint32_t v[32] = {};
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < kTiles; ++t) {
         if (kFp8) {
           const uint32_t u = *reinterpret_cast<const uint32_t*>(entry + 4 * t);
 #pragma unroll
@@ -780,11 +785,10 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     cp_async_wait<0>();
   } else if (warp < kWarpCopy) {
     // ---------------------------------------------------------------- rows
-    // Each warp's elected thread copies half of a tile's rows: rows in their
-    // order 16 at a time, others by gathers of four. (Copies of 16 bytes a
-    // thread moved 27 bytes a clock at most.)
-    const int part = warp - kWarpRows;
-    int* table = row_table + part * a.n_max;
+    // One thread copies a tile's rows: rows in their order 16 at a time, others
+    // by gathers of four. (Copies of 16 bytes a thread moved 27 bytes a clock at
+    // most.)
+    int* table = row_table;
     int s = 0;
     uint32_t phase = 1;
     unsigned n = 0;
@@ -799,34 +803,27 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
         __syncwarp();
       }
       if (elect_one()) {
-        const int step = p.src ? 4 : 16;
-        const int copies = (piece.n / step + kRowWarps - 1 - part) / kRowWarps;
-        const uint32_t bytes = copies * step * kChunk;
         for (int c = piece.lo; c < piece.hi; ++c) {
           good = good && wait_bar(&ctl->empty[s], phase, abort_flag, err);
           if (!good) break;
-          uint8_t* to = smem + static_cast<size_t>(s) * stage_bytes(a.n_max) + 2 * kATile;
-          mbar_arrive_expect_tx(&ctl->full[s], bytes);
+          uint8_t* to = smem + static_cast<size_t>(s) * stage_bytes(kTiles, a.n_max) + kTiles * kATile;
+          mbar_arrive_expect_tx(&ctl->full[s], piece.n * kChunk);
           if (p.src) {
-            const int4* rows = reinterpret_cast<const int4*>(table) + part;
-            to += part * 4 * kChunk;
+            const int4* rows = reinterpret_cast<const int4*>(table);
             int4 next = rows[0];
 #pragma unroll 1
-            for (int i = 0; i < copies; ++i) {
+            for (int i = 4; i <= piece.n; i += 4) {
               const int4 r = next;
-              rows += kRowWarps;
-              if (i + 1 < copies) next = rows[0];
+              ++rows;
+              if (i < piece.n) next = rows[0];
               tma_gather4(to, &xmap, c * kChunk, r, &ctl->full[s]);
-              to += kRowWarps * 4 * kChunk;
+              to += 4 * kChunk;
             }
           } else {
-            to += part * 16 * kChunk;
-            int r = piece.row0 + part * 16;
 #pragma unroll 1
-            for (int i = 0; i < copies; ++i) {
+            for (int r = piece.row0; r < piece.row0 + piece.n; r += 16) {
               tma_load_2d(to, &xmap, c * kChunk, r, &ctl->full[s]);
-              r += kRowWarps * 16;
-              to += kRowWarps * 16 * kChunk;
+              to += 16 * kChunk;
             }
           }
           ++n;
@@ -856,7 +853,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
         for (int c = piece.lo; c < piece.hi; ++c) {
           good = wait_bar(&ctl->empty[s], phase, abort_flag, err);
           if (!good) break;
-          uint8_t* st = smem + static_cast<size_t>(s) * stage_bytes(a.n_max);
+          uint8_t* st = smem + static_cast<size_t>(s) * stage_bytes(kTiles, a.n_max);
           mbar_arrive_expect_tx(&ctl->full[s], (second ? 2 : 1) * kTileTx);
           tma_load_3d(st, &map0, c * kChunk, row, piece.e, &ctl->full[s]);
           if (second)
@@ -875,16 +872,22 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
           mbar_wait(&ctl->full[i % a.stages], (i / a.stages) & 1, err);
     }
     __syncwarp();
-  } else {
+  } else if (warp < kWarpMma + kTiles) {
     // ---------------------------------------------------------------- MMAs
+    // A thread a tile: what a chunk's waits, operands and commit take of one
+    // thread is more than the tensor pipe takes for small tiles.
     if (elect_one()) {
+      const int tile = warp - kWarpMma;
       const uint32_t idesc0 = ((kFp8 ? 0u : 5u) << 7) | (1u << 23) | (8u << 24);
+      const uint32_t stage_step = stage_bytes(kTiles, a.n_max) >> 4;
+      const uint32_t base0 = smem_addr(smem) >> 4;
+      uint32_t base = base0;  // of the stage, in 16 bytes
       unsigned uses[2] = {0, 0}, scales = 0;
       int half = 0, s = 0;
       uint32_t phase = 0;
       bool good = true;
       while (good && walk.next(&piece)) {
-        const bool big = piece.n > kHalfN, second = two_tiles(piece);
+        const bool big = kTiles == 2 && piece.n > kHalfN, mine = tile == 0 || two_tiles(piece);
         const int h = big ? 0 : half;
         if (big) {
           good = wait_bar(&ctl->sum_empty[0], (uses[0]++ & 1) ^ 1, abort_flag, err) &&
@@ -893,32 +896,38 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
           good = wait_bar(&ctl->sum_empty[h], (uses[h]++ & 1) ^ 1, abort_flag, err);
           half ^= 1;
         }
-        const uint32_t d0 = tmem + kSumCol + (big ? 0 : h * kMaxN), d1 = d0 + (big ? kMaxN : kHalfN);
+        const uint32_t d = tmem + kSumCol + (big ? 0 : h * kMaxN) + tile * (big ? kMaxN : kHalfN);
         const uint32_t idesc = idesc0 | (static_cast<uint32_t>(piece.n >> 3) << 17);
+        uint32_t sa = 0;
         for (int c = piece.lo; good && c < piece.hi; ++c) {
           const int buf = scales & 1;
-          if (c == piece.lo || (c & 3) == 0)
-            good = wait_bar(&ctl->scale_full[buf], (scales >> 1) & 1, abort_flag, err);
-          good = good && wait_bar(&ctl->full[s], phase, abort_flag, err);
+          if (c == piece.lo || (c & 3) == 0) {
+            good = mbar_try_wait(&ctl->scale_full[buf], (scales >> 1) & 1) ||
+                   wait_bar(&ctl->scale_full[buf], (scales >> 1) & 1, abort_flag, err);
+            tc_fence_after();
+            sa = tmem + buf * kScaleCols + (c & 3) * 8;
+          }
+          if (!mbar_try_wait(&ctl->full[s], phase))
+            good = good && wait_bar(&ctl->full[s], phase, abort_flag, err);
           if (!good) break;
-          tc_fence_after();
-          const uint32_t base = smem_addr(smem + static_cast<size_t>(s) * stage_bytes(a.n_max));
-          const uint64_t a0 = umma_desc(base, 0, 1024), a1 = umma_desc(base + kATile, 0, 1024);
-          const uint64_t b0 = umma_desc(base + 2 * kATile, 0, 1024);
-          const uint32_t sa = tmem + buf * kScaleCols + (c & 3) * 8, sb = sa + 32;
+          if (mine) {
+            const uint32_t at = base + tile * (kATile >> 4), bt = base + kTiles * (kATile >> 4);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t id = idesc | (static_cast<uint32_t>(k) << 4) | (static_cast<uint32_t>(k) << 29);
-            mma_scaled(d0, a0 + 2 * k, b0 + 2 * k, id, sa, sb, k > 0 || c > piece.lo);
-            if (second) mma_scaled(d1, a1 + 2 * k, b0 + 2 * k, id, sa + 4, sb, k > 0 || c > piece.lo);
+            for (int k = 0; k < 4; ++k)
+              mma_scaled(d, at + 2 * k, bt + 2 * k,
+                         idesc | (static_cast<uint32_t>(k) << 4) | (static_cast<uint32_t>(k) << 29),
+                         sa + tile * 4, sa + 32, k > 0 || c > piece.lo);
           }
           mma_commit(&ctl->empty[s]);
+          sa += 8;
           if ((c & 3) == 3 || c + 1 == piece.hi) {
             mma_commit(&ctl->scale_empty[buf]);
             ++scales;
           }
+          base += stage_step;
           if (++s == a.stages) {
             s = 0;
+            base = base0;
             phase ^= 1;
           }
         }
@@ -967,8 +976,8 @@ __global__ void grouped_reset_kernel(int* counters) {
 
 // --------------------------------------------------- routes, tokens' sums --
 
-constexpr int kGroupThreads = 1024, kGroupWarps = kGroupThreads / 32;
-constexpr int kGroupAhead = 8;
+constexpr int kGroupThreads = 256, kGroupWarps = kGroupThreads / 32;
+constexpr int kGroupAhead = 4, kGroupSlots = 1024, kGroupBlocks = 16;
 
 struct GroupArgs {
   const int* idx;    // [slots]
@@ -981,20 +990,25 @@ struct GroupArgs {
   int* counters;     // two products' [kMaxShares]
 };
 
-// A stable counting sort by one block: each warp counts, then places, its own
-// stretch of the slots.
+// A stable counting sort by a cluster of blocks: each warp counts, then places,
+// its own stretch of the slots; blocks read one another's counts. (One block
+// took 126 us for 49,152 slots.)
 __global__ void __launch_bounds__(kGroupThreads) group_kernel(const GroupArgs a) {
-  extern __shared__ int count[];  // [kGroupWarps][experts]
-  __shared__ int total[32], before;
+  extern __shared__ int count[];  // [kGroupWarps][experts], [experts] of the block
+  __shared__ int total[kGroupWarps], before;
+  const int rank = blockIdx.x, blocks = gridDim.x;  // one cluster
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x < 2 * kMaxShares) a.counters[threadIdx.x] = 0;
+  int* sums = count + kGroupWarps * a.experts;
+  for (int i = rank * kGroupThreads + threadIdx.x; i < 2 * kMaxShares; i += blocks * kGroupThreads)
+    a.counters[i] = 0;
   for (int i = threadIdx.x; i < kGroupWarps * a.experts; i += kGroupThreads) count[i] = 0;
   __syncthreads();
   int* mine = count + warp * a.experts;
-  const int each = ((a.slots + kGroupThreads - 1) / kGroupThreads) * 32;  // slots of a warp
-  const int s0 = min(warp * each, a.slots), s1 = min(s0 + each, a.slots);
+  const int warps = blocks * kGroupWarps;
+  const int each = (a.slots / 32 + warps) / warps * 32;  // slots of a warp
+  const int s0 = min((rank * kGroupWarps + warp) * each, a.slots), s1 = min(s0 + each, a.slots);
   auto walk = [&](auto&& f) {
     for (int base = s0; base < s1; base += 32 * kGroupAhead) {
       int e[kGroupAhead];
@@ -1004,42 +1018,56 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(const GroupArgs a)
         e[i] = s < s1 ? a.idx[s] - a.lo : a.experts;
         if (e[i] >= a.experts || e[i] < 0) e[i] = a.experts;  // none of these
       }
-#pragma unroll
-      for (int i = 0; i < kGroupAhead; ++i) {
-        if (base + i * 32 >= s1) break;
-        // the lanes with this lane's expert (a match instruction took 3,000
-        // clocks for 32 experts: 12,000 slots 41 us)
+#pragma unroll 1
+      for (int i = 0; i < kGroupAhead && base + i * 32 < s1; ++i) {
+        const int x = i == 0 ? e[0] : i == 1 ? e[1] : i == 2 ? e[2] : e[3];
+        // the lanes with this lane's expert
         unsigned same = 0xffffffffu;
         for (int b = 1; b <= a.experts; b <<= 1) {
-          const unsigned set = __ballot_sync(0xffffffffu, e[i] & b);
-          same &= (e[i] & b) ? set : ~set;
+          const unsigned set = __ballot_sync(0xffffffffu, x & b);
+          same &= (x & b) ? set : ~set;
         }
         const int first = __ffs(same) - 1;
         int at = 0;
-        if (lane == first && e[i] < a.experts) {
-          at = mine[e[i]];
-          mine[e[i]] = at + __popc(same);
+        if (lane == first && x < a.experts) {
+          at = mine[x];
+          mine[x] = at + __popc(same);
         }
         at = __shfl_sync(0xffffffffu, at, first) + __popc(same & ((1u << lane) - 1));
         __syncwarp();
-        if (e[i] < a.experts) f(base + i * 32 + lane, at);
+        if (x < a.experts) f(base + i * 32 + lane, at);
       }
     }
   };
   walk([](int, int) {});
   __syncthreads();
-  // counts to first places: over the experts, and the warps of one
+  // this block's counts, and its warps' places in them
+  for (int e = threadIdx.x; e < a.experts; e += kGroupThreads) {
+    int sum = 0;
+    for (int w = 0; w < kGroupWarps; ++w) {
+      const int c = count[w * a.experts + e];
+      count[w * a.experts + e] = sum;
+      sum += c;
+    }
+    sums[e] = sum;
+  }
   if (threadIdx.x == 0) before = 0;
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  // first places: over the experts, and the blocks before this one
   for (int e0 = 0; e0 < a.experts; e0 += kGroupThreads) {
     const int e = e0 + threadIdx.x;
-    int sum = 0;
+    int all = 0, earlier = 0;
     if (e < a.experts)
-      for (int w = 0; w < kGroupWarps; ++w) {
-        const int c = count[w * a.experts + e];
-        count[w * a.experts + e] = sum;
-        sum += c;
+      for (int r = 0; r < blocks; ++r) {
+        uint32_t from;
+        int c;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(smem_addr(sums + e)), "r"(r));
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(c) : "r"(from) : "memory");
+        if (r < rank) earlier += c;
+        all += c;
       }
-    int incl = sum;
+    int incl = all;
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, incl, s);
@@ -1047,25 +1075,17 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(const GroupArgs a)
     }
     if (lane == 31) total[warp] = incl;
     __syncthreads();
-    if (warp == 0) {
-      const int t = total[lane];
-      int i = t;
-#pragma unroll
-      for (int s = 1; s < 32; s <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, i, s);
-        if (lane >= s) i += u;
-      }
-      total[lane] = i - t;
-    }
+    int first = before + incl - all;
+    for (int w = 0; w < warp; ++w) first += total[w];
     __syncthreads();
-    const int first = before + total[warp] + incl - sum;
-    __syncthreads();
+    if (threadIdx.x == kGroupThreads - 1) before = first + all;
     if (e < a.experts) {
-      a.offsets[e] = first;
-      for (int w = 0; w < kGroupWarps; ++w) count[w * a.experts + e] += first;
-      if (e == a.experts - 1) a.offsets[a.experts] = first + sum;
+      if (rank == 0) {
+        a.offsets[e] = first;
+        if (e == a.experts - 1) a.offsets[a.experts] = first + all;
+      }
+      for (int w = 0; w < kGroupWarps; ++w) count[w * a.experts + e] += first + earlier;
     }
-    if (threadIdx.x == kGroupThreads - 1) before = first + sum;
     __syncthreads();
   }
   walk([&](int s, int at) {
@@ -1073,6 +1093,10 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(const GroupArgs a)
     a.token[at] = s / a.topk;
     a.weight[at] = a.wt[s];
   });
+  // until then the others read this block's counts
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // out[t] = the sum of the token's slots in route order; slots of experts that
@@ -1094,11 +1118,13 @@ __global__ void __launch_bounds__(256) experts_combine_kernel(const uint16_t* __
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       r[k] = make_uint4(0, 0, 0, 0);
-      if (k0 + k < topk) {
-        const int s = t * topk + k0 + k, e = idx[s] - lo;
-        if (e >= 0 && e < experts)
-          r[k] = __ldcs(reinterpret_cast<const uint4*>(y + static_cast<size_t>(s) * hidden) + v);
-      }
+      if (k0 + k < topk)  // (before it is known whether it was written)
+        r[k] = __ldcs(reinterpret_cast<const uint4*>(y + (static_cast<size_t>(t) * topk + k0 + k) * hidden) + v);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int e = k0 + k < topk ? idx[t * topk + k0 + k] - lo : -1;
+      if (e < 0 || e >= experts) r[k] = make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -1126,14 +1152,15 @@ int sm_count() {
 }
 
 struct Shape {
-  int n_max, stages;
+  int tiles, n_max, stages;
 };
 Shape tile_shape(const GroupedProblem& p) {
   const long long rows = p.rows, each = p.experts;  // rows of a group on average
   const int n_max = rows <= 8 * each ? 16 : rows <= 24 * each ? 32 : rows <= 64 * each ? kHalfN : kMaxN;
+  const int tiles = p.w[1] == nullptr && n_max == kMaxN ? 1 : 2;
   int stages = kMaxStages;
-  while (smem_bytes(n_max, stages, p.experts) > kMaxSmem) --stages;
-  return {n_max, stages};
+  while (smem_bytes(tiles, n_max, stages, p.experts) > kMaxSmem) --stages;
+  return {tiles, n_max, stages};
 }
 
 size_t parts_bytes(const GroupedProblem& p) {
@@ -1194,12 +1221,13 @@ cudaError_t launch(GroupedProblem p, int* counters, float* parts, void* gathered
   a.parts = parts;
   if (a.shares < 1) return cudaErrorInvalidDevice;
   if (gated && p.fp8) return cudaErrorInvalidValue;
-  auto kernel = gated ? grouped_kernel<false, true>
-                      : p.fp8 ? grouped_kernel<true, false> : grouped_kernel<false, false>;
+  auto kernel = gated ? grouped_kernel<false, true, 2>
+                : s.tiles == 1 ? (p.fp8 ? grouped_kernel<true, false, 1> : grouped_kernel<false, false, 1>)
+                               : (p.fp8 ? grouped_kernel<true, false, 2> : grouped_kernel<false, false, 2>);
   cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), static_cast<int>(kMaxSmem));
   if (e != cudaSuccess) return e;
   return launch_pdl(kernel, dim3(a.shares), dim3(kThreads),
-                    smem_bytes(s.n_max, s.stages, p.experts), st, map0, map1, xmap, a);
+                    smem_bytes(s.tiles, s.n_max, s.stages, p.experts), st, map0, map1, xmap, a);
 }
 
 // Pieces of a buffer, 256-byte aligned.
@@ -1295,10 +1323,28 @@ cudaError_t experts_forward(const ExpertsProblem& p, void* ws, cudaStream_t st) 
   a.token = w.token;
   a.weight = w.weight;
   a.counters = w.counters;
-  const size_t smem = sizeof(int) * kGroupWarps * p.experts;
-  cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(group_kernel),
-                                       static_cast<int>(sizeof(int)) * kGroupWarps * kGroupedMaxExperts);
-  if (e == cudaSuccess) e = launch_pdl(group_kernel, dim3(1), dim3(kGroupThreads), smem, st, a);
+  const void* group = reinterpret_cast<const void*>(group_kernel);
+  cudaError_t e = set_max_dynamic_smem(
+      group, static_cast<int>(sizeof(int)) * (kGroupWarps + 1) * kGroupedMaxExperts);
+  int blocks = 1;
+  while (blocks < kGroupBlocks && a.slots > blocks * kGroupSlots) blocks *= 2;
+  if (e == cudaSuccess && blocks > 8)  // more than every device has to take
+    e = cudaFuncSetAttribute(group, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return e;
+  prefer_max_shared(group);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kGroupThreads);
+  cfg.dynamicSmemBytes = sizeof(int) * (kGroupWarps + 1) * p.experts;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {static_cast<unsigned>(blocks), 1, 1};
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, group_kernel, a);
   if (e != cudaSuccess) return e;
   const GroupedProblem g = gate_up(p, w);
   e = launch(g, w.counters, w.parts, w.gathered, st);
