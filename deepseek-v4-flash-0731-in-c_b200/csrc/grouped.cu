@@ -11,14 +11,19 @@
 // large M: a decode step's experts are read at the same cost as a GEMV's.
 //
 // One block per SM takes an equal share of all (tile, 128-column chunk) units
-// laid end to end; a tile is 256 outputs (128 gate and 128 up outputs; 128
-// where groups are large) of up to 192 rows. A tile that a share's end cuts is written as fp32 parts,
+// laid end to end; a tile is 256 outputs (or 128 gate and 128 up outputs) of
+// up to 192 rows. A tile that a share's end cuts is written as fp32 parts,
 // and whoever brings its last part adds them in the order of the columns, so
 // that results do not depend on timing.
 //
 // Roles: warps 0-7 epilogue, 8-11 scales (to TMEM, each warp the copy of its
-// lane quarter), 12 copies of rows of x, 13 copies of weights, 14-15 MMAs (a
-// tile of 128 outputs each).
+// lane quarter), 12-15 other rows of x, 16 copies by TMA (weights, and rows that lie in
+// their order), 17-18 MMAs (a tile of 128 outputs each).
+//
+// What bounds it where the weights' bytes do not: the TMA engine brings a row of
+// 128 bytes of shared memory in some 2.7 clocks, whatever its bytes in memory, so
+// 256 weights' rows of a chunk take 690 clocks; then the shared memory's own
+// bandwidth, 64 KB a chunk for the E2M1 tiles' two halves and 384 bytes a row.
 #include "grouped.cuh"
 
 #include <cuda_bf16.h>
@@ -32,8 +37,9 @@ namespace {
 constexpr int kChunk = 128;              // columns of a stage: one row of swizzled shared memory
 constexpr int kTileRows = 128;           // M of an instruction
 constexpr int kATile = kTileRows * kChunk;
-constexpr int kEpiWarps = 8, kScaleWarps = 4;
-constexpr int kWarpRows = kEpiWarps + kScaleWarps, kWarpCopy = kWarpRows + 1;
+constexpr int kTiles = 2;                // of 128 outputs, on the same rows of x: gate and up, or 256 outputs
+constexpr int kEpiWarps = 8, kScaleWarps = 4, kRowWarps = 4;
+constexpr int kWarpRows = kEpiWarps + kScaleWarps, kWarpCopy = kWarpRows + kRowWarps;
 constexpr int kWarpMma = kWarpCopy + 1;  // and the next, for a second tile
 constexpr int kThreads = 32 * (kWarpMma + 2);
 constexpr int kBlockCols = 16;           // rows of a group that an epilogue step takes
@@ -68,16 +74,17 @@ struct alignas(16) Control {
 };
 
 // The ring of scales: an entry holds four chunks' of 256 outputs and n_max rows.
-// Behind it a tile's rows of x.
+// Behind it the rows of x of two pieces.
+__host__ __device__ constexpr int row_table_ints(int n_max) { return n_max + 16; }
 constexpr int kScaleEntries = 4, kScaleBytes = 2 * kTileRows * 16;
 __host__ __device__ constexpr int scale_entry_bytes(int n_max) { return kScaleBytes + n_max * 4; }
 __host__ __device__ constexpr int scale_ring_bytes(int n_max) {
-  return kScaleEntries * scale_entry_bytes(n_max) + n_max * 4;
+  return kScaleEntries * scale_entry_bytes(n_max) + 2 * row_table_ints(n_max) * 4;
 }
 
-__host__ __device__ constexpr int stage_bytes(int tiles, int n_max) { return tiles * kATile + n_max * kChunk; }
-__host__ __device__ inline size_t smem_bytes(int tiles, int n_max, int stages, int experts) {
-  return static_cast<size_t>(stages) * stage_bytes(tiles, n_max) + scale_ring_bytes(n_max) +
+__host__ __device__ constexpr int stage_bytes(int n_max) { return kTiles * kATile + n_max * kChunk; }
+__host__ __device__ inline size_t smem_bytes(int n_max, int stages, int experts) {
+  return static_cast<size_t>(stages) * stage_bytes(n_max) + scale_ring_bytes(n_max) +
          sizeof(Control) + (kMaxShares + 1) * sizeof(long long) +
          (experts + 1) * (sizeof(long long) + sizeof(int));
 }
@@ -133,18 +140,6 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
           smem_addr(bar))
       : "memory");
 }
-// Four rows of a tensor map with one-row boxes, one behind the other; a row
-// outside the map is zeros.
-__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, int x, const int4& y,
-                                            uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w),
-      "r"(smem_addr(bar))
-      : "memory");
-}
-
 // 8 consecutive TMEM columns of this thread's lane.
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -159,27 +154,20 @@ __device__ __forceinline__ void tmem_ld_wait8(uint32_t (&r)[8]) {
                  "+r"(r[7])::"memory");
 }
 
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
-      "%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_ld_wait16(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
-                 "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
-                 "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
-}
-
 __device__ __forceinline__ void cp_async16(uint32_t to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void cp_async4(uint32_t to, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+// Zeros where there is nothing to be read.
+__device__ __forceinline__ void cp_async16_or_0(uint32_t to, const void* from, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0)
+               : "memory");
+}
+// This thread's arrival once all its copies so far are there.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -194,19 +182,21 @@ __device__ __forceinline__ void bar_sync(int id, int threads) {
 // ------------------------------------------------------------------ plan --
 
 // How a group of n rows is cut: tiles of the same number of rows, a multiple
-// of 16, and what a chunk of one costs. Up to some 90 rows a chunk costs what
-// its weights take to come from memory, beyond that what the MMAs take.
+// of 16, and what a chunk of one costs in clocks (measured: 740 for 16 rows, 830
+// for 48, 930 for 80, where two tiles' sums fit in TMEM; beyond that the epilogue,
+// some 67 clocks a row, is not overlapped).
+// With every chunk counted alike the slowest block took 558 us where the mean was
+// 455 (2,000 tokens of 4096 x 2048, gate and up).
 struct Cut {
   int tiles, rows, cost;
 };
-constexpr int kMemoryCost = 90;
 constexpr int kSnapTiles = 8;  // shares of so many tiles on average are not cut
-__device__ __forceinline__ Cut cut_group(int n, int n_max) {
+__device__ __forceinline__ Cut cut_group(int n, int n_max, int chunks) {
   Cut c;
   c.tiles = (n + n_max - 1) / n_max;
   c.rows = c.tiles ? ((n + c.tiles - 1) / c.tiles + 15) & ~15 : 16;
   c.tiles = c.tiles ? (n + c.rows - 1) / c.rows : 0;
-  c.cost = c.rows > kMemoryCost ? c.rows : kMemoryCost;
+  c.cost = 690 + 3 * c.rows + (c.rows > kHalfN ? 67 * c.rows / chunks : 0);
   return c;
 }
 
@@ -245,7 +235,7 @@ struct Walk {
   int e, row_tile, t, lo;   // the next piece
   long long left;           // from its tile's start to the share's end, in cost
 
-  __device__ __forceinline__ void recut() { cut = cut_group(offsets[e + 1] - offsets[e], n_max); }
+  __device__ __forceinline__ void recut() { cut = cut_group(offsets[e + 1] - offsets[e], n_max, chunks); }
   // prefix [experts + 1]: cost before each group; the share is b0 .. b1.
   __device__ __forceinline__ void begin(const long long* prefix, long long b0, long long b1) {
     left = 0;
@@ -292,13 +282,13 @@ struct Walk {
 
 // -------------------------------------------------------------- products --
 
-template <bool kFp8, bool kGated, int kTiles>
+template <bool kFp8, bool kGated>
 __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUtensorMap map1,
     const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Args a) {
   extern __shared__ __align__(1024) uint8_t smem[];
   const GroupedProblem& p = a.p;
-  uint8_t* scale_ring = smem + static_cast<size_t>(a.stages) * stage_bytes(kTiles, a.n_max);
+  uint8_t* scale_ring = smem + static_cast<size_t>(a.stages) * stage_bytes(a.n_max);
   int* row_table = reinterpret_cast<int*>(scale_ring + kScaleEntries * scale_entry_bytes(a.n_max));
   Control* ctl = reinterpret_cast<Control*>(scale_ring + scale_ring_bytes(a.n_max));
   long long* bounds = reinterpret_cast<long long*>(ctl + 1);  // [shares + 1] in cost
@@ -309,12 +299,11 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int chunks = p.width / kChunk;
   constexpr int kOuts = kGated ? kTileRows : kTiles * kTileRows;  // of a tile
-  static_assert(!kGated || kTiles == 2, "gate and up");
   const int row_tiles = (p.outs + kOuts - 1) / kOuts;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.stages; ++i) {
-      mbar_init(&ctl->full[i], 2);  // rows and weights
+      mbar_init(&ctl->full[i], 1 + (p.src ? 32 * kRowWarps : 0));  // copies by TMA, row threads
       mbar_init(&ctl->empty[i], kTiles);
     }
     for (int i = 0; i < 2; ++i) {
@@ -364,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     long long tiles = 0;
     for (int e0 = 0; e0 <= p.experts; e0 += 32) {
       const int e = e0 + lane;
-      const Cut c = cut_group(e < p.experts ? offsets[e + 1] - offsets[e] : 0, a.n_max);
+      const Cut c = cut_group(e < p.experts ? offsets[e + 1] - offsets[e] : 0, a.n_max, chunks);
       tiles += c.tiles;
       const long long mine = static_cast<long long>(c.tiles) * row_tiles * chunks * c.cost;
       long long incl = mine;
@@ -382,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
       // Shares of a few chunks at least: a cut costs two fp32 parts, their
       // writing, meeting and reading.
       constexpr int kMinChunks = 4;
-      const long long most = run / (kMinChunks * kMemoryCost);
+      const long long most = run / (kMinChunks * 738);
       ctl->shares = most < 1 ? 1 : most < a.shares ? static_cast<int>(most) : a.shares;
       ctl->snap = tiles * row_tiles >= static_cast<long long>(kSnapTiles) * ctl->shares;
     }
@@ -398,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     long long b = total * c / shares;
     if (ctl->snap && c > 0 && c < shares) {
       const int e = group_at(prefix, p.experts, b);
-      const Cut g = cut_group(offsets[e + 1] - offsets[e], a.n_max);
+      const Cut g = cut_group(offsets[e + 1] - offsets[e], a.n_max, chunks);
       const unsigned tile = chunks * g.cost;
       b = prefix[e] + static_cast<long long>((static_cast<unsigned long long>(b - prefix[e]) + tile / 2) / tile) * tile;
     }
@@ -417,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
   walk.begin(prefix, me < shares ? bound(me) : 0, share_end);
   Piece piece;
   auto two_tiles = [&](const Piece& q) {
-    return kGated || (kTiles == 2 && q.row_tile * kOuts + kTileRows < p.outs);
+    return kGated || q.row_tile * kOuts + kTileRows < p.outs;
   };
 
   if (warp < kEpiWarps) {
@@ -432,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
       const long long start = share_end - walk.left;
       const int cost = walk.cut.cost;
       if (!walk.next(&piece)) break;
-      const bool big = kTiles == 2 && piece.n > kHalfN;
+      const bool big = piece.n > kHalfN;
       const int blocks = piece.n / kBlockCols;
       // this lane's row of a block: its weight, or its row of out
       auto lane_row = [&](int b) {
@@ -477,9 +466,9 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
         for (int r = side * 8; r < piece.n; r += 16) {
           uint32_t r0[8], r1[8];
           tmem_ld8(sums + r, r0);
-          if (kTiles == 2) tmem_ld8(sums1 + r, r1);  // (not used where there is no second tile)
+          tmem_ld8(sums1 + r, r1);  // (not used where there is no second tile)
           tmem_ld_wait8(r0);
-          if (kTiles == 2) tmem_ld_wait8(r1);
+          tmem_ld_wait8(r1);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             float* q = mine + static_cast<size_t>(r + i) * kTileRows;
@@ -503,46 +492,45 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
         if (!last) continue;
         __threadfence();
       }
-      // the sums of a block's 16 rows, this lane's output(s); from TMEM they are
-      // asked for a block ahead
-      uint32_t ahead0[16], ahead1[16];
-      if (!cut && side < blocks) {
-        tmem_ld16(sums + side * kBlockCols, ahead0);
-        if (kTiles == 2) tmem_ld16(sums1 + side * kBlockCols, ahead1);
-      }
-      auto take = [&](int b, float (&v0)[16], float (&v1)[16]) {
+      // the sums of 8 rows from r on, this lane's output(s)
+      auto take = [&](int r, float* v0, float* v1) {
         if (!cut) {
-          tmem_ld_wait16(ahead0);
-          if (kTiles == 2) tmem_ld_wait16(ahead1);
+          uint32_t r0[8], r1[8];
+          tmem_ld8(sums + r, r0);
+          tmem_ld8(sums1 + r, r1);
+          tmem_ld_wait8(r0);
+          tmem_ld_wait8(r1);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            v0[i] = __uint_as_float(ahead0[i]);
-            v1[i] = kTiles == 2 ? __uint_as_float(ahead1[i]) : 0.f;
-          }
-          if (b + 2 < blocks) {
-            tmem_ld16(sums + (b + 2) * kBlockCols, ahead0);
-            if (kTiles == 2) tmem_ld16(sums1 + (b + 2) * kBlockCols, ahead1);
+          for (int i = 0; i < 8; ++i) {
+            v0[i] = __uint_as_float(r0[i]);
+            v1[i] = __uint_as_float(r1[i]);
           }
           return;
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v0[i] = v1[i] = 0.f;
+        for (int i = 0; i < 8; ++i) v0[i] = v1[i] = 0.f;
+        // two parts at a time, added in their order
 #pragma unroll 1
-        for (int c = c0; c <= c1; ++c) {
-          if (chunk_at(bound(c) - start, chunks, cost) >= chunk_at(bound(c + 1) - start, chunks, cost))
-            continue;
-          const float* q = part_of(c) + static_cast<size_t>(b) * kBlockCols * kTileRows;
-          float x0[16], x1[16];
+        for (int c = c0; c <= c1; c += 2) {
+          float x[2][16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            x0[i] = __ldcg(q + i * kTileRows);
-            x1[i] = second ? __ldcg(q + tile_floats + i * kTileRows) : 0.f;
+          for (int k = 0; k < 2; ++k) {
+            const bool in = c + k <= c1 && chunk_at(bound(c + k) - start, chunks, cost) <
+                                               chunk_at(bound(c + k + 1) - start, chunks, cost);
+            const float* q = in ? part_of(c + k) + static_cast<size_t>(r) * kTileRows : nullptr;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              x[k][i] = in ? __ldcg(q + i * kTileRows) : 0.f;
+              x[k][8 + i] = in && second ? __ldcg(q + tile_floats + i * kTileRows) : 0.f;
+            }
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            v0[i] += x0[i];
-            v1[i] += x1[i];
-          }
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              v0[i] += x[k][i];
+              v1[i] += x[k][8 + i];
+            }
         }
       };
       // (not unrolled, nor in the parts above and below: what a piece runs once has
@@ -552,9 +540,10 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
       for (int b = side; b < blocks; b += 2) {
         const int row_data = row_next;
         row_next = lane_row(b + 2);
-        float v0[16], v1[16];
-        take(b, v0, v1);
         if (kGated) {
+          float v0[16], v1[16];
+          take(b * kBlockCols, v0, v1);
+          take(b * kBlockCols + 8, v0 + 8, v1 + 8);
           const int n = min(kBlockCols, piece.rows - b * kBlockCols);
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
@@ -599,8 +588,11 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
           flip ^= 1;
         } else {
           const int o0 = piece.row_tile * kOuts + at, o1 = o0 + kTileRows;
-          const bool in0 = o0 < p.outs, in1 = kTiles == 2 && o1 < p.outs;
-          {
+          const bool in0 = o0 < p.outs, in1 = o1 < p.outs;
+#pragma unroll 1
+          for (int r = 0; r < kBlockCols; r += 8) {
+            float v0[8], v1[8];
+            take(b * kBlockCols + r, v0, v1);
             if (a.wide) {
               // BF16, four outputs of a row a lane: pairs of rows as a word, and
               // two exchanges turn rows into outputs (half the time of stores
@@ -611,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
                 const float* v = t ? v1 : v0;
                 const int o = (t ? o1 : o0) - k;
 #pragma unroll
-                for (int j = 0; j < 16; j += 4) {
+                for (int j = 0; j < 8; j += 4) {
                   uint32_t w0 = pack_bf16x2(v[j], v[j + 1]), w1 = pack_bf16x2(v[j + 2], v[j + 3]);
                   // lane 2i: rows j and j + 2 of outputs 2i, 2i + 1; lane 2i + 1: the others
                   const uint32_t x0 = __shfl_xor_sync(0xffffffffu, w0, 1);
@@ -622,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
                   // lane 4i + k: row j + (k & 1) + (k & 2) of outputs 4i .. 4i + 3
                   const uint32_t y = __shfl_xor_sync(0xffffffffu, (k & 2) ? w0 : w1, 2);
                   const uint2 word = (k & 2) ? make_uint2(y, w1) : make_uint2(w0, y);
-                  const int d = __shfl_sync(0xffffffffu, row_data, j + k);
+                  const int d = __shfl_sync(0xffffffffu, row_data, r + j + k);
                   if (d >= 0 && o < p.outs)
                     *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + d * p.out_stride + o) = word;
                 }
@@ -635,13 +627,13 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
               };
               if (p.bf16) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                  put(static_cast<__nv_bfloat16*>(p.out), __shfl_sync(0xffffffffu, row_data, j),
+                for (int j = 0; j < 8; ++j)
+                  put(static_cast<__nv_bfloat16*>(p.out), __shfl_sync(0xffffffffu, row_data, r + j),
                       __float2bfloat16_rn(v0[j]), __float2bfloat16_rn(v1[j]));
               } else {
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                  put(static_cast<float*>(p.out), __shfl_sync(0xffffffffu, row_data, j), v0[j], v1[j]);
+                for (int j = 0; j < 8; ++j)
+                  put(static_cast<float*>(p.out), __shfl_sync(0xffffffffu, row_data, r + j), v0[j], v1[j]);
               }
             }
           }
@@ -785,58 +777,65 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     cp_async_wait<0>();
   } else if (warp < kWarpCopy) {
     // ---------------------------------------------------------------- rows
-    // One thread copies a tile's rows: rows in their order 16 at a time, others
-    // by gathers of four. (Copies of 16 bytes a thread moved 27 bytes a clock at
-    // most.)
-    int* table = row_table;
-    int s = 0;
+    // Rows that are not in their order (those that are come by TMA): 16 bytes a
+    // thread, eight threads a row, swizzled. (Gathers by TMA take 48 clocks for four
+    // rows; bringing the rows into their order first and copying them by TMA, beside
+    // the weights, 930 clocks a chunk of 48 rows where this takes 800.) The loop is short and asks for a row's number one copy
+    // ahead: with the numbers in registers and the loop unrolled it ran from the
+    // second-level instruction cache and took 800 clocks for 16 rows as for 192.
+    const int st = threadIdx.x - 32 * kWarpRows;
+    const uint8_t* x_from = p.xq + (st & 7) * 16;
+    const uint32_t x_to = kTiles * kATile + (st >> 3) * kChunk + (((st & 7) ^ ((st >> 3) & 7)) << 4);
+    Piece next;
+    int found[2];  // of the next piece, asked for while this one's are copied; -1: zeros
+    auto find_rows = [&] {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = st + i * 32 * kRowWarps;
+        int v = -1;
+        if (r < next.rows) v = p.src[next.row0 + r];
+        found[i] = v >= 0 && v < p.x_rows ? v : -1;
+      }
+    };
+    int s = 0, turn = 0;
     uint32_t phase = 1;
-    unsigned n = 0;
-    bool good = true;
-    while (walk.next(&piece)) {
-      if (p.src) {
-        for (int r = lane; r < piece.n; r += 32) {
-          int v = -1;  // outside the map: zeros
-          if (r < piece.rows) v = p.src[piece.row0 + r];
-          table[r] = v;
-        }
-        __syncwarp();
-      }
-      if (elect_one()) {
-        for (int c = piece.lo; c < piece.hi; ++c) {
-          good = good && wait_bar(&ctl->empty[s], phase, abort_flag, err);
-          if (!good) break;
-          uint8_t* to = smem + static_cast<size_t>(s) * stage_bytes(kTiles, a.n_max) + kTiles * kATile;
-          mbar_arrive_expect_tx(&ctl->full[s], piece.n * kChunk);
-          if (p.src) {
-            const int4* rows = reinterpret_cast<const int4*>(table);
-            int4 next = rows[0];
+    bool good = true, more = p.src && walk.next(&next);
+    if (more) find_rows();
+    while (more) {
+      int* table = row_table + turn * row_table_ints(a.n_max);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (st + i * 32 * kRowWarps < a.n_max) table[st + i * 32 * kRowWarps] = found[i];
+      bar_sync(5, 32 * kRowWarps);  // (two tables: nobody is two pieces behind)
+      piece = next;
+      more = walk.next(&next);
+      if (more) find_rows();
+      table += st >> 3;
+      const uint8_t* from = x_from + piece.lo * kChunk;
 #pragma unroll 1
-            for (int i = 4; i <= piece.n; i += 4) {
-              const int4 r = next;
-              ++rows;
-              if (i < piece.n) next = rows[0];
-              tma_gather4(to, &xmap, c * kChunk, r, &ctl->full[s]);
-              to += 4 * kChunk;
-            }
-          } else {
+      for (int c = piece.lo; c < piece.hi; ++c) {
+        good = good && wait_bar(&ctl->empty[s], phase, abort_flag, err);
+        if (good) {
+          uint32_t to = smem_addr(smem + static_cast<size_t>(s) * stage_bytes(a.n_max)) + x_to;
+          int ahead = table[0];
 #pragma unroll 1
-            for (int r = piece.row0; r < piece.row0 + piece.n; r += 16) {
-              tma_load_2d(to, &xmap, c * kChunk, r, &ctl->full[s]);
-              to += 16 * kChunk;
-            }
+          for (int r = 16; r <= piece.n; r += 16) {
+            const int row = ahead;
+            ahead = table[r];  // (one entry of 16 behind the tile's last row)
+            cp_async16_or_0(to, from + static_cast<size_t>(max(row, 0)) * p.width, row >= 0);
+            to += 16 * kChunk;
           }
-          ++n;
-          if (++s == a.stages) {
-            s = 0;
-            phase ^= 1;
-          }
+          cp_async_arrive(&ctl->full[s]);
         }
-        // after an abort: no copy may be under way when the block ends
-        if (!good && n > 0) mbar_wait(&ctl->full[(n - 1) % a.stages], ((n - 1) / a.stages) & 1, err);
+        from += kChunk;
+        if (++s == a.stages) {
+          s = 0;
+          phase ^= 1;
+        }
       }
-      __syncwarp();
+      turn ^= 1;
     }
+    cp_async_wait<0>();
   } else if (warp == kWarpCopy) {
     // -------------------------------------------------------------- copies
     if (lane == 0) {
@@ -850,15 +849,18 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
         // with what is read)
         constexpr int kTileTx = kFp8 ? kATile : kATile / 2;
         const int row = piece.row_tile * kOuts;
+        const int x_rows = p.src ? 0 : piece.n;
         for (int c = piece.lo; c < piece.hi; ++c) {
           good = wait_bar(&ctl->empty[s], phase, abort_flag, err);
           if (!good) break;
-          uint8_t* st = smem + static_cast<size_t>(s) * stage_bytes(kTiles, a.n_max);
-          mbar_arrive_expect_tx(&ctl->full[s], (second ? 2 : 1) * kTileTx);
+          uint8_t* st = smem + static_cast<size_t>(s) * stage_bytes(a.n_max);
+          mbar_arrive_expect_tx(&ctl->full[s], (second ? 2 : 1) * kTileTx + x_rows * kChunk);
           tma_load_3d(st, &map0, c * kChunk, row, piece.e, &ctl->full[s]);
           if (second)
             tma_load_3d(st + kATile, kGated ? &map1 : &map0, c * kChunk,
                         kGated ? row : row + kTileRows, piece.e, &ctl->full[s]);
+          for (int r = 0; r < x_rows; r += 16)
+            tma_load_2d(st + (kTiles * kTileRows + r) * kChunk, &xmap, c * kChunk, piece.row0 + r, &ctl->full[s]);
           ++n;
           if (++s == a.stages) {
             s = 0;
@@ -866,7 +868,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
           }
         }
       }
-      // after an abort: as above
+      // after an abort: no copy may be under way when the block ends
       if (!good)
         for (unsigned i = n < static_cast<unsigned>(a.stages) ? 0 : n - a.stages; i < n; ++i)
           mbar_wait(&ctl->full[i % a.stages], (i / a.stages) & 1, err);
@@ -879,7 +881,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     if (elect_one()) {
       const int tile = warp - kWarpMma;
       const uint32_t idesc0 = ((kFp8 ? 0u : 5u) << 7) | (1u << 23) | (8u << 24);
-      const uint32_t stage_step = stage_bytes(kTiles, a.n_max) >> 4;
+      const uint32_t stage_step = stage_bytes(a.n_max) >> 4;
       const uint32_t base0 = smem_addr(smem) >> 4;
       uint32_t base = base0;  // of the stage, in 16 bytes
       unsigned uses[2] = {0, 0}, scales = 0;
@@ -887,7 +889,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
       uint32_t phase = 0;
       bool good = true;
       while (good && walk.next(&piece)) {
-        const bool big = kTiles == 2 && piece.n > kHalfN, mine = tile == 0 || two_tiles(piece);
+        const bool big = piece.n > kHalfN, mine = tile == 0 || two_tiles(piece);
         const int h = big ? 0 : half;
         if (big) {
           good = wait_bar(&ctl->sum_empty[0], (uses[0]++ & 1) ^ 1, abort_flag, err) &&
@@ -910,6 +912,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
           if (!mbar_try_wait(&ctl->full[s], phase))
             good = good && wait_bar(&ctl->full[s], phase, abort_flag, err);
           if (!good) break;
+          fence_async_smem();  // the rows' copies are ordinary writes
           if (mine) {
             const uint32_t at = base + tile * (kATile >> 4), bt = base + kTiles * (kATile >> 4);
 #pragma unroll
@@ -947,25 +950,6 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                  "r"(kTmemCols)
                  : "memory");
-}
-
-// Rows src[r] of x and their scales one behind the other, zeros for rows that
-// are none. A block a row.
-__global__ void __launch_bounds__(128) gather_rows_kernel(const uint8_t* __restrict__ xq,
-                                                          const uint8_t* __restrict__ xs,
-                                                          const int* __restrict__ src, int x_rows,
-                                                          int width, uint8_t* __restrict__ yq,
-                                                          uint8_t* __restrict__ ys) {
-  pdl_wait();
-  pdl_trigger();
-  const size_t r = blockIdx.x;
-  const int v = src[r], groups = width / kChunk;
-  const bool there = v >= 0 && v < x_rows;
-  const size_t from = there ? v : 0;
-  const uint4* a = reinterpret_cast<const uint4*>(xq + from * width);
-  uint4* b = reinterpret_cast<uint4*>(yq + r * width);
-  for (int i = threadIdx.x; i < width / 16; i += 128) b[i] = there ? a[i] : make_uint4(0, 0, 0, 0);
-  for (int i = threadIdx.x; i < groups; i += 128) ys[r * groups + i] = there ? xs[from * groups + i] : 0x7F;
 }
 
 __global__ void grouped_reset_kernel(int* counters) {
@@ -1152,15 +1136,24 @@ int sm_count() {
 }
 
 struct Shape {
-  int tiles, n_max, stages;
+  int n_max, stages;
 };
 Shape tile_shape(const GroupedProblem& p) {
   const long long rows = p.rows, each = p.experts;  // rows of a group on average
-  const int n_max = rows <= 8 * each ? 16 : rows <= 24 * each ? 32 : rows <= 64 * each ? kHalfN : kMaxN;
-  const int tiles = p.w[1] == nullptr && n_max == kMaxN ? 1 : 2;
+  const int outs = p.w[1] ? kTileRows : kTiles * kTileRows;
+  // Small tiles for small groups leave more stages. Long sums make up for an
+  // epilogue that is not overlapped (8,192 tokens of 4096 x 2048: 2244 us, 2702
+  // with 96 rows), short ones do not (2048 rows of 1024: 135 us, 115 with 96).
+  int n_max = rows <= 8 * each ? 16 : rows <= 24 * each ? 32 : p.width >= 24 * kChunk ? kMaxN : kHalfN;
+  // Fewer rows a tile where there would be too few tiles: cutting one along its
+  // columns costs more (777 rows of 24 groups, 1003 outputs: 24 us, 39 with tiles
+  // of 96)
+  const long long row_tiles = (p.outs + outs - 1) / outs;
+  while (n_max > 32 && row_tiles * ((rows + n_max - 1) / n_max) < 2ll * sm_count())
+    n_max = n_max > kHalfN ? kHalfN : 32;
   int stages = kMaxStages;
-  while (smem_bytes(tiles, n_max, stages, p.experts) > kMaxSmem) --stages;
-  return {tiles, n_max, stages};
+  while (smem_bytes(n_max, stages, p.experts) > kMaxSmem) --stages;
+  return {n_max, stages};
 }
 
 size_t parts_bytes(const GroupedProblem& p) {
@@ -1169,21 +1162,6 @@ size_t parts_bytes(const GroupedProblem& p) {
 
 constexpr size_t kCounterBytes = kMaxShares * sizeof(int);
 
-size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
-
-// Rows that are not in their order are brought into it beforehand where a
-// group has more than a few: their copy by TMA gathers takes 48 clocks for four
-// rows, which the weights' copy covers up to some 16 rows a tile (32 tokens of
-// 7168 x 2048: 646 us, 655 with the copy).
-bool gathers_first(const GroupedProblem& p, bool has_src) {
-  return has_src && p.rows > 16ll * p.experts;
-}
-size_t gather_bytes(const GroupedProblem& p, bool has_src) {
-  if (!gathers_first(p, has_src)) return 0;
-  return up256(static_cast<size_t>(p.rows) * p.width) +
-         up256(static_cast<size_t>(p.rows) * (p.width / kChunk));
-}
-
 bool weight_map(CUtensorMap* m, const GroupedProblem& p, const uint8_t* w) {
   if (p.fp8)
     return make_tma_map_u8_3d(m, w, p.width, p.outs, p.width, p.experts,
@@ -1191,23 +1169,11 @@ bool weight_map(CUtensorMap* m, const GroupedProblem& p, const uint8_t* w) {
   return make_tma_map_u4_3d(m, w, p.width, p.outs, p.experts, kTileRows);
 }
 
-// gathered: gather_bytes() where the rows are brought into their order first.
-cudaError_t launch(GroupedProblem p, int* counters, float* parts, void* gathered, cudaStream_t st) {
+cudaError_t launch(const GroupedProblem& p, int* counters, float* parts, cudaStream_t st) {
   const bool gated = p.w[1] != nullptr;
-  if (gathers_first(p, p.src != nullptr)) {
-    uint8_t* yq = static_cast<uint8_t*>(gathered);
-    uint8_t* ys = yq + up256(static_cast<size_t>(p.rows) * p.width);
-    cudaError_t e = launch_pdl(gather_rows_kernel, dim3(p.rows), dim3(128), 0, st, p.xq, p.xs, p.src,
-                               p.x_rows, p.width, yq, ys);
-    if (e != cudaSuccess) return e;
-    p.xq = yq;
-    p.xs = ys;
-    p.src = nullptr;
-    p.x_rows = p.rows;
-  }
   CUtensorMap map0, map1, xmap;
   if (!weight_map(&map0, p, p.w[0]) || !weight_map(&map1, p, gated ? p.w[1] : p.w[0]) ||
-      !make_tma_map_u8(&xmap, p.xq, p.width, p.x_rows, kChunk, p.src ? 1 : 16, true, false))
+      !make_tma_map_u8(&xmap, p.xq, p.width, p.x_rows, kChunk, 16, true, false))
     return cudaErrorInvalidValue;
   Args a;
   a.p = p;
@@ -1221,13 +1187,12 @@ cudaError_t launch(GroupedProblem p, int* counters, float* parts, void* gathered
   a.parts = parts;
   if (a.shares < 1) return cudaErrorInvalidDevice;
   if (gated && p.fp8) return cudaErrorInvalidValue;
-  auto kernel = gated ? grouped_kernel<false, true, 2>
-                : s.tiles == 1 ? (p.fp8 ? grouped_kernel<true, false, 1> : grouped_kernel<false, false, 1>)
-                               : (p.fp8 ? grouped_kernel<true, false, 2> : grouped_kernel<false, false, 2>);
+  auto kernel = gated ? grouped_kernel<false, true>
+                      : p.fp8 ? grouped_kernel<true, false> : grouped_kernel<false, false>;
   cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), static_cast<int>(kMaxSmem));
   if (e != cudaSuccess) return e;
   return launch_pdl(kernel, dim3(a.shares), dim3(kThreads),
-                    smem_bytes(s.tiles, s.n_max, s.stages, p.experts), st, map0, map1, xmap, a);
+                    smem_bytes(s.n_max, s.stages, p.experts), st, map0, map1, xmap, a);
 }
 
 // Pieces of a buffer, 256-byte aligned.
@@ -1245,7 +1210,7 @@ struct Carver {
 struct ExpertsWork {
   int *counters, *offsets, *slot, *token;
   float *weight, *parts;
-  uint8_t *hq, *hs, *gathered;
+  uint8_t *hq, *hs;
   uint16_t* y;
   size_t bytes;
 };
@@ -1283,9 +1248,7 @@ ExpertsWork experts_work(const ExpertsProblem& p, void* base) {
   w.hq = c.take<uint8_t>(slots * p.inter);
   w.hs = c.take<uint8_t>(slots * (p.inter / 128));
   w.y = c.take<uint16_t>(slots * p.hidden);
-  const GroupedProblem g = gate_up(p, w);
-  w.parts = c.take<float>(parts_bytes(g) / sizeof(float));
-  w.gathered = c.take<uint8_t>(gather_bytes(g, true));
+  w.parts = c.take<float>(parts_bytes(gate_up(p, w)) / sizeof(float));
   w.bytes = c.used;
   return w;
 }
@@ -1293,7 +1256,7 @@ ExpertsWork experts_work(const ExpertsProblem& p, void* base) {
 }  // namespace
 
 size_t grouped_workspace_bytes(const GroupedProblem& p) {
-  return kCounterBytes + up256(parts_bytes(p)) + gather_bytes(p, true);  // should src be given
+  return kCounterBytes + parts_bytes(p);
 }
 
 cudaError_t grouped_reset(void* ws, cudaStream_t st) {
@@ -1302,8 +1265,8 @@ cudaError_t grouped_reset(void* ws, cudaStream_t st) {
 
 cudaError_t grouped_forward(const GroupedProblem& p, void* ws, cudaStream_t st) {
   if (p.rows <= 0) return cudaSuccess;
-  char* at = static_cast<char*>(ws) + kCounterBytes;
-  return launch(p, static_cast<int*>(ws), reinterpret_cast<float*>(at), at + up256(parts_bytes(p)), st);
+  return launch(p, static_cast<int*>(ws),
+                reinterpret_cast<float*>(static_cast<char*>(ws) + kCounterBytes), st);
 }
 
 size_t experts_workspace_bytes(const ExpertsProblem& p) { return experts_work(p, nullptr).bytes; }
@@ -1347,7 +1310,7 @@ cudaError_t experts_forward(const ExpertsProblem& p, void* ws, cudaStream_t st) 
   e = cudaLaunchKernelEx(&cfg, group_kernel, a);
   if (e != cudaSuccess) return e;
   const GroupedProblem g = gate_up(p, w);
-  e = launch(g, w.counters, w.parts, w.gathered, st);
+  e = launch(g, w.counters, w.parts, st);
   if (e != cudaSuccess) return e;
   GroupedProblem d;
   d.experts = p.experts;
@@ -1365,7 +1328,7 @@ cudaError_t experts_forward(const ExpertsProblem& p, void* ws, cudaStream_t st) 
   d.out = w.y;
   d.out_stride = p.hidden;
   d.err = p.err;
-  e = launch(d, w.counters + kMaxShares, w.parts, nullptr, st);
+  e = launch(d, w.counters + kMaxShares, w.parts, st);
   if (e != cudaSuccess) return e;
   const long long vecs = static_cast<long long>(p.n) * (p.hidden / 8);
   return launch_pdl(experts_combine_kernel, dim3(static_cast<unsigned>((vecs + 255) / 256)), dim3(256),
