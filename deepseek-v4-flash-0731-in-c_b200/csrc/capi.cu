@@ -1865,7 +1865,8 @@ bool experts_problem(const char* who, const dsv4cuda_moe_layer* L, int n, dsv4::
   }
   const dsv4::MoeConfig& c = L->cfg;
   const int experts = dsv4::moe_local_hi(c) - c.expert_lo;
-  if (c.hidden % 128 || c.moe_inter % 128 || experts < 1 || experts > dsv4::kGroupedMaxExperts ||
+  if (c.hidden % 128 || c.moe_inter % 128 || c.hidden > 1 << 20 || c.moe_inter > 1 << 20 ||
+      experts < 1 || experts > dsv4::kGroupedMaxExperts ||
       static_cast<long long>(n) * c.topk > 0x3FFFFFFFll ||
       static_cast<long long>(n) * (c.hidden / 8) > 0x7FFFFFFF00ll) {
     record_error("%s: hidden %d and moe_inter %d must be multiples of 128, experts 1..1024, routes "
@@ -1888,9 +1889,10 @@ bool experts_problem(const char* who, const dsv4cuda_moe_layer* L, int n, dsv4::
 bool grouped_problem(const char* who, const dsv4cuda_grouped_shape* s, dsv4::GroupedProblem* p) {
   if (!s || s->n_groups < 1 || s->n_groups > dsv4::kGroupedMaxExperts || s->n_rows < 0 ||
       s->n_rows > 0x3FFFFFFF || s->x_rows < 0 || s->out_rows < 0 || s->outs < 1 || s->width < 128 ||
-      s->width % 128 || s->outs > 0x3FFFFFFF || (s->out_stride && s->out_stride < s->outs)) {
-    record_error("%s: bad shape (1..1024 groups, width a multiple of 128, out_stride at least outs)",
-                 who);
+      s->width % 128 || s->width > 1 << 20 || s->outs > 0x3FFFFFFF ||
+      (s->out_stride && s->out_stride < s->outs)) {
+    record_error("%s: bad shape (1..1024 groups, width a multiple of 128 up to 2^20, out_stride at "
+                 "least outs)", who);
     return false;
   }
   p->experts = s->n_groups;

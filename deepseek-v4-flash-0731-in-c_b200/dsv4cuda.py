@@ -401,6 +401,7 @@ class MoeLayer:
         u8 = torch.uint8
         if xq.dim() != 2 or xq.shape[1] != self.hidden:
             raise ValueError(f"xq: [n][{self.hidden}] is wanted")
+        _here(xq, "xq")
         _check(lib.dsv4cuda_moe_experts(
             self.handle, _dev(xq, "xq", u8), _dev(xs, "xs", u8, n * (self.hidden // 128)),
             _dev(idx, "idx", torch.int32, n * self.topk), _dev(wt, "wt", torch.float32, n * self.topk),
@@ -677,6 +678,14 @@ def _dev(t, name, dtype, numel=None):
     return t.data_ptr()
 
 
+def _here(t, name):
+    """The calls launch on the current device: its tensors have to be there."""
+    import torch
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is cuda:"
+                         f"{torch.cuda.current_device()}")
+
+
 def _rows_of(t, name, shape, dtype):
     """Elements between the rows (0: of one row, or of none between them) of a CUDA tensor
     [rows][width] of `shape` and `dtype`."""
@@ -702,6 +711,7 @@ def _float_rows(t, name, width=None):
     if not (bf16 or dtype is torch.float32) or len(shape) != 2 or width not in (None, shape[1]):
         raise ValueError(f"{name}: a CUDA tensor [rows][{width or 'width'}] of bfloat16 or float32 is "
                          f"wanted, got {dtype} {list(shape)}")
+    _here(t, name)
     return dtype, 1 if bf16 else 0, shape
 
 
@@ -960,6 +970,7 @@ def _grouped_shape(out, xq, w, n_rows):
                          "the other")
     if out.shape[0] > 1 and out.stride(0) < outs:
         raise ValueError("out: the rows must not overlap")
+    _here(out, "out")
     return GroupedShape(groups, n_rows, xq.shape[0], out.shape[0], outs, width, int(held == width),
                         int(out.dtype is torch.bfloat16), out.stride(0) if out.shape[0] > 1 else 0)
 

@@ -292,7 +292,7 @@ int dsv4cuda_moe_experts(dsv4cuda_moe_layer *L, const uint8_t *xq, const uint8_t
  * groups may be empty. One group is a dense product. src, dst [n_rows] may be
  * NULL (row r); a src outside x_rows stands for zeros, a dst outside out_rows
  * is not written, nor are the rows of out that no dst names. width is a
- * multiple of 128. Weights: fp8 = 0 packed E2M1 (the low nibble first) with
+ * multiple of 128 up to 2^20. Weights: fp8 = 0 packed E2M1 (the low nibble first) with
  * E8M0 ws [n_groups][outs][width / 32]; fp8 = 1 E4M3 with ws
  * [n_groups][ceil(outs / 128)][width / 128]. x as above. out: BF16 or fp32, the
  * fp32 sums rounded once. Results are the same from call to call. DEVICE
