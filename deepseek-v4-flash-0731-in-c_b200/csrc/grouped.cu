@@ -69,7 +69,8 @@ struct alignas(16) Control {
   int abort_flag;
   int shares, snap;
   int last;      // the block brought a tile's last part
-  alignas(16) uint32_t top[2][2][4][kBlockCols];  // largest |h| of a warp's 32 outputs
+  alignas(16) float top[2][2][4][kBlockCols];  // largest |h| of a warp's 32 outputs
+  alignas(16) float factor[2][4][kBlockCols];  // rows' weights over their blocks' scales
   alignas(16) uint8_t codes[2][kBlockCols][kTileRows];
 };
 
@@ -139,6 +140,45 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
       "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
           smem_addr(bar))
       : "memory");
+}
+// 16 consecutive TMEM columns of this thread's lane, of two tiles.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+        "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_wait16(float (&r)[16], float (&s)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]),
+                 "+f"(r[6]), "+f"(r[7]), "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]),
+                 "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]), "+f"(s[0]), "+f"(s[1]),
+                 "+f"(s[2]), "+f"(s[3]), "+f"(s[4]), "+f"(s[5]), "+f"(s[6]), "+f"(s[7]),
+                 "+f"(s[8]), "+f"(s[9]), "+f"(s[10]), "+f"(s[11]), "+f"(s[12]), "+f"(s[13]),
+                 "+f"(s[14]), "+f"(s[15])::"memory");
+}
+// The smaller or larger of two, NaN if one is.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float a) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));
+  return r;
+}
+// The largest magnitude of a warp's, NaN if one is.
+__device__ __forceinline__ float warp_top(float a) {
+  float r;
+  asm volatile("redux.sync.max.abs.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(a));
+  return r;
 }
 // 8 consecutive TMEM columns of this thread's lane.
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
@@ -492,45 +532,33 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
         if (!last) continue;
         __threadfence();
       }
-      // the sums of 8 rows from r on, this lane's output(s)
-      auto take = [&](int r, float* v0, float* v1) {
+      // the sums of 16 rows from r on, this lane's output(s)
+      auto take = [&](int r, float (&v0)[16], float (&v1)[16]) {
         if (!cut) {
-          uint32_t r0[8], r1[8];
-          tmem_ld8(sums + r, r0);
-          tmem_ld8(sums1 + r, r1);
-          tmem_ld_wait8(r0);
-          tmem_ld_wait8(r1);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            v0[i] = __uint_as_float(r0[i]);
-            v1[i] = __uint_as_float(r1[i]);
-          }
+          tmem_ld16(sums + r, v0);
+          tmem_ld16(sums1 + r, v1);
+          tmem_ld_wait16(v0, v1);
           return;
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v0[i] = v1[i] = 0.f;
-        // two parts at a time, added in their order
+        for (int i = 0; i < 16; ++i) v0[i] = v1[i] = 0.f;
+        // the parts added in their order, all of one asked for at once
 #pragma unroll 1
-        for (int c = c0; c <= c1; c += 2) {
-          float x[2][16];
+        for (int c = c0; c <= c1; ++c) {
+          if (chunk_at(bound(c) - start, chunks, cost) >= chunk_at(bound(c + 1) - start, chunks, cost))
+            continue;
+          const float* q = part_of(c) + static_cast<size_t>(r) * kTileRows;
+          float x[32];
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const bool in = c + k <= c1 && chunk_at(bound(c + k) - start, chunks, cost) <
-                                               chunk_at(bound(c + k + 1) - start, chunks, cost);
-            const float* q = in ? part_of(c + k) + static_cast<size_t>(r) * kTileRows : nullptr;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              x[k][i] = in ? __ldcg(q + i * kTileRows) : 0.f;
-              x[k][8 + i] = in && second ? __ldcg(q + tile_floats + i * kTileRows) : 0.f;
-            }
+          for (int i = 0; i < 16; ++i) {
+            x[i] = __ldcg(q + i * kTileRows);
+            x[16 + i] = second ? __ldcg(q + tile_floats + i * kTileRows) : 0.f;
           }
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              v0[i] += x[k][i];
-              v1[i] += x[k][8 + i];
-            }
+          for (int i = 0; i < 16; ++i) {
+            v0[i] += x[i];
+            v1[i] += x[16 + i];
+          }
         }
       };
       // (not unrolled, nor in the parts above and below: what a piece runs once has
@@ -540,43 +568,57 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
       for (int b = side; b < blocks; b += 2) {
         const int row_data = row_next;
         row_next = lane_row(b + 2);
+        float v0[16], v1[16];
+        take(b * kBlockCols, v0, v1);
         if (kGated) {
-          float v0[16], v1[16];
-          take(b * kBlockCols, v0, v1);
-          take(b * kBlockCols + 8, v0 + 8, v1 + 8);
+          // A row's weight w is the same for all of its outputs, and rounding keeps an
+          // order: the block's largest |h| is the largest |silu u| times |w|, and w over
+          // the scale, a power of two, is one factor. So an output costs a limit, an
+          // exponential, a reciprocal, two products and a maximum.
           const int n = min(kBlockCols, piece.rows - b * kBlockCols);
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const float g = fminf(v0[j], p.limit), u = fminf(fmaxf(v1[j], -p.limit), p.limit);
-            const float y = __fdividef(g, 1.f + ex2_approx(-g * kLog2e)) * u *
-                            __int_as_float(__shfl_sync(0xffffffffu, row_data, j));
-            v0[j] = v0[j] != v0[j] || v1[j] != v1[j] ? NAN : y;  // (lost in the limits)
-            const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(v0[j]) & 0x7FFFFFFFu);
-            if (lane == j) ctl->top[side][flip][quarter][j] = top;
+            const float g = min_nan(v0[j], p.limit), u = min_nan(max_nan(v1[j], -p.limit), p.limit);
+            v0[j] = g * rcp_approx(1.f + ex2_approx(-g * kLog2e)) * u;
+            v1[j] = warp_top(v0[j]);
+          }
+          if (lane == 0) {
+            float4* top = reinterpret_cast<float4*>(ctl->top[side][flip][quarter]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              top[j] = make_float4(v1[4 * j], v1[4 * j + 1], v1[4 * j + 2], v1[4 * j + 3]);
           }
           bar_sync(2 + side, 128);
           // lane l of each warp: block's scale of row l
-          const uint32_t(*tops)[kBlockCols] = ctl->top[side][flip];
+          const float(*tops)[kBlockCols] = ctl->top[side][flip];
           const int l = lane & 15;
-          const uint32_t m = max(max(tops[0][l], tops[1][l]), max(tops[2][l], tops[3][l]));
+          const float w = __int_as_float(row_data);
+          const float m = max_nan(max_nan(tops[0][l], tops[1][l]), max_nan(tops[2][l], tops[3][l])) * fabsf(w);
           uint32_t e8 = 255;  // an infinity or NaN makes the block NaN
-          float inv = NAN;
-          if (m < 0x7F800000u) {
-            e8 = __float_as_uint(pow2_scale_448(__uint_as_float(m))) >> 23;
-            inv = __uint_as_float((254u - e8) << 23);
+          float factor = NAN;
+          if (m < INFINITY) {
+            e8 = __float_as_uint(pow2_scale_448(m)) >> 23;
+            // (w over the scale may pass the largest float where h does not)
+            factor = w * __uint_as_float((254u - e8) << 23);
+            factor = fminf(fmaxf(factor, -3.402823466e38f), 3.402823466e38f);
           }
+          if (lane < 16) ctl->factor[side][quarter][l] = factor;
           if (quarter == 0 && lane < n)
             p.hs[static_cast<size_t>(piece.row0 + b * kBlockCols + lane) * (p.outs / kTileRows) +
                  piece.row_tile] = static_cast<uint8_t>(e8);
+          __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 16; j += 2) {
-            unsigned short t;
-            asm("{ .reg .b16 h; cvt.rn.satfinite.e4m3x2.f32 h, %2, %1; mov.b16 %0, h; }"
-                : "=h"(t)
-                : "f"(v0[j] * __shfl_sync(0xffffffffu, inv, j)),
-                  "f"(v0[j + 1] * __shfl_sync(0xffffffffu, inv, j + 1)));
-            ctl->codes[side][j][at] = static_cast<uint8_t>(t);
-            ctl->codes[side][j + 1][at] = static_cast<uint8_t>(t >> 8);
+          for (int j = 0; j < 16; j += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(&ctl->factor[side][quarter][j]);
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+              unsigned short t;
+              asm("{ .reg .b16 h; cvt.rn.satfinite.e4m3x2.f32 h, %2, %1; mov.b16 %0, h; }"
+                  : "=h"(t)
+                  : "f"(v0[j + i] * (i ? f.z : f.x)), "f"(v0[j + i + 1] * (i ? f.w : f.y)));
+              ctl->codes[side][j + i][at] = static_cast<uint8_t>(t);
+              ctl->codes[side][j + i + 1][at] = static_cast<uint8_t>(t >> 8);
+            }
           }
           bar_sync(2 + side, 128);
           const int t = (threadIdx.x & 127) >> 3, v = threadIdx.x & 7;
@@ -589,10 +631,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
         } else {
           const int o0 = piece.row_tile * kOuts + at, o1 = o0 + kTileRows;
           const bool in0 = o0 < p.outs, in1 = o1 < p.outs;
-#pragma unroll 1
-          for (int r = 0; r < kBlockCols; r += 8) {
-            float v0[8], v1[8];
-            take(b * kBlockCols + r, v0, v1);
+          {
             if (a.wide) {
               // BF16, four outputs of a row a lane: pairs of rows as a word, and
               // two exchanges turn rows into outputs (half the time of stores
@@ -603,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
                 const float* v = t ? v1 : v0;
                 const int o = (t ? o1 : o0) - k;
 #pragma unroll
-                for (int j = 0; j < 8; j += 4) {
+                for (int j = 0; j < 16; j += 4) {
                   uint32_t w0 = pack_bf16x2(v[j], v[j + 1]), w1 = pack_bf16x2(v[j + 2], v[j + 3]);
                   // lane 2i: rows j and j + 2 of outputs 2i, 2i + 1; lane 2i + 1: the others
                   const uint32_t x0 = __shfl_xor_sync(0xffffffffu, w0, 1);
@@ -614,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
                   // lane 4i + k: row j + (k & 1) + (k & 2) of outputs 4i .. 4i + 3
                   const uint32_t y = __shfl_xor_sync(0xffffffffu, (k & 2) ? w0 : w1, 2);
                   const uint2 word = (k & 2) ? make_uint2(y, w1) : make_uint2(w0, y);
-                  const int d = __shfl_sync(0xffffffffu, row_data, r + j + k);
+                  const int d = __shfl_sync(0xffffffffu, row_data, j + k);
                   if (d >= 0 && o < p.outs)
                     *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + d * p.out_stride + o) = word;
                 }
@@ -627,13 +666,13 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
               };
               if (p.bf16) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  put(static_cast<__nv_bfloat16*>(p.out), __shfl_sync(0xffffffffu, row_data, r + j),
+                for (int j = 0; j < 16; ++j)
+                  put(static_cast<__nv_bfloat16*>(p.out), __shfl_sync(0xffffffffu, row_data, j),
                       __float2bfloat16_rn(v0[j]), __float2bfloat16_rn(v1[j]));
               } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  put(static_cast<float*>(p.out), __shfl_sync(0xffffffffu, row_data, r + j), v0[j], v1[j]);
+                for (int j = 0; j < 16; ++j)
+                  put(static_cast<float*>(p.out), __shfl_sync(0xffffffffu, row_data, j), v0[j], v1[j]);
               }
             }
           }
