@@ -67,7 +67,8 @@ struct alignas(16) Control {
   uint64_t fin;
   uint32_t tmem;
   int abort_flag;
-  int shares, snap;
+  int plan[2][kThreads / 32];  // of the warps
+  long long costs[kThreads / 32];
   int last;      // the block brought a tile's last part
   alignas(16) float top[2][2][4][kBlockCols];  // largest |h| of a warp's 32 outputs
   alignas(16) float factor[2][4][kBlockCols];  // rows' weights over their blocks' scales
@@ -231,12 +232,14 @@ struct Cut {
   int tiles, rows, cost;
 };
 constexpr int kSnapTiles = 8;  // shares of so many tiles on average are not cut
-__device__ __forceinline__ Cut cut_group(int n, int n_max, int chunks) {
+constexpr int kJoin = 8000;      // what a tile's parts take to meet, in clocks
+// (flat: shares are single tiles, and a chunk counts 1)
+__device__ __forceinline__ Cut cut_group(int n, int n_max, int chunks, bool flat) {
   Cut c;
   c.tiles = (n + n_max - 1) / n_max;
   c.rows = c.tiles ? ((n + c.tiles - 1) / c.tiles + 15) & ~15 : 16;
   c.tiles = c.tiles ? (n + c.rows - 1) / c.rows : 0;
-  c.cost = 690 + 3 * c.rows + (c.rows > kHalfN ? 67 * c.rows / chunks : 0);
+  c.cost = flat ? 1 : 690 + 3 * c.rows + (c.rows > kHalfN ? 67 * c.rows / chunks : 0);
   return c;
 }
 
@@ -275,13 +278,13 @@ struct Walk {
   int e, row_tile, t, lo;   // the next piece
   long long left;           // from its tile's start to the share's end, in cost
 
-  __device__ __forceinline__ void recut() { cut = cut_group(offsets[e + 1] - offsets[e], n_max, chunks); }
+  __device__ __forceinline__ void recut(bool flat) { cut = cut_group(offsets[e + 1] - offsets[e], n_max, chunks, flat); }
   // prefix [experts + 1]: cost before each group; the share is b0 .. b1.
-  __device__ __forceinline__ void begin(const long long* prefix, long long b0, long long b1) {
+  __device__ __forceinline__ void begin(const long long* prefix, long long b0, long long b1, bool flat) {
     left = 0;
     if (b0 >= b1) return;
     e = group_at(prefix, experts, b0);
-    recut();
+    recut(flat);
     const long long tile = static_cast<long long>(chunks) * cut.cost, d = b0 - prefix[e];
     const int item = static_cast<int>(d / tile);
     row_tile = item / cut.tiles;
@@ -312,7 +315,7 @@ struct Walk {
       if (++row_tile == row_tiles && left > 0) {
         row_tile = 0;
         do ++e; while (e + 1 < experts && offsets[e + 1] == offsets[e]);
-        recut();
+        recut(false);  // (a flat share is one tile)
         if (cut.tiles == 0) left = 0;
       }
     }
@@ -374,60 +377,85 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
   for (int e = threadIdx.x; e <= p.experts; e += kThreads)
     offsets[e] = min(max(p.offsets[e], 0), p.rows);
   __syncthreads();
-  if (warp == 0) {
-    long long run = 0;
-    int at = 0;  // offsets in ascending order
-    for (int e0 = 0; e0 <= p.experts; e0 += 32) {
-      const int e = e0 + lane;
-      int o = e <= p.experts ? offsets[e] : p.rows;
-      o = max(o, at);
+  // A thread an expert: offsets in ascending order, and how many tiles there are.
+  // (One warp took some 4 us for 256 experts.)
+  int tiles = 0, widest = 0;
+  for (int e0 = 0, at = 0; e0 <= p.experts; e0 += kThreads) {
+    const int e = e0 + threadIdx.x;
+    int o = e <= p.experts ? offsets[e] : 0;
 #pragma unroll
-      for (int s = 1; s < 32; s <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, o, s);
-        if (lane >= s) o = max(o, u);
-      }
-      if (e <= p.experts) offsets[e] = o;
-      at = __shfl_sync(0xffffffffu, o, 31);
+    for (int s = 1; s < 32; s <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, o, s);
+      if (lane >= s) o = max(o, u);
     }
-    __syncwarp();
-    long long tiles = 0;
-    for (int e0 = 0; e0 <= p.experts; e0 += 32) {
-      const int e = e0 + lane;
-      const Cut c = cut_group(e < p.experts ? offsets[e + 1] - offsets[e] : 0, a.n_max, chunks);
-      tiles += c.tiles;
-      const long long mine = static_cast<long long>(c.tiles) * row_tiles * chunks * c.cost;
-      long long incl = mine;
-#pragma unroll
-      for (int s = 1; s < 32; s <<= 1) {
-        const long long u = __shfl_up_sync(0xffffffffu, incl, s);
-        if (lane >= s) incl += u;
-      }
-      if (e <= p.experts) prefix[e] = run + incl - mine;
-      run += __shfl_sync(0xffffffffu, incl, 31);
-    }
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, s);
-    if (lane == 0) {
-      // Shares of a few chunks at least: a cut costs two fp32 parts, their
-      // writing, meeting and reading.
-      constexpr int kMinChunks = 4;
-      const long long most = run / (kMinChunks * 738);
-      ctl->shares = most < 1 ? 1 : most < a.shares ? static_cast<int>(most) : a.shares;
-      ctl->snap = tiles * row_tiles >= static_cast<long long>(kSnapTiles) * ctl->shares;
-    }
+    if (lane == 31) ctl->plan[0][warp] = o;
+    __syncthreads();
+    const int other = lane < kThreads / 32 ? ctl->plan[0][lane] : 0;
+    o = max(max(o, at), __reduce_max_sync(0xffffffffu, lane < warp ? other : 0));
+    at = max(at, __reduce_max_sync(0xffffffffu, other));
+    if (e <= p.experts) offsets[e] = o;
+    __syncthreads();
   }
+  for (int e = threadIdx.x; e < p.experts; e += kThreads) {
+    const Cut c = cut_group(offsets[e + 1] - offsets[e], a.n_max, chunks, false);
+    tiles += c.tiles;
+    if (c.tiles) widest = max(widest, c.cost);
+  }
+  tiles = __reduce_add_sync(0xffffffffu, tiles);
+  widest = __reduce_max_sync(0xffffffffu, widest);
+  if (lane == 0) {
+    ctl->plan[0][warp] = tiles;
+    ctl->plan[1][warp] = widest;
+  }
+  __syncthreads();
+  tiles = __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? ctl->plan[0][lane] : 0);
+  widest = __reduce_max_sync(0xffffffffu, lane < kThreads / 32 ? ctl->plan[1][lane] : 0);
+  // No more tiles than blocks: a block each, without cuts, where the largest
+  // takes no longer than an equal share and the parts' meeting.
+  const long long all_tiles = static_cast<long long>(tiles) * row_tiles;
+  const bool flat = all_tiles <= a.shares &&
+                    widest * chunks * (a.shares - all_tiles) <= static_cast<long long>(kJoin) * a.shares;
+  // Cost before each group.
+  long long run = 0;
+  for (int e0 = 0; e0 <= p.experts; e0 += kThreads) {
+    const int e = e0 + threadIdx.x;
+    const Cut c = cut_group(e < p.experts ? offsets[e + 1] - offsets[e] : 0, a.n_max, chunks, flat);
+    const long long mine = static_cast<long long>(c.tiles) * row_tiles * chunks * c.cost;
+    long long incl = mine;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, incl, s);
+      if (lane >= s) incl += u;
+    }
+    if (lane == 31) ctl->costs[warp] = incl;
+    __syncthreads();
+    long long before = run;
+#pragma unroll 4
+    for (int w = 0; w < kThreads / 32; ++w) {
+      const long long c = ctl->costs[w];
+      if (w < warp) before += c;
+      run += c;
+    }
+    if (e <= p.experts) prefix[e] = before + incl - mine;
+    __syncthreads();
+  }
+  // Otherwise shares of a few chunks at least: a cut costs two fp32 parts, their
+  // writing, meeting and reading.
+  constexpr int kMinChunks = 4;
+  const long long most = flat ? all_tiles : run / (kMinChunks * 738);
+  const int shares = most < 1 ? 1 : most < a.shares ? static_cast<int>(most) : a.shares;
+  const bool snap = all_tiles >= static_cast<long long>(kSnapTiles) * shares;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ctl->tmem;
-  const int shares = ctl->shares;
   // Where each share begins. Shares of many tiles take whole ones.
   for (int c = threadIdx.x; c <= shares; c += kThreads) {
     const long long total = prefix[p.experts];
     long long b = total * c / shares;
-    if (ctl->snap && c > 0 && c < shares) {
+    if (snap && c > 0 && c < shares) {
       const int e = group_at(prefix, p.experts, b);
-      const Cut g = cut_group(offsets[e + 1] - offsets[e], a.n_max, chunks);
+      const Cut g = cut_group(offsets[e + 1] - offsets[e], a.n_max, chunks, flat);
       const unsigned tile = chunks * g.cost;
       b = prefix[e] + static_cast<long long>((static_cast<unsigned long long>(b - prefix[e]) + tile / 2) / tile) * tile;
     }
@@ -443,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
   walk.chunks = chunks;
   walk.n_max = a.n_max;
   const long long share_end = me < shares ? bound(me + 1) : 0;
-  walk.begin(prefix, me < shares ? bound(me) : 0, share_end);
+  walk.begin(prefix, me < shares ? bound(me) : 0, share_end, flat);
   Piece piece;
   auto two_tiles = [&](const Piece& q) {
     return kGated || q.row_tile * kOuts + kTileRows < p.outs;
@@ -503,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
       if (cut) {
         float* mine = part_of(me);
 #pragma unroll 1
-        for (int r = side * 8; r < piece.n; r += 16) {
+        for (int r = side * 8; r < piece.rows; r += 16) {
           uint32_t r0[8], r1[8];
           tmem_ld8(sums + r, r0);
           tmem_ld8(sums1 + r, r1);  // (not used where there is no second tile)
@@ -511,6 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
           tmem_ld_wait8(r1);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
+            if (r + i >= piece.rows) break;
             float* q = mine + static_cast<size_t>(r + i) * kTileRows;
             __stcg(q, __uint_as_float(r0[i]));
             if (second) __stcg(q + tile_floats, __uint_as_float(r1[i]));
@@ -551,8 +580,9 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
           float x[32];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            x[i] = __ldcg(q + i * kTileRows);
-            x[16 + i] = second ? __ldcg(q + tile_floats + i * kTileRows) : 0.f;
+            const bool in = r + i < piece.rows;
+            x[i] = in ? __ldcg(q + i * kTileRows) : 0.f;
+            x[16 + i] = in && second ? __ldcg(q + tile_floats + i * kTileRows) : 0.f;
           }
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
