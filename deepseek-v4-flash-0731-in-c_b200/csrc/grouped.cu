@@ -53,6 +53,7 @@ constexpr size_t kMaxSmem = 227 * 1024;
 
 struct Args {
   GroupedProblem p;
+  bool early;         // offsets are of a kernel that the one before this has waited for
   int shares;         // blocks
   int n_max, stages;  // rows of a tile; stages of the ring
   bool wide;          // out is BF16 and takes four outputs of a row at once
@@ -232,13 +233,19 @@ struct Cut {
   int tiles, rows, cost;
 };
 constexpr int kSnapTiles = 8;  // shares of so many tiles on average are not cut
-constexpr int kJoin = 8000;      // what a tile's parts take to meet, in clocks
+constexpr int kJoin = 20000;      // what a tile's parts take to meet, in clocks
 // (flat: shares are single tiles, and a chunk counts 1)
 __device__ __forceinline__ Cut cut_group(int n, int n_max, int chunks, bool flat) {
   Cut c;
-  c.tiles = (n + n_max - 1) / n_max;
-  c.rows = c.tiles ? ((n + c.tiles - 1) / c.tiles + 15) & ~15 : 16;
-  c.tiles = c.tiles ? (n + c.rows - 1) / c.rows : 0;
+  const int sixteens = (n + 15) >> 4, most = n_max >> 4;
+  c.tiles = n > 0;
+  int each = max(sixteens, 1);
+  if (sixteens > most) {  // (three divisions: 500 clocks that most groups need not wait for)
+    c.tiles = (sixteens + most - 1) / most;
+    each = (sixteens + c.tiles - 1) / c.tiles;
+    c.tiles = (sixteens + each - 1) / each;
+  }
+  c.rows = each * 16;
   c.cost = flat ? 1 : 690 + 3 * c.rows + (c.rows > kHalfN ? 67 * c.rows / chunks : 0);
   return c;
 }
@@ -249,6 +256,16 @@ struct Piece {
   int row0, rows, n;   // first row of the tile, rows there are, columns of the MMAs
   int lo, hi;          // chunks
 };
+
+// d / by, quotients of a few million at most off by a handful at first: a
+// fraction of what a division of 64 bits takes.
+__device__ __forceinline__ int quotient(long long d, long long by) {
+  int q = static_cast<int>(static_cast<float>(d) * __frcp_rn(static_cast<float>(by)));
+  long long rest = d - q * by;
+  while (rest < 0) rest += by, --q;
+  while (rest >= by) rest -= by, ++q;
+  return q;
+}
 
 // The chunk of a tile of `cost` a chunk in which position d behind its start lies.
 __device__ __forceinline__ int chunk_at(long long d, int chunks, int cost) {
@@ -286,8 +303,8 @@ struct Walk {
     e = group_at(prefix, experts, b0);
     recut(flat);
     const long long tile = static_cast<long long>(chunks) * cut.cost, d = b0 - prefix[e];
-    const int item = static_cast<int>(d / tile);
-    row_tile = item / cut.tiles;
+    const int item = quotient(d, tile);
+    row_tile = cut.tiles == 1 ? item : item / cut.tiles;
     t = item - row_tile * cut.tiles;
     const long long start = prefix[e] + item * tile;
     lo = chunk_at(b0 - start, chunks, cut.cost);
@@ -371,11 +388,24 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  pdl_wait();  // offsets, rows and counters of the kernels before
-  pdl_trigger();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl->tmem;
+  const int me = blockIdx.x;
+  Walk walk;
+  walk.offsets = offsets;
+  walk.experts = p.experts;
+  walk.row_tiles = row_tiles;
+  walk.chunks = chunks;
+  walk.n_max = a.n_max;
+  // The plan. (Its 4 us are mostly code that a block runs once, from beyond the
+  // instruction caches; a rehearsal while the kernel before runs only delayed the
+  // blocks that start late.)
+  if (!a.early) pdl_wait();  // offsets, rows and counters of the kernels before
   // offsets that are out of order or beyond `rows` leave groups empty
   for (int e = threadIdx.x; e <= p.experts; e += kThreads)
-    offsets[e] = min(max(p.offsets[e], 0), p.rows);
+    offsets[e] = min(max(__ldcg(p.offsets + e), 0), p.rows);
   __syncthreads();
   // A thread an expert: offsets in ascending order, and how many tiles there are.
   // (One warp took some 4 us for 256 experts.)
@@ -396,10 +426,14 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     if (e <= p.experts) offsets[e] = o;
     __syncthreads();
   }
-  for (int e = threadIdx.x; e < p.experts; e += kThreads) {
-    const Cut c = cut_group(offsets[e + 1] - offsets[e], a.n_max, chunks, false);
-    tiles += c.tiles;
-    if (c.tiles) widest = max(widest, c.cost);
+  constexpr int kEach = (kGroupedMaxExperts + 1 + kThreads - 1) / kThreads;
+  Cut cuts[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int e = i * kThreads + threadIdx.x;
+    cuts[i] = cut_group(e < p.experts ? offsets[e + 1] - offsets[e] : 0, a.n_max, chunks, false);
+    tiles += cuts[i].tiles;
+    if (cuts[i].tiles) widest = max(widest, cuts[i].cost);
   }
   tiles = __reduce_add_sync(0xffffffffu, tiles);
   widest = __reduce_max_sync(0xffffffffu, widest);
@@ -417,10 +451,12 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
                     widest * chunks * (a.shares - all_tiles) <= static_cast<long long>(kJoin) * a.shares;
   // Cost before each group.
   long long run = 0;
-  for (int e0 = 0; e0 <= p.experts; e0 += kThreads) {
-    const int e = e0 + threadIdx.x;
-    const Cut c = cut_group(e < p.experts ? offsets[e + 1] - offsets[e] : 0, a.n_max, chunks, flat);
-    const long long mine = static_cast<long long>(c.tiles) * row_tiles * chunks * c.cost;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    if (i * kThreads > p.experts) break;
+    const int e = i * kThreads + threadIdx.x;
+    const long long mine =
+        static_cast<long long>(cuts[i].tiles) * row_tiles * (chunks * (flat ? 1 : cuts[i].cost));
     long long incl = mine;
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
@@ -429,13 +465,15 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     }
     if (lane == 31) ctl->costs[warp] = incl;
     __syncthreads();
-    long long before = run;
-#pragma unroll 4
-    for (int w = 0; w < kThreads / 32; ++w) {
-      const long long c = ctl->costs[w];
-      if (w < warp) before += c;
-      run += c;
-    }
+    // (sums of the warps by 26 and by 38 bits)
+    const long long other = lane < kThreads / 32 ? ctl->costs[lane] : 0;
+    const unsigned low = other & 0x3FFFFFF, high = static_cast<unsigned>(other >> 26);
+    auto sum = [&](bool in) {
+      return __reduce_add_sync(0xffffffffu, in ? low : 0u) +
+             (static_cast<long long>(__reduce_add_sync(0xffffffffu, in ? high : 0u)) << 26);
+    };
+    const long long before = run + sum(lane < warp);
+    run += sum(true);
     if (e <= p.experts) prefix[e] = before + incl - mine;
     __syncthreads();
   }
@@ -445,10 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
   const long long most = flat ? all_tiles : run / (kMinChunks * 738);
   const int shares = most < 1 ? 1 : most < a.shares ? static_cast<int>(most) : a.shares;
   const bool snap = all_tiles >= static_cast<long long>(kSnapTiles) * shares;
-  tc_fence_before();
   __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = ctl->tmem;
   // Where each share begins. Shares of many tiles take whole ones.
   for (int c = threadIdx.x; c <= shares; c += kThreads) {
     const long long total = prefix[p.experts];
@@ -462,16 +497,11 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     bounds[c] = b;
   }
   __syncthreads();
-  auto bound = [&](int c) { return bounds[c]; };  // c <= shares
-  const int me = blockIdx.x;
-  Walk walk;
-  walk.offsets = offsets;
-  walk.experts = p.experts;
-  walk.row_tiles = row_tiles;
-  walk.chunks = chunks;
-  walk.n_max = a.n_max;
-  const long long share_end = me < shares ? bound(me + 1) : 0;
-  walk.begin(prefix, me < shares ? bound(me) : 0, share_end, flat);
+  const long long share_end = me < shares ? bounds[me + 1] : 0;
+  walk.begin(prefix, me < shares ? bounds[me] : 0, share_end, flat);
+  if (a.early) pdl_wait();
+  pdl_trigger();
+  auto bound = [&](int c) { return bounds[c]; };
   Piece piece;
   auto two_tiles = [&](const Piece& q) {
     return kGated || q.row_tile * kOuts + kTileRows < p.outs;
@@ -580,9 +610,8 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
           float x[32];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const bool in = r + i < piece.rows;
-            x[i] = in ? __ldcg(q + i * kTileRows) : 0.f;
-            x[16 + i] = in && second ? __ldcg(q + tile_floats + i * kTileRows) : 0.f;
+            x[i] = __ldcg(q + i * kTileRows);  // (what is behind the tile's rows is not used)
+            x[16 + i] = second ? __ldcg(q + tile_floats + i * kTileRows) : 0.f;
           }
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -1238,7 +1267,7 @@ bool weight_map(CUtensorMap* m, const GroupedProblem& p, const uint8_t* w) {
   return make_tma_map_u4_3d(m, w, p.width, p.outs, p.experts, kTileRows);
 }
 
-cudaError_t launch(const GroupedProblem& p, int* counters, float* parts, cudaStream_t st) {
+cudaError_t launch(const GroupedProblem& p, bool early, int* counters, float* parts, cudaStream_t st) {
   const bool gated = p.w[1] != nullptr;
   CUtensorMap map0, map1, xmap;
   if (!weight_map(&map0, p, p.w[0]) || !weight_map(&map1, p, gated ? p.w[1] : p.w[0]) ||
@@ -1246,6 +1275,7 @@ cudaError_t launch(const GroupedProblem& p, int* counters, float* parts, cudaStr
     return cudaErrorInvalidValue;
   Args a;
   a.p = p;
+  a.early = early;
   a.shares = sm_count();
   const Shape s = tile_shape(p);
   a.n_max = s.n_max;
@@ -1334,7 +1364,7 @@ cudaError_t grouped_reset(void* ws, cudaStream_t st) {
 
 cudaError_t grouped_forward(const GroupedProblem& p, void* ws, cudaStream_t st) {
   if (p.rows <= 0) return cudaSuccess;
-  return launch(p, static_cast<int*>(ws),
+  return launch(p, false, static_cast<int*>(ws),
                 reinterpret_cast<float*>(static_cast<char*>(ws) + kCounterBytes), st);
 }
 
@@ -1379,7 +1409,7 @@ cudaError_t experts_forward(const ExpertsProblem& p, void* ws, cudaStream_t st) 
   e = cudaLaunchKernelEx(&cfg, group_kernel, a);
   if (e != cudaSuccess) return e;
   const GroupedProblem g = gate_up(p, w);
-  e = launch(g, w.counters, w.parts, st);
+  e = launch(g, false, w.counters, w.parts, st);
   if (e != cudaSuccess) return e;
   GroupedProblem d;
   d.experts = p.experts;
@@ -1397,7 +1427,7 @@ cudaError_t experts_forward(const ExpertsProblem& p, void* ws, cudaStream_t st) 
   d.out = w.y;
   d.out_stride = p.hidden;
   d.err = p.err;
-  e = launch(d, w.counters + kMaxShares, w.parts, st);
+  e = launch(d, true, w.counters + kMaxShares, w.parts, st);
   if (e != cudaSuccess) return e;
   const long long vecs = static_cast<long long>(p.n) * (p.hidden / 8);
   return launch_pdl(experts_combine_kernel, dim3(static_cast<unsigned>((vecs + 255) / 256)), dim3(256),
