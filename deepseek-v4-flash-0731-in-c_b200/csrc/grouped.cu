@@ -55,7 +55,7 @@ struct Args {
   GroupedProblem p;
   bool early;         // offsets are of a kernel that the one before this has waited for
   int shares;         // blocks
-  int n_max, stages;  // rows of a tile; stages of the ring
+  int n_max, stages;  // rows of a tile at most; stages of the ring that hold so many
   bool wide;          // out is BF16 and takes four outputs of a row at once
   int* counters;      // [kMaxShares] chunks whose parts are there
   float* parts;       // [shares][2][2][n_max][128]
@@ -68,7 +68,7 @@ struct alignas(16) Control {
   uint64_t fin;
   uint32_t tmem;
   int abort_flag;
-  int plan[2][kThreads / 32];  // of the warps
+  int plan[3][kThreads / 32];  // of the warps
   long long costs[kThreads / 32];
   int last;      // the block brought a tile's last part
   alignas(16) float top[2][2][4][kBlockCols];  // largest |h| of a warp's 32 outputs
@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
   const int row_tiles = (p.outs + kOuts - 1) / kOuts;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < a.stages; ++i) {
+    for (int i = 0; i < kMaxStages; ++i) {
       mbar_init(&ctl->full[i], 1 + (p.src ? 32 * kRowWarps : 0));  // copies by TMA, row threads
       mbar_init(&ctl->empty[i], kTiles);
     }
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
   __syncthreads();
   // A thread an expert: offsets in ascending order, and how many tiles there are.
   // (One warp took some 4 us for 256 experts.)
-  int tiles = 0, widest = 0;
+  int tiles = 0, widest = 0, tallest = 16;
   for (int e0 = 0, at = 0; e0 <= p.experts; e0 += kThreads) {
     const int e = e0 + threadIdx.x;
     int o = e <= p.experts ? offsets[e] : 0;
@@ -434,16 +434,24 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     cuts[i] = cut_group(e < p.experts ? offsets[e + 1] - offsets[e] : 0, a.n_max, chunks, false);
     tiles += cuts[i].tiles;
     if (cuts[i].tiles) widest = max(widest, cuts[i].cost);
+    tallest = max(tallest, cuts[i].rows);
   }
   tiles = __reduce_add_sync(0xffffffffu, tiles);
   widest = __reduce_max_sync(0xffffffffu, widest);
+  tallest = __reduce_max_sync(0xffffffffu, tallest);
   if (lane == 0) {
     ctl->plan[0][warp] = tiles;
     ctl->plan[1][warp] = widest;
+    ctl->plan[2][warp] = tallest;
   }
   __syncthreads();
   tiles = __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? ctl->plan[0][lane] : 0);
   widest = __reduce_max_sync(0xffffffffu, lane < kThreads / 32 ? ctl->plan[1][lane] : 0);
+  tallest = __reduce_max_sync(0xffffffffu, lane < kThreads / 32 ? ctl->plan[2][lane] : 0);
+  // The ring in stages for the rows that the largest tile has.
+  const int stage = stage_bytes(tallest);
+  int stages = a.stages;
+  while (stages < kMaxStages && (stages + 1) * stage <= a.stages * stage_bytes(a.n_max)) ++stages;
   // No more tiles than blocks: a block each, without cuts, where the largest
   // takes no longer than an equal share and the parts' meeting.
   const long long all_tiles = static_cast<long long>(tiles) * row_tiles;
@@ -914,7 +922,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
       for (int c = piece.lo; c < piece.hi; ++c) {
         good = good && wait_bar(&ctl->empty[s], phase, abort_flag, err);
         if (good) {
-          uint32_t to = smem_addr(smem + static_cast<size_t>(s) * stage_bytes(a.n_max)) + x_to;
+          uint32_t to = smem_addr(smem + s * stage) + x_to;
           int ahead = table[0];
 #pragma unroll 1
           for (int r = 16; r <= piece.n; r += 16) {
@@ -926,7 +934,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
           cp_async_arrive(&ctl->full[s]);
         }
         from += kChunk;
-        if (++s == a.stages) {
+        if (++s == stages) {
           s = 0;
           phase ^= 1;
         }
@@ -951,7 +959,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
         for (int c = piece.lo; c < piece.hi; ++c) {
           good = wait_bar(&ctl->empty[s], phase, abort_flag, err);
           if (!good) break;
-          uint8_t* st = smem + static_cast<size_t>(s) * stage_bytes(a.n_max);
+          uint8_t* st = smem + s * stage;
           mbar_arrive_expect_tx(&ctl->full[s], (second ? 2 : 1) * kTileTx + x_rows * kChunk);
           tma_load_3d(st, &map0, c * kChunk, row, piece.e, &ctl->full[s]);
           if (second)
@@ -960,7 +968,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
           for (int r = 0; r < x_rows; r += 16)
             tma_load_2d(st + (kTiles * kTileRows + r) * kChunk, &xmap, c * kChunk, piece.row0 + r, &ctl->full[s]);
           ++n;
-          if (++s == a.stages) {
+          if (++s == stages) {
             s = 0;
             phase ^= 1;
           }
@@ -968,8 +976,8 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
       }
       // after an abort: no copy may be under way when the block ends
       if (!good)
-        for (unsigned i = n < static_cast<unsigned>(a.stages) ? 0 : n - a.stages; i < n; ++i)
-          mbar_wait(&ctl->full[i % a.stages], (i / a.stages) & 1, err);
+        for (unsigned i = n < static_cast<unsigned>(stages) ? 0 : n - stages; i < n; ++i)
+          mbar_wait(&ctl->full[i % stages], (i / stages) & 1, err);
     }
     __syncwarp();
   } else if (warp < kWarpMma + kTiles) {
@@ -979,7 +987,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     if (elect_one()) {
       const int tile = warp - kWarpMma;
       const uint32_t idesc0 = ((kFp8 ? 0u : 5u) << 7) | (1u << 23) | (8u << 24);
-      const uint32_t stage_step = stage_bytes(a.n_max) >> 4;
+      const uint32_t stage_step = stage >> 4;
       const uint32_t base0 = smem_addr(smem) >> 4;
       uint32_t base = base0;  // of the stage, in 16 bytes
       unsigned uses[2] = {0, 0}, scales = 0;
@@ -1026,7 +1034,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
             ++scales;
           }
           base += stage_step;
-          if (++s == a.stages) {
+          if (++s == stages) {
             s = 0;
             base = base0;
             phase ^= 1;
