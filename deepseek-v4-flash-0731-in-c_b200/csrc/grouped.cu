@@ -44,7 +44,7 @@ constexpr int kWarpMma = kWarpCopy + 1;  // and the next, for a second tile
 constexpr int kThreads = 32 * (kWarpMma + 2);
 constexpr int kBlockCols = 16;           // rows of a group that an epilogue step takes
 constexpr int kMaxN = 192, kHalfN = 96;  // rows of a tile; up to kHalfN two tiles' sums fit in TMEM
-constexpr int kMaxStages = 5;
+constexpr int kMaxStages = 6;
 // TMEM columns: two buffers of scales (four chunks: 2 x 4 columns of weights'
 // and 8 of rows' scales each), then the sums.
 constexpr int kScaleCols = 64, kSumCol = 2 * kScaleCols, kTmemCols = 512;
@@ -55,7 +55,7 @@ struct Args {
   GroupedProblem p;
   bool early;         // offsets are of a kernel that the one before this has waited for
   int shares;         // blocks
-  int n_max, stages;  // rows of a tile at most; stages of the ring that hold so many
+  int n_max, ring;    // rows of a tile at most; bytes of the ring of stages
   bool wide;          // out is BF16 and takes four outputs of a row at once
   int* counters;      // [kMaxShares] chunks whose parts are there
   float* parts;       // [shares][2][2][n_max][128]
@@ -86,9 +86,9 @@ __host__ __device__ constexpr int scale_ring_bytes(int n_max) {
 }
 
 __host__ __device__ constexpr int stage_bytes(int n_max) { return kTiles * kATile + n_max * kChunk; }
-__host__ __device__ inline size_t smem_bytes(int n_max, int stages, int experts) {
-  return static_cast<size_t>(stages) * stage_bytes(n_max) + scale_ring_bytes(n_max) +
-         sizeof(Control) + (kMaxShares + 1) * sizeof(long long) +
+// Shared memory behind the ring of stages.
+__host__ __device__ inline size_t rest_bytes(int n_max, int experts) {
+  return scale_ring_bytes(n_max) + sizeof(Control) + (kMaxShares + 1) * sizeof(long long) +
          (experts + 1) * (sizeof(long long) + sizeof(int));
 }
 
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Args a) {
   extern __shared__ __align__(1024) uint8_t smem[];
   const GroupedProblem& p = a.p;
-  uint8_t* scale_ring = smem + static_cast<size_t>(a.stages) * stage_bytes(a.n_max);
+  uint8_t* scale_ring = smem + a.ring;
   int* row_table = reinterpret_cast<int*>(scale_ring + kScaleEntries * scale_entry_bytes(a.n_max));
   Control* ctl = reinterpret_cast<Control*>(scale_ring + scale_ring_bytes(a.n_max));
   long long* bounds = reinterpret_cast<long long*>(ctl + 1);  // [shares + 1] in cost
@@ -450,8 +450,8 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
   tallest = __reduce_max_sync(0xffffffffu, lane < kThreads / 32 ? ctl->plan[2][lane] : 0);
   // The ring in stages for the rows that the largest tile has.
   const int stage = stage_bytes(tallest);
-  int stages = a.stages;
-  while (stages < kMaxStages && (stages + 1) * stage <= a.stages * stage_bytes(a.n_max)) ++stages;
+  int stages = 2;
+  while (stages < kMaxStages && (stages + 1) * stage <= a.ring) ++stages;
   // No more tiles than blocks: a block each, without cuts, where the largest
   // takes no longer than an equal share and the parts' meeting.
   const long long all_tiles = static_cast<long long>(tiles) * row_tiles;
@@ -1241,10 +1241,7 @@ int sm_count() {
   return sms < kMaxShares ? sms : kMaxShares;
 }
 
-struct Shape {
-  int n_max, stages;
-};
-Shape tile_shape(const GroupedProblem& p) {
+int tile_rows(const GroupedProblem& p) {
   const long long rows = p.rows, each = p.experts;  // rows of a group on average
   const int outs = p.w[1] ? kTileRows : kTiles * kTileRows;
   // Small tiles for small groups leave more stages. Long sums make up for an
@@ -1257,13 +1254,11 @@ Shape tile_shape(const GroupedProblem& p) {
   const long long row_tiles = (p.outs + outs - 1) / outs;
   while (n_max > 32 && row_tiles * ((rows + n_max - 1) / n_max) < 2ll * sm_count())
     n_max = n_max > kHalfN ? kHalfN : 32;
-  int stages = kMaxStages;
-  while (smem_bytes(n_max, stages, p.experts) > kMaxSmem) --stages;
-  return {n_max, stages};
+  return n_max;
 }
 
 size_t parts_bytes(const GroupedProblem& p) {
-  return static_cast<size_t>(sm_count()) * 4 * tile_shape(p).n_max * kTileRows * sizeof(float);
+  return static_cast<size_t>(sm_count()) * 4 * tile_rows(p) * kTileRows * sizeof(float);
 }
 
 constexpr size_t kCounterBytes = kMaxShares * sizeof(int);
@@ -1285,9 +1280,8 @@ cudaError_t launch(const GroupedProblem& p, bool early, int* counters, float* pa
   a.p = p;
   a.early = early;
   a.shares = sm_count();
-  const Shape s = tile_shape(p);
-  a.n_max = s.n_max;
-  a.stages = s.stages;
+  a.n_max = tile_rows(p);
+  a.ring = static_cast<int>((kMaxSmem - rest_bytes(a.n_max, p.experts)) & ~static_cast<size_t>(1023));
   a.wide = p.bf16 && p.outs % 4 == 0 && p.out_stride % 4 == 0 &&
            reinterpret_cast<uintptr_t>(p.out) % 8 == 0;
   a.counters = counters;
@@ -1299,7 +1293,7 @@ cudaError_t launch(const GroupedProblem& p, bool early, int* counters, float* pa
   cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), static_cast<int>(kMaxSmem));
   if (e != cudaSuccess) return e;
   return launch_pdl(kernel, dim3(a.shares), dim3(kThreads),
-                    smem_bytes(s.n_max, s.stages, p.experts), st, map0, map1, xmap, a);
+                    a.ring + rest_bytes(a.n_max, p.experts), st, map0, map1, xmap, a);
 }
 
 // Pieces of a buffer, 256-byte aligned.
