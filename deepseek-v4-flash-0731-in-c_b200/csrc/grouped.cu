@@ -48,7 +48,7 @@ constexpr int kMaxStages = 6;
 // TMEM columns: two buffers of scales (four chunks: 2 x 4 columns of weights'
 // and 8 of rows' scales each), then the sums.
 constexpr int kScaleCols = 64, kSumCol = 2 * kScaleCols, kTmemCols = 512;
-constexpr int kMaxShares = 256;          // blocks
+constexpr int kMaxShares = 160;          // blocks
 constexpr size_t kMaxSmem = 227 * 1024;
 
 struct Args {
@@ -79,7 +79,7 @@ struct alignas(16) Control {
 // The ring of scales: an entry holds four chunks' of 256 outputs and n_max rows.
 // Behind it the rows of x of two pieces.
 __host__ __device__ constexpr int row_table_ints(int n_max) { return n_max + 16; }
-constexpr int kScaleEntries = 4, kScaleBytes = 2 * kTileRows * 16;
+constexpr int kScaleEntries = 3, kScaleBytes = 2 * kTileRows * 16;
 __host__ __device__ constexpr int scale_entry_bytes(int n_max) { return kScaleBytes + n_max * 4; }
 __host__ __device__ constexpr int scale_ring_bytes(int n_max) {
   return kScaleEntries * scale_entry_bytes(n_max) + 2 * row_table_ints(n_max) * 4;
