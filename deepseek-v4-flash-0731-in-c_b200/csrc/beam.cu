@@ -550,6 +550,12 @@ __global__ void __launch_bounds__(kThreads<kFew>, kBlocks<kFew>) beam_kernel(con
   pdl_trigger();
   for (int u = rank, slot = 0; u < units; u += a.blocks, ++slot) {
     const int b = u / a.parts;
+    // nothing of a dead beam's row is read (of a prompt just begun all but one)
+    if (!(fabsf(a.p.score[static_cast<long long>(g) * a.p.beams + b]) < INFINITY)) {
+      if (threadIdx.x == 0) part[slot] = {0.0, -INFINITY};
+      if (threadIdx.x < a.p.cands) keys[slot * a.p.cands + threadIdx.x] = 0;
+      continue;
+    }
     take_part<kBf16, kFew>(sh.held, a, static_cast<long long>(g) * a.p.beams + b, u - b * a.parts, part + slot,
                      keys + slot * a.p.cands);
   }
