@@ -1890,9 +1890,12 @@ bool grouped_problem(const char* who, const dsv4cuda_grouped_shape* s, dsv4::Gro
   if (!s || s->n_groups < 1 || s->n_groups > dsv4::kGroupedMaxExperts || s->n_rows < 0 ||
       s->n_rows > 0x3FFFFFFF || s->x_rows < 0 || s->out_rows < 0 || s->outs < 1 || s->width < 128 ||
       s->width % 128 || s->width > 1 << 20 || s->outs > 0x3FFFFFFF ||
-      (s->out_stride && s->out_stride < s->outs)) {
+      (s->out_stride && s->out_stride < s->outs) ||
+      // (tiles are counted in 31 bits)
+      static_cast<long long>(s->n_groups) * s->outs > 1ll << 36 ||
+      static_cast<long long>(s->n_rows) * s->outs > 1ll << 40) {
     record_error("%s: bad shape (1..1024 groups, width a multiple of 128 up to 2^20, out_stride at "
-                 "least outs)", who);
+                 "least outs, outs times groups up to 2^36, times rows up to 2^40)", who);
     return false;
   }
   p->experts = s->n_groups;

@@ -291,9 +291,10 @@ int dsv4cuda_moe_experts(dsv4cuda_moe_layer *L, const uint8_t *xq, const uint8_t
  * offsets [n_groups + 1] are read on the device, ascending, at most n_rows;
  * groups may be empty. One group is a dense product. src, dst [n_rows] may be
  * NULL (row r); a src outside x_rows stands for zeros, a dst outside out_rows
- * is not written, nor are the rows of out that no dst names. width is a
- * multiple of 128 up to 2^20. Weights: fp8 = 0 packed E2M1 (the low nibble first) with
- * E8M0 ws [n_groups][outs][width / 32]; fp8 = 1 E4M3 with ws
+ * is not written, nor are the rows of out that no dst names (a row that two
+ * name gets each value from one of them). width is a multiple of 128 up to
+ * 2^20, outs times groups at most 2^36, outs times rows 2^40. Weights: fp8 = 0
+ * packed E2M1 (the low nibble first) with E8M0 ws [n_groups][outs][width / 32]; fp8 = 1 E4M3 with ws
  * [n_groups][ceil(outs / 128)][width / 128]. x as above. out: BF16 or fp32, the
  * fp32 sums rounded once. Results are the same from call to call. DEVICE
  * pointers; xq 16-byte aligned, w 32, ws 4 (E2M1). workspace as above. */

@@ -153,6 +153,10 @@ def test_c_grouped():
         bad[i] = v
         refused(f(P, P, P, P, P, P, None, None, C.byref(S(*bad)), None, 0, None), "bad shape")
         assert dsv4cuda.lib.dsv4cuda_grouped_workspace_bytes(C.byref(S(*bad))) == 0
+    refused(f(P, P, P, P, P, P, None, None, C.byref(S(1024, 10, 10, 10, 1 << 27, 256, 0, 1, 0)), None, 0, None),
+            "bad shape")
+    refused(f(P, P, P, P, P, P, None, None, C.byref(S(1, 1 << 21, 10, 10, 1 << 20, 256, 0, 1, 0)), None, 0, None),
+            "bad shape")
     s = C.byref(S(*good))
     for args in ((None, P, P, P, P, P), (P, None, P, P, P, P), (P, P, P, P, P, None), (P, P + 8, P, P, P, P),
                  (P, P, P, P + 16, P, P), (P, P, P, P, P + 2, P), (P + 1, P, P, P, P, P)):
