@@ -96,10 +96,12 @@ __device__ __forceinline__ uint2 codes8(const float (&v)[kVec], float inv) {
 
 // The magnitude bits order like the magnitudes, infinities and NaN above all.
 __device__ __forceinline__ uint32_t top8(const float (&v)[kVec]) {
-  uint32_t m = 0;
+  float m = fabsf(v[0]);
 #pragma unroll
-  for (int k = 0; k < kVec; ++k) m = max(m, __float_as_uint(v[k]) & 0x7FFFFFFFu);
-  return m;
+  for (int k = 1; k + 1 < kVec; k += 2)
+    asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(fabsf(v[k])), "f"(fabsf(v[k + 1])));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v[kVec - 1])));
+  return __float_as_uint(m);
 }
 
 struct NormArgs {
@@ -188,7 +190,8 @@ __device__ __forceinline__ void finish_row(const NormArgs& a, long long row, boo
     const int i = (tid + j * a.threads) * kVec, n = min(kVec, p.width - i);
     const bool in = live && n > 0;
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) v[j][k] = k < n ? v[j][k] * rs * gain[j].get(k) : 0.f;
+    for (int k = 0; k < kVec; ++k)  // (0 behind the row's end, but in rows that are NaN)
+      v[j][k] = v[j][k] * rs * gain[j].get(k);
     if (p.out && in) store8<kBf16>(const_cast<char*>(at(p.out, p.out_stride)), i, n, a.wide_o, v[j]);
     uint32_t top = top8(v[j]);
 #pragma unroll
@@ -196,7 +199,8 @@ __device__ __forceinline__ void finish_row(const NormArgs& a, long long row, boo
     uint2 c = make_uint2(0x7F7F7F7Fu, 0x7F7F7F7Fu);  // an infinity or NaN makes the block NaN
     uint32_t e8 = 255;
     if (top < 0x7F800000u) {
-      e8 = __float_as_uint(pow2_scale_448(__uint_as_float(top))) >> 23;
+      // the exponent of top / 448, rounded up
+      e8 = (__float_as_uint(fmaxf(__uint_as_float(top), 1e-4f) * (1.0f / 448.0f)) + 0x7FFFFFu) >> 23;
       c = codes8(v[j], __uint_as_float((254u - e8) << 23));
     }
     if (!in) continue;
