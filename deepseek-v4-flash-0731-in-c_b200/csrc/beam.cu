@@ -244,10 +244,10 @@ __device__ __forceinline__ void take_part(Held& h, const BeamArgs& a, long long 
       const int at = atomicAdd(&h.jobs, 1);
       if (at < kJobs) h.job[at] = static_cast<uint32_t>(step) << kTidBits | tid;
     }
-    // looked at after one step, two, four, and every fourth from there (of two
-    // steps both at once)
+    // looked at after one step, two, four, eight and so on, as the limit's next
+    // tightening takes twice the values (of two steps both at once)
     if (i0 + kSpan < i1 && i0 + 2 * kSpan >= i1 && step == 0) continue;
-    if ((step & (step < 4 ? step + 1 : 3)) != (step < 4 ? 0 : 3) && i0 + kSpan < i1) continue;
+    if ((step & (step + 1)) != 0 && i0 + kSpan < i1) continue;
     __syncthreads();
     const int jobs = h.jobs;
     if (jobs <= kJobs) {
