@@ -535,6 +535,12 @@ __host__ __device__ inline int slots_of(int beams, int parts, int blocks) {
   return (beams * parts + blocks - 1) / blocks;
 }
 
+// 64 prompts of eight beams, 129,280 BF16 logits: 66 us, 2.0 TB/s. A step of a
+// block (32 values a thread) takes some 3,000 clocks where the exponentials of the
+// four blocks of an SM alone take 2,048; the looks, the parts' ends and the merge
+// (5 us) come one after the other, and barriers are what most warps wait at. One
+// prompt of four beams, fp32: 16 us, of which the host's call is 10, reading and
+// choosing 5 and the merge 6 overlapped with the next call's start.
 template <bool kBf16, bool kFew>
 __global__ void __launch_bounds__(kThreads<kFew>, kBlocks<kFew>) beam_kernel(const BeamArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];  // this block's parts, then their keys
@@ -556,8 +562,8 @@ __global__ void __launch_bounds__(kThreads<kFew>, kBlocks<kFew>) beam_kernel(con
       if (threadIdx.x < a.p.cands) keys[slot * a.p.cands + threadIdx.x] = 0;
       continue;
     }
-    take_part<kBf16, kFew>(sh.held, a, static_cast<long long>(g) * a.p.beams + b, u - b * a.parts, part + slot,
-                     keys + slot * a.p.cands);
+    take_part<kBf16, kFew>(sh.held, a, static_cast<long long>(g) * a.p.beams + b, u - b * a.parts,
+                           part + slot, keys + slot * a.p.cands);
   }
   cluster_arrive();
   cluster_wait();
@@ -579,7 +585,8 @@ void deal(const BeamProblem& p, int span, int places, BeamArgs* a) {
     const int each = (steps + n - 1) / n;
     if (n > 1 && (steps + n - 2) / (n - 1) == each) continue;  // no shorter
     for (int blocks = 1; blocks <= kMaxBlocks && blocks < 2 * p.beams * n; blocks *= 2) {
-      const double waves = static_cast<double>((static_cast<long long>(p.groups) * blocks + places - 1) / places);
+      const double waves =
+          static_cast<double>((static_cast<long long>(p.groups) * blocks + places - 1) / places);
       const double cost = waves * slots_of(p.beams, n, blocks) * (each + 3) + p.beams * n / 64 + n / 8;
       if (a->parts == 0 || cost < least) {
         least = cost;

@@ -2082,7 +2082,8 @@ bool beam_problem(const char* who, const dsv4cuda_beam_shape* s, dsv4::BeamProbl
   static_assert(DSV4CUDA_MAX_BEAMS == dsv4::kMaxBeams, "limit");
   static_assert(DSV4CUDA_MAX_BEAM_CANDIDATES == dsv4::kMaxBeamCandidates, "limit");
   if (!s || s->n_groups < 0 || s->beams < 1 || s->beams > dsv4::kMaxBeams || s->n_cands < 1 ||
-      s->n_cands > dsv4::kMaxBeamCandidates || s->vocab < 1 || s->vocab > 0x3FFFFFFF || (s->stride && s->stride < s->vocab) ||
+      s->n_cands > dsv4::kMaxBeamCandidates || s->vocab < 1 || s->vocab > 0x3FFFFFFF ||
+      (s->stride && s->stride < s->vocab) ||
       static_cast<long long>(s->n_groups) * s->beams > 0x7FFFFFFFll) {
     record_error("%s: bad shape (1..%d beams and candidates, stride at least vocab)", who,
                  dsv4::kMaxBeams);

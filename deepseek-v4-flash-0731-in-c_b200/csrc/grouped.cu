@@ -17,13 +17,18 @@
 // that results do not depend on timing.
 //
 // Roles: warps 0-7 epilogue, 8-11 scales (to TMEM, each warp the copy of its
-// lane quarter), 12-15 other rows of x, 16 copies by TMA (weights, and rows that lie in
-// their order), 17-18 MMAs (a tile of 128 outputs each).
+// lane quarter), 12-15 rows of x that are gathered, 16 copies by TMA (weights, and
+// rows that lie in their order), 17-18 MMAs (a tile of 128 outputs each).
 //
-// What bounds it where the weights' bytes do not: the TMA engine brings a row of
-// 128 bytes of shared memory in some 2.7 clocks, whatever its bytes in memory, so
-// 256 weights' rows of a chunk take 690 clocks; then the shared memory's own
-// bandwidth, 64 KB a chunk for the E2M1 tiles' two halves and 384 bytes a row.
+// What bounds it: with few rows a group HBM (32 tokens of 8 routes over 256
+// experts of 7168 x 2048: 641 us, 5.98 TB/s of the 6.45 of a copy), as long as six
+// stages are under way. With more the TMA engine, which brings a row of 128 bytes
+// of shared memory in some 2.7 clocks, whatever its bytes in memory, so that 256
+// weights' rows of a chunk take 690 clocks; and the shared memory's own
+// bandwidth, 64 KB a chunk for writing and reading expanded E2M1 tiles and 384
+// bytes a row (256 experts of 4096 x 2048: 2,000 tokens 877 us, 8,192 tokens 2.2
+// ms, 1.1 PFLOP/s at the power cap). With one token launches, the plan and the
+// first bytes' way (38 us).
 #include "grouped.cuh"
 
 #include <cuda_bf16.h>
@@ -224,16 +229,17 @@ __device__ __forceinline__ void bar_sync(int id, int threads) {
 // ------------------------------------------------------------------ plan --
 
 // How a group of n rows is cut: tiles of the same number of rows, a multiple
-// of 16, and what a chunk of one costs in clocks (measured: 740 for 16 rows, 830
-// for 48, 930 for 80, where two tiles' sums fit in TMEM; beyond that the epilogue,
-// some 67 clocks a row, is not overlapped).
-// With every chunk counted alike the slowest block took 558 us where the mean was
-// 455 (2,000 tokens of 4096 x 2048, gate and up).
+// of 16, and what a chunk of one costs in clocks (as measured: 740 for 16 rows, 830
+// for 48, 930 for 80, where two tiles' sums fit in TMEM; beyond that the epilogue
+// is not overlapped). With every chunk counted alike the slowest block took 558 us
+// where the mean was 455 (2,000 tokens of 4096 x 2048, gate and up).
 struct Cut {
   int tiles, rows, cost;
 };
 constexpr int kSnapTiles = 8;  // shares of so many tiles on average are not cut
-constexpr int kJoin = 20000;      // what a tile's parts take to meet, in clocks
+// What a tile's parts take to meet, in such clocks (one group of 8 rows: 64 tiles
+// of 56 chunks 22.9 us cut and 25.1 whole, 96 tiles of 32 chunks 21.5 and 18.4).
+constexpr int kJoin = 20000;
 // (flat: shares are single tiles, and a chunk counts 1)
 __device__ __forceinline__ Cut cut_group(int n, int n_max, int chunks, bool flat) {
   Cut c;
@@ -295,7 +301,9 @@ struct Walk {
   int e, row_tile, t, lo;   // the next piece
   long long left;           // from its tile's start to the share's end, in cost
 
-  __device__ __forceinline__ void recut(bool flat) { cut = cut_group(offsets[e + 1] - offsets[e], n_max, chunks, flat); }
+  __device__ __forceinline__ void recut(bool flat) {
+    cut = cut_group(offsets[e + 1] - offsets[e], n_max, chunks, flat);
+  }
   // prefix [experts + 1]: cost before each group; the share is b0 .. b1.
   __device__ __forceinline__ void begin(const long long* prefix, long long b0, long long b1, bool flat) {
     left = 0;
@@ -499,8 +507,8 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     if (snap && c > 0 && c < shares) {
       const int e = group_at(prefix, p.experts, b);
       const Cut g = cut_group(offsets[e + 1] - offsets[e], a.n_max, chunks, flat);
-      const unsigned tile = chunks * g.cost;
-      b = prefix[e] + static_cast<long long>((static_cast<unsigned long long>(b - prefix[e]) + tile / 2) / tile) * tile;
+      const long long tile = chunks * g.cost;
+      b = prefix[e] + (b - prefix[e] + tile / 2) / tile * tile;
     }
     bounds[c] = b;
   }
@@ -883,12 +891,13 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
     cp_async_wait<0>();
   } else if (warp < kWarpCopy) {
     // ---------------------------------------------------------------- rows
-    // Rows that are not in their order (those that are come by TMA): 16 bytes a
-    // thread, eight threads a row, swizzled. (Gathers by TMA take 48 clocks for four
-    // rows; bringing the rows into their order first and copying them by TMA, beside
-    // the weights, 930 clocks a chunk of 48 rows where this takes 800.) The loop is short and asks for a row's number one copy
-    // ahead: with the numbers in registers and the loop unrolled it ran from the
-    // second-level instruction cache and took 800 clocks for 16 rows as for 192.
+    // Rows that are not in their order: 16 bytes a thread, eight threads a row,
+    // swizzled. (Gathers by TMA take 48 clocks for four rows; bringing the rows into
+    // their order first and copying them by TMA, beside the weights, 930 clocks a
+    // chunk of 48 rows where this takes 800.) The loop is short and asks for a row's
+    // number one copy ahead: with the numbers in registers and the loop unrolled it
+    // ran from the second-level instruction cache and took 800 clocks for 16 rows as
+    // for 192.
     const int st = threadIdx.x - 32 * kWarpRows;
     const uint8_t* x_from = p.xq + (st & 7) * 16;
     const uint32_t x_to = kTiles * kATile + (st >> 3) * kChunk + (((st & 7) ^ ((st >> 3) & 7)) << 4);
@@ -966,7 +975,8 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
             tma_load_3d(st + kATile, kGated ? &map1 : &map0, c * kChunk,
                         kGated ? row : row + kTileRows, piece.e, &ctl->full[s]);
           for (int r = 0; r < x_rows; r += 16)
-            tma_load_2d(st + (kTiles * kTileRows + r) * kChunk, &xmap, c * kChunk, piece.row0 + r, &ctl->full[s]);
+            tma_load_2d(st + (kTiles * kTileRows + r) * kChunk, &xmap, c * kChunk, piece.row0 + r,
+                        &ctl->full[s]);
           ++n;
           if (++s == stages) {
             s = 0;
@@ -1218,7 +1228,8 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(const GroupArgs a)
 
 // out[t] = the sum of the token's slots in route order; slots of experts that
 // are not here were not written. The slots are BF16, which is what a GEMV of
-// the layer hands on; their sum is fp32 and rounded once.
+// the layer hands on; their sum is fp32 and rounded once. Bound by their reading:
+// 8,192 tokens of six 93 us, 5.0 TB/s.
 __global__ void __launch_bounds__(256) experts_combine_kernel(const uint16_t* __restrict__ y,
                                                               const int* __restrict__ idx, int n, int topk,
                                                               int hidden, int lo, int experts,
@@ -1236,7 +1247,8 @@ __global__ void __launch_bounds__(256) experts_combine_kernel(const uint16_t* __
     for (int k = 0; k < 8; ++k) {
       r[k] = make_uint4(0, 0, 0, 0);
       if (k0 + k < topk)  // (before it is known whether it was written)
-        r[k] = __ldcs(reinterpret_cast<const uint4*>(y + (static_cast<size_t>(t) * topk + k0 + k) * hidden) + v);
+        r[k] = __ldcs(
+            reinterpret_cast<const uint4*>(y + (static_cast<size_t>(t) * topk + k0 + k) * hidden) + v);
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -1271,13 +1283,17 @@ int sm_count() {
 int tile_rows(const GroupedProblem& p) {
   const long long rows = p.rows, each = p.experts;  // rows of a group on average
   const int outs = p.w[1] ? kTileRows : kTiles * kTileRows;
-  // Small tiles for small groups leave more stages. Long sums make up for an
-  // epilogue that is not overlapped (8,192 tokens of 4096 x 2048: 2244 us, 2702
-  // with 96 rows), short ones do not (2048 rows of 1024: 135 us, 115 with 96).
-  int n_max = rows <= 8 * each ? 16 : rows <= 24 * each ? 32 : p.width >= 24 * kChunk ? kMaxN : kHalfN;
-  // Fewer rows a tile where there would be too few tiles: cutting one along its
-  // columns costs more (777 rows of 24 groups, 1003 outputs: 24 us, 39 with tiles
-  // of 96)
+  // Rows of a tile. Small ones leave more of the parts' memory unused and more of
+  // the ring to stages (256 experts of 4096 x 2048: 100 tokens 515 us with 16, 522
+  // with 32; 500 tokens 578 with 32, 601 with 96). Beyond 96 the sums fill TMEM and
+  // the epilogue is not overlapped, which long sums of large groups make up for
+  // (8,192 tokens 2162 us with 192, 2216 with 96; 2,000 tokens, uneven, 913 and 929),
+  // others not (1,500 tokens 741, 693 with 96; 2048 rows of 1024 columns 135, 127
+  // with 96).
+  int n_max = rows <= 8 * each ? 16 : rows <= 24 * each ? 32 : kHalfN;
+  if (rows > 40 * each && p.width >= 24 * kChunk) n_max = kMaxN;
+  // Fewer where there would be too few tiles: to cut one along its columns costs
+  // more (777 rows of 24 groups, 1003 outputs: 17.4 us with 32, 19.9 with 96)
   const long long row_tiles = (p.outs + outs - 1) / outs;
   while (n_max > 32 && row_tiles * ((rows + n_max - 1) / n_max) < 2ll * sm_count())
     n_max = n_max > kHalfN ? kHalfN : 32;
@@ -1364,6 +1380,26 @@ GroupedProblem gate_up(const ExpertsProblem& p, const ExpertsWork& w) {
   return g;
 }
 
+GroupedProblem down(const ExpertsProblem& p, const ExpertsWork& w) {
+  GroupedProblem d;
+  d.experts = p.experts;
+  d.rows = p.n * p.topk;
+  d.outs = p.hidden;
+  d.width = p.inter;
+  d.w[0] = p.w2;
+  d.ws[0] = p.s2;
+  d.xq = w.hq;
+  d.xs = w.hs;
+  d.x_rows = d.rows;
+  d.offsets = w.offsets;
+  d.dst = w.slot;
+  d.out_rows = d.rows;
+  d.out = w.y;
+  d.out_stride = p.hidden;
+  d.err = p.err;
+  return d;
+}
+
 ExpertsWork experts_work(const ExpertsProblem& p, void* base) {
   Carver c{static_cast<char*>(base)};
   const size_t slots = static_cast<size_t>(p.n) * p.topk;
@@ -1376,7 +1412,9 @@ ExpertsWork experts_work(const ExpertsProblem& p, void* base) {
   w.hq = c.take<uint8_t>(slots * p.inter);
   w.hs = c.take<uint8_t>(slots * (p.inter / 128));
   w.y = c.take<uint16_t>(slots * p.hidden);
-  w.parts = c.take<float>(parts_bytes(gate_up(p, w)) / sizeof(float));
+  // (either product may have the larger tiles)
+  const size_t parts[2] = {parts_bytes(gate_up(p, w)), parts_bytes(down(p, w))};
+  w.parts = c.take<float>((parts[0] > parts[1] ? parts[0] : parts[1]) / sizeof(float));
   w.bytes = c.used;
   return w;
 }
@@ -1437,26 +1475,9 @@ cudaError_t experts_forward(const ExpertsProblem& p, void* ws, cudaStream_t st) 
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   e = cudaLaunchKernelEx(&cfg, group_kernel, a);
   if (e != cudaSuccess) return e;
-  const GroupedProblem g = gate_up(p, w);
-  e = launch(g, false, w.counters, w.parts, st);
+  e = launch(gate_up(p, w), false, w.counters, w.parts, st);
   if (e != cudaSuccess) return e;
-  GroupedProblem d;
-  d.experts = p.experts;
-  d.rows = g.rows;
-  d.outs = p.hidden;
-  d.width = p.inter;
-  d.w[0] = p.w2;
-  d.ws[0] = p.s2;
-  d.xq = w.hq;
-  d.xs = w.hs;
-  d.x_rows = g.rows;
-  d.offsets = w.offsets;
-  d.dst = w.slot;
-  d.out_rows = g.rows;
-  d.out = w.y;
-  d.out_stride = p.hidden;
-  d.err = p.err;
-  e = launch(d, true, w.counters + kMaxShares, w.parts, st);
+  e = launch(down(p, w), true, w.counters + kMaxShares, w.parts, st);
   if (e != cudaSuccess) return e;
   const long long vecs = static_cast<long long>(p.n) * (p.hidden / 8);
   return launch_pdl(experts_combine_kernel, dim3(static_cast<unsigned>((vecs + 255) / 256)), dim3(256),

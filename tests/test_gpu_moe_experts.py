@@ -78,6 +78,26 @@ CASES = [  # n, hidden, inter, experts, topk
 ]
 
 
+# either product may have the longer sums, the wider rows and so the larger tiles
+UNEVEN = [(1500, 128, 4096, 2, 2), (600, 7168, 128, 2, 2), (5000, 128, 3584, 3, 2), (3000, 3584, 128, 4, 1)]
+
+
+@pytest.mark.parametrize("n,hidden,inter,experts,topk", UNEVEN)
+def test_uneven(cuda, n, hidden, inter, experts, topk):
+    layer, w = layer_of(cuda, hidden, inter, experts, topk)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(4)
+    xq, xs = ref.activations(n, hidden, g)
+    idx, wt = routes(n, experts, topk)
+    need = layer.experts_workspace_bytes(n)
+    room = torch.full((need + 65536,), 0x5A, dtype=torch.uint8, device="cuda")
+    out = check(cuda, layer, w, xq, xs, idx, wt)
+    again = torch.empty_like(out)
+    layer.experts(xq, xs, idx, wt, again, workspace=room[:need])
+    assert torch.equal(out, again) and bool((room[need:] == 0x5A).all())
+    layer.close()
+
+
 @pytest.mark.parametrize("n,hidden,inter,experts,topk", CASES)
 def test_experts(cuda, n, hidden, inter, experts, topk):
     layer, w = layer_of(cuda, hidden, inter, experts, topk)
