@@ -523,10 +523,13 @@ __device__ __forceinline__ void merge_group(Merge& sh, const BeamArgs& a, int g,
   const unsigned lost = ~mothers & (p.beams == 32 ? 0xffffffffu : (1u << p.beams) - 1);
   const unsigned moves = __ballot_sync(0xffffffffu, beam && !stays);
   if (!beam) return;
+  // (dst may be slot itself: read by all before it is written)
   const int home = stays ? mother : nth_bit(lost, __popc(moves & ((1u << lane) - 1)));
   const long long row = static_cast<long long>(g) * p.beams;
-  p.dst[at] = p.slot[row + home];
-  p.src[at] = mother >= 0 ? p.slot[row + mother] : -1;
+  const int to = p.slot[row + home], from = mother >= 0 ? p.slot[row + mother] : -1;
+  __syncwarp(p.beams == 32 ? 0xffffffffu : (1u << p.beams) - 1);
+  p.dst[at] = to;
+  p.src[at] = from;
 }
 
 constexpr int kMaxBlocks = 16;  // of a cluster

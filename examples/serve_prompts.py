@@ -50,17 +50,18 @@ class Layer:
         the pool, each attends to its sequence, and the logits come out."""
         x = self.embed[tokens]
         q = self.rope((x @ self.wq.T).view(-1, HEADS, DIM), pos).bfloat16()
-        kv = self.rope(x @ self.wkv.T, pos).bfloat16().float()
+        kv = (x @ self.wkv.T).bfloat16()
+        a = pos[:, None].float() * self.freq[None]
         rows = torch.empty(len(tokens), dtype=torch.int64, device="cuda")
         server.pool.append(slots, counts, rows)
-        server.cache.write(kv, rows)
+        server.pool.write(0, kv, rows, rope_cos=a.cos(), rope_sin=a.sin())
         # each slot's rows of q: its new tokens, none for the others
         new = torch.zeros(SLOTS, dtype=torch.int32, device="cuda")
         new[slots.long()] = counts
         order = torch.argsort(torch.repeat_interleave(slots, counts), stable=True)
         q_start = torch.zeros(SLOTS + 1, dtype=torch.int32, device="cuda")
         q_start[1:] = new.cumsum(0)
-        a = pos[order][:, None].float() * self.freq[None]
+        a = a[order]
         out = torch.empty_like(q)
         d4.paged_attn(out, q[order], server.pool, 0, q_start, int(counts.max()), server.max_len,
                       DIM ** -0.5, sink=self.sink, rope_cos=a.cos().contiguous(),

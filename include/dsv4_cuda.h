@@ -629,7 +629,7 @@ int dsv4cuda_paged_compact(const dsv4cuda_paged *p, int *table_out, int *refs_ou
  * [nope + rope_dim] (BF16, or fp32 when bf16 is 0; `stride` elements apart,
  * 0: nope + rope_dim) goes to row rows[i] of layer `layer`'s cache, as
  * dsv4cuda_paged_append gave them (rows outside the pages, -1 among them, are
- * left out; a row named twice gets one of the two):
+ * left out; what a row named twice holds is a mixture):
  *   v = kv / sqrt(mean kv^2 + eps) * gain        (gain NULL: v = kv)
  *   the first nope dims as E4M3 codes with one E8M0 scale per 64,
  *   pair (2j, 2j + 1) of the others turned by rope_cos / rope_sin [n]
@@ -721,6 +721,7 @@ int dsv4cuda_token_logprobs(const void *logits, int bf16, int rows, int vocab, l
  *       dst[i] and comes from src[i] (-1: from none). A parent's first child
  *       stays where it is (dst = src), the others take the slots of beams
  *       without children, so dsv4cuda_paged_fork(dst, src) puts all in place.
+ *       dst may be slot itself.
  * beams and n_cands 1 .. 32, vocab below 2^30. DEVICE pointers, async on stream,
  * capturable; no workspace. */
 #define DSV4CUDA_MAX_BEAMS 32

@@ -194,3 +194,22 @@ def test_captured_and_on_streams(cuda):
     for r in got:
         for a, w in zip(r, want):
             assert torch.equal(a.cpu(), w)
+
+
+@pytest.mark.parametrize("beams", [5, 32])
+def test_slots_in_place(cuda, beams):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(11)
+    x = torch.randn(4 * beams, 700, device="cuda", generator=g) * 3
+    score = -torch.rand(4, beams, device="cuda", generator=g)
+    slot = torch.randperm(4 * beams, device="cuda", generator=g).int().view(4, beams)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    outs = []
+    for dst in (torch.empty(4, beams, **i32), slot.clone()):
+        at = slot if not outs else dst
+        p, t, nxt, src = (torch.empty(4, n, **i32) for n in (beams, beams, beams, beams))
+        total = torch.empty(4, beams, device="cuda")
+        cuda.beam_select(x, score, p, t, total, nxt, slot=at, dst=dst, src=src)
+        outs.append((p, t, total, nxt, dst, src))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
