@@ -401,11 +401,13 @@ class MoeLayer:
         u8 = torch.uint8
         if xq.dim() != 2 or xq.shape[1] != self.hidden:
             raise ValueError(f"xq: [n][{self.hidden}] is wanted")
-        _here(xq, "xq")
+        on = _here(xq, "xq")
         _check(lib.dsv4cuda_moe_experts(
-            self.handle, _dev(xq, "xq", u8), _dev(xs, "xs", u8, n * (self.hidden // 128)),
-            _dev(idx, "idx", torch.int32, n * self.topk), _dev(wt, "wt", torch.float32, n * self.topk),
-            n, _dev(out, "out", torch.bfloat16, n * self.hidden), _dev(workspace, "workspace", u8),
+            self.handle, _dev(xq, "xq", u8), _dev(xs, "xs", u8, n * (self.hidden // 128), on),
+            _dev(idx, "idx", torch.int32, n * self.topk, on),
+            _dev(wt, "wt", torch.float32, n * self.topk, on), n,
+            _dev(out, "out", torch.bfloat16, n * self.hidden, on),
+            _dev(workspace, "workspace", u8, None, on),
             0 if workspace is None else workspace.numel(), _stream(stream)))
 
     def routed_slots(self, n_tokens):
@@ -666,10 +668,13 @@ lib.dsv4cuda_token_logprobs.argtypes = [vp, C.c_int, C.c_int, C.c_int, C.c_longl
                                         C.c_int, vp, vp, vp]
 
 
-def _dev(t, name, dtype, numel=None):
-    """The address of a contiguous CUDA tensor of `dtype` (None passes as NULL)."""
+def _dev(t, name, dtype, numel=None, on=None):
+    """The address of a contiguous CUDA tensor of `dtype` (None passes as NULL), of the
+    device `on` where that is given."""
     if t is None:
         return None
+    if on is not None and t.get_device() != on:
+        raise ValueError(f"{name} is on {t.device}, the call's other tensors are on cuda:{on}")
     if not (t.dtype is dtype and t.is_cuda and t.is_contiguous()):
         raise ValueError(f"{name}: a contiguous CUDA tensor of {dtype} is wanted, got {t.dtype} "
                          f"on {t.device}")
@@ -679,18 +684,20 @@ def _dev(t, name, dtype, numel=None):
 
 
 def _here(t, name):
-    """The calls launch on the current device: its tensors have to be there."""
+    """The current device, on which a call launches: its tensors have to be there."""
     import torch
-    if t.get_device() != torch.cuda.current_device():
-        raise ValueError(f"{name} is on {t.device}, the current device is cuda:"
-                         f"{torch.cuda.current_device()}")
+    here = torch.cuda.current_device()
+    if t.get_device() != here:
+        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{here}")
+    return here
 
 
-def _rows_of(t, name, shape, dtype):
+def _rows_of(t, name, shape, dtype, on=None):
     """Elements between the rows (0: of one row, or of none between them) of a CUDA tensor
     [rows][width] of `shape` and `dtype`."""
-    if t.dtype is not dtype or t.shape != shape or not t.is_cuda:
-        raise ValueError(f"{name}: a CUDA tensor {list(shape)} of {dtype} is wanted, got {t.dtype} "
+    if t.dtype is not dtype or t.shape != shape or not t.is_cuda or on not in (None, t.get_device()):
+        raise ValueError(f"{name}: a tensor {list(shape)} of {dtype} on "
+                         f"{'CUDA' if on is None else f'cuda:{on}'} is wanted, got {t.dtype} "
                          f"{list(t.shape)} on {t.device}")
     n, width = shape
     stride, inner = t.stride()
@@ -704,15 +711,14 @@ def _rows_of(t, name, shape, dtype):
 
 
 def _float_rows(t, name, width=None):
-    """(dtype, 1 for BF16 or 0 for fp32, shape) of rows [n][width]."""
+    """(dtype, 1 for BF16 or 0 for fp32, shape, device) of rows [n][width] on the current device."""
     import torch
     dtype, shape = t.dtype, t.shape
     bf16 = dtype is torch.bfloat16
     if not (bf16 or dtype is torch.float32) or len(shape) != 2 or width not in (None, shape[1]):
         raise ValueError(f"{name}: a CUDA tensor [rows][{width or 'width'}] of bfloat16 or float32 is "
                          f"wanted, got {dtype} {list(shape)}")
-    _here(t, name)
-    return dtype, 1 if bf16 else 0, shape
+    return dtype, 1 if bf16 else 0, shape, _here(t, name)
 
 
 class PagedCache:
@@ -780,13 +786,16 @@ class PagedCache:
         if not 0 <= layer < len(self.caches):
             raise ValueError(f"layer {layer} of {len(self.caches)}")
         d = self._dims[0] + self._dims[1]
-        dtype, bf16, shape = _float_rows(kv, "kv", d)
+        dtype, bf16, shape, on = _float_rows(kv, "kv", d)
+        if self.status_word.get_device() != on:
+            raise ValueError(f"kv is on cuda:{on}, the pool on {self.status_word.device}")
         stride, n = _rows_of(kv, "kv", shape, dtype), shape[0]
         half = n * (self._dims[1] // 2)
         _check(lib.dsv4cuda_paged_write(
-            self._ref, layer, kv.data_ptr(), bf16, stride, _dev(rows, "rows", self._i64, n), n,
-            _dev(gain, "gain", torch.bfloat16, d), eps, _dev(rope_cos, "rope_cos", torch.float32, half),
-            _dev(rope_sin, "rope_sin", torch.float32, half), _stream(stream)))
+            self._ref, layer, kv.data_ptr(), bf16, stride, _dev(rows, "rows", self._i64, n, on), n,
+            _dev(gain, "gain", torch.bfloat16, d, on), eps,
+            _dev(rope_cos, "rope_cos", torch.float32, half, on),
+            _dev(rope_sin, "rope_sin", torch.float32, half, on), _stream(stream)))
 
     def fork(self, dst, src, stream=None):
         """Slots dst become copies of slots src (-1: emptied); int32 CUDA tensors."""
@@ -896,30 +905,31 @@ def norm_quant(x, gain, codes, scales, eps=1e-6, residual=None, sum_out=None, ou
     them. sum_out (may be x or residual) receives x + residual, out the normalised rows; both
     of x's type."""
     import torch
-    dtype, bf16, size = _float_rows(x, "x")
+    dtype, bf16, size, on = _float_rows(x, "x")
     n, width = size
     u8, q = torch.uint8, _rows_of(x, "x", size, dtype)
     r = s = o = 0
     at_r = at_s = at_o = None
     if residual is not None:
-        r, at_r = _rows_of(residual, "residual", size, dtype), residual.data_ptr()
+        r, at_r = _rows_of(residual, "residual", size, dtype, on), residual.data_ptr()
     if sum_out is not None:
-        s, at_s = _rows_of(sum_out, "sum_out", size, dtype), sum_out.data_ptr()
+        s, at_s = _rows_of(sum_out, "sum_out", size, dtype, on), sum_out.data_ptr()
     if out is not None:
-        o, at_o = _rows_of(out, "out", size, dtype), out.data_ptr()
+        o, at_o = _rows_of(out, "out", size, dtype, on), out.data_ptr()
     _check(lib.dsv4cuda_norm_quant(
-        x.data_ptr(), at_r, at_s, at_o, _dev(gain, "gain", torch.bfloat16, width),
-        _dev(codes, "codes", u8, n * width), _dev(scales, "scales", u8, n * ((width + 127) // 128)),
+        x.data_ptr(), at_r, at_s, at_o, _dev(gain, "gain", torch.bfloat16, width, on),
+        _dev(codes, "codes", u8, n * width, on),
+        _dev(scales, "scales", u8, n * ((width + 127) // 128), on),
         _norm_shape(n, width, bf16, eps, q, r, s, o), _stream(stream)))
 
 
 def _beam_shape(logits, score, cands, eos):
-    dtype, bf16, (n, vocab) = _float_rows(logits, "logits")
+    dtype, bf16, (n, vocab), on = _float_rows(logits, "logits")
     if score.dim() != 2 or n != score.numel():
         raise ValueError("score [groups][beams] and logits [groups * beams][vocab] are wanted")
     groups, beams = score.shape
     return BeamShape(groups, beams, cands, vocab, bf16, eos,
-                     _rows_of(logits, "logits", logits.shape, dtype))
+                     _rows_of(logits, "logits", logits.shape, dtype)), on
 
 
 def beam_select(logits, score, parent, token, total, next, slot=None, dst=None, src=None, eos=-1,
@@ -933,13 +943,14 @@ def beam_select(logits, score, parent, token, total, next, slot=None, dst=None, 
     i32, f32 = torch.int32, torch.float32
     if parent.dim() != 2:
         raise ValueError("parent [groups][candidates] is wanted")
-    shape = _beam_shape(logits, score, parent.shape[1], eos)
+    shape, on = _beam_shape(logits, score, parent.shape[1], eos)
     all_c, all_b = shape.n_groups * shape.n_cands, shape.n_groups * shape.beams
     _check(lib.dsv4cuda_beam_select(
-        logits.data_ptr(), _dev(score, "score", f32), _dev(parent, "parent", i32, all_c),
-        _dev(token, "token", i32, all_c), _dev(total, "total", f32, all_c),
-        _dev(next, "next", i32, all_b), _dev(slot, "slot", i32, all_b), _dev(dst, "dst", i32, all_b),
-        _dev(src, "src", i32, all_b), C.byref(shape), _stream(stream)))
+        logits.data_ptr(), _dev(score, "score", f32, None, on), _dev(parent, "parent", i32, all_c, on),
+        _dev(token, "token", i32, all_c, on), _dev(total, "total", f32, all_c, on),
+        _dev(next, "next", i32, all_b, on), _dev(slot, "slot", i32, all_b, on),
+        _dev(dst, "dst", i32, all_b, on), _dev(src, "src", i32, all_b, on), C.byref(shape),
+        _stream(stream)))
 
 
 # ------------------------------------------------------- grouped products --
@@ -970,7 +981,6 @@ def _grouped_shape(out, xq, w, n_rows):
                          "the other")
     if out.shape[0] > 1 and out.stride(0) < outs:
         raise ValueError("out: the rows must not overlap")
-    _here(out, "out")
     return GroupedShape(groups, n_rows, xq.shape[0], out.shape[0], outs, width, int(held == width),
                         int(out.dtype is torch.bfloat16), out.stride(0) if out.shape[0] > 1 else 0)
 
@@ -990,14 +1000,15 @@ def grouped_gemm(out, xq, xs, w, ws, offsets, src=None, dst=None, workspace=None
     import torch
     u8, i32 = torch.uint8, torch.int32
     rows = src.numel() if src is not None else dst.numel() if dst is not None else xq.shape[0]
-    s = _grouped_shape(out, xq, w, rows)
+    s, on = _grouped_shape(out, xq, w, rows), _here(out, "out")
     scales = s.n_groups * (((s.outs + 127) // 128) * (s.width // 128) if s.fp8
                            else s.outs * (s.width // 32))
     _check(lib.dsv4cuda_grouped_gemm(
-        out.data_ptr(), _dev(xq, "xq", u8), _dev(xs, "xs", u8, s.x_rows * (s.width // 128)),
-        _dev(w, "w", u8), _dev(ws, "ws", u8, scales), _dev(offsets, "offsets", i32, s.n_groups + 1),
-        _dev(src, "src", i32, rows), _dev(dst, "dst", i32, rows), C.byref(s),
-        _dev(workspace, "workspace", u8), 0 if workspace is None else workspace.numel(),
+        out.data_ptr(), _dev(xq, "xq", u8, None, on), _dev(xs, "xs", u8, s.x_rows * (s.width // 128), on),
+        _dev(w, "w", u8, None, on), _dev(ws, "ws", u8, scales, on),
+        _dev(offsets, "offsets", i32, s.n_groups + 1, on), _dev(src, "src", i32, rows, on),
+        _dev(dst, "dst", i32, rows, on), C.byref(s), _dev(workspace, "workspace", u8, None, on),
+        0 if workspace is None else workspace.numel(),
         _stream(stream)))
 
 

@@ -54,6 +54,7 @@ def test_norm(calls):
                 dict(x=On((256,), BF)), dict(x=On((4, 256), BF, device=1)),
                 dict(residual=On((3, 256), BF)), dict(residual=On((4, 256), F32)),
                 dict(sum_out=On((4, 256), BF, (100, 1))), dict(out=On((4, 255), BF)),
+                dict(codes=On((4, 256), U8, device=1)), dict(out=On((4, 256), BF, device=1)),
                 dict(gain=On((255,), BF)), dict(gain=On((256,), F32)), dict(codes=On((4, 255), U8)),
                 dict(scales=On((4, 1), U8)), dict(codes=On((4, 256), torch.int8))):
         with pytest.raises(ValueError):
@@ -79,9 +80,10 @@ def test_grouped(calls):
     assert s[1].out_stride == 128
     for bad in (dict(w=On((3, 100, 100), U8)), dict(w=On((3, 99, 128), U8)), dict(w=On((100, 128), U8)),
                 dict(ws=On((3, 100, 7), U8)), dict(xs=On((5, 1), U8)), dict(offsets=On((3,), I32)),
-                dict(dst=On((8,), I32)), dict(src=On((9,), torch.int64)), dict(out=On((9, 100), torch.float16)),
+                dict(dst=On((8,), I32)), dict(src=On((9,), torch.int64)),
+                dict(out=On((9, 100), torch.float16)),
                 dict(out=On((9, 100), BF, (50, 1))), dict(out=On((9, 100), BF, device=1)),
-                dict(workspace=On((1 << 20,), F32))):
+                dict(w=On((3, 100, 128), U8, device=1)), dict(workspace=On((1 << 20,), F32))):
         with pytest.raises(ValueError):
             grouped(calls, **bad)
     assert len(calls) == 2
@@ -96,7 +98,8 @@ def test_experts(calls):
     assert calls[0][1][5] == 7
     for bad in (dict(xq=On((7, 128), U8)), dict(xq=On((7, 256), torch.int8)), dict(xs=On((7, 1), U8)),
                 dict(idx=On((7, 2), torch.int64)), dict(wt=On((7, 1), F32)), dict(out=On((7, 256), F32)),
-                dict(out=On((6, 256), BF)), dict(xq=On((7, 256), U8, device=1))):
+                dict(out=On((6, 256), BF)), dict(idx=On((7, 2), I32, device=1)),
+                dict(xq=On((7, 256), U8, device=1))):
         with pytest.raises(ValueError):
             layer.experts(**{**a, **bad})
     layer.handle = C.c_void_p()
@@ -105,13 +108,15 @@ def test_experts(calls):
 def test_write(calls):
     pool = object.__new__(dsv4cuda.PagedCache)
     pool.caches, pool._dims, pool._i64, pool._ref = [None, None], (448, 64), torch.int64, None
+    pool.status_word = On((1,), I32)
     a = dict(layer=1, kv=On((5, 512), BF, (520, 1)), rows=On((5,), torch.int64), gain=On((512,), BF),
              rope_cos=On((5, 32), F32), rope_sin=On((5, 32), F32), stream=0)
     pool.write(**a)
     assert calls[0][1][1] == 1 and calls[0][1][4] == 520
     for bad in (dict(layer=2), dict(layer=-1), dict(kv=On((5, 448), BF)), dict(kv=On((5, 512), BF, (0, 1))),
                 dict(rows=On((4,), torch.int64)), dict(rows=On((5,), I32)), dict(gain=On((448,), BF)),
-                dict(rope_cos=On((4, 32), F32)), dict(rope_sin=On((5, 32), BF))):
+                dict(rows=On((5,), torch.int64, device=1)), dict(rope_cos=On((4, 32), F32)),
+                dict(rope_sin=On((5, 32), BF))):
         with pytest.raises(ValueError):
             pool.write(**{**a, **bad})
 
@@ -128,9 +133,11 @@ def test_beam(calls):
     beam()
     s = calls[0][1][9]._obj
     assert (s.n_groups, s.beams, s.n_cands, s.vocab, s.bf16, s.eos, s.stride) == (2, 3, 4, 50, 1, 7, 64)
-    for bad in (dict(logits=On((5, 50), BF)), dict(logits=On((6, 50), BF, (0, 1))), dict(score=On((6,), F32)),
+    for bad in (dict(logits=On((5, 50), BF)), dict(logits=On((6, 50), BF, (0, 1))),
+                dict(score=On((6,), F32)),
                 dict(score=On((2, 3), BF)), dict(token=On((2, 3), I32)), dict(next=On((2, 2), I32)),
-                dict(total=On((2, 4), BF)), dict(dst=On((2, 2), I32)), dict(parent=On((8,), I32))):
+                dict(slot=On((2, 3), I32, device=1)), dict(total=On((2, 4), BF)),
+                dict(dst=On((2, 2), I32)), dict(parent=On((8,), I32))):
         with pytest.raises(ValueError):
             beam(**bad)
 
@@ -147,27 +154,33 @@ def refused(rc, word):
 def test_c_grouped():
     S, f = dsv4cuda.GroupedShape, dsv4cuda.lib.dsv4cuda_grouped_gemm
     good = (2, 10, 10, 10, 64, 256, 0, 1, 0)
-    for i, v in ((0, 0), (0, 1025), (1, -1), (2, -1), (3, -1), (4, 0), (5, 0), (5, 200), (5, (1 << 20) + 128),
+    for i, v in ((0, 0), (0, 1025), (1, -1), (2, -1), (3, -1), (4, 0), (5, 0), (5, 200), (5,
+    (1 << 20) + 128),
                  (8, 63)):
         bad = list(good)
         bad[i] = v
         refused(f(P, P, P, P, P, P, None, None, C.byref(S(*bad)), None, 0, None), "bad shape")
         assert dsv4cuda.lib.dsv4cuda_grouped_workspace_bytes(C.byref(S(*bad))) == 0
-    refused(f(P, P, P, P, P, P, None, None, C.byref(S(1024, 10, 10, 10, 1 << 27, 256, 0, 1, 0)), None, 0, None),
+    refused(f(P, P, P, P, P, P, None, None, C.byref(S(1024, 10, 10, 10, 1 << 27, 256, 0, 1, 0)), None, 0,
+    None),
             "bad shape")
-    refused(f(P, P, P, P, P, P, None, None, C.byref(S(1, 1 << 21, 10, 10, 1 << 20, 256, 0, 1, 0)), None, 0, None),
+    refused(f(P, P, P, P, P, P, None, None, C.byref(S(1, 1 << 21, 10, 10, 1 << 20, 256, 0, 1, 0)), None, 0,
+    None),
             "bad shape")
     s = C.byref(S(*good))
-    for args in ((None, P, P, P, P, P), (P, None, P, P, P, P), (P, P, P, P, P, None), (P, P + 8, P, P, P, P),
+    for args in ((None, P, P, P, P, P), (P, None, P, P, P, P), (P, P, P, P, P, None), (P, P + 8, P, P, P,
+    P),
                  (P, P, P, P + 16, P, P), (P, P, P, P, P + 2, P), (P + 1, P, P, P, P, P)):
         refused(f(*args, None, None, s, None, 0, None), "bad arguments")
-    assert f(None, None, None, None, None, None, None, None, C.byref(S(2, 0, 0, 0, 64, 256, 0, 1, 0)), None, 0,
+    assert f(None, None, None, None, None, None, None, None, C.byref(S(2, 0, 0, 0, 64, 256, 0, 1, 0)),
+    None, 0,
              None) == 0  # nothing to do
 
 
 def test_c_norm_and_beams():
     S, f = dsv4cuda.NormShape, dsv4cuda.lib.dsv4cuda_norm_quant
-    for s in ((1, 0, 1, 1e-6), (1, 32769, 1, 1e-6), (-1, 8, 1, 1e-6), (1, 8, 1, 0.0), (1, 8, 1, float("nan")),
+    for s in ((1, 0, 1, 1e-6), (1, 32769, 1, 1e-6), (-1, 8, 1, 1e-6), (1, 8, 1, 0.0), (1, 8, 1,
+    float("nan")),
               (1, 8, 1, float("inf"))):
         refused(f(P, None, None, None, None, P, P, C.byref(S(*s)), None), "bad shape")
     ok = S(2, 8, 1, 1e-6)
