@@ -186,3 +186,21 @@ def test_capture_without_a_workspace_is_refused(cuda):
         with pytest.raises(cuda.Dsv4CudaError, match="workspace"):
             cuda.grouped_gemm(out, xq, xs, w, ws, offsets)
         out.fill_(1)
+
+
+@pytest.mark.parametrize("counts,outs,width,fp8,bf16", [
+    ([i % 4 for i in range(1024)], 130, 256, False, True),    # more groups than threads
+    ([0] * 700 + [5] + [0] * 200 + [40, 0], 257, 384, False, False),
+    ([8], 1024, 4096, False, False),                          # few tiles: cut along the columns
+    ([8], 1024, 2048, False, False),                          # or not
+    ([300, 1, 1, 80, 17], 640, 3584, False, False),           # tiles of several sizes
+    ([90, 16, 150], 2500, 1024, True, True),
+])
+def test_plans(cuda, counts, outs, width, fp8, bf16):
+    xq, xs, w, ws, offsets = setup(counts, outs, width, fp8, seed=9)
+    out = torch.full((sum(counts), outs), 7.0, dtype=torch.bfloat16 if bf16 else torch.float32, device="cuda")
+    cuda.grouped_gemm(out, xq, xs, w, ws, offsets)
+    near(out, *want(xq, xs, w, ws, offsets))
+    again = torch.empty_like(out)
+    cuda.grouped_gemm(again, xq, xs, w, ws, offsets)
+    assert torch.equal(out, again) and cuda.device_error() == 0

@@ -205,3 +205,36 @@ def test_against_the_layers_forward(cuda):
     layer.experts(xq, xs, torch.tensor(idx).int().cuda(), torch.tensor(wt).float().cuda(), out)
     assert float((out.double() - y.double()).norm()) <= 0.03 * float(y.double().norm())
     layer.close()
+
+
+def test_route_weights(cuda):
+    """Zero, negative, tiny and huge ones; an infinity or NaN stays with its token."""
+    layer, w = layer_of(cuda, 256, 256, 5, 2)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(6)
+    xq, xs = ref.activations(120, 256, g)
+    idx, wt = routes(120, 5, 2)
+    xq[3] = 0                                 # gate and up of zero, with a huge weight
+    wt[::7, 0], wt[1::7], wt[2::7, 1] = 0.0, -2.5, 1e-30
+    wt[3], wt[10, 0], wt[17] = 3e38, 1e-45, 1e12
+    out = check(cuda, layer, w, xq, xs, idx, wt)
+    assert bool((out[3] == 0).all())
+    wt[40, 1], wt[41, 0] = float("inf"), float("nan")
+    again = torch.empty_like(out)
+    layer.experts(xq, xs, idx, wt, again)
+    bad = torch.zeros(120, dtype=torch.bool, device="cuda")
+    bad[40:42] = True
+    assert bool(torch.isnan(again[bad]).all()) and torch.equal(again[~bad], out[~bad])
+    layer.close()
+
+
+@pytest.mark.parametrize("n,experts,topk,part", [(32, 300, 2, None), (33, 300, 2, None), (8, 1024, 8, None),
+                                                 (11, 900, 6, (200, 870)), (400, 1000, 3, (1, 999))])
+def test_many_experts(cuda, n, experts, topk, part):
+    layer, w = layer_of(cuda, 128, 128, experts, topk, part=part)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(7)
+    xq, xs = ref.activations(n, 128, g)
+    idx, wt = routes(n, experts, topk)
+    check(cuda, layer, w, xq, xs, idx, wt, lo=part[0] if part else 0)
+    layer.close()
