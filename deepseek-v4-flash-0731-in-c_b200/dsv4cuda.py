@@ -125,9 +125,11 @@ def _f32(a):
     return np.ascontiguousarray(a, dtype=np.float32)
 
 
-def _stream(stream):
+def _stream(stream, on=None):
     if stream is None:
         import torch
+        if on is not None:  # the current device, where it is known (0.4 us)
+            return torch._C._cuda_getCurrentRawStream(on)
         # the current stream's handle without a Stream object around it (3 us a call)
         return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
     return stream
@@ -408,7 +410,7 @@ class MoeLayer:
             _dev(wt, "wt", torch.float32, n * self.topk, on), n,
             _dev(out, "out", torch.bfloat16, n * self.hidden, on),
             _dev(workspace, "workspace", u8, None, on),
-            0 if workspace is None else workspace.numel(), _stream(stream)))
+            0 if workspace is None else workspace.numel(), _stream(stream, on)))
 
     def routed_slots(self, n_tokens):
         """torch CUDA float32 view [n][topk][H] of the layer's routed slots."""
@@ -673,9 +675,9 @@ def _dev(t, name, dtype, numel=None, on=None):
     device `on` where that is given."""
     if t is None:
         return None
-    if on is not None and t.get_device() != on:
+    if on is not None and t.get_device() != on:  # (-1 on the host)
         raise ValueError(f"{name} is on {t.device}, the call's other tensors are on cuda:{on}")
-    if not (t.dtype is dtype and t.is_cuda and t.is_contiguous()):
+    if not (t.dtype is dtype and (on is not None or t.is_cuda) and t.is_contiguous()):
         raise ValueError(f"{name}: a contiguous CUDA tensor of {dtype} is wanted, got {t.dtype} "
                          f"on {t.device}")
     if numel is not None and t.numel() < numel:
@@ -695,7 +697,7 @@ def _here(t, name):
 def _rows_of(t, name, shape, dtype, on=None):
     """Elements between the rows (0: of one row, or of none between them) of a CUDA tensor
     [rows][width] of `shape` and `dtype`."""
-    if t.dtype is not dtype or t.shape != shape or not t.is_cuda or on not in (None, t.get_device()):
+    if t.dtype is not dtype or t.shape != shape or not (t.is_cuda if on is None else t.get_device() == on):
         raise ValueError(f"{name}: a tensor {list(shape)} of {dtype} on "
                          f"{'CUDA' if on is None else f'cuda:{on}'} is wanted, got {t.dtype} "
                          f"{list(t.shape)} on {t.device}")
@@ -789,13 +791,13 @@ class PagedCache:
         dtype, bf16, shape, on = _float_rows(kv, "kv", d)
         if self.status_word.get_device() != on:
             raise ValueError(f"kv is on cuda:{on}, the pool on {self.status_word.device}")
-        stride, n = _rows_of(kv, "kv", shape, dtype), shape[0]
+        stride, n = _rows_of(kv, "kv", shape, dtype, on), shape[0]
         half = n * (self._dims[1] // 2)
         _check(lib.dsv4cuda_paged_write(
             self._ref, layer, kv.data_ptr(), bf16, stride, _dev(rows, "rows", self._i64, n, on), n,
             _dev(gain, "gain", torch.bfloat16, d, on), eps,
             _dev(rope_cos, "rope_cos", torch.float32, half, on),
-            _dev(rope_sin, "rope_sin", torch.float32, half, on), _stream(stream)))
+            _dev(rope_sin, "rope_sin", torch.float32, half, on), _stream(stream, on)))
 
     def fork(self, dst, src, stream=None):
         """Slots dst become copies of slots src (-1: emptied); int32 CUDA tensors."""
@@ -907,7 +909,7 @@ def norm_quant(x, gain, codes, scales, eps=1e-6, residual=None, sum_out=None, ou
     import torch
     dtype, bf16, size, on = _float_rows(x, "x")
     n, width = size
-    u8, q = torch.uint8, _rows_of(x, "x", size, dtype)
+    u8, q = torch.uint8, _rows_of(x, "x", size, dtype, on)
     r = s = o = 0
     at_r = at_s = at_o = None
     if residual is not None:
@@ -920,7 +922,7 @@ def norm_quant(x, gain, codes, scales, eps=1e-6, residual=None, sum_out=None, ou
         x.data_ptr(), at_r, at_s, at_o, _dev(gain, "gain", torch.bfloat16, width, on),
         _dev(codes, "codes", u8, n * width, on),
         _dev(scales, "scales", u8, n * ((width + 127) // 128), on),
-        _norm_shape(n, width, bf16, eps, q, r, s, o), _stream(stream)))
+        _norm_shape(n, width, bf16, eps, q, r, s, o), _stream(stream, on)))
 
 
 def _beam_shape(logits, score, cands, eos):
@@ -929,7 +931,7 @@ def _beam_shape(logits, score, cands, eos):
         raise ValueError("score [groups][beams] and logits [groups * beams][vocab] are wanted")
     groups, beams = score.shape
     return BeamShape(groups, beams, cands, vocab, bf16, eos,
-                     _rows_of(logits, "logits", logits.shape, dtype)), on
+                     _rows_of(logits, "logits", logits.shape, dtype, on)), on
 
 
 def beam_select(logits, score, parent, token, total, next, slot=None, dst=None, src=None, eos=-1,
@@ -950,7 +952,7 @@ def beam_select(logits, score, parent, token, total, next, slot=None, dst=None, 
         _dev(token, "token", i32, all_c, on), _dev(total, "total", f32, all_c, on),
         _dev(next, "next", i32, all_b, on), _dev(slot, "slot", i32, all_b, on),
         _dev(dst, "dst", i32, all_b, on), _dev(src, "src", i32, all_b, on), C.byref(shape),
-        _stream(stream)))
+        _stream(stream, on)))
 
 
 # ------------------------------------------------------- grouped products --
@@ -1008,8 +1010,7 @@ def grouped_gemm(out, xq, xs, w, ws, offsets, src=None, dst=None, workspace=None
         _dev(w, "w", u8, None, on), _dev(ws, "ws", u8, scales, on),
         _dev(offsets, "offsets", i32, s.n_groups + 1, on), _dev(src, "src", i32, rows, on),
         _dev(dst, "dst", i32, rows, on), C.byref(s), _dev(workspace, "workspace", u8, None, on),
-        0 if workspace is None else workspace.numel(),
-        _stream(stream)))
+        0 if workspace is None else workspace.numel(), _stream(stream, on)))
 
 
 def token_logprobs(logits, tokens, logprob, entropy=None, rank=None, top_id=None, top_logprob=None,
