@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
   walk.row_tiles = row_tiles;
   walk.chunks = chunks;
   walk.n_max = a.n_max;
-  // The plan. (Its 4 us are mostly code that a block runs once, from beyond the
+  // The plan. (Its 3 us are mostly code that a block runs once, from beyond the
   // instruction caches; a rehearsal while the kernel before runs only delayed the
   // blocks that start late.)
   if (!a.early) pdl_wait();  // offsets, rows and counters of the kernels before
