@@ -848,7 +848,6 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
       cp_async_wait<kScaleEntries - 2>();
       bar_sync(4, 32 * kScaleWarps);  // all have this entry's copies, and have read the one before
       const uint8_t* entry = scale_ring + (n % kScaleEntries) * entry_bytes;
-      fetch();
       const int buf = n & 1;
       // (no break after an abort: the others wait at the barrier above)
       wait_bar(&ctl->scale_empty[buf], ((n >> 1) & 1) ^ 1, abort_flag, err);
@@ -887,6 +886,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&ctl->scale_full[buf]);
+      fetch();  // (into the entry before; behind the store, since the first MMA waits for that)
     }
     cp_async_wait<0>();
   } else if (warp < kWarpCopy) {
