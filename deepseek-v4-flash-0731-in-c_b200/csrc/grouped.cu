@@ -28,7 +28,7 @@
 // bandwidth, 64 KB a chunk for writing and reading expanded E2M1 tiles and 384
 // bytes a row (256 experts of 4096 x 2048: 2,000 tokens 877 us, 8,192 tokens 2.2
 // ms, 1.1 PFLOP/s at the power cap). With one token launches, the plan and the
-// first bytes' way (38 us).
+// first bytes' way (36.7 us).
 #include "grouped.cuh"
 
 #include <cuda_bf16.h>
