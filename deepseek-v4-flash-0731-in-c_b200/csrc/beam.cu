@@ -39,7 +39,7 @@ constexpr int kMaxWarps = 16;
 using Key = unsigned long long;           // ordered value above inverted index; 0: nothing
 
 constexpr double kLn2 = 0.69314718055994530942;
-constexpr double kLog2eRest = 1.4426950408889634074 - static_cast<double>(kLog2e);
+constexpr double kLog2e64 = 1.4426950408889634074;
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -49,9 +49,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 __constant__ double kReciprocal[12] = {0.0, 1.0, 1.0 / 2, 1.0 / 3, 1.0 / 4, 1.0 / 5,
                                         1.0 / 6, 1.0 / 7, 1.0 / 8, 1.0 / 9, 1.0 / 10, 1.0 / 11};
-// 2^x for x <= 2 to 1e-13 of itself (0 below 2^-1000): Taylor's series around the
-// nearest whole number. One copy of it, since it is seldom run.
-__device__ __noinline__ double pow2(double x) {
+// e^x for x <= 0 to 1e-13 of itself (0 below 2^-1000), as 2^(x log2 e): Taylor's
+// series around the nearest whole number. One copy of it, since it is seldom run.
+__device__ __noinline__ double exp_down(double x) {
+  x *= kLog2e64;
   if (!(x > -1000.0)) return x == x ? 0.0 : x;
   const double n = rint(x), t = (x - n) * kLn2;
   double r = 1.0;
@@ -86,7 +87,7 @@ __device__ __forceinline__ float below(float x) {
 }
 
 struct Part {
-  double z;  // sum of 2^(x log2 e - m)
+  double z;  // sum of e^(x - m)
   float m;   // -inf: of nothing
 };
 
@@ -190,10 +191,12 @@ __device__ __forceinline__ void take_part(Held& h, const BeamArgs& a, long long 
   next.load(x, i0, i1, a.wide);
   __syncthreads();  // the part before has been written down
   if (tid == 0) h.n = h.jobs = 0;
-  // The sum is of 2^(v log2 e - c), c = ref log2 e: ref is a maximum of some
-  // values of this thread, moved when one exceeds it by more than 8 (some thread
-  // of a warp has a new maximum at every step).
-  float ref = -INFINITY, c = 0.f;
+  // The sum is of e^(v - ref): ref is a maximum of some values of this thread, moved
+  // when one exceeds it by more than 8 (some thread of a warp has a new maximum at
+  // every step). The difference is taken before it is scaled: v log2 e - ref log2 e
+  // keeps the rounding of its second product, 2^18 where a row's masked values
+  // are -1e9, and nothing is left of a sum that is moved by such powers.
+  float ref = -INFINITY, base = 0.f;  // base: ref, or 0 before there is one
   float above = -INFINITY;  // candidates exceed it; -inf never is one
   double z = 0.0;
   const int part_i0 = i0;
@@ -208,16 +211,14 @@ __device__ __forceinline__ void take_part(Held& h, const BeamArgs& a, long long 
     for (int k = 1; k + 1 < kEach; k += 2) top = max3(top, v[k], v[k + 1]);
     top = fmaxf(top, v[kEach - 1]);
     if (top > ref + 8.f) {
-      const float to = top * kLog2e;
-      if (ref != -INFINITY) z *= pow2(static_cast<double>(c) - static_cast<double>(to));
-      ref = top;
-      c = to;
+      if (ref != -INFINITY) z *= exp_down(static_cast<double>(ref) - top);
+      ref = base = top;
     }
     float z0 = 0.f, z1 = 0.f;
 #pragma unroll
     for (int k = 0; k < kEach; k += 2) {
-      z0 += ex2_approx(fmaf(v[k], kLog2e, -c));
-      z1 += ex2_approx(fmaf(v[k + 1], kLog2e, -c));
+      z0 += ex2_approx((v[k] - base) * kLog2e);
+      z1 += ex2_approx((v[k + 1] - base) * kLog2e);
     }
     z += z0 + z1;
     if (step == 0) {
@@ -328,12 +329,9 @@ __device__ __forceinline__ void take_part(Held& h, const BeamArgs& a, long long 
   }
   thin(h, list, kept, p.cands);  // sorted
   list ^= 1;
-  // the block's sum, relative to the largest c; a thread whose ref is not the
-  // row's maximum is corrected for log2 e's rounding by its own (the rest of it is
-  // below 2^-25 of the distance between them)
-  if (ref != -INFINITY) z *= pow2(static_cast<double>(ref) * kLog2eRest);  // (NaN stays)
-  const float mine = ref != -INFINITY ? c : -INFINITY, top = warp_max(mine);
-  if (mine != -INFINITY) z *= pow2(static_cast<double>(c) - static_cast<double>(top));
+  // the block's sum, relative to its largest ref (NaN stays)
+  const float top = warp_max(ref);
+  if (ref != -INFINITY) z *= exp_down(static_cast<double>(ref) - top);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
   if (lane == 0) {
@@ -345,7 +343,7 @@ __device__ __forceinline__ void take_part(Held& h, const BeamArgs& a, long long 
     const bool in = lane < kWarps;
     const float one = in ? h.m[lane] : -INFINITY, all = warp_max(one);
     z = in ? h.z[lane] : 0.0;
-    if (one != -INFINITY) z *= pow2(static_cast<double>(one) - static_cast<double>(all));
+    if (one != -INFINITY) z *= exp_down(static_cast<double>(one) - all);
 #pragma unroll
     for (int o = kWarps / 2; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
     if (lane == 0) *out = {z, all};
@@ -465,10 +463,10 @@ __device__ __forceinline__ void merge_group(Merge& sh, const BeamArgs& a, int g,
     double z = 0.0;
 #pragma unroll
     for (int i = 0; i < kMaxParts / 32; ++i)  // (NaN stays; a part of nothing has z 0)
-      if (i * 32 < a.parts) z += q[i].m == -INFINITY ? q[i].z : q[i].z * pow2(static_cast<double>(q[i].m) - m);
+      if (i * 32 < a.parts) z += q[i].m == -INFINITY ? q[i].z : q[i].z * exp_down(static_cast<double>(q[i].m) - m);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-    if (lane == 0) sh.moved[b] = score - (m + log2(z)) * kLn2;
+    if (lane == 0) sh.moved[b] = score - (m + log2(z) * kLn2);
   }
   if (warp < units) best_key(warp);
   __syncthreads();
