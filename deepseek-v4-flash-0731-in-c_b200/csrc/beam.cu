@@ -411,7 +411,7 @@ __device__ __forceinline__ unsigned long long ld_block(const void* q, int rank) 
 
 struct Merge {
   Cand list[kMaxWarps][32];
-  double moved[kMaxBeams];
+  double top[kMaxBeams], rest[kMaxBeams];
 };
 
 // One prompt's parts: the block that merges them.
@@ -448,7 +448,8 @@ __device__ __forceinline__ void merge_group(Merge& sh, const BeamArgs& a, int g,
         if (first + i + w < a.parts) k[i] = best_of(k[i], k[i + w]);
   };
   if (warp < units) load_keys(warp);
-  // what a row's values are moved by: its score less its log sum
+  // A row's total is (x - top) + rest: top its maximum, rest the score less the log
+  // of the sum beside it. (Added up first, both would be lost beside a large top.)
   for (int b = warp; b < p.beams; b += kWarps) {
     const long long row = static_cast<long long>(g) * p.beams + b;
     const double score = p.score[row];
@@ -466,7 +467,10 @@ __device__ __forceinline__ void merge_group(Merge& sh, const BeamArgs& a, int g,
       if (i * 32 < a.parts) z += q[i].m == -INFINITY ? q[i].z : q[i].z * exp_down(static_cast<double>(q[i].m) - m);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-    if (lane == 0) sh.moved[b] = score - (m + log2(z) * kLn2);
+    if (lane == 0) {
+      sh.top[b] = m;
+      sh.rest[b] = score - log2(z) * kLn2;
+    }
   }
   if (warp < units) best_key(warp);
   __syncthreads();
@@ -479,7 +483,7 @@ __device__ __forceinline__ void merge_group(Merge& sh, const BeamArgs& a, int g,
     const int b = u / takes;
     Cand c = {0.0, -1};
     if (k[0]) {
-      c.total = key_value(k[0]) + sh.moved[b];
+      c.total = (static_cast<double>(key_value(k[0])) - sh.top[b]) + sh.rest[b];
       // a dead beam, or a row with a NaN or +inf, has no candidates
       if (fabs(c.total) <= 1.7e308) c.place = static_cast<long long>(b) << 32 | key_index(k[0]);
     }
