@@ -106,6 +106,17 @@ __device__ __forceinline__ uint32_t top8(const float (&v)[kVec]) {
   return __float_as_uint(m);
 }
 
+// Whether a row's mean of squares and eps add up to more than fp32 holds (values
+// from 1.8e19 on; NaN) or to so little that squares have lost bits. Its values are
+// then squared again, times square_scale (2^-76 or 2^76), eps times its square.
+__device__ __forceinline__ bool square_odd(float sum) {
+  constexpr uint32_t kLow = 0x0DA24260u, kHigh = 0x7F61B1E6u;  // 1e-30, 3e38
+  return __float_as_uint(sum) - kLow > kHigh - kLow;
+}
+__device__ __forceinline__ float square_scale(float sum) {
+  return sum < 1.f ? 7.555786372591432e22f : 1.3234889800848443e-23f;
+}
+
 struct NormArgs {
   NormProblem p;
   int threads;                       // of a row
@@ -162,27 +173,26 @@ __device__ __forceinline__ void finish_row(const NormArgs& a, long long row, boo
     return s;
   };
   float mean = row_sum(squares) / p.width, eps = p.eps;
-  // Squares beyond fp32 (values from 1.8e19 on): again, of values times
-  // 2^-76. All rows of a block take the step together.
-  const bool over = !(mean <= 3.0e38f);
-  if (__syncthreads_or(over)) {
-    constexpr float kDown = 1.3234889800848443e-23f;  // 2^-76
+  // All rows of a block take the step together.
+  const bool odd = square_odd(mean + eps);
+  if (__syncthreads_or(odd)) {
+    const float scale = square_scale(mean + eps);
     squares = 0.f;
 #pragma unroll
     for (int j = 0; j < kVecs; ++j)
 #pragma unroll
       for (int k = 0; k < kVec; ++k) {
-        const float d = v[j][k] * kDown;
+        const float d = v[j][k] * scale;
         squares = fmaf(d, d, squares);
       }
     const float m = row_sum(squares) / p.width;
-    if (over) {
+    if (odd) {
       mean = m;
-      eps = 0.f;  // eps 2^-152 is nothing beside it
+      eps = eps * scale * scale;
 #pragma unroll
       for (int j = 0; j < kVecs; ++j)
 #pragma unroll
-        for (int k = 0; k < kVec; ++k) v[j][k] *= kDown;
+        for (int k = 0; k < kVec; ++k) v[j][k] *= scale;
     }
   }
   const float rs = rsqrtf(mean + eps);
@@ -310,7 +320,7 @@ __global__ void __launch_bounds__(32 * kLatentWarps) latent_write_kernel(const L
     const float x0 = value(c.nope + 2 * q), x1 = value(c.nope + 2 * q + 1);
     squares = fmaf(x0, x0, fmaf(x1, x1, squares));
   }
-  float rs = 1.f, down = 1.f;
+  float rs = 1.f, scale = 1.f;
   if (p.gain) {
     const float d = static_cast<float>(c.nope + c.rope_dim);
     auto warp_sum = [](float s) {
@@ -319,19 +329,19 @@ __global__ void __launch_bounds__(32 * kLatentWarps) latent_write_kernel(const L
       return s;
     };
     float mean = warp_sum(squares) / d, eps = p.eps;
-    if (!(mean <= 3.0e38f)) {  // squares beyond fp32: of values times 2^-76
-      down = 1.3234889800848443e-23f;
+    if (square_odd(mean + eps)) {
+      scale = square_scale(mean + eps);
       squares = 0.f;
 #pragma unroll
       for (int j = 0; j < kVecs; ++j)
 #pragma unroll
-        for (int k = 0; k < kVec; ++k) squares = fmaf(v[j][k] * down, v[j][k] * down, squares);
+        for (int k = 0; k < kVec; ++k) squares = fmaf(v[j][k] * scale, v[j][k] * scale, squares);
       for (int q = lane; q < pairs; q += 32) {
-        const float x0 = value(c.nope + 2 * q) * down, x1 = value(c.nope + 2 * q + 1) * down;
+        const float x0 = value(c.nope + 2 * q) * scale, x1 = value(c.nope + 2 * q + 1) * scale;
         squares = fmaf(x0, x0, fmaf(x1, x1, squares));
       }
       mean = warp_sum(squares) / d;
-      eps = 0.f;
+      eps = eps * scale * scale;
     }
     rs = rsqrtf(mean + eps);
   }
@@ -341,7 +351,7 @@ __global__ void __launch_bounds__(32 * kLatentWarps) latent_write_kernel(const L
     const int at = lane + 32 * j;
     if (p.gain) {
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) v[j][k] = v[j][k] * down * rs * gain[j].get(k);
+      for (int k = 0; k < kVec; ++k) v[j][k] = v[j][k] * scale * rs * gain[j].get(k);
     }
     uint32_t top = top8(v[j]);
 #pragma unroll
@@ -361,8 +371,8 @@ __global__ void __launch_bounds__(32 * kLatentWarps) latent_write_kernel(const L
     float x0 = p0, x1 = p1;
     if (q != lane) { x0 = value(c.nope + 2 * q); x1 = value(c.nope + 2 * q + 1); }
     if (p.gain) {
-      x0 = x0 * down * rs * bf16_widen(p.gain[c.nope + 2 * q]);
-      x1 = x1 * down * rs * bf16_widen(p.gain[c.nope + 2 * q + 1]);
+      x0 = x0 * scale * rs * bf16_widen(p.gain[c.nope + 2 * q]);
+      x1 = x1 * scale * rs * bf16_widen(p.gain[c.nope + 2 * q + 1]);
     }
     if (p.rope_cos) {
       if (q != lane) { co = p.rope_cos[i * pairs + q]; si = p.rope_sin[i * pairs + q]; }
