@@ -336,6 +336,7 @@ struct dsv4cuda_moe_layer {
   float* d_out = nullptr;
   int* d_tok = nullptr;
   int max_tokens = 0;
+  int device = 0;             // that holds the experts' weights
   // expert-GEMV timing (dsv4cuda_moe_timing_*): event quadruples per forward
   std::vector<cudaEvent_t> events;
   int timed = 0;
@@ -392,8 +393,13 @@ int layer_finish(dsv4cuda_moe_layer* L, int max_tokens) {
   L->max_tokens = max_tokens;
   L->ws_bytes = dsv4::moe_workspace_bytes(L->cfg, max_tokens) +
                 al(sizeof(float) * max_tokens * L->cfg.hidden) * 2 + al(sizeof(int) * max_tokens);
-  cudaError_t e = cudaMalloc(&L->ws_mem, L->ws_bytes);
+  cudaError_t e = cudaGetDevice(&L->device);
+  if (e == cudaSuccess) e = cudaMalloc(&L->ws_mem, L->ws_bytes);
   if (e != cudaSuccess) { record_error("workspace cudaMalloc: %s", cudaGetErrorString(e)); return -1; }
+  cudaPointerAttributes at{};  // (adopted weights may be another's)
+  if (L->w.w1 && cudaPointerGetAttributes(&at, L->w.w1) == cudaSuccess && at.type == cudaMemoryTypeDevice)
+    L->device = at.device;
+  (void)cudaGetLastError();
   cudaMemset(L->ws_mem, 0, L->ws_bytes);
   dsv4::moe_workspace_carve(&L->ws, L->cfg, max_tokens, L->ws_mem);
   char* p = static_cast<char*>(L->ws_mem) + L->ws.bytes;
@@ -1943,6 +1949,12 @@ DSV4_API int dsv4cuda_moe_experts(dsv4cuda_moe_layer* L, const uint8_t* xq, cons
       !aligned(p.s3, 4) || !aligned(p.s2, 4)) {
     record_error("%s: bad arguments (xq, out and the layer's w1, w3, w2 32-byte aligned, its scales 4)",
                  who);
+    return -1;
+  }
+  int here = -1;
+  if (cudaGetDevice(&here) != cudaSuccess || here != L->device) {
+    record_error("%s: the layer's weights are on device %d, the current device is %d", who, L->device,
+                 here);
     return -1;
   }
   p.xq = xq;

@@ -347,6 +347,7 @@ class MoeLayer:
     same keys holding numpy arrays (copied in) or torch CUDA tensors
     (adopted, device=True).
     """
+    on = None  # the device of adopted weights
 
     def __init__(self, layer: dict, max_tokens: int = 8, device: bool = False,
                  expert_range=None):
@@ -382,6 +383,8 @@ class MoeLayer:
             _check(fn(C.byref(self.handle), C.byref(self.cfg), C.byref(w), max_tokens))
         self.hidden = layer["hidden"]
         self.topk = layer["topk"]
+        if device and hasattr(layer["w1"], "get_device"):
+            self.on = layer["w1"].get_device()
 
     def forward_local(self, x, token_ids=None, stream=None):
         """Router, this device's experts and the shared expert (EP step 1)."""
@@ -404,6 +407,8 @@ class MoeLayer:
         if xq.dim() != 2 or xq.shape[1] != self.hidden:
             raise ValueError(f"xq: [n][{self.hidden}] is wanted")
         on = _here(xq, "xq")
+        if self.on is not None and self.on != on:
+            raise ValueError(f"the layer is on cuda:{self.on}, the call's tensors are on cuda:{on}")
         _check(lib.dsv4cuda_moe_experts(
             self.handle, _dev(xq, "xq", u8), _dev(xs, "xs", u8, n * (self.hidden // 128), on),
             _dev(idx, "idx", torch.int32, n * self.topk, on),

@@ -275,7 +275,8 @@ int dsv4cuda_moe_forward_noalloc(const dsv4cuda_moe_config *cfg,
  * a value of h that is not finite its block of 128. The router and the shared
  * expert are not part of it. hidden and moe_inter have to be multiples of 128,
  * at most 1024 experts; idx, wt, out are DEVICE pointers, xq, w1, w3, w2 and
- * out aligned to 32 bytes. workspace may be NULL (a buffer per thread and
+ * out aligned to 32 bytes, on the device of the layer's weights, which has to be
+ * the current one. workspace may be NULL (a buffer per thread and
  * stream that grows); give one, 256-byte aligned, while capturing. Calls that
  * share a workspace must not overlap. */
 size_t dsv4cuda_moe_experts_workspace_bytes(const dsv4cuda_moe_layer *L, int n_tokens);
