@@ -1951,6 +1951,10 @@ DSV4_API int dsv4cuda_moe_experts(dsv4cuda_moe_layer* L, const uint8_t* xq, cons
                  who);
     return -1;
   }
+  if (!p.w1 || !p.s1 || !p.w3 || !p.s3 || !p.w2 || !p.s2) {
+    record_error("%s: the layer has no routed experts", who);
+    return -1;
+  }
   int here = -1;
   if (cudaGetDevice(&here) != cudaSuccess || here != L->device) {
     record_error("%s: the layer's weights are on device %d, the current device is %d", who, L->device,
