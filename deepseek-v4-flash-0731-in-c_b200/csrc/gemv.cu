@@ -19,6 +19,7 @@
 // as fmaf on the widened values). Activations are read through L1 (every
 // lane of a warp reads the same few lines); weights bypass L1.
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 #include <utility>
 #include <vector>
@@ -123,17 +124,36 @@ bool make_tma_map_u4_3d(CUtensorMap* out, const void* base, uint64_t cols, uint6
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Made when it is first wanted, which may be while a stream is being captured, by
+// this thread or another: the allocation is let through (nothing of it enters the
+// graph) and cleared on a stream of its own.
 unsigned int* device_error_word() {
-  static unsigned int* words[64] = {};
+  static std::atomic<unsigned int*> words[64] = {};
+  static std::mutex mu;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
-  if (!words[dev]) {
-    unsigned int* w = nullptr;
-    if (cudaMalloc(&w, sizeof(unsigned int)) != cudaSuccess) return nullptr;
-    cudaMemset(w, 0, sizeof(unsigned int));
-    words[dev] = w;
+  unsigned int* w = words[dev].load(std::memory_order_acquire);
+  if (w) return w;
+  std::lock_guard<std::mutex> lock(mu);
+  w = words[dev].load(std::memory_order_relaxed);
+  if (w) return w;
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
+  cudaStream_t st = nullptr;
+  cudaError_t e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+  if (e == cudaSuccess) {
+    e = cudaMalloc(&w, sizeof(unsigned int));
+    if (e == cudaSuccess) e = cudaMemsetAsync(w, 0, sizeof(unsigned int), st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    cudaStreamDestroy(st);
   }
-  return words[dev];
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) {
+    if (w) cudaFree(w);
+    return nullptr;
+  }
+  words[dev].store(w, std::memory_order_release);
+  return w;
 }
 
 namespace {
