@@ -394,6 +394,7 @@ class MoeLayer:
 
     def experts_workspace_bytes(self, n_tokens) -> int:
         """Workspace of an experts call of n_tokens."""
+        _int(n_tokens)
         return lib.dsv4cuda_moe_experts_workspace_bytes(self.handle, n_tokens)
 
     def experts(self, xq, xs, idx, wt, out, workspace=None, stream=None):
@@ -406,6 +407,7 @@ class MoeLayer:
         u8 = torch.uint8
         if xq.dim() != 2 or xq.shape[1] != self.hidden:
             raise ValueError(f"xq: [n][{self.hidden}] is wanted")
+        _int(n)
         on = _here(xq, "xq")
         if self.on is not None and self.on != on:
             raise ValueError(f"the layer is on cuda:{self.on}, the call's tensors are on cuda:{on}")
@@ -690,6 +692,13 @@ def _dev(t, name, dtype, numel=None, on=None):
     return t.data_ptr()
 
 
+def _int(*sizes):
+    """Sizes that the library takes in 32 bits (ctypes would cut longer ones off)."""
+    for n in sizes:
+        if not -1 << 31 <= n < 1 << 31:
+            raise ValueError(f"{n} is beyond 31 bits")
+
+
 def _here(t, name):
     """The current device, on which a call launches: its tensors have to be there."""
     import torch
@@ -725,6 +734,8 @@ def _float_rows(t, name, width=None):
     if not (bf16 or dtype is torch.float32) or len(shape) != 2 or width not in (None, shape[1]):
         raise ValueError(f"{name}: a CUDA tensor [rows][{width or 'width'}] of bfloat16 or float32 is "
                          f"wanted, got {dtype} {list(shape)}")
+    if shape[0] >> 31 or shape[1] >> 31:
+        _int(*shape)
     return dtype, 1 if bf16 else 0, shape, _here(t, name)
 
 
@@ -935,6 +946,7 @@ def _beam_shape(logits, score, cands, eos):
     if score.dim() != 2 or n != score.numel():
         raise ValueError("score [groups][beams] and logits [groups * beams][vocab] are wanted")
     groups, beams = score.shape
+    _int(groups, beams, cands, eos)
     return BeamShape(groups, beams, cands, vocab, bf16, eos,
                      _rows_of(logits, "logits", logits.shape, dtype, on)), on
 
@@ -988,6 +1000,7 @@ def _grouped_shape(out, xq, w, n_rows):
                          "the other")
     if out.shape[0] > 1 and out.stride(0) < outs:
         raise ValueError("out: the rows must not overlap")
+    _int(groups, n_rows, xq.shape[0], out.shape[0], outs, width)
     return GroupedShape(groups, n_rows, xq.shape[0], out.shape[0], outs, width, int(held == width),
                         int(out.dtype is torch.bfloat16), out.stride(0) if out.shape[0] > 1 else 0)
 
