@@ -413,7 +413,7 @@ cudaError_t norm_quant(const NormProblem& p, cudaStream_t st) {
   a.threads = ((vecs + per - 1) / per + 31) / 32 * 32;
   if (a.threads > 1024) return cudaErrorInvalidValue;
   const int rows = a.threads >= 128 ? 1 : 128 / a.threads;
-  const dim3 grid(static_cast<unsigned>((p.rows + rows - 1) / rows)), block(rows * a.threads);
+  const dim3 grid(static_cast<unsigned>((p.rows - 1) / rows + 1)), block(rows * a.threads);
   auto run = [&](auto bf16) {
     constexpr bool kB = decltype(bf16)::value;
     auto kernel = per == 1 ? norm_quant_kernel<kB, 1, 256> : per == 2 ? norm_quant_kernel<kB, 2, 256>
@@ -431,7 +431,7 @@ cudaError_t latent_write(const LatentWrite& p, cudaStream_t st) {
   a.wide = reinterpret_cast<uintptr_t>(p.kv) % 16 == 0 && (p.n <= 1 || p.stride * size % 16 == 0);
   a.wide_g = reinterpret_cast<uintptr_t>(p.gain) % 16 == 0;
   auto kernel = p.bf16 ? latent_write_kernel<true> : latent_write_kernel<false>;
-  return launch_pdl(kernel, dim3(static_cast<unsigned>((p.n + kLatentWarps - 1) / kLatentWarps)),
+  return launch_pdl(kernel, dim3(static_cast<unsigned>((p.n - 1) / kLatentWarps + 1)),
                     dim3(32 * kLatentWarps), 0, st, a);
 }
 
