@@ -671,11 +671,19 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(
           const float m = max_nan(max_nan(tops[0][l], tops[1][l]), max_nan(tops[2][l], tops[3][l])) * fabsf(w);
           uint32_t e8 = 255;  // an infinity or NaN makes the block NaN
           float factor = NAN;
+          bool huge = false;
           if (m < INFINITY) {
             e8 = __float_as_uint(pow2_scale_448(m)) >> 23;
-            // (w over the scale may pass the largest float where h does not)
-            factor = w * __uint_as_float((254u - e8) << 23);
-            factor = fminf(fmaxf(factor, -3.402823466e38f), 3.402823466e38f);
+            const float inv = __uint_as_float((254u - e8) << 23);
+            factor = w * inv;
+            // w over the scale may pass the largest float where h does not (weights
+            // from 8e31 on): the other part then goes to the row's outputs
+            huge = fabsf(factor) == INFINITY;
+            if (huge) factor = w * 0x1p-64f * inv;
+          }
+          if (__any_sync(0xffffffffu, huge)) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v0[j] *= __shfl_sync(0xffffffffu, huge ? 0x1p64f : 1.f, j);
           }
           if (lane < 16) ctl->factor[side][quarter][l] = factor;
           if (quarter == 0 && lane < n)
