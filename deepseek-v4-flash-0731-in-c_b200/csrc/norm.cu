@@ -5,9 +5,8 @@
 //   per 128 columns: 2^e the smallest power of two with max |y| <= 448 2^e,
 //   codes = E4M3(y / 2^e)
 //
-// One read and one write: a row stays in the registers of its threads, eight
-// consecutive values a vector, so that 16 lanes hold a block of 128 and its
-// maximum is four shuffles. Sum and square are fp32 from the inputs' sum on;
+// One read and one write: a row stays with its threads, eight consecutive values a
+// vector, so that 16 lanes hold a block of 128 and its maximum is four shuffles. Sum and square are fp32 from the inputs' sum on;
 // each output is rounded once, from fp32.
 #include "norm.cuh"
 
@@ -28,6 +27,8 @@ constexpr int kVec = 8;  // values of a vector
 template <bool kBf16>
 struct Raw {
   uint4 w[kBf16 ? 1 : 2];
+  // Rows that are not whole aligned vectors are read and written value by value (4096
+  // BF16 rows of 7167: 131 us, 50 where they are 7168 wide).
   __device__ __forceinline__ void load(const void* row, int i, int n, bool wide) {
     const char* p = static_cast<const char*>(row) + static_cast<size_t>(i) * (kBf16 ? 2 : 4);
     if (wide && n >= kVec) {
@@ -125,10 +126,13 @@ struct NormArgs {
 
 // The row that its threads hold in v: sum, norm, output. Whole block.
 //
-// 4096 BF16 rows of 7168 with residual, sum and codes: 56.7 us, 4.66 TB/s of the 6.45
-// that a copy reaches: a block's reads, meeting and writes follow one another, and
-// the registers hold four or five rows an SM. Rows streamed through shared memory
-// by blocks that stay took 67 us.
+// 4096 BF16 rows of 7168 with residual, sum, normed rows and codes: 56.7 us, 4.66
+// TB/s of the 6.45 that a copy reaches: a block's reads, meeting and writes follow
+// one another, and the registers hold four rows an SM, not quite: above 4,096
+// columns a thread's 64 spill some 140 bytes (fp32 rows 290; three blocks an SM,
+// which spill nothing, took 58.6 us). fp32 rows with residual, sum and codes 86 us,
+// 4.4 TB/s (BF16 50). Rows streamed through shared memory by blocks that stay took
+// 67 us.
 template <bool kBf16, int kVecs>
 __device__ __forceinline__ void finish_row(const NormArgs& a, long long row, bool live, int tid,
                                            float (&v)[kVecs][kVec], float* part) {

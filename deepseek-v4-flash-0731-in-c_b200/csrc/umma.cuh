@@ -11,7 +11,7 @@
 namespace dsv4 {
 namespace {
 
-constexpr unsigned kErrWait = 2u;  // device error bit: a wait in an attention kernel timed out
+constexpr unsigned kErrWait = 2u;  // device error bit: a wait in an attention kernel or a grouped product timed out
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Byte offset of the 16-byte chunk (row, dc) in a 128-byte-swizzled tile

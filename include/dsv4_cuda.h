@@ -129,7 +129,7 @@ void dsv4cuda_shutdown(void);
 const char *dsv4cuda_last_error(void);
 /* Device-side error flags of the current device (synchronous): bit 0 = a
  * GEMV kernel gave up waiting on a shared-memory barrier, bit 1 = the
- * attention kernel did (bounded waits; the results of that launch are
+ * attention kernel or a grouped product did (bounded waits; the results of that launch are
  * invalid), bit 2 = an attention key index >= kv_rows was skipped.
  * clear != 0 resets them. */
 int dsv4cuda_device_error(unsigned int *flags, int clear);
@@ -267,6 +267,8 @@ int dsv4cuda_moe_forward_noalloc(const dsv4cuda_moe_config *cfg,
  *   out [n][hidden] BF16 = the sum of h w2 over the token's routes, in their
  *         order; the slots that are summed are BF16, as the layer's GEMVs
  *         leave them.
+ * Before it is quantised h errs by (10 + 2 |x w1|) 2^-24 of itself beside its sums
+ * (sigmoids below 2^-126 are 0).
  * Products are summed in fp32 in an order of their own: results agree with
  * dsv4cuda_moe_forward's within the rounding of its BF16 boundaries, and are
  * the same from call to call. Routes to experts that are not here (an
@@ -712,7 +714,9 @@ int dsv4cuda_token_logprobs(const void *logits, int bf16, int rows, int vocab, l
  * beam that is not there. The n_cands best continuations of a group by
  *   total = score[b] + log softmax(row b)[t]
  * come out in descending order, the lower (beam, token) first among equals
- * (totals are compared in 64 bits): parent, token, total [n_groups][n_cands];
+ * (totals are compared in 64 bits; the log of a row's sum behind one errs by less
+ * than 2^-17, so beams whose totals are nearer may change places, and beams with
+ * equal rows and scores do not): parent, token, total [n_groups][n_cands];
  * -1, -1, -inf where fewer are left: a logit of -inf is masked, a row with a NaN
  * or +inf has no continuations, nor has a beam whose score is not finite.
  *   next [n_groups][beams]  the candidates that go on, in order: those whose
@@ -753,7 +757,7 @@ int dsv4cuda_beam_select(const void *logits, const float *score, int *parent, in
  * `*_stride` elements apart (0: width). fp32 from the inputs on (y is taken of
  * the sum before it is rounded), each output rounded once. gain [width] BF16
  * (NULL: 1). A block of 128 with a NaN or infinity gets scale 255. width 1 ..
- * 32768, eps > 0. DEVICE pointers, async on stream, capturable. */
+ * 32768, eps above 0 up to 3e38. DEVICE pointers, async on stream, capturable. */
 typedef struct {
     int n_rows, width;
     int bf16;
